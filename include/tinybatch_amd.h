@@ -667,6 +667,80 @@ int32_t tb_rms_norm_partials(const float* partials, int32_t splits, void* residu
                              int64_t out_row_stride, int32_t rows, int32_t dim, float eps,
                              int32_t dtype, hipStream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Speculative decoding: a step whose rows are trees of drafted tokens. No counterpart in
+ * the reference, which decodes one token per sequence and step (src/tinybatch/engine.py:99-126).
+ * Sequence b's rows row_starts[b] .. row_starts[b+1]-1 are its nodes: node 0 the root (the last
+ * token it has emitted), every other node behind its parent. cached[b] positions of the sequence
+ * are in the cache; node i's K/V belong to position cached[b] + i of its block table (append them
+ * first, tb_kv_append), whatever its depth; its RoPE position is cached[b] + depth.
+ * At most TB_TREE_MAX_NODES nodes per tree where a limit is named. */
+#define TB_TREE_MAX_NODES 1024
+
+/* Attention of every node over the cached positions and the nodes of its mask:
+ *   S_i = {0 .. cached-1} + {cached + j : bit j of mask[row]},  out = softmax(scale q.K[S_i]) V[S_i].
+ * A node that sees nothing gives 0; positions outside S_i have no effect, also where they
+ * hold infinities or NaN. fp32 / fp16 / bf16, head_dim 64 or 128, block_size a power of two,
+ * any query heads per kv head, any scale.
+ *   q [num_rows][num_heads][head_dim], out [num_rows][num_heads * head_dim]: row strides in
+ *     elements, 16-byte aligned rows; block_tables [num_seqs][max_blocks_per_seq];
+ *   row_seq [num_rows]: each row's sequence (-1: a row of none, left as it is);
+ *   mask [num_rows][mask_words] 32-bit words, bit j % 32 of word j / 32 = node j is seen; bits
+ *     past the tree are ignored;
+ *   positions [num_rows] (int64) with rope tables: q holds the projections before rotation and is
+ *     rotated at them (as tb_kv_append_rope rotates k). */
+int32_t tb_tree_attention(const void* q, int64_t q_row_stride, const void* pool, int64_t num_blocks,
+                          void* out, int64_t out_row_stride, const int32_t* block_tables,
+                          int32_t max_blocks_per_seq, const int32_t* row_starts, const int32_t* cached,
+                          int32_t num_seqs, const int32_t* row_seq, int32_t num_rows,
+                          const uint32_t* mask, int32_t mask_words, int32_t num_heads,
+                          int32_t num_kv_heads, int32_t head_dim, int32_t block_size, float scale,
+                          int32_t dtype, const int64_t* positions, const float* rope_cos,
+                          const float* rope_sin, int32_t rope_max_position, hipStream_t stream);
+
+/* Which drafts the target keeps, and the token that follows them. Row r of probs
+ * [num_rows][vocab] is the target's distribution after node r, row r of draft_probs (or NULL) the
+ * one that node r's children were drawn from, independently; uniforms[r] in [0, 1) is node r's
+ * random number, the root's serves the token drawn at the end. From the root on, the children of
+ * the reached node are tried in row order, p its row, q its draft row, x the child's token:
+ *   draft_probs NULL: left = 1 - the sum of p over the tokens refused here; kept where p(x) > 0
+ *     and u left < p(x) (a token refused before holds 0);
+ *   otherwise: a = 0, s = 1 at first; kept where u q(x) s < p(x) - a q(x); a refusal makes
+ *     a += s, s = sum_i max(p_i - a q_i, 0).
+ * The emitted tokens then follow the target's distribution. The token after the path is the
+ * first i with w_0 + .. + w_i > u sum(w), w = p without the refused tokens or max(p - a q, 0);
+ * where w is all zero p itself, -1 where that is too. Entries that are NaN or below 0 count
+ * as 0; a token outside [0, vocab) is refused. All of it is decided in 64 bits.
+ *   parents [num_rows]: a node's parent inside its tree, smaller than itself; -1 for the root;
+ *   accepted [num_seqs][width]: the path's nodes from the root on, then -1;
+ *   num_accepted [num_seqs]: how many (0 for a sequence without rows);
+ *   out_tokens [num_seqs][width] (int64): the path's tokens behind the root, then the token
+ *     drawn: num_accepted of them, then -1. width >= every tree's nodes.
+ * dtype is that of probs and draft_probs; row strides in elements. */
+int32_t tb_tree_verify(const void* probs, int64_t probs_row_stride, const void* draft_probs,
+                       int64_t draft_row_stride, int32_t vocab, int32_t dtype, const int64_t* tokens,
+                       const float* uniforms, const int32_t* parents, const int32_t* row_starts,
+                       int32_t num_seqs, int32_t* accepted, int32_t* num_accepted, int64_t* out_tokens,
+                       int32_t width, hipStream_t stream);
+
+/* The same for greedy decoding: target_ids [num_rows] (int64) is the target's choice after each
+ * node (tb_linear_argmax); the first child that holds it is kept. Trees of any size. */
+int32_t tb_tree_verify_greedy(const int64_t* target_ids, const int64_t* tokens, const int32_t* parents,
+                              const int32_t* row_starts, int32_t num_seqs, int32_t* accepted,
+                              int32_t* num_accepted, int64_t* out_tokens, int32_t width,
+                              hipStream_t stream);
+
+/* Moves the kept nodes' K/V rows to the positions they now have, in every layer: the row at
+ * position cached + accepted[b][j] to position cached + j, j < num_accepted[b]. accepted and
+ * num_accepted are tb_tree_verify's (device memory; rising nodes, entries past the count
+ * unread); entries not behind their place are in it already. storage: the layers' pools,
+ * layer_stride_bytes apart. Two sequences must not share the blocks that hold their nodes. */
+int32_t tb_tree_commit(void* storage, int32_t num_layers, int64_t layer_stride_bytes, int64_t num_blocks,
+                       const int32_t* block_tables, int32_t max_blocks_per_seq, const int32_t* cached,
+                       int32_t num_seqs, const int32_t* accepted, int32_t width,
+                       const int32_t* num_accepted, int32_t num_kv_heads, int32_t head_dim,
+                       int32_t block_size, int32_t dtype, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

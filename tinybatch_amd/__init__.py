@@ -6,6 +6,10 @@ PagedKVCache (src/tinybatch/kv_cache.py of the reference) on top.
 """
 from .metadata import StepMetadata, build_step_metadata
 from .kv_cache import PagedKVCache
+from .tree import (TreeMetadata, TreeVerdict, build_tree_metadata, commit_tree, tree_append, tree_attention,
+                   verify_tree, verify_tree_greedy)
 from . import ops
 
-__all__ = ["PagedKVCache", "StepMetadata", "build_step_metadata", "ops"]
+__all__ = ["PagedKVCache", "StepMetadata", "TreeMetadata", "TreeVerdict", "build_step_metadata",
+           "build_tree_metadata", "commit_tree", "ops", "tree_append", "tree_attention", "verify_tree",
+           "verify_tree_greedy"]

@@ -134,6 +134,17 @@ SIGNATURES = {
     "tb_block_copy": (c_i32, [c_vp, c_i32, c_i64, c_vp, c_vp, c_i32, c_i64, c_vp]),
     "tb_block_gather": (c_i32, [c_vp, c_i64, c_vp, c_i32, c_vp, c_i64, c_vp]),
     "tb_block_scatter": (c_i32, [c_vp, c_vp, c_i64, c_vp, c_i32, c_i64, c_vp]),
+    "tb_tree_attention": (c_i32, [
+        c_vp, c_i64, c_vp, c_i64, c_vp, c_i64,   # q, q stride, pool, num_blocks, out, out stride
+        c_vp, c_i32, c_vp, c_vp, c_i32, c_vp, c_i32,   # block tables, max_nb, row starts, cached, seqs, row_seq, rows
+        c_vp, c_i32,                             # mask, words
+        c_i32, c_i32, c_i32, c_i32, c_f32, c_i32,   # heads, kv heads, head_dim, block_size, scale, dtype
+        c_vp, c_vp, c_vp, c_i32, c_vp]),         # positions, rope cos, sin, max position, stream
+    "tb_tree_verify": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i32, c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp,
+                               c_vp, c_i32, c_vp]),
+    "tb_tree_verify_greedy": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp, c_i32, c_vp]),
+    "tb_tree_commit": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_vp, c_i32, c_vp, c_i32, c_vp, c_i32, c_vp, c_i32, c_i32,
+                               c_i32, c_i32, c_vp]),
     "tb_rms_norm": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i32, c_i32, c_f32, c_i32, c_vp]),
     "tb_rope_qk": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_i32,
                            c_vp]),

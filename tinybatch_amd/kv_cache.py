@@ -28,7 +28,7 @@ from __future__ import annotations
 import numpy as np
 import torch
 
-from . import _lib, ops
+from . import _lib, ops, tree
 from .metadata import StepMetadata, build_step_metadata, columns_pay
 
 
@@ -221,6 +221,30 @@ class PagedKVCache:
     def copy_blocks(self, src, dst) -> None:
         """pool_l[dst[i]] <- pool_l[src[i]] in every layer (K3, one launch)."""
         ops.block_copy(self.pools, src, dst)
+
+    # ---- speculative decoding (tree.py) --------------------------------------
+    def tree_metadata(self, parents, cached_lens, block_tables, *, num_heads: int, visible=None) -> tree.TreeMetadata:
+        """The metadata of a step whose rows are trees of drafted tokens (tree.build_tree_metadata),
+        uploaded: one for all layers of the step."""
+        return tree.build_tree_metadata(parents, cached_lens, block_tables, block_size=self.block_size,
+                                        num_blocks=self.num_blocks, num_heads=num_heads,
+                                        num_kv_heads=self.n_kv_heads, head_dim=self.head_dim, dtype=self.dtype,
+                                        visible=visible).to(self.device)
+
+    def tree_append(self, layer: int, k: torch.Tensor, v: torch.Tensor, meta: tree.TreeMetadata,
+                    rope: ops.Rope | None = None) -> None:
+        """The nodes' K/V rows into their slots, behind the cached positions."""
+        tree.tree_append(self.pools[layer], k, v, meta, rope=rope)
+
+    def tree_attention(self, layer: int, q: torch.Tensor, meta: tree.TreeMetadata, *, scale: float | None = None,
+                       out: torch.Tensor | None = None, rope: ops.Rope | None = None,
+                       mask: torch.Tensor | None = None) -> torch.Tensor:
+        """[T, Hq*D]: every node over its sequence's cached positions and the nodes it sees."""
+        return tree.tree_attention(q, self.pools[layer], meta, scale=scale, out=out, rope=rope, mask=mask)
+
+    def commit_tree(self, meta: tree.TreeMetadata, accepted: torch.Tensor, num_accepted: torch.Tensor) -> None:
+        """The kept nodes' rows to the positions they now have, in every layer (one launch)."""
+        tree.commit_tree(self.storage, meta, accepted, num_accepted)
 
     def swap_out(self, blocks, staging: list[torch.Tensor]) -> None:
         """staging[l][i] <- pools[l][blocks[i]] for every layer."""

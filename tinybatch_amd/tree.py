@@ -1,0 +1,396 @@
+"""Speculative decoding over the paged cache: steps whose rows are trees of drafted tokens.
+
+The reference decodes one token per sequence and step (src/tinybatch/engine.py:99-126); here a
+step carries, for every sequence, the last token it emitted (the root) and drafted tokens
+below it, each a child of an earlier node (a chain of drafts is the tree of one child each):
+
+    meta = cache.tree_metadata(parents, cached_lens, block_tables, num_heads=n_heads)
+    for layer in range(n_layers):                       # q, k, v of all nodes, before rotation
+        cache.tree_append(layer, k, v, meta, rope=rope)
+        attn = cache.tree_attention(layer, q, meta, rope=rope)
+    verdict = verify_tree(meta, tokens, uniforms, probs, draft_probs)   # or verify_tree_greedy
+    cache.commit_tree(meta, verdict.accepted, verdict.num_accepted)
+    # sequence b has emitted verdict.tokens[b, :num_accepted[b]] and has
+    # cached_lens[b] + num_accepted[b] positions in its cache; the last token is the next root
+
+Everything is enqueued on the tensors' device's current stream, nothing synchronises; the
+verdict stays on the device and the commit reads it there.
+"""
+from __future__ import annotations
+
+import contextlib
+import math
+from dataclasses import dataclass
+from typing import NamedTuple
+
+import numpy as np
+import torch
+
+from . import _lib
+from .metadata import pad4
+from .ops import Rope, _check_pool, _rows_view, kv_append
+
+MAX_NODES = 1024             # TB_TREE_MAX_NODES
+
+
+@dataclass
+class TreeMetadata:
+    """One step's trees: built by build_tree_metadata, uploaded by ``to`` and used by every
+    layer's calls."""
+    num_rows: int
+    num_seqs: int
+    max_nodes: int               # nodes of the largest tree
+    mask_words: int              # 32-bit words of a row's mask
+    # the cache part (None / 0 without cached_lens)
+    block_size: int
+    num_blocks: int
+    max_blocks_per_seq: int
+    num_heads: int | None
+    num_kv_heads: int | None
+    head_dim: int | None
+    dtype: torch.dtype | None
+    # host copies
+    parents_np: np.ndarray       # [T] inside the tree, -1 for a root
+    row_starts_np: np.ndarray    # [B + 1]
+    depths_np: np.ndarray        # [T]
+    mask_np: np.ndarray          # [T, mask_words] uint32
+    row_seq_np: np.ndarray       # [T]
+    cached_np: np.ndarray | None
+    block_tables_np: np.ndarray | None
+    slot_mapping_np: np.ndarray | None
+    # device views (one backing buffer)
+    device: torch.device | None = None
+    parents: torch.Tensor | None = None
+    row_starts: torch.Tensor | None = None
+    mask: torch.Tensor | None = None          # [T, mask_words] int32
+    row_seq: torch.Tensor | None = None
+    positions: torch.Tensor | None = None     # [T] int64: cached + depth, the nodes' RoPE positions
+    cached: torch.Tensor | None = None
+    block_tables: torch.Tensor | None = None
+    slot_mapping: torch.Tensor | None = None
+
+    def to(self, device: torch.device) -> "TreeMetadata":
+        """Upload every array with one host-to-device copy (views into one buffer)."""
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        has_cache = self.cached_np is not None
+        start = self.cached_np[self.row_seq_np] if has_cache else 0
+        positions = (self.depths_np + start).astype(np.int64)
+        parts = [("positions", positions.view(np.int32)), ("parents", self.parents_np),
+                 ("row_starts", self.row_starts_np), ("mask", self.mask_np.view(np.int32).reshape(-1)),
+                 ("row_seq", self.row_seq_np)]
+        if has_cache:
+            parts += [("cached", self.cached_np), ("block_tables", self.block_tables_np.reshape(-1)),
+                      ("slot_mapping", self.slot_mapping_np)]
+        host = np.zeros(sum(pad4(x.size) for _, x in parts), dtype=np.int32)
+        at, spans = 0, {}
+        for name, x in parts:
+            host[at:at + x.size] = x
+            spans[name] = (at, x.size)
+            at += pad4(x.size)
+        src = torch.from_numpy(host)
+        if device.type == "cuda":
+            src = src.pin_memory()
+        buf = src.to(device, non_blocking=True)
+        for name, (o, size) in spans.items():
+            setattr(self, name, buf.narrow(0, o, size))
+        self.positions = self.positions.view(torch.int64)
+        self.mask = self.mask.view(-1, self.mask_words)
+        if has_cache:
+            self.block_tables = self.block_tables.view(-1, self.max_blocks_per_seq)
+        self.device = device
+        return self
+
+
+def _masks(parents, visible, words: int) -> np.ndarray:
+    """[T, words] uint32: bit j of row i = node j is seen by node i."""
+    raw = bytearray()
+    size = 4 * words
+    for b, tree in enumerate(parents):
+        if visible is not None and visible[b] is not None:
+            v = np.asarray(visible[b], dtype=bool)
+            if v.shape != (len(tree), len(tree)):
+                raise ValueError(f"visible[{b}] must be [{len(tree)}, {len(tree)}], got {v.shape}")
+            rows = np.packbits(v, axis=1, bitorder="little")
+            full = np.zeros((len(tree), size), dtype=np.uint8)
+            full[:, :rows.shape[1]] = rows
+            raw += full.tobytes()
+            continue
+        seen: list[int] = []
+        for i, p in enumerate(tree):
+            seen.append((seen[p] if p >= 0 else 0) | (1 << i))
+        for m in seen:
+            raw += m.to_bytes(size, "little")
+    return np.frombuffer(bytes(raw), dtype=np.uint32).reshape(-1, words)
+
+
+def build_tree_metadata(parents, cached_lens=None, block_tables=None, *, block_size: int = 0, num_blocks: int = 0,
+                        num_heads: int | None = None, num_kv_heads: int | None = None, head_dim: int | None = None,
+                        dtype: torch.dtype | None = None, visible=None) -> TreeMetadata:
+    """The metadata of a step of trees (host lists in, ``to(device)`` uploads it).
+
+    parents[b][i] is the parent of sequence b's node i inside its tree: -1 for node 0, the
+    root, and an earlier node for every other (no nodes: a sequence without rows). The step's
+    flat rows are the trees one behind the other. cached_lens[b] positions of sequence b are in
+    the cache; block_tables[b] covers them and one position per node behind them (node i at
+    cached_lens[b] + i). Without cached_lens the trees alone (verify_tree needs no more).
+
+    A node sees the cached positions, itself and its ancestors, or the nodes that
+    visible[b] ([nodes, nodes] booleans, row i for node i) names; a row that sees nothing
+    gives 0.
+
+    A table too short, or a block id outside the pool, raises IndexError; two nodes of the step
+    in one slot raise ValueError.
+    """
+    parents = [list(t) for t in parents]
+    sizes = [len(t) for t in parents]
+    max_nodes = max(sizes, default=0)
+    if max_nodes > MAX_NODES:
+        raise ValueError(f"a tree of {max_nodes} nodes; at most {MAX_NODES} are served")
+    depths: list[int] = []
+    for b, tree in enumerate(parents):
+        first = len(depths)
+        for i, p in enumerate(tree):
+            if (p != -1) if i == 0 else not 0 <= p < i:
+                raise ValueError(f"parents[{b}][{i}] is {p}: node 0 has parent -1, every other node an earlier one")
+            depths.append(0 if i == 0 else depths[first + p] + 1)
+    if visible is not None and len(visible) != len(parents):
+        raise ValueError("visible needs one entry per sequence")
+    words = max(1, -(-max_nodes // 32))
+    row_starts = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32)
+    T, B = int(row_starts[-1]), len(parents)
+    meta = TreeMetadata(
+        num_rows=T, num_seqs=B, max_nodes=max_nodes, mask_words=words, block_size=block_size, num_blocks=num_blocks,
+        max_blocks_per_seq=0, num_heads=num_heads, num_kv_heads=num_kv_heads, head_dim=head_dim, dtype=dtype,
+        parents_np=np.array([p for t in parents for p in t], dtype=np.int32), row_starts_np=row_starts,
+        depths_np=np.array(depths, dtype=np.int64), mask_np=_masks(parents, visible, words),
+        row_seq_np=np.repeat(np.arange(B, dtype=np.int32), sizes), cached_np=None, block_tables_np=None,
+        slot_mapping_np=None)
+    if cached_lens is None:
+        if block_tables is not None:
+            raise ValueError("block_tables without cached_lens")
+        return meta
+    if block_tables is None or len(block_tables) != B or len(cached_lens) != B:
+        raise ValueError("cached_lens and block_tables need one entry per sequence")
+    if block_size <= 0 or block_size & (block_size - 1) or num_blocks <= 0:
+        raise ValueError("block_size must be a power of two and num_blocks positive")
+    if num_heads is None or num_kv_heads is None or head_dim is None or dtype not in _lib.DTYPE_CODE:
+        raise ValueError("num_heads, num_kv_heads, head_dim and dtype (fp32, fp16, bf16) describe the attention's calls")
+    if num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads:
+        raise ValueError(f"num_heads {num_heads} is not a multiple of kv heads {num_kv_heads}")
+    cached = np.array([int(c) for c in cached_lens], dtype=np.int64)
+    ends = cached + np.array(sizes, dtype=np.int64)
+    if B and (cached.min() < 0 or ends.max() > (1 << 30)):
+        raise ValueError("cached_lens must be >= 0 (and a context at most 2^30 positions)")
+    need = -(-ends // block_size)
+    for b, table in enumerate(block_tables):
+        if need[b] > len(table):
+            raise IndexError(f"sequence {b} needs {need[b]} blocks for {ends[b]} positions, table has {len(table)}")
+    max_nb = max(1, int(need.max()) if B else 1)
+    tables = np.zeros((B, max_nb), dtype=np.int32)
+    for b, table in enumerate(block_tables):
+        ids = np.asarray(table[:need[b]], dtype=np.int64)
+        if ids.size and (ids.min() < 0 or ids.max() >= num_blocks):
+            raise IndexError(f"block_tables[{b}] holds a block id outside the pool of {num_blocks} blocks")
+        tables[b, :need[b]] = ids
+    seq = meta.row_seq_np
+    pos = cached[seq] + np.arange(T) - row_starts[:-1][seq]
+    slots = tables[seq, pos // block_size].astype(np.int64) * block_size + pos % block_size
+    if np.unique(slots).size != T:
+        raise ValueError("two nodes of the step share a pool slot: give each tree blocks of its own")
+    if T and slots.max() > np.iinfo(np.int32).max:
+        raise ValueError("a pool of more than 2^31 slots")
+    meta.cached_np = cached.astype(np.int32)
+    meta.block_tables_np = tables
+    meta.max_blocks_per_seq = max_nb
+    meta.slot_mapping_np = slots.astype(np.int32)
+    return meta
+
+
+def _on(device: torch.device):
+    """The launch's device made the current one where it is not."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _check_meta(meta: TreeMetadata, device: torch.device, cache: bool) -> None:
+    if meta.device is None:
+        raise ValueError("metadata has not been uploaded (call meta.to(device))")
+    if meta.device != device:
+        raise ValueError(f"metadata is on {meta.device}, the tensors on {device}")
+    if cache and meta.cached is None:
+        raise ValueError("metadata was built without cached_lens and block_tables")
+
+
+def tree_append(pool: torch.Tensor, k: torch.Tensor, v: torch.Tensor, meta: TreeMetadata,
+                rope: Rope | None = None) -> None:
+    """The nodes' K/V rows [T, kv_heads, head_dim] into their slots (ops.kv_append); with ``rope``
+    k is the projection before rotation, rotated at cached + depth on the way."""
+    _check_meta(meta, pool.device, True)
+    if pool.dim() == 5 and (pool.shape[3] != meta.block_size or pool.shape[0] < meta.num_blocks):
+        raise ValueError(f"metadata is for {meta.num_blocks} blocks of {meta.block_size} positions")
+    with _on(pool.device):
+        kv_append(pool, k, v, meta.slot_mapping, rope=rope, positions=meta.positions if rope is not None else None)
+
+
+def tree_attention(q: torch.Tensor, pool: torch.Tensor, meta: TreeMetadata, *, scale: float | None = None,
+                   out: torch.Tensor | None = None, rope: Rope | None = None,
+                   mask: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of every node of the step over its sequence's cached positions and the nodes it
+    sees (tb_tree_attention); the nodes' K/V must be in the pool (tree_append, same stream).
+
+    q: [T, num_heads, head_dim] in the pool's dtype; returns [T, num_heads * head_dim]. ``scale``:
+    1 / sqrt(head_dim) by default. With ``rope`` q is the projection before rotation. ``mask``
+    ([T, meta.mask_words] int32 on the GPU, bit j % 32 of word j / 32: node j is seen) replaces the
+    metadata's, for masks made on the device. A row that sees nothing gives 0.
+    """
+    nb, hkv, bs, d = _check_pool(pool)
+    _lib.require_gpu_tensor("q", q)
+    if q.device != pool.device:
+        raise ValueError(f"q is on {q.device}, the pool on {pool.device}")
+    _check_meta(meta, pool.device, True)
+    if q.dtype != pool.dtype or q.dtype != meta.dtype:
+        raise TypeError(f"q {q.dtype}, pool {pool.dtype} and metadata {meta.dtype} differ in dtype")
+    if (hkv, d, bs) != (meta.num_kv_heads, meta.head_dim, meta.block_size) or nb < meta.num_blocks:
+        raise ValueError(f"metadata is for {meta.num_blocks} blocks of {meta.block_size} positions, "
+                         f"{meta.num_kv_heads} kv heads of {meta.head_dim}; the pool is {tuple(pool.shape)}")
+    hq, T = meta.num_heads, meta.num_rows
+    qs = _rows_view("q", q, hq, d)
+    if q.shape[0] != T:
+        raise ValueError(f"q has {q.shape[0]} rows, metadata describes {T}")
+    if out is None:
+        out = torch.empty(T, hq * d, device=q.device, dtype=q.dtype)
+    else:
+        _lib.require_gpu_tensor("out", out)
+        if out.dtype != q.dtype or out.shape[0] != T or out.device != q.device:
+            raise ValueError("out must match q's dtype, device and row count")
+    os_ = _rows_view("out", out, hq, d)
+    if mask is None:
+        mask = meta.mask
+    elif (mask.dtype != torch.int32 or mask.device != q.device or mask.shape != (T, meta.mask_words)
+          or not mask.is_contiguous()):
+        raise TypeError(f"mask must be a contiguous int32 [{T}, {meta.mask_words}] tensor on {q.device}")
+    if rope is not None:
+        rope.check(d, q.device)
+    with _on(q.device):
+        st = _lib.lib().tb_tree_attention(
+            q.data_ptr(), qs, pool.data_ptr(), nb, out.data_ptr(), os_, meta.block_tables.data_ptr(),
+            meta.max_blocks_per_seq, meta.row_starts.data_ptr(), meta.cached.data_ptr(), meta.num_seqs,
+            meta.row_seq.data_ptr(), T, mask.data_ptr(), meta.mask_words, hq, hkv, d, bs,
+            1.0 / math.sqrt(d) if scale is None else float(scale), _lib.DTYPE_CODE[q.dtype], meta.positions.data_ptr(),
+            None if rope is None else rope.cos.data_ptr(), None if rope is None else rope.sin.data_ptr(),
+            0 if rope is None else rope.max_position, _lib.stream_handle(q.device))
+    _lib.check(st, "tb_tree_attention")
+    return out
+
+
+class TreeVerdict(NamedTuple):
+    """What a verification kept, on the device."""
+    accepted: torch.Tensor       # [B, max_nodes] int32: the path's nodes from the root on, then -1
+    num_accepted: torch.Tensor   # [B] int32: how many (0 for a sequence without rows)
+    tokens: torch.Tensor         # [B, max_nodes] int64: num_accepted tokens emitted (the last one drawn), then -1
+
+
+def _verdict(meta: TreeMetadata, device: torch.device) -> TreeVerdict:
+    width = max(meta.max_nodes, 1)
+    return TreeVerdict(torch.empty(meta.num_seqs, width, dtype=torch.int32, device=device),
+                       torch.empty(meta.num_seqs, dtype=torch.int32, device=device),
+                       torch.empty(meta.num_seqs, width, dtype=torch.int64, device=device))
+
+
+def _node_values(name: str, t: torch.Tensor, dtype: torch.dtype, rows: int, device: torch.device) -> None:
+    if t.dtype != dtype or t.device != device or t.shape != (rows,) or not t.is_contiguous():
+        raise TypeError(f"{name} must be a contiguous {dtype} [{rows}] tensor on {device}")
+
+
+def verify_tree(meta: TreeMetadata, tokens: torch.Tensor, uniforms: torch.Tensor, probs: torch.Tensor,
+                draft_probs: torch.Tensor | None = None) -> TreeVerdict:
+    """Which drafts the target's probabilities keep, and the token after them (tb_tree_verify;
+    the rule is written there): the emitted tokens follow the target's distribution.
+
+    probs [T, vocab] (fp32, fp16 or bf16, rows that sum to 1): row r the target's distribution
+    after node r. tokens [T] int64. uniforms [T] fp32 in [0, 1): one random number per node; the
+    root's serves the token drawn at the end. draft_probs, in probs' dtype: row r the distribution
+    that node r's children were drawn from, each independently; None for drafts that were not
+    drawn at random (a draft model's most likely tokens).
+    """
+    _lib.require_gpu_tensor("probs", probs)
+    device, T = probs.device, meta.num_rows
+    _check_meta(meta, device, False)
+    if probs.dtype not in _lib.DTYPE_CODE:
+        raise TypeError(f"unsupported probs dtype {probs.dtype}")
+    for name, t in (("probs", probs), ("draft_probs", draft_probs)):
+        if t is None:
+            continue
+        if t.dim() != 2 or t.shape != probs.shape or t.shape[0] != T or t.shape[1] < 1 or t.stride(1) != 1:
+            raise ValueError(f"{name} must be [{T}, vocab] with contiguous rows, got {tuple(t.shape)}")
+        if t.dtype != probs.dtype or t.device != device:
+            raise TypeError(f"{name} must share probs' dtype and device")
+    vocab = probs.shape[1]
+    if vocab >= 1 << 30:
+        raise ValueError("a vocabulary of 2^30 tokens or more")
+    _node_values("tokens", tokens, torch.int64, T, device)
+    _node_values("uniforms", uniforms, torch.float32, T, device)
+    v = _verdict(meta, device)
+    if T == 0:
+        return v._replace(accepted=v.accepted.fill_(-1), num_accepted=v.num_accepted.zero_(), tokens=v.tokens.fill_(-1))
+    with _on(device):
+        st = _lib.lib().tb_tree_verify(
+            probs.data_ptr(), max(probs.stride(0), vocab), None if draft_probs is None else draft_probs.data_ptr(),
+            0 if draft_probs is None else max(draft_probs.stride(0), vocab), vocab, _lib.DTYPE_CODE[probs.dtype],
+            tokens.data_ptr(), uniforms.data_ptr(), meta.parents.data_ptr(), meta.row_starts.data_ptr(),
+            meta.num_seqs, v.accepted.data_ptr(), v.num_accepted.data_ptr(), v.tokens.data_ptr(),
+            v.accepted.shape[1], _lib.stream_handle(device))
+    _lib.check(st, "tb_tree_verify")
+    return v
+
+
+def verify_tree_greedy(meta: TreeMetadata, tokens: torch.Tensor, target_ids: torch.Tensor) -> TreeVerdict:
+    """verify_tree for greedy decoding: target_ids [T] int64 is the target's choice after each node
+    (layer_ops.linear_argmax, or an argmax of the logits); a child that holds it is kept."""
+    _lib.require_gpu_tensor("target_ids", target_ids)
+    device, T = target_ids.device, meta.num_rows
+    _check_meta(meta, device, False)
+    _node_values("target_ids", target_ids, torch.int64, T, device)
+    _node_values("tokens", tokens, torch.int64, T, device)
+    v = _verdict(meta, device)
+    if T == 0:
+        return v._replace(accepted=v.accepted.fill_(-1), num_accepted=v.num_accepted.zero_(), tokens=v.tokens.fill_(-1))
+    with _on(device):
+        st = _lib.lib().tb_tree_verify_greedy(
+            target_ids.data_ptr(), tokens.data_ptr(), meta.parents.data_ptr(), meta.row_starts.data_ptr(),
+            meta.num_seqs, v.accepted.data_ptr(), v.num_accepted.data_ptr(), v.tokens.data_ptr(),
+            v.accepted.shape[1], _lib.stream_handle(device))
+    _lib.check(st, "tb_tree_verify_greedy")
+    return v
+
+
+def commit_tree(storage: torch.Tensor, meta: TreeMetadata, accepted: torch.Tensor,
+                num_accepted: torch.Tensor) -> None:
+    """The kept nodes' K/V rows to the positions they now have, in every layer (tb_tree_commit):
+    position cached + accepted[b][j] to cached + j. storage: the layers' pools
+    [layers, num_blocks, 2, kv_heads, block_size, head_dim] (PagedKVCache.storage); accepted
+    and num_accepted as verify_tree gives them (nodes rising along a row)."""
+    _lib.require_gpu_tensor("storage", storage)
+    if storage.dim() != 6 or storage.shape[2] != 2 or not storage.is_contiguous():
+        raise ValueError("storage must be a contiguous [layers, num_blocks, 2, kv_heads, block_size, head_dim] tensor")
+    if storage.dtype not in _lib.DTYPE_CODE:
+        raise TypeError(f"unsupported pool dtype {storage.dtype}")
+    device = storage.device
+    _check_meta(meta, device, True)
+    layers, nb, _, hkv, bs, d = storage.shape
+    if bs != meta.block_size or nb < meta.num_blocks:
+        raise ValueError(f"metadata is for {meta.num_blocks} blocks of {meta.block_size} positions")
+    B = meta.num_seqs
+    if (accepted.dtype != torch.int32 or accepted.device != device or accepted.dim() != 2
+            or accepted.shape[0] != B or accepted.shape[1] < 1 or not accepted.is_contiguous()):
+        raise TypeError(f"accepted must be a contiguous int32 [{B}, nodes] tensor on {device}")
+    _node_values("num_accepted", num_accepted, torch.int32, B, device)
+    with _on(device):
+        st = _lib.lib().tb_tree_commit(
+            storage.data_ptr(), layers, storage.stride(0) * storage.element_size(), nb, meta.block_tables.data_ptr(),
+            meta.max_blocks_per_seq, meta.cached.data_ptr(), B, accepted.data_ptr(), accepted.shape[1],
+            num_accepted.data_ptr(), hkv, d, bs, _lib.DTYPE_CODE[storage.dtype], _lib.stream_handle(device))
+    _lib.check(st, "tb_tree_commit")
