@@ -687,16 +687,35 @@ int32_t tb_rms_norm_partials(const float* partials, int32_t splits, void* residu
  *   row_seq [num_rows]: each row's sequence (-1: a row of none, left as it is);
  *   mask [num_rows][mask_words] 32-bit words, bit j % 32 of word j / 32 = node j is seen; bits
  *     past the tree are ignored;
+ *   work [num_work][12], split_rows [num_split_rows][4], column_blocks, partial_slots:
+ *     tb_build_tree_work's for this call's sizes (device memory, 16-byte aligned; block_size < 16
+ *     needs none); workspace: tb_tree_attention_workspace_bytes, 16-byte aligned, for contexts cut
+ *     into parts. Calls that may overlap in time need their own workspace;
  *   positions [num_rows] (int64) with rope tables: q holds the projections before rotation and is
  *     rotated at them (as tb_kv_append_rope rotates k). */
 int32_t tb_tree_attention(const void* q, int64_t q_row_stride, const void* pool, int64_t num_blocks,
                           void* out, int64_t out_row_stride, const int32_t* block_tables,
                           int32_t max_blocks_per_seq, const int32_t* row_starts, const int32_t* cached,
                           int32_t num_seqs, const int32_t* row_seq, int32_t num_rows,
-                          const uint32_t* mask, int32_t mask_words, int32_t num_heads,
-                          int32_t num_kv_heads, int32_t head_dim, int32_t block_size, float scale,
+                          const uint32_t* mask, int32_t mask_words, const int32_t* work,
+                          int32_t num_work, int32_t column_blocks, const int32_t* split_rows,
+                          int32_t num_split_rows, int32_t partial_slots, void* workspace,
+                          size_t workspace_bytes, int32_t num_heads, int32_t num_kv_heads,
+                          int32_t head_dim, int32_t block_size, float scale,
                           int32_t dtype, const int64_t* positions, const float* rope_cos,
                           const float* rope_sin, int32_t rope_max_position, hipStream_t stream);
+
+/* The work list of tb_tree_attention (host memory, no device call): cached [num_seqs] positions and
+ * nodes [num_seqs] rows of each sequence, in row order, on a GPU of num_cus CUs and num_xcds XCDs.
+ * counts [4]: work entries (12 int32 each), split rows (4 int32 each), partial slots, column
+ * blocks per workgroup. work and split NULL: the counts alone. An entry is (first row, sequence,
+ * cached, nodes, first column, kv head, first chunk of 32 positions, chunks, partial slot of node 0
+ * or -1, 0, 0, 0), with 0 nodes for a padding entry; entry g is meant for XCD g % num_xcds. */
+int32_t tb_build_tree_work(const int32_t* cached, const int32_t* nodes, int32_t num_seqs,
+                           int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
+                           int32_t num_cus, int32_t num_xcds, int32_t* work, int32_t work_capacity,
+                           int32_t* split, int32_t split_capacity, int32_t* counts);
+size_t tb_tree_attention_workspace_bytes(int32_t partial_slots, int32_t num_heads, int32_t head_dim);
 
 /* Which drafts the target keeps, and the token that follows them. Row r of probs
  * [num_rows][vocab] is the target's distribution after node r, row r of draft_probs (or NULL) the

@@ -426,7 +426,7 @@ def test_verify_greedy(sizes):
 
 
 # ---- commit ---------------------------------------------------------------------------
-@pytest.mark.parametrize("dtype,hkv,d,bs", [(torch.bfloat16, 2, 64, 16), (torch.float32, 8, 128, 32), (torch.float16, 1, 8, 4)])
+@pytest.mark.parametrize("dtype,hkv,d,bs", [(torch.bfloat16, 2, 64, 16), (torch.float32, 8, 128, 32), (torch.float16, 1, 64, 4)])
 def test_commit_moves_rows_and_nothing_else(dtype, hkv, d, bs):
     g = torch.Generator().manual_seed(bs)
     parents = random_trees(2, [1, 40, 0, 9, 200, 17])

@@ -46,6 +46,38 @@ struct smath<bf16_t> {
   }
 };
 
+// The 32x32x16 products of a 16-bit type, and sums of its packed pairs.
+typedef float float16_t __attribute__((ext_vector_type(16)));
+
+template <typename Tag>
+struct cmath;
+template <>
+struct cmath<f16_t> {
+  typedef shalf8_t vec8_t;
+  static __device__ __forceinline__ float16_t mfma(su32x4_t a, su32x4_t b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(shalf8_t, a), __builtin_bit_cast(shalf8_t, b), c,
+                                                   0, 0, 0);
+  }
+  // acc + the two halves of p (times one each); subnormal halves count, as in the products
+  // (measured: thousands of weights of 2^-16 .. 2^-22 beside one of 1)
+  static __device__ __forceinline__ float add2(uint32_t p, uint32_t ones, float acc) {
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(half2_t, p), __builtin_bit_cast(half2_t, ones), acc, false);
+  }
+  static constexpr uint32_t ONES = 0x3C003C00u;
+};
+template <>
+struct cmath<bf16_t> {
+  typedef sbf168_t vec8_t;
+  static __device__ __forceinline__ float16_t mfma(su32x4_t a, su32x4_t b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(sbf168_t, a), __builtin_bit_cast(sbf168_t, b),
+                                                    c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ float add2(uint32_t p, uint32_t ones, float acc) {
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf162_t, p), __builtin_bit_cast(bf162_t, ones), acc, false);
+  }
+  static constexpr uint32_t ONES = 0x3F803F80u;
+};
+
 // The LDS layout of a 16-position tile: K row r keeps its 16-byte chunk c in
 // slot c ^ (r & 7), so the A-operand reads (16 rows x 16 bytes per 16 lanes) cover
 // every bank; V row r keeps chunk c in slot c ^ 2 (r & 3), so do the transpose

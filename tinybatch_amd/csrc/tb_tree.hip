@@ -7,7 +7,28 @@
 //   out[i][h] = sum_{t in S_i} e^(s_t - m) v_t / sum_{t in S_i} e^(s_t - m),  s_t = scale q[i][h] . k_t,
 // with m the running maximum of the scores seen so far. A node that sees nothing gives 0.
 // What a node does not see has no effect on it, also where it is infinite or NaN.
-#include "tb_common.h"
+//
+// Work: the n nodes and the rep query heads of a kv head make n * rep columns, column =
+// node * rep + head, that read the same K/V rows whatever their masks. A workgroup takes
+// 32 CB consecutive columns of a (sequence, kv head) and a part of the context; its waves
+// take the part's chunks of 32 positions in turn, each through a ring of its own in LDS
+// filled by direct global->LDS loads, with no barrier between them, and join their softmax
+// states in LDS at the end. A context cut into parts leaves a partial per part, joined by
+// a second launch.
+//
+// Math per chunk and block of 32 columns (C rows are positions or dims, C columns the block's):
+//   S^T[pos][col] = K[pos][:] . q[col][:]        A = K rows from LDS, B = q in registers
+//   O^T[d][col]  += V^T[d][pos] . P^T[pos][col]  A = V^T from LDS, B = the S^T registers
+// 16-bit: v_mfma_f32_32x32x16, V^T by LDS transpose reads; the weights P are rounded to the
+// element type for the product, and their sum is taken of the rounded ones. fp32:
+// v_mfma_f32_32x32x2_f32, nothing rounded further. The reference maximum of a column moves
+// only when a score outgrows it by 8 (weights to 2^8), so that the accumulators are rescaled
+// a few times per context.
+#include <algorithm>
+#include <exception>
+#include <vector>
+
+#include "tb_stream.h"
 
 namespace tb {
 
@@ -30,10 +51,24 @@ struct tree_args {
   float scale;
   const int64_t* positions;    // [T], for the rotation of q
   rope_tables rope;
+  const int4* work;            // three per workgroup, see tb_build_tree_work
+  const int4* split;           // (row, first partial slot, parts, slots between parts)
+  float* ws_acc;               // [slots][Hq][D]
+  float* ws_ml;                // [slots][Hq][2]
+  float scale_log2e;           // > 0: the scale's size times log2(e), or 1 for a scale of 0
+  float q_sign;                // 1, -1 or 0 (NaN: a NaN scale): multiplies q, so that masked scores stay -inf
 };
 
-// One wave per (row, head), lane l the positions l, l + 64, ...: each lane holds a softmax
-// state of its own, merged across the wave at the end. Any block size.
+// Whether node `row` of a tree of n nodes with `cached` positions before it sees anything.
+__device__ __forceinline__ bool tree_sees(const uint32_t* mask, int cached, int n) {
+  if (cached > 0) return true;
+  for (int w = 0; 32 * w < n; ++w)
+    if (mask[w] & (n - 32 * w >= 32 ? ~0u : (1u << (n - 32 * w)) - 1)) return true;
+  return false;
+}
+
+// Blocks of fewer than 16 positions: one wave per (row, head), lane l the positions l, l + 64, ...: each
+// lane holds a softmax state of its own, merged across the wave at the end.
 template <typename Tag, int D>
 __global__ __launch_bounds__(64) void tree_rows_kernel(const tree_args a) {
   using T = typename elem<Tag>::type;
@@ -126,6 +161,507 @@ __global__ __launch_bounds__(64) void tree_rows_kernel(const tree_args a) {
   }
 }
 
+
+// ---- column blocks over the matrix unit --------------------------------------------
+template <typename Tag, int D>
+struct tshape {
+  static constexpr int EB = elem<Tag>::bytes;
+  static constexpr int RB = EB * D;             // bytes per K or V row
+  static constexpr int TB = 16 * RB;            // bytes of a 16-position tile
+  static constexpr int CK = 32;                 // positions per chunk
+  static constexpr int HALF = CK * RB;          // a chunk's K (or V) rows
+  static constexpr int SLOT = 2 * HALF;
+  static constexpr int PPR = RB / 16;           // 16-byte pieces per row
+  static constexpr int RPL = 64 / PPR;          // rows per direct load
+  static constexpr int LD = HALF / 1024;        // direct loads per half
+  static constexpr int QS = PPR / 2;            // 16-byte pieces of a lane's q (the other half's lane holds the rest)
+  static constexpr int NB = D / 32;             // O^T blocks of 32 dims
+  // K row r keeps its piece p in slot p ^ kswz(r), V row r in slot p ^ vswz(r), so that the operand
+  // reads of 16 (K) and 32 (V, 16-bit transpose reads) lanes cover all 64 banks
+  static __device__ __forceinline__ int kswz(int r) { return RB == 128 ? (r & 7) ^ ((r >> 3) & 1) : r & 15; }
+  static __device__ __forceinline__ int vswz(int r) {
+    return EB == 4 ? 0 : D == 64 ? 2 * (r & 3) : (0xCA60 >> (4 * (r & 3))) & 15;
+  }
+};
+
+template <typename Tag, int D, int CB, int NW, int R, int OCC>
+__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
+void tree_columns_kernel(const tree_args a) {
+  using S = tshape<Tag, D>;
+  using T = typename elem<Tag>::type;
+  constexpr int RB = S::RB, CK = S::CK, NB = S::NB, QS = S::QS, LD = S::LD;
+  constexpr bool F32 = S::EB == 4;
+  constexpr int MERGE = NW * 64 * (16 * NB + 2) * 4;
+  constexpr int LDS = NW * R * S::SLOT > MERGE ? NW * R * S::SLOT : MERGE;
+  __shared__ __align__(1024) char lds_all[LDS];
+
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, lcol = lane & 31, half = lane >> 5;
+  const int4 w0 = a.work[3 * blockIdx.x], w1 = a.work[3 * blockIdx.x + 1], w2 = a.work[3 * blockIdx.x + 2];
+  const int row0 = w0.x, seq = w0.y, cached = w0.z, nodes = w0.w;
+  if (nodes == 0) return;                       // a padding entry (whole workgroup)
+  const int col0 = w1.x, kvh = w1.y, chunk0 = w1.z, chunks = w1.w;
+  const int limit = cached + nodes, ncols = nodes * a.rep;
+  char* const lds = lds_all + wave * (R * S::SLOT);
+
+  // this lane's columns: node my_row, head hd (past the last column: a repeat, not stored)
+  int my_row[CB], hd[CB];
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    const int col = min(col0 + 32 * cb + lcol, ncols - 1);
+    my_row[cb] = col / a.rep;
+    hd[cb] = kvh * a.rep + col - my_row[cb] * a.rep;
+  }
+  // ---- q (B operand: dims 8 half .. of every 16 in 16 bits, 4 half .. of every 8 in fp32) ----
+  vec16 q[CB][QS];
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    const char* const qrow = a.q + (int64_t)(row0 + my_row[cb]) * a.q_row_bytes + (int64_t)hd[cb] * RB + 16 * half;
+#pragma unroll
+    for (int s = 0; s < QS; ++s) q[cb][s] = ld16(qrow + 32 * s);
+  }
+
+  // ---- direct loads: the wave's k-th chunk is chunk0 + wave + NW k ----
+  const int64_t head_bytes = ((int64_t)1 << a.log2_bs) * RB;
+  const int64_t blk_bytes = 2 * (int64_t)a.num_kv_heads * head_bytes, v_off = a.num_kv_heads * head_bytes;
+  const int sub_mask = (1 << (a.log2_bs - 4)) - 1;                // 16-position tiles per block - 1
+  const int32_t* const table = a.block_tables + (int64_t)seq * a.max_nb;
+  const char* const pool_kvh = a.pool + kvh * head_bytes;
+  const int last_tile = (limit - 1) >> 4;
+  const int lrow = lane / S::PPR, lpiece = lane % S::PPR;
+  const int n = (chunks - wave + NW - 1) / NW;                    // this wave's chunks (<= 0: none)
+  int id0 = 0;
+  auto load_ids = [&](int k) {                  // lane j: the block of tile j % 2 of chunk k + j / 2
+    const int t = min(2 * (chunk0 + wave + NW * (k + (lane >> 1))) + (lane & 1), last_tile);
+    const int b = table[(t << 4) >> a.log2_bs];
+    return (b < 0 || b >= a.num_blocks) ? 0 : b;   // host validates; stay inside the pool
+  };
+  int ids = load_ids(0);
+  asm volatile("" : "+v"(ids));                 // the block ids have landed: no wait inside the loop
+  auto issue = [&](int k, bool is_v) {
+    if (k - id0 >= 32) {                        // uniform, once per 32 chunks
+      id0 = k;
+      ids = load_ids(k);
+    }
+    const int c = chunk0 + wave + NW * k;
+    char* const dst = lds + (k % R) * S::SLOT + (is_v ? S::HALF : 0);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int tile = min(2 * c + t, last_tile);
+      const int rmax = limit - 1 - 16 * tile;   // rows past it repeat the last position
+      const int64_t b = __builtin_amdgcn_readlane(ids, 2 * (k - id0) + t);
+      const char* const base = pool_kvh + b * blk_bytes + (int64_t)(tile & sub_mask) * S::TB + (is_v ? v_off : 0);
+#pragma unroll
+      for (int i = 0; i < LD / 2; ++i) {
+        const int r = S::RPL * i + lrow;
+        s_dma16_l2((uint32_t)(min(r, rmax) * RB + 16 * (lpiece ^ (is_v ? S::vswz(r) : S::kswz(16 * t + r)))), base,
+                   dst + (t * (LD / 2) + i) * 1024);
+      }
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < R; ++k)
+    if (k < n) {
+      issue(k, false);
+      issue(k, true);
+    }
+
+  // ---- q rotated (RoPE at the node's position), its sign, complete here ----
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    if (a.rope.cos) {
+      constexpr int E = 16 / S::EB;             // elements of a piece
+      const int64_t r = a.rope.row(a.positions[row0 + my_row[cb]], D / 2) + E * half;
+#pragma unroll
+      for (int s = 0; s < QS / 2; ++s)          // pieces s and s + QS/2 pair (dims i and i + D/2)
+        rope_pair<T>(q[cb][s], q[cb][s + QS / 2], a.rope.cos + r + 2 * E * s, a.rope.sin + r + 2 * E * s);
+    }
+    if (a.q_sign != 1.f) {
+#pragma unroll
+      for (int s = 0; s < QS; ++s) {
+        constexpr int E = 16 / S::EB;
+        T x[E];
+        __builtin_memcpy(x, &q[cb][s], 16);
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[e] = (T)((float)x[e] * a.q_sign);
+        __builtin_memcpy(&q[cb][s], x, 16);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < QS; ++s)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(q[cb][s].w[i]));
+  }
+
+  uint32_t ones = 0;                            // in a register: as a literal the bf16 dot product read it wrong
+  if constexpr (!F32) ones = cmath<Tag>::ONES;
+  asm volatile("" : "+v"(ones));
+  float m[CB], l[CB];                           // reference max (scaled, base 2), this lane's share of the sum
+  float16_t acc[CB][NB];                        // O^T[32 b + 8 (r / 4) + 4 half + r % 4][col]
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    m[cb] = -INFINITY, l[cb] = 0.f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[cb][b][r] = 0.f;
+  }
+  // operand addresses of this lane in a slot
+  uint32_t ka[QS], va[NB];
+#pragma unroll
+  for (int s = 0; s < QS; ++s) ka[s] = (uint32_t)(lcol * RB + 16 * ((2 * s + half) ^ S::kswz(lcol)));
+  {
+    const int li = lane & 15, rv = 4 * half + (li >> 2);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int c = 4 * b + 2 * ((lane >> 4) & 1) + ((li & 3) >> 1);
+      va[b] = F32 ? (uint32_t)(S::HALF + 4 * half * RB + 128 * b + 4 * lcol)
+                  : (uint32_t)(S::HALF + rv * RB + 16 * (c ^ S::vswz(rv)) + 8 * (li & 1));
+    }
+  }
+  const float sl2e = a.scale_log2e;
+
+  float16_t sc[CB];                             // S^T, then P: positions 8 (r / 4) + 4 half + r % 4 of a chunk
+  su32x4_t pb[CB][2];                           // 16-bit P: B operands of 16 positions each
+  uint32_t vis[CB];                             // a masked chunk's seen positions
+  auto scores = [&](const char* base) {
+    if constexpr (!F32) {
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sc[cb][r] = 0.f;
+      constexpr int KG = 4;                     // operands read KG ahead of their products
+      su32x4_t kf[2][KG];
+      auto read = [&](int g) {
+#pragma unroll
+        for (int i = 0; i < KG; ++i) kf[g & 1][i] = *reinterpret_cast<const su32x4_t*>(base + ka[KG * g + i]);
+      };
+      read(0);
+#pragma unroll
+      for (int g = 0; g < QS / KG; ++g) {
+        if (g + 1 < QS / KG) read(g + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < KG; ++i)
+#pragma unroll
+          for (int cb = 0; cb < CB; ++cb)
+            sc[cb] = cmath<Tag>::mfma(kf[g & 1][i], __builtin_bit_cast(su32x4_t, q[cb][KG * g + i]), sc[cb]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+      float16_t d[CB][2];
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) d[cb][0][r] = d[cb][1][r] = 0.f;
+#pragma unroll
+      for (int s = 0; s < QS; ++s) {
+        const vec16 kv = ld16(base + ka[s]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int cb = 0; cb < CB; ++cb)
+            d[cb][i & 1] = __builtin_amdgcn_mfma_f32_32x32x2f32(bits_to_f32(kv.w[i]), bits_to_f32(q[cb][s].w[i]),
+                                                                d[cb][i & 1], 0, 0, 0);
+      }
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) sc[cb] = d[cb][0] + d[cb][1];
+    }
+  };
+  // the online softmax of chunk c: sc -> P, and the state's rescale
+  auto softmax = [&](int c, bool masked) {
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+      if (masked) {                             // kept a branch: most chunks lie in the cache
+        asm volatile("");
+        // the mask's bits from node 32 c - cached on; those before node 0 are cached positions
+        const uint32_t* const mrow = a.mask + (int64_t)(row0 + my_row[cb]) * a.mask_words;
+        const int off = CK * c - cached, w = off >> 5;
+        const uint32_t lo = w < 0 ? ~0u : w < a.mask_words ? mrow[w] : 0u;
+        const uint32_t hi = w + 1 < a.mask_words ? mrow[w + 1] : 0u;
+        vis[cb] = __builtin_amdgcn_alignbit(hi, lo, off & 31);
+        if (limit - CK * c < 32) vis[cb] &= (1u << (limit - CK * c)) - 1;
+        const uint32_t mine = vis[cb] >> (4 * half);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!(mine & (1u << (8 * (r >> 2) + (r & 3))))) sc[cb][r] = -INFINITY;
+      }
+      float cm = max_f32(sc[cb][0], sc[cb][1]);
+#pragma unroll
+      for (int e = 2; e < 16; e += 2) cm = max3_f32(cm, sc[cb][e], sc[cb][e + 1]);
+      cm *= sl2e;
+      if (__any(cm > m[cb] + 8.f)) {
+        const float m_new = fmaxf(m[cb], max_xor32(cm));
+        const float alpha = fast_exp2(m[cb] - (m_new == -INFINITY ? 0.f : m_new));   // 0 while m = -inf
+        m[cb] = m_new;
+        l[cb] *= alpha;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[cb][b] *= alpha;
+      }
+      const float neg_m = m[cb] == -INFINITY ? 0.f : -m[cb];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[cb][r] = fast_exp2(fmaf(sc[cb][r], sl2e, neg_m));
+      if constexpr (!F32) {
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          float p[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) p[j] = sc[cb][8 * w + j];
+          pb[cb][w] = smath<Tag>::pack8(p);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) l[cb] = cmath<Tag>::add2(pb[cb][w][j], ones, l[cb]);   // of the rounded P
+        }
+      } else {
+        const float16_t& p = sc[cb];
+        l[cb] += (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]))) +
+                 (((p[8] + p[9]) + (p[10] + p[11])) + ((p[12] + p[13]) + (p[14] + p[15])));
+      }
+    }
+  };
+  // O^T += V^T.P of the chunk in a slot
+  auto values = [&](const char* base) {
+    if constexpr (!F32) {
+      uint2 vf[2][NB][2];
+      auto read = [&](int w) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const char* const vp = base + va[b] + 16 * w * RB;
+          vf[w][b][0] = lds_read_tr16(vp);
+          vf[w][b][1] = lds_read_tr16(vp + 8 * RB);
+        }
+      };
+      read(0);
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        if (w == 0) read(1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const uint2 lo = vf[w][b][0], hi = vf[w][b][1];
+#pragma unroll
+          for (int cb = 0; cb < CB; ++cb)
+            acc[cb][b] = cmath<Tag>::mfma(su32x4_t{lo.x, lo.y, hi.x, hi.y}, pb[cb][w], acc[cb][b]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const float v = *reinterpret_cast<const float*>(base + va[b] + (8 * (r >> 2) + (r & 3)) * RB);
+#pragma unroll
+          for (int cb = 0; cb < CB; ++cb)
+            acc[cb][b] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, sc[cb][r], acc[cb][b], 0, 0, 0);
+        }
+    }
+  };
+  // a masked chunk whose V rows hold an infinity or NaN: position by position, the unseen ones left
+  // out (a weight of 0 times an infinity is no 0)
+  auto values_finite = [&](const char* base) {
+    bool ok = true;
+    for (int i = 0; i < S::HALF / 1024; ++i) {
+      const vec16 v = ld16(base + S::HALF + 1024 * i + 16 * lane);
+      constexpr uint32_t E1 = F32 ? 0x7F800000u : sizeof(T) == 2 && __is_same(T, _Float16) ? 0x7C00u : 0x7F80u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        ok &= (v.w[j] & E1) != E1;
+        if (!F32) ok &= ((v.w[j] >> 16) & E1) != E1;
+      }
+    }
+    return __all(ok);
+  };
+  auto values_apart = [&](const char* base) {
+#pragma unroll 1
+    for (int pos = 0; pos < CK; ++pos) {
+      const int reg = 4 * (pos >> 3) + (pos & 3);
+      const bool here = half == ((pos >> 2) & 1);
+#pragma unroll
+      for (int cb = 0; cb < CB; ++cb) {
+        float p = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float x;
+          if constexpr (F32) x = sc[cb][r];
+          else {
+            T e[2];
+            const uint32_t word = pb[cb][r >> 3][(r & 7) >> 1];
+            __builtin_memcpy(e, &word, 4);
+            x = (float)e[r & 1];
+          }
+          p = r == reg ? x : p;
+        }
+        const float other = __shfl_xor(p, 32);
+        p = here ? p : other;
+        if ((vis[cb] >> pos) & 1) {
+#pragma unroll
+          for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {       // dims 32 b + 8 g + 4 half ..
+              const char* const vp = base + S::HALF + pos * RB +
+                                     (F32 ? 128 * b + 32 * g + 16 * half : 16 * ((4 * b + g) ^ S::vswz(pos)) + 8 * half);
+              T e[4];
+              __builtin_memcpy(e, __builtin_assume_aligned(vp, 8), 4 * sizeof(T));
+#pragma unroll
+              for (int j = 0; j < 4; ++j) acc[cb][b][4 * g + j] = fmaf(p, (float)e[j], acc[cb][b][4 * g + j]);
+            }
+        }
+      }
+    }
+  };
+
+  // Loads of chunk k + R's K follow chunk k's scores, its V's chunk k's products. Outstanding when
+  // chunk k's K (or V) must be there: the halves issued behind it.
+  for (int k = 0; k < n; ++k) {
+    const int c = chunk0 + wave + NW * k;
+    const char* const base = lds + (k % R) * S::SLOT;
+    const int ahead = min(R - 1, n - 1 - k);    // chunks issued behind chunk k
+    if (ahead == R - 1) s_vm_wait_le(LD * (1 + 2 * (R - 1)));
+    else s_vm_wait_le(LD * (1 + 2 * ahead));
+    scores(base);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the K rows are in registers: their slot is free
+    const bool more = k + R < n;
+    if (more) issue(k + R, false);
+    const bool masked = CK * c + CK > cached;
+    softmax(c, masked);
+    if (more) s_vm_wait_le(LD * (1 + 2 * (R - 1)));
+    else s_vm_wait_le(LD * 2 * ahead);
+    if (masked && !values_finite(base)) values_apart(base);
+    else values(base);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (more) issue(k + R, true);
+  }
+
+  // ---- the waves' states joined; wave w stores the 4-dim groups w, w + NW, ... of a column ----
+  const int slot = w2.x, slot_rows = w2.y;      // slot < 0: the whole context, the output itself
+#pragma unroll
+  for (int cb = 0; cb < CB; ++cb) {
+    l[cb] = sum_xor32(l[cb]);
+    __syncthreads();
+    float* const mine = reinterpret_cast<float*>(lds_all) + wave * (64 * (16 * NB + 2)) + lane;
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mine[64 * (16 * b + r)] = acc[cb][b][r];
+    mine[64 * 16 * NB] = m[cb];
+    mine[64 * (16 * NB + 1)] = l[cb];
+    __syncthreads();
+    const float* const all = reinterpret_cast<const float*>(lds_all) + lane;
+    constexpr int WS = 64 * (16 * NB + 2);
+    float mw[NW], M = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      mw[w] = all[w * WS + 64 * 16 * NB];
+      M = fmaxf(M, mw[w]);
+    }
+    const float M_safe = M == -INFINITY ? 0.f : M;
+#pragma unroll
+    for (int w = 0; w < NW; ++w) {
+      mw[w] = fast_exp2(mw[w] - M_safe);         // 0 for a wave that saw nothing
+      L += all[w * WS + 64 * (16 * NB + 1)] * mw[w];
+    }
+    if (col0 + 32 * cb + lcol >= ncols) continue;
+    const int row = row0 + my_row[cb];
+    float inv = 1.f;
+    if (slot < 0) {
+      inv = 1.f / L;
+      if (!(L > 0.f) && !tree_sees(a.mask + (int64_t)row * a.mask_words, cached, nodes)) inv = 0.f;
+    }
+    for (int g = wave; g < 4 * NB; g += NW) {   // dims 8 g + 4 half ..
+      float4_t o = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < NW; ++w) {
+        const float* const src = all + w * WS + 64 * 4 * g;
+        o += float4_t{src[0], src[64], src[128], src[192]} * mw[w];
+      }
+      if (slot < 0) {
+        typedef T t4_t __attribute__((ext_vector_type(4)));
+        t4_t t;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[j] = (T)(o[j] * inv);
+        st_through(a.out + (int64_t)row * a.out_row_bytes + (int64_t)hd[cb] * RB + (8 * g + 4 * half) * S::EB, t);
+      } else {
+        const int64_t at = (int64_t)(slot + my_row[cb]) * a.num_heads + hd[cb];
+        *reinterpret_cast<float4_t*>(a.ws_acc + at * D + 8 * g + 4 * half) = o;
+        if (g == 0 && half == 0) *reinterpret_cast<float2*>(a.ws_ml + at * 2) = make_float2(M, L);
+      }
+    }
+  }
+  (void)slot_rows;
+}
+
+// The partials of a row's parts joined: thread = 4 dims of a head.
+template <typename Tag, int D>
+__global__ __launch_bounds__(64) void tree_join_kernel(const tree_args a) {
+  using T = typename elem<Tag>::type;
+  constexpr int QPH = D / 4, BATCH = 8;
+  const int col = threadIdx.x + 64 * blockIdx.y;
+  if (col >= a.num_heads * QPH) return;
+  const int4 rec = a.split[blockIdx.x];
+  const int row = rec.x, first = rec.y, parts = rec.z, step = rec.w;
+  const int head = col / QPH, d4 = col - head * QPH;
+  float M = -INFINITY, L = 0.f;
+  float4_t o = float4_t{0.f, 0.f, 0.f, 0.f};
+  for (int p0 = 0; p0 < parts; p0 += BATCH) {
+    float2 ml[BATCH];
+    float4_t av[BATCH];
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      ml[k] = make_float2(-INFINITY, 0.f);
+      av[k] = float4_t{0.f, 0.f, 0.f, 0.f};
+      if (p0 + k < parts) {
+        const int64_t at = (int64_t)(first + (p0 + k) * step) * a.num_heads + head;
+        ml[k] = *reinterpret_cast<const float2*>(a.ws_ml + at * 2);
+        av[k] = *reinterpret_cast<const float4_t*>(a.ws_acc + at * D + 4 * d4);
+      }
+    }
+    float mb = M;
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) mb = fmaxf(mb, ml[k].x);
+    const float safe = mb == -INFINITY ? 0.f : mb, keep = fast_exp2(M - safe);
+    L *= keep;
+    o *= keep;
+#pragma unroll
+    for (int k = 0; k < BATCH; ++k) {
+      const float w = fast_exp2(ml[k].x - safe);   // 0 for a part that saw nothing
+      L = fmaf(ml[k].y, w, L);
+      o += av[k] * w;
+    }
+    M = mb;
+  }
+  float inv = 1.f / L;
+  if (!(L > 0.f)) {
+    const int seq = a.row_seq[row], r0 = a.row_starts[seq];
+    if (!tree_sees(a.mask + (int64_t)row * a.mask_words, a.cached[seq], a.row_starts[seq + 1] - r0)) inv = 0.f;
+  }
+  typedef T t4_t __attribute__((ext_vector_type(4)));
+  t4_t t;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) t[j] = (T)(o[j] * inv);
+  st_through(a.out + (int64_t)row * a.out_row_bytes + ((int64_t)head * D + 4 * d4) * sizeof(T), t);
+}
+
+// Waves and ring slots of a kernel: 128 KiB of LDS, a workgroup on a CU.
+template <typename Tag, int D>
+struct tlaunch {
+  static constexpr int SLOT = tshape<Tag, D>::SLOT;
+  static constexpr int NW = SLOT == 8192 ? 8 : 4;
+  static constexpr int R = SLOT == 32768 ? 1 : 2;
+  static constexpr int OCC = NW / 4;
+};
+
+template <typename Tag, int D>
+static void launch_columns(const tree_args& a, int num_work, int blocks, int num_split, hipStream_t stream) {
+  using L = tlaunch<Tag, D>;
+  if (blocks == 1)
+    hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 1, L::NW, L::R, L::OCC>), dim3(num_work), dim3(64 * L::NW), 0, stream, a);
+  else
+    hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 2, L::NW, L::R, L::OCC>), dim3(num_work), dim3(64 * L::NW), 0, stream, a);
+  if (num_split > 0)
+    hipLaunchKernelGGL((tree_join_kernel<Tag, D>), dim3(num_split, (a.num_heads * (D / 4) + 63) / 64), dim3(64), 0,
+                       stream, a);
+}
+
 template <typename Tag>
 static void launch_rows(const tree_args& a, int num_rows, int head_dim, hipStream_t stream) {
   const dim3 grid(num_rows, a.num_heads);
@@ -135,12 +671,147 @@ static void launch_rows(const tree_args& a, int num_rows, int head_dim, hipStrea
 
 }  // namespace tb
 
+
+// ---- the work list (host, no device call) ------------------------------------------
+namespace {
+
+struct tree_price {
+  int chunks_round;            // chunks a workgroup's waves take at once
+  double start, alone, full;   // us: a workgroup's start and end; a round alone on its CU; on a full chip
+  int cus;
+};
+
+// Chunks of a sequence's context.
+inline int tree_chunks(int cached, int nodes) { return nodes > 0 ? (cached + nodes + 31) / 32 : 0; }
+
+// The part length in rounds of least cost; 0: no context is cut.
+int tree_part_rounds(const tree_price& price, const int32_t* cached, const int32_t* nodes, int num_seqs, int rep,
+                     int cols, int num_kv_heads, double slot_bytes) {
+  int longest = 0;
+  for (int b = 0; b < num_seqs; ++b) longest = std::max(longest, tree_chunks(cached[b], nodes[b]));
+  const int most = (longest + price.chunks_round - 1) / price.chunks_round;
+  auto cost = [&](int part) {
+    double rounds = 0, wgs = 0, slots = 0;
+    for (int b = 0; b < num_seqs; ++b) {
+      if (nodes[b] <= 0) continue;
+      const int r = (tree_chunks(cached[b], nodes[b]) + price.chunks_round - 1) / price.chunks_round;
+      const int groups = (nodes[b] * rep + cols - 1) / cols, parts = (r + part - 1) / part;
+      rounds += (double)r * groups;
+      wgs += (double)parts * groups;
+      if (parts > 1) slots += (double)parts * nodes[b];
+    }
+    const double one = price.start + std::min(part, most) * price.alone;
+    const double all = (wgs * price.start + rounds * price.full) * num_kv_heads / price.cus +
+                       0.5 * std::min(part, most) * price.full;
+    return std::max(one, all) + (slots > 0 ? 4.0 + 2 * slots * slot_bytes / 4e6 : 0.);
+  };
+  int best = 0;
+  double least = cost(std::max(most, 1));
+  for (int part = 1; part < most; part += part < 8 ? 1 : part < 32 ? 4 : 16) {
+    const double c = cost(part);
+    if (c < 0.97 * least) least = c, best = part;
+  }
+  return best;
+}
+
+struct tree_piece {
+  int seq, kvh, chunk0, chunks, slot, groups;
+};
+
+}  // namespace
+
+extern "C" int32_t tb_build_tree_work(const int32_t* cached, const int32_t* nodes, int32_t num_seqs,
+                                      int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
+                                      int32_t num_cus, int32_t num_xcds, int32_t* work, int32_t work_capacity,
+                                      int32_t* split, int32_t split_capacity, int32_t* counts) try {
+  TB_CHECK_ARG(num_seqs >= 0 && num_heads > 0 && num_kv_heads > 0 && num_heads % num_kv_heads == 0);
+  TB_CHECK_ARG(dtype >= TB_DTYPE_F32 && dtype <= TB_DTYPE_BF16 && num_cus > 0 && num_xcds > 0 && counts);
+  if (head_dim != 64 && head_dim != 128) return TB_ERR_UNSUPPORTED;
+  TB_CHECK_ARG(num_seqs == 0 || (cached && nodes));
+  const int rep = num_heads / num_kv_heads;
+  int64_t rows = 0;
+  int most_cols = 0;
+  for (int b = 0; b < num_seqs; ++b) {
+    TB_CHECK_ARG(cached[b] >= 0 && nodes[b] >= 0 && (int64_t)cached[b] + nodes[b] <= (1 << 30));
+    TB_CHECK_ARG((int64_t)nodes[b] * rep < (1 << 28));
+    most_cols = std::max(most_cols, nodes[b] * rep);
+    rows += nodes[b];
+  }
+  TB_CHECK_ARG(rows < (1 << 30));
+  const int blocks = most_cols > 32 ? 2 : 1, cols = 32 * blocks;
+  const int slot_kb = head_dim * (dtype == TB_DTYPE_F32 ? 4 : 2) * 64 / 1024;   // a chunk's K and V rows
+  tree_price price{slot_kb == 8 ? 8 : 4, 4.0, 1.2, 3.3, num_cus};
+  const int part = tree_part_rounds(price, cached, nodes, num_seqs, rep, cols, num_kv_heads,
+                                    (double)num_heads * (head_dim + 2) * 4) * price.chunks_round;
+  std::vector<tree_piece> pieces;
+  int64_t slots = 0, num_split = 0, row0 = 0;
+  std::vector<int32_t> first(num_seqs + 1);
+  for (int b = 0; b < num_seqs; ++b) {
+    first[b] = (int32_t)row0;
+    row0 += nodes[b];
+    const int all = tree_chunks(cached[b], nodes[b]);
+    if (all == 0) continue;
+    const int parts = part ? (all + part - 1) / part : 1;
+    for (int i = 0; i < parts; ++i)
+      for (int h = 0; h < num_kv_heads; ++h)
+        pieces.push_back({b, h, part * i, part ? std::min(part, all - part * i) : all,
+                          parts > 1 ? (int)(slots + (int64_t)i * nodes[b]) : -1, (nodes[b] * rep + cols - 1) / cols});
+    if (parts > 1) {
+      for (int i = 0; i < nodes[b]; ++i, ++num_split)
+        if (split && num_split < split_capacity) {
+          int32_t* const s = split + 4 * num_split;
+          s[0] = first[b] + i, s[1] = (int32_t)(slots + i), s[2] = parts, s[3] = nodes[b];
+        }
+      slots += (int64_t)parts * nodes[b];
+    }
+    TB_CHECK_ARG(slots < (1 << 30));
+  }
+  // longest first; the column groups of one piece, which read the same rows, on one XCD
+  std::stable_sort(pieces.begin(), pieces.end(),
+                   [](const tree_piece& x, const tree_piece& y) { return x.chunks > y.chunks; });
+  std::vector<std::vector<std::pair<int, int>>> lists(num_xcds);
+  std::vector<int64_t> load(num_xcds, 0);
+  for (int i = 0; i < (int)pieces.size(); ++i) {
+    const int x = (int)(std::min_element(load.begin(), load.end()) - load.begin());
+    for (int g = 0; g < pieces[i].groups; ++g) lists[x].push_back({i, g});
+    load[x] += (int64_t)pieces[i].groups * (pieces[i].chunks + 8);
+  }
+  size_t depth = 0;
+  for (auto& l : lists) depth = std::max(depth, l.size());
+  TB_CHECK_ARG(depth * num_xcds < ((size_t)1 << 30));
+  const int64_t n = (int64_t)depth * num_xcds;
+  counts[0] = (int32_t)n, counts[1] = (int32_t)num_split, counts[2] = (int32_t)slots, counts[3] = blocks;
+  if (!work && !split) return TB_OK;
+  TB_CHECK_ARG((n == 0 || work) && work_capacity >= n && (num_split == 0 || split) && split_capacity >= num_split);
+  for (size_t j = 0; j < depth; ++j)
+    for (int x = 0; x < num_xcds; ++x) {
+      int32_t* const w = work + 12 * (j * num_xcds + x);
+      std::fill(w, w + 12, 0);
+      if (j >= lists[x].size()) continue;
+      const tree_piece& p = pieces[lists[x][j].first];
+      w[0] = first[p.seq], w[1] = p.seq, w[2] = cached[p.seq], w[3] = nodes[p.seq];
+      w[4] = lists[x][j].second * cols, w[5] = p.kvh, w[6] = p.chunk0, w[7] = p.chunks;
+      w[8] = p.slot;
+    }
+  return TB_OK;
+} catch (const std::exception&) {
+  return TB_ERR_INVALID_ARG;
+}
+
+extern "C" size_t tb_tree_attention_workspace_bytes(int32_t partial_slots, int32_t num_heads, int32_t head_dim) {
+  if (partial_slots <= 0 || num_heads <= 0 || head_dim <= 0) return 0;
+  return (size_t)partial_slots * num_heads * (head_dim + 2) * sizeof(float);
+}
+
 extern "C" int32_t tb_tree_attention(const void* q, int64_t q_row_stride, const void* pool, int64_t num_blocks,
                                      void* out, int64_t out_row_stride, const int32_t* block_tables,
                                      int32_t max_blocks_per_seq, const int32_t* row_starts, const int32_t* cached,
                                      int32_t num_seqs, const int32_t* row_seq, int32_t num_rows,
-                                     const uint32_t* mask, int32_t mask_words, int32_t num_heads,
-                                     int32_t num_kv_heads, int32_t head_dim, int32_t block_size, float scale,
+                                     const uint32_t* mask, int32_t mask_words, const int32_t* work,
+                                     int32_t num_work, int32_t column_blocks, const int32_t* split_rows,
+                                     int32_t num_split_rows, int32_t partial_slots, void* workspace,
+                                     size_t workspace_bytes, int32_t num_heads, int32_t num_kv_heads,
+                                     int32_t head_dim, int32_t block_size, float scale,
                                      int32_t dtype, const int64_t* positions, const float* rope_cos,
                                      const float* rope_sin, int32_t rope_max_position, hipStream_t stream) {
   using namespace tb;
@@ -178,8 +849,36 @@ extern "C" int32_t tb_tree_attention(const void* q, int64_t q_row_stride, const 
   a.scale = scale;
   a.positions = positions;
   a.rope = rope_tables{rope_cos, rope_sin, rope_max_position};
-  if (dtype == TB_DTYPE_F32) launch_rows<f32_t>(a, num_rows, head_dim, stream);
-  else if (dtype == TB_DTYPE_F16) launch_rows<f16_t>(a, num_rows, head_dim, stream);
-  else launch_rows<bf16_t>(a, num_rows, head_dim, stream);
+  if (block_size < 16) {       // a 16-position tile would lie in several blocks
+    if (dtype == TB_DTYPE_F32) launch_rows<f32_t>(a, num_rows, head_dim, stream);
+    else if (dtype == TB_DTYPE_F16) launch_rows<f16_t>(a, num_rows, head_dim, stream);
+    else launch_rows<bf16_t>(a, num_rows, head_dim, stream);
+    TB_RETURN_LAUNCH_STATUS();
+  }
+  TB_CHECK_ARG(num_work >= 0 && num_split_rows >= 0 && num_split_rows <= num_rows && partial_slots >= 0);
+  TB_CHECK_ARG((column_blocks == 1 || column_blocks == 2) && (num_split_rows == 0 || partial_slots > 0));
+  if (num_work == 0) return TB_OK;
+  TB_CHECK_ARG(work && ((uintptr_t)work & 15u) == 0 && (num_split_rows == 0 || split_rows) &&
+               ((uintptr_t)split_rows & 15u) == 0);
+  if (partial_slots > 0)
+    TB_CHECK_ARG(workspace && ((uintptr_t)workspace & 15u) == 0 &&
+                 workspace_bytes >= tb_tree_attention_workspace_bytes(partial_slots, num_heads, head_dim));
+  a.work = (const int4*)work;
+  a.split = (const int4*)split_rows;
+  a.ws_acc = (float*)workspace;
+  a.ws_ml = (float*)workspace + (size_t)partial_slots * num_heads * head_dim;
+  const float s2 = fabsf(scale) * 1.4426950408889634f;
+  a.scale_log2e = s2 > 0.f ? s2 : 1.f;
+  a.q_sign = scale > 0.f ? 1.f : scale < 0.f ? -1.f : scale;   // 0, or a NaN
+  const bool d64 = head_dim == 64;
+  if (dtype == TB_DTYPE_F32)
+    d64 ? launch_columns<f32_t, 64>(a, num_work, column_blocks, num_split_rows, stream)
+        : launch_columns<f32_t, 128>(a, num_work, column_blocks, num_split_rows, stream);
+  else if (dtype == TB_DTYPE_F16)
+    d64 ? launch_columns<f16_t, 64>(a, num_work, column_blocks, num_split_rows, stream)
+        : launch_columns<f16_t, 128>(a, num_work, column_blocks, num_split_rows, stream);
+  else
+    d64 ? launch_columns<bf16_t, 64>(a, num_work, column_blocks, num_split_rows, stream)
+        : launch_columns<bf16_t, 128>(a, num_work, column_blocks, num_split_rows, stream);
   TB_RETURN_LAUNCH_STATUS();
 }

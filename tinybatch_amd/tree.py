@@ -31,6 +31,7 @@ from .metadata import pad4
 from .ops import Rope, _check_pool, _rows_view, kv_append
 
 MAX_NODES = 1024             # TB_TREE_MAX_NODES
+NUM_CUS, NUM_XCDS = 256, 8   # MI355X, for which the work lists are made
 
 
 @dataclass
@@ -58,6 +59,11 @@ class TreeMetadata:
     cached_np: np.ndarray | None
     block_tables_np: np.ndarray | None
     slot_mapping_np: np.ndarray | None
+    # tb_tree_attention's work list
+    work_np: np.ndarray | None = None         # [n, 12]
+    split_np: np.ndarray | None = None        # [rows of contexts cut into parts, 4]
+    partial_slots: int = 0
+    column_blocks: int = 1
     # device views (one backing buffer)
     device: torch.device | None = None
     parents: torch.Tensor | None = None
@@ -68,6 +74,8 @@ class TreeMetadata:
     cached: torch.Tensor | None = None
     block_tables: torch.Tensor | None = None
     slot_mapping: torch.Tensor | None = None
+    work: torch.Tensor | None = None
+    split: torch.Tensor | None = None
 
     def to(self, device: torch.device) -> "TreeMetadata":
         """Upload every array with one host-to-device copy (views into one buffer)."""
@@ -82,7 +90,8 @@ class TreeMetadata:
                  ("row_seq", self.row_seq_np)]
         if has_cache:
             parts += [("cached", self.cached_np), ("block_tables", self.block_tables_np.reshape(-1)),
-                      ("slot_mapping", self.slot_mapping_np)]
+                      ("slot_mapping", self.slot_mapping_np), ("work", self.work_np.reshape(-1)),
+                      ("split", self.split_np.reshape(-1))]
         host = np.zeros(sum(pad4(x.size) for _, x in parts), dtype=np.int32)
         at, spans = 0, {}
         for name, x in parts:
@@ -123,6 +132,21 @@ def _masks(parents, visible, words: int) -> np.ndarray:
         for m in seen:
             raw += m.to_bytes(size, "little")
     return np.frombuffer(bytes(raw), dtype=np.uint32).reshape(-1, words)
+
+
+def _attach_work(meta: TreeMetadata) -> None:
+    """The work list of the step's attention calls (tb_build_tree_work)."""
+    L = _lib.lib()
+    nodes = np.diff(meta.row_starts_np).astype(np.int32)
+    counts = np.zeros(4, dtype=np.int32)
+    head = (meta.cached_np.ctypes.data, nodes.ctypes.data, meta.num_seqs, meta.num_heads, meta.num_kv_heads,
+            meta.head_dim, _lib.DTYPE_CODE[meta.dtype], NUM_CUS, NUM_XCDS)
+    _lib.check(L.tb_build_tree_work(*head, None, 0, None, 0, counts.ctypes.data), "tb_build_tree_work")
+    work, split = np.zeros((int(counts[0]), 12), dtype=np.int32), np.zeros((int(counts[1]), 4), dtype=np.int32)
+    _lib.check(L.tb_build_tree_work(*head, work.ctypes.data, work.shape[0], split.ctypes.data, split.shape[0],
+                                    counts.ctypes.data), "tb_build_tree_work")
+    meta.work_np, meta.split_np = work, split
+    meta.partial_slots, meta.column_blocks = int(counts[2]), int(counts[3])
 
 
 def build_tree_metadata(parents, cached_lens=None, block_tables=None, *, block_size: int = 0, num_blocks: int = 0,
@@ -177,6 +201,8 @@ def build_tree_metadata(parents, cached_lens=None, block_tables=None, *, block_s
         raise ValueError("block_size must be a power of two and num_blocks positive")
     if num_heads is None or num_kv_heads is None or head_dim is None or dtype not in _lib.DTYPE_CODE:
         raise ValueError("num_heads, num_kv_heads, head_dim and dtype (fp32, fp16, bf16) describe the attention's calls")
+    if head_dim not in (64, 128):
+        raise ValueError(f"head_dim {head_dim} is not served (64 and 128 are)")
     if num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads:
         raise ValueError(f"num_heads {num_heads} is not a multiple of kv heads {num_kv_heads}")
     cached = np.array([int(c) for c in cached_lens], dtype=np.int64)
@@ -205,6 +231,7 @@ def build_tree_metadata(parents, cached_lens=None, block_tables=None, *, block_s
     meta.block_tables_np = tables
     meta.max_blocks_per_seq = max_nb
     meta.slot_mapping_np = slots.astype(np.int32)
+    _attach_work(meta)
     return meta
 
 
@@ -274,11 +301,16 @@ def tree_attention(q: torch.Tensor, pool: torch.Tensor, meta: TreeMetadata, *, s
         raise TypeError(f"mask must be a contiguous int32 [{T}, {meta.mask_words}] tensor on {q.device}")
     if rope is not None:
         rope.check(d, q.device)
+    ws = None
+    if meta.partial_slots:                   # from the caching allocator: each call, stream and graph its own
+        ws = torch.empty(meta.partial_slots * hq * (d + 2), device=q.device, dtype=torch.float32)
     with _on(q.device):
         st = _lib.lib().tb_tree_attention(
             q.data_ptr(), qs, pool.data_ptr(), nb, out.data_ptr(), os_, meta.block_tables.data_ptr(),
             meta.max_blocks_per_seq, meta.row_starts.data_ptr(), meta.cached.data_ptr(), meta.num_seqs,
-            meta.row_seq.data_ptr(), T, mask.data_ptr(), meta.mask_words, hq, hkv, d, bs,
+            meta.row_seq.data_ptr(), T, mask.data_ptr(), meta.mask_words, meta.work.data_ptr(),
+            meta.work_np.shape[0], meta.column_blocks, meta.split.data_ptr(), meta.split_np.shape[0],
+            meta.partial_slots, None if ws is None else ws.data_ptr(), 0 if ws is None else 4 * ws.numel(), hq, hkv, d, bs,
             1.0 / math.sqrt(d) if scale is None else float(scale), _lib.DTYPE_CODE[q.dtype], meta.positions.data_ptr(),
             None if rope is None else rope.cos.data_ptr(), None if rope is None else rope.sin.data_ptr(),
             0 if rope is None else rope.max_position, _lib.stream_handle(q.device))
