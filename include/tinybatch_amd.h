@@ -734,13 +734,19 @@ size_t tb_tree_attention_workspace_bytes(int32_t partial_slots, int32_t num_head
  *   accepted [num_seqs][width]: the path's nodes from the root on, then -1;
  *   num_accepted [num_seqs]: how many (0 for a sequence without rows);
  *   out_tokens [num_seqs][width] (int64): the path's tokens behind the root, then the token
- *     drawn: num_accepted of them, then -1. width >= every tree's nodes.
+ *     drawn: num_accepted of them, then -1. width >= every tree's nodes;
+ *   max_children: the most children a node has (a hint: it decides how many of the sums that
+ *     refusals need get launches over the whole GPU);
+ *   workspace: tb_tree_verify_workspace_bytes, 8-byte aligned; calls that may overlap in time need
+ *     their own.
  * dtype is that of probs and draft_probs; row strides in elements. */
+size_t tb_tree_verify_workspace_bytes(int32_t num_seqs, int32_t vocab);
 int32_t tb_tree_verify(const void* probs, int64_t probs_row_stride, const void* draft_probs,
                        int64_t draft_row_stride, int32_t vocab, int32_t dtype, const int64_t* tokens,
                        const float* uniforms, const int32_t* parents, const int32_t* row_starts,
-                       int32_t num_seqs, int32_t* accepted, int32_t* num_accepted, int64_t* out_tokens,
-                       int32_t width, hipStream_t stream);
+                       int32_t num_seqs, int32_t max_children, int32_t* accepted, int32_t* num_accepted,
+                       int64_t* out_tokens, int32_t width, void* workspace, size_t workspace_bytes,
+                       hipStream_t stream);
 
 /* The same for greedy decoding: target_ids [num_rows] (int64) is the target's choice after each
  * node (tb_linear_argmax); the first child that holds it is kept. Trees of any size. */

@@ -105,14 +105,19 @@ def test_entries_reject_bad_arguments_without_launching():
     L, f = _lib.lib(), ctypes.c_void_p(4096)
     bad, unsupported = _lib.TB_ERR_INVALID_ARG, _lib.TB_ERR_UNSUPPORTED
 
-    def verify(probs=f, stride=100, draft=None, dstride=0, vocab=100, dt=0, tokens=f, seqs=2, width=4, acc=f):
-        return L.tb_tree_verify(probs, stride, draft, dstride, vocab, dt, tokens, f, f, f, seqs, acc, f, f, width, None)
+    def verify(probs=f, stride=100, draft=None, dstride=0, vocab=100, dt=0, tokens=f, seqs=2, width=4, acc=f,
+               children=1, ws=f, wsb=1 << 20):
+        return L.tb_tree_verify(probs, stride, draft, dstride, vocab, dt, tokens, f, f, f, seqs, children, acc, f, f,
+                                width, ws, wsb, None)
 
     assert verify(stride=99) == bad                    # rows overlap
     assert verify(draft=f, dstride=99) == bad
     assert verify(vocab=0) == bad and verify(dt=3) == bad and verify(width=0) == bad
     assert verify(probs=None) == bad and verify(tokens=None) == bad and verify(acc=None) == bad
+    assert verify(children=-1) == bad and verify(ws=None) == bad and verify(ws=ctypes.c_void_p(4100)) == bad
+    assert verify(wsb=L.tb_tree_verify_workspace_bytes(2, 100) - 1) == bad
     assert verify(width=MAX_NODES + 1) == unsupported
+    assert verify(vocab=1 << 25, stride=1 << 25, wsb=1 << 30) == unsupported
     assert verify(seqs=0, probs=None) == _lib.TB_OK
     assert L.tb_tree_verify_greedy(f, f, f, f, 2, f, f, f, 0, None) == bad
     assert L.tb_tree_verify_greedy(None, f, f, f, 2, f, f, f, 4, None) == bad
@@ -126,3 +131,63 @@ def test_entries_reject_bad_arguments_without_launching():
     assert commit(bs=12) == bad and commit(width=0) == bad and commit(hkv=0) == bad
     assert commit(d=4) == unsupported                            # rows of 8 bytes
     assert commit(layers=0) == _lib.TB_OK and commit(seqs=0) == _lib.TB_OK
+
+    def attention(q=f, d=64, bs=16, hq=14, hkv=2, dt=1, qs=896, words=1, work=f, nw=8, blocks=1, split=None, ns=0, slots=0,
+                  ws=None, wsb=0, rows=4, rc=None, rs=None, rmax=0):
+        return L.tb_tree_attention(q, qs, f, 64, f, 896, f, 4, f, f, 2, f, rows, f, words, work, nw, blocks, split, ns,
+                                   slots, ws, wsb, hq, hkv, d, bs, 0.125, dt, f, rc, rs, rmax, None)
+
+    assert attention(d=96) == unsupported
+    assert attention(hq=13) == bad and attention(bs=12) == bad and attention(dt=3) == bad and attention(words=0) == bad
+    assert attention(q=None) == bad and attention(q=ctypes.c_void_p(4104)) == bad
+    assert attention(qs=895) == bad and attention(qs=900) == bad          # rows overlap; rows not 16-byte aligned
+    assert attention(blocks=3) == bad and attention(work=None) == bad and attention(work=ctypes.c_void_p(4104)) == bad
+    assert attention(ns=1, split=f) == bad                                # split rows without partial slots
+    assert attention(ns=1, slots=2) == bad                                # ... without their records
+    assert attention(ns=1, slots=2, split=f) == bad                       # ... without a workspace
+    assert attention(ns=1, slots=2, split=f, ws=f, wsb=2 * 14 * 66 * 4 - 1) == bad
+    assert attention(ns=5, slots=9, split=f, ws=f, wsb=1 << 20) == bad    # more split rows than rows
+    assert attention(rc=f, rmax=64) == bad and attention(rc=f, rs=f, rmax=0) == bad
+    assert attention(rows=0, q=None) == _lib.TB_OK and attention(nw=0) == _lib.TB_OK
+    assert L.tb_tree_attention_workspace_bytes(10, 14, 64) == 10 * 14 * 66 * 4
+
+
+@pytest.mark.parametrize("hq,hkv,d,dtype", [(14, 2, 64, torch.bfloat16), (32, 8, 128, torch.float16), (5, 5, 128, torch.float32),
+                                            (33, 1, 64, torch.float32)])
+@pytest.mark.parametrize("sizes,cached", [([5], [600]), ([60, 0, 3, 33], [0, 50, 7000, 31]), ([1] * 70, list(range(0, 7000, 100))),
+                                          ([1024], [0]), ([0, 0], [4, 0]), ([], [])])
+def test_work_covers_every_context_once(hq, hkv, d, dtype, sizes, cached):
+    """Every (sequence, kv head, column group) has each chunk of its context in one entry, parts of one length;
+    its partial slots are its own; entry g's piece stays on XCD g % 8."""
+    parents = [list(range(-1, n - 1)) for n in sizes]
+    at, tables = 0, []
+    for c, n in zip(cached, sizes):
+        k = -(-(c + n) // 16)
+        tables.append(list(range(at, at + k)))
+        at += k
+    m = build_tree_metadata(parents, cached, tables, block_size=16, num_blocks=max(at, 1), num_heads=hq, num_kv_heads=hkv,
+                            head_dim=d, dtype=dtype)
+    cols, rep = 32 * m.column_blocks, hq // hkv
+    assert m.work_np.shape[0] % 8 == 0
+    seen, slots, where = {}, {}, {}
+    for g, (row0, seq, c, n, col0, kvh, chunk0, chunks, slot, *zero) in enumerate(m.work_np.tolist()):
+        assert zero == [0, 0, 0]
+        if n == 0:
+            continue
+        assert (row0, c, n) == (m.row_starts_np[seq], cached[seq], sizes[seq]) and chunks > 0
+        seen.setdefault((seq, kvh, col0), []).extend(range(chunk0, chunk0 + chunks))
+        slots.setdefault(seq, {})[chunk0] = slot
+        assert where.setdefault((seq, kvh, chunk0), g % 8) == g % 8
+    want = {(b, h, x): list(range(-(-(cached[b] + n) // 32))) for b, n in enumerate(sizes) for h in range(hkv)
+            for x in range(0, n * rep, cols)}
+    assert {k: sorted(v) for k, v in seen.items()} == want
+    used, records = [], []
+    for seq, by in slots.items():
+        n, parts = sizes[seq], [by[k] for k in sorted(by)]
+        if len(parts) == 1:
+            assert parts == [-1]
+            continue
+        assert parts == [parts[0] + i * n for i in range(len(parts))]
+        used += range(parts[0], parts[0] + len(parts) * n)
+        records += [[int(m.row_starts_np[seq]) + i, parts[0] + i, len(parts), n] for i in range(n)]
+    assert sorted(used) == list(range(m.partial_slots)) and sorted(m.split_np.tolist()) == sorted(records)

@@ -17,11 +17,29 @@
 // and those below 0 count as 0.
 // Everything is decided in 64 bits: products and differences of 32-bit inputs are then as
 // good as exact, and a sum of 150000 terms does not move the border between two tokens.
+#include <algorithm>
+
 #include "tb_common.h"
 
 namespace tb {
 
-constexpr int VERIFY_THREADS = 1024;
+// A call is a chain of launches with no atomics between them. Launch 0: every workgroup
+// of a sequence walks its tree until it needs a sum over the vocabulary, and sums its own
+// stretch of the row; launch r + 1: every workgroup adds up launch r's stretches in order, goes on
+// with the walk, and sums its stretch again; the last launch, one workgroup per sequence, finds
+// the border's stretch, thread and token. A chain, and drafts that were not drawn, need one sum
+// whatever is refused; a tree of drawn drafts one more per refusal that has a sibling
+// behind it: up to MAX_ROUNDS of those in launches of their own, the rest in the last one.
+constexpr int SUM_THREADS = 256, FIND_THREADS = 1024;
+constexpr int MAX_ROUNDS = 3;
+constexpr int MAX_STRETCHES = 64;
+constexpr int MAX_STRETCH = 1 << 18;               // tokens whose refused ones are kept as bits in LDS
+
+struct verify_state {
+  double a;                    // the refusals' share of q so far (drafts drawn)
+  int32_t cur, next, len;      // the reached node, the child to try next, the path's length
+  int32_t round;               // the launch whose stretches sum up what is left at `cur`; -1: another test first
+};
 
 struct verify_args {
   const void* probs;           // [T][V]
@@ -36,160 +54,402 @@ struct verify_args {
   int32_t* accepted;           // [B][width]
   int32_t* num_accepted;       // [B]
   int64_t* out_tokens;         // [B][width]
-  int32_t width;
+  int32_t width, num_seqs;
+  int32_t stretches;           // workgroups of a sequence
+  verify_state* states;        // [launch][B]
+  double* sums;                // [launch][B][stretches]
 };
 
+template <int N>
+__device__ __forceinline__ double scan64(double x, int lane) {   // inclusive, over the wave
+#pragma unroll
+  for (int o = 1; o < N; o *= 2) {
+    const double y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
 __device__ __forceinline__ double sum64(double x) {
 #pragma unroll
   for (int o = 1; o < 64; o *= 2) x += __shfl_xor(x, o);
   return x;
 }
 
-// One workgroup per sequence: the tree in LDS, every thread walks it the same way; sums over
-// the vocabulary by all threads, thread t the tokens t, t + 1024, ...
+// A sequence's tree in LDS: what a walk looks at of every node.
+struct verify_tree {
+  int32_t *tok, *par;
+  float *p, *q, *u;            // of the node's token in its parent's rows; its random number
+  static __host__ __device__ size_t bytes(int nodes) { return (size_t)nodes * 20; }
+  __device__ verify_tree(char* lds, int nodes)
+      : tok((int32_t*)lds), par(tok + nodes), p((float*)(par + nodes)), q(p + nodes), u(q + nodes) {}
+};
+
 template <typename T>
-__global__ __launch_bounds__(VERIFY_THREADS) void verify_kernel(const verify_args a) {
-  __shared__ int32_t tok[TB_TREE_MAX_NODES], par[TB_TREE_MAX_NODES], path[TB_TREE_MAX_NODES];
-  __shared__ int32_t refused[TB_TREE_MAX_NODES];
-  __shared__ double part[VERIFY_THREADS / 64];
-  const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int row0 = a.row_starts[seq], n = min(a.row_starts[seq + 1] - row0, TB_TREE_MAX_NODES);
+__device__ __forceinline__ void load_tree(const verify_args& a, const verify_tree& t, int row0, int n) {
+  for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    const int64_t x = a.tokens[row0 + i];
+    const int par = a.parents[row0 + i];
+    const bool known = x >= 0 && x < a.vocab && par >= 0 && par < n;
+    t.tok[i] = known ? (int32_t)x : -1;
+    t.par[i] = par;
+    t.u[i] = a.uniforms[row0 + i];
+    t.p[i] = known ? (float)((const T*)a.probs)[(row0 + par) * a.probs_stride + x] : 0.f;
+    t.q[i] = known && a.draft ? (float)((const T*)a.draft)[(row0 + par) * a.draft_stride + x] : 0.f;
+  }
+}
+
+// The walk from a state on, by one wave, until the path ends or a sum is needed; `s` is the sum
+// at st.a. Nodes kept are written to path[] (LDS) as they come.
+__device__ __forceinline__ void walk(const verify_tree& t, int n, bool drawn, double s, verify_state& st,
+                                     int32_t* path, int lane, int launch) {
+  auto child = [&](int from) -> int {              // the next child of st.cur from row `from` on, or n
+    for (int i0 = from & ~63; i0 < n; i0 += 64) {
+      const int i = i0 + lane;
+      const uint64_t hit = __ballot(i < n && i >= from && t.par[i < n ? i : 0] == st.cur);
+      if (hit) return i0 + __ffsll((unsigned long long)hit) - 1;
+    }
+    return n;
+  };
+  int i = child(st.next), first = i;               // `first`: st.cur's first child, where refused tokens start
+  for (;;) {
+    st.round = launch;
+    st.next = i;
+    if (i >= n) return;                            // every child refused, or none: the path ends at st.cur
+    const double u = (double)t.u[i], p = (double)t.p[i], q = (double)t.q[i];
+    bool keep;
+    if (drawn) {
+      keep = u * q * s < p - st.a * q;
+    } else {
+      // a token refused before holds nothing
+      const int x = t.tok[i];
+      bool again = false;
+      for (int i0 = first & ~63; i0 < i; i0 += 64) {
+        const int k = i0 + lane;
+        again |= __ballot(k < i && k >= first && t.par[k] == st.cur && t.tok[k] == x) != 0;
+      }
+      keep = !again && p > 0. && u * s < p;
+      if (!keep && !again && p > 0.) s -= p;
+    }
+    if (keep) {
+      st.cur = i;
+      st.a = 0.;
+      s = 1.;
+      if (lane == 0) path[st.len] = i;
+      ++st.len;
+      i = first = child(i + 1);
+    } else {
+      i = child(i + 1);
+      if (drawn) {
+        st.a += s;
+        st.next = i;
+        st.round = i < n ? -1 : launch;
+        return;                                    // the sum at the new a: for the next test or for the token
+      }
+    }
+  }
+}
+
+// A row of the vocabulary in 16-byte chunks of the memory it lies in: chunk c holds tokens
+// c E - shift .. + E - 1. The draft's row is read chunk by chunk too where it is aligned alike.
+template <typename T>
+struct verify_row {
+  static constexpr int E = 16 / sizeof(T);
+  const char* p;               // the aligned chunk 0
+  const T* q;                  // the draft's row, token 0; null without
+  int shift, vocab, chunks;
+  bool q_alike;
+  double a;
+  const uint32_t* bits;        // refused tokens from token bit0 on; null: none
+  int bit0;
+
+  __device__ verify_row(const verify_args& v, int row, double a_) : vocab(v.vocab), a(a_), bits(nullptr), bit0(0) {
+    const uintptr_t at = (uintptr_t)((const T*)v.probs + (int64_t)row * v.probs_stride);
+    shift = (int)((at & 15) / sizeof(T));
+    p = (const char*)(at & ~(uintptr_t)15);
+    chunks = (vocab + shift + E - 1) / E;
+    q = v.draft && a_ != 0. ? (const T*)v.draft + (int64_t)row * v.draft_stride : nullptr;
+    q_alike = ((uintptr_t)q & 15) == (at & 15);
+  }
+  struct chunk {
+    T p[E], q[E];
+  };
+  __device__ __forceinline__ chunk load(int c) const {
+    chunk x;
+    const vec16 v = ld16(p + (int64_t)c * 16);     // its 16 bytes hold a token of the row: inside its page
+    __builtin_memcpy(x.p, &v, 16);
+    if (q) {
+      if (q_alike) {
+        const vec16 w = ld16((const char*)q - shift * (int)sizeof(T) + (int64_t)c * 16);
+        __builtin_memcpy(x.q, &w, 16);
+      } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j) x.q[j] = q[min(max(c * E - shift + j, 0), vocab - 1)];
+      }
+    }
+    return x;
+  }
+  // what is left of the chunk's j-th token
+  __device__ __forceinline__ double weight(const chunk& x, int c, int j, bool edge) const {
+    double w = (double)(float)x.p[j];
+    if (q) w = fma(-a, (double)(float)x.q[j], w);
+    const int i = c * E - shift + j;
+    if (edge && (i < 0 || i >= vocab)) return 0.;
+    if (bits && ((bits[(i - bit0) >> 5] >> ((i - bit0) & 31)) & 1)) return 0.;
+    return w > 0. ? w : 0.;
+  }
+  __device__ __forceinline__ double sum(const chunk& x, int c) const {
+    const bool edge = c == 0 || c == chunks - 1;
+    double s = 0.;
+#pragma unroll
+    for (int j = 0; j < E; ++j) s += weight(x, c, j, edge);
+    return s;
+  }
+  // this thread's share of chunks [b, e): every nth from b + i on
+  __device__ __forceinline__ double share(int b, int e, int i, int nth) const {
+    constexpr int U = 4;                           // chunks in flight
+    double s = 0.;
+    int c = b + i;
+    for (; c + (U - 1) * nth < e; c += U * nth) {
+      chunk x[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) x[k] = load(c + k * nth);
+#pragma unroll
+      for (int k = 0; k < U; ++k) s += sum(x[k], c + k * nth);
+    }
+    for (; c < e; c += nth) s += sum(load(c), c);
+    return s;
+  }
+  // the refused tokens among chunks [b, e) as bits; by all threads
+  __device__ void refuse(const verify_tree& t, int n, int cur, uint32_t* lds, int b, int e) {
+    bit0 = b * E - shift;
+    const int count = (e - b) * E;
+    for (int k = threadIdx.x; k < (count + 31) / 32; k += blockDim.x) lds[k] = 0;
+    __syncthreads();
+    for (int k = threadIdx.x; k < n; k += blockDim.x) {
+      const int x = t.tok[k] - bit0;
+      if (t.par[k] == cur && t.tok[k] >= 0 && x >= 0 && x < count) atomicOr(&lds[x >> 5], 1u << (x & 31));
+    }
+    __syncthreads();
+    bits = lds;
+  }
+};
+
+__device__ __forceinline__ int stretch_begin(int chunks, int stretches, int g) {
+  return (int)((int64_t)chunks * g / stretches);
+}
+
+template <typename T>
+__global__ __launch_bounds__(SUM_THREADS) void verify_sum_kernel(const verify_args a, int launch) {
+  extern __shared__ __align__(16) char lds[];
+  __shared__ double part[SUM_THREADS / 64];
+  __shared__ verify_state shared;
+  const int seq = blockIdx.x, g = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int row0 = a.row_starts[seq], n = min(a.row_starts[seq + 1] - row0, a.width);
   int32_t* const acc = a.accepted + (int64_t)seq * a.width;
   int64_t* const out = a.out_tokens + (int64_t)seq * a.width;
-  for (int i = tid; i < a.width; i += VERIFY_THREADS) acc[i] = -1, out[i] = -1;
-  if (n <= 0) {
-    if (tid == 0) a.num_accepted[seq] = 0;
-    return;
+  verify_state st{0., 0, 1, 1, 0};
+  double s = 1.;
+  if (launch > 0) {
+    st = a.states[(int64_t)(launch - 1) * a.num_seqs + seq];
+    if (n > 0 && st.round < 0) {
+      const double* const sums = a.sums + ((int64_t)(launch - 1) * a.num_seqs + seq) * a.stretches;
+      s = sum64(lane < a.stretches ? sums[lane] : 0.);
+    } else {                                       // this sequence's sum is there already
+      if (g == 0 && tid == 0) a.states[(int64_t)launch * a.num_seqs + seq] = st;
+      return;
+    }
+  } else if (g == 0) {
+    for (int i = tid; i < a.width; i += SUM_THREADS) acc[i] = -1, out[i] = -1;
+    if (n <= 0 && tid == 0) {
+      a.states[seq] = st;
+      a.num_accepted[seq] = 0;
+    }
   }
-  for (int i = tid; i < n; i += VERIFY_THREADS) {
-    const int64_t t = a.tokens[row0 + i];
-    tok[i] = t >= 0 && t < a.vocab ? (int32_t)t : -1;
-    par[i] = a.parents[row0 + i];
+  if (n <= 0) return;
+  const verify_tree t(lds, a.width);
+  int32_t* const path = (int32_t*)(lds + verify_tree::bytes(a.width));
+  load_tree<T>(a, t, row0, n);
+  __syncthreads();
+  const int len0 = launch > 0 ? st.len : 0;
+  if (wave == 0) {
+    if (launch == 0 && lane == 0) path[0] = 0;
+    walk(t, n, a.draft != nullptr, s, st, path, lane, launch);
+    if (lane == 0) shared = st;
   }
   __syncthreads();
+  st = shared;
+  if (g == 0) {
+    for (int i = len0 + tid; i < st.len; i += SUM_THREADS) {
+      acc[i] = path[i];
+      if (i > 0) out[i - 1] = a.tokens[row0 + path[i]];
+    }
+    if (tid == 0) a.states[(int64_t)launch * a.num_seqs + seq] = st;
+  }
+  verify_row<T> row(a, row0 + st.cur, st.a);
+  const int b = stretch_begin(row.chunks, a.stretches, g), e = stretch_begin(row.chunks, a.stretches, g + 1);
+  if (!a.draft) row.refuse(t, n, st.cur, (uint32_t*)(path + a.width), b, e);
+  const double x = sum64(row.share(b, e, tid, SUM_THREADS));
+  if (lane == 0) part[wave] = x;
+  __syncthreads();
+  if (tid == 0) {
+    double w = 0.;
+#pragma unroll
+    for (int k = 0; k < SUM_THREADS / 64; ++k) w += part[k];
+    a.sums[((int64_t)launch * a.num_seqs + seq) * a.stretches + g] = w;
+  }
+}
 
-  const T *p = nullptr, *q = nullptr;
-  auto at_row = [&](int node) {
-    p = (const T*)a.probs + (int64_t)(row0 + node) * a.probs_stride;
-    q = a.draft ? (const T*)a.draft + (int64_t)(row0 + node) * a.draft_stride : nullptr;
-  };
-  // what is left of token i after the refusals so far (`nref` refused tokens, or a)
-  int nref = 0;
-  double s = 1., ra = 0.;
-  bool whole = false;
-  auto weight = [&](int i) -> double {
-    double w = (double)(float)p[i];
-    if (whole) return w > 0. ? w : 0.;
-    if (q) w -= ra * (double)(float)q[i];
-    else
-      for (int k = 0; k < nref; ++k)
-        if (refused[k] == i) w = 0.;
-    return w > 0. ? w : 0.;
-  };
-  auto reduce = [&](double x) -> double {          // over the workgroup
+// The last launch: the walk's rest where more sums are needed than there were launches, and the token.
+template <typename T>
+__global__ __launch_bounds__(FIND_THREADS) void verify_find_kernel(const verify_args a, int launches) {
+  extern __shared__ __align__(16) char lds[];
+  constexpr int NW = FIND_THREADS / 64, E = verify_row<T>::E;
+  __shared__ double part[NW], before_s;
+  __shared__ verify_state shared;
+  __shared__ int32_t first, last, token;
+  const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int row0 = a.row_starts[seq], n = min(a.row_starts[seq + 1] - row0, a.width);
+  if (n <= 0) return;
+  int32_t* const acc = a.accepted + (int64_t)seq * a.width;
+  int64_t* const out = a.out_tokens + (int64_t)seq * a.width;
+  verify_state st = a.states[(int64_t)(launches - 1) * a.num_seqs + seq];
+  const verify_tree t(lds, a.width);
+  int32_t* const path = (int32_t*)(lds + verify_tree::bytes(a.width));
+  uint32_t* const bits = (uint32_t*)(path + a.width);
+  const bool pending = st.round < 0;
+  if (pending || !a.draft) {
+    load_tree<T>(a, t, row0, n);
+    __syncthreads();
+  }
+  auto total = [&](double x) -> double {           // over the workgroup
     x = sum64(x);
     __syncthreads();
     if (lane == 0) part[wave] = x;
     __syncthreads();
-    double t = 0.;
-    for (int w = 0; w < VERIFY_THREADS / 64; ++w) t += part[w];
-    return t;
+    return sum64(lane < NW ? part[lane] : 0.);
   };
-  auto total = [&]() -> double {
-    double x = 0.;
-    for (int i = tid; i < a.vocab; i += VERIFY_THREADS) x += weight(i);
-    return reduce(x);
+  // the first of the threads' ranges that passes the border, x this thread's sum: its thread and
+  // what lies before it; the last one that holds anything where none passes
+  auto pick = [&](double x, double border, double& before) -> int {
+    const double run = scan64<64>(x, lane);
+    __syncthreads();
+    if (lane == 63) part[wave] = run;
+    if (tid == 0) first = FIND_THREADS, last = -1;
+    __syncthreads();
+    const double head = scan64<NW>(lane < NW ? part[lane] : 0., lane);   // of the waves, inclusive
+    const double base = before + (wave ? __shfl(head, wave - 1) : 0.);
+    if (x > 0.) {
+      if (base + run > border) atomicMin(&first, tid);
+      atomicMax(&last, tid);
+    }
+    __syncthreads();
+    const int at = first < FIND_THREADS ? first : last;
+    if (tid == at) before_s = base + (run - x);
+    __syncthreads();
+    before = before_s;
+    return at;
   };
 
-  int cur = 0, len = 1;
-  at_row(0);
-  if (tid == 0) path[0] = 0;
-  for (int i = 1; i < n; ++i) {
-    if (par[i] != cur) continue;
-    const int x = tok[i];
-    const double u = (double)a.uniforms[row0 + i];
-    double px = x < 0 ? 0. : (double)(float)p[x];
-    bool keep;
-    if (q) {
-      const double qx = x < 0 ? 0. : (double)(float)q[x];
-      keep = u * qx * s < px - ra * qx;
-    } else {
-      bool again = false;
-      for (int k = 0; k < nref; ++k) again |= refused[k] == x;
-      if (again) px = 0.;
-      keep = px > 0. && u * s < px;
-      if (!keep) s -= px > 0. ? px : 0.;
+  if (pending) {
+    // the rest of the walk by this workgroup alone
+    double s = sum64(lane < a.stretches ? a.sums[((int64_t)(launches - 1) * a.num_seqs + seq) * a.stretches + lane] : 0.);
+    const int len0 = st.len;
+    for (;;) {
+      if (wave == 0) {
+        walk(t, n, true, s, st, path, lane, launches);
+        if (lane == 0) shared = st;
+      }
+      __syncthreads();
+      st = shared;
+      __syncthreads();
+      if (st.round >= 0) break;
+      const verify_row<T> row(a, row0 + st.cur, st.a);
+      s = total(row.share(0, row.chunks, tid, FIND_THREADS));
     }
-    if (keep) {
-      cur = i;
-      nref = 0, s = 1., ra = 0.;
-      at_row(i);
-      if (tid == 0) path[len] = i;
-      ++len;
-    } else if (q) {
-      ra += s;
-      s = total();
-    } else {
-      __syncthreads();
-      if (tid == 0) refused[nref] = x;
-      ++nref;
-      __syncthreads();
+    for (int i = len0 + tid; i < st.len; i += FIND_THREADS) {
+      acc[i] = path[i];
+      out[i - 1] = a.tokens[row0 + path[i]];
     }
   }
-  __syncthreads();
 
-  // the next token: the border's place by sums of contiguous stretches
-  double w = total();
-  if (!(w > 0.)) {
-    whole = true;
-    w = total();
+  verify_row<T> row(a, row0 + st.cur, st.a);
+  const double u = (double)a.uniforms[row0];
+  int b = 0, e = row.chunks;
+  double before = 0., border = 0., w;
+  if (!pending) {                                  // the stretch, from its launch's sums
+    const double x = lane < a.stretches ? a.sums[((int64_t)st.round * a.num_seqs + seq) * a.stretches + lane] : 0.;
+    const double run = scan64<64>(x, lane);
+    w = __shfl(run, 63);
+    border = u * w;
+    const uint64_t some = __ballot(x > 0.), past = __ballot(x > 0. && run > border);
+    if (w > 0.) {
+      const int g = past ? __ffsll((unsigned long long)past) - 1 : 63 - __clzll((long long)some);
+      b = stretch_begin(row.chunks, a.stretches, g), e = stretch_begin(row.chunks, a.stretches, g + 1);
+      before = __shfl(run - x, g);
+      if (!a.draft) row.refuse(t, n, st.cur, bits, b, e);
+    }
+  } else {
+    w = total(row.share(b, e, tid, FIND_THREADS));
+    border = u * w;
+  }
+  if (!(w > 0.)) {                                 // nothing is left: the row as it is
+    row.q = nullptr;
+    row.bits = nullptr;
+    w = total(row.share(b, e, tid, FIND_THREADS));
+    border = u * w;
   }
   int next = -1;
   if (w > 0.) {
-    const double border = (double)a.uniforms[row0] * w;
-    int lo = 0, hi = a.vocab;
-    double before = 0.;
-    while (hi - lo > 1) {
-      const int step = (hi - lo + VERIFY_THREADS - 1) / VERIFY_THREADS;
-      const int b = min(hi, lo + tid * step), e = min(hi, b + step);
-      double x = 0.;
-      for (int i = b; i < e; ++i) x += weight(i);
-      // sums of the threads before this one
-      double run = x;
-      for (int o = 1; o < 64; o *= 2) {
-        const double y = __shfl_up(run, o);
-        if (lane >= o) run += y;
-      }
-      __syncthreads();
-      if (lane == 63) part[wave] = run;
-      __syncthreads();
-      double base = before;
-      for (int v = 0; v < wave; ++v) base += part[v];
-      // the first stretch whose end passes the border; the last with any weight if none does
-      const bool past = x > 0. && base + run > border;
-      const bool some = x > 0.;
-      __shared__ int32_t first, last;
-      if (tid == 0) first = VERIFY_THREADS, last = -1;
-      __syncthreads();
-      if (past) atomicMin(&first, tid);
-      if (some) atomicMax(&last, tid);
-      __syncthreads();
-      const int pick = first < VERIFY_THREADS ? first : last;
-      __shared__ double start;
-      if (tid == pick) start = base + run - x;
-      __syncthreads();
-      before = start;
-      lo = lo + pick * step;
-      hi = min(hi, lo + step);
-      __syncthreads();
+    // by waves of neighbouring chunks, until a thread has a few neighbouring chunks of its own
+    while (e - b > FIND_THREADS * 4) {
+      const int step = (e - b + NW - 1) / NW, wb = min(e, b + wave * step), we = min(e, wb + step);
+      const double x = sum64(row.share(wb, we, lane, 64));
+      const int at = pick(lane == 0 ? x : 0., border, before) >> 6;
+      b = min(e, b + at * step);
+      e = min(e, b + step);
     }
-    next = lo;
+    const int step = (e - b + FIND_THREADS - 1) / FIND_THREADS;
+    const int tb = min(e, b + tid * step), te = min(e, tb + step);
+    double x = 0.;
+    for (int c = tb; c < te; ++c) x += row.sum(row.load(c), c);
+    const int at = pick(x, border, before);
+    if (tid == at) {
+      int found = -1;
+      double run = before;
+      for (int c = tb; c < te; ++c) {
+        const auto k = row.load(c);
+        const bool edge = c == 0 || c == row.chunks - 1;
+        for (int j = 0; j < E; ++j) {
+          const double y = row.weight(k, c, j, edge);
+          if (!(y > 0.) || (found >= 0 && run > border)) continue;
+          run += y;
+          found = c * E - row.shift + j;           // the last one so far; the first that passes stays
+        }
+      }
+      token = found;
+    }
+    __syncthreads();
+    next = token;
   }
-  for (int i = tid; i < min(len, a.width); i += VERIFY_THREADS) {
-    acc[i] = path[i];
-    out[i] = i + 1 < len ? a.tokens[row0 + path[i + 1]] : (int64_t)next;
+  if (tid == 0) {
+    out[st.len - 1] = (int64_t)next;
+    a.num_accepted[seq] = st.len;
   }
-  if (tid == 0) a.num_accepted[seq] = len;
+}
+
+// Workgroups of a sequence: about four per CU over the batch, and few enough tokens for the bits.
+static int verify_stretches(int num_seqs, int vocab) {
+  const int want = std::min(1024 / std::max(num_seqs, 1), std::max(vocab / 1024, 1));
+  return std::min(std::max({want, (vocab + MAX_STRETCH - 1) / MAX_STRETCH, 1}), MAX_STRETCHES);
+}
+
+template <typename T>
+static void launch_verify(const verify_args& a, int rounds, hipStream_t stream) {
+  const int per = (a.vocab + 16 + a.stretches - 1) / a.stretches + 16;   // tokens of a stretch, at most
+  const size_t lds = verify_tree::bytes(a.width) + 4 * (size_t)a.width + (a.draft ? 0 : (size_t)(per / 32 + 1) * 4);
+  for (int r = 0; r <= rounds; ++r)
+    hipLaunchKernelGGL((verify_sum_kernel<T>), dim3(a.num_seqs, a.stretches), dim3(SUM_THREADS), lds, stream, a, r);
+  hipLaunchKernelGGL((verify_find_kernel<T>), dim3(a.num_seqs), dim3(FIND_THREADS), lds, stream, a, rounds + 1);
 }
 
 // The same walk for greedy targets: a child is kept where its token is the target's choice
@@ -264,24 +524,38 @@ __global__ __launch_bounds__(256) void commit_kernel(char* storage, int64_t laye
 
 }  // namespace tb
 
+extern "C" size_t tb_tree_verify_workspace_bytes(int32_t num_seqs, int32_t vocab) {
+  using namespace tb;
+  if (num_seqs <= 0 || vocab <= 0) return 0;
+  return (size_t)(MAX_ROUNDS + 1) * num_seqs *
+         (sizeof(verify_state) + sizeof(double) * verify_stretches(num_seqs, vocab));
+}
+
 extern "C" int32_t tb_tree_verify(const void* probs, int64_t probs_row_stride, const void* draft_probs,
                                   int64_t draft_row_stride, int32_t vocab, int32_t dtype, const int64_t* tokens,
                                   const float* uniforms, const int32_t* parents, const int32_t* row_starts,
-                                  int32_t num_seqs, int32_t* accepted, int32_t* num_accepted, int64_t* out_tokens,
-                                  int32_t width, hipStream_t stream) {
+                                  int32_t num_seqs, int32_t max_children, int32_t* accepted, int32_t* num_accepted,
+                                  int64_t* out_tokens, int32_t width, void* workspace, size_t workspace_bytes,
+                                  hipStream_t stream) {
   using namespace tb;
-  TB_CHECK_ARG(num_seqs >= 0 && vocab > 0 && width > 0);
+  TB_CHECK_ARG(num_seqs >= 0 && vocab > 0 && width > 0 && max_children >= 0);
   TB_CHECK_ARG(dtype >= TB_DTYPE_F32 && dtype <= TB_DTYPE_BF16);
-  if (width > TB_TREE_MAX_NODES) return TB_ERR_UNSUPPORTED;
+  if (width > TB_TREE_MAX_NODES || vocab > MAX_STRETCHES * (MAX_STRETCH - 64)) return TB_ERR_UNSUPPORTED;
   if (num_seqs == 0) return TB_OK;
   TB_CHECK_ARG(probs && tokens && uniforms && parents && row_starts && accepted && num_accepted && out_tokens);
   TB_CHECK_ARG(probs_row_stride >= vocab && (!draft_probs || draft_row_stride >= vocab));
+  TB_CHECK_ARG(workspace && ((uintptr_t)workspace & 7u) == 0 &&
+               workspace_bytes >= tb_tree_verify_workspace_bytes(num_seqs, vocab));
+  const int stretches = verify_stretches(num_seqs, vocab);
+  // sums that tests of later siblings need: none in a chain, or where the drafts were not drawn
+  const int rounds = draft_probs ? std::min(std::max(max_children - 1, 0), MAX_ROUNDS) : 0;
+  verify_state* const states = (verify_state*)workspace;
   const verify_args a{probs, probs_row_stride, draft_probs, draft_row_stride, vocab, tokens, uniforms, parents,
-                      row_starts, accepted, num_accepted, out_tokens, width};
-  const dim3 grid(num_seqs), block(VERIFY_THREADS);
-  if (dtype == TB_DTYPE_F32) hipLaunchKernelGGL((verify_kernel<float>), grid, block, 0, stream, a);
-  else if (dtype == TB_DTYPE_F16) hipLaunchKernelGGL((verify_kernel<_Float16>), grid, block, 0, stream, a);
-  else hipLaunchKernelGGL((verify_kernel<__bf16>), grid, block, 0, stream, a);
+                      row_starts, accepted, num_accepted, out_tokens, width, num_seqs, stretches, states,
+                      (double*)(states + (size_t)(MAX_ROUNDS + 1) * num_seqs)};
+  if (dtype == TB_DTYPE_F32) launch_verify<float>(a, rounds, stream);
+  else if (dtype == TB_DTYPE_F16) launch_verify<_Float16>(a, rounds, stream);
+  else launch_verify<__bf16>(a, rounds, stream);
   TB_RETURN_LAUNCH_STATUS();
 }
 

@@ -31,6 +31,7 @@ from .metadata import pad4
 from .ops import Rope, _check_pool, _rows_view, kv_append
 
 MAX_NODES = 1024             # TB_TREE_MAX_NODES
+MAX_VOCAB = 64 * ((1 << 18) - 64)
 NUM_CUS, NUM_XCDS = 256, 8   # MI355X, for which the work lists are made
 
 
@@ -41,6 +42,7 @@ class TreeMetadata:
     num_rows: int
     num_seqs: int
     max_nodes: int               # nodes of the largest tree
+    max_children: int            # of one node
     mask_words: int              # 32-bit words of a row's mask
     # the cache part (None / 0 without cached_lens)
     block_size: int
@@ -182,10 +184,11 @@ def build_tree_metadata(parents, cached_lens=None, block_tables=None, *, block_s
     if visible is not None and len(visible) != len(parents):
         raise ValueError("visible needs one entry per sequence")
     words = max(1, -(-max_nodes // 32))
+    children = max((int(np.bincount(np.array(t[1:], dtype=np.int64)).max()) for t in parents if len(t) > 1), default=0)
     row_starts = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32)
     T, B = int(row_starts[-1]), len(parents)
     meta = TreeMetadata(
-        num_rows=T, num_seqs=B, max_nodes=max_nodes, mask_words=words, block_size=block_size, num_blocks=num_blocks,
+        num_rows=T, num_seqs=B, max_nodes=max_nodes, max_children=children, mask_words=words, block_size=block_size, num_blocks=num_blocks,
         max_blocks_per_seq=0, num_heads=num_heads, num_kv_heads=num_kv_heads, head_dim=head_dim, dtype=dtype,
         parents_np=np.array([p for t in parents for p in t], dtype=np.int32), row_starts_np=row_starts,
         depths_np=np.array(depths, dtype=np.int64), mask_np=_masks(parents, visible, words),
@@ -361,20 +364,22 @@ def verify_tree(meta: TreeMetadata, tokens: torch.Tensor, uniforms: torch.Tensor
         if t.dtype != probs.dtype or t.device != device:
             raise TypeError(f"{name} must share probs' dtype and device")
     vocab = probs.shape[1]
-    if vocab >= 1 << 30:
-        raise ValueError("a vocabulary of 2^30 tokens or more")
+    if vocab > MAX_VOCAB:
+        raise ValueError(f"a vocabulary of {vocab} tokens; at most {MAX_VOCAB} are served")
     _node_values("tokens", tokens, torch.int64, T, device)
     _node_values("uniforms", uniforms, torch.float32, T, device)
     v = _verdict(meta, device)
+    L = _lib.lib()
+    ws = torch.empty(L.tb_tree_verify_workspace_bytes(meta.num_seqs, vocab), device=device, dtype=torch.uint8)
     if T == 0:
         return v._replace(accepted=v.accepted.fill_(-1), num_accepted=v.num_accepted.zero_(), tokens=v.tokens.fill_(-1))
     with _on(device):
-        st = _lib.lib().tb_tree_verify(
+        st = L.tb_tree_verify(
             probs.data_ptr(), max(probs.stride(0), vocab), None if draft_probs is None else draft_probs.data_ptr(),
             0 if draft_probs is None else max(draft_probs.stride(0), vocab), vocab, _lib.DTYPE_CODE[probs.dtype],
             tokens.data_ptr(), uniforms.data_ptr(), meta.parents.data_ptr(), meta.row_starts.data_ptr(),
-            meta.num_seqs, v.accepted.data_ptr(), v.num_accepted.data_ptr(), v.tokens.data_ptr(),
-            v.accepted.shape[1], _lib.stream_handle(device))
+            meta.num_seqs, meta.max_children, v.accepted.data_ptr(), v.num_accepted.data_ptr(), v.tokens.data_ptr(),
+            v.accepted.shape[1], ws.data_ptr(), ws.numel(), _lib.stream_handle(device))
     _lib.check(st, "tb_tree_verify")
     return v
 
