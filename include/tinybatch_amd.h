@@ -740,7 +740,7 @@ size_t tb_tree_attention_workspace_bytes(int32_t partial_slots, int32_t num_head
  *   workspace: tb_tree_verify_workspace_bytes, 8-byte aligned; calls that may overlap in time need
  *     their own.
  * dtype is that of probs and draft_probs; row strides in elements. */
-size_t tb_tree_verify_workspace_bytes(int32_t num_seqs, int32_t vocab);
+size_t tb_tree_verify_workspace_bytes(int32_t num_seqs, int32_t vocab, int32_t width);
 int32_t tb_tree_verify(const void* probs, int64_t probs_row_stride, const void* draft_probs,
                        int64_t draft_row_stride, int32_t vocab, int32_t dtype, const int64_t* tokens,
                        const float* uniforms, const int32_t* parents, const int32_t* row_starts,

@@ -115,7 +115,7 @@ def test_entries_reject_bad_arguments_without_launching():
     assert verify(vocab=0) == bad and verify(dt=3) == bad and verify(width=0) == bad
     assert verify(probs=None) == bad and verify(tokens=None) == bad and verify(acc=None) == bad
     assert verify(children=-1) == bad and verify(ws=None) == bad and verify(ws=ctypes.c_void_p(4100)) == bad
-    assert verify(wsb=L.tb_tree_verify_workspace_bytes(2, 100) - 1) == bad
+    assert verify(wsb=L.tb_tree_verify_workspace_bytes(2, 100, 4) - 1) == bad
     assert verify(width=MAX_NODES + 1) == unsupported
     assert verify(vocab=1 << 25, stride=1 << 25, wsb=1 << 30) == unsupported
     assert verify(seqs=0, probs=None) == _lib.TB_OK

@@ -145,7 +145,7 @@ SIGNATURES = {
     "tb_build_tree_work": (c_i32, [c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp, c_i32, c_vp,
                                    c_i32, c_vp]),
     "tb_tree_attention_workspace_bytes": (c_sz, [c_i32, c_i32, c_i32]),
-    "tb_tree_verify_workspace_bytes": (c_sz, [c_i32, c_i32]),
+    "tb_tree_verify_workspace_bytes": (c_sz, [c_i32, c_i32, c_i32]),
     "tb_tree_verify": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i32,   # probs, stride, draft, stride, vocab, dtype
                                c_vp, c_vp, c_vp, c_vp, c_i32, c_i32,     # tokens, uniforms, parents, row starts, seqs, children
                                c_vp, c_vp, c_vp, c_i32, c_vp, c_sz, c_vp]),   # outputs, width, workspace, bytes, stream

@@ -10,11 +10,13 @@
 //
 // Work: the n nodes and the rep query heads of a kv head make n * rep columns, column =
 // node * rep + head, that read the same K/V rows whatever their masks. A workgroup takes
-// 32 CB consecutive columns of a (sequence, kv head) and a part of the context; its waves
-// take the part's chunks of 32 positions in turn, each through a ring of its own in LDS
-// filled by direct global->LDS loads, with no barrier between them, and join their softmax
-// states in LDS at the end. A context cut into parts leaves a partial per part, joined by
-// a second launch.
+// consecutive columns of a (sequence, kv head) and a part of the context.
+// - Up to 64 columns (32 CB): its waves take the part's chunks of 32 positions in turn, each
+//   through a ring of its own in LDS filled by direct global->LDS loads, with no barrier between
+//   them, and join their softmax states in LDS at the end.
+// - More, in 16 bits: 128 columns, 32 for each of four waves, which share the chunks: 64 positions
+//   through a ring of two, one barrier each, so that a K or V row loaded meets 128 columns.
+// A context cut into parts leaves a partial per part, joined by a second launch.
 //
 // Math per chunk and block of 32 columns (C rows are positions or dims, C columns the block's):
 //   S^T[pos][col] = K[pos][:] . q[col][:]        A = K rows from LDS, B = q in registers
@@ -184,15 +186,20 @@ struct tshape {
   }
 };
 
-template <typename Tag, int D, int CB, int NW, int R, int OCC>
+// CW = 1: every wave all 32 CB columns and positions of its own; CW = NW: 32 columns a wave (CB = 1).
+template <typename Tag, int D, int CB, int NW, int R, int OCC, int CW>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
 void tree_columns_kernel(const tree_args a) {
   using S = tshape<Tag, D>;
   using T = typename elem<Tag>::type;
   constexpr int RB = S::RB, CK = S::CK, NB = S::NB, QS = S::QS, LD = S::LD;
   constexpr bool F32 = S::EB == 4;
-  constexpr int MERGE = NW * 64 * (16 * NB + 2) * 4;
-  constexpr int LDS = NW * R * S::SLOT > MERGE ? NW * R * S::SLOT : MERGE;
+  constexpr bool SHARED = CW > 1;
+  constexpr int SUB = SHARED ? 2 : 1;           // chunks of 32 positions in a ring slot
+  constexpr int HALF = SUB * S::HALF, SLOT = 2 * HALF;
+  constexpr int MERGE = SHARED ? 0 : NW * 64 * (16 * NB + 2) * 4, RINGS = SHARED ? 1 : NW;
+  constexpr int LDS = RINGS * R * SLOT > MERGE ? RINGS * R * SLOT : MERGE;
+  static_assert(!SHARED || (CB == 1 && CW == NW && NW == 2 * SUB && R == 2 && !F32), "wave w loads tile w of a slot");
   __shared__ __align__(1024) char lds_all[LDS];
 
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -200,9 +207,9 @@ void tree_columns_kernel(const tree_args a) {
   const int4 w0 = a.work[3 * blockIdx.x], w1 = a.work[3 * blockIdx.x + 1], w2 = a.work[3 * blockIdx.x + 2];
   const int row0 = w0.x, seq = w0.y, cached = w0.z, nodes = w0.w;
   if (nodes == 0) return;                       // a padding entry (whole workgroup)
-  const int col0 = w1.x, kvh = w1.y, chunk0 = w1.z, chunks = w1.w;
+  const int col0 = w1.x + (SHARED ? 32 * wave : 0), kvh = w1.y, chunk0 = w1.z, chunks = w1.w;
   const int limit = cached + nodes, ncols = nodes * a.rep;
-  char* const lds = lds_all + wave * (R * S::SLOT);
+  char* const lds = lds_all + (SHARED ? 0 : wave * (R * SLOT));
 
   // this lane's columns: node my_row, head hd (past the last column: a repeat, not stored)
   int my_row[CB], hd[CB];
@@ -221,7 +228,8 @@ void tree_columns_kernel(const tree_args a) {
     for (int s = 0; s < QS; ++s) q[cb][s] = ld16(qrow + 32 * s);
   }
 
-  // ---- direct loads: the wave's k-th chunk is chunk0 + wave + NW k ----
+  // ---- direct loads: the wave's k-th chunk is chunk0 + wave + NW k; shared: the k-th slot holds chunks
+  // chunk0 + 2 k and the next, of which this wave loads 16 positions ----
   const int64_t head_bytes = ((int64_t)1 << a.log2_bs) * RB;
   const int64_t blk_bytes = 2 * (int64_t)a.num_kv_heads * head_bytes, v_off = a.num_kv_heads * head_bytes;
   const int sub_mask = (1 << (a.log2_bs - 4)) - 1;                // 16-position tiles per block - 1
@@ -229,38 +237,41 @@ void tree_columns_kernel(const tree_args a) {
   const char* const pool_kvh = a.pool + kvh * head_bytes;
   const int last_tile = (limit - 1) >> 4;
   const int lrow = lane / S::PPR, lpiece = lane % S::PPR;
-  const int n = (chunks - wave + NW - 1) / NW;                    // this wave's chunks (<= 0: none)
+  const int n = SHARED ? (chunks + SUB - 1) / SUB : (chunks - wave + NW - 1) / NW;   // its slots (<= 0: none)
+  constexpr int TILES = SHARED ? 1 : 2, IDS = 64 / TILES;         // tiles it loads of a slot; slots whose ids fit
+  auto tile_of = [&](int k, int t) {
+    return min(SHARED ? 2 * chunk0 + NW * k + wave : 2 * (chunk0 + wave + NW * k) + t, last_tile);
+  };
   int id0 = 0;
-  auto load_ids = [&](int k) {                  // lane j: the block of tile j % 2 of chunk k + j / 2
-    const int t = min(2 * (chunk0 + wave + NW * (k + (lane >> 1))) + (lane & 1), last_tile);
+  auto load_ids = [&](int k) {                  // lane j: the block of tile j % TILES of slot k + j / TILES
+    const int t = tile_of(k + lane / TILES, lane % TILES);
     const int b = table[(t << 4) >> a.log2_bs];
     return (b < 0 || b >= a.num_blocks) ? 0 : b;   // host validates; stay inside the pool
   };
   int ids = load_ids(0);
   asm volatile("" : "+v"(ids));                 // the block ids have landed: no wait inside the loop
   auto issue = [&](int k, bool is_v) {
-    if (k - id0 >= 32) {                        // uniform, once per 32 chunks
+    if (k - id0 >= IDS) {                       // uniform, once per 32 or 64 slots
       id0 = k;
       ids = load_ids(k);
     }
-    const int c = chunk0 + wave + NW * k;
-    char* const dst = lds + (k % R) * S::SLOT + (is_v ? S::HALF : 0);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int tile = min(2 * c + t, last_tile);
+    for (int t = 0; t < TILES; ++t) {
+      const int tile = tile_of(k, t), at = SHARED ? wave : t;     // its place in the slot
       const int rmax = limit - 1 - 16 * tile;   // rows past it repeat the last position
-      const int64_t b = __builtin_amdgcn_readlane(ids, 2 * (k - id0) + t);
+      const int64_t b = __builtin_amdgcn_readlane(ids, TILES * (k - id0) + t);
       const char* const base = pool_kvh + b * blk_bytes + (int64_t)(tile & sub_mask) * S::TB + (is_v ? v_off : 0);
+      char* const dst = lds + (k % R) * SLOT + (is_v ? HALF : 0) + at * S::TB;
 #pragma unroll
       for (int i = 0; i < LD / 2; ++i) {
         const int r = S::RPL * i + lrow;
-        s_dma16_l2((uint32_t)(min(r, rmax) * RB + 16 * (lpiece ^ (is_v ? S::vswz(r) : S::kswz(16 * t + r)))), base,
-                   dst + (t * (LD / 2) + i) * 1024);
+        s_dma16_l2((uint32_t)(min(r, rmax) * RB + 16 * (lpiece ^ (is_v ? S::vswz(r) : S::kswz(r)))), base,
+                   dst + i * 1024);
       }
     }
   };
 #pragma unroll
-  for (int k = 0; k < R; ++k)
+  for (int k = 0; k < (SHARED ? 1 : R); ++k)
     if (k < n) {
       issue(k, false);
       issue(k, true);
@@ -315,8 +326,8 @@ void tree_columns_kernel(const tree_args a) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       const int c = 4 * b + 2 * ((lane >> 4) & 1) + ((li & 3) >> 1);
-      va[b] = F32 ? (uint32_t)(S::HALF + 4 * half * RB + 128 * b + 4 * lcol)
-                  : (uint32_t)(S::HALF + rv * RB + 16 * (c ^ S::vswz(rv)) + 8 * (li & 1));
+      va[b] = F32 ? (uint32_t)(HALF + 4 * half * RB + 128 * b + 4 * lcol)
+                  : (uint32_t)(HALF + rv * RB + 16 * (c ^ S::vswz(rv)) + 8 * (li & 1));
     }
   }
   const float sl2e = a.scale_log2e;
@@ -461,7 +472,7 @@ void tree_columns_kernel(const tree_args a) {
   auto values_finite = [&](const char* base) {
     bool ok = true;
     for (int i = 0; i < S::HALF / 1024; ++i) {
-      const vec16 v = ld16(base + S::HALF + 1024 * i + 16 * lane);
+      const vec16 v = ld16(base + HALF + 1024 * i + 16 * lane);
       constexpr uint32_t E1 = F32 ? 0x7F800000u : sizeof(T) == 2 && __is_same(T, _Float16) ? 0x7C00u : 0x7F80u;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -498,7 +509,7 @@ void tree_columns_kernel(const tree_args a) {
           for (int b = 0; b < NB; ++b)
 #pragma unroll
             for (int g = 0; g < 4; ++g) {       // dims 32 b + 8 g + 4 half ..
-              const char* const vp = base + S::HALF + pos * RB +
+              const char* const vp = base + HALF + pos * RB +
                                      (F32 ? 128 * b + 32 * g + 16 * half : 16 * ((4 * b + g) ^ S::vswz(pos)) + 8 * half);
               T e[4];
               __builtin_memcpy(e, __builtin_assume_aligned(vp, 8), 4 * sizeof(T));
@@ -510,30 +521,85 @@ void tree_columns_kernel(const tree_args a) {
     }
   };
 
-  // Loads of chunk k + R's K follow chunk k's scores, its V's chunk k's products. Outstanding when
-  // chunk k's K (or V) must be there: the halves issued behind it.
-  for (int k = 0; k < n; ++k) {
-    const int c = chunk0 + wave + NW * k;
-    const char* const base = lds + (k % R) * S::SLOT;
-    const int ahead = min(R - 1, n - 1 - k);    // chunks issued behind chunk k
-    if (ahead == R - 1) s_vm_wait_le(LD * (1 + 2 * (R - 1)));
-    else s_vm_wait_le(LD * (1 + 2 * ahead));
-    scores(base);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the K rows are in registers: their slot is free
-    const bool more = k + R < n;
-    if (more) issue(k + R, false);
-    const bool masked = CK * c + CK > cached;
-    softmax(c, masked);
-    if (more) s_vm_wait_le(LD * (1 + 2 * (R - 1)));
-    else s_vm_wait_le(LD * 2 * ahead);
+  auto chunk_values = [&](const char* base, bool masked) {
     if (masked && !values_finite(base)) values_apart(base);
     else values(base);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (more) issue(k + R, true);
+  };
+  if constexpr (SHARED) {
+    const bool busy = col0 < ncols;
+    for (int k = 0; k < n; ++k) {
+      // the wave's loads of slot k have landed and its reads of slot k - 1 are done: behind the barrier
+      // all of slot k is in LDS and the other one is free
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      if (k + 1 < n) {
+        issue(k + 1, false);
+        issue(k + 1, true);
+      }
+#pragma unroll 1
+      for (int t = 0; t < SUB; ++t) {
+        const int c = chunk0 + SUB * k + t;
+        if (!busy || c >= chunk0 + chunks) break;
+        const char* const base = lds + (k % R) * SLOT + t * S::HALF;
+        const bool masked = CK * c + CK > cached;
+        scores(base);
+        softmax(c, masked);
+        chunk_values(base, masked);
+      }
+    }
+  } else {
+    // Loads of chunk k + R's K follow chunk k's scores, its V's chunk k's products. Outstanding when
+    // chunk k's K (or V) must be there: the halves issued behind it.
+    for (int k = 0; k < n; ++k) {
+      const int c = chunk0 + wave + NW * k;
+      const char* const base = lds + (k % R) * SLOT;
+      const int ahead = min(R - 1, n - 1 - k);    // chunks issued behind chunk k
+      if (ahead == R - 1) s_vm_wait_le(LD * (1 + 2 * (R - 1)));
+      else s_vm_wait_le(LD * (1 + 2 * ahead));
+      scores(base);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the K rows are in registers: their slot is free
+      const bool more = k + R < n;
+      if (more) issue(k + R, false);
+      const bool masked = CK * c + CK > cached;
+      softmax(c, masked);
+      if (more) s_vm_wait_le(LD * (1 + 2 * (R - 1)));
+      else s_vm_wait_le(LD * 2 * ahead);
+      chunk_values(base, masked);
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (more) issue(k + R, true);
+    }
   }
 
+  if constexpr (SHARED) {                       // a wave's columns are its own
+    const float L = sum_xor32(l[0]);
+    const int slot = w2.x, row = row0 + my_row[0];
+    if (col0 + lcol >= ncols) return;
+    float inv = 1.f;
+    if (slot < 0) {
+      inv = 1.f / L;
+      if (!(L > 0.f) && !tree_sees(a.mask + (int64_t)row * a.mask_words, cached, nodes)) inv = 0.f;
+    }
+    typedef T t4_t __attribute__((ext_vector_type(4)));
+    const int64_t at = (int64_t)(slot + my_row[0]) * a.num_heads + hd[0];
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {             // dims 32 b + 8 g + 4 half ..
+        const float4_t o = {acc[0][b][4 * g], acc[0][b][4 * g + 1], acc[0][b][4 * g + 2], acc[0][b][4 * g + 3]};
+        if (slot < 0) {
+          t4_t t;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) t[j] = (T)(o[j] * inv);
+          st_through(a.out + (int64_t)row * a.out_row_bytes + (int64_t)hd[0] * RB + (32 * b + 8 * g + 4 * half) * S::EB, t);
+        } else {
+          *reinterpret_cast<float4_t*>(a.ws_acc + at * D + 32 * b + 8 * g + 4 * half) = o;
+        }
+      }
+    if (slot >= 0 && half == 0) *reinterpret_cast<float2*>(a.ws_ml + at * 2) = make_float2(m[0], L);
+    return;
+  }
   // ---- the waves' states joined; wave w stores the 4-dim groups w, w + NW, ... of a column ----
-  const int slot = w2.x, slot_rows = w2.y;      // slot < 0: the whole context, the output itself
+  if constexpr (!SHARED) {
+  const int slot = w2.x;                        // < 0: the whole context, the output itself
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
     l[cb] = sum_xor32(l[cb]);
@@ -587,7 +653,7 @@ void tree_columns_kernel(const tree_args a) {
       }
     }
   }
-  (void)slot_rows;
+  }
 }
 
 // The partials of a row's parts joined: thread = 4 dims of a head.
@@ -641,7 +707,7 @@ __global__ __launch_bounds__(64) void tree_join_kernel(const tree_args a) {
   st_through(a.out + (int64_t)row * a.out_row_bytes + ((int64_t)head * D + 4 * d4) * sizeof(T), t);
 }
 
-// Waves and ring slots of a kernel: 128 KiB of LDS, a workgroup on a CU.
+// Waves and ring slots of the waves with positions of their own: 128 KiB of LDS, a workgroup on a CU.
 template <typename Tag, int D>
 struct tlaunch {
   static constexpr int SLOT = tshape<Tag, D>::SLOT;
@@ -653,10 +719,15 @@ struct tlaunch {
 template <typename Tag, int D>
 static void launch_columns(const tree_args& a, int num_work, int blocks, int num_split, hipStream_t stream) {
   using L = tlaunch<Tag, D>;
-  if (blocks == 1)
-    hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 1, L::NW, L::R, L::OCC>), dim3(num_work), dim3(64 * L::NW), 0, stream, a);
-  else
-    hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 2, L::NW, L::R, L::OCC>), dim3(num_work), dim3(64 * L::NW), 0, stream, a);
+  const dim3 grid(num_work), block(64 * L::NW);
+  if (blocks == 1) {
+    hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 1, L::NW, L::R, L::OCC, 1>), grid, block, 0, stream, a);
+  } else if (blocks == 2) {
+    hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 2, L::NW, L::R, L::OCC, 1>), grid, block, 0, stream, a);
+  } else {
+    if constexpr (elem<Tag>::bytes == 2)
+      hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 1, 4, 2, 2, 4>), grid, dim3(256), 0, stream, a);
+  }
   if (num_split > 0)
     hipLaunchKernelGGL((tree_join_kernel<Tag, D>), dim3(num_split, (a.num_heads * (D / 4) + 63) / 64), dim3(64), 0,
                        stream, a);
@@ -738,9 +809,11 @@ extern "C" int32_t tb_build_tree_work(const int32_t* cached, const int32_t* node
     rows += nodes[b];
   }
   TB_CHECK_ARG(rows < (1 << 30));
-  const int blocks = most_cols > 32 ? 2 : 1, cols = 32 * blocks;
-  const int slot_kb = head_dim * (dtype == TB_DTYPE_F32 ? 4 : 2) * 64 / 1024;   // a chunk's K and V rows
+  const bool f32 = dtype == TB_DTYPE_F32;
+  const int blocks = most_cols <= 32 ? 1 : most_cols <= 64 || f32 ? 2 : 4, cols = 32 * blocks;
+  const int slot_kb = head_dim * (f32 ? 4 : 2) * 64 / 1024;   // a chunk's K and V rows
   tree_price price{slot_kb == 8 ? 8 : 4, 4.0, 1.2, 3.3, num_cus};
+  if (blocks == 4) price = {2, 4.0, head_dim == 64 ? 1.0 : 1.6, head_dim == 64 ? 0.65 : 1.1, num_cus};
   const int part = tree_part_rounds(price, cached, nodes, num_seqs, rep, cols, num_kv_heads,
                                     (double)num_heads * (head_dim + 2) * 4) * price.chunks_round;
   std::vector<tree_piece> pieces;
@@ -856,7 +929,8 @@ extern "C" int32_t tb_tree_attention(const void* q, int64_t q_row_stride, const 
     TB_RETURN_LAUNCH_STATUS();
   }
   TB_CHECK_ARG(num_work >= 0 && num_split_rows >= 0 && num_split_rows <= num_rows && partial_slots >= 0);
-  TB_CHECK_ARG((column_blocks == 1 || column_blocks == 2) && (num_split_rows == 0 || partial_slots > 0));
+  TB_CHECK_ARG(column_blocks == 1 || column_blocks == 2 || (column_blocks == 4 && dtype != TB_DTYPE_F32));
+  TB_CHECK_ARG((num_split_rows == 0 || partial_slots > 0));
   if (num_work == 0) return TB_OK;
   TB_CHECK_ARG(work && ((uintptr_t)work & 15u) == 0 && (num_split_rows == 0 || split_rows) &&
                ((uintptr_t)split_rows & 15u) == 0);

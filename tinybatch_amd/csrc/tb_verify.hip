@@ -29,9 +29,10 @@ namespace tb {
 // with the walk, and sums its stretch again; the last launch, one workgroup per sequence, finds
 // the border's stretch, thread and token. A chain, and drafts that were not drawn, need one sum
 // whatever is refused; a tree of drawn drafts one more per refusal that has a sibling
-// behind it: up to MAX_ROUNDS of those in launches of their own, the rest in the last one.
-constexpr int SUM_THREADS = 256, FIND_THREADS = 1024;
-constexpr int MAX_ROUNDS = 3;
+// behind it: up to MAX_ROUNDS of those in launches of their own, the rest in the last one. What
+// a later launch starts from (the state, the nodes' values, the sums) it loads at once.
+constexpr int SUM_THREADS = 256, FIND_THREADS = 512, FIND_CHUNKS = 4;
+constexpr int MAX_ROUNDS = 5;
 constexpr int MAX_STRETCHES = 64;
 constexpr int MAX_STRETCH = 1 << 18;               // tokens whose refused ones are kept as bits in LDS
 
@@ -39,6 +40,8 @@ struct verify_state {
   double a;                    // the refusals' share of q so far (drafts drawn)
   int32_t cur, next, len;      // the reached node, the child to try next, the path's length
   int32_t round;               // the launch whose stretches sum up what is left at `cur`; -1: another test first
+  int32_t row0, n;             // the sequence's rows
+  float u;                     // the root's random number
 };
 
 struct verify_args {
@@ -58,6 +61,7 @@ struct verify_args {
   int32_t stretches;           // workgroups of a sequence
   verify_state* states;        // [launch][B]
   double* sums;                // [launch][B][stretches]
+  int32_t* nodes;              // [B][5][width]: verify_tree's arrays
 };
 
 template <int N>
@@ -96,6 +100,11 @@ __device__ __forceinline__ void load_tree(const verify_args& a, const verify_tre
     t.p[i] = known ? (float)((const T*)a.probs)[(row0 + par) * a.probs_stride + x] : 0.f;
     t.q[i] = known && a.draft ? (float)((const T*)a.draft)[(row0 + par) * a.draft_stride + x] : 0.f;
   }
+}
+// The same from what launch 0 kept; entries past the sequence's nodes hold anything.
+__device__ __forceinline__ void load_tree(const verify_args& a, const verify_tree& t, int seq, bool values) {
+  const int32_t* const from = a.nodes + (int64_t)seq * 5 * a.width;
+  for (int i = threadIdx.x; i < (values ? 5 : 2) * a.width; i += blockDim.x) t.tok[i] = from[i];
 }
 
 // The walk from a state on, by one wave, until the path ends or a sum is needed; `s` is the sum
@@ -244,47 +253,48 @@ __global__ __launch_bounds__(SUM_THREADS) void verify_sum_kernel(const verify_ar
   __shared__ double part[SUM_THREADS / 64];
   __shared__ verify_state shared;
   const int seq = blockIdx.x, g = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int row0 = a.row_starts[seq], n = min(a.row_starts[seq + 1] - row0, a.width);
   int32_t* const acc = a.accepted + (int64_t)seq * a.width;
   int64_t* const out = a.out_tokens + (int64_t)seq * a.width;
-  verify_state st{0., 0, 1, 1, 0};
-  double s = 1.;
-  if (launch > 0) {
-    st = a.states[(int64_t)(launch - 1) * a.num_seqs + seq];
-    if (n > 0 && st.round < 0) {
-      const double* const sums = a.sums + ((int64_t)(launch - 1) * a.num_seqs + seq) * a.stretches;
-      s = sum64(lane < a.stretches ? sums[lane] : 0.);
-    } else {                                       // this sequence's sum is there already
-      if (g == 0 && tid == 0) a.states[(int64_t)launch * a.num_seqs + seq] = st;
-      return;
-    }
-  } else if (g == 0) {
-    for (int i = tid; i < a.width; i += SUM_THREADS) acc[i] = -1, out[i] = -1;
-    if (n <= 0 && tid == 0) {
-      a.states[seq] = st;
-      a.num_accepted[seq] = 0;
-    }
-  }
-  if (n <= 0) return;
   const verify_tree t(lds, a.width);
   int32_t* const path = (int32_t*)(lds + verify_tree::bytes(a.width));
-  load_tree<T>(a, t, row0, n);
+  verify_state st;
+  double s = 1.;
+  if (launch > 0) {
+    const int64_t before = (int64_t)(launch - 1) * a.num_seqs + seq;
+    st = a.states[before];
+    const double x = lane < a.stretches ? a.sums[before * a.stretches + lane] : 0.;
+    load_tree(a, t, seq, true);
+    if (st.n <= 0 || st.round >= 0) {              // this sequence's sum is there already
+      if (g == 0 && tid == 0) a.states[before + a.num_seqs] = st;
+      return;
+    }
+    s = sum64(x);
+  } else {
+    const int row0 = a.row_starts[seq], n = min(a.row_starts[seq + 1] - row0, a.width);
+    st = verify_state{0., 0, 1, 1, 0, row0, n, 0.f};
+    if (n > 0) load_tree<T>(a, t, row0, n);
+    if (g == 0)
+      for (int i = tid; i < a.width; i += SUM_THREADS) acc[i] = -1, out[i] = -1;
+    if (n <= 0) {
+      if (g == 0 && tid == 0) {
+        a.states[seq] = st;
+        a.num_accepted[seq] = 0;
+      }
+      return;
+    }
+  }
   __syncthreads();
-  const int len0 = launch > 0 ? st.len : 0;
+  const int row0 = st.row0, n = st.n, len0 = launch > 0 ? st.len : 0;
   if (wave == 0) {
-    if (launch == 0 && lane == 0) path[0] = 0;
+    if (launch == 0) {
+      st.u = t.u[0];
+      if (lane == 0) path[0] = 0;
+    }
     walk(t, n, a.draft != nullptr, s, st, path, lane, launch);
     if (lane == 0) shared = st;
   }
   __syncthreads();
   st = shared;
-  if (g == 0) {
-    for (int i = len0 + tid; i < st.len; i += SUM_THREADS) {
-      acc[i] = path[i];
-      if (i > 0) out[i - 1] = a.tokens[row0 + path[i]];
-    }
-    if (tid == 0) a.states[(int64_t)launch * a.num_seqs + seq] = st;
-  }
   verify_row<T> row(a, row0 + st.cur, st.a);
   const int b = stretch_begin(row.chunks, a.stretches, g), e = stretch_begin(row.chunks, a.stretches, g + 1);
   if (!a.draft) row.refuse(t, n, st.cur, (uint32_t*)(path + a.width), b, e);
@@ -297,6 +307,15 @@ __global__ __launch_bounds__(SUM_THREADS) void verify_sum_kernel(const verify_ar
     for (int k = 0; k < SUM_THREADS / 64; ++k) w += part[k];
     a.sums[((int64_t)launch * a.num_seqs + seq) * a.stretches + g] = w;
   }
+  if (g == 0) {
+    for (int i = len0 + tid; i < st.len; i += SUM_THREADS) {
+      acc[i] = path[i];
+      if (i > 0) out[i - 1] = a.tokens[row0 + path[i]];
+    }
+    if (tid == 0) a.states[(int64_t)launch * a.num_seqs + seq] = st;
+    if (launch == 0)
+      for (int i = tid; i < 5 * a.width; i += SUM_THREADS) a.nodes[(int64_t)seq * 5 * a.width + i] = t.tok[i];
+  }
 }
 
 // The last launch: the walk's rest where more sums are needed than there were launches, and the token.
@@ -308,19 +327,24 @@ __global__ __launch_bounds__(FIND_THREADS) void verify_find_kernel(const verify_
   __shared__ verify_state shared;
   __shared__ int32_t first, last, token;
   const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int row0 = a.row_starts[seq], n = min(a.row_starts[seq + 1] - row0, a.width);
-  if (n <= 0) return;
   int32_t* const acc = a.accepted + (int64_t)seq * a.width;
   int64_t* const out = a.out_tokens + (int64_t)seq * a.width;
   verify_state st = a.states[(int64_t)(launches - 1) * a.num_seqs + seq];
   const verify_tree t(lds, a.width);
   int32_t* const path = (int32_t*)(lds + verify_tree::bytes(a.width));
   uint32_t* const bits = (uint32_t*)(path + a.width);
+  // the sums: of launch 0 where there was no other, else where the state says
+  double sum = lane < a.stretches ? a.sums[(int64_t)seq * a.stretches + lane] : 0.;
+  if (!a.draft) load_tree(a, t, seq, false);
+  if (st.n <= 0) return;
+  const int row0 = st.row0, n = st.n;
   const bool pending = st.round < 0;
-  if (pending || !a.draft) {
-    load_tree<T>(a, t, row0, n);
-    __syncthreads();
+  if (launches > 1) {
+    const int r = pending ? launches - 1 : st.round;
+    sum = lane < a.stretches ? a.sums[((int64_t)r * a.num_seqs + seq) * a.stretches + lane] : 0.;
+    if (pending) load_tree(a, t, seq, true);
   }
+  __syncthreads();
   auto total = [&](double x) -> double {           // over the workgroup
     x = sum64(x);
     __syncthreads();
@@ -352,7 +376,7 @@ __global__ __launch_bounds__(FIND_THREADS) void verify_find_kernel(const verify_
 
   if (pending) {
     // the rest of the walk by this workgroup alone
-    double s = sum64(lane < a.stretches ? a.sums[((int64_t)(launches - 1) * a.num_seqs + seq) * a.stretches + lane] : 0.);
+    double s = sum64(sum);
     const int len0 = st.len;
     for (;;) {
       if (wave == 0) {
@@ -373,12 +397,11 @@ __global__ __launch_bounds__(FIND_THREADS) void verify_find_kernel(const verify_
   }
 
   verify_row<T> row(a, row0 + st.cur, st.a);
-  const double u = (double)a.uniforms[row0];
+  const double u = (double)st.u;
   int b = 0, e = row.chunks;
   double before = 0., border = 0., w;
   if (!pending) {                                  // the stretch, from its launch's sums
-    const double x = lane < a.stretches ? a.sums[((int64_t)st.round * a.num_seqs + seq) * a.stretches + lane] : 0.;
-    const double run = scan64<64>(x, lane);
+    const double x = sum, run = scan64<64>(x, lane);
     w = __shfl(run, 63);
     border = u * w;
     const uint64_t some = __ballot(x > 0.), past = __ballot(x > 0. && run > border);
@@ -401,7 +424,7 @@ __global__ __launch_bounds__(FIND_THREADS) void verify_find_kernel(const verify_
   int next = -1;
   if (w > 0.) {
     // by waves of neighbouring chunks, until a thread has a few neighbouring chunks of its own
-    while (e - b > FIND_THREADS * 4) {
+    while (e - b > FIND_THREADS * FIND_CHUNKS) {
       const int step = (e - b + NW - 1) / NW, wb = min(e, b + wave * step), we = min(e, wb + step);
       const double x = sum64(row.share(wb, we, lane, 64));
       const int at = pick(lane == 0 ? x : 0., border, before) >> 6;
@@ -410,22 +433,27 @@ __global__ __launch_bounds__(FIND_THREADS) void verify_find_kernel(const verify_
     }
     const int step = (e - b + FIND_THREADS - 1) / FIND_THREADS;
     const int tb = min(e, b + tid * step), te = min(e, tb + step);
-    double x = 0.;
-    for (int c = tb; c < te; ++c) x += row.sum(row.load(c), c);
-    const int at = pick(x, border, before);
+    typename verify_row<T>::chunk x[FIND_CHUNKS];
+#pragma unroll
+    for (int k = 0; k < FIND_CHUNKS; ++k) x[k] = row.load(min(tb + k, row.chunks - 1));
+    double mine = 0.;
+#pragma unroll
+    for (int k = 0; k < FIND_CHUNKS; ++k) mine += tb + k < te ? row.sum(x[k], tb + k) : 0.;
+    const int at = pick(mine, border, before);
     if (tid == at) {
       int found = -1;
       double run = before;
-      for (int c = tb; c < te; ++c) {
-        const auto k = row.load(c);
-        const bool edge = c == 0 || c == row.chunks - 1;
+#pragma unroll
+      for (int k = 0; k < FIND_CHUNKS; ++k)
+#pragma unroll
         for (int j = 0; j < E; ++j) {
-          const double y = row.weight(k, c, j, edge);
-          if (!(y > 0.) || (found >= 0 && run > border)) continue;
-          run += y;
-          found = c * E - row.shift + j;           // the last one so far; the first that passes stays
+          const int c = tb + k;
+          const double y = c < te ? row.weight(x[k], c, j, true) : 0.;
+          if (y > 0. && (found < 0 || !(run > border))) {
+            run += y;
+            found = c * E - row.shift + j;         // the last one so far; the first that passes stays
+          }
         }
-      }
       token = found;
     }
     __syncthreads();
@@ -524,11 +552,11 @@ __global__ __launch_bounds__(256) void commit_kernel(char* storage, int64_t laye
 
 }  // namespace tb
 
-extern "C" size_t tb_tree_verify_workspace_bytes(int32_t num_seqs, int32_t vocab) {
+extern "C" size_t tb_tree_verify_workspace_bytes(int32_t num_seqs, int32_t vocab, int32_t width) {
   using namespace tb;
-  if (num_seqs <= 0 || vocab <= 0) return 0;
-  return (size_t)(MAX_ROUNDS + 1) * num_seqs *
-         (sizeof(verify_state) + sizeof(double) * verify_stretches(num_seqs, vocab));
+  if (num_seqs <= 0 || vocab <= 0 || width <= 0) return 0;
+  return (size_t)num_seqs * ((MAX_ROUNDS + 1) * (sizeof(verify_state) + sizeof(double) * verify_stretches(num_seqs, vocab)) +
+                             verify_tree::bytes(width));
 }
 
 extern "C" int32_t tb_tree_verify(const void* probs, int64_t probs_row_stride, const void* draft_probs,
@@ -545,14 +573,15 @@ extern "C" int32_t tb_tree_verify(const void* probs, int64_t probs_row_stride, c
   TB_CHECK_ARG(probs && tokens && uniforms && parents && row_starts && accepted && num_accepted && out_tokens);
   TB_CHECK_ARG(probs_row_stride >= vocab && (!draft_probs || draft_row_stride >= vocab));
   TB_CHECK_ARG(workspace && ((uintptr_t)workspace & 7u) == 0 &&
-               workspace_bytes >= tb_tree_verify_workspace_bytes(num_seqs, vocab));
+               workspace_bytes >= tb_tree_verify_workspace_bytes(num_seqs, vocab, width));
   const int stretches = verify_stretches(num_seqs, vocab);
   // sums that tests of later siblings need: none in a chain, or where the drafts were not drawn
   const int rounds = draft_probs ? std::min(std::max(max_children - 1, 0), MAX_ROUNDS) : 0;
   verify_state* const states = (verify_state*)workspace;
+  double* const sums = (double*)(states + (size_t)(MAX_ROUNDS + 1) * num_seqs);
   const verify_args a{probs, probs_row_stride, draft_probs, draft_row_stride, vocab, tokens, uniforms, parents,
                       row_starts, accepted, num_accepted, out_tokens, width, num_seqs, stretches, states,
-                      (double*)(states + (size_t)(MAX_ROUNDS + 1) * num_seqs)};
+                      sums, (int32_t*)(sums + (size_t)(MAX_ROUNDS + 1) * num_seqs * stretches)};
   if (dtype == TB_DTYPE_F32) launch_verify<float>(a, rounds, stream);
   else if (dtype == TB_DTYPE_F16) launch_verify<_Float16>(a, rounds, stream);
   else launch_verify<__bf16>(a, rounds, stream);

@@ -370,7 +370,7 @@ def verify_tree(meta: TreeMetadata, tokens: torch.Tensor, uniforms: torch.Tensor
     _node_values("uniforms", uniforms, torch.float32, T, device)
     v = _verdict(meta, device)
     L = _lib.lib()
-    ws = torch.empty(L.tb_tree_verify_workspace_bytes(meta.num_seqs, vocab), device=device, dtype=torch.uint8)
+    ws = torch.empty(L.tb_tree_verify_workspace_bytes(meta.num_seqs, vocab, v.accepted.shape[1]), device=device, dtype=torch.uint8)
     if T == 0:
         return v._replace(accepted=v.accepted.fill_(-1), num_accepted=v.num_accepted.zero_(), tokens=v.tokens.fill_(-1))
     with _on(device):
