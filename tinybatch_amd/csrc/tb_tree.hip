@@ -11,11 +11,12 @@
 // Work: the n nodes and the rep query heads of a kv head make n * rep columns, column =
 // node * rep + head, that read the same K/V rows whatever their masks. A workgroup takes
 // consecutive columns of a (sequence, kv head) and a part of the context.
-// - Up to 64 columns (32 CB): its waves take the part's chunks of 32 positions in turn, each
-//   through a ring of its own in LDS filled by direct global->LDS loads, with no barrier between
-//   them, and join their softmax states in LDS at the end.
-// - More, in 16 bits: 128 columns, 32 for each of four waves, which share the chunks: 64 positions
-//   through a ring of two, one barrier each, so that a K or V row loaded meets 128 columns.
+// - tree_columns_kernel, up to 64 columns (32 CB), fp32 any number: its waves take the part's chunks
+//   of 32 positions in turn, each through a ring of its own in LDS filled by direct global->LDS
+//   loads, with no barrier between them, and join their softmax states in LDS at the end.
+// - tree_shared_kernel, more in 16 bits: 128 columns, 32 for each of four waves, which share chunks
+//   of 64 positions through a ring of two, one barrier each, so that a K or V row loaded meets
+//   128 columns.
 // A context cut into parts leaves a partial per part, joined by a second launch.
 //
 // Math per chunk and block of 32 columns (C rows are positions or dims, C columns the block's):
@@ -28,6 +29,7 @@
 // a few times per context.
 #include <algorithm>
 #include <exception>
+#include <type_traits>
 #include <vector>
 
 #include "tb_stream.h"
@@ -186,20 +188,112 @@ struct tshape {
   }
 };
 
-// CW = 1: every wave all 32 CB columns and positions of its own; CW = NW: 32 columns a wave (CB = 1).
-template <typename Tag, int D, int CB, int NW, int R, int OCC, int CW>
+// The seen positions p0 .. p0 + 31 of a node (p0 a multiple of 32): the cached ones and its mask's bits.
+__device__ __forceinline__ uint32_t tree_seen(const uint32_t* mask, int words, int cached, int limit, int p0) {
+  const int off = p0 - cached, w = off >> 5;       // nodes off .. off + 31
+  const uint32_t lo = w < 0 ? ~0u : w < words ? mask[w] : 0u;
+  const uint32_t hi = w + 1 < 0 ? ~0u : w + 1 < words ? mask[w + 1] : 0u;
+  const uint32_t seen = __builtin_amdgcn_alignbit(hi, lo, off & 31);
+  return limit - p0 >= 32 ? seen : limit > p0 ? seen & ((1u << (limit - p0)) - 1) : 0u;
+}
+// The scores of unseen positions to -inf: register r holds position 8 (r / 4) + 4 half + r % 4.
+__device__ __forceinline__ void tree_hide(float16_t& sc, uint32_t seen, int half) {
+  const uint32_t mine = seen >> (4 * half);
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    if (!(mine & (1u << (8 * (r >> 2) + (r & 3))))) sc[r] = -INFINITY;
+}
+// Whether BYTES of V rows in LDS (a wave's reads) hold no infinity or NaN.
+template <typename T, int BYTES>
+__device__ __forceinline__ bool tree_finite(const char* v, int lane) {
+  constexpr bool F32 = sizeof(T) == 4;
+  constexpr uint32_t E = F32 ? 0x7F800000u : __is_same(T, _Float16) ? 0x7C00u : 0x7F80u;
+  bool ok = true;
+  for (int i = 0; i < BYTES / 1024; ++i) {
+    const vec16 x = ld16(v + 1024 * i + 16 * lane);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      ok &= (x.w[j] & E) != E;
+      if (!F32) ok &= ((x.w[j] >> 16) & E) != E;
+    }
+  }
+  return __all(ok);
+}
+// O^T += V^T.P of 32 positions one by one, the unseen ones left out: a weight of 0 times an infinity is
+// no 0. p(r): this lane's weight of register r.
+template <typename Tag, int D, typename P>
+__device__ __forceinline__ void tree_values_apart(float16_t (&acc)[D / 32], const char* v, uint32_t seen, int half,
+                                                  P&& p) {
+  using S = tshape<Tag, D>;
+  using T = typename elem<Tag>::type;
+  constexpr bool F32 = S::EB == 4;
+#pragma unroll 1
+  for (int pos = 0; pos < 32; ++pos) {
+    const int reg = 4 * (pos >> 3) + (pos & 3);
+    float mine = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mine = r == reg ? p(r) : mine;
+    const float other = __shfl_xor(mine, 32);
+    const float w = half == ((pos >> 2) & 1) ? mine : other;
+    if ((seen >> pos) & 1) {
+#pragma unroll
+      for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {           // dims 32 b + 8 g + 4 half ..
+          const char* const vp =
+              v + pos * S::RB + (F32 ? 128 * b + 32 * g + 16 * half : 16 * ((4 * b + g) ^ S::vswz(pos)) + 8 * half);
+          T e[4];
+          __builtin_memcpy(e, __builtin_assume_aligned(vp, 8), 4 * sizeof(T));
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[b][4 * g + j] = fmaf(w, (float)e[j], acc[b][4 * g + j]);
+        }
+    }
+  }
+}
+// Element i of a packed 16-bit operand.
+template <typename T>
+__device__ __forceinline__ float tree_unpack(su32x4_t x, int i) {
+  T e[2];
+  const uint32_t word = x[i >> 1];
+  __builtin_memcpy(e, &word, 4);
+  return (float)e[i & 1];
+}
+// q of a column rotated (RoPE at the node's position), its sign, complete on return.
+template <typename Tag, int D, int QS>
+__device__ __forceinline__ void tree_q(vec16 (&q)[QS], const tree_args& a, int row, int half) {
+  using T = typename elem<Tag>::type;
+  constexpr int E = 16 / sizeof(T);
+  if (a.rope.cos) {
+    const int64_t r = a.rope.row(a.positions[row], D / 2) + E * half;
+#pragma unroll
+    for (int s = 0; s < QS / 2; ++s)            // pieces s and s + QS/2 pair (dims i and i + D/2)
+      rope_pair<T>(q[s], q[s + QS / 2], a.rope.cos + r + 2 * E * s, a.rope.sin + r + 2 * E * s);
+  }
+  if (a.q_sign != 1.f) {
+#pragma unroll
+    for (int s = 0; s < QS; ++s) {
+      T x[E];
+      __builtin_memcpy(x, &q[s], 16);
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = (T)((float)x[e] * a.q_sign);
+      __builtin_memcpy(&q[s], x, 16);
+    }
+  }
+#pragma unroll
+  for (int s = 0; s < QS; ++s)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(q[s].w[i]));
+}
+
+template <typename Tag, int D, int CB, int NW, int R, int OCC>
 __global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
 void tree_columns_kernel(const tree_args a) {
   using S = tshape<Tag, D>;
   using T = typename elem<Tag>::type;
   constexpr int RB = S::RB, CK = S::CK, NB = S::NB, QS = S::QS, LD = S::LD;
   constexpr bool F32 = S::EB == 4;
-  constexpr bool SHARED = CW > 1;
-  constexpr int SUB = SHARED ? 2 : 1;           // chunks of 32 positions in a ring slot
-  constexpr int HALF = SUB * S::HALF, SLOT = 2 * HALF;
-  constexpr int MERGE = SHARED ? 0 : NW * 64 * (16 * NB + 2) * 4, RINGS = SHARED ? 1 : NW;
-  constexpr int LDS = RINGS * R * SLOT > MERGE ? RINGS * R * SLOT : MERGE;
-  static_assert(!SHARED || (CB == 1 && CW == NW && NW == 2 * SUB && R == 2 && !F32), "wave w loads tile w of a slot");
+  constexpr int MERGE = NW * 64 * (16 * NB + 2) * 4;
+  constexpr int LDS = NW * R * S::SLOT > MERGE ? NW * R * S::SLOT : MERGE;
   __shared__ __align__(1024) char lds_all[LDS];
 
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -207,9 +301,9 @@ void tree_columns_kernel(const tree_args a) {
   const int4 w0 = a.work[3 * blockIdx.x], w1 = a.work[3 * blockIdx.x + 1], w2 = a.work[3 * blockIdx.x + 2];
   const int row0 = w0.x, seq = w0.y, cached = w0.z, nodes = w0.w;
   if (nodes == 0) return;                       // a padding entry (whole workgroup)
-  const int col0 = w1.x + (SHARED ? 32 * wave : 0), kvh = w1.y, chunk0 = w1.z, chunks = w1.w;
+  const int col0 = w1.x, kvh = w1.y, chunk0 = w1.z, chunks = w1.w;
   const int limit = cached + nodes, ncols = nodes * a.rep;
-  char* const lds = lds_all + (SHARED ? 0 : wave * (R * SLOT));
+  char* const lds = lds_all + wave * (R * S::SLOT);
 
   // this lane's columns: node my_row, head hd (past the last column: a repeat, not stored)
   int my_row[CB], hd[CB];
@@ -228,8 +322,7 @@ void tree_columns_kernel(const tree_args a) {
     for (int s = 0; s < QS; ++s) q[cb][s] = ld16(qrow + 32 * s);
   }
 
-  // ---- direct loads: the wave's k-th chunk is chunk0 + wave + NW k; shared: the k-th slot holds chunks
-  // chunk0 + 2 k and the next, of which this wave loads 16 positions ----
+  // ---- direct loads: the wave's k-th chunk is chunk0 + wave + NW k ----
   const int64_t head_bytes = ((int64_t)1 << a.log2_bs) * RB;
   const int64_t blk_bytes = 2 * (int64_t)a.num_kv_heads * head_bytes, v_off = a.num_kv_heads * head_bytes;
   const int sub_mask = (1 << (a.log2_bs - 4)) - 1;                // 16-position tiles per block - 1
@@ -237,72 +330,45 @@ void tree_columns_kernel(const tree_args a) {
   const char* const pool_kvh = a.pool + kvh * head_bytes;
   const int last_tile = (limit - 1) >> 4;
   const int lrow = lane / S::PPR, lpiece = lane % S::PPR;
-  const int n = SHARED ? (chunks + SUB - 1) / SUB : (chunks - wave + NW - 1) / NW;   // its slots (<= 0: none)
-  constexpr int TILES = SHARED ? 1 : 2, IDS = 64 / TILES;         // tiles it loads of a slot; slots whose ids fit
-  auto tile_of = [&](int k, int t) {
-    return min(SHARED ? 2 * chunk0 + NW * k + wave : 2 * (chunk0 + wave + NW * k) + t, last_tile);
-  };
+  const int n = (chunks - wave + NW - 1) / NW;                    // this wave's chunks (<= 0: none)
   int id0 = 0;
-  auto load_ids = [&](int k) {                  // lane j: the block of tile j % TILES of slot k + j / TILES
-    const int t = tile_of(k + lane / TILES, lane % TILES);
+  auto load_ids = [&](int k) {                  // lane j: the block of tile j % 2 of chunk k + j / 2
+    const int t = min(2 * (chunk0 + wave + NW * (k + (lane >> 1))) + (lane & 1), last_tile);
     const int b = table[(t << 4) >> a.log2_bs];
     return (b < 0 || b >= a.num_blocks) ? 0 : b;   // host validates; stay inside the pool
   };
   int ids = load_ids(0);
   asm volatile("" : "+v"(ids));                 // the block ids have landed: no wait inside the loop
   auto issue = [&](int k, bool is_v) {
-    if (k - id0 >= IDS) {                       // uniform, once per 32 or 64 slots
+    if (k - id0 >= 32) {                        // uniform, once per 32 chunks
       id0 = k;
       ids = load_ids(k);
     }
+    const int c = chunk0 + wave + NW * k;
+    char* const dst = lds + (k % R) * S::SLOT + (is_v ? S::HALF : 0);
 #pragma unroll
-    for (int t = 0; t < TILES; ++t) {
-      const int tile = tile_of(k, t), at = SHARED ? wave : t;     // its place in the slot
+    for (int t = 0; t < 2; ++t) {
+      const int tile = min(2 * c + t, last_tile);
       const int rmax = limit - 1 - 16 * tile;   // rows past it repeat the last position
-      const int64_t b = __builtin_amdgcn_readlane(ids, TILES * (k - id0) + t);
+      const int64_t b = __builtin_amdgcn_readlane(ids, 2 * (k - id0) + t);
       const char* const base = pool_kvh + b * blk_bytes + (int64_t)(tile & sub_mask) * S::TB + (is_v ? v_off : 0);
-      char* const dst = lds + (k % R) * SLOT + (is_v ? HALF : 0) + at * S::TB;
 #pragma unroll
       for (int i = 0; i < LD / 2; ++i) {
         const int r = S::RPL * i + lrow;
-        s_dma16_l2((uint32_t)(min(r, rmax) * RB + 16 * (lpiece ^ (is_v ? S::vswz(r) : S::kswz(r)))), base,
-                   dst + i * 1024);
+        s_dma16_l2((uint32_t)(min(r, rmax) * RB + 16 * (lpiece ^ (is_v ? S::vswz(r) : S::kswz(16 * t + r)))), base,
+                   dst + (t * (LD / 2) + i) * 1024);
       }
     }
   };
 #pragma unroll
-  for (int k = 0; k < (SHARED ? 1 : R); ++k)
+  for (int k = 0; k < R; ++k)
     if (k < n) {
       issue(k, false);
       issue(k, true);
     }
 
-  // ---- q rotated (RoPE at the node's position), its sign, complete here ----
 #pragma unroll
-  for (int cb = 0; cb < CB; ++cb) {
-    if (a.rope.cos) {
-      constexpr int E = 16 / S::EB;             // elements of a piece
-      const int64_t r = a.rope.row(a.positions[row0 + my_row[cb]], D / 2) + E * half;
-#pragma unroll
-      for (int s = 0; s < QS / 2; ++s)          // pieces s and s + QS/2 pair (dims i and i + D/2)
-        rope_pair<T>(q[cb][s], q[cb][s + QS / 2], a.rope.cos + r + 2 * E * s, a.rope.sin + r + 2 * E * s);
-    }
-    if (a.q_sign != 1.f) {
-#pragma unroll
-      for (int s = 0; s < QS; ++s) {
-        constexpr int E = 16 / S::EB;
-        T x[E];
-        __builtin_memcpy(x, &q[cb][s], 16);
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[e] = (T)((float)x[e] * a.q_sign);
-        __builtin_memcpy(&q[cb][s], x, 16);
-      }
-    }
-#pragma unroll
-    for (int s = 0; s < QS; ++s)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(q[cb][s].w[i]));
-  }
+  for (int cb = 0; cb < CB; ++cb) tree_q<Tag, D>(q[cb], a, row0 + my_row[cb], half);
 
   uint32_t ones = 0;                            // in a register: as a literal the bf16 dot product read it wrong
   if constexpr (!F32) ones = cmath<Tag>::ONES;
@@ -326,8 +392,8 @@ void tree_columns_kernel(const tree_args a) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       const int c = 4 * b + 2 * ((lane >> 4) & 1) + ((li & 3) >> 1);
-      va[b] = F32 ? (uint32_t)(HALF + 4 * half * RB + 128 * b + 4 * lcol)
-                  : (uint32_t)(HALF + rv * RB + 16 * (c ^ S::vswz(rv)) + 8 * (li & 1));
+      va[b] = F32 ? (uint32_t)(S::HALF + 4 * half * RB + 128 * b + 4 * lcol)
+                  : (uint32_t)(S::HALF + rv * RB + 16 * (c ^ S::vswz(rv)) + 8 * (li & 1));
     }
   }
   const float sl2e = a.scale_log2e;
@@ -380,22 +446,12 @@ void tree_columns_kernel(const tree_args a) {
     }
   };
   // the online softmax of chunk c: sc -> P, and the state's rescale
-  auto softmax = [&](int c, bool masked) {
+  auto softmax = [&](int c, auto masked) {
 #pragma unroll
     for (int cb = 0; cb < CB; ++cb) {
-      if (masked) {                             // kept a branch: most chunks lie in the cache
-        asm volatile("");
-        // the mask's bits from node 32 c - cached on; those before node 0 are cached positions
-        const uint32_t* const mrow = a.mask + (int64_t)(row0 + my_row[cb]) * a.mask_words;
-        const int off = CK * c - cached, w = off >> 5;
-        const uint32_t lo = w < 0 ? ~0u : w < a.mask_words ? mrow[w] : 0u;
-        const uint32_t hi = w + 1 < a.mask_words ? mrow[w + 1] : 0u;
-        vis[cb] = __builtin_amdgcn_alignbit(hi, lo, off & 31);
-        if (limit - CK * c < 32) vis[cb] &= (1u << (limit - CK * c)) - 1;
-        const uint32_t mine = vis[cb] >> (4 * half);
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (!(mine & (1u << (8 * (r >> 2) + (r & 3))))) sc[cb][r] = -INFINITY;
+      if constexpr (masked.value) {
+        vis[cb] = tree_seen(a.mask + (int64_t)(row0 + my_row[cb]) * a.mask_words, a.mask_words, cached, limit, CK * c);
+        tree_hide(sc[cb], vis[cb], half);
       }
       float cm = max_f32(sc[cb][0], sc[cb][1]);
 #pragma unroll
@@ -467,138 +523,46 @@ void tree_columns_kernel(const tree_args a) {
         }
     }
   };
-  // a masked chunk whose V rows hold an infinity or NaN: position by position, the unseen ones left
-  // out (a weight of 0 times an infinity is no 0)
-  auto values_finite = [&](const char* base) {
-    bool ok = true;
-    for (int i = 0; i < S::HALF / 1024; ++i) {
-      const vec16 v = ld16(base + HALF + 1024 * i + 16 * lane);
-      constexpr uint32_t E1 = F32 ? 0x7F800000u : sizeof(T) == 2 && __is_same(T, _Float16) ? 0x7C00u : 0x7F80u;
+  // Loads of chunk k + R's K follow chunk k's scores, its V's chunk k's products. Outstanding when
+  // chunk k's K (or V) must be there: the halves issued behind it.
+  auto step = [&](int k, auto masked) {
+    const int c = chunk0 + wave + NW * k;
+    const char* const base = lds + (k % R) * S::SLOT;
+    const int ahead = min(R - 1, n - 1 - k);    // chunks issued behind chunk k
+    if (ahead == R - 1) s_vm_wait_le(LD * (1 + 2 * (R - 1)));
+    else s_vm_wait_le(LD * (1 + 2 * ahead));
+    scores(base);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the K rows are in registers: their slot is free
+    const bool more = k + R < n;
+    if (more) issue(k + R, false);
+    softmax(c, masked);
+    if (more) s_vm_wait_le(LD * (1 + 2 * (R - 1)));
+    else s_vm_wait_le(LD * 2 * ahead);
+    bool plain = true;
+    if constexpr (masked.value) {
+      plain = tree_finite<T, S::HALF>(base + S::HALF, lane);
+      if (!plain) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        ok &= (v.w[j] & E1) != E1;
-        if (!F32) ok &= ((v.w[j] >> 16) & E1) != E1;
+        for (int cb = 0; cb < CB; ++cb)
+          tree_values_apart<Tag, D>(acc[cb], base + S::HALF, vis[cb], half, [&](int r) {
+            if constexpr (F32) return sc[cb][r];
+            else return tree_unpack<T>(pb[cb][r >> 3], r & 7);
+          });
       }
     }
-    return __all(ok);
+    if (plain) values(base);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    if (more) issue(k + R, true);
   };
-  auto values_apart = [&](const char* base) {
-#pragma unroll 1
-    for (int pos = 0; pos < CK; ++pos) {
-      const int reg = 4 * (pos >> 3) + (pos & 3);
-      const bool here = half == ((pos >> 2) & 1);
-#pragma unroll
-      for (int cb = 0; cb < CB; ++cb) {
-        float p = 0.f;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float x;
-          if constexpr (F32) x = sc[cb][r];
-          else {
-            T e[2];
-            const uint32_t word = pb[cb][r >> 3][(r & 7) >> 1];
-            __builtin_memcpy(e, &word, 4);
-            x = (float)e[r & 1];
-          }
-          p = r == reg ? x : p;
-        }
-        const float other = __shfl_xor(p, 32);
-        p = here ? p : other;
-        if ((vis[cb] >> pos) & 1) {
-#pragma unroll
-          for (int b = 0; b < NB; ++b)
-#pragma unroll
-            for (int g = 0; g < 4; ++g) {       // dims 32 b + 8 g + 4 half ..
-              const char* const vp = base + HALF + pos * RB +
-                                     (F32 ? 128 * b + 32 * g + 16 * half : 16 * ((4 * b + g) ^ S::vswz(pos)) + 8 * half);
-              T e[4];
-              __builtin_memcpy(e, __builtin_assume_aligned(vp, 8), 4 * sizeof(T));
-#pragma unroll
-              for (int j = 0; j < 4; ++j) acc[cb][b][4 * g + j] = fmaf(p, (float)e[j], acc[cb][b][4 * g + j]);
-            }
-        }
-      }
-    }
-  };
+  // the chunks that lie in the cache whole, then those with nodes: two loops, so that the mask costs the
+  // long one neither instructions nor registers
+  const int inside = cached / CK - 1 - chunk0 - wave;
+  const int plain = inside < 0 ? 0 : min(n, inside / NW + 1);
+  int k = 0;
+  for (; k < plain; ++k) step(k, std::false_type{});
+  for (; k < n; ++k) step(k, std::true_type{});
 
-  auto chunk_values = [&](const char* base, bool masked) {
-    if (masked && !values_finite(base)) values_apart(base);
-    else values(base);
-  };
-  if constexpr (SHARED) {
-    const bool busy = col0 < ncols;
-    for (int k = 0; k < n; ++k) {
-      // the wave's loads of slot k have landed and its reads of slot k - 1 are done: behind the barrier
-      // all of slot k is in LDS and the other one is free
-      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (k + 1 < n) {
-        issue(k + 1, false);
-        issue(k + 1, true);
-      }
-#pragma unroll 1
-      for (int t = 0; t < SUB; ++t) {
-        const int c = chunk0 + SUB * k + t;
-        if (!busy || c >= chunk0 + chunks) break;
-        const char* const base = lds + (k % R) * SLOT + t * S::HALF;
-        const bool masked = CK * c + CK > cached;
-        scores(base);
-        softmax(c, masked);
-        chunk_values(base, masked);
-      }
-    }
-  } else {
-    // Loads of chunk k + R's K follow chunk k's scores, its V's chunk k's products. Outstanding when
-    // chunk k's K (or V) must be there: the halves issued behind it.
-    for (int k = 0; k < n; ++k) {
-      const int c = chunk0 + wave + NW * k;
-      const char* const base = lds + (k % R) * SLOT;
-      const int ahead = min(R - 1, n - 1 - k);    // chunks issued behind chunk k
-      if (ahead == R - 1) s_vm_wait_le(LD * (1 + 2 * (R - 1)));
-      else s_vm_wait_le(LD * (1 + 2 * ahead));
-      scores(base);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the K rows are in registers: their slot is free
-      const bool more = k + R < n;
-      if (more) issue(k + R, false);
-      const bool masked = CK * c + CK > cached;
-      softmax(c, masked);
-      if (more) s_vm_wait_le(LD * (1 + 2 * (R - 1)));
-      else s_vm_wait_le(LD * 2 * ahead);
-      chunk_values(base, masked);
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      if (more) issue(k + R, true);
-    }
-  }
-
-  if constexpr (SHARED) {                       // a wave's columns are its own
-    const float L = sum_xor32(l[0]);
-    const int slot = w2.x, row = row0 + my_row[0];
-    if (col0 + lcol >= ncols) return;
-    float inv = 1.f;
-    if (slot < 0) {
-      inv = 1.f / L;
-      if (!(L > 0.f) && !tree_sees(a.mask + (int64_t)row * a.mask_words, cached, nodes)) inv = 0.f;
-    }
-    typedef T t4_t __attribute__((ext_vector_type(4)));
-    const int64_t at = (int64_t)(slot + my_row[0]) * a.num_heads + hd[0];
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {             // dims 32 b + 8 g + 4 half ..
-        const float4_t o = {acc[0][b][4 * g], acc[0][b][4 * g + 1], acc[0][b][4 * g + 2], acc[0][b][4 * g + 3]};
-        if (slot < 0) {
-          t4_t t;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) t[j] = (T)(o[j] * inv);
-          st_through(a.out + (int64_t)row * a.out_row_bytes + (int64_t)hd[0] * RB + (32 * b + 8 * g + 4 * half) * S::EB, t);
-        } else {
-          *reinterpret_cast<float4_t*>(a.ws_acc + at * D + 32 * b + 8 * g + 4 * half) = o;
-        }
-      }
-    if (slot >= 0 && half == 0) *reinterpret_cast<float2*>(a.ws_ml + at * 2) = make_float2(m[0], L);
-    return;
-  }
   // ---- the waves' states joined; wave w stores the 4-dim groups w, w + NW, ... of a column ----
-  if constexpr (!SHARED) {
   const int slot = w2.x;                        // < 0: the whole context, the output itself
 #pragma unroll
   for (int cb = 0; cb < CB; ++cb) {
@@ -653,7 +617,225 @@ void tree_columns_kernel(const tree_args a) {
       }
     }
   }
+}
+
+// 128 columns, 32 a wave; the four waves share chunks of 64 positions, of which wave w loads tile w.
+template <typename Tag, int D>
+__global__ __launch_bounds__(256, 2) void tree_shared_kernel(const tree_args a) {
+  using S = tshape<Tag, D>;
+  using M = cmath<Tag>;
+  using T = typename elem<Tag>::type;
+  constexpr int RB = S::RB, NB = S::NB, QS = S::QS, NW = 4, CK = 64, HALF = CK * RB, SLOT = 2 * HALF;
+  __shared__ __align__(1024) char lds[2 * SLOT];
+
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, lcol = lane & 31, half = lane >> 5;
+  const int4 w0 = a.work[3 * blockIdx.x], w1 = a.work[3 * blockIdx.x + 1], w2 = a.work[3 * blockIdx.x + 2];
+  const int row0 = w0.x, seq = w0.y, cached = w0.z, nodes = w0.w;
+  if (nodes == 0) return;                       // a padding entry (whole workgroup)
+  const int col0 = w1.x + 32 * wave, kvh = w1.y, chunk0 = w1.z, chunks = w1.w;   // chunks of 32, chunk0 even
+  const int limit = cached + nodes, ncols = nodes * a.rep;
+  const int col = min(col0 + lcol, ncols - 1), my_row = col / a.rep, hd = kvh * a.rep + col - my_row * a.rep;
+
+  vec16 q[QS];
+  {
+    const char* const qrow = a.q + (int64_t)(row0 + my_row) * a.q_row_bytes + (int64_t)hd * RB + 16 * half;
+#pragma unroll
+    for (int s = 0; s < QS; ++s) q[s] = ld16(qrow + 32 * s);
   }
+  // ---- direct loads ----
+  const int64_t head_bytes = ((int64_t)1 << a.log2_bs) * RB;
+  const int64_t blk_bytes = 2 * (int64_t)a.num_kv_heads * head_bytes, v_off = a.num_kv_heads * head_bytes;
+  const int sub_mask = (1 << (a.log2_bs - 4)) - 1;
+  const int32_t* const table = a.block_tables + (int64_t)seq * a.max_nb;
+  const char* const pool_kvh = a.pool + kvh * head_bytes;
+  const int last_tile = (limit - 1) >> 4, tile0 = 2 * chunk0 + wave;
+  const int lrow = lane / S::PPR, lpiece = lane % S::PPR;
+  const int n = (chunks + 1) / 2;
+  int id0 = 0;
+  auto load_ids = [&](int k) {                  // lane j: the block of this wave's tile in slot k + j
+    const int b = table[(min(tile0 + NW * (k + lane), last_tile) << 4) >> a.log2_bs];
+    return (b < 0 || b >= a.num_blocks) ? 0 : b;   // host validates; stay inside the pool
+  };
+  int ids = load_ids(0);
+  asm volatile("" : "+v"(ids));                 // the block ids have landed: no wait inside the loop
+  auto issue = [&](int k) {
+    if (k - id0 >= 64) {                        // uniform, once per 64 slots
+      id0 = k;
+      ids = load_ids(k);
+    }
+    const int tile = min(tile0 + NW * k, last_tile), rmax = limit - 1 - 16 * tile;   // rows past it repeat the last position
+    const int64_t b = __builtin_amdgcn_readlane(ids, k - id0);
+    const char* const base = pool_kvh + b * blk_bytes + (int64_t)(tile & sub_mask) * S::TB;
+    char* const dst = lds + (k & 1) * SLOT + wave * S::TB;
+#pragma unroll
+    for (int i = 0; i < S::TB / 1024; ++i) {
+      const int r = S::RPL * i + lrow;
+      const uint32_t row = (uint32_t)(min(r, rmax) * RB);
+      s_dma16_l2(row + 16 * (lpiece ^ S::kswz(r)), base, dst + 1024 * i);
+      s_dma16_l2(row + 16 * (lpiece ^ S::vswz(r)), base + v_off, dst + HALF + 1024 * i);
+    }
+  };
+  issue(0);
+  tree_q<Tag, D>(q, a, row0 + my_row, half);
+
+  uint32_t ones = M::ONES;                      // in a register: as a literal the bf16 dot product read it wrong
+  asm volatile("" : "+v"(ones));
+  float m = -INFINITY, l = 0.f;
+  float16_t acc[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[b][r] = 0.f;
+  uint32_t ka[QS], va[NB];
+#pragma unroll
+  for (int s = 0; s < QS; ++s) ka[s] = (uint32_t)(lcol * RB + 16 * ((2 * s + half) ^ S::kswz(lcol)));
+  {
+    const int li = lane & 15, rv = 4 * half + (li >> 2);
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const int c = 4 * b + 2 * ((lane >> 4) & 1) + ((li & 3) >> 1);
+      va[b] = (uint32_t)(HALF + rv * RB + 16 * (c ^ S::vswz(rv)) + 8 * (li & 1));
+    }
+  }
+  const float sl2e = a.scale_log2e;
+  const bool busy = col0 < ncols;
+  auto step = [&](int k, auto masked) {
+    // the wave's loads of slot k have landed and its reads of slot k - 1 are done: behind the barrier
+    // all of slot k is in LDS and the other one is free
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (k + 1 < n) issue(k + 1);
+    if (!busy) return;
+    const char* const base = lds + (k & 1) * SLOT;
+    const int p0 = 32 * chunk0 + CK * k;
+    // ---- scores: two chains of products, operands read KG slices ahead of them ----
+    float16_t sc[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sc[t][r] = 0.f;
+    {
+      constexpr int KG = 2;
+      su32x4_t kf[2][KG][2];
+      auto read = [&](int g) {
+#pragma unroll
+        for (int i = 0; i < KG; ++i)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            kf[g & 1][i][t] = *reinterpret_cast<const su32x4_t*>(base + ka[KG * g + i] + 32 * t * RB);
+      };
+      read(0);
+#pragma unroll
+      for (int g = 0; g < QS / KG; ++g) {
+        if (g + 1 < QS / KG) read(g + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < KG; ++i)
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            sc[t] = M::mfma(kf[g & 1][i][t], __builtin_bit_cast(su32x4_t, q[KG * g + i]), sc[t]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    // ---- online softmax ----
+    uint32_t seen[2];
+    if constexpr (masked.value) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        seen[t] = tree_seen(a.mask + (int64_t)(row0 + my_row) * a.mask_words, a.mask_words, cached, limit, p0 + 32 * t);
+        tree_hide(sc[t], seen[t], half);
+      }
+    }
+    float cm = max_f32(sc[0][0], sc[0][1]);
+#pragma unroll
+    for (int e = 2; e < 32; e += 2) cm = max3_f32(cm, sc[e >> 4][e & 15], sc[e >> 4][(e & 15) + 1]);
+    cm *= sl2e;
+    if (__any(cm > m + 8.f)) {
+      const float m_new = fmaxf(m, max_xor32(cm));
+      const float alpha = fast_exp2(m - (m_new == -INFINITY ? 0.f : m_new));   // 0 while m = -inf
+      m = m_new;
+      l *= alpha;
+#pragma unroll
+      for (int b = 0; b < NB; ++b) acc[b] *= alpha;
+    }
+    const float neg_m = m == -INFINITY ? 0.f : -m;
+    su32x4_t pb[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      float p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) p[j] = fast_exp2(fmaf(sc[w >> 1][8 * (w & 1) + j], sl2e, neg_m));
+      pb[w] = smath<Tag>::pack8(p);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) l = M::add2(pb[w][j], ones, l);   // of the rounded P that multiplies V
+    }
+    // ---- values ----
+    bool plain = true;
+    if constexpr (masked.value) {
+      plain = tree_finite<T, HALF>(base + HALF, lane);
+      if (!plain) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          tree_values_apart<Tag, D>(acc, base + HALF + 32 * t * RB, seen[t], half,
+                                    [&](int r) { return tree_unpack<T>(pb[2 * t + (r >> 3)], r & 7); });
+      }
+    }
+    if (plain) {
+      uint2 vf[2][NB][2];
+      auto read = [&](int w) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const char* const vp = base + va[b] + 16 * w * RB;
+          vf[w & 1][b][0] = lds_read_tr16(vp);
+          vf[w & 1][b][1] = lds_read_tr16(vp + 8 * RB);
+        }
+      };
+      read(0);
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        if (w + 1 < 4) read(w + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const uint2 lo = vf[w & 1][b][0], hi = vf[w & 1][b][1];
+          acc[b] = M::mfma(su32x4_t{lo.x, lo.y, hi.x, hi.y}, pb[w], acc[b]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  };
+  // the slots that lie in the cache whole, then those with nodes: two loops, so that the mask costs the
+  // long one neither instructions nor registers
+  const int plain = max(0, min(n, (cached - 32 * chunk0) / CK));
+  int k = 0;
+  for (; k < plain; ++k) step(k, std::false_type{});
+  for (; k < n; ++k) step(k, std::true_type{});
+
+  l = sum_xor32(l);
+  if (col0 + lcol >= ncols) return;
+  const int slot = w2.x, row = row0 + my_row;   // slot < 0: the whole context, the output itself
+  float inv = 1.f;
+  if (slot < 0) {
+    inv = 1.f / l;
+    if (!(l > 0.f) && !tree_sees(a.mask + (int64_t)row * a.mask_words, cached, nodes)) inv = 0.f;
+  }
+  typedef T t4_t __attribute__((ext_vector_type(4)));
+  const int64_t at = (int64_t)(slot + my_row) * a.num_heads + hd;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {               // dims 32 b + 8 g + 4 half ..
+      const float4_t o = {acc[b][4 * g], acc[b][4 * g + 1], acc[b][4 * g + 2], acc[b][4 * g + 3]};
+      if (slot < 0) {
+        t4_t t;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t[j] = (T)(o[j] * inv);
+        st_through(a.out + (int64_t)row * a.out_row_bytes + (int64_t)hd * RB + (32 * b + 8 * g + 4 * half) * S::EB, t);
+      } else {
+        *reinterpret_cast<float4_t*>(a.ws_acc + at * D + 32 * b + 8 * g + 4 * half) = o;
+      }
+    }
+  if (slot >= 0 && half == 0) *reinterpret_cast<float2*>(a.ws_ml + at * 2) = make_float2(m, l);
 }
 
 // The partials of a row's parts joined: thread = 4 dims of a head.
@@ -721,12 +903,12 @@ static void launch_columns(const tree_args& a, int num_work, int blocks, int num
   using L = tlaunch<Tag, D>;
   const dim3 grid(num_work), block(64 * L::NW);
   if (blocks == 1) {
-    hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 1, L::NW, L::R, L::OCC, 1>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 1, L::NW, L::R, L::OCC>), grid, block, 0, stream, a);
   } else if (blocks == 2) {
-    hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 2, L::NW, L::R, L::OCC, 1>), grid, block, 0, stream, a);
+    hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 2, L::NW, L::R, L::OCC>), grid, block, 0, stream, a);
   } else {
     if constexpr (elem<Tag>::bytes == 2)
-      hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 1, 4, 2, 2, 4>), grid, dim3(256), 0, stream, a);
+      hipLaunchKernelGGL((tree_shared_kernel<Tag, D>), grid, dim3(256), 0, stream, a);
   }
   if (num_split > 0)
     hipLaunchKernelGGL((tree_join_kernel<Tag, D>), dim3(num_split, (a.num_heads * (D / 4) + 63) / 64), dim3(64), 0,
