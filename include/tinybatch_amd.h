@@ -710,7 +710,7 @@ int32_t tb_tree_attention(const void* q, int64_t q_row_stride, const void* pool,
  * counts [4]: work entries (12 int32 each), split rows (4 int32 each), partial slots, column
  * blocks per workgroup. work and split NULL: the counts alone. An entry is (first row, sequence,
  * cached, nodes, first column, kv head, first chunk of 32 positions, chunks, partial slot of node 0
- * or -1, 0, 0, 0), with 0 nodes for a padding entry; entry g is meant for XCD g % num_xcds. */
+ * or -1, whether no other entry reads its K/V rows, 0, 0), with 0 nodes for a padding entry; entry g is meant for XCD g % num_xcds. */
 int32_t tb_build_tree_work(const int32_t* cached, const int32_t* nodes, int32_t num_seqs,
                            int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
                            int32_t num_cus, int32_t num_xcds, int32_t* work, int32_t work_capacity,

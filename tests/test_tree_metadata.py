@@ -170,10 +170,11 @@ def test_work_covers_every_context_once(hq, hkv, d, dtype, sizes, cached):
     cols, rep = 32 * m.column_blocks, hq // hkv
     assert m.work_np.shape[0] % 8 == 0
     seen, slots, where = {}, {}, {}
-    for g, (row0, seq, c, n, col0, kvh, chunk0, chunks, slot, *zero) in enumerate(m.work_np.tolist()):
-        assert zero == [0, 0, 0]
+    for g, (row0, seq, c, n, col0, kvh, chunk0, chunks, slot, once, *zero) in enumerate(m.work_np.tolist()):
+        assert zero == [0, 0]
         if n == 0:
             continue
+        assert once == (n * rep <= cols)
         assert (row0, c, n) == (m.row_starts_np[seq], cached[seq], sizes[seq]) and chunks > 0
         seen.setdefault((seq, kvh, col0), []).extend(range(chunk0, chunk0 + chunks))
         slots.setdefault(seq, {})[chunk0] = slot

@@ -9,15 +9,13 @@
 // What a node does not see has no effect on it, also where it is infinite or NaN.
 //
 // Work: the n nodes and the rep query heads of a kv head make n * rep columns, column =
-// node * rep + head, that read the same K/V rows whatever their masks. A workgroup takes
-// consecutive columns of a (sequence, kv head) and a part of the context.
-// - tree_columns_kernel, up to 64 columns (32 CB), fp32 any number: its waves take the part's chunks
-//   of 32 positions in turn, each through a ring of its own in LDS filled by direct global->LDS
-//   loads, with no barrier between them, and join their softmax states in LDS at the end.
-// - tree_shared_kernel, more in 16 bits: 128 columns, 32 for each of four waves, which share chunks
-//   of 64 positions through a ring of two, one barrier each, so that a K or V row loaded meets
-//   128 columns.
-// A context cut into parts leaves a partial per part, joined by a second launch.
+// node * rep + head, that read the same K/V rows whatever their masks. A workgroup of four
+// waves takes 32 CW consecutive columns of a (sequence, kv head) and a part of the context, which
+// it walks in chunks of CK positions through a ring of two in LDS: every wave loads a quarter of
+// the next chunk (direct global->LDS loads) and computes on the present one, one barrier between.
+// A wave holds 32 columns; with CW < 4 several waves hold the same ones, each a part of a
+// chunk's positions, and join their softmax states in LDS at the end. A context cut into parts
+// leaves a partial per part, joined by a second launch.
 //
 // Math per chunk and block of 32 columns (C rows are positions or dims, C columns the block's):
 //   S^T[pos][col] = K[pos][:] . q[col][:]        A = K rows from LDS, B = q in registers
@@ -285,355 +283,29 @@ __device__ __forceinline__ void tree_q(vec16 (&q)[QS], const tree_args& a, int r
     for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(q[s].w[i]));
 }
 
-template <typename Tag, int D, int CB, int NW, int R, int OCC>
-__global__ __launch_bounds__(64 * NW) __attribute__((amdgpu_waves_per_eu(OCC, OCC)))
-void tree_columns_kernel(const tree_args a) {
+// 32 CW columns: the four waves share chunks of CK positions, of which each loads a quarter. CW of them take
+// 32 columns each, 4 / CW the same columns, each a part of a chunk's positions, joined at the end.
+template <typename Tag, int D, int CW, int CK>
+__global__ __launch_bounds__(256, D * elem<Tag>::bytes * CK < 32768 ? 2 : 1) void tree_columns_kernel(const tree_args a) {
   using S = tshape<Tag, D>;
-  using T = typename elem<Tag>::type;
-  constexpr int RB = S::RB, CK = S::CK, NB = S::NB, QS = S::QS, LD = S::LD;
   constexpr bool F32 = S::EB == 4;
-  constexpr int MERGE = NW * 64 * (16 * NB + 2) * 4;
-  constexpr int LDS = NW * R * S::SLOT > MERGE ? NW * R * S::SLOT : MERGE;
-  __shared__ __align__(1024) char lds_all[LDS];
-
-  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63, lcol = lane & 31, half = lane >> 5;
-  const int4 w0 = a.work[3 * blockIdx.x], w1 = a.work[3 * blockIdx.x + 1], w2 = a.work[3 * blockIdx.x + 2];
-  const int row0 = w0.x, seq = w0.y, cached = w0.z, nodes = w0.w;
-  if (nodes == 0) return;                       // a padding entry (whole workgroup)
-  const int col0 = w1.x, kvh = w1.y, chunk0 = w1.z, chunks = w1.w;
-  const int limit = cached + nodes, ncols = nodes * a.rep;
-  char* const lds = lds_all + wave * (R * S::SLOT);
-
-  // this lane's columns: node my_row, head hd (past the last column: a repeat, not stored)
-  int my_row[CB], hd[CB];
-#pragma unroll
-  for (int cb = 0; cb < CB; ++cb) {
-    const int col = min(col0 + 32 * cb + lcol, ncols - 1);
-    my_row[cb] = col / a.rep;
-    hd[cb] = kvh * a.rep + col - my_row[cb] * a.rep;
-  }
-  // ---- q (B operand: dims 8 half .. of every 16 in 16 bits, 4 half .. of every 8 in fp32) ----
-  vec16 q[CB][QS];
-#pragma unroll
-  for (int cb = 0; cb < CB; ++cb) {
-    const char* const qrow = a.q + (int64_t)(row0 + my_row[cb]) * a.q_row_bytes + (int64_t)hd[cb] * RB + 16 * half;
-#pragma unroll
-    for (int s = 0; s < QS; ++s) q[cb][s] = ld16(qrow + 32 * s);
-  }
-
-  // ---- direct loads: the wave's k-th chunk is chunk0 + wave + NW k ----
-  const int64_t head_bytes = ((int64_t)1 << a.log2_bs) * RB;
-  const int64_t blk_bytes = 2 * (int64_t)a.num_kv_heads * head_bytes, v_off = a.num_kv_heads * head_bytes;
-  const int sub_mask = (1 << (a.log2_bs - 4)) - 1;                // 16-position tiles per block - 1
-  const int32_t* const table = a.block_tables + (int64_t)seq * a.max_nb;
-  const char* const pool_kvh = a.pool + kvh * head_bytes;
-  const int last_tile = (limit - 1) >> 4;
-  const int lrow = lane / S::PPR, lpiece = lane % S::PPR;
-  const int n = (chunks - wave + NW - 1) / NW;                    // this wave's chunks (<= 0: none)
-  int id0 = 0;
-  auto load_ids = [&](int k) {                  // lane j: the block of tile j % 2 of chunk k + j / 2
-    const int t = min(2 * (chunk0 + wave + NW * (k + (lane >> 1))) + (lane & 1), last_tile);
-    const int b = table[(t << 4) >> a.log2_bs];
-    return (b < 0 || b >= a.num_blocks) ? 0 : b;   // host validates; stay inside the pool
-  };
-  int ids = load_ids(0);
-  asm volatile("" : "+v"(ids));                 // the block ids have landed: no wait inside the loop
-  auto issue = [&](int k, bool is_v) {
-    if (k - id0 >= 32) {                        // uniform, once per 32 chunks
-      id0 = k;
-      ids = load_ids(k);
-    }
-    const int c = chunk0 + wave + NW * k;
-    char* const dst = lds + (k % R) * S::SLOT + (is_v ? S::HALF : 0);
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const int tile = min(2 * c + t, last_tile);
-      const int rmax = limit - 1 - 16 * tile;   // rows past it repeat the last position
-      const int64_t b = __builtin_amdgcn_readlane(ids, 2 * (k - id0) + t);
-      const char* const base = pool_kvh + b * blk_bytes + (int64_t)(tile & sub_mask) * S::TB + (is_v ? v_off : 0);
-#pragma unroll
-      for (int i = 0; i < LD / 2; ++i) {
-        const int r = S::RPL * i + lrow;
-        s_dma16_l2((uint32_t)(min(r, rmax) * RB + 16 * (lpiece ^ (is_v ? S::vswz(r) : S::kswz(16 * t + r)))), base,
-                   dst + (t * (LD / 2) + i) * 1024);
-      }
-    }
-  };
-#pragma unroll
-  for (int k = 0; k < R; ++k)
-    if (k < n) {
-      issue(k, false);
-      issue(k, true);
-    }
-
-#pragma unroll
-  for (int cb = 0; cb < CB; ++cb) tree_q<Tag, D>(q[cb], a, row0 + my_row[cb], half);
-
-  uint32_t ones = 0;                            // in a register: as a literal the bf16 dot product read it wrong
-  if constexpr (!F32) ones = cmath<Tag>::ONES;
-  asm volatile("" : "+v"(ones));
-  float m[CB], l[CB];                           // reference max (scaled, base 2), this lane's share of the sum
-  float16_t acc[CB][NB];                        // O^T[32 b + 8 (r / 4) + 4 half + r % 4][col]
-#pragma unroll
-  for (int cb = 0; cb < CB; ++cb) {
-    m[cb] = -INFINITY, l[cb] = 0.f;
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[cb][b][r] = 0.f;
-  }
-  // operand addresses of this lane in a slot
-  uint32_t ka[QS], va[NB];
-#pragma unroll
-  for (int s = 0; s < QS; ++s) ka[s] = (uint32_t)(lcol * RB + 16 * ((2 * s + half) ^ S::kswz(lcol)));
-  {
-    const int li = lane & 15, rv = 4 * half + (li >> 2);
-#pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int c = 4 * b + 2 * ((lane >> 4) & 1) + ((li & 3) >> 1);
-      va[b] = F32 ? (uint32_t)(S::HALF + 4 * half * RB + 128 * b + 4 * lcol)
-                  : (uint32_t)(S::HALF + rv * RB + 16 * (c ^ S::vswz(rv)) + 8 * (li & 1));
-    }
-  }
-  const float sl2e = a.scale_log2e;
-
-  float16_t sc[CB];                             // S^T, then P: positions 8 (r / 4) + 4 half + r % 4 of a chunk
-  su32x4_t pb[CB][2];                           // 16-bit P: B operands of 16 positions each
-  uint32_t vis[CB];                             // a masked chunk's seen positions
-  auto scores = [&](const char* base) {
-    if constexpr (!F32) {
-#pragma unroll
-      for (int cb = 0; cb < CB; ++cb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sc[cb][r] = 0.f;
-      constexpr int KG = 4;                     // operands read KG ahead of their products
-      su32x4_t kf[2][KG];
-      auto read = [&](int g) {
-#pragma unroll
-        for (int i = 0; i < KG; ++i) kf[g & 1][i] = *reinterpret_cast<const su32x4_t*>(base + ka[KG * g + i]);
-      };
-      read(0);
-#pragma unroll
-      for (int g = 0; g < QS / KG; ++g) {
-        if (g + 1 < QS / KG) read(g + 1);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int i = 0; i < KG; ++i)
-#pragma unroll
-          for (int cb = 0; cb < CB; ++cb)
-            sc[cb] = cmath<Tag>::mfma(kf[g & 1][i], __builtin_bit_cast(su32x4_t, q[cb][KG * g + i]), sc[cb]);
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    } else {
-      float16_t d[CB][2];
-#pragma unroll
-      for (int cb = 0; cb < CB; ++cb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) d[cb][0][r] = d[cb][1][r] = 0.f;
-#pragma unroll
-      for (int s = 0; s < QS; ++s) {
-        const vec16 kv = ld16(base + ka[s]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int cb = 0; cb < CB; ++cb)
-            d[cb][i & 1] = __builtin_amdgcn_mfma_f32_32x32x2f32(bits_to_f32(kv.w[i]), bits_to_f32(q[cb][s].w[i]),
-                                                                d[cb][i & 1], 0, 0, 0);
-      }
-#pragma unroll
-      for (int cb = 0; cb < CB; ++cb) sc[cb] = d[cb][0] + d[cb][1];
-    }
-  };
-  // the online softmax of chunk c: sc -> P, and the state's rescale
-  auto softmax = [&](int c, auto masked) {
-#pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-      if constexpr (masked.value) {
-        vis[cb] = tree_seen(a.mask + (int64_t)(row0 + my_row[cb]) * a.mask_words, a.mask_words, cached, limit, CK * c);
-        tree_hide(sc[cb], vis[cb], half);
-      }
-      float cm = max_f32(sc[cb][0], sc[cb][1]);
-#pragma unroll
-      for (int e = 2; e < 16; e += 2) cm = max3_f32(cm, sc[cb][e], sc[cb][e + 1]);
-      cm *= sl2e;
-      if (__any(cm > m[cb] + 8.f)) {
-        const float m_new = fmaxf(m[cb], max_xor32(cm));
-        const float alpha = fast_exp2(m[cb] - (m_new == -INFINITY ? 0.f : m_new));   // 0 while m = -inf
-        m[cb] = m_new;
-        l[cb] *= alpha;
-#pragma unroll
-        for (int b = 0; b < NB; ++b) acc[cb][b] *= alpha;
-      }
-      const float neg_m = m[cb] == -INFINITY ? 0.f : -m[cb];
-#pragma unroll
-      for (int r = 0; r < 16; ++r) sc[cb][r] = fast_exp2(fmaf(sc[cb][r], sl2e, neg_m));
-      if constexpr (!F32) {
-#pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          float p[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j) p[j] = sc[cb][8 * w + j];
-          pb[cb][w] = smath<Tag>::pack8(p);
-#pragma unroll
-          for (int j = 0; j < 4; ++j) l[cb] = cmath<Tag>::add2(pb[cb][w][j], ones, l[cb]);   // of the rounded P
-        }
-      } else {
-        const float16_t& p = sc[cb];
-        l[cb] += (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]))) +
-                 (((p[8] + p[9]) + (p[10] + p[11])) + ((p[12] + p[13]) + (p[14] + p[15])));
-      }
-    }
-  };
-  // O^T += V^T.P of the chunk in a slot
-  auto values = [&](const char* base) {
-    if constexpr (!F32) {
-      uint2 vf[2][NB][2];
-      auto read = [&](int w) {
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const char* const vp = base + va[b] + 16 * w * RB;
-          vf[w][b][0] = lds_read_tr16(vp);
-          vf[w][b][1] = lds_read_tr16(vp + 8 * RB);
-        }
-      };
-      read(0);
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        if (w == 0) read(1);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const uint2 lo = vf[w][b][0], hi = vf[w][b][1];
-#pragma unroll
-          for (int cb = 0; cb < CB; ++cb)
-            acc[cb][b] = cmath<Tag>::mfma(su32x4_t{lo.x, lo.y, hi.x, hi.y}, pb[cb][w], acc[cb][b]);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
-    } else {
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-#pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const float v = *reinterpret_cast<const float*>(base + va[b] + (8 * (r >> 2) + (r & 3)) * RB);
-#pragma unroll
-          for (int cb = 0; cb < CB; ++cb)
-            acc[cb][b] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, sc[cb][r], acc[cb][b], 0, 0, 0);
-        }
-    }
-  };
-  // Loads of chunk k + R's K follow chunk k's scores, its V's chunk k's products. Outstanding when
-  // chunk k's K (or V) must be there: the halves issued behind it.
-  auto step = [&](int k, auto masked) {
-    const int c = chunk0 + wave + NW * k;
-    const char* const base = lds + (k % R) * S::SLOT;
-    const int ahead = min(R - 1, n - 1 - k);    // chunks issued behind chunk k
-    if (ahead == R - 1) s_vm_wait_le(LD * (1 + 2 * (R - 1)));
-    else s_vm_wait_le(LD * (1 + 2 * ahead));
-    scores(base);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");   // the K rows are in registers: their slot is free
-    const bool more = k + R < n;
-    if (more) issue(k + R, false);
-    softmax(c, masked);
-    if (more) s_vm_wait_le(LD * (1 + 2 * (R - 1)));
-    else s_vm_wait_le(LD * 2 * ahead);
-    bool plain = true;
-    if constexpr (masked.value) {
-      plain = tree_finite<T, S::HALF>(base + S::HALF, lane);
-      if (!plain) {
-#pragma unroll
-        for (int cb = 0; cb < CB; ++cb)
-          tree_values_apart<Tag, D>(acc[cb], base + S::HALF, vis[cb], half, [&](int r) {
-            if constexpr (F32) return sc[cb][r];
-            else return tree_unpack<T>(pb[cb][r >> 3], r & 7);
-          });
-      }
-    }
-    if (plain) values(base);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    if (more) issue(k + R, true);
-  };
-  // the chunks that lie in the cache whole, then those with nodes: two loops, so that the mask costs the
-  // long one neither instructions nor registers
-  const int inside = cached / CK - 1 - chunk0 - wave;
-  const int plain = inside < 0 ? 0 : min(n, inside / NW + 1);
-  int k = 0;
-  for (; k < plain; ++k) step(k, std::false_type{});
-  for (; k < n; ++k) step(k, std::true_type{});
-
-  // ---- the waves' states joined; wave w stores the 4-dim groups w, w + NW, ... of a column ----
-  const int slot = w2.x;                        // < 0: the whole context, the output itself
-#pragma unroll
-  for (int cb = 0; cb < CB; ++cb) {
-    l[cb] = sum_xor32(l[cb]);
-    __syncthreads();
-    float* const mine = reinterpret_cast<float*>(lds_all) + wave * (64 * (16 * NB + 2)) + lane;
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mine[64 * (16 * b + r)] = acc[cb][b][r];
-    mine[64 * 16 * NB] = m[cb];
-    mine[64 * (16 * NB + 1)] = l[cb];
-    __syncthreads();
-    const float* const all = reinterpret_cast<const float*>(lds_all) + lane;
-    constexpr int WS = 64 * (16 * NB + 2);
-    float mw[NW], M = -INFINITY, L = 0.f;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      mw[w] = all[w * WS + 64 * 16 * NB];
-      M = fmaxf(M, mw[w]);
-    }
-    const float M_safe = M == -INFINITY ? 0.f : M;
-#pragma unroll
-    for (int w = 0; w < NW; ++w) {
-      mw[w] = fast_exp2(mw[w] - M_safe);         // 0 for a wave that saw nothing
-      L += all[w * WS + 64 * (16 * NB + 1)] * mw[w];
-    }
-    if (col0 + 32 * cb + lcol >= ncols) continue;
-    const int row = row0 + my_row[cb];
-    float inv = 1.f;
-    if (slot < 0) {
-      inv = 1.f / L;
-      if (!(L > 0.f) && !tree_sees(a.mask + (int64_t)row * a.mask_words, cached, nodes)) inv = 0.f;
-    }
-    for (int g = wave; g < 4 * NB; g += NW) {   // dims 8 g + 4 half ..
-      float4_t o = float4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < NW; ++w) {
-        const float* const src = all + w * WS + 64 * 4 * g;
-        o += float4_t{src[0], src[64], src[128], src[192]} * mw[w];
-      }
-      if (slot < 0) {
-        typedef T t4_t __attribute__((ext_vector_type(4)));
-        t4_t t;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) t[j] = (T)(o[j] * inv);
-        st_through(a.out + (int64_t)row * a.out_row_bytes + (int64_t)hd[cb] * RB + (8 * g + 4 * half) * S::EB, t);
-      } else {
-        const int64_t at = (int64_t)(slot + my_row[cb]) * a.num_heads + hd[cb];
-        *reinterpret_cast<float4_t*>(a.ws_acc + at * D + 8 * g + 4 * half) = o;
-        if (g == 0 && half == 0) *reinterpret_cast<float2*>(a.ws_ml + at * 2) = make_float2(M, L);
-      }
-    }
-  }
-}
-
-// 128 columns, 32 a wave; the four waves share chunks of 64 positions, of which wave w loads tile w.
-template <typename Tag, int D>
-__global__ __launch_bounds__(256, 2) void tree_shared_kernel(const tree_args a) {
-  using S = tshape<Tag, D>;
-  using M = cmath<Tag>;
   using T = typename elem<Tag>::type;
-  constexpr int RB = S::RB, NB = S::NB, QS = S::QS, NW = 4, CK = 64, HALF = CK * RB, SLOT = 2 * HALF;
-  __shared__ __align__(1024) char lds[2 * SLOT];
+  constexpr int RB = S::RB, NB = S::NB, QS = S::QS, NW = 4, HALF = CK * RB, SLOT = 2 * HALF;
+  constexpr int SETS = NW / CW, TL = CK / 32 / SETS;   // waves on a column; 32-position tiles a wave takes of a chunk
+  constexpr int TILES = CK / 64;                // 16-position tiles a wave loads of a chunk
+  constexpr int WS = 64 * (16 * NB + 2);        // floats of a wave's state
+  constexpr int LDS = SETS > 1 && NW * WS * 4 > 2 * SLOT ? NW * WS * 4 : 2 * SLOT;
+  static_assert(TL >= 1 && TILES >= 1, "a tile for every wave");
+  __shared__ __align__(1024) char lds[LDS];
 
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int lane = threadIdx.x & 63, lcol = lane & 31, half = lane >> 5;
   const int4 w0 = a.work[3 * blockIdx.x], w1 = a.work[3 * blockIdx.x + 1], w2 = a.work[3 * blockIdx.x + 2];
   const int row0 = w0.x, seq = w0.y, cached = w0.z, nodes = w0.w;
   if (nodes == 0) return;                       // a padding entry (whole workgroup)
-  const int col0 = w1.x + 32 * wave, kvh = w1.y, chunk0 = w1.z, chunks = w1.w;   // chunks of 32, chunk0 even
+  const int set = wave / CW;                    // its tiles start at position 32 TL set of a chunk
+  const bool once = w2.y;                       // no other workgroup reads these K/V rows
+  const int col0 = w1.x + 32 * (wave % CW), kvh = w1.y, chunk0 = w1.z, chunks = w1.w;   // chunks of 32, chunk0 even
   const int limit = cached + nodes, ncols = nodes * a.rep;
   const int col = min(col0 + lcol, ncols - 1), my_row = col / a.rep, hd = kvh * a.rep + col - my_row * a.rep;
 
@@ -649,37 +321,48 @@ __global__ __launch_bounds__(256, 2) void tree_shared_kernel(const tree_args a) 
   const int sub_mask = (1 << (a.log2_bs - 4)) - 1;
   const int32_t* const table = a.block_tables + (int64_t)seq * a.max_nb;
   const char* const pool_kvh = a.pool + kvh * head_bytes;
-  const int last_tile = (limit - 1) >> 4, tile0 = 2 * chunk0 + wave;
+  const int last_tile = (limit - 1) >> 4, tile0 = 2 * chunk0 + TILES * wave;
   const int lrow = lane / S::PPR, lpiece = lane % S::PPR;
-  const int n = (chunks + 1) / 2;
+  const int n = (32 * chunks + CK - 1) / CK;
   int id0 = 0;
-  auto load_ids = [&](int k) {                  // lane j: the block of this wave's tile in slot k + j
-    const int b = table[(min(tile0 + NW * (k + lane), last_tile) << 4) >> a.log2_bs];
+  auto tile_of = [&](int k, int t) { return min(tile0 + CK / 16 * k + t, last_tile); };
+  auto load_ids = [&](int k) {                  // lane j: the block of tile j % TILES of slot k + j / TILES
+    const int b = table[(tile_of(k + lane / TILES, lane % TILES) << 4) >> a.log2_bs];
     return (b < 0 || b >= a.num_blocks) ? 0 : b;   // host validates; stay inside the pool
   };
   int ids = load_ids(0);
   asm volatile("" : "+v"(ids));                 // the block ids have landed: no wait inside the loop
   auto issue = [&](int k) {
-    if (k - id0 >= 64) {                        // uniform, once per 64 slots
+    if (k - id0 >= 64 / TILES) {                // uniform, once per 64 or 32 slots
       id0 = k;
       ids = load_ids(k);
     }
-    const int tile = min(tile0 + NW * k, last_tile), rmax = limit - 1 - 16 * tile;   // rows past it repeat the last position
-    const int64_t b = __builtin_amdgcn_readlane(ids, k - id0);
-    const char* const base = pool_kvh + b * blk_bytes + (int64_t)(tile & sub_mask) * S::TB;
-    char* const dst = lds + (k & 1) * SLOT + wave * S::TB;
 #pragma unroll
-    for (int i = 0; i < S::TB / 1024; ++i) {
-      const int r = S::RPL * i + lrow;
-      const uint32_t row = (uint32_t)(min(r, rmax) * RB);
-      s_dma16_l2(row + 16 * (lpiece ^ S::kswz(r)), base, dst + 1024 * i);
-      s_dma16_l2(row + 16 * (lpiece ^ S::vswz(r)), base + v_off, dst + HALF + 1024 * i);
+    for (int t = 0; t < TILES; ++t) {
+      const int tile = tile_of(k, t), rmax = limit - 1 - 16 * tile;   // rows past it repeat the last position
+      const int64_t b = __builtin_amdgcn_readlane(ids, TILES * (k - id0) + t);
+      const char* const base = pool_kvh + b * blk_bytes + (int64_t)(tile & sub_mask) * S::TB;
+      char* const dst = lds + (k & 1) * SLOT + (TILES * wave + t) * S::TB;
+#pragma unroll
+      for (int i = 0; i < S::TB / 1024; ++i) {
+        const int r = S::RPL * i + lrow;
+        const uint32_t row = (uint32_t)(min(r, rmax) * RB);
+        const uint32_t ko = row + 16 * (lpiece ^ S::kswz(r)), vo = row + 16 * (lpiece ^ S::vswz(r));
+        if (once) {
+          s_dma16_s(ko, base, dst + 1024 * i);
+          s_dma16_s(vo, base + v_off, dst + HALF + 1024 * i);
+        } else {
+          s_dma16_l2(ko, base, dst + 1024 * i);
+          s_dma16_l2(vo, base + v_off, dst + HALF + 1024 * i);
+        }
+      }
     }
   };
   issue(0);
   tree_q<Tag, D>(q, a, row0 + my_row, half);
 
-  uint32_t ones = M::ONES;                      // in a register: as a literal the bf16 dot product read it wrong
+  uint32_t ones = 0;                            // in a register: as a literal the bf16 dot product read it wrong
+  if constexpr (!F32) ones = cmath<Tag>::ONES;
   asm volatile("" : "+v"(ones));
   float m = -INFINITY, l = 0.f;
   float16_t acc[NB];
@@ -695,7 +378,8 @@ __global__ __launch_bounds__(256, 2) void tree_shared_kernel(const tree_args a) 
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       const int c = 4 * b + 2 * ((lane >> 4) & 1) + ((li & 3) >> 1);
-      va[b] = (uint32_t)(HALF + rv * RB + 16 * (c ^ S::vswz(rv)) + 8 * (li & 1));
+      va[b] = F32 ? (uint32_t)(HALF + 4 * half * RB + 128 * b + 4 * lcol)
+                  : (uint32_t)(HALF + rv * RB + 16 * (c ^ S::vswz(rv)) + 8 * (li & 1));
     }
   }
   const float sl2e = a.scale_log2e;
@@ -706,22 +390,22 @@ __global__ __launch_bounds__(256, 2) void tree_shared_kernel(const tree_args a) 
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     if (k + 1 < n) issue(k + 1);
     if (!busy) return;
-    const char* const base = lds + (k & 1) * SLOT;
-    const int p0 = 32 * chunk0 + CK * k;
-    // ---- scores: two chains of products, operands read KG slices ahead of them ----
-    float16_t sc[2];
+    const char* const base = lds + (k & 1) * SLOT + set * (32 * TL * RB);
+    const int p0 = 32 * chunk0 + CK * k + 32 * TL * set;
+    // ---- scores: operands read KG pieces ahead of their products ----
+    float16_t sc[TL];
+    if constexpr (!F32) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < TL; ++t)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sc[t][r] = 0.f;
-    {
-      constexpr int KG = 2;
-      su32x4_t kf[2][KG][2];
+        for (int r = 0; r < 16; ++r) sc[t][r] = 0.f;
+      constexpr int KG = 4 / TL;
+      su32x4_t kf[2][KG][TL];
       auto read = [&](int g) {
 #pragma unroll
         for (int i = 0; i < KG; ++i)
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
+          for (int t = 0; t < TL; ++t)
             kf[g & 1][i][t] = *reinterpret_cast<const su32x4_t*>(base + ka[KG * g + i] + 32 * t * RB);
       };
       read(0);
@@ -732,23 +416,49 @@ __global__ __launch_bounds__(256, 2) void tree_shared_kernel(const tree_args a) 
 #pragma unroll
         for (int i = 0; i < KG; ++i)
 #pragma unroll
-          for (int t = 0; t < 2; ++t)
-            sc[t] = M::mfma(kf[g & 1][i][t], __builtin_bit_cast(su32x4_t, q[KG * g + i]), sc[t]);
+          for (int t = 0; t < TL; ++t)
+            sc[t] = cmath<Tag>::mfma(kf[g & 1][i][t], __builtin_bit_cast(su32x4_t, q[KG * g + i]), sc[t]);
         __builtin_amdgcn_sched_barrier(0);
       }
+    } else {
+      float16_t d[TL][2];                       // two chains a tile
+#pragma unroll
+      for (int t = 0; t < TL; ++t)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) d[t][0][r] = d[t][1][r] = 0.f;
+      vec16 kf[2][TL];
+      auto read = [&](int s) {
+#pragma unroll
+        for (int t = 0; t < TL; ++t) kf[s & 1][t] = ld16(base + ka[s] + 32 * t * RB);
+      };
+      read(0);
+#pragma unroll
+      for (int s = 0; s < QS; ++s) {
+        if (s + 1 < QS) read(s + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int t = 0; t < TL; ++t)
+            d[t][i & 1] = __builtin_amdgcn_mfma_f32_32x32x2f32(bits_to_f32(kf[s & 1][t].w[i]), bits_to_f32(q[s].w[i]),
+                                                               d[t][i & 1], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+#pragma unroll
+      for (int t = 0; t < TL; ++t) sc[t] = d[t][0] + d[t][1];
     }
     // ---- online softmax ----
-    uint32_t seen[2];
+    uint32_t seen[TL];
     if constexpr (masked.value) {
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < TL; ++t) {
         seen[t] = tree_seen(a.mask + (int64_t)(row0 + my_row) * a.mask_words, a.mask_words, cached, limit, p0 + 32 * t);
         tree_hide(sc[t], seen[t], half);
       }
     }
     float cm = max_f32(sc[0][0], sc[0][1]);
 #pragma unroll
-    for (int e = 2; e < 32; e += 2) cm = max3_f32(cm, sc[e >> 4][e & 15], sc[e >> 4][(e & 15) + 1]);
+    for (int e = 2; e < 16 * TL; e += 2) cm = max3_f32(cm, sc[e >> 4][e & 15], sc[e >> 4][(e & 15) + 1]);
     cm *= sl2e;
     if (__any(cm > m + 8.f)) {
       const float m_new = fmaxf(m, max_xor32(cm));
@@ -759,28 +469,61 @@ __global__ __launch_bounds__(256, 2) void tree_shared_kernel(const tree_args a) 
       for (int b = 0; b < NB; ++b) acc[b] *= alpha;
     }
     const float neg_m = m == -INFINITY ? 0.f : -m;
-    su32x4_t pb[4];
+    su32x4_t pb[2 * TL];                        // 16-bit P: B operands of 16 positions each
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      float p[8];
+    for (int t = 0; t < TL; ++t)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) p[j] = fast_exp2(fmaf(sc[w >> 1][8 * (w & 1) + j], sl2e, neg_m));
-      pb[w] = smath<Tag>::pack8(p);
+      for (int r = 0; r < 16; ++r) sc[t][r] = fast_exp2(fmaf(sc[t][r], sl2e, neg_m));
+    if constexpr (!F32) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) l = M::add2(pb[w][j], ones, l);   // of the rounded P that multiplies V
+      for (int w = 0; w < 2 * TL; ++w) {
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = sc[w >> 1][8 * (w & 1) + j];
+        pb[w] = smath<Tag>::pack8(p);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) l = cmath<Tag>::add2(pb[w][j], ones, l);   // of the rounded P that multiplies V
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < TL; ++t) {
+        const float16_t& p = sc[t];
+        l += (((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]))) +
+             (((p[8] + p[9]) + (p[10] + p[11])) + ((p[12] + p[13]) + (p[14] + p[15])));
+      }
     }
     // ---- values ----
     bool plain = true;
     if constexpr (masked.value) {
-      plain = tree_finite<T, HALF>(base + HALF, lane);
+      plain = tree_finite<T, 32 * TL * RB>(base + HALF, lane);
       if (!plain) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-          tree_values_apart<Tag, D>(acc, base + HALF + 32 * t * RB, seen[t], half,
-                                    [&](int r) { return tree_unpack<T>(pb[2 * t + (r >> 3)], r & 7); });
+        for (int t = 0; t < TL; ++t)
+          tree_values_apart<Tag, D>(acc, base + HALF + 32 * t * RB, seen[t], half, [&](int r) {
+            if constexpr (F32) return sc[t][r];
+            else return tree_unpack<T>(pb[2 * t + (r >> 3)], r & 7);
+          });
       }
     }
-    if (plain) {
+    if (!plain) {
+    } else if constexpr (F32) {
+      float vf[2][NB];
+      auto read = [&](int i) {                  // position register i of the wave's 16 TL
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          vf[i & 1][b] = *reinterpret_cast<const float*>(base + va[b] + (32 * (i >> 4) + 8 * ((i & 15) >> 2) + (i & 3)) * RB);
+      };
+      read(0);
+#pragma unroll
+      for (int i = 0; i < 16 * TL; ++i) {
+        if (i + 1 < 16 * TL) read(i + 1);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+          acc[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(vf[i & 1][b], sc[i >> 4][i & 15], acc[b], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
       uint2 vf[2][NB][2];
       auto read = [&](int w) {
 #pragma unroll
@@ -792,13 +535,13 @@ __global__ __launch_bounds__(256, 2) void tree_shared_kernel(const tree_args a) 
       };
       read(0);
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        if (w + 1 < 4) read(w + 1);
+      for (int w = 0; w < 2 * TL; ++w) {
+        if (w + 1 < 2 * TL) read(w + 1);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
           const uint2 lo = vf[w & 1][b][0], hi = vf[w & 1][b][1];
-          acc[b] = M::mfma(su32x4_t{lo.x, lo.y, hi.x, hi.y}, pb[w], acc[b]);
+          acc[b] = cmath<Tag>::mfma(su32x4_t{lo.x, lo.y, hi.x, hi.y}, pb[w], acc[b]);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -812,8 +555,33 @@ __global__ __launch_bounds__(256, 2) void tree_shared_kernel(const tree_args a) 
   for (; k < n; ++k) step(k, std::true_type{});
 
   l = sum_xor32(l);
-  if (col0 + lcol >= ncols) return;
+  const bool mine = col0 + lcol < ncols;
   const int slot = w2.x, row = row0 + my_row;   // slot < 0: the whole context, the output itself
+  const float* all = nullptr;                   // the sets' states of these columns
+  float f[SETS];
+  if constexpr (SETS > 1) {
+    float* const state = reinterpret_cast<float*>(lds) + lane;
+    __syncthreads();
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) state[wave * WS + 64 * (16 * b + r)] = acc[b][r];
+    state[wave * WS + 64 * 16 * NB] = m;
+    state[wave * WS + 64 * (16 * NB + 1)] = l;
+    __syncthreads();
+    all = state + (wave % CW) * WS;
+    m = -INFINITY;
+#pragma unroll
+    for (int s = 0; s < SETS; ++s) m = fmaxf(m, all[s * CW * WS + 64 * 16 * NB]);
+    const float safe = m == -INFINITY ? 0.f : m;
+    l = 0.f;
+#pragma unroll
+    for (int s = 0; s < SETS; ++s) {
+      f[s] = fast_exp2(all[s * CW * WS + 64 * 16 * NB] - safe);   // 0 for a set that saw nothing
+      l += all[s * CW * WS + 64 * (16 * NB + 1)] * f[s];
+    }
+  }
+  if (!mine) return;
   float inv = 1.f;
   if (slot < 0) {
     inv = 1.f / l;
@@ -824,8 +592,19 @@ __global__ __launch_bounds__(256, 2) void tree_shared_kernel(const tree_args a) 
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {               // dims 32 b + 8 g + 4 half ..
-      const float4_t o = {acc[b][4 * g], acc[b][4 * g + 1], acc[b][4 * g + 2], acc[b][4 * g + 3]};
+    for (int g = 0; g < 4; ++g) {               // dims 32 b + 8 g + 4 half ..: the group of set g % SETS
+      float4_t o;
+      if constexpr (SETS == 1) {
+        o = float4_t{acc[b][4 * g], acc[b][4 * g + 1], acc[b][4 * g + 2], acc[b][4 * g + 3]};
+      } else {
+        if (g % SETS != set) continue;
+        o = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < SETS; ++s) {
+          const float* const x = all + s * CW * WS + 64 * (16 * b + 4 * g);
+          o += float4_t{x[0], x[64], x[128], x[192]} * f[s];
+        }
+      }
       if (slot < 0) {
         t4_t t;
 #pragma unroll
@@ -835,7 +614,7 @@ __global__ __launch_bounds__(256, 2) void tree_shared_kernel(const tree_args a) 
         *reinterpret_cast<float4_t*>(a.ws_acc + at * D + 32 * b + 8 * g + 4 * half) = o;
       }
     }
-  if (slot >= 0 && half == 0) *reinterpret_cast<float2*>(a.ws_ml + at * 2) = make_float2(m, l);
+  if (slot >= 0 && half == 0 && set == 0) *reinterpret_cast<float2*>(a.ws_ml + at * 2) = make_float2(m, l);
 }
 
 // The partials of a row's parts joined: thread = 4 dims of a head.
@@ -889,27 +668,13 @@ __global__ __launch_bounds__(64) void tree_join_kernel(const tree_args a) {
   st_through(a.out + (int64_t)row * a.out_row_bytes + ((int64_t)head * D + 4 * d4) * sizeof(T), t);
 }
 
-// Waves and ring slots of the waves with positions of their own: 128 KiB of LDS, a workgroup on a CU.
-template <typename Tag, int D>
-struct tlaunch {
-  static constexpr int SLOT = tshape<Tag, D>::SLOT;
-  static constexpr int NW = SLOT == 8192 ? 8 : 4;
-  static constexpr int R = SLOT == 32768 ? 1 : 2;
-  static constexpr int OCC = NW / 4;
-};
-
 template <typename Tag, int D>
 static void launch_columns(const tree_args& a, int num_work, int blocks, int num_split, hipStream_t stream) {
-  using L = tlaunch<Tag, D>;
-  const dim3 grid(num_work), block(64 * L::NW);
-  if (blocks == 1) {
-    hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 1, L::NW, L::R, L::OCC>), grid, block, 0, stream, a);
-  } else if (blocks == 2) {
-    hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 2, L::NW, L::R, L::OCC>), grid, block, 0, stream, a);
-  } else {
-    if constexpr (elem<Tag>::bytes == 2)
-      hipLaunchKernelGGL((tree_shared_kernel<Tag, D>), grid, dim3(256), 0, stream, a);
-  }
+  const dim3 grid(num_work), block(256);
+  if constexpr (tshape<Tag, D>::RB == 128)
+    if (blocks == 1) hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 1, 128>), grid, block, 0, stream, a);
+  if (blocks == 2) hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 2, 64>), grid, block, 0, stream, a);
+  else if (blocks == 4) hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 4, 64>), grid, block, 0, stream, a);
   if (num_split > 0)
     hipLaunchKernelGGL((tree_join_kernel<Tag, D>), dim3(num_split, (a.num_heads * (D / 4) + 63) / 64), dim3(64), 0,
                        stream, a);
@@ -991,11 +756,9 @@ extern "C" int32_t tb_build_tree_work(const int32_t* cached, const int32_t* node
     rows += nodes[b];
   }
   TB_CHECK_ARG(rows < (1 << 30));
-  const bool f32 = dtype == TB_DTYPE_F32;
-  const int blocks = most_cols <= 32 ? 1 : most_cols <= 64 || f32 ? 2 : 4, cols = 32 * blocks;
-  const int slot_kb = head_dim * (f32 ? 4 : 2) * 64 / 1024;   // a chunk's K and V rows
-  tree_price price{slot_kb == 8 ? 8 : 4, 4.0, 1.2, 3.3, num_cus};
-  if (blocks == 4) price = {2, 4.0, head_dim == 64 ? 1.0 : 1.6, head_dim == 64 ? 0.65 : 1.1, num_cus};
+  const int row_bytes = head_dim * (dtype == TB_DTYPE_F32 ? 4 : 2);
+  const int blocks = most_cols <= 32 && row_bytes == 128 ? 1 : most_cols <= 64 ? 2 : 4, cols = 32 * blocks;
+  const tree_price price{blocks == 1 ? 4 : 2, 4.0, head_dim == 64 ? 1.0 : 1.6, head_dim == 64 ? 0.65 : 1.1, num_cus};
   const int part = tree_part_rounds(price, cached, nodes, num_seqs, rep, cols, num_kv_heads,
                                     (double)num_heads * (head_dim + 2) * 4) * price.chunks_round;
   std::vector<tree_piece> pieces;
@@ -1046,7 +809,7 @@ extern "C" int32_t tb_build_tree_work(const int32_t* cached, const int32_t* node
       const tree_piece& p = pieces[lists[x][j].first];
       w[0] = first[p.seq], w[1] = p.seq, w[2] = cached[p.seq], w[3] = nodes[p.seq];
       w[4] = lists[x][j].second * cols, w[5] = p.kvh, w[6] = p.chunk0, w[7] = p.chunks;
-      w[8] = p.slot;
+      w[8] = p.slot, w[9] = p.groups == 1;
     }
   return TB_OK;
 } catch (const std::exception&) {
@@ -1111,7 +874,7 @@ extern "C" int32_t tb_tree_attention(const void* q, int64_t q_row_stride, const 
     TB_RETURN_LAUNCH_STATUS();
   }
   TB_CHECK_ARG(num_work >= 0 && num_split_rows >= 0 && num_split_rows <= num_rows && partial_slots >= 0);
-  TB_CHECK_ARG(column_blocks == 1 || column_blocks == 2 || (column_blocks == 4 && dtype != TB_DTYPE_F32));
+  TB_CHECK_ARG((column_blocks == 1 && head_dim * eb == 128) || column_blocks == 2 || column_blocks == 4);
   TB_CHECK_ARG((num_split_rows == 0 || partial_slots > 0));
   if (num_work == 0) return TB_OK;
   TB_CHECK_ARG(work && ((uintptr_t)work & 15u) == 0 && (num_split_rows == 0 || split_rows) &&
