@@ -26,6 +26,7 @@
 // only when a score outgrows it by 8 (weights to 2^8), so that the accumulators are rescaled
 // a few times per context.
 #include <algorithm>
+#include <cmath>
 #include <exception>
 #include <type_traits>
 #include <vector>
@@ -57,6 +58,7 @@ struct tree_args {
   const int4* split;           // (row, first partial slot, parts, slots between parts)
   float* ws_acc;               // [slots][Hq][D]
   float* ws_ml;                // [slots][Hq][2]
+  int64_t slots;
   float scale_log2e;           // > 0: the scale's size times log2(e), or 1 for a scale of 0
   float q_sign;                // 1, -1 or 0 (NaN: a NaN scale): multiplies q, so that masked scores stay -inf
 };
@@ -617,27 +619,29 @@ __global__ __launch_bounds__(256, D * elem<Tag>::bytes * CK < 32768 ? 2 : 1) voi
   if (slot >= 0 && half == 0 && set == 0) *reinterpret_cast<float2*>(a.ws_ml + at * 2) = make_float2(m, l);
 }
 
-// The partials of a row's parts joined: thread = 4 dims of a head.
-template <typename Tag, int D>
-__global__ __launch_bounds__(64) void tree_join_kernel(const tree_args a) {
+// The partials of a row's parts joined: lane = 4 dims of a head, wave w the parts w, w + NW, ...; the waves'
+// states meet in LDS. One wave up to 16 parts.
+template <typename Tag, int D, int NW>
+__global__ __launch_bounds__(64 * NW) void tree_join_kernel(const tree_args a) {
   using T = typename elem<Tag>::type;
   constexpr int QPH = D / 4, BATCH = 8;
-  const int col = threadIdx.x + 64 * blockIdx.y;
-  if (col >= a.num_heads * QPH) return;
+  __shared__ float state[NW > 1 ? (NW - 1) * 64 * 6 : 1];
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int col = min(lane + 64 * (int)blockIdx.y, a.num_heads * QPH - 1);
   const int4 rec = a.split[blockIdx.x];
   const int row = rec.x, first = rec.y, parts = rec.z, step = rec.w;
   const int head = col / QPH, d4 = col - head * QPH;
   float M = -INFINITY, L = 0.f;
   float4_t o = float4_t{0.f, 0.f, 0.f, 0.f};
-  for (int p0 = 0; p0 < parts; p0 += BATCH) {
+  for (int p0 = wave; p0 < parts; p0 += BATCH * NW) {
     float2 ml[BATCH];
     float4_t av[BATCH];
 #pragma unroll
     for (int k = 0; k < BATCH; ++k) {
       ml[k] = make_float2(-INFINITY, 0.f);
       av[k] = float4_t{0.f, 0.f, 0.f, 0.f};
-      if (p0 + k < parts) {
-        const int64_t at = (int64_t)(first + (p0 + k) * step) * a.num_heads + head;
+      if (p0 + k * NW < parts) {
+        const int64_t at = (int64_t)(first + (p0 + k * NW) * step) * a.num_heads + head;
         ml[k] = *reinterpret_cast<const float2*>(a.ws_ml + at * 2);
         av[k] = *reinterpret_cast<const float4_t*>(a.ws_acc + at * D + 4 * d4);
       }
@@ -656,6 +660,28 @@ __global__ __launch_bounds__(64) void tree_join_kernel(const tree_args a) {
     }
     M = mb;
   }
+  if constexpr (NW > 1) {
+    if (wave > 0) {
+      float* const s = state + (wave - 1) * 64 * 6 + lane;
+      s[0] = M, s[64] = L, s[128] = o[0], s[192] = o[1], s[256] = o[2], s[320] = o[3];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+    float mb = M;
+#pragma unroll
+    for (int w = 0; w < NW - 1; ++w) mb = fmaxf(mb, state[w * 64 * 6 + lane]);
+    const float safe = mb == -INFINITY ? 0.f : mb, keep = fast_exp2(M - safe);
+    L *= keep;
+    o *= keep;
+#pragma unroll
+    for (int w = 0; w < NW - 1; ++w) {
+      const float* const s = state + w * 64 * 6 + lane;
+      const float f = fast_exp2(s[0] - safe);
+      L = fmaf(s[64], f, L);
+      o += float4_t{s[128], s[192], s[256], s[320]} * f;
+    }
+  }
+  if (lane + 64 * (int)blockIdx.y >= a.num_heads * QPH) return;
   float inv = 1.f / L;
   if (!(L > 0.f)) {
     const int seq = a.row_seq[row], r0 = a.row_starts[seq];
@@ -675,9 +701,12 @@ static void launch_columns(const tree_args& a, int num_work, int blocks, int num
     if (blocks == 1) hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 1, 128>), grid, block, 0, stream, a);
   if (blocks == 2) hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 2, 64>), grid, block, 0, stream, a);
   else if (blocks == 4) hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 4, 64>), grid, block, 0, stream, a);
-  if (num_split > 0)
-    hipLaunchKernelGGL((tree_join_kernel<Tag, D>), dim3(num_split, (a.num_heads * (D / 4) + 63) / 64), dim3(64), 0,
-                       stream, a);
+  if (num_split > 0) {
+    const dim3 rows(num_split, (a.num_heads * (D / 4) + 63) / 64);
+    // partial_slots / num_split: the parts of a row on average
+    if (a.slots > 16 * (int64_t)num_split) hipLaunchKernelGGL((tree_join_kernel<Tag, D, 4>), rows, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((tree_join_kernel<Tag, D, 1>), rows, dim3(64), 0, stream, a);
+  }
 }
 
 template <typename Tag>
@@ -693,9 +722,13 @@ static void launch_rows(const tree_args& a, int num_rows, int head_dim, hipStrea
 // ---- the work list (host, no device call) ------------------------------------------
 namespace {
 
+// What a work list costs, in proportions that were fitted to the times of 53 steps cut in every
+// way (12 geometries and types, 1 to 100 sequences, contexts of 300 to 30000 positions, 2 to 64 nodes): the
+// cut it picks is on average 2% slower than the best one. A round is a chunk of a workgroup.
 struct tree_price {
-  int chunks_round;            // chunks a workgroup's waves take at once
-  double start, alone, full;   // us: a workgroup's start and end; a round alone on its CU; on a full chip
+  int chunks_round;            // chunks of 32 positions in a round
+  int on_cu;                   // workgroups a CU holds
+  double full;                 // a CU's time for each round
   int cus;
 };
 
@@ -709,19 +742,24 @@ int tree_part_rounds(const tree_price& price, const int32_t* cached, const int32
   for (int b = 0; b < num_seqs; ++b) longest = std::max(longest, tree_chunks(cached[b], nodes[b]));
   const int most = (longest + price.chunks_round - 1) / price.chunks_round;
   auto cost = [&](int part) {
-    double rounds = 0, wgs = 0, slots = 0;
+    const int len = std::min(part, most);
+    double rounds = 0, wgs = 0, whole = 0, slots = 0;
     for (int b = 0; b < num_seqs; ++b) {
       if (nodes[b] <= 0) continue;
       const int r = (tree_chunks(cached[b], nodes[b]) + price.chunks_round - 1) / price.chunks_round;
       const int groups = (nodes[b] * rep + cols - 1) / cols, parts = (r + part - 1) / part;
-      rounds += (double)r * groups;
-      wgs += (double)parts * groups;
+      rounds += (double)r * groups * num_kv_heads;
+      wgs += (double)parts * groups * num_kv_heads;
+      whole += (double)(r / len) * groups * num_kv_heads;   // of the full length
       if (parts > 1) slots += (double)parts * nodes[b];
     }
-    const double one = price.start + std::min(part, most) * price.alone;
-    const double all = (wgs * price.start + rounds * price.full) * num_kv_heads / price.cus +
-                       0.5 * std::min(part, most) * price.full;
-    return std::max(one, all) + (slots > 0 ? 4.0 + 2 * slots * slot_bytes / 4e6 : 0.);
+    double t = len * 1.45 * price.full;          // the longest workgroup
+    if (wgs > price.cus) {                       // CUs shared: their work evened out, or whole turns of full workgroups
+      const double turn = len * price.full * price.on_cu;
+      t = std::max({t, (rounds * price.full + wgs * 1.5) / price.cus + 0.2 * turn,
+                    2.8 * turn * std::floor(whole / (price.cus * price.on_cu))});
+    }
+    return 6.8 + t + (slots > 0 ? 2.3 + 2 * slots * slot_bytes / 2.3e6 : 0.);   // and the join
   };
   int best = 0;
   double least = cost(std::max(most, 1));
@@ -758,7 +796,12 @@ extern "C" int32_t tb_build_tree_work(const int32_t* cached, const int32_t* node
   TB_CHECK_ARG(rows < (1 << 30));
   const int row_bytes = head_dim * (dtype == TB_DTYPE_F32 ? 4 : 2);
   const int blocks = most_cols <= 32 && row_bytes == 128 ? 1 : most_cols <= 64 ? 2 : 4, cols = 32 * blocks;
-  const tree_price price{blocks == 1 ? 4 : 2, 4.0, head_dim == 64 ? 1.0 : 1.6, head_dim == 64 ? 0.65 : 1.1, num_cus};
+  const double full = dtype == TB_DTYPE_F32 ? (head_dim == 64 ? 3.6 : blocks == 2 ? 7.2 : 10.6)
+                      : head_dim == 128         ? 1.5
+                      : blocks == 1             ? 1.73
+                      : blocks == 2             ? 0.93
+                                                : 0.6;
+  const tree_price price{blocks == 1 ? 4 : 2, row_bytes == 512 ? 1 : 2, full, num_cus};
   const int part = tree_part_rounds(price, cached, nodes, num_seqs, rep, cols, num_kv_heads,
                                     (double)num_heads * (head_dim + 2) * 4) * price.chunks_round;
   std::vector<tree_piece> pieces;
@@ -885,6 +928,7 @@ extern "C" int32_t tb_tree_attention(const void* q, int64_t q_row_stride, const 
   a.work = (const int4*)work;
   a.split = (const int4*)split_rows;
   a.ws_acc = (float*)workspace;
+  a.slots = partial_slots;
   a.ws_ml = (float*)workspace + (size_t)partial_slots * num_heads * head_dim;
   const float s2 = fabsf(scale) * 1.4426950408889634f;
   a.scale_log2e = s2 > 0.f ? s2 : 1.f;
