@@ -691,6 +691,9 @@ int32_t tb_rms_norm_partials(const float* partials, int32_t splits, void* residu
  *     tb_build_tree_work's for this call's sizes (device memory, 16-byte aligned; block_size < 16
  *     needs none); workspace: tb_tree_attention_workspace_bytes, 16-byte aligned, for contexts cut
  *     into parts. Calls that may overlap in time need their own workspace;
+ *   arrivals (may be NULL; only where the list's counts[4] is not 0): arrival_units >= counts[4]
+ *     counters, zero before the first call and left zero by every call; they save the launch that
+ *     joins the parts. Calls that may overlap in time (two streams, two replayed graphs) need their own;
  *   positions [num_rows] (int64) with rope tables: q holds the projections before rotation and is
  *     rotated at them (as tb_kv_append_rope rotates k). */
 int32_t tb_tree_attention(const void* q, int64_t q_row_stride, const void* pool, int64_t num_blocks,
@@ -700,17 +703,19 @@ int32_t tb_tree_attention(const void* q, int64_t q_row_stride, const void* pool,
                           const uint32_t* mask, int32_t mask_words, const int32_t* work,
                           int32_t num_work, int32_t column_blocks, const int32_t* split_rows,
                           int32_t num_split_rows, int32_t partial_slots, void* workspace,
-                          size_t workspace_bytes, int32_t num_heads, int32_t num_kv_heads,
+                          size_t workspace_bytes, uint32_t* arrivals, int32_t arrival_units,
+                          int32_t num_heads, int32_t num_kv_heads,
                           int32_t head_dim, int32_t block_size, float scale,
                           int32_t dtype, const int64_t* positions, const float* rope_cos,
                           const float* rope_sin, int32_t rope_max_position, hipStream_t stream);
 
 /* The work list of tb_tree_attention (host memory, no device call): cached [num_seqs] positions and
  * nodes [num_seqs] rows of each sequence, in row order, on a GPU of num_cus CUs and num_xcds XCDs.
- * counts [4]: work entries (12 int32 each), split rows (4 int32 each), partial slots, column
- * blocks per workgroup. work and split NULL: the counts alone. An entry is (first row, sequence,
+ * counts [5]: work entries (12 int32 each), split rows (4 int32 each), partial slots, column
+ * blocks per workgroup, and the arrival counters of a call that joins the parts in its one launch
+ * (0: no parts, or too much to join there). work and split NULL: the counts alone. An entry is (first row, sequence,
  * cached, nodes, first column, kv head, first chunk of 32 positions, chunks, partial slot of node 0
- * or -1, whether no other entry reads its K/V rows, 0, 0), with 0 nodes for a padding entry; entry g is meant for XCD g % num_xcds. */
+ * or -1, whether no other entry reads its K/V rows, arrival counter, part | parts << 16), with 0 nodes for a padding entry; entry g is meant for XCD g % num_xcds. */
 int32_t tb_build_tree_work(const int32_t* cached, const int32_t* nodes, int32_t num_seqs,
                            int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
                            int32_t num_cus, int32_t num_xcds, int32_t* work, int32_t work_capacity,
@@ -738,7 +743,10 @@ size_t tb_tree_attention_workspace_bytes(int32_t partial_slots, int32_t num_head
  *   max_children: the most children a node has (a hint: it decides how many of the sums that
  *     refusals need get launches over the whole GPU);
  *   workspace: tb_tree_verify_workspace_bytes, 8-byte aligned; calls that may overlap in time need
- *     their own.
+ *     their own;
+ *   arrivals [arrival_units >= num_seqs] (may be NULL): counters, zero before the first call and left
+ *     zero by every call, which save a launch; calls that may overlap in time (two streams, two
+ *     replayed graphs) need their own.
  * dtype is that of probs and draft_probs; row strides in elements. */
 size_t tb_tree_verify_workspace_bytes(int32_t num_seqs, int32_t vocab, int32_t width);
 int32_t tb_tree_verify(const void* probs, int64_t probs_row_stride, const void* draft_probs,
@@ -746,7 +754,7 @@ int32_t tb_tree_verify(const void* probs, int64_t probs_row_stride, const void* 
                        const float* uniforms, const int32_t* parents, const int32_t* row_starts,
                        int32_t num_seqs, int32_t max_children, int32_t* accepted, int32_t* num_accepted,
                        int64_t* out_tokens, int32_t width, void* workspace, size_t workspace_bytes,
-                       hipStream_t stream);
+                       uint32_t* arrivals, int32_t arrival_units, hipStream_t stream);
 
 /* The same for greedy decoding: target_ids [num_rows] (int64) is the target's choice after each
  * node (tb_linear_argmax); the first child that holds it is kept. Trees of any size. */

@@ -106,9 +106,9 @@ def test_entries_reject_bad_arguments_without_launching():
     bad, unsupported = _lib.TB_ERR_INVALID_ARG, _lib.TB_ERR_UNSUPPORTED
 
     def verify(probs=f, stride=100, draft=None, dstride=0, vocab=100, dt=0, tokens=f, seqs=2, width=4, acc=f,
-               children=1, ws=f, wsb=1 << 20):
+               children=1, ws=f, wsb=1 << 20, arrivals=None, units=0):
         return L.tb_tree_verify(probs, stride, draft, dstride, vocab, dt, tokens, f, f, f, seqs, children, acc, f, f,
-                                width, ws, wsb, None)
+                                width, ws, wsb, arrivals, units, None)
 
     assert verify(stride=99) == bad                    # rows overlap
     assert verify(draft=f, dstride=99) == bad
@@ -116,6 +116,7 @@ def test_entries_reject_bad_arguments_without_launching():
     assert verify(probs=None) == bad and verify(tokens=None) == bad and verify(acc=None) == bad
     assert verify(children=-1) == bad and verify(ws=None) == bad and verify(ws=ctypes.c_void_p(4100)) == bad
     assert verify(wsb=L.tb_tree_verify_workspace_bytes(2, 100, 4) - 1) == bad
+    assert verify(arrivals=f, units=1) == bad                    # fewer counters than sequences
     assert verify(width=MAX_NODES + 1) == unsupported
     assert verify(vocab=1 << 25, stride=1 << 25, wsb=1 << 30) == unsupported
     assert verify(seqs=0, probs=None) == _lib.TB_OK
@@ -133,9 +134,9 @@ def test_entries_reject_bad_arguments_without_launching():
     assert commit(layers=0) == _lib.TB_OK and commit(seqs=0) == _lib.TB_OK
 
     def attention(q=f, d=64, bs=16, hq=14, hkv=2, dt=1, qs=896, words=1, work=f, nw=8, blocks=1, split=None, ns=0, slots=0,
-                  ws=None, wsb=0, rows=4, rc=None, rs=None, rmax=0):
+                  ws=None, wsb=0, rows=4, rc=None, rs=None, rmax=0, arrivals=None, units=0):
         return L.tb_tree_attention(q, qs, f, 64, f, 896, f, 4, f, f, 2, f, rows, f, words, work, nw, blocks, split, ns,
-                                   slots, ws, wsb, hq, hkv, d, bs, 0.125, dt, f, rc, rs, rmax, None)
+                                   slots, ws, wsb, arrivals, units, hq, hkv, d, bs, 0.125, dt, f, rc, rs, rmax, None)
 
     assert attention(d=96) == unsupported
     assert attention(hq=13) == bad and attention(bs=12) == bad and attention(dt=3) == bad and attention(words=0) == bad
@@ -147,6 +148,7 @@ def test_entries_reject_bad_arguments_without_launching():
     assert attention(ns=1, slots=2, split=f) == bad                       # ... without a workspace
     assert attention(ns=1, slots=2, split=f, ws=f, wsb=2 * 14 * 66 * 4 - 1) == bad
     assert attention(ns=5, slots=9, split=f, ws=f, wsb=1 << 20) == bad    # more split rows than rows
+    assert attention(ns=1, slots=2, split=f, ws=f, wsb=1 << 20, arrivals=f, units=0) == bad
     assert attention(rc=f, rmax=64) == bad and attention(rc=f, rs=f, rmax=0) == bad
     assert attention(rows=0, q=None) == _lib.TB_OK and attention(nw=0) == _lib.TB_OK
     assert L.tb_tree_attention_workspace_bytes(10, 14, 64) == 10 * 14 * 66 * 4
@@ -169,15 +171,17 @@ def test_work_covers_every_context_once(hq, hkv, d, dtype, sizes, cached):
                             head_dim=d, dtype=dtype)
     cols, rep = 32 * m.column_blocks, hq // hkv
     assert m.work_np.shape[0] % 8 == 0
-    seen, slots, where = {}, {}, {}
-    for g, (row0, seq, c, n, col0, kvh, chunk0, chunks, slot, once, *zero) in enumerate(m.work_np.tolist()):
-        assert zero == [0, 0]
+    seen, slots, where, units, orders = {}, {}, {}, {}, {}
+    for g, (row0, seq, c, n, col0, kvh, chunk0, chunks, slot, once, unit, order) in enumerate(m.work_np.tolist()):
         if n == 0:
             continue
         assert once == (n * rep <= cols)
         assert (row0, c, n) == (m.row_starts_np[seq], cached[seq], sizes[seq]) and chunks > 0
         seen.setdefault((seq, kvh, col0), []).extend(range(chunk0, chunk0 + chunks))
         slots.setdefault(seq, {})[chunk0] = slot
+        if slot >= 0:
+            assert units.setdefault((seq, kvh, col0), unit) == unit
+            orders.setdefault(unit, {})[order & 0xFFFF] = (chunk0, order >> 16)
         assert where.setdefault((seq, kvh, chunk0), g % 8) == g % 8
     want = {(b, h, x): list(range(-(-(cached[b] + n) // 32))) for b, n in enumerate(sizes) for h in range(hkv)
             for x in range(0, n * rep, cols)}
@@ -191,4 +195,9 @@ def test_work_covers_every_context_once(hq, hkv, d, dtype, sizes, cached):
         assert parts == [parts[0] + i * n for i in range(len(parts))]
         used += range(parts[0], parts[0] + len(parts) * n)
         records += [[int(m.row_starts_np[seq]) + i, parts[0] + i, len(parts), n] for i in range(n)]
+    if m.units:                                  # parts in the order of their chunks, a counter for each unit
+        assert sorted(units.values()) == list(range(m.units))
+        for by in orders.values():
+            assert sorted(by) == list(range(len(by))) and all(n == len(by) for _, n in by.values())
+            assert [by[i][0] for i in range(len(by))] == sorted(x for x, _ in by.values())
     assert sorted(used) == list(range(m.partial_slots)) and sorted(m.split_np.tolist()) == sorted(records)

@@ -139,7 +139,7 @@ SIGNATURES = {
         c_vp, c_i32, c_vp, c_vp, c_i32, c_vp, c_i32,   # block tables, max_nb, row starts, cached, seqs, row_seq, rows
         c_vp, c_i32,                             # mask, words
         c_vp, c_i32, c_i32, c_vp, c_i32, c_i32,  # work, count, column blocks, split rows, count, partial slots
-        c_vp, c_sz,                              # workspace, bytes
+        c_vp, c_sz, c_vp, c_i32,                 # workspace, bytes, arrivals, units
         c_i32, c_i32, c_i32, c_i32, c_f32, c_i32,   # heads, kv heads, head_dim, block_size, scale, dtype
         c_vp, c_vp, c_vp, c_i32, c_vp]),         # positions, rope cos, sin, max position, stream
     "tb_build_tree_work": (c_i32, [c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp, c_i32, c_vp,
@@ -148,7 +148,8 @@ SIGNATURES = {
     "tb_tree_verify_workspace_bytes": (c_sz, [c_i32, c_i32, c_i32]),
     "tb_tree_verify": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i32,   # probs, stride, draft, stride, vocab, dtype
                                c_vp, c_vp, c_vp, c_vp, c_i32, c_i32,     # tokens, uniforms, parents, row starts, seqs, children
-                               c_vp, c_vp, c_vp, c_i32, c_vp, c_sz, c_vp]),   # outputs, width, workspace, bytes, stream
+                               c_vp, c_vp, c_vp, c_i32, c_vp, c_sz,      # outputs, width, workspace, bytes
+                               c_vp, c_i32, c_vp]),                      # arrivals, units, stream
     "tb_tree_verify_greedy": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp, c_i32, c_vp]),
     "tb_tree_commit": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_vp, c_i32, c_vp, c_i32, c_vp, c_i32, c_vp, c_i32, c_i32,
                                c_i32, c_i32, c_vp]),

@@ -15,7 +15,8 @@
 // the next chunk (direct global->LDS loads) and computes on the present one, one barrier between.
 // A wave holds 32 columns; with CW < 4 several waves hold the same ones, each a part of a
 // chunk's positions, and join their softmax states in LDS at the end. A context cut into parts
-// leaves a partial per part, joined by a second launch.
+// leaves a partial per part, joined by the workgroup of a (sequence, kv head, columns) that arrives
+// last where there is little to join and the caller gives arrival counters, else by a second launch.
 //
 // Math per chunk and block of 32 columns (C rows are positions or dims, C columns the block's):
 //   S^T[pos][col] = K[pos][:] . q[col][:]        A = K rows from LDS, B = q in registers
@@ -59,6 +60,7 @@ struct tree_args {
   float* ws_acc;               // [slots][Hq][D]
   float* ws_ml;                // [slots][Hq][2]
   int64_t slots;
+  uint32_t* arrivals;          // [units], zero between calls; null: tree_join_kernel joins
   float scale_log2e;           // > 0: the scale's size times log2(e), or 1 for a scale of 0
   float q_sign;                // 1, -1 or 0 (NaN: a NaN scale): multiplies q, so that masked scores stay -inf
 };
@@ -283,6 +285,57 @@ __device__ __forceinline__ void tree_q(vec16 (&q)[QS], const tree_args& a, int r
   for (int s = 0; s < QS; ++s)
 #pragma unroll
     for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(q[s].w[i]));
+}
+
+// The join of a unit's parts by its last workgroup: what the others wrote is read past the L2s, which the
+// XCDs do not share. Thread = 4 dims of a column.
+template <typename Tag, int D, int CW>
+__device__ __forceinline__ void tree_join_here(const tree_args& a, int row0, int cached, int nodes, int col0, int kvh,
+                                               int first, int parts) {
+  using T = typename elem<Tag>::type;
+  constexpr int QPC = D / 4, BATCH = 4;
+  auto load2 = [](const float* p) {
+    return __builtin_bit_cast(float2, __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+  };
+  for (int i = threadIdx.x; i < 32 * CW * QPC; i += 256) {
+    const int col = col0 + i / QPC, d4 = i % QPC;
+    if (col >= nodes * a.rep) break;
+    const int node = col / a.rep, head = kvh * a.rep + col - node * a.rep;
+    float M = -INFINITY, L = 0.f;
+    float4_t o = float4_t{0.f, 0.f, 0.f, 0.f};
+    for (int p0 = 0; p0 < parts; p0 += BATCH) {
+      float2 ml[BATCH], lo[BATCH], hi[BATCH];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const int64_t at = (int64_t)(first + min(p0 + k, parts - 1) * nodes + node) * a.num_heads + head;
+        ml[k] = load2(a.ws_ml + at * 2);
+        lo[k] = load2(a.ws_acc + at * D + 4 * d4);
+        hi[k] = load2(a.ws_acc + at * D + 4 * d4 + 2);
+      }
+      float mb = M;
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) mb = fmaxf(mb, ml[k].x);
+      const float safe = mb == -INFINITY ? 0.f : mb, keep = fast_exp2(M - safe);
+      L *= keep;
+      o *= keep;
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        if (p0 + k >= parts) break;
+        const float w = fast_exp2(ml[k].x - safe);   // 0 for a part that saw nothing
+        L = fmaf(ml[k].y, w, L);
+        o += float4_t{lo[k].x, lo[k].y, hi[k].x, hi[k].y} * w;
+      }
+      M = mb;
+    }
+    const int row = row0 + node;
+    float inv = 1.f / L;
+    if (!(L > 0.f) && !tree_sees(a.mask + (int64_t)row * a.mask_words, cached, nodes)) inv = 0.f;
+    typedef T t4_t __attribute__((ext_vector_type(4)));
+    t4_t t;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) t[j] = (T)(o[j] * inv);
+    st_through(a.out + (int64_t)row * a.out_row_bytes + ((int64_t)head * D + 4 * d4) * sizeof(T), t);
+  }
 }
 
 // 32 CW columns: the four waves share chunks of CK positions, of which each loads a quarter. CW of them take
@@ -583,40 +636,61 @@ __global__ __launch_bounds__(256, D * elem<Tag>::bytes * CK < 32768 ? 2 : 1) voi
       l += all[s * CW * WS + 64 * (16 * NB + 1)] * f[s];
     }
   }
-  if (!mine) return;
-  float inv = 1.f;
-  if (slot < 0) {
-    inv = 1.f / l;
-    if (!(l > 0.f) && !tree_sees(a.mask + (int64_t)row * a.mask_words, cached, nodes)) inv = 0.f;
-  }
-  typedef T t4_t __attribute__((ext_vector_type(4)));
-  const int64_t at = (int64_t)(slot + my_row) * a.num_heads + hd;
+  const bool here = slot >= 0 && a.arrivals != nullptr;   // the last workgroup joins the parts
+  if (mine) {
+    float inv = 1.f;
+    if (slot < 0) {
+      inv = 1.f / l;
+      if (!(l > 0.f) && !tree_sees(a.mask + (int64_t)row * a.mask_words, cached, nodes)) inv = 0.f;
+    }
+    typedef T t4_t __attribute__((ext_vector_type(4)));
+    const int64_t at = (int64_t)(slot + my_row) * a.num_heads + hd;
 #pragma unroll
-  for (int b = 0; b < NB; ++b)
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {               // dims 32 b + 8 g + 4 half ..: the group of set g % SETS
-      float4_t o;
-      if constexpr (SETS == 1) {
-        o = float4_t{acc[b][4 * g], acc[b][4 * g + 1], acc[b][4 * g + 2], acc[b][4 * g + 3]};
-      } else {
-        if (g % SETS != set) continue;
-        o = float4_t{0.f, 0.f, 0.f, 0.f};
+      for (int g = 0; g < 4; ++g) {             // dims 32 b + 8 g + 4 half ..: the group of set g % SETS
+        float4_t o;
+        if constexpr (SETS == 1) {
+          o = float4_t{acc[b][4 * g], acc[b][4 * g + 1], acc[b][4 * g + 2], acc[b][4 * g + 3]};
+        } else {
+          if (g % SETS != set) continue;
+          o = float4_t{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int s = 0; s < SETS; ++s) {
-          const float* const x = all + s * CW * WS + 64 * (16 * b + 4 * g);
-          o += float4_t{x[0], x[64], x[128], x[192]} * f[s];
+          for (int s = 0; s < SETS; ++s) {
+            const float* const x = all + s * CW * WS + 64 * (16 * b + 4 * g);
+            o += float4_t{x[0], x[64], x[128], x[192]} * f[s];
+          }
+        }
+        float* const partial = a.ws_acc + at * D + 32 * b + 8 * g + 4 * half;
+        if (slot < 0) {
+          t4_t t;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) t[j] = (T)(o[j] * inv);
+          st_through(a.out + (int64_t)row * a.out_row_bytes + (int64_t)hd * RB + (32 * b + 8 * g + 4 * half) * S::EB, t);
+        } else if (here) {
+          st_through(partial, o);
+        } else {
+          *reinterpret_cast<float4_t*>(partial) = o;
         }
       }
-      if (slot < 0) {
-        t4_t t;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) t[j] = (T)(o[j] * inv);
-        st_through(a.out + (int64_t)row * a.out_row_bytes + (int64_t)hd * RB + (32 * b + 8 * g + 4 * half) * S::EB, t);
-      } else {
-        *reinterpret_cast<float4_t*>(a.ws_acc + at * D + 32 * b + 8 * g + 4 * half) = o;
-      }
+    if (slot >= 0 && half == 0 && set == 0) {
+      if (here) st8_through(a.ws_ml + at * 2, make_float2(m, l));
+      else *reinterpret_cast<float2*>(a.ws_ml + at * 2) = make_float2(m, l);
     }
-  if (slot >= 0 && half == 0 && set == 0) *reinterpret_cast<float2*>(a.ws_ml + at * 2) = make_float2(m, l);
+  }
+  if (!here) return;
+  __shared__ uint32_t arrived;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the wave's partials are in memory
+  __syncthreads();
+  const int parts = w2.w >> 16, part = w2.w & 0xFFFF;
+  if (threadIdx.x == 0) {
+    arrived = __hip_atomic_fetch_add(&a.arrivals[w2.z], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (arrived == (uint32_t)parts - 1)
+      __hip_atomic_store(&a.arrivals[w2.z], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  if (arrived == (uint32_t)parts - 1)
+    tree_join_here<Tag, D, CW>(a, row0, cached, nodes, w1.x, kvh, slot - part * nodes, parts);
 }
 
 // The partials of a row's parts joined: lane = 4 dims of a head, wave w the parts w, w + NW, ...; the waves'
@@ -701,7 +775,7 @@ static void launch_columns(const tree_args& a, int num_work, int blocks, int num
     if (blocks == 1) hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 1, 128>), grid, block, 0, stream, a);
   if (blocks == 2) hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 2, 64>), grid, block, 0, stream, a);
   else if (blocks == 4) hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 4, 64>), grid, block, 0, stream, a);
-  if (num_split > 0) {
+  if (num_split > 0 && !a.arrivals) {
     const dim3 rows(num_split, (a.num_heads * (D / 4) + 63) / 64);
     // partial_slots / num_split: the parts of a row on average
     if (a.slots > 16 * (int64_t)num_split) hipLaunchKernelGGL((tree_join_kernel<Tag, D, 4>), rows, dim3(256), 0, stream, a);
@@ -771,8 +845,12 @@ int tree_part_rounds(const tree_price& price, const int32_t* cached, const int32
 }
 
 struct tree_piece {
-  int seq, kvh, chunk0, chunks, slot, groups;
+  int seq, kvh, chunk0, chunks, slot, groups, unit, order;   // order: part | parts << 16
 };
+
+// The most bytes of partials that a unit's last workgroup joins: a workgroup reads them at some 60 GB/s,
+// a launch of its own takes 2.5 us of the GPU and 3 us of the host.
+constexpr int64_t JOIN_HERE_BYTES = 192 << 10;
 
 }  // namespace
 
@@ -805,19 +883,24 @@ extern "C" int32_t tb_build_tree_work(const int32_t* cached, const int32_t* node
   const int part = tree_part_rounds(price, cached, nodes, num_seqs, rep, cols, num_kv_heads,
                                     (double)num_heads * (head_dim + 2) * 4) * price.chunks_round;
   std::vector<tree_piece> pieces;
-  int64_t slots = 0, num_split = 0, row0 = 0;
+  int64_t slots = 0, num_split = 0, row0 = 0, units = 0;
+  bool here = true;
   std::vector<int32_t> first(num_seqs + 1);
   for (int b = 0; b < num_seqs; ++b) {
     first[b] = (int32_t)row0;
     row0 += nodes[b];
     const int all = tree_chunks(cached[b], nodes[b]);
     if (all == 0) continue;
-    const int parts = part ? (all + part - 1) / part : 1;
+    const int parts = part ? (all + part - 1) / part : 1, groups = (nodes[b] * rep + cols - 1) / cols;
+    const bool few = parts < (1 << 15);
     for (int i = 0; i < parts; ++i)
       for (int h = 0; h < num_kv_heads; ++h)
         pieces.push_back({b, h, part * i, part ? std::min(part, all - part * i) : all,
-                          parts > 1 ? (int)(slots + (int64_t)i * nodes[b]) : -1, (nodes[b] * rep + cols - 1) / cols});
+                          parts > 1 ? (int)(slots + (int64_t)i * nodes[b]) : -1, groups, (int)(units + h * groups),
+                          few ? i | parts << 16 : 0});
     if (parts > 1) {
+      here &= few && (int64_t)parts * std::min(cols, nodes[b] * rep) * head_dim * 4 <= JOIN_HERE_BYTES;
+      units += (int64_t)groups * num_kv_heads;
       for (int i = 0; i < nodes[b]; ++i, ++num_split)
         if (split && num_split < split_capacity) {
           int32_t* const s = split + 4 * num_split;
@@ -825,7 +908,7 @@ extern "C" int32_t tb_build_tree_work(const int32_t* cached, const int32_t* node
         }
       slots += (int64_t)parts * nodes[b];
     }
-    TB_CHECK_ARG(slots < (1 << 30));
+    TB_CHECK_ARG(slots < (1 << 30) && units < (1 << 30));
   }
   // longest first; the column groups of one piece, which read the same rows, on one XCD
   std::stable_sort(pieces.begin(), pieces.end(),
@@ -842,6 +925,7 @@ extern "C" int32_t tb_build_tree_work(const int32_t* cached, const int32_t* node
   TB_CHECK_ARG(depth * num_xcds < ((size_t)1 << 30));
   const int64_t n = (int64_t)depth * num_xcds;
   counts[0] = (int32_t)n, counts[1] = (int32_t)num_split, counts[2] = (int32_t)slots, counts[3] = blocks;
+  counts[4] = here ? (int32_t)units : 0;
   if (!work && !split) return TB_OK;
   TB_CHECK_ARG((n == 0 || work) && work_capacity >= n && (num_split == 0 || split) && split_capacity >= num_split);
   for (size_t j = 0; j < depth; ++j)
@@ -852,7 +936,7 @@ extern "C" int32_t tb_build_tree_work(const int32_t* cached, const int32_t* node
       const tree_piece& p = pieces[lists[x][j].first];
       w[0] = first[p.seq], w[1] = p.seq, w[2] = cached[p.seq], w[3] = nodes[p.seq];
       w[4] = lists[x][j].second * cols, w[5] = p.kvh, w[6] = p.chunk0, w[7] = p.chunks;
-      w[8] = p.slot, w[9] = p.groups == 1;
+      w[8] = p.slot, w[9] = p.groups == 1, w[10] = p.unit + lists[x][j].second, w[11] = p.order;
     }
   return TB_OK;
 } catch (const std::exception&) {
@@ -871,7 +955,8 @@ extern "C" int32_t tb_tree_attention(const void* q, int64_t q_row_stride, const 
                                      const uint32_t* mask, int32_t mask_words, const int32_t* work,
                                      int32_t num_work, int32_t column_blocks, const int32_t* split_rows,
                                      int32_t num_split_rows, int32_t partial_slots, void* workspace,
-                                     size_t workspace_bytes, int32_t num_heads, int32_t num_kv_heads,
+                                     size_t workspace_bytes, uint32_t* arrivals, int32_t arrival_units,
+                                     int32_t num_heads, int32_t num_kv_heads,
                                      int32_t head_dim, int32_t block_size, float scale,
                                      int32_t dtype, const int64_t* positions, const float* rope_cos,
                                      const float* rope_sin, int32_t rope_max_position, hipStream_t stream) {
@@ -925,6 +1010,8 @@ extern "C" int32_t tb_tree_attention(const void* q, int64_t q_row_stride, const 
   if (partial_slots > 0)
     TB_CHECK_ARG(workspace && ((uintptr_t)workspace & 15u) == 0 &&
                  workspace_bytes >= tb_tree_attention_workspace_bytes(partial_slots, num_heads, head_dim));
+  TB_CHECK_ARG(!arrivals || (arrival_units > 0 && ((uintptr_t)arrivals & 3u) == 0));
+  a.arrivals = partial_slots > 0 ? arrivals : nullptr;
   a.work = (const int4*)work;
   a.split = (const int4*)split_rows;
   a.ws_acc = (float*)workspace;

@@ -23,15 +23,17 @@
 
 namespace tb {
 
-// A call is a chain of launches with no atomics between them. Launch 0: every workgroup
-// of a sequence walks its tree until it needs a sum over the vocabulary, and sums its own
-// stretch of the row; launch r + 1: every workgroup adds up launch r's stretches in order, goes on
-// with the walk, and sums its stretch again; the last launch, one workgroup per sequence, finds
-// the border's stretch, thread and token. A chain, and drafts that were not drawn, need one sum
-// whatever is refused; a tree of drawn drafts one more per refusal that has a sibling
-// behind it: up to MAX_ROUNDS of those in launches of their own, the rest in the last one. What
-// a later launch starts from (the state, the nodes' values, the sums) it loads at once.
-constexpr int SUM_THREADS = 256, FIND_THREADS = 512, FIND_CHUNKS = 4;
+// A call is a chain of launches. Launch 0: every workgroup of a sequence walks its tree until it
+// needs a sum over the vocabulary, and sums its own stretch of the row; launch r + 1: every workgroup
+// adds up launch r's stretches in order, goes on with the walk, and sums its stretch again. A
+// chain, and drafts that were not drawn, need one sum whatever is refused; a tree of drawn
+// drafts one more per refusal that has a sibling behind it: up to MAX_ROUNDS of those in launches of
+// their own, the rest by one workgroup at the end. What a later launch starts from (the state,
+// the nodes' values, the sums) it loads at once.
+// The end, by one workgroup per sequence, finds the border's stretch, thread and token: the
+// workgroup of the last sum launch that arrives last where the caller gives arrival counters, else
+// a launch of its own (a graph's replays may overlap, and then no counter is theirs alone).
+constexpr int SUM_THREADS = 256, FIND_CHUNKS = 8;   // chunks of a thread at the end: up to 64 tokens, a lane each
 constexpr int MAX_ROUNDS = 5;
 constexpr int MAX_STRETCHES = 64;
 constexpr int MAX_STRETCH = 1 << 18;               // tokens whose refused ones are kept as bits in LDS
@@ -62,6 +64,7 @@ struct verify_args {
   verify_state* states;        // [launch][B]
   double* sums;                // [launch][B][stretches]
   int32_t* nodes;              // [B][5][width]: verify_tree's arrays
+  uint32_t* arrivals;          // [B], zero between calls; null: the end is a launch of its own
 };
 
 template <int N>
@@ -111,7 +114,7 @@ __device__ __forceinline__ void load_tree(const verify_args& a, const verify_tre
 // at st.a. Nodes kept are written to path[] (LDS) as they come.
 __device__ __forceinline__ void walk(const verify_tree& t, int n, bool drawn, double s, verify_state& st,
                                      int32_t* path, int lane, int launch) {
-  auto child = [&](int from) -> int {              // the next child of st.cur from row `from` on, or n
+  auto child = [&](int from) __attribute__((always_inline)) -> int {              // the next child of st.cur from row `from` on, or n
     for (int i0 = from & ~63; i0 < n; i0 += 64) {
       const int i = i0 + lane;
       const uint64_t hit = __ballot(i < n && i >= from && t.par[i < n ? i : 0] == st.cur);
@@ -159,79 +162,111 @@ __device__ __forceinline__ void walk(const verify_tree& t, int n, bool drawn, do
 }
 
 // A row of the vocabulary in 16-byte chunks of the memory it lies in: chunk c holds tokens
-// c E - shift .. + E - 1. The draft's row is read chunk by chunk too where it is aligned alike.
-template <typename T>
+// c E - shift .. + E - 1. What is left of a token: max(p - a q, 0) where the drafts were drawn (the draft's
+// row is read chunk by chunk too where it is aligned alike; before a refusal a = 0, and the target's row
+// stands in for it), otherwise p without the refused tokens.
+template <typename T, bool DRAWN>
 struct verify_row {
   static constexpr int E = 16 / sizeof(T);
   const char* p;               // the aligned chunk 0
-  const T* q;                  // the draft's row, token 0; null without
+  const T* q;                  // the draft's row, token 0
   int shift, vocab, chunks;
-  bool q_alike;
+  bool alike;
   double a;
-  const uint32_t* bits;        // refused tokens from token bit0 on; null: none
-  int bit0;
+  const uint32_t* bits;        // refused tokens from chunk first on, a bit each; null: none
+  int first;
 
-  __device__ verify_row(const verify_args& v, int row, double a_) : vocab(v.vocab), a(a_), bits(nullptr), bit0(0) {
-    const uintptr_t at = (uintptr_t)((const T*)v.probs + (int64_t)row * v.probs_stride);
-    shift = (int)((at & 15) / sizeof(T));
-    p = (const char*)(at & ~(uintptr_t)15);
+  __device__ verify_row(const verify_args& v, int row, double a_) : vocab(v.vocab), bits(nullptr), first(0) {
+    const T* const at = (const T*)v.probs + (int64_t)row * v.probs_stride;
+    shift = (int)(((uintptr_t)at & 15) / sizeof(T));
+    p = (const char*)((uintptr_t)at & ~(uintptr_t)15);
     chunks = (vocab + shift + E - 1) / E;
-    q = v.draft && a_ != 0. ? (const T*)v.draft + (int64_t)row * v.draft_stride : nullptr;
-    q_alike = ((uintptr_t)q & 15) == (at & 15);
+    draft(DRAWN && a_ != 0. ? (const T*)v.draft + (int64_t)row * v.draft_stride : at, a_);
+  }
+  __device__ __forceinline__ void draft(const T* q_, double a_) {
+    q = q_, a = a_;
+    alike = (((uintptr_t)q ^ (uintptr_t)shift * sizeof(T)) & 15) == 0;
+  }
+  // the row as it is
+  __device__ __forceinline__ void whole() {
+    bits = nullptr;
+    draft((const T*)p + shift, 0.);
   }
   struct chunk {
-    T p[E], q[E];
+    T p[E], q[DRAWN ? E : 1];
   };
   __device__ __forceinline__ chunk load(int c) const {
     chunk x;
     const vec16 v = ld16(p + (int64_t)c * 16);     // its 16 bytes hold a token of the row: inside its page
     __builtin_memcpy(x.p, &v, 16);
-    if (q) {
-      if (q_alike) {
-        const vec16 w = ld16((const char*)q - shift * (int)sizeof(T) + (int64_t)c * 16);
-        __builtin_memcpy(x.q, &w, 16);
+    if constexpr (DRAWN) {
+      vec16 w;
+      if (alike) {
+        w = ld16((const char*)q - shift * (int)sizeof(T) + (int64_t)c * 16);
       } else {
+        T e[E];
 #pragma unroll
-        for (int j = 0; j < E; ++j) x.q[j] = q[min(max(c * E - shift + j, 0), vocab - 1)];
+        for (int j = 0; j < E; ++j) e[j] = q[min(max(c * E - shift + j, 0), vocab - 1)];
+        __builtin_memcpy(&w, e, 16);
       }
+      __builtin_memcpy(x.q, &w, 16);
     }
     return x;
   }
-  // what is left of the chunk's j-th token
-  __device__ __forceinline__ double weight(const chunk& x, int c, int j, bool edge) const {
-    double w = (double)(float)x.p[j];
-    if (q) w = fma(-a, (double)(float)x.q[j], w);
-    const int i = c * E - shift + j;
-    if (edge && (i < 0 || i >= vocab)) return 0.;
-    if (bits && ((bits[(i - bit0) >> 5] >> ((i - bit0) & 31)) & 1)) return 0.;
+  // what is left of a token whose values are x and y
+  __device__ __forceinline__ double left(T x, T y, uint32_t gone) const {
+    double w = (double)(float)x;
+    if constexpr (DRAWN) w = fma(-a, (double)(float)y, w);
+    else if (gone & 1) w = 0.;
     return w > 0. ? w : 0.;
+  }
+  // the refused tokens of chunk c
+  __device__ __forceinline__ uint32_t gone(int c) const {
+    const int bit = (c - first) * E;
+    return !DRAWN && bits ? bits[bit >> 5] >> (bit & 31) : 0u;
+  }
+  __device__ __forceinline__ double weight(int i) const {
+    if (i < 0 || i >= vocab) return 0.;
+    const int c = (i + shift) / E;
+    return left(((const T*)p)[i + shift], DRAWN ? q[i] : (T)0, gone(c) >> (i + shift - c * E));
   }
   __device__ __forceinline__ double sum(const chunk& x, int c) const {
     const bool edge = c == 0 || c == chunks - 1;
+    const uint32_t no = gone(c);
     double s = 0.;
 #pragma unroll
-    for (int j = 0; j < E; ++j) s += weight(x, c, j, edge);
+    for (int j = 0; j < E; ++j) {
+      const int i = c * E - shift + j;
+      s += edge && (i < 0 || i >= vocab) ? 0. : left(x.p[j], x.q[DRAWN ? j : 0], no >> j);
+    }
     return s;
   }
   // this thread's share of chunks [b, e): every nth from b + i on
   __device__ __forceinline__ double share(int b, int e, int i, int nth) const {
     constexpr int U = 4;                           // chunks in flight
     double s = 0.;
-    int c = b + i;
-    for (; c + (U - 1) * nth < e; c += U * nth) {
+    for (int c = b + i; c < e; c += U * nth) {
       chunk x[U];
 #pragma unroll
-      for (int k = 0; k < U; ++k) x[k] = load(c + k * nth);
+      for (int k = 0; k < U; ++k) x[k] = load(min(c + k * nth, e - 1));
 #pragma unroll
-      for (int k = 0; k < U; ++k) s += sum(x[k], c + k * nth);
+      for (int k = 0; k < U; ++k) s += c + k * nth < e ? sum(x[k], c + k * nth) : 0.;
     }
-    for (; c < e; c += nth) s += sum(load(c), c);
     return s;
   }
+  // chunks [b, e) by one thread
+  __device__ __forceinline__ double run(int b, int e) const { return share(b, e, 0, 1); }
   // the refused tokens among chunks [b, e) as bits; by all threads
-  __device__ void refuse(const verify_tree& t, int n, int cur, uint32_t* lds, int b, int e) {
-    bit0 = b * E - shift;
-    const int count = (e - b) * E;
+  __device__ __forceinline__ void refuse(const verify_tree& t, int n, int cur, uint32_t* lds, int b, int e) {
+    first = b;
+    const int bit0 = b * E - shift, count = (e - b) * E;
+    bool any = false;
+    for (int k = threadIdx.x; k < n; k += blockDim.x) {
+      const int x = t.tok[k] - bit0;
+      any |= t.par[k] == cur && t.tok[k] >= 0 && x >= 0 && x < count;
+    }
+    bits = nullptr;
+    if (!__syncthreads_or(any)) return;            // none of them lies here
     for (int k = threadIdx.x; k < (count + 31) / 32; k += blockDim.x) lds[k] = 0;
     __syncthreads();
     for (int k = threadIdx.x; k < n; k += blockDim.x) {
@@ -247,217 +282,119 @@ __device__ __forceinline__ int stretch_begin(int chunks, int stretches, int g) {
   return (int)((int64_t)chunks * g / stretches);
 }
 
-template <typename T>
-__global__ __launch_bounds__(SUM_THREADS) void verify_sum_kernel(const verify_args a, int launch) {
-  extern __shared__ __align__(16) char lds[];
-  __shared__ double part[SUM_THREADS / 64];
-  __shared__ verify_state shared;
-  const int seq = blockIdx.x, g = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  int32_t* const acc = a.accepted + (int64_t)seq * a.width;
-  int64_t* const out = a.out_tokens + (int64_t)seq * a.width;
-  const verify_tree t(lds, a.width);
-  int32_t* const path = (int32_t*)(lds + verify_tree::bytes(a.width));
+// What the end of a call shares in LDS.
+struct find_lds {
+  double part[SUM_THREADS / 64], before;
   verify_state st;
-  double s = 1.;
-  if (launch > 0) {
-    const int64_t before = (int64_t)(launch - 1) * a.num_seqs + seq;
-    st = a.states[before];
-    const double x = lane < a.stretches ? a.sums[before * a.stretches + lane] : 0.;
-    load_tree(a, t, seq, true);
-    if (st.n <= 0 || st.round >= 0) {              // this sequence's sum is there already
-      if (g == 0 && tid == 0) a.states[before + a.num_seqs] = st;
-      return;
-    }
-    s = sum64(x);
-  } else {
-    const int row0 = a.row_starts[seq], n = min(a.row_starts[seq + 1] - row0, a.width);
-    st = verify_state{0., 0, 1, 1, 0, row0, n, 0.f};
-    if (n > 0) load_tree<T>(a, t, row0, n);
-    if (g == 0)
-      for (int i = tid; i < a.width; i += SUM_THREADS) acc[i] = -1, out[i] = -1;
-    if (n <= 0) {
-      if (g == 0 && tid == 0) {
-        a.states[seq] = st;
-        a.num_accepted[seq] = 0;
-      }
-      return;
-    }
-  }
-  __syncthreads();
-  const int row0 = st.row0, n = st.n, len0 = launch > 0 ? st.len : 0;
-  if (wave == 0) {
-    if (launch == 0) {
-      st.u = t.u[0];
-      if (lane == 0) path[0] = 0;
-    }
-    walk(t, n, a.draft != nullptr, s, st, path, lane, launch);
-    if (lane == 0) shared = st;
-  }
-  __syncthreads();
-  st = shared;
-  verify_row<T> row(a, row0 + st.cur, st.a);
-  const int b = stretch_begin(row.chunks, a.stretches, g), e = stretch_begin(row.chunks, a.stretches, g + 1);
-  if (!a.draft) row.refuse(t, n, st.cur, (uint32_t*)(path + a.width), b, e);
-  const double x = sum64(row.share(b, e, tid, SUM_THREADS));
-  if (lane == 0) part[wave] = x;
-  __syncthreads();
-  if (tid == 0) {
-    double w = 0.;
-#pragma unroll
-    for (int k = 0; k < SUM_THREADS / 64; ++k) w += part[k];
-    a.sums[((int64_t)launch * a.num_seqs + seq) * a.stretches + g] = w;
-  }
-  if (g == 0) {
-    for (int i = len0 + tid; i < st.len; i += SUM_THREADS) {
-      acc[i] = path[i];
-      if (i > 0) out[i - 1] = a.tokens[row0 + path[i]];
-    }
-    if (tid == 0) a.states[(int64_t)launch * a.num_seqs + seq] = st;
-    if (launch == 0)
-      for (int i = tid; i < 5 * a.width; i += SUM_THREADS) a.nodes[(int64_t)seq * 5 * a.width + i] = t.tok[i];
-  }
-}
+  int32_t first, last;
+};
 
-// The last launch: the walk's rest where more sums are needed than there were launches, and the token.
-template <typename T>
-__global__ __launch_bounds__(FIND_THREADS) void verify_find_kernel(const verify_args a, int launches) {
-  extern __shared__ __align__(16) char lds[];
-  constexpr int NW = FIND_THREADS / 64, E = verify_row<T>::E;
-  __shared__ double part[NW], before_s;
-  __shared__ verify_state shared;
-  __shared__ int32_t first, last, token;
-  const int seq = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// The end of a call for one sequence, by a workgroup: the walk's rest where its last sum was not
+// the one for the token, and the token. `sum`: lane g's stretch g of the state's sum.
+template <typename T, bool DRAWN>
+__device__ __forceinline__ void verify_finish(const verify_args& a, int seq, verify_state st, double sum, const verify_tree& t,
+                              int32_t* path, uint32_t* bits, find_lds& f) {
+  constexpr int NT = SUM_THREADS, NW = NT / 64, E = verify_row<T, DRAWN>::E;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row0 = st.row0, n = st.n;
   int32_t* const acc = a.accepted + (int64_t)seq * a.width;
   int64_t* const out = a.out_tokens + (int64_t)seq * a.width;
-  verify_state st = a.states[(int64_t)(launches - 1) * a.num_seqs + seq];
-  const verify_tree t(lds, a.width);
-  int32_t* const path = (int32_t*)(lds + verify_tree::bytes(a.width));
-  uint32_t* const bits = (uint32_t*)(path + a.width);
-  // the sums: of launch 0 where there was no other, else where the state says
-  double sum = lane < a.stretches ? a.sums[(int64_t)seq * a.stretches + lane] : 0.;
-  if (!a.draft) load_tree(a, t, seq, false);
-  if (st.n <= 0) return;
-  const int row0 = st.row0, n = st.n;
-  const bool pending = st.round < 0;
-  if (launches > 1) {
-    const int r = pending ? launches - 1 : st.round;
-    sum = lane < a.stretches ? a.sums[((int64_t)r * a.num_seqs + seq) * a.stretches + lane] : 0.;
-    if (pending) load_tree(a, t, seq, true);
-  }
-  __syncthreads();
-  auto total = [&](double x) -> double {           // over the workgroup
+  auto total = [&](double x) __attribute__((always_inline)) -> double {           // over the workgroup
     x = sum64(x);
     __syncthreads();
-    if (lane == 0) part[wave] = x;
+    if (lane == 0) f.part[wave] = x;
     __syncthreads();
-    return sum64(lane < NW ? part[lane] : 0.);
+    return sum64(lane < NW ? f.part[lane] : 0.);
   };
   // the first of the threads' ranges that passes the border, x this thread's sum: its thread and
   // what lies before it; the last one that holds anything where none passes
-  auto pick = [&](double x, double border, double& before) -> int {
+  auto pick = [&](double x, double border, double& before) __attribute__((always_inline)) -> int {
     const double run = scan64<64>(x, lane);
     __syncthreads();
-    if (lane == 63) part[wave] = run;
-    if (tid == 0) first = FIND_THREADS, last = -1;
+    if (lane == 63) f.part[wave] = run;
+    if (tid == 0) f.first = NT, f.last = -1;
     __syncthreads();
-    const double head = scan64<NW>(lane < NW ? part[lane] : 0., lane);   // of the waves, inclusive
-    const double base = before + (wave ? __shfl(head, wave - 1) : 0.);
-    if (x > 0.) {
-      if (base + run > border) atomicMin(&first, tid);
-      atomicMax(&last, tid);
+    double base = before;
+#pragma unroll
+    for (int w = 0; w < NW - 1; ++w) base += w < wave ? f.part[w] : 0.;
+    const uint64_t past = __ballot(x > 0. && base + run > border), some = __ballot(x > 0.);
+    if (lane == 0 && some) {
+      if (past) atomicMin(&f.first, 64 * wave + __ffsll((unsigned long long)past) - 1);
+      atomicMax(&f.last, 64 * wave + 63 - __clzll((long long)some));
     }
     __syncthreads();
-    const int at = first < FIND_THREADS ? first : last;
-    if (tid == at) before_s = base + (run - x);
+    const int at = f.first < NT ? f.first : f.last;
+    if (tid == at) f.before = base + (run - x);
     __syncthreads();
-    before = before_s;
+    before = f.before;
     return at;
   };
 
+  const bool pending = DRAWN && st.round < 0;
   if (pending) {
-    // the rest of the walk by this workgroup alone
     double s = sum64(sum);
     const int len0 = st.len;
     for (;;) {
       if (wave == 0) {
-        walk(t, n, true, s, st, path, lane, launches);
-        if (lane == 0) shared = st;
+        walk(t, n, true, s, st, path, lane, 0);
+        if (lane == 0) f.st = st;
       }
       __syncthreads();
-      st = shared;
+      st = f.st;
       __syncthreads();
       if (st.round >= 0) break;
-      const verify_row<T> row(a, row0 + st.cur, st.a);
-      s = total(row.share(0, row.chunks, tid, FIND_THREADS));
+      const verify_row<T, DRAWN> row(a, row0 + st.cur, st.a);
+      s = total(row.share(0, row.chunks, tid, NT));
     }
-    for (int i = len0 + tid; i < st.len; i += FIND_THREADS) {
+    for (int i = len0 + tid; i < st.len; i += NT) {
       acc[i] = path[i];
       out[i - 1] = a.tokens[row0 + path[i]];
     }
   }
 
-  verify_row<T> row(a, row0 + st.cur, st.a);
+  verify_row<T, DRAWN> row(a, row0 + st.cur, st.a);
   const double u = (double)st.u;
   int b = 0, e = row.chunks;
   double before = 0., border = 0., w;
-  if (!pending) {                                  // the stretch, from its launch's sums
-    const double x = sum, run = scan64<64>(x, lane);
+  if (!pending) {                                  // the stretch
+    const double run = scan64<64>(sum, lane);
     w = __shfl(run, 63);
     border = u * w;
-    const uint64_t some = __ballot(x > 0.), past = __ballot(x > 0. && run > border);
+    const uint64_t some = __ballot(sum > 0.), past = __ballot(sum > 0. && run > border);
     if (w > 0.) {
       const int g = past ? __ffsll((unsigned long long)past) - 1 : 63 - __clzll((long long)some);
       b = stretch_begin(row.chunks, a.stretches, g), e = stretch_begin(row.chunks, a.stretches, g + 1);
-      before = __shfl(run - x, g);
-      if (!a.draft) row.refuse(t, n, st.cur, bits, b, e);
+      before = __shfl(run - sum, g);
+      if constexpr (!DRAWN) row.refuse(t, n, st.cur, bits, b, e);
     }
   } else {
-    w = total(row.share(b, e, tid, FIND_THREADS));
+    w = total(row.share(b, e, tid, NT));
     border = u * w;
   }
   if (!(w > 0.)) {                                 // nothing is left: the row as it is
-    row.q = nullptr;
-    row.bits = nullptr;
-    w = total(row.share(b, e, tid, FIND_THREADS));
+    row.whole();
+    w = total(row.share(b, e, tid, NT));
     border = u * w;
   }
   int next = -1;
   if (w > 0.) {
     // by waves of neighbouring chunks, until a thread has a few neighbouring chunks of its own
-    while (e - b > FIND_THREADS * FIND_CHUNKS) {
+    while (e - b > NT * FIND_CHUNKS) {
       const int step = (e - b + NW - 1) / NW, wb = min(e, b + wave * step), we = min(e, wb + step);
       const double x = sum64(row.share(wb, we, lane, 64));
       const int at = pick(lane == 0 ? x : 0., border, before) >> 6;
       b = min(e, b + at * step);
       e = min(e, b + step);
     }
-    const int step = (e - b + FIND_THREADS - 1) / FIND_THREADS;
+    const int step = (e - b + NT - 1) / NT;
     const int tb = min(e, b + tid * step), te = min(e, tb + step);
-    typename verify_row<T>::chunk x[FIND_CHUNKS];
-#pragma unroll
-    for (int k = 0; k < FIND_CHUNKS; ++k) x[k] = row.load(min(tb + k, row.chunks - 1));
-    double mine = 0.;
-#pragma unroll
-    for (int k = 0; k < FIND_CHUNKS; ++k) mine += tb + k < te ? row.sum(x[k], tb + k) : 0.;
-    const int at = pick(mine, border, before);
-    if (tid == at) {
-      int found = -1;
-      double run = before;
-#pragma unroll
-      for (int k = 0; k < FIND_CHUNKS; ++k)
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-          const int c = tb + k;
-          const double y = c < te ? row.weight(x[k], c, j, true) : 0.;
-          if (y > 0. && (found < 0 || !(run > border))) {
-            run += y;
-            found = c * E - row.shift + j;         // the last one so far; the first that passes stays
-          }
-        }
-      token = found;
+    const int at = pick(row.run(tb, te), border, before);
+    // that thread's tokens, one a lane
+    if (wave == 0) {
+      const int tb0 = min(e, b + at * step), te0 = min(e, tb0 + step), i = tb0 * E - row.shift + lane;
+      const double y = i < te0 * E - row.shift ? row.weight(i) : 0., run = before + scan64<64>(y, lane);
+      const uint64_t some = __ballot(y > 0.), past = __ballot(y > 0. && run > border);
+      if (some) next = tb0 * E - row.shift + (past ? __ffsll((unsigned long long)past) - 1 : 63 - __clzll((long long)some));
     }
-    __syncthreads();
-    next = token;
   }
   if (tid == 0) {
     out[st.len - 1] = (int64_t)next;
@@ -465,19 +402,162 @@ __global__ __launch_bounds__(FIND_THREADS) void verify_find_kernel(const verify_
   }
 }
 
-// Workgroups of a sequence: about four per CU over the batch, and few enough tokens for the bits.
+// END: the last sum launch of a call with arrival counters; it ends the call.
+template <typename T, bool DRAWN, bool END>
+__global__ __launch_bounds__(SUM_THREADS) void verify_sum_kernel(const verify_args a, int launch) {
+  extern __shared__ __align__(16) char lds[];
+  __shared__ find_lds f;
+  const int seq = blockIdx.x, g = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  int32_t* const acc = a.accepted + (int64_t)seq * a.width;
+  int64_t* const out = a.out_tokens + (int64_t)seq * a.width;
+  const verify_tree t(lds, a.width);
+  int32_t* const path = (int32_t*)(lds + verify_tree::bytes(a.width));
+  uint32_t* const bits = (uint32_t*)(path + a.width);
+  verify_state st;
+  double s = 1., y = 0.;       // the sum that the walk goes on with; lane g's stretch g of the sum for the token
+  bool summed = false;         // that one is there already
+  if (launch > 0) {
+    const int64_t before = (int64_t)(launch - 1) * a.num_seqs + seq;
+    st = a.states[before];
+    const double x = lane < a.stretches ? a.sums[before * a.stretches + lane] : 0.;
+    load_tree(a, t, seq, true);
+    summed = st.n <= 0 || st.round >= 0;
+    if (summed) {
+      if (g != 0) return;
+      if (!END && tid == 0) a.states[before + a.num_seqs] = st;
+      if (!END || st.n <= 0) return;
+      if (lane < a.stretches) y = a.sums[((int64_t)st.round * a.num_seqs + seq) * a.stretches + lane];
+    }
+    s = sum64(x);
+  } else {
+    const int row0 = a.row_starts[seq], n = min(a.row_starts[seq + 1] - row0, a.width);
+    st = verify_state{0., 0, 1, 1, 0, row0, n, 0.f};
+    if (n > 0) load_tree<T>(a, t, row0, n);
+    if (n <= 0) {
+      if (g == 0) {
+        for (int i = tid; i < a.width; i += SUM_THREADS) acc[i] = -1, out[i] = -1;
+        if (tid == 0) {
+          a.states[seq] = st;
+          a.num_accepted[seq] = 0;
+        }
+      }
+      return;
+    }
+  }
+  __syncthreads();
+  if (!summed) {
+    const int row0 = st.row0, n = st.n, len0 = launch > 0 ? st.len : 0;
+    if (wave == 0) {
+      if (launch == 0) {
+        st.u = t.u[0];
+        if (lane == 0) path[0] = 0;
+      }
+      walk(t, n, DRAWN, s, st, path, lane, launch);
+      if (lane == 0) f.st = st;
+    }
+    __syncthreads();
+    st = f.st;
+    verify_row<T, DRAWN> row(a, row0 + st.cur, st.a);
+    const int b = stretch_begin(row.chunks, a.stretches, g), e = stretch_begin(row.chunks, a.stretches, g + 1);
+    if constexpr (!DRAWN) row.refuse(t, n, st.cur, bits, b, e);
+    const double x = sum64(row.share(b, e, tid, SUM_THREADS));
+    if (lane == 0) f.part[wave] = x;
+    __syncthreads();
+    double* const sums = a.sums + ((int64_t)launch * a.num_seqs + seq) * a.stretches;
+    if (tid == 0) {
+      double w = 0.;
+#pragma unroll
+      for (int k = 0; k < SUM_THREADS / 64; ++k) w += f.part[k];
+      if constexpr (END) {
+        // past the L2s, which the XCDs do not share, and there before the arrival counts
+        __hip_atomic_store((uint64_t*)&sums[g], __builtin_bit_cast(uint64_t, w), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const uint32_t before = __hip_atomic_fetch_add(&a.arrivals[seq], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        f.first = before == (uint32_t)a.stretches - 1;
+        if (f.first) __hip_atomic_store(&a.arrivals[seq], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      } else {
+        sums[g] = w;
+      }
+    }
+    bool writes = g == 0;                          // of all workgroups, which went the same way
+    if constexpr (END) {
+      __syncthreads();
+      if (!f.first) return;                        // the last one to arrive ends the call, and writes all of it
+      writes = true;
+    }
+    if (writes) {
+      if (launch == 0)
+        for (int i = tid; i < a.width; i += SUM_THREADS) {
+          if (i >= st.len) acc[i] = -1, out[i] = -1;
+          else if (i == st.len - 1 && !END) out[i] = -1;
+        }
+      for (int i = len0 + tid; i < st.len; i += SUM_THREADS) {
+        acc[i] = path[i];
+        if (i > 0) out[i - 1] = a.tokens[row0 + path[i]];
+      }
+    }
+    if constexpr (END) {
+      if (lane < a.stretches)
+        y = __builtin_bit_cast(double, __hip_atomic_load((uint64_t*)&sums[lane], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
+    } else if (g == 0) {
+      if (tid == 0) a.states[(int64_t)launch * a.num_seqs + seq] = st;
+      if (launch == 0)
+        for (int i = tid; i < 5 * a.width; i += SUM_THREADS) a.nodes[(int64_t)seq * 5 * a.width + i] = t.tok[i];
+    }
+  }
+  if constexpr (END) {
+    __syncthreads();
+    verify_finish<T, DRAWN>(a, seq, st, y, t, path, bits, f);
+  }
+}
+
+// The end as a launch of its own, after `launches` sum launches.
+template <typename T, bool DRAWN>
+__global__ __launch_bounds__(SUM_THREADS) void verify_find_kernel(const verify_args a, int launches) {
+  extern __shared__ __align__(16) char lds[];
+  __shared__ find_lds f;
+  const int seq = blockIdx.x, lane = threadIdx.x & 63;
+  const verify_state st = a.states[(int64_t)(launches - 1) * a.num_seqs + seq];
+  const verify_tree t(lds, a.width);
+  int32_t* const path = (int32_t*)(lds + verify_tree::bytes(a.width));
+  // the sums: of launch 0 where there was no other, else where the state says
+  double sum = lane < a.stretches ? a.sums[(int64_t)seq * a.stretches + lane] : 0.;
+  if constexpr (!DRAWN) load_tree(a, t, seq, false);
+  if (st.n <= 0) return;
+  const bool pending = st.round < 0;
+  if (launches > 1) {
+    const int r = pending ? launches - 1 : st.round;
+    sum = lane < a.stretches ? a.sums[((int64_t)r * a.num_seqs + seq) * a.stretches + lane] : 0.;
+  }
+  if (pending) load_tree(a, t, seq, true);
+  __syncthreads();
+  verify_finish<T, DRAWN>(a, seq, st, sum, t, path, (uint32_t*)(path + a.width), f);
+}
+
+// Workgroups of a sequence: about four per CU over the batch, few enough tokens for the end's threads
+// (one step of FIND_CHUNKS chunks each, 16-byte chunks of fp32) and for the bits.
 static int verify_stretches(int num_seqs, int vocab) {
-  const int want = std::min(1024 / std::max(num_seqs, 1), std::max(vocab / 1024, 1));
-  return std::min(std::max({want, (vocab + MAX_STRETCH - 1) / MAX_STRETCH, 1}), MAX_STRETCHES);
+  const int fill = std::min(1024 / std::max(num_seqs, 1), std::max(vocab / 1024, 1));
+  const int once = (vocab + SUM_THREADS * FIND_CHUNKS * 4 - 64) / (SUM_THREADS * FIND_CHUNKS * 4 - 64);
+  const int bits = (vocab + MAX_STRETCH - 1) / MAX_STRETCH;
+  return std::min(std::max({fill, std::min(once, 32), bits, 1}), MAX_STRETCHES);
+}
+
+template <typename T, bool DRAWN>
+static void launch_verify_as(const verify_args& a, int rounds, hipStream_t stream) {
+  const int per = (a.vocab + 16 + a.stretches - 1) / a.stretches + 16;   // tokens of a stretch, at most
+  const size_t lds = verify_tree::bytes(a.width) + 4 * (size_t)a.width + (DRAWN ? 0 : (size_t)(per / 32 + 1) * 4);
+  const dim3 grid(a.num_seqs, a.stretches), block(SUM_THREADS);
+  for (int r = 0; r < rounds + (a.arrivals ? 0 : 1); ++r)
+    hipLaunchKernelGGL((verify_sum_kernel<T, DRAWN, false>), grid, block, lds, stream, a, r);
+  if (a.arrivals) hipLaunchKernelGGL((verify_sum_kernel<T, DRAWN, true>), grid, block, lds, stream, a, rounds);
+  else hipLaunchKernelGGL((verify_find_kernel<T, DRAWN>), dim3(a.num_seqs), block, lds, stream, a, rounds + 1);
 }
 
 template <typename T>
 static void launch_verify(const verify_args& a, int rounds, hipStream_t stream) {
-  const int per = (a.vocab + 16 + a.stretches - 1) / a.stretches + 16;   // tokens of a stretch, at most
-  const size_t lds = verify_tree::bytes(a.width) + 4 * (size_t)a.width + (a.draft ? 0 : (size_t)(per / 32 + 1) * 4);
-  for (int r = 0; r <= rounds; ++r)
-    hipLaunchKernelGGL((verify_sum_kernel<T>), dim3(a.num_seqs, a.stretches), dim3(SUM_THREADS), lds, stream, a, r);
-  hipLaunchKernelGGL((verify_find_kernel<T>), dim3(a.num_seqs), dim3(FIND_THREADS), lds, stream, a, rounds + 1);
+  if (a.draft) launch_verify_as<T, true>(a, rounds, stream);
+  else launch_verify_as<T, false>(a, rounds, stream);
 }
 
 // The same walk for greedy targets: a child is kept where its token is the target's choice
@@ -564,7 +644,7 @@ extern "C" int32_t tb_tree_verify(const void* probs, int64_t probs_row_stride, c
                                   const float* uniforms, const int32_t* parents, const int32_t* row_starts,
                                   int32_t num_seqs, int32_t max_children, int32_t* accepted, int32_t* num_accepted,
                                   int64_t* out_tokens, int32_t width, void* workspace, size_t workspace_bytes,
-                                  hipStream_t stream) {
+                                  uint32_t* arrivals, int32_t arrival_units, hipStream_t stream) {
   using namespace tb;
   TB_CHECK_ARG(num_seqs >= 0 && vocab > 0 && width > 0 && max_children >= 0);
   TB_CHECK_ARG(dtype >= TB_DTYPE_F32 && dtype <= TB_DTYPE_BF16);
@@ -574,6 +654,7 @@ extern "C" int32_t tb_tree_verify(const void* probs, int64_t probs_row_stride, c
   TB_CHECK_ARG(probs_row_stride >= vocab && (!draft_probs || draft_row_stride >= vocab));
   TB_CHECK_ARG(workspace && ((uintptr_t)workspace & 7u) == 0 &&
                workspace_bytes >= tb_tree_verify_workspace_bytes(num_seqs, vocab, width));
+  TB_CHECK_ARG(!arrivals || (arrival_units >= num_seqs && ((uintptr_t)arrivals & 3u) == 0));
   const int stretches = verify_stretches(num_seqs, vocab);
   // sums that tests of later siblings need: none in a chain, or where the drafts were not drawn
   const int rounds = draft_probs ? std::min(std::max(max_children - 1, 0), MAX_ROUNDS) : 0;
@@ -581,7 +662,7 @@ extern "C" int32_t tb_tree_verify(const void* probs, int64_t probs_row_stride, c
   double* const sums = (double*)(states + (size_t)(MAX_ROUNDS + 1) * num_seqs);
   const verify_args a{probs, probs_row_stride, draft_probs, draft_row_stride, vocab, tokens, uniforms, parents,
                       row_starts, accepted, num_accepted, out_tokens, width, num_seqs, stretches, states,
-                      sums, (int32_t*)(sums + (size_t)(MAX_ROUNDS + 1) * num_seqs * stretches)};
+                      sums, (int32_t*)(sums + (size_t)(MAX_ROUNDS + 1) * num_seqs * stretches), arrivals};
   if (dtype == TB_DTYPE_F32) launch_verify<float>(a, rounds, stream);
   else if (dtype == TB_DTYPE_F16) launch_verify<_Float16>(a, rounds, stream);
   else launch_verify<__bf16>(a, rounds, stream);

@@ -18,7 +18,6 @@ verdict stays on the device and the commit reads it there.
 """
 from __future__ import annotations
 
-import contextlib
 import math
 from dataclasses import dataclass
 from typing import NamedTuple
@@ -66,6 +65,7 @@ class TreeMetadata:
     split_np: np.ndarray | None = None        # [rows of contexts cut into parts, 4]
     partial_slots: int = 0
     column_blocks: int = 1
+    units: int = 0                            # arrival counters of a call that joins its parts itself
     # device views (one backing buffer)
     device: torch.device | None = None
     parents: torch.Tensor | None = None
@@ -78,6 +78,7 @@ class TreeMetadata:
     slot_mapping: torch.Tensor | None = None
     work: torch.Tensor | None = None
     split: torch.Tensor | None = None
+    addresses: tuple | None = None            # of the arrays, in the order that the calls take them
 
     def to(self, device: torch.device) -> "TreeMetadata":
         """Upload every array with one host-to-device copy (views into one buffer)."""
@@ -111,6 +112,10 @@ class TreeMetadata:
         if has_cache:
             self.block_tables = self.block_tables.view(-1, self.max_blocks_per_seq)
         self.device = device
+        self.addresses = None
+        if has_cache:
+            self.addresses = (self.block_tables.data_ptr(), self.max_blocks_per_seq, self.row_starts.data_ptr(),
+                              self.cached.data_ptr(), self.num_seqs, self.row_seq.data_ptr(), self.num_rows)
         return self
 
 
@@ -140,7 +145,7 @@ def _attach_work(meta: TreeMetadata) -> None:
     """The work list of the step's attention calls (tb_build_tree_work)."""
     L = _lib.lib()
     nodes = np.diff(meta.row_starts_np).astype(np.int32)
-    counts = np.zeros(4, dtype=np.int32)
+    counts = np.zeros(5, dtype=np.int32)
     head = (meta.cached_np.ctypes.data, nodes.ctypes.data, meta.num_seqs, meta.num_heads, meta.num_kv_heads,
             meta.head_dim, _lib.DTYPE_CODE[meta.dtype], NUM_CUS, NUM_XCDS)
     _lib.check(L.tb_build_tree_work(*head, None, 0, None, 0, counts.ctypes.data), "tb_build_tree_work")
@@ -148,7 +153,7 @@ def _attach_work(meta: TreeMetadata) -> None:
     _lib.check(L.tb_build_tree_work(*head, work.ctypes.data, work.shape[0], split.ctypes.data, split.shape[0],
                                     counts.ctypes.data), "tb_build_tree_work")
     meta.work_np, meta.split_np = work, split
-    meta.partial_slots, meta.column_blocks = int(counts[2]), int(counts[3])
+    meta.partial_slots, meta.column_blocks, meta.units = int(counts[2]), int(counts[3]), int(counts[4])
 
 
 def build_tree_metadata(parents, cached_lens=None, block_tables=None, *, block_size: int = 0, num_blocks: int = 0,
@@ -238,11 +243,40 @@ def build_tree_metadata(parents, cached_lens=None, block_tables=None, *, block_s
     return meta
 
 
-def _on(device: torch.device):
-    """The launch's device made the current one where it is not."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+class _Scratch:
+    """What the calls on one stream of one device share, since they are ordered: a workspace, and
+    arrival counters (zero between calls: every call leaves them zero)."""
+
+    def __init__(self, device: torch.device):
+        self.workspace = torch.empty(1 << 20, dtype=torch.uint8, device=device)
+        self.arrivals = torch.zeros(4096, dtype=torch.int32, device=device)
+
+
+_SCRATCH: dict[tuple[int, int], _Scratch] = {}
+_KEPT_BYTES = 32 << 20       # larger workspaces are allocated call by call
+
+
+def _scratch(device: torch.device, stream: int, nbytes: int, units: int):
+    """(workspace, its bytes, arrival counters or None, their number) of a call on the current
+    stream. A call that is being captured gets a workspace of its own and no counters: its graph
+    may be replayed beside anything."""
+    if torch._C._cuda_isCurrentStreamCapturing():
+        return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes, None, 0
+    s = _SCRATCH.get((device.index, stream))
+    if s is None:
+        s = _SCRATCH[device.index, stream] = _Scratch(device)
+    if s.arrivals.shape[0] < units:
+        s.arrivals = torch.zeros(2 * units, dtype=torch.int32, device=device)
+    if nbytes > _KEPT_BYTES:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes, s.arrivals, units
+    if s.workspace.shape[0] < nbytes:
+        s.workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return s.workspace, nbytes, s.arrivals, units
+
+
+def _elsewhere(device: torch.device) -> bool:
+    """Whether the tensors' device is not the current one."""
+    return device.index != torch._C._cuda_getDevice()
 
 
 def _check_meta(meta: TreeMetadata, device: torch.device, cache: bool) -> None:
@@ -258,10 +292,11 @@ def tree_append(pool: torch.Tensor, k: torch.Tensor, v: torch.Tensor, meta: Tree
                 rope: Rope | None = None) -> None:
     """The nodes' K/V rows [T, kv_heads, head_dim] into their slots (ops.kv_append); with ``rope``
     k is the projection before rotation, rotated at cached + depth on the way."""
+    _lib.require_gpu_tensor("pool", pool)
     _check_meta(meta, pool.device, True)
     if pool.dim() == 5 and (pool.shape[3] != meta.block_size or pool.shape[0] < meta.num_blocks):
         raise ValueError(f"metadata is for {meta.num_blocks} blocks of {meta.block_size} positions")
-    with _on(pool.device):
+    with torch.cuda.device(pool.device):
         kv_append(pool, k, v, meta.slot_mapping, rope=rope, positions=meta.positions if rope is not None else None)
 
 
@@ -277,46 +312,53 @@ def tree_attention(q: torch.Tensor, pool: torch.Tensor, meta: TreeMetadata, *, s
     metadata's, for masks made on the device. A row that sees nothing gives 0.
     """
     nb, hkv, bs, d = _check_pool(pool)
-    _lib.require_gpu_tensor("q", q)
-    if q.device != pool.device:
-        raise ValueError(f"q is on {q.device}, the pool on {pool.device}")
-    _check_meta(meta, pool.device, True)
-    if q.dtype != pool.dtype or q.dtype != meta.dtype:
-        raise TypeError(f"q {q.dtype}, pool {pool.dtype} and metadata {meta.dtype} differ in dtype")
-    if (hkv, d, bs) != (meta.num_kv_heads, meta.head_dim, meta.block_size) or nb < meta.num_blocks:
+    device, dtype = pool.device, pool.dtype
+    if q.device != device:
+        _lib.require_gpu_tensor("q", q)
+        raise ValueError(f"q is on {q.device}, the pool on {device}")
+    _check_meta(meta, device, True)
+    if q.dtype != dtype or meta.dtype != dtype:
+        raise TypeError(f"q {q.dtype}, pool {dtype} and metadata {meta.dtype} differ in dtype")
+    if hkv != meta.num_kv_heads or d != meta.head_dim or bs != meta.block_size or nb < meta.num_blocks:
         raise ValueError(f"metadata is for {meta.num_blocks} blocks of {meta.block_size} positions, "
                          f"{meta.num_kv_heads} kv heads of {meta.head_dim}; the pool is {tuple(pool.shape)}")
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return tree_attention(q, pool, meta, scale=scale, out=out, rope=rope, mask=mask)
     hq, T = meta.num_heads, meta.num_rows
     qs = _rows_view("q", q, hq, d)
     if q.shape[0] != T:
         raise ValueError(f"q has {q.shape[0]} rows, metadata describes {T}")
     if out is None:
-        out = torch.empty(T, hq * d, device=q.device, dtype=q.dtype)
+        out, os_ = torch.empty(T, hq * d, device=device, dtype=dtype), hq * d
     else:
-        _lib.require_gpu_tensor("out", out)
-        if out.dtype != q.dtype or out.shape[0] != T or out.device != q.device:
+        if out.dtype != dtype or out.shape[0] != T or out.device != device:
             raise ValueError("out must match q's dtype, device and row count")
-    os_ = _rows_view("out", out, hq, d)
+        os_ = _rows_view("out", out, hq, d)
     if mask is None:
         mask = meta.mask
-    elif (mask.dtype != torch.int32 or mask.device != q.device or mask.shape != (T, meta.mask_words)
+    elif (mask.dtype != torch.int32 or mask.device != device or mask.shape != (T, meta.mask_words)
           or not mask.is_contiguous()):
-        raise TypeError(f"mask must be a contiguous int32 [{T}, {meta.mask_words}] tensor on {q.device}")
+        raise TypeError(f"mask must be a contiguous int32 [{T}, {meta.mask_words}] tensor on {device}")
+    cos = sin = positions = None
+    longest = 0
     if rope is not None:
-        rope.check(d, q.device)
-    ws = None
-    if meta.partial_slots:                   # from the caching allocator: each call, stream and graph its own
-        ws = torch.empty(meta.partial_slots * hq * (d + 2), device=q.device, dtype=torch.float32)
-    with _on(q.device):
-        st = _lib.lib().tb_tree_attention(
-            q.data_ptr(), qs, pool.data_ptr(), nb, out.data_ptr(), os_, meta.block_tables.data_ptr(),
-            meta.max_blocks_per_seq, meta.row_starts.data_ptr(), meta.cached.data_ptr(), meta.num_seqs,
-            meta.row_seq.data_ptr(), T, mask.data_ptr(), meta.mask_words, meta.work.data_ptr(),
-            meta.work_np.shape[0], meta.column_blocks, meta.split.data_ptr(), meta.split_np.shape[0],
-            meta.partial_slots, None if ws is None else ws.data_ptr(), 0 if ws is None else 4 * ws.numel(), hq, hkv, d, bs,
-            1.0 / math.sqrt(d) if scale is None else float(scale), _lib.DTYPE_CODE[q.dtype], meta.positions.data_ptr(),
-            None if rope is None else rope.cos.data_ptr(), None if rope is None else rope.sin.data_ptr(),
-            0 if rope is None else rope.max_position, _lib.stream_handle(q.device))
+        rope.check(d, device)
+        cos, sin, longest = rope.cos.data_ptr(), rope.sin.data_ptr(), rope.max_position
+        positions = meta.positions.data_ptr()
+    stream = _lib.stream_handle(device)
+    slots, units = meta.partial_slots, meta.units
+    ws = arrivals = None
+    ws_bytes = 0
+    if slots and bs >= 16:
+        ws, ws_bytes, arrivals, units = _scratch(device, stream, slots * hq * (d + 2) * 4, units)
+    st = _lib.lib().tb_tree_attention(
+        q.data_ptr(), qs, pool.data_ptr(), nb, out.data_ptr(), os_, *meta.addresses, mask.data_ptr(),
+        meta.mask_words, meta.work.data_ptr(), meta.work_np.shape[0], meta.column_blocks, meta.split.data_ptr(),
+        meta.split_np.shape[0], slots, None if ws is None else ws.data_ptr(), ws_bytes,
+        None if arrivals is None or not units else arrivals.data_ptr(), units, hq, hkv, d, bs,
+        1.0 / math.sqrt(d) if scale is None else float(scale), _lib.DTYPE_CODE[dtype], positions, cos, sin, longest,
+        stream)
     _lib.check(st, "tb_tree_attention")
     return out
 
@@ -335,6 +377,13 @@ def _verdict(meta: TreeMetadata, device: torch.device) -> TreeVerdict:
                        torch.empty(meta.num_seqs, width, dtype=torch.int64, device=device))
 
 
+def _vocab_rows(name: str, t: torch.Tensor, rows: int) -> int:
+    """The row stride of a [rows, vocab] tensor of contiguous rows."""
+    if t.dim() != 2 or t.shape[0] != rows or t.shape[1] < 1 or t.stride(1) != 1:
+        raise ValueError(f"{name} must be [{rows}, vocab] with contiguous rows, got {tuple(t.shape)}")
+    return t.stride(0) if rows > 1 else t.shape[1]
+
+
 def _node_values(name: str, t: torch.Tensor, dtype: torch.dtype, rows: int, device: torch.device) -> None:
     if t.dtype != dtype or t.device != device or t.shape != (rows,) or not t.is_contiguous():
         raise TypeError(f"{name} must be a contiguous {dtype} [{rows}] tensor on {device}")
@@ -351,35 +400,39 @@ def verify_tree(meta: TreeMetadata, tokens: torch.Tensor, uniforms: torch.Tensor
     that node r's children were drawn from, each independently; None for drafts that were not
     drawn at random (a draft model's most likely tokens).
     """
+    device, T, dtype = probs.device, meta.num_rows, probs.dtype
     _lib.require_gpu_tensor("probs", probs)
-    device, T = probs.device, meta.num_rows
     _check_meta(meta, device, False)
-    if probs.dtype not in _lib.DTYPE_CODE:
-        raise TypeError(f"unsupported probs dtype {probs.dtype}")
-    for name, t in (("probs", probs), ("draft_probs", draft_probs)):
-        if t is None:
-            continue
-        if t.dim() != 2 or t.shape != probs.shape or t.shape[0] != T or t.shape[1] < 1 or t.stride(1) != 1:
-            raise ValueError(f"{name} must be [{T}, vocab] with contiguous rows, got {tuple(t.shape)}")
-        if t.dtype != probs.dtype or t.device != device:
-            raise TypeError(f"{name} must share probs' dtype and device")
+    if dtype not in _lib.DTYPE_CODE:
+        raise TypeError(f"unsupported probs dtype {dtype}")
+    stride = _vocab_rows("probs", probs, T)
     vocab = probs.shape[1]
+    draft, draft_stride = None, 0
+    if draft_probs is not None:
+        if draft_probs.dtype != dtype or draft_probs.device != device:
+            raise TypeError("draft_probs must share probs' dtype and device")
+        draft_stride = _vocab_rows("draft_probs", draft_probs, T)
+        if draft_probs.shape[1] != vocab:
+            raise ValueError(f"draft_probs must be [{T}, {vocab}], got {tuple(draft_probs.shape)}")
+        draft = draft_probs.data_ptr()
     if vocab > MAX_VOCAB:
         raise ValueError(f"a vocabulary of {vocab} tokens; at most {MAX_VOCAB} are served")
     _node_values("tokens", tokens, torch.int64, T, device)
     _node_values("uniforms", uniforms, torch.float32, T, device)
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return verify_tree(meta, tokens, uniforms, probs, draft_probs)
     v = _verdict(meta, device)
-    L = _lib.lib()
-    ws = torch.empty(L.tb_tree_verify_workspace_bytes(meta.num_seqs, vocab, v.accepted.shape[1]), device=device, dtype=torch.uint8)
     if T == 0:
         return v._replace(accepted=v.accepted.fill_(-1), num_accepted=v.num_accepted.zero_(), tokens=v.tokens.fill_(-1))
-    with _on(device):
-        st = L.tb_tree_verify(
-            probs.data_ptr(), max(probs.stride(0), vocab), None if draft_probs is None else draft_probs.data_ptr(),
-            0 if draft_probs is None else max(draft_probs.stride(0), vocab), vocab, _lib.DTYPE_CODE[probs.dtype],
-            tokens.data_ptr(), uniforms.data_ptr(), meta.parents.data_ptr(), meta.row_starts.data_ptr(),
-            meta.num_seqs, meta.max_children, v.accepted.data_ptr(), v.num_accepted.data_ptr(), v.tokens.data_ptr(),
-            v.accepted.shape[1], ws.data_ptr(), ws.numel(), _lib.stream_handle(device))
+    L, B, width = _lib.lib(), meta.num_seqs, meta.max_nodes
+    stream = _lib.stream_handle(device)
+    ws, ws_bytes, arrivals, units = _scratch(device, stream, L.tb_tree_verify_workspace_bytes(B, vocab, width), B)
+    st = L.tb_tree_verify(
+        probs.data_ptr(), stride, draft, draft_stride, vocab, _lib.DTYPE_CODE[dtype], tokens.data_ptr(),
+        uniforms.data_ptr(), meta.parents.data_ptr(), meta.row_starts.data_ptr(), B, meta.max_children,
+        v.accepted.data_ptr(), v.num_accepted.data_ptr(), v.tokens.data_ptr(), width, ws.data_ptr(), ws_bytes,
+        None if arrivals is None else arrivals.data_ptr(), units, stream)
     _lib.check(st, "tb_tree_verify")
     return v
 
@@ -392,14 +445,15 @@ def verify_tree_greedy(meta: TreeMetadata, tokens: torch.Tensor, target_ids: tor
     _check_meta(meta, device, False)
     _node_values("target_ids", target_ids, torch.int64, T, device)
     _node_values("tokens", tokens, torch.int64, T, device)
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return verify_tree_greedy(meta, tokens, target_ids)
     v = _verdict(meta, device)
-    if T == 0:
-        return v._replace(accepted=v.accepted.fill_(-1), num_accepted=v.num_accepted.zero_(), tokens=v.tokens.fill_(-1))
-    with _on(device):
-        st = _lib.lib().tb_tree_verify_greedy(
-            target_ids.data_ptr(), tokens.data_ptr(), meta.parents.data_ptr(), meta.row_starts.data_ptr(),
-            meta.num_seqs, v.accepted.data_ptr(), v.num_accepted.data_ptr(), v.tokens.data_ptr(),
-            v.accepted.shape[1], _lib.stream_handle(device))
+    st = _lib.lib().tb_tree_verify_greedy(
+        meta.row_starts.data_ptr() if T == 0 else target_ids.data_ptr(),     # no rows: nothing is read
+        meta.row_starts.data_ptr() if T == 0 else tokens.data_ptr(), meta.parents.data_ptr(),
+        meta.row_starts.data_ptr(), meta.num_seqs, v.accepted.data_ptr(), v.num_accepted.data_ptr(),
+        v.tokens.data_ptr(), v.accepted.shape[1], _lib.stream_handle(device))
     _lib.check(st, "tb_tree_verify_greedy")
     return v
 
@@ -425,9 +479,11 @@ def commit_tree(storage: torch.Tensor, meta: TreeMetadata, accepted: torch.Tenso
             or accepted.shape[0] != B or accepted.shape[1] < 1 or not accepted.is_contiguous()):
         raise TypeError(f"accepted must be a contiguous int32 [{B}, nodes] tensor on {device}")
     _node_values("num_accepted", num_accepted, torch.int32, B, device)
-    with _on(device):
-        st = _lib.lib().tb_tree_commit(
-            storage.data_ptr(), layers, storage.stride(0) * storage.element_size(), nb, meta.block_tables.data_ptr(),
-            meta.max_blocks_per_seq, meta.cached.data_ptr(), B, accepted.data_ptr(), accepted.shape[1],
-            num_accepted.data_ptr(), hkv, d, bs, _lib.DTYPE_CODE[storage.dtype], _lib.stream_handle(device))
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return commit_tree(storage, meta, accepted, num_accepted)
+    st = _lib.lib().tb_tree_commit(
+        storage.data_ptr(), layers, storage.stride(0) * storage.element_size(), nb, meta.addresses[0],
+        meta.max_blocks_per_seq, meta.addresses[3], B, accepted.data_ptr(), accepted.shape[1],
+        num_accepted.data_ptr(), hkv, d, bs, _lib.DTYPE_CODE[storage.dtype], _lib.stream_handle(device))
     _lib.check(st, "tb_tree_commit")
