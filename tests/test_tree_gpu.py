@@ -568,6 +568,82 @@ def test_streams_and_graphs():
             assert all(torch.equal(x, y) for x, y in zip(got[1] + got[2], verdict + greedy)), f"replay {i}"
 
 
+@pytest.mark.parametrize("dtype,hq,hkv,d", [(torch.bfloat16, 14, 2, 64), (torch.float16, 16, 4, 64), (torch.bfloat16, 8, 4, 128),
+                                            (torch.float32, 4, 2, 64), (torch.float32, 6, 6, 128)])
+def test_parts_joined_here_and_by_a_launch(dtype, hq, hkv, d):
+    """Few parts of few columns are joined by the last workgroup to arrive in an eager call, by a launch in a
+    captured one: the same bits, the counters back at zero, calls one behind the other and of two streams."""
+    from tinybatch_amd.tree import _SCRATCH
+    vis = np.tril(np.ones((3, 3), dtype=bool))
+    vis[1] = False
+    cases = [Case(51, hq, hkv, d, dtype, [4], [600]), Case(52, hq, hkv, d, dtype, [3, 4, 1], [0, 700, 333], visible=[vis, None, None])]
+    made = [(c, c.meta(), c.q.to(DEV), c.pool.to(DEV)) for c in cases]
+    assert all(m.units for _, m, _, _ in made)         # these sizes take that way
+    want = []
+    for c, m, q, pool in made:
+        want.append(tree_attention(q, pool, m))
+        c.check(want[-1])
+    assert not want[1][1].any()                        # a row that sees nothing, whole or in parts
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for i in range(6):
+        got = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                got += [tree_attention(q, pool, m) for _, m, q, pool in (made if i % 2 else made[::-1])]
+        torch.cuda.synchronize()
+        for k, o in enumerate(got):
+            assert torch.equal(o, want[k % 2 if i % 2 else 1 - k % 2])
+    assert all(not s.arrivals.any() for s in _SCRATCH.values())
+    for (c, m, q, pool), w in zip(made, want):
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            out = tree_attention(q, pool, m)
+        for _ in range(3):
+            out.zero_()
+            assert torch.equal(tree_attention(q, pool, m), w)
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out, w)
+
+
+@pytest.mark.parametrize("drafts", [False, True])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_verify_ends_here_and_by_a_launch(dtype, drafts):
+    # the same of verification, whose captured calls end in a launch of their own
+    from tinybatch_amd.tree import _SCRATCH
+    for seed, sizes in ((61, [30, 1, 0, 12]), (62, [100, 70])):
+        case = verify_case(seed, sizes, 5003, dtype, drafts, sharp=2.0, noise=2.0)
+        meta = build_tree_metadata(case[0]).to(DEV)
+        args = [None if x is None else x.to(DEV) for x in case[1:]]
+        want = verify_tree(meta, *args)
+        check_verify(*case, want)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=s):
+            got = verify_tree(meta, *args)
+        for _ in range(3):
+            for t in got:
+                t.zero_()
+            again = verify_tree(meta, *args)
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) and torch.equal(x, z) for x, y, z in zip(want, got, again))
+    assert all(not s.arrivals.any() for s in _SCRATCH.values())
+
+
+def test_verify_with_a_hint_too_small():
+    # max_children only says how many launches sums get: a caller's mistake costs time, not the result
+    case = verify_case(63, [40, 9], 3001, torch.float32, True, sharp=3.0, noise=3.0)
+    meta = build_tree_metadata(case[0]).to(DEV)
+    for children in (0, 1, 2, 50):
+        meta.max_children = children
+        check_verify(*case, verify_tree(meta, *[x.to(DEV) for x in case[1:]]))
+
+
 def test_commit_replays_from_a_graph():
     hkv, d, bs = 2, 64, 16
     g = torch.Generator(device=DEV).manual_seed(5)
@@ -613,6 +689,14 @@ def test_calls_that_do_not_fit_are_refused():
         tree_attention(q, pool, meta, mask=meta.mask[:3])
     with pytest.raises(ValueError, match="out"):
         tree_attention(q, pool, meta, out=torch.empty(4, 384, device=DEV))
+    short = Rope(torch.zeros(31, 32, device=DEV), torch.zeros(31, 32, device=DEV))
+    with pytest.raises(IndexError, match="rope"):
+        tree_attention(q, pool, meta, rope=short)
+    from tinybatch_amd import tree_append
+    with pytest.raises(IndexError, match="rope"):
+        tree_append(pool, q[:, :2], q[:, 2:4], meta, rope=short)
+    with pytest.raises(RuntimeError, match="invalid"):           # rows that are not 16-byte aligned
+        tree_attention(torch.zeros(4, 385, dtype=torch.float16, device=DEV)[:, 1:], pool, meta)
     t, u, p = torch.zeros(4, dtype=torch.int64, device=DEV), torch.zeros(4, device=DEV), torch.zeros(4, 9, device=DEV)
     with pytest.raises(ValueError, match="probs"):
         verify_tree(meta, t, u, p[:3])

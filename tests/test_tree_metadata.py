@@ -72,6 +72,11 @@ def test_lists_that_do_not_fit_are_refused():
     with pytest.raises(ValueError, match="share a pool slot"):
         meta_of([[-1], [-1]], [3, 3], [[7], [7]])
     meta_of([[-1], [-1]], [16, 16], [[7, 8], [7, 9]])            # a shared prefix is fine
+    with pytest.raises(ValueError, match="another sequence's cached"):
+        meta_of([[-1], [-1]], [4, 9], [[7], [7]])                # the first's node would overwrite the second's position 4
+    with pytest.raises(ValueError, match="another sequence's cached"):
+        meta_of([[-1], []], [20, 32], [[6, 7], [5, 7]])
+    meta_of([[-1], []], [20, 20], [[6, 7], [5, 7]])              # behind what the other one has there
     with pytest.raises(ValueError, match=">= 0"):
         meta_of([[-1]], [-1], [[0]])
     with pytest.raises(ValueError, match="multiple"):

@@ -293,48 +293,62 @@ template <typename Tag, int D, int CW>
 __device__ __forceinline__ void tree_join_here(const tree_args& a, int row0, int cached, int nodes, int col0, int kvh,
                                                int first, int parts) {
   using T = typename elem<Tag>::type;
-  constexpr int QPC = D / 4, BATCH = 4;
+  constexpr int QPC = D / 4, BATCH = 8, ITEMS = 2;   // parts and columns of a thread in flight
   auto load2 = [](const float* p) {
     return __builtin_bit_cast(float2, __hip_atomic_load((const uint64_t*)p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT));
   };
-  for (int i = threadIdx.x; i < 32 * CW * QPC; i += 256) {
-    const int col = col0 + i / QPC, d4 = i % QPC;
-    if (col >= nodes * a.rep) break;
-    const int node = col / a.rep, head = kvh * a.rep + col - node * a.rep;
-    float M = -INFINITY, L = 0.f;
-    float4_t o = float4_t{0.f, 0.f, 0.f, 0.f};
+  const int items = min(32 * CW, nodes * a.rep - col0) * QPC;
+  for (int i0 = threadIdx.x; i0 < items; i0 += 256 * ITEMS) {
+    float M[ITEMS], L[ITEMS];
+    float4_t o[ITEMS];
+#pragma unroll
+    for (int t = 0; t < ITEMS; ++t) M[t] = -INFINITY, L[t] = 0.f, o[t] = float4_t{0.f, 0.f, 0.f, 0.f};
     for (int p0 = 0; p0 < parts; p0 += BATCH) {
-      float2 ml[BATCH], lo[BATCH], hi[BATCH];
+      float2 ml[ITEMS][BATCH], lo[ITEMS][BATCH], hi[ITEMS][BATCH];
 #pragma unroll
-      for (int k = 0; k < BATCH; ++k) {
-        const int64_t at = (int64_t)(first + min(p0 + k, parts - 1) * nodes + node) * a.num_heads + head;
-        ml[k] = load2(a.ws_ml + at * 2);
-        lo[k] = load2(a.ws_acc + at * D + 4 * d4);
-        hi[k] = load2(a.ws_acc + at * D + 4 * d4 + 2);
+      for (int t = 0; t < ITEMS; ++t) {
+        const int i = min(i0 + 256 * t, items - 1), col = col0 + i / QPC, node = col / a.rep;
+        const int head = kvh * a.rep + col - node * a.rep;
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+          const int64_t at = (int64_t)(first + min(p0 + k, parts - 1) * nodes + node) * a.num_heads + head;
+          ml[t][k] = load2(a.ws_ml + at * 2);
+          lo[t][k] = load2(a.ws_acc + at * D + 4 * (i % QPC));
+          hi[t][k] = load2(a.ws_acc + at * D + 4 * (i % QPC) + 2);
+        }
       }
-      float mb = M;
 #pragma unroll
-      for (int k = 0; k < BATCH; ++k) mb = fmaxf(mb, ml[k].x);
-      const float safe = mb == -INFINITY ? 0.f : mb, keep = fast_exp2(M - safe);
-      L *= keep;
-      o *= keep;
+      for (int t = 0; t < ITEMS; ++t) {
+        float mb = M[t];
 #pragma unroll
-      for (int k = 0; k < BATCH; ++k) {
-        if (p0 + k >= parts) break;
-        const float w = fast_exp2(ml[k].x - safe);   // 0 for a part that saw nothing
-        L = fmaf(ml[k].y, w, L);
-        o += float4_t{lo[k].x, lo[k].y, hi[k].x, hi[k].y} * w;
+        for (int k = 0; k < BATCH; ++k) mb = fmaxf(mb, ml[t][k].x);
+        const float safe = mb == -INFINITY ? 0.f : mb, keep = fast_exp2(M[t] - safe);
+        L[t] *= keep;
+        o[t] *= keep;
+#pragma unroll
+        for (int k = 0; k < BATCH; ++k) {
+          const float w = p0 + k < parts ? fast_exp2(ml[t][k].x - safe) : 0.f;   // 0 for a part that saw nothing
+          if (p0 + k < parts) {
+            L[t] = fmaf(ml[t][k].y, w, L[t]);
+            o[t] += float4_t{lo[t][k].x, lo[t][k].y, hi[t][k].x, hi[t][k].y} * w;
+          }
+        }
+        M[t] = mb;
       }
-      M = mb;
     }
-    const int row = row0 + node;
-    float inv = 1.f / L;
-    if (!(L > 0.f) && !tree_sees(a.mask + (int64_t)row * a.mask_words, cached, nodes)) inv = 0.f;
-    typedef T t4_t __attribute__((ext_vector_type(4)));
-    t4_t t;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) t[j] = (T)(o[j] * inv);
-    st_through(a.out + (int64_t)row * a.out_row_bytes + ((int64_t)head * D + 4 * d4) * sizeof(T), t);
+    for (int t = 0; t < ITEMS; ++t) {
+      const int i = i0 + 256 * t;
+      if (i >= items) break;
+      const int col = col0 + i / QPC, node = col / a.rep, head = kvh * a.rep + col - node * a.rep, row = row0 + node;
+      float inv = 1.f / L[t];
+      if (!(L[t] > 0.f) && !tree_sees(a.mask + (int64_t)row * a.mask_words, cached, nodes)) inv = 0.f;
+      typedef T t4_t __attribute__((ext_vector_type(4)));
+      t4_t x;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) x[j] = (T)(o[t][j] * inv);
+      st_through(a.out + (int64_t)row * a.out_row_bytes + ((int64_t)head * D + 4 * (i % QPC)) * sizeof(T), x);
+    }
   }
 }
 
@@ -848,9 +862,9 @@ struct tree_piece {
   int seq, kvh, chunk0, chunks, slot, groups, unit, order;   // order: part | parts << 16
 };
 
-// The most bytes of partials that a unit's last workgroup joins: a workgroup reads them at some 60 GB/s,
-// a launch of its own takes 2.5 us of the GPU and 3 us of the host.
-constexpr int64_t JOIN_HERE_BYTES = 192 << 10;
+// What a unit's last workgroup joins: 4 of a thread's columns in two steps, 16 parts in two more. Such a
+// join takes 2 to 4 us; a launch of its own 2.5 us of the GPU and 3 us of the host.
+constexpr int JOIN_HERE_FLOATS = 4096, JOIN_HERE_PARTS = 16;
 
 }  // namespace
 
@@ -899,7 +913,7 @@ extern "C" int32_t tb_build_tree_work(const int32_t* cached, const int32_t* node
                           parts > 1 ? (int)(slots + (int64_t)i * nodes[b]) : -1, groups, (int)(units + h * groups),
                           few ? i | parts << 16 : 0});
     if (parts > 1) {
-      here &= few && (int64_t)parts * std::min(cols, nodes[b] * rep) * head_dim * 4 <= JOIN_HERE_BYTES;
+      here &= parts <= JOIN_HERE_PARTS && std::min(cols, nodes[b] * rep) * head_dim <= JOIN_HERE_FLOATS;
       units += (int64_t)groups * num_kv_heads;
       for (int i = 0; i < nodes[b]; ++i, ++num_split)
         if (split && num_split < split_capacity) {

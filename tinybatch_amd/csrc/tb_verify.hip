@@ -110,55 +110,102 @@ __device__ __forceinline__ void load_tree(const verify_args& a, const verify_tre
   for (int i = threadIdx.x; i < (values ? 5 : 2) * a.width; i += blockDim.x) t.tok[i] = from[i];
 }
 
+// The walk's view of a tree: trees of up to 64 nodes in registers, lane i node i (a test then takes
+// some 100 cycles instead of 700), larger ones in LDS.
+template <bool SMALL>
+struct walk_nodes {
+  const verify_tree& t;
+  int n, lane, par, tok;
+  float p, q, u;
+  __device__ __forceinline__ walk_nodes(const verify_tree& t_, int n_, int lane_) : t(t_), n(n_), lane(lane_) {
+    if constexpr (SMALL) {
+      const int i = min(lane, n - 1);
+      par = lane < n ? t.par[i] : -2;
+      tok = t.tok[i], p = t.p[i], q = t.q[i], u = t.u[i];
+    }
+  }
+  static __device__ __forceinline__ float at(float x, int i) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i));
+  }
+  __device__ __forceinline__ void get(int i, int& x, double& p_, double& q_, double& u_) const {
+    if constexpr (SMALL)
+      x = __builtin_amdgcn_readlane(tok, i), p_ = (double)at(p, i), q_ = (double)at(q, i), u_ = (double)at(u, i);
+    else
+      x = t.tok[i], p_ = (double)t.p[i], q_ = (double)t.q[i], u_ = (double)t.u[i];
+  }
+  // the first child of `cur` from row `from` on, or n
+  __device__ __forceinline__ int child(int cur, int from) const {
+    if constexpr (SMALL) {
+      const uint64_t hit = __ballot(par == cur && lane >= from);
+      return hit ? __ffsll((unsigned long long)hit) - 1 : n;
+    } else {
+      for (int i0 = from & ~63; i0 < n; i0 += 64) {
+        const int i = i0 + lane;
+        const uint64_t hit = __ballot(i < n && i >= from && t.par[i < n ? i : 0] == cur);
+        if (hit) return i0 + __ffsll((unsigned long long)hit) - 1;
+      }
+      return n;
+    }
+  }
+  // whether a child of `cur` in rows [from, to) holds token x
+  __device__ __forceinline__ bool holds(int cur, int x, int from, int to) const {
+    if constexpr (SMALL) {
+      return __ballot(par == cur && tok == x && lane >= from && lane < to) != 0;
+    } else {
+      bool any = false;
+      for (int i0 = from & ~63; i0 < to; i0 += 64) {
+        const int k = i0 + lane;
+        any |= __ballot(k < to && k >= from && t.par[k < n ? k : 0] == cur && t.tok[k < n ? k : 0] == x) != 0;
+      }
+      return any;
+    }
+  }
+};
+
 // The walk from a state on, by one wave, until the path ends or a sum is needed; `s` is the sum
 // at st.a. Nodes kept are written to path[] (LDS) as they come.
-__device__ __forceinline__ void walk(const verify_tree& t, int n, bool drawn, double s, verify_state& st,
-                                     int32_t* path, int lane, int launch) {
-  auto child = [&](int from) __attribute__((always_inline)) -> int {              // the next child of st.cur from row `from` on, or n
-    for (int i0 = from & ~63; i0 < n; i0 += 64) {
-      const int i = i0 + lane;
-      const uint64_t hit = __ballot(i < n && i >= from && t.par[i < n ? i : 0] == st.cur);
-      if (hit) return i0 + __ffsll((unsigned long long)hit) - 1;
-    }
-    return n;
-  };
-  int i = child(st.next), first = i;               // `first`: st.cur's first child, where refused tokens start
-  for (;;) {
-    st.round = launch;
-    st.next = i;
-    if (i >= n) return;                            // every child refused, or none: the path ends at st.cur
-    const double u = (double)t.u[i], p = (double)t.p[i], q = (double)t.q[i];
+template <bool SMALL>
+__device__ __forceinline__ void walk_as(const verify_tree& t, int n, bool drawn, double s, verify_state& st,
+                                        int32_t* path, int lane, int launch) {
+  const walk_nodes<SMALL> nodes(t, n, lane);
+  int cur = __builtin_amdgcn_readfirstlane(st.cur);
+  int i = nodes.child(cur, __builtin_amdgcn_readfirstlane(st.next)), first = i;   // cur's first child: refused tokens start there
+  st.round = launch;
+  while (i < n) {                                  // else every child refused, or none: the path ends at cur
+    int x;
+    double p, q, u;
+    nodes.get(i, x, p, q, u);
     bool keep;
     if (drawn) {
       keep = u * q * s < p - st.a * q;
     } else {
-      // a token refused before holds nothing
-      const int x = t.tok[i];
-      bool again = false;
-      for (int i0 = first & ~63; i0 < i; i0 += 64) {
-        const int k = i0 + lane;
-        again |= __ballot(k < i && k >= first && t.par[k] == st.cur && t.tok[k] == x) != 0;
-      }
+      const bool again = nodes.holds(cur, x, first, i);   // a token refused before holds nothing
       keep = !again && p > 0. && u * s < p;
       if (!keep && !again && p > 0.) s -= p;
     }
-    if (keep) {
-      st.cur = i;
+    if (__builtin_amdgcn_readfirstlane(keep)) {
+      cur = i;
       st.a = 0.;
       s = 1.;
       if (lane == 0) path[st.len] = i;
       ++st.len;
-      i = first = child(i + 1);
+      i = first = nodes.child(cur, i + 1);
     } else {
-      i = child(i + 1);
-      if (drawn) {
+      i = nodes.child(cur, i + 1);
+      if (drawn) {                                 // the sum at the new a: for the next test or for the token
         st.a += s;
-        st.next = i;
-        st.round = i < n ? -1 : launch;
-        return;                                    // the sum at the new a: for the next test or for the token
+        if (i < n) st.round = -1;
+        break;
       }
     }
   }
+  st.cur = cur;
+  st.next = i;
+}
+__device__ __forceinline__ void walk(const verify_tree& t, int n, bool drawn, double s, verify_state& st,
+                                     int32_t* path, int lane, int launch) {
+  if (n <= 64) walk_as<true>(t, n, drawn, s, st, path, lane, launch);
+  else walk_as<false>(t, n, drawn, s, st, path, lane, launch);
 }
 
 // A row of the vocabulary in 16-byte chunks of the memory it lies in: chunk c holds tokens
@@ -254,8 +301,6 @@ struct verify_row {
     }
     return s;
   }
-  // chunks [b, e) by one thread
-  __device__ __forceinline__ double run(int b, int e) const { return share(b, e, 0, 1); }
   // the refused tokens among chunks [b, e) as bits; by all threads
   __device__ __forceinline__ void refuse(const verify_tree& t, int n, int cur, uint32_t* lds, int b, int e) {
     first = b;
@@ -287,6 +332,7 @@ struct find_lds {
   double part[SUM_THREADS / 64], before;
   verify_state st;
   int32_t first, last;
+  double chunk[SUM_THREADS * FIND_CHUNKS];         // sums of the stretch's chunks
 };
 
 // The end of a call for one sequence, by a workgroup: the walk's rest where its last sum was not
@@ -385,9 +431,21 @@ __device__ __forceinline__ void verify_finish(const verify_args& a, int seq, ver
       b = min(e, b + at * step);
       e = min(e, b + step);
     }
+    // the chunks' sums, read side by side, then summed by threads of neighbouring ones
+    constexpr int U = 4;
+    for (int c = b + tid; c < e; c += U * NT) {
+      typename verify_row<T, DRAWN>::chunk x[U];
+#pragma unroll
+      for (int k = 0; k < U; ++k) x[k] = row.load(min(c + k * NT, e - 1));
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (c + k * NT < e) f.chunk[c + k * NT - b] = row.sum(x[k], c + k * NT);
+    }
+    __syncthreads();
     const int step = (e - b + NT - 1) / NT;
-    const int tb = min(e, b + tid * step), te = min(e, tb + step);
-    const int at = pick(row.run(tb, te), border, before);
+    double mine = 0.;
+    for (int c = tid * step; c < min(e - b, (tid + 1) * step); ++c) mine += f.chunk[c];
+    const int at = pick(mine, border, before);
     // that thread's tokens, one a lane
     if (wave == 0) {
       const int tb0 = min(e, b + at * step), te0 = min(e, tb0 + step), i = tb0 * E - row.shift + lane;

@@ -19,7 +19,7 @@ verdict stays on the device and the commit reads it there.
 from __future__ import annotations
 
 import math
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from typing import NamedTuple
 
 import numpy as np
@@ -79,6 +79,8 @@ class TreeMetadata:
     work: torch.Tensor | None = None
     split: torch.Tensor | None = None
     addresses: tuple | None = None            # of the arrays, in the order that the calls take them
+    longest: int = 0                          # the largest RoPE position, plus one
+    verify_bytes: dict = field(default_factory=dict)   # workspace of verify_tree by vocabulary
 
     def to(self, device: torch.device) -> "TreeMetadata":
         """Upload every array with one host-to-device copy (views into one buffer)."""
@@ -233,12 +235,21 @@ def build_tree_metadata(parents, cached_lens=None, block_tables=None, *, block_s
     slots = tables[seq, pos // block_size].astype(np.int64) * block_size + pos % block_size
     if np.unique(slots).size != T:
         raise ValueError("two nodes of the step share a pool slot: give each tree blocks of its own")
+    # a node's row must not fall on another sequence's cached positions: in its block those reach
+    # from offset 0 up to its cached length, the nodes from some offset on
+    first_node = np.full(num_blocks, block_size, dtype=np.int64)
+    np.minimum.at(first_node, tables[seq, pos // block_size], pos % block_size)
+    covered = np.clip(cached[:, None] - block_size * np.arange(max_nb), 0, block_size)
+    if (covered > first_node[tables]).any():
+        raise ValueError("a tree's nodes fall on another sequence's cached positions: give each tree blocks of its own "
+                         "behind a shared prefix of whole blocks")
     if T and slots.max() > np.iinfo(np.int32).max:
         raise ValueError("a pool of more than 2^31 slots")
     meta.cached_np = cached.astype(np.int32)
     meta.block_tables_np = tables
     meta.max_blocks_per_seq = max_nb
     meta.slot_mapping_np = slots.astype(np.int32)
+    meta.longest = int((cached[seq] + meta.depths_np).max()) + 1 if T else 0
     _attach_work(meta)
     return meta
 
@@ -288,6 +299,12 @@ def _check_meta(meta: TreeMetadata, device: torch.device, cache: bool) -> None:
         raise ValueError("metadata was built without cached_lens and block_tables")
 
 
+def _check_rope(rope: Rope, meta: TreeMetadata, head_dim: int, device: torch.device) -> None:
+    rope.check(head_dim, device)
+    if rope.max_position < meta.longest:
+        raise IndexError(f"rope tables of {rope.max_position} positions, the step's nodes reach {meta.longest}")
+
+
 def tree_append(pool: torch.Tensor, k: torch.Tensor, v: torch.Tensor, meta: TreeMetadata,
                 rope: Rope | None = None) -> None:
     """The nodes' K/V rows [T, kv_heads, head_dim] into their slots (ops.kv_append); with ``rope``
@@ -296,6 +313,8 @@ def tree_append(pool: torch.Tensor, k: torch.Tensor, v: torch.Tensor, meta: Tree
     _check_meta(meta, pool.device, True)
     if pool.dim() == 5 and (pool.shape[3] != meta.block_size or pool.shape[0] < meta.num_blocks):
         raise ValueError(f"metadata is for {meta.num_blocks} blocks of {meta.block_size} positions")
+    if rope is not None:
+        _check_rope(rope, meta, pool.shape[-1], pool.device)
     with torch.cuda.device(pool.device):
         kv_append(pool, k, v, meta.slot_mapping, rope=rope, positions=meta.positions if rope is not None else None)
 
@@ -343,7 +362,7 @@ def tree_attention(q: torch.Tensor, pool: torch.Tensor, meta: TreeMetadata, *, s
     cos = sin = positions = None
     longest = 0
     if rope is not None:
-        rope.check(d, device)
+        _check_rope(rope, meta, d, device)
         cos, sin, longest = rope.cos.data_ptr(), rope.sin.data_ptr(), rope.max_position
         positions = meta.positions.data_ptr()
     stream = _lib.stream_handle(device)
@@ -427,7 +446,10 @@ def verify_tree(meta: TreeMetadata, tokens: torch.Tensor, uniforms: torch.Tensor
         return v._replace(accepted=v.accepted.fill_(-1), num_accepted=v.num_accepted.zero_(), tokens=v.tokens.fill_(-1))
     L, B, width = _lib.lib(), meta.num_seqs, meta.max_nodes
     stream = _lib.stream_handle(device)
-    ws, ws_bytes, arrivals, units = _scratch(device, stream, L.tb_tree_verify_workspace_bytes(B, vocab, width), B)
+    need = meta.verify_bytes.get(vocab)
+    if need is None:
+        need = meta.verify_bytes[vocab] = L.tb_tree_verify_workspace_bytes(B, vocab, width)
+    ws, ws_bytes, arrivals, units = _scratch(device, stream, need, B)
     st = L.tb_tree_verify(
         probs.data_ptr(), stride, draft, draft_stride, vocab, _lib.DTYPE_CODE[dtype], tokens.data_ptr(),
         uniforms.data_ptr(), meta.parents.data_ptr(), meta.row_starts.data_ptr(), B, meta.max_children,
