@@ -29,7 +29,9 @@
 #include <algorithm>
 #include <cmath>
 #include <exception>
+#include <functional>
 #include <type_traits>
+#include <utility>
 #include <vector>
 
 #include "tb_stream.h"
@@ -810,50 +812,85 @@ static void launch_rows(const tree_args& a, int num_rows, int head_dim, hipStrea
 // ---- the work list (host, no device call) ------------------------------------------
 namespace {
 
-// What a work list costs, in proportions that were fitted to the times of 53 steps cut in every
-// way (12 geometries and types, 1 to 100 sequences, contexts of 300 to 30000 positions, 2 to 64 nodes): the
-// cut it picks is on average 2% slower than the best one. A round is a chunk of a workgroup.
+// What a work list costs, in us, fitted to the times of 61 steps cut in every way (14 geometries and
+// types, 1 to 100 sequences, contexts of 300 to 30000 positions, 2 to 64 nodes): the cut it picks is on
+// average 1.2% slower than the best one, 18% at most. A round is a chunk of a workgroup.
 struct tree_price {
   int chunks_round;            // chunks of 32 positions in a round
   int on_cu;                   // workgroups a CU holds
-  double full;                 // a CU's time for each round
+  double full;                 // a CU's time for each round of the workgroups it holds
   int cus;
+  double row_bytes;            // of a K or V row
 };
 
 // Chunks of a sequence's context.
 inline int tree_chunks(int cached, int nodes) { return nodes > 0 ? (cached + nodes + 31) / 32 : 0; }
 
+// A context of `chunks` in parts of up to `part` chunks (0: not cut), all of one length but the last: their
+// length, a multiple of a round.
+inline int tree_even(int chunks, int part, int round) {
+  const int parts = part > 0 ? (chunks + part - 1) / part : 1;
+  return ((chunks + parts - 1) / parts + round - 1) / round * round;
+}
+
 // The part length in rounds of least cost; 0: no context is cut.
 int tree_part_rounds(const tree_price& price, const int32_t* cached, const int32_t* nodes, int num_seqs, int rep,
                      int cols, int num_kv_heads, double slot_bytes) {
-  int longest = 0;
-  for (int b = 0; b < num_seqs; ++b) longest = std::max(longest, tree_chunks(cached[b], nodes[b]));
-  const int most = (longest + price.chunks_round - 1) / price.chunks_round;
+  constexpr double START = 3.7, START_ROUNDS = 2.4, ALONE = 1.4, BYTES_US = 7.2e6, JOIN = 0.65, JOIN_BATCH = 0.63,
+                   PARTIAL_BYTES_US = 3.3e6;
+  int most = 0;
+  double kv_bytes = 0;         // read; half as fast to come by where several workgroups read them
+  bool once = true;
+  for (int b = 0; b < num_seqs; ++b) {
+    most = std::max(most, (tree_chunks(cached[b], nodes[b]) + price.chunks_round - 1) / price.chunks_round);
+    kv_bytes += 64. * tree_chunks(cached[b], nodes[b]) * price.row_bytes * num_kv_heads;
+    once &= nodes[b] * rep <= cols;
+  }
+  std::vector<std::pair<int, int64_t>> pieces;   // (rounds, workgroups)
   auto cost = [&](int part) {
-    const int len = std::min(part, most);
-    double rounds = 0, wgs = 0, whole = 0, slots = 0;
+    pieces.clear();
+    int64_t count = 0;
+    double slots = 0;
+    int most_parts = 1;
     for (int b = 0; b < num_seqs; ++b) {
       if (nodes[b] <= 0) continue;
       const int r = (tree_chunks(cached[b], nodes[b]) + price.chunks_round - 1) / price.chunks_round;
-      const int groups = (nodes[b] * rep + cols - 1) / cols, parts = (r + part - 1) / part;
-      rounds += (double)r * groups * num_kv_heads;
-      wgs += (double)parts * groups * num_kv_heads;
-      whole += (double)(r / len) * groups * num_kv_heads;   // of the full length
-      if (parts > 1) slots += (double)parts * nodes[b];
+      const int even = tree_even(r, part, 1), parts = (r + even - 1) / even;
+      const int64_t wgs = (int64_t)((nodes[b] * rep + cols - 1) / cols) * num_kv_heads;
+      if (parts > 1) {
+        pieces.push_back({even, wgs * (parts - 1)});
+        slots += (double)parts * nodes[b];
+        most_parts = std::max(most_parts, parts);
+      }
+      pieces.push_back({r - even * (parts - 1), wgs});
+      count += wgs * parts;
     }
-    double t = len * 1.45 * price.full;          // the longest workgroup
-    if (wgs > price.cus) {                       // CUs shared: their work evened out, or whole turns of full workgroups
-      const double turn = len * price.full * price.on_cu;
-      t = std::max({t, (rounds * price.full + wgs * 1.5) / price.cus + 0.2 * turn,
-                    2.8 * turn * std::floor(whole / (price.cus * price.on_cu))});
+    // the longest first, each where a place is free first: a piece starts when those before it have
+    // filled the places evenly
+    std::sort(pieces.begin(), pieces.end(), std::greater<>());
+    const bool alone = count <= price.cus;
+    const double places = (double)price.cus * (alone ? 1 : price.on_cu);
+    double end = 0, work = 0, seen = 0;
+    for (const auto& [len, n] : pieces) {
+      const double one = len + START_ROUNDS;
+      const double first = seen < places ? 0 : work / places;
+      const double last = seen + n - 1 < places ? 0 : (work + (n - 1) * one) / places;
+      end = std::max(end, std::max(first, last) + one);
+      work += n * one;
+      seen += n;
     }
-    return 6.8 + t + (slots > 0 ? 2.3 + 2 * slots * slot_bytes / 2.3e6 : 0.);   // and the join
+    const double t = end * price.full * (alone ? ALONE : price.on_cu);
+    const double mem = kv_bytes / BYTES_US * (once ? 1. : 0.5);
+    double join = 0;
+    if (slots > 0)
+      join = JOIN + JOIN_BATCH * ((most_parts + 7) / (most_parts <= 16 ? 8 : 32)) + slots * slot_bytes / PARTIAL_BYTES_US;
+    return START + std::max(t, mem) + join;
   };
   int best = 0;
-  double least = cost(std::max(most, 1));
-  for (int part = 1; part < most; part += part < 8 ? 1 : part < 32 ? 4 : 16) {
+  double least = cost(0);
+  for (int part = 1; part < most; part += part < 6 ? 1 : part < 16 ? 2 : part < 32 ? 4 : part < 48 ? 8 : part < 96 ? 16 : 32) {
     const double c = cost(part);
-    if (c < 0.97 * least) least = c, best = part;
+    if (c < least) least = c, best = part;
   }
   return best;
 }
@@ -888,12 +925,12 @@ extern "C" int32_t tb_build_tree_work(const int32_t* cached, const int32_t* node
   TB_CHECK_ARG(rows < (1 << 30));
   const int row_bytes = head_dim * (dtype == TB_DTYPE_F32 ? 4 : 2);
   const int blocks = most_cols <= 32 && row_bytes == 128 ? 1 : most_cols <= 64 ? 2 : 4, cols = 32 * blocks;
-  const double full = dtype == TB_DTYPE_F32 ? (head_dim == 64 ? 3.6 : blocks == 2 ? 7.2 : 10.6)
-                      : head_dim == 128         ? 1.5
-                      : blocks == 1             ? 1.73
-                      : blocks == 2             ? 0.93
-                                                : 0.6;
-  const tree_price price{blocks == 1 ? 4 : 2, row_bytes == 512 ? 1 : 2, full, num_cus};
+  const double full = dtype == TB_DTYPE_F32 ? (head_dim == 64 ? (blocks == 2 ? 1.24 : 2.16) : blocks == 2 ? 2.92 : 5.54)
+                      : head_dim == 128     ? (blocks == 2 ? 0.8 : 1.04)
+                      : blocks == 1         ? 0.64
+                      : blocks == 2         ? 0.44
+                                            : 0.51;
+  const tree_price price{blocks == 1 ? 4 : 2, row_bytes == 512 ? 1 : 2, full, num_cus, (double)row_bytes};
   const int part = tree_part_rounds(price, cached, nodes, num_seqs, rep, cols, num_kv_heads,
                                     (double)num_heads * (head_dim + 2) * 4) * price.chunks_round;
   std::vector<tree_piece> pieces;
@@ -905,11 +942,12 @@ extern "C" int32_t tb_build_tree_work(const int32_t* cached, const int32_t* node
     row0 += nodes[b];
     const int all = tree_chunks(cached[b], nodes[b]);
     if (all == 0) continue;
-    const int parts = part ? (all + part - 1) / part : 1, groups = (nodes[b] * rep + cols - 1) / cols;
+    const int groups = (nodes[b] * rep + cols - 1) / cols, even = tree_even(all, part, price.chunks_round);
+    const int parts = (all + even - 1) / even;
     const bool few = parts < (1 << 15);
     for (int i = 0; i < parts; ++i)
       for (int h = 0; h < num_kv_heads; ++h)
-        pieces.push_back({b, h, part * i, part ? std::min(part, all - part * i) : all,
+        pieces.push_back({b, h, even * i, std::min(even, all - even * i),
                           parts > 1 ? (int)(slots + (int64_t)i * nodes[b]) : -1, groups, (int)(units + h * groups),
                           few ? i | parts << 16 : 0});
     if (parts > 1) {
