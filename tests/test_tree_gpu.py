@@ -6,6 +6,8 @@ h |out|; the weights that multiply V are rounded to the type (h each) and their 
 so 2 h sum p|v|; a score's fp32 sum of d products by (d + 4) 2^-24 sum|q k| (its weight by that
 relatively, and the sum of weights again), and the sums over the context by 2^-24 a term. Verification
 and commit are exact."""
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -461,6 +463,24 @@ def test_commit_moves_rows_and_nothing_else(dtype, hkv, d, bs):
     assert torch.equal(dev.cpu(), want)
 
 
+def test_commit_of_paths_that_are_none():
+    """Nodes outside the sequence's table, negative counts and counts past the row: what lies outside the
+    table is left out, no other block changes."""
+    parents, cached = [[-1, 0, 1], [-1, 0], [-1, 0, 0, 0]], [14, 32, 5]
+    tables = [[9, 4], [2, 7, 5], [11]]
+    storage = torch.randn(2, 13, 2, 2, 16, 64, generator=torch.Generator().manual_seed(3))
+    acc = torch.tensor([[0, 2, 2 ** 31 - 1, 2 ** 30], [0, 1, -2 ** 31, 10 ** 6], [0, 3, 40, -7]], dtype=torch.int32)
+    num = torch.tensor([4, -3, 2 ** 31 - 1], dtype=torch.int32)
+    want = storage.clone()
+    want[:, 9, :, :, 15] = storage[:, 4, :, :, 0]      # positions 16 and 8 to 15 and 6
+    want[:, 11, :, :, 6] = storage[:, 11, :, :, 8]
+    meta = build_tree_metadata(parents, cached, tables, block_size=16, num_blocks=13, num_heads=2, num_kv_heads=2,
+                               head_dim=64, dtype=torch.float32).to(DEV)
+    dev = storage.to(DEV)
+    commit_tree(dev, meta, acc.to(DEV), num.to(DEV))
+    assert torch.equal(dev.cpu(), want)
+
+
 # ---- together ----------------------------------------------------------------------------
 def step_case(cache, parents, cached, tables, hq, seed, rope):
     g = torch.Generator(device=DEV).manual_seed(seed)
@@ -566,6 +586,31 @@ def test_streams_and_graphs():
         for (_, got), w in zip(graphs, want):
             assert torch.equal(got[0], w), f"replay {i}"
             assert all(torch.equal(x, y) for x, y in zip(got[1] + got[2], verdict + greedy)), f"replay {i}"
+
+
+def test_threads_on_one_stream():
+    """Calls of several threads on the same stream share its workspace, and none disturbs another."""
+    c = Case(41, 14, 2, 64, torch.float32, [6, 20], [9000, 700])
+    m, q, pool = c.meta(), c.q.to(DEV), c.pool.to(DEV)
+    cases = [verify_case(s, [20, 6, 1], 30011, torch.float32, True) for s in (42, 43, 44)]
+    metas = [build_tree_metadata(v[0]).to(DEV) for v in cases]
+    args = [[x.to(DEV) for x in v[1:]] for v in cases]
+    want, verdicts = tree_attention(q, pool, m), [verify_tree(vm, *a) for vm, a in zip(metas, args)]
+    wrong = []
+
+    def work(i):
+        torch.cuda.set_device(DEV)
+        for _ in range(100):
+            got = [tree_attention(q, pool, m)] if i == 3 else list(verify_tree(metas[i], *args[i]))
+            if not all(torch.equal(x, y) for x, y in zip(got, [want] if i == 3 else verdicts[i])):
+                wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
 
 
 @pytest.mark.parametrize("dtype,hq,hkv,d", [(torch.bfloat16, 14, 2, 64), (torch.float16, 16, 4, 64), (torch.bfloat16, 8, 4, 128),

@@ -9,7 +9,7 @@ import torch
 
 from oracle import tree as oracle
 from tinybatch_amd import _lib, build_tree_metadata, commit_tree, tree_attention, verify_tree, verify_tree_greedy
-from tinybatch_amd.tree import MAX_NODES
+from tinybatch_amd.tree import MAX_NODES, MAX_VOCAB
 
 
 def random_trees(seed, sizes):
@@ -93,6 +93,11 @@ def test_lists_that_do_not_fit_are_refused():
         build_tree_metadata([[-1, 0]], visible=[np.ones((2, 3), dtype=bool)])
 
 
+def test_tables_end_with_no_block():
+    m = meta_of([[-1], [-1, 0], []], [40, 3, 0], [[7, 8, 9, 10], [5, 6], [4]])
+    assert m.block_tables_np.tolist() == [[7, 8, 9], [5, -1, -1], [-1, -1, -1]]
+
+
 def test_no_cpu_fallback():
     m = meta_of([[-1, 0]], [0], [[0]]).to(torch.device("cpu"))
     with pytest.raises(RuntimeError, match="GPU"):
@@ -124,6 +129,8 @@ def test_entries_reject_bad_arguments_without_launching():
     assert verify(arrivals=f, units=1) == bad                    # fewer counters than sequences
     assert verify(width=MAX_NODES + 1) == unsupported
     assert verify(vocab=1 << 25, stride=1 << 25, wsb=1 << 30) == unsupported
+    assert verify(vocab=MAX_VOCAB + 1, stride=1 << 25, wsb=1 << 30) == unsupported
+    assert verify(vocab=MAX_VOCAB, stride=1 << 25, ws=None) == bad
     assert verify(seqs=0, probs=None) == _lib.TB_OK
     assert L.tb_tree_verify_greedy(f, f, f, f, 2, f, f, f, 0, None) == bad
     assert L.tb_tree_verify_greedy(None, f, f, f, 2, f, f, f, 4, None) == bad

@@ -36,7 +36,7 @@ namespace tb {
 constexpr int SUM_THREADS = 256, FIND_CHUNKS = 8;   // chunks of a thread at the end: up to 64 tokens, a lane each
 constexpr int MAX_ROUNDS = 5;
 constexpr int MAX_STRETCHES = 64;
-constexpr int MAX_STRETCH = 1 << 18;               // tokens whose refused ones are kept as bits in LDS
+constexpr int MAX_STRETCH = 1 << 17;               // tokens whose refused ones are kept as bits in LDS
 
 struct verify_state {
   double a;                    // the refusals' share of q so far (drafts drawn)
@@ -86,7 +86,8 @@ __device__ __forceinline__ double sum64(double x) {
 struct verify_tree {
   int32_t *tok, *par;
   float *p, *q, *u;            // of the node's token in its parent's rows; its random number
-  static __host__ __device__ size_t bytes(int nodes) { return (size_t)nodes * 20; }
+  static constexpr size_t BYTES = 20;              // of a node
+  static __host__ __device__ size_t bytes(int nodes) { return nodes * BYTES; }
   __device__ verify_tree(char* lds, int nodes)
       : tok((int32_t*)lds), par(tok + nodes), p((float*)(par + nodes)), q(p + nodes), u(q + nodes) {}
 };
@@ -368,7 +369,7 @@ __device__ __forceinline__ void verify_finish(const verify_args& a, int seq, ver
       atomicMax(&f.last, 64 * wave + 63 - __clzll((long long)some));
     }
     __syncthreads();
-    const int at = f.first < NT ? f.first : f.last;
+    const int at = max(f.first < NT ? f.first : f.last, 0);
     if (tid == at) f.before = base + (run - x);
     __syncthreads();
     before = f.before;
@@ -601,6 +602,9 @@ static int verify_stretches(int num_seqs, int vocab) {
   return std::min(std::max({fill, std::min(once, 32), bits, 1}), MAX_STRETCHES);
 }
 
+static_assert(verify_tree::BYTES * TB_TREE_MAX_NODES + 4 * TB_TREE_MAX_NODES + MAX_STRETCH / 8 + 4 + sizeof(find_lds) <=
+                  65536, "what a workgroup may ask for at its launch");
+
 template <typename T, bool DRAWN>
 static void launch_verify_as(const verify_args& a, int rounds, hipStream_t stream) {
   const int per = (a.vocab + 16 + a.stretches - 1) / a.stretches + 16;   // tokens of a stretch, at most
@@ -658,7 +662,8 @@ __global__ __launch_bounds__(64) void verify_greedy_kernel(const int64_t* target
 
 // commit: node path[j] of a sequence lies at position cached + path[j] and belongs at cached + j.
 // path rises, so path[j] >= j: a thread that moves one 16-byte column of the rows in order never
-// reads a row it has written, and no other thread touches its column.
+// reads a row it has written, and no other thread touches its column. A position outside the table or
+// a block outside the pool (a path that is none) is left out.
 __global__ __launch_bounds__(256) void commit_kernel(char* storage, int64_t layer_bytes, int64_t num_blocks,
                                                      const int32_t* block_tables, int32_t max_nb,
                                                      const int32_t* cached, const int32_t* accepted, int32_t width,
@@ -673,17 +678,17 @@ __global__ __launch_bounds__(256) void commit_kernel(char* storage, int64_t laye
   const int32_t* const path = accepted + (int64_t)seq * width;
   const int64_t head_bytes = (int64_t)bs * row_vecs * 16;
   char* const base = storage + layer * layer_bytes + kvh * head_bytes + 16 * piece;
-  auto slot = [&](int pos) -> char* {
-    const int blk = pos >> log2_bs;
-    const int64_t b = blk < max_nb ? table[blk] : -1;
+  auto slot = [&](int64_t pos) -> char* {
+    const int64_t blk = pos >> log2_bs;
+    const int64_t b = blk >= 0 && blk < max_nb ? table[blk] : -1;
     if (b < 0 || b >= num_blocks) return nullptr;
     return base + b * (2 * num_kv_heads) * head_bytes + (int64_t)(pos & (bs - 1)) * row_vecs * 16;
   };
   for (int j = 0; j < len; ++j) {
     const int i = path[j];
     if (i <= j) continue;                          // in its place already (or no node)
-    const char* const from = slot(c + i);
-    char* const to = slot(c + j);
+    const char* const from = slot((int64_t)c + i);
+    char* const to = slot((int64_t)c + j);
     if (from && to) st16(to, ld16(from));
   }
 }

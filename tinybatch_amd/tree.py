@@ -19,6 +19,7 @@ verdict stays on the device and the commit reads it there.
 from __future__ import annotations
 
 import math
+import threading
 from dataclasses import dataclass, field
 from typing import NamedTuple
 
@@ -30,7 +31,7 @@ from .metadata import pad4
 from .ops import Rope, _check_pool, _rows_view, kv_append
 
 MAX_NODES = 1024             # TB_TREE_MAX_NODES
-MAX_VOCAB = 64 * ((1 << 18) - 64)
+MAX_VOCAB = 64 * ((1 << 17) - 64)
 NUM_CUS, NUM_XCDS = 256, 8   # MI355X, for which the work lists are made
 
 
@@ -224,7 +225,7 @@ def build_tree_metadata(parents, cached_lens=None, block_tables=None, *, block_s
         if need[b] > len(table):
             raise IndexError(f"sequence {b} needs {need[b]} blocks for {ends[b]} positions, table has {len(table)}")
     max_nb = max(1, int(need.max()) if B else 1)
-    tables = np.zeros((B, max_nb), dtype=np.int32)
+    tables = np.full((B, max_nb), -1, dtype=np.int32)            # -1: no block
     for b, table in enumerate(block_tables):
         ids = np.asarray(table[:need[b]], dtype=np.int64)
         if ids.size and (ids.min() < 0 or ids.max() >= num_blocks):
@@ -237,7 +238,8 @@ def build_tree_metadata(parents, cached_lens=None, block_tables=None, *, block_s
         raise ValueError("two nodes of the step share a pool slot: give each tree blocks of its own")
     # a node's row must not fall on another sequence's cached positions: in its block those reach
     # from offset 0 up to its cached length, the nodes from some offset on
-    first_node = np.full(num_blocks, block_size, dtype=np.int64)
+    first_node = np.empty(num_blocks, dtype=np.int64)            # of the blocks that the tables name
+    first_node[tables] = block_size
     np.minimum.at(first_node, tables[seq, pos // block_size], pos % block_size)
     covered = np.clip(cached[:, None] - block_size * np.arange(max_nb), 0, block_size)
     if (covered > first_node[tables]).any():
@@ -256,33 +258,44 @@ def build_tree_metadata(parents, cached_lens=None, block_tables=None, *, block_s
 
 class _Scratch:
     """What the calls on one stream of one device share, since they are ordered: a workspace, and
-    arrival counters (zero between calls: every call leaves them zero)."""
+    arrival counters (zero between calls: every call leaves them zero). A call holds the lock until
+    its launches are on the stream: those of another thread do not come between them."""
 
     def __init__(self, device: torch.device):
+        self.lock = threading.RLock()
         self.workspace = torch.empty(1 << 20, dtype=torch.uint8, device=device)
         self.arrivals = torch.zeros(4096, dtype=torch.int32, device=device)
 
 
 _SCRATCH: dict[tuple[int, int], _Scratch] = {}
+_SCRATCH_LOCK = threading.RLock()
 _KEPT_BYTES = 32 << 20       # larger workspaces are allocated call by call
 
 
 def _scratch(device: torch.device, stream: int, nbytes: int, units: int):
-    """(workspace, its bytes, arrival counters or None, their number) of a call on the current
-    stream. A call that is being captured gets a workspace of its own and no counters: its graph
-    may be replayed beside anything."""
+    """(lock to release after the launches, workspace, its bytes, arrival counters or None, their number)
+    of a call on the current stream. A call that is being captured gets a workspace of its own and no
+    counters: its graph may be replayed beside anything."""
     if torch._C._cuda_isCurrentStreamCapturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes, None, 0
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        _SCRATCH_LOCK.acquire()
+        return _SCRATCH_LOCK, ws, nbytes, None, 0
     s = _SCRATCH.get((device.index, stream))
     if s is None:
-        s = _SCRATCH[device.index, stream] = _Scratch(device)
-    if s.arrivals.shape[0] < units:
-        s.arrivals = torch.zeros(2 * units, dtype=torch.int32, device=device)
-    if nbytes > _KEPT_BYTES:
-        return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes, s.arrivals, units
-    if s.workspace.shape[0] < nbytes:
-        s.workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return s.workspace, nbytes, s.arrivals, units
+        with _SCRATCH_LOCK:
+            s = _SCRATCH.setdefault((device.index, stream), _Scratch(device))
+    s.lock.acquire()
+    try:
+        if s.arrivals.shape[0] < units:
+            s.arrivals = torch.zeros(2 * units, dtype=torch.int32, device=device)
+        if nbytes > _KEPT_BYTES:
+            return s.lock, torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes, s.arrivals, units
+        if s.workspace.shape[0] < nbytes:
+            s.workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    except BaseException:
+        s.lock.release()
+        raise
+    return s.lock, s.workspace, nbytes, s.arrivals, units
 
 
 def _elsewhere(device: torch.device) -> bool:
@@ -367,17 +380,21 @@ def tree_attention(q: torch.Tensor, pool: torch.Tensor, meta: TreeMetadata, *, s
         positions = meta.positions.data_ptr()
     stream = _lib.stream_handle(device)
     slots, units = meta.partial_slots, meta.units
-    ws = arrivals = None
+    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
+    lock = ws = arrivals = None
     ws_bytes = 0
     if slots and bs >= 16:
-        ws, ws_bytes, arrivals, units = _scratch(device, stream, slots * hq * (d + 2) * 4, units)
-    st = _lib.lib().tb_tree_attention(
-        q.data_ptr(), qs, pool.data_ptr(), nb, out.data_ptr(), os_, *meta.addresses, mask.data_ptr(),
-        meta.mask_words, meta.work.data_ptr(), meta.work_np.shape[0], meta.column_blocks, meta.split.data_ptr(),
-        meta.split_np.shape[0], slots, None if ws is None else ws.data_ptr(), ws_bytes,
-        None if arrivals is None or not units else arrivals.data_ptr(), units, hq, hkv, d, bs,
-        1.0 / math.sqrt(d) if scale is None else float(scale), _lib.DTYPE_CODE[dtype], positions, cos, sin, longest,
-        stream)
+        lock, ws, ws_bytes, arrivals, units = _scratch(device, stream, slots * hq * (d + 2) * 4, units)
+    try:
+        st = _lib.lib().tb_tree_attention(
+            q.data_ptr(), qs, pool.data_ptr(), nb, out.data_ptr(), os_, *meta.addresses, mask.data_ptr(),
+            meta.mask_words, meta.work.data_ptr(), meta.work_np.shape[0], meta.column_blocks, meta.split.data_ptr(),
+            meta.split_np.shape[0], slots, None if ws is None else ws.data_ptr(), ws_bytes,
+            None if arrivals is None or not units else arrivals.data_ptr(), units, hq, hkv, d, bs, scale,
+            _lib.DTYPE_CODE[dtype], positions, cos, sin, longest, stream)
+    finally:
+        if lock is not None:
+            lock.release()
     _lib.check(st, "tb_tree_attention")
     return out
 
@@ -449,12 +466,15 @@ def verify_tree(meta: TreeMetadata, tokens: torch.Tensor, uniforms: torch.Tensor
     need = meta.verify_bytes.get(vocab)
     if need is None:
         need = meta.verify_bytes[vocab] = L.tb_tree_verify_workspace_bytes(B, vocab, width)
-    ws, ws_bytes, arrivals, units = _scratch(device, stream, need, B)
-    st = L.tb_tree_verify(
-        probs.data_ptr(), stride, draft, draft_stride, vocab, _lib.DTYPE_CODE[dtype], tokens.data_ptr(),
-        uniforms.data_ptr(), meta.parents.data_ptr(), meta.row_starts.data_ptr(), B, meta.max_children,
-        v.accepted.data_ptr(), v.num_accepted.data_ptr(), v.tokens.data_ptr(), width, ws.data_ptr(), ws_bytes,
-        None if arrivals is None else arrivals.data_ptr(), units, stream)
+    lock, ws, ws_bytes, arrivals, units = _scratch(device, stream, need, B)
+    try:
+        st = L.tb_tree_verify(
+            probs.data_ptr(), stride, draft, draft_stride, vocab, _lib.DTYPE_CODE[dtype], tokens.data_ptr(),
+            uniforms.data_ptr(), meta.parents.data_ptr(), meta.row_starts.data_ptr(), B, meta.max_children,
+            v.accepted.data_ptr(), v.num_accepted.data_ptr(), v.tokens.data_ptr(), width, ws.data_ptr(), ws_bytes,
+            None if arrivals is None else arrivals.data_ptr(), units, stream)
+    finally:
+        lock.release()
     _lib.check(st, "tb_tree_verify")
     return v
 
