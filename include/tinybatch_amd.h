@@ -677,6 +677,27 @@ int32_t tb_rms_norm_partials(const float* partials, int32_t splits, void* residu
  * At most TB_TREE_MAX_NODES nodes per tree where a limit is named. */
 #define TB_TREE_MAX_NODES 1024
 
+/* A step's arrays from the trees (host memory, no device call): parents [num_rows], a node's parent
+ * inside its tree (-1 for node 0, else an earlier node); row_starts [num_seqs + 1] from 0. Writes
+ *   mask [num_rows][mask_words]: every node's ancestors and itself (mask_words >= nodes / 32 of a tree);
+ *   positions [num_rows]: cached[b] + depth, the RoPE positions; row_seq [num_rows];
+ *   slot_mapping [num_rows] (tb_kv_append's): node i at position cached[b] + i of its block table.
+ * cached NULL: the trees alone (depths for positions, no slots); the tables are then unread.
+ * info [4]: the most children of a node, the largest position plus one, and on an error what is wrong
+ * and where: a parent (its row), a table too short or a block id outside the pool (the sequence;
+ * TB_ERR_INDEX for these two, TB_ERR_INVALID_ARG for the others), slots past 2^31 (the sequence), two nodes in
+ * one slot, a node on a cached position of its own or another sequence (the block). */
+#define TB_TREE_FAULT_PARENT 1
+#define TB_TREE_FAULT_TABLE 2
+#define TB_TREE_FAULT_BLOCK 3
+#define TB_TREE_FAULT_SLOTS 4
+#define TB_TREE_FAULT_SHARED 5
+#define TB_TREE_FAULT_CACHED 6
+int32_t tb_build_tree_rows(const int32_t* parents, const int32_t* row_starts, int32_t num_seqs,
+                           const int32_t* cached, const int32_t* block_tables, int32_t max_blocks_per_seq,
+                           int32_t block_size, int64_t num_blocks, uint32_t* mask, int32_t mask_words,
+                           int64_t* positions, int32_t* row_seq, int32_t* slot_mapping, int32_t* info);
+
 /* Attention of every node over the cached positions and the nodes of its mask:
  *   S_i = {0 .. cached-1} + {cached + j : bit j of mask[row]},  out = softmax(scale q.K[S_i]) V[S_i].
  * A node that sees nothing gives 0; positions outside S_i have no effect, also where they

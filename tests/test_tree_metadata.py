@@ -98,6 +98,54 @@ def test_tables_end_with_no_block():
     assert m.block_tables_np.tolist() == [[7, 8, 9], [5, -1, -1], [-1, -1, -1]]
 
 
+@pytest.mark.parametrize("as_", [np.asarray, torch.tensor, tuple])
+def test_lists_of_any_kind(as_):
+    m = meta_of([as_([-1, 0, 0]), as_([-1])], as_([20, 5]), [as_([3, 9, 1, 1, 1]), as_([2])])
+    n = meta_of([[-1, 0, 0], [-1]], [20, 5], [[3, 9], [2]])
+    for name in ("parents_np", "positions_np", "mask_np", "block_tables_np", "slot_mapping_np", "work_np"):
+        assert np.array_equal(getattr(m, name), getattr(n, name)), name
+    long = meta_of([[-1]], [5], [list(range(63, -1, -1)) * 4])      # far longer than its context
+    assert long.block_tables_np.tolist() == [[63]] and long.slot_mapping_np.tolist() == [63 * 16 + 5]
+
+
+def test_rows_entry_names_what_is_wrong():
+    L = _lib.lib()
+
+    def rows(parents=(-1, 0, -1), starts=(0, 2, 3), cached=(14, 3), tables=((5, 6), (7, 7)), bs=16, nb=8, words=1, nul=None):
+        a = [np.array(x, dtype=np.int32) for x in (parents, starts, cached, tables)]
+        t = len(parents)
+        out = [np.zeros((t, max(words, 1)), np.uint32), np.zeros(t, np.int64), np.zeros(t, np.int32), np.zeros(t, np.int32)]
+        info = np.zeros(4, np.int32)
+        ptr = {i: x.ctypes.data for i, x in enumerate(a + out)}
+        if nul is not None:
+            ptr[nul] = None
+        st = L.tb_build_tree_rows(ptr[0], ptr[1], len(starts) - 1, ptr[2], ptr[3], a[3].shape[1], bs, nb, ptr[4], words,
+                                  ptr[5], ptr[6], ptr[7], info.ctypes.data)
+        return st, info.tolist(), out
+
+    bad, index = _lib.TB_ERR_INVALID_ARG, _lib.TB_ERR_INDEX
+    st, info, (mask, positions, seq, slots) = rows()
+    assert st == _lib.TB_OK and info == [1, 16, 0, 0]
+    assert mask[:, 0].tolist() == [1, 3, 1] and positions.tolist() == [14, 15, 3] and seq.tolist() == [0, 0, 1]
+    assert slots.tolist() == [5 * 16 + 14, 5 * 16 + 15, 7 * 16 + 3]
+    assert rows(nul=2)[1:][0] == [1, 2, 0, 0]                        # the trees alone: depths
+    for parents, at in (((-1, 1, -1), 1), ((-1, -1, -1), 1), ((0, 0, -1), 0), ((-1, 0, 0), 2), ((-1, -2, -1), 1)):
+        st, info, _ = rows(parents=parents)
+        assert st == bad and info[2:] == [1, at]
+    assert rows(cached=(14, 31), tables=((5,), (7,)))[0] == index
+    assert rows(cached=(14, 31), tables=((5,), (7,)))[1][2:] == [2, 1]
+    assert rows(tables=((5, 6), (8, 7)))[0] == index and rows(tables=((5, 6), (8, 7)))[1][2:] == [3, 1]
+    assert rows(tables=((-1, 6), (7, 7)))[1][2:] == [3, 0]
+    assert rows(nb=1 << 28, tables=((5, 6), ((1 << 28) - 1, 7)))[1][2:] == [4, 1]
+    assert rows(cached=(14, 15), tables=((5, 6), (5, 7)))[1][2:] == [5, 5]
+    assert rows(cached=(14, 16), tables=((5, 6), (5, 7)))[1][2:] == [6, 5]
+    assert rows(cached=(16, 0), tables=((5, 5), (7, 7)))[1][2:] == [6, 5]   # a block twice in one table
+    for kw in (dict(nul=0), dict(nul=1), dict(nul=3), dict(nul=4), dict(nul=5), dict(nul=6), dict(nul=7), dict(bs=12),
+               dict(nb=0), dict(words=0), dict(cached=(-1, 3)), dict(starts=(0, 3, 2)), dict(starts=(1, 2, 3))):
+        assert rows(**kw)[0] == bad, kw
+    assert rows(parents=range(-1, 32), starts=(0, 33), cached=(0,), tables=((0, 1, 2),), words=1)[0] == bad
+
+
 def test_no_cpu_fallback():
     m = meta_of([[-1, 0]], [0], [[0]]).to(torch.device("cpu"))
     with pytest.raises(RuntimeError, match="GPU"):

@@ -142,6 +142,8 @@ SIGNATURES = {
         c_vp, c_sz, c_vp, c_i32,                 # workspace, bytes, arrivals, units
         c_i32, c_i32, c_i32, c_i32, c_f32, c_i32,   # heads, kv heads, head_dim, block_size, scale, dtype
         c_vp, c_vp, c_vp, c_i32, c_vp]),         # positions, rope cos, sin, max position, stream
+    "tb_build_tree_rows": (c_i32, [c_vp, c_vp, c_i32, c_vp, c_vp, c_i32, c_i32, c_i64, c_vp, c_i32, c_vp, c_vp, c_vp,
+                                   c_vp]),
     "tb_build_tree_work": (c_i32, [c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp, c_i32, c_vp,
                                    c_i32, c_vp]),
     "tb_tree_attention_workspace_bytes": (c_sz, [c_i32, c_i32, c_i32]),

@@ -995,6 +995,90 @@ extern "C" int32_t tb_build_tree_work(const int32_t* cached, const int32_t* node
   return TB_ERR_INVALID_ARG;
 }
 
+extern "C" int32_t tb_build_tree_rows(const int32_t* parents, const int32_t* row_starts, int32_t num_seqs,
+                                      const int32_t* cached, const int32_t* block_tables,
+                                      int32_t max_blocks_per_seq, int32_t block_size, int64_t num_blocks,
+                                      uint32_t* mask, int32_t mask_words, int64_t* positions, int32_t* row_seq,
+                                      int32_t* slot_mapping, int32_t* info) try {
+  TB_CHECK_ARG(num_seqs >= 0 && row_starts && row_starts[0] == 0 && mask_words > 0 && info);
+  std::fill(info, info + 4, 0);
+  for (int b = 0; b < num_seqs; ++b)
+    TB_CHECK_ARG(row_starts[b + 1] >= row_starts[b] && (row_starts[b + 1] - row_starts[b] + 31) / 32 <= mask_words);
+  if (cached) {
+    TB_CHECK_ARG(block_size > 0 && (block_size & (block_size - 1)) == 0 && num_blocks > 0 && max_blocks_per_seq >= 0);
+    TB_CHECK_ARG((num_seqs == 0 || block_tables) && (row_starts[num_seqs] == 0 || slot_mapping));
+  }
+  if (row_starts[num_seqs] == 0 && !cached) return TB_OK;
+  TB_CHECK_ARG(row_starts[num_seqs] == 0 || (parents && mask && positions && row_seq));
+  auto fault = [&](int32_t reason, int64_t where, int32_t status) {
+    info[2] = reason, info[3] = (int32_t)where;
+    return status;
+  };
+  std::vector<int32_t> children;
+  for (int b = 0; b < num_seqs; ++b) {
+    const int row0 = row_starts[b], n = row_starts[b + 1] - row0, words = (n + 31) / 32;
+    const int64_t start = cached ? cached[b] : 0;
+    TB_CHECK_ARG(start >= 0 && start + n <= (1 << 30));
+    children.assign(n, 0);
+    for (int i = 0; i < n; ++i) {
+      const int p = parents[row0 + i], r = row0 + i;
+      uint32_t* const m = mask + (int64_t)r * mask_words;
+      if (i == 0 ? p != -1 : p < 0 || p >= i) return fault(TB_TREE_FAULT_PARENT, r, TB_ERR_INVALID_ARG);
+      std::fill(m, m + mask_words, 0u);
+      if (i > 0) {
+        const uint32_t* const above = m - (int64_t)(i - p) * mask_words;
+        std::copy(above, above + words, m);
+        info[0] = std::max(info[0], ++children[p]);
+      }
+      m[i >> 5] |= 1u << (i & 31);
+      positions[r] = i > 0 ? positions[row0 + p] + 1 : start;
+      row_seq[r] = b;
+      info[1] = std::max<int32_t>(info[1], (int32_t)positions[r] + 1);
+    }
+  }
+  if (!cached) return TB_OK;
+  // the blocks that nodes lie in, each with the offsets that they take there
+  struct span {
+    int32_t block, lo, hi;
+    bool operator<(const span& o) const { return block != o.block ? block < o.block : lo < o.lo; }
+  };
+  std::vector<span> spans;
+  std::vector<bool> taken(num_blocks, false);
+  const int log2_bs = __builtin_ctz(block_size);
+  for (int b = 0; b < num_seqs; ++b) {
+    const int32_t* const table = block_tables + (int64_t)b * max_blocks_per_seq;
+    const int row0 = row_starts[b], n = row_starts[b + 1] - row0, end = cached[b] + n;
+    const int need = (int)(((int64_t)end + block_size - 1) >> log2_bs);
+    if (need > max_blocks_per_seq) return fault(TB_TREE_FAULT_TABLE, b, TB_ERR_INDEX);
+    for (int j = 0; j < need; ++j)
+      if (table[j] < 0 || table[j] >= num_blocks) return fault(TB_TREE_FAULT_BLOCK, b, TB_ERR_INDEX);
+    for (int p = cached[b]; p < end;) {
+      const int block = table[p >> log2_bs], lo = p & (block_size - 1), hi = std::min(block_size, lo + end - p);
+      if (((int64_t)block << log2_bs) + hi > INT32_MAX) return fault(TB_TREE_FAULT_SLOTS, b, TB_ERR_INVALID_ARG);
+      for (int o = lo; o < hi; ++o) slot_mapping[row0 + p - cached[b] + o - lo] = (block << log2_bs) + o;
+      spans.push_back({block, lo, hi});
+      taken[block] = true;
+      p += hi - lo;
+    }
+  }
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    if (spans[i].block == spans[i - 1].block && spans[i].lo < spans[i - 1].hi)
+      return fault(TB_TREE_FAULT_SHARED, spans[i].block, TB_ERR_INVALID_ARG);
+  // no node on a cached position, its own sequence's or another's
+  for (int b = 0; b < num_seqs; ++b)
+    for (int64_t j = 0; j << log2_bs < cached[b]; ++j) {
+      const int block = block_tables[(int64_t)b * max_blocks_per_seq + j];
+      if (!taken[block]) continue;
+      const auto at = std::lower_bound(spans.begin(), spans.end(), span{block, 0, 0});
+      if (at->lo < std::min<int64_t>(cached[b] - (j << log2_bs), block_size))
+        return fault(TB_TREE_FAULT_CACHED, block, TB_ERR_INVALID_ARG);
+    }
+  return TB_OK;
+} catch (const std::exception&) {
+  return TB_ERR_INVALID_ARG;
+}
+
 extern "C" size_t tb_tree_attention_workspace_bytes(int32_t partial_slots, int32_t num_heads, int32_t head_dim) {
   if (partial_slots <= 0 || num_heads <= 0 || head_dim <= 0) return 0;
   return (size_t)partial_slots * num_heads * (head_dim + 2) * sizeof(float);

@@ -18,6 +18,7 @@ verdict stays on the device and the commit reads it there.
 """
 from __future__ import annotations
 
+import itertools
 import math
 import threading
 from dataclasses import dataclass, field
@@ -32,6 +33,7 @@ from .ops import Rope, _check_pool, _rows_view, kv_append
 
 MAX_NODES = 1024             # TB_TREE_MAX_NODES
 MAX_VOCAB = 64 * ((1 << 17) - 64)
+_FAULT_PARENT, _FAULT_BLOCK, _FAULT_SLOTS, _FAULT_SHARED, _FAULT_CACHED = 1, 3, 4, 5, 6   # TB_TREE_FAULT_*
 NUM_CUS, NUM_XCDS = 256, 8   # MI355X, for which the work lists are made
 
 
@@ -55,7 +57,7 @@ class TreeMetadata:
     # host copies
     parents_np: np.ndarray       # [T] inside the tree, -1 for a root
     row_starts_np: np.ndarray    # [B + 1]
-    depths_np: np.ndarray        # [T]
+    positions_np: np.ndarray     # [T] int64: cached + depth, the nodes' RoPE positions (no cache: the depth)
     mask_np: np.ndarray          # [T, mask_words] uint32
     row_seq_np: np.ndarray       # [T]
     cached_np: np.ndarray | None
@@ -73,7 +75,7 @@ class TreeMetadata:
     row_starts: torch.Tensor | None = None
     mask: torch.Tensor | None = None          # [T, mask_words] int32
     row_seq: torch.Tensor | None = None
-    positions: torch.Tensor | None = None     # [T] int64: cached + depth, the nodes' RoPE positions
+    positions: torch.Tensor | None = None     # [T] int64
     cached: torch.Tensor | None = None
     block_tables: torch.Tensor | None = None
     slot_mapping: torch.Tensor | None = None
@@ -83,15 +85,18 @@ class TreeMetadata:
     longest: int = 0                          # the largest RoPE position, plus one
     verify_bytes: dict = field(default_factory=dict)   # workspace of verify_tree by vocabulary
 
+    @property
+    def depths_np(self) -> np.ndarray:
+        """[T]: every node's depth in its tree."""
+        return self.positions_np - (0 if self.cached_np is None else self.cached_np[self.row_seq_np])
+
     def to(self, device: torch.device) -> "TreeMetadata":
         """Upload every array with one host-to-device copy (views into one buffer)."""
         device = torch.device(device)
         if device.type == "cuda" and device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
         has_cache = self.cached_np is not None
-        start = self.cached_np[self.row_seq_np] if has_cache else 0
-        positions = (self.depths_np + start).astype(np.int64)
-        parts = [("positions", positions.view(np.int32)), ("parents", self.parents_np),
+        parts = [("positions", self.positions_np.view(np.int32)), ("parents", self.parents_np),
                  ("row_starts", self.row_starts_np), ("mask", self.mask_np.view(np.int32).reshape(-1)),
                  ("row_seq", self.row_seq_np)]
         if has_cache:
@@ -122,26 +127,25 @@ class TreeMetadata:
         return self
 
 
-def _masks(parents, visible, words: int) -> np.ndarray:
-    """[T, words] uint32: bit j of row i = node j is seen by node i."""
-    raw = bytearray()
-    size = 4 * words
-    for b, tree in enumerate(parents):
-        if visible is not None and visible[b] is not None:
-            v = np.asarray(visible[b], dtype=bool)
-            if v.shape != (len(tree), len(tree)):
-                raise ValueError(f"visible[{b}] must be [{len(tree)}, {len(tree)}], got {v.shape}")
-            rows = np.packbits(v, axis=1, bitorder="little")
-            full = np.zeros((len(tree), size), dtype=np.uint8)
-            full[:, :rows.shape[1]] = rows
-            raw += full.tobytes()
+def _flat(lists, lens: np.ndarray, lo: int) -> np.ndarray:
+    """The lists' integers one behind the other, what int32 does not hold at its ends."""
+    flat = np.fromiter(itertools.chain.from_iterable(lists), np.int64, int(lens.sum()))
+    return np.clip(flat, lo, np.iinfo(np.int32).max).astype(np.int32)
+
+
+def _see(mask: np.ndarray, visible, row_starts: np.ndarray) -> None:
+    """The sequences that name the nodes their rows see."""
+    for b, v in enumerate(visible):
+        if v is None:
             continue
-        seen: list[int] = []
-        for i, p in enumerate(tree):
-            seen.append((seen[p] if p >= 0 else 0) | (1 << i))
-        for m in seen:
-            raw += m.to_bytes(size, "little")
-    return np.frombuffer(bytes(raw), dtype=np.uint32).reshape(-1, words)
+        first, n = int(row_starts[b]), int(row_starts[b + 1] - row_starts[b])
+        v = np.asarray(v, dtype=bool)
+        if v.shape != (n, n):
+            raise ValueError(f"visible[{b}] must be [{n}, {n}], got {v.shape}")
+        rows = np.packbits(v, axis=1, bitorder="little")
+        own = mask[first:first + n].view(np.uint8)
+        own[:] = 0
+        own[:, :rows.shape[1]] = rows
 
 
 def _attach_work(meta: TreeMetadata) -> None:
@@ -177,81 +181,81 @@ def build_tree_metadata(parents, cached_lens=None, block_tables=None, *, block_s
     A table too short, or a block id outside the pool, raises IndexError; two nodes of the step
     in one slot raise ValueError.
     """
-    parents = [list(t) for t in parents]
-    sizes = [len(t) for t in parents]
-    max_nodes = max(sizes, default=0)
+    parents = list(parents)
+    B = len(parents)
+    sizes = np.fromiter(map(len, parents), np.int64, B)
+    T, max_nodes = int(sizes.sum()), int(sizes.max(initial=0))
     if max_nodes > MAX_NODES:
         raise ValueError(f"a tree of {max_nodes} nodes; at most {MAX_NODES} are served")
-    depths: list[int] = []
-    for b, tree in enumerate(parents):
-        first = len(depths)
-        for i, p in enumerate(tree):
-            if (p != -1) if i == 0 else not 0 <= p < i:
-                raise ValueError(f"parents[{b}][{i}] is {p}: node 0 has parent -1, every other node an earlier one")
-            depths.append(0 if i == 0 else depths[first + p] + 1)
-    if visible is not None and len(visible) != len(parents):
+    if visible is not None and len(visible) != B:
         raise ValueError("visible needs one entry per sequence")
     words = max(1, -(-max_nodes // 32))
-    children = max((int(np.bincount(np.array(t[1:], dtype=np.int64)).max()) for t in parents if len(t) > 1), default=0)
     row_starts = np.concatenate([[0], np.cumsum(sizes)]).astype(np.int32)
-    T, B = int(row_starts[-1]), len(parents)
-    meta = TreeMetadata(
-        num_rows=T, num_seqs=B, max_nodes=max_nodes, max_children=children, mask_words=words, block_size=block_size, num_blocks=num_blocks,
-        max_blocks_per_seq=0, num_heads=num_heads, num_kv_heads=num_kv_heads, head_dim=head_dim, dtype=dtype,
-        parents_np=np.array([p for t in parents for p in t], dtype=np.int32), row_starts_np=row_starts,
-        depths_np=np.array(depths, dtype=np.int64), mask_np=_masks(parents, visible, words),
-        row_seq_np=np.repeat(np.arange(B, dtype=np.int32), sizes), cached_np=None, block_tables_np=None,
-        slot_mapping_np=None)
+    flat, mask = _flat(parents, sizes, -2), np.empty((T, words), dtype=np.uint32)
+    positions, row_seq = np.empty(T, dtype=np.int64), np.empty(T, dtype=np.int32)
+    cached = tables = slots = None
+    max_nb = 0
     if cached_lens is None:
         if block_tables is not None:
             raise ValueError("block_tables without cached_lens")
+    else:
+        if block_tables is None or len(block_tables) != B or len(cached_lens) != B:
+            raise ValueError("cached_lens and block_tables need one entry per sequence")
+        if block_size <= 0 or block_size & (block_size - 1) or num_blocks <= 0:
+            raise ValueError("block_size must be a power of two and num_blocks positive")
+        if num_heads is None or num_kv_heads is None or head_dim is None or dtype not in _lib.DTYPE_CODE:
+            raise ValueError("num_heads, num_kv_heads, head_dim and dtype (fp32, fp16, bf16) describe the attention's calls")
+        if head_dim not in (64, 128):
+            raise ValueError(f"head_dim {head_dim} is not served (64 and 128 are)")
+        if num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads:
+            raise ValueError(f"num_heads {num_heads} is not a multiple of kv heads {num_kv_heads}")
+        ends = np.fromiter(cached_lens, np.int64, B) + sizes
+        if B and ((ends < sizes).any() or ends.max() > (1 << 30)):
+            raise ValueError("cached_lens must be >= 0 (and a context at most 2^30 positions)")
+        cached = (ends - sizes).astype(np.int32)
+        need, lens = -(-ends // block_size), np.fromiter(map(len, block_tables), np.int64, B)
+        if (lens < need).any():
+            b = int(np.argmax(lens < need))
+            raise IndexError(f"sequence {b} needs {need[b]} blocks for {ends[b]} positions, table has {lens[b]}")
+        max_nb = max(1, int(need.max(initial=0)))
+        tables = np.full((B, max_nb), -1, dtype=np.int32)            # -1: no block
+        if (lens <= 2 * need + 64).all():
+            ids, at = _flat(block_tables, lens, -1), np.cumsum(lens) - lens
+        else:                                                        # tables made longer than they are used
+            ids, at = _flat([t[:k] for t, k in zip(block_tables, need)], need, -1), np.cumsum(need) - need
+        inside = np.arange(max_nb) < need[:, None]
+        tables[inside] = ids[(at[:, None] + np.arange(max_nb))[inside]]
+        slots = np.empty(T, dtype=np.int32)
+    info = np.zeros(4, dtype=np.int32)
+    st = _lib.lib().tb_build_tree_rows(
+        flat.ctypes.data, row_starts.ctypes.data, B, None if cached is None else cached.ctypes.data,
+        None if cached is None else tables.ctypes.data, max_nb, block_size, num_blocks, mask.ctypes.data, words,
+        positions.ctypes.data, row_seq.ctypes.data, None if cached is None else slots.ctypes.data, info.ctypes.data)
+    if st != _lib.TB_OK:
+        fault, where = int(info[2]), int(info[3])
+        if fault == _FAULT_PARENT:
+            b = int(np.searchsorted(row_starts, where, side="right")) - 1
+            i = where - int(row_starts[b])
+            raise ValueError(f"parents[{b}][{i}] is {parents[b][i]}: node 0 has parent -1, every other node an earlier one")
+        if fault == _FAULT_BLOCK:
+            raise IndexError(f"block_tables[{where}] holds a block id outside the pool of {num_blocks} blocks")
+        if fault == _FAULT_SLOTS:
+            raise ValueError("a pool of more than 2^31 slots")
+        if fault == _FAULT_SHARED:
+            raise ValueError(f"two nodes of the step share a pool slot (block {where}): give each tree blocks of its own")
+        if fault == _FAULT_CACHED:
+            raise ValueError(f"a tree's nodes fall on another sequence's cached positions (block {where}): give each tree "
+                             "blocks of its own behind a shared prefix of whole blocks")
+        _lib.check(st, "tb_build_tree_rows")
+    if visible is not None:
+        _see(mask, visible, row_starts)
+    meta = TreeMetadata(
+        num_rows=T, num_seqs=B, max_nodes=max_nodes, max_children=int(info[0]), mask_words=words, block_size=block_size,
+        num_blocks=num_blocks, max_blocks_per_seq=max_nb, num_heads=num_heads, num_kv_heads=num_kv_heads,
+        head_dim=head_dim, dtype=dtype, parents_np=flat, row_starts_np=row_starts, positions_np=positions, mask_np=mask,
+        row_seq_np=row_seq, cached_np=cached, block_tables_np=tables, slot_mapping_np=slots, longest=int(info[1]))
+    if cached is None:
         return meta
-    if block_tables is None or len(block_tables) != B or len(cached_lens) != B:
-        raise ValueError("cached_lens and block_tables need one entry per sequence")
-    if block_size <= 0 or block_size & (block_size - 1) or num_blocks <= 0:
-        raise ValueError("block_size must be a power of two and num_blocks positive")
-    if num_heads is None or num_kv_heads is None or head_dim is None or dtype not in _lib.DTYPE_CODE:
-        raise ValueError("num_heads, num_kv_heads, head_dim and dtype (fp32, fp16, bf16) describe the attention's calls")
-    if head_dim not in (64, 128):
-        raise ValueError(f"head_dim {head_dim} is not served (64 and 128 are)")
-    if num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads:
-        raise ValueError(f"num_heads {num_heads} is not a multiple of kv heads {num_kv_heads}")
-    cached = np.array([int(c) for c in cached_lens], dtype=np.int64)
-    ends = cached + np.array(sizes, dtype=np.int64)
-    if B and (cached.min() < 0 or ends.max() > (1 << 30)):
-        raise ValueError("cached_lens must be >= 0 (and a context at most 2^30 positions)")
-    need = -(-ends // block_size)
-    for b, table in enumerate(block_tables):
-        if need[b] > len(table):
-            raise IndexError(f"sequence {b} needs {need[b]} blocks for {ends[b]} positions, table has {len(table)}")
-    max_nb = max(1, int(need.max()) if B else 1)
-    tables = np.full((B, max_nb), -1, dtype=np.int32)            # -1: no block
-    for b, table in enumerate(block_tables):
-        ids = np.asarray(table[:need[b]], dtype=np.int64)
-        if ids.size and (ids.min() < 0 or ids.max() >= num_blocks):
-            raise IndexError(f"block_tables[{b}] holds a block id outside the pool of {num_blocks} blocks")
-        tables[b, :need[b]] = ids
-    seq = meta.row_seq_np
-    pos = cached[seq] + np.arange(T) - row_starts[:-1][seq]
-    slots = tables[seq, pos // block_size].astype(np.int64) * block_size + pos % block_size
-    if np.unique(slots).size != T:
-        raise ValueError("two nodes of the step share a pool slot: give each tree blocks of its own")
-    # a node's row must not fall on another sequence's cached positions: in its block those reach
-    # from offset 0 up to its cached length, the nodes from some offset on
-    first_node = np.empty(num_blocks, dtype=np.int64)            # of the blocks that the tables name
-    first_node[tables] = block_size
-    np.minimum.at(first_node, tables[seq, pos // block_size], pos % block_size)
-    covered = np.clip(cached[:, None] - block_size * np.arange(max_nb), 0, block_size)
-    if (covered > first_node[tables]).any():
-        raise ValueError("a tree's nodes fall on another sequence's cached positions: give each tree blocks of its own "
-                         "behind a shared prefix of whole blocks")
-    if T and slots.max() > np.iinfo(np.int32).max:
-        raise ValueError("a pool of more than 2^31 slots")
-    meta.cached_np = cached.astype(np.int32)
-    meta.block_tables_np = tables
-    meta.max_blocks_per_seq = max_nb
-    meta.slot_mapping_np = slots.astype(np.int32)
-    meta.longest = int((cached[seq] + meta.depths_np).max()) + 1 if T else 0
     _attach_work(meta)
     return meta
 
