@@ -812,13 +812,19 @@ static void launch_rows(const tree_args& a, int num_rows, int head_dim, hipStrea
 // ---- the work list (host, no device call) ------------------------------------------
 namespace {
 
-// What a work list costs, in us, fitted to the times of 61 steps cut in every way (14 geometries and
-// types, 1 to 100 sequences, contexts of 300 to 30000 positions, 2 to 64 nodes): the cut it picks is on
-// average 1.2% slower than the best one, 18% at most. A round is a chunk of a workgroup.
+// What a work list costs, in us, fitted to the times of 87 steps in every number of column blocks and cut
+// (14 geometries and types, 1 to 100 sequences, contexts of 300 to 30000 positions, 2 to 128 nodes): the list it
+// picks is on average 0.9% slower than the best one, 8% at most. A round is a chunk of a workgroup. The blocks
+// of a workgroup are part of the pick: few read K/V once more per 32 CW columns, but waste fewer columns and have
+// their waves share a chunk's positions. 32 sequences of 26 nodes at 14 / 2 heads of 64 (182 columns), 2000
+// positions: 19.3 us with two blocks against 21.9 with four, in fp32 (16 sequences) 32.8 against 45.8; 32 of 32 nodes
+// at 32 / 8 heads of 128, 8000 positions: 170 against 154. Up to 64 columns a third and fourth block would stand
+// idle; one block pays in rows of 128 bytes alone (chunks of 128 positions fit the LDS twice): 64 of 4 nodes at 14 / 2
+// heads of 64, 16000 positions, 66 us against 69.
 struct tree_price {
   int chunks_round;            // chunks of 32 positions in a round
   int on_cu;                   // workgroups a CU holds
-  double full;                 // a CU's time for each round of the workgroups it holds
+  double full;                 // a CU's time for each round of a workgroup, when it holds on_cu of them
   int cus;
   double row_bytes;            // of a K or V row
 };
@@ -833,18 +839,16 @@ inline int tree_even(int chunks, int part, int round) {
   return ((chunks + parts - 1) / parts + round - 1) / round * round;
 }
 
-// The part length in rounds of least cost; 0: no context is cut.
+// The part length in rounds of least cost, and that cost; 0: no context is cut.
 int tree_part_rounds(const tree_price& price, const int32_t* cached, const int32_t* nodes, int num_seqs, int rep,
-                     int cols, int num_kv_heads, double slot_bytes) {
-  constexpr double START = 3.7, START_ROUNDS = 2.4, ALONE = 1.4, BYTES_US = 7.2e6, JOIN = 0.65, JOIN_BATCH = 0.63,
-                   PARTIAL_BYTES_US = 3.3e6;
+                     int cols, int num_kv_heads, double slot_bytes, double& least) {
+  constexpr double START = 4.9, START_ROUNDS = 1.8, ALONE = 1.38, BYTES_US = 6.8e6, JOIN = 0.71, JOIN_BATCH = 0.47,
+                   PARTIAL_BYTES_US = 2.8e6;
   int most = 0;
-  double kv_bytes = 0;         // read; half as fast to come by where several workgroups read them
-  bool once = true;
+  double kv_bytes = 0;
   for (int b = 0; b < num_seqs; ++b) {
     most = std::max(most, (tree_chunks(cached[b], nodes[b]) + price.chunks_round - 1) / price.chunks_round);
     kv_bytes += 64. * tree_chunks(cached[b], nodes[b]) * price.row_bytes * num_kv_heads;
-    once &= nodes[b] * rep <= cols;
   }
   std::vector<std::pair<int, int64_t>> pieces;   // (rounds, workgroups)
   auto cost = [&](int part) {
@@ -880,14 +884,14 @@ int tree_part_rounds(const tree_price& price, const int32_t* cached, const int32
       seen += n;
     }
     const double t = end * price.full * (alone ? ALONE : price.on_cu);
-    const double mem = kv_bytes / BYTES_US * (once ? 1. : 0.5);
+    const double mem = kv_bytes / BYTES_US;
     double join = 0;
     if (slots > 0)
       join = JOIN + JOIN_BATCH * ((most_parts + 7) / (most_parts <= 16 ? 8 : 32)) + slots * slot_bytes / PARTIAL_BYTES_US;
-    return START + std::max(t, mem) + join;
+    return START + std::cbrt(t * t * t + mem * mem * mem) + join;   // the two hide each other, less so where alike
   };
   int best = 0;
-  double least = cost(0);
+  least = cost(0);
   for (int part = 1; part < most; part += part < 6 ? 1 : part < 16 ? 2 : part < 32 ? 4 : part < 48 ? 8 : part < 96 ? 16 : 32) {
     const double c = cost(part);
     if (c < least) least = c, best = part;
@@ -924,15 +928,22 @@ extern "C" int32_t tb_build_tree_work(const int32_t* cached, const int32_t* node
   }
   TB_CHECK_ARG(rows < (1 << 30));
   const int row_bytes = head_dim * (dtype == TB_DTYPE_F32 ? 4 : 2);
-  const int blocks = most_cols <= 32 && row_bytes == 128 ? 1 : most_cols <= 64 ? 2 : 4, cols = 32 * blocks;
-  const double full = dtype == TB_DTYPE_F32 ? (head_dim == 64 ? (blocks == 2 ? 1.24 : 2.16) : blocks == 2 ? 2.92 : 5.54)
-                      : head_dim == 128     ? (blocks == 2 ? 0.8 : 1.04)
-                      : blocks == 1         ? 0.64
-                      : blocks == 2         ? 0.44
-                                            : 0.51;
-  const tree_price price{blocks == 1 ? 4 : 2, row_bytes == 512 ? 1 : 2, full, num_cus, (double)row_bytes};
-  const int part = tree_part_rounds(price, cached, nodes, num_seqs, rep, cols, num_kv_heads,
-                                    (double)num_heads * (head_dim + 2) * 4) * price.chunks_round;
+  int blocks = 0, part = 0;
+  double least = 0;
+  for (const int n : {1, 2, 4}) {
+    if (n == 1 ? most_cols > 32 || row_bytes != 128 : n == 4 && most_cols <= 64) continue;
+    const double full = dtype == TB_DTYPE_F32 ? (head_dim == 64 ? (n == 2 ? 1.26 : 1.82) : n == 2 ? 3.43 : 5.61)
+                        : head_dim == 128     ? (n == 2 ? 0.636 : 1.01)
+                        : n == 1              ? 0.356
+                        : n == 2              ? 0.353
+                                              : 0.515;
+    const tree_price price{n == 1 ? 4 : 2, row_bytes == 512 ? 1 : 2, full, num_cus, (double)row_bytes};
+    double cost = 0;
+    const int rounds = tree_part_rounds(price, cached, nodes, num_seqs, rep, 32 * n, num_kv_heads,
+                                        (double)num_heads * (head_dim + 2) * 4, cost);
+    if (blocks == 0 || cost < least) blocks = n, part = rounds * price.chunks_round, least = cost;
+  }
+  const int cols = 32 * blocks, round = blocks == 1 ? 4 : 2;
   std::vector<tree_piece> pieces;
   int64_t slots = 0, num_split = 0, row0 = 0, units = 0;
   bool here = true;
@@ -942,7 +953,7 @@ extern "C" int32_t tb_build_tree_work(const int32_t* cached, const int32_t* node
     row0 += nodes[b];
     const int all = tree_chunks(cached[b], nodes[b]);
     if (all == 0) continue;
-    const int groups = (nodes[b] * rep + cols - 1) / cols, even = tree_even(all, part, price.chunks_round);
+    const int groups = (nodes[b] * rep + cols - 1) / cols, even = tree_even(all, part, round);
     const int parts = (all + even - 1) / even;
     const bool few = parts < (1 << 15);
     for (int i = 0; i < parts; ++i)
