@@ -683,7 +683,7 @@ int32_t tb_rms_norm_partials(const float* partials, int32_t splits, void* residu
  *   positions [num_rows]: cached[b] + depth, the RoPE positions; row_seq [num_rows];
  *   slot_mapping [num_rows] (tb_kv_append's): node i at position cached[b] + i of its block table.
  * cached NULL: the trees alone (depths for positions, no slots); the tables are then unread.
- * info [4]: the most children of a node, the largest position plus one, and on an error what is wrong
+ * info [4]: the most refusals of a walk that leave a sibling to test (max_refusals below), the largest position plus one, and on an error what is wrong
  * and where: a parent (its row), a table too short or a block id outside the pool (the sequence;
  * TB_ERR_INDEX for these two, TB_ERR_INVALID_ARG for the others), slots past 2^31 (the sequence), two nodes in
  * one slot, a node on a cached position of its own or another sequence (the block). */
@@ -761,8 +761,8 @@ size_t tb_tree_attention_workspace_bytes(int32_t partial_slots, int32_t num_head
  *   num_accepted [num_seqs]: how many (0 for a sequence without rows);
  *   out_tokens [num_seqs][width] (int64): the path's tokens behind the root, then the token
  *     drawn: num_accepted of them, then -1. width >= every tree's nodes;
- *   max_children: the most children a node has (a hint: it decides how many of the sums that
- *     refusals need get launches over the whole GPU);
+ *   max_refusals: the most refusals of a walk from the root that leave a sibling to test (tb_build_tree_rows'
+ *     info[0]; a hint: it decides how many of the sums that such tests need get launches over the whole GPU);
  *   workspace: tb_tree_verify_workspace_bytes, 8-byte aligned; calls that may overlap in time need
  *     their own;
  *   arrivals [arrival_units >= num_seqs] (may be NULL): counters, zero before the first call and left
@@ -773,7 +773,7 @@ size_t tb_tree_verify_workspace_bytes(int32_t num_seqs, int32_t vocab, int32_t w
 int32_t tb_tree_verify(const void* probs, int64_t probs_row_stride, const void* draft_probs,
                        int64_t draft_row_stride, int32_t vocab, int32_t dtype, const int64_t* tokens,
                        const float* uniforms, const int32_t* parents, const int32_t* row_starts,
-                       int32_t num_seqs, int32_t max_children, int32_t* accepted, int32_t* num_accepted,
+                       int32_t num_seqs, int32_t max_refusals, int32_t* accepted, int32_t* num_accepted,
                        int64_t* out_tokens, int32_t width, void* workspace, size_t workspace_bytes,
                        uint32_t* arrivals, int32_t arrival_units, hipStream_t stream);
 

@@ -681,11 +681,11 @@ def test_verify_ends_here_and_by_a_launch(dtype, drafts):
 
 
 def test_verify_with_a_hint_too_small():
-    # max_children only says how many launches sums get: a caller's mistake costs time, not the result
+    # max_refusals only says how many launches sums get: a caller's mistake costs time, not the result
     case = verify_case(63, [40, 9], 3001, torch.float32, True, sharp=3.0, noise=3.0)
     meta = build_tree_metadata(case[0]).to(DEV)
-    for children in (0, 1, 2, 50):
-        meta.max_children = children
+    for refusals in (0, 1, 2, 50):
+        meta.max_refusals = refusals
         check_verify(*case, verify_tree(meta, *[x.to(DEV) for x in case[1:]]))
 
 

@@ -108,6 +108,18 @@ def test_lists_of_any_kind(as_):
     assert long.block_tables_np.tolist() == [[63]] and long.slot_mapping_np.tolist() == [63 * 16 + 5]
 
 
+def test_refusals_of_a_walk():
+    def most(tree, node):
+        below = [i for i in range(node + 1, len(tree)) if tree[i] == node]
+        return max([len(below) - 1, 0] + [k + most(tree, i) for k, i in enumerate(below)])
+
+    for seed in range(20):
+        trees = random_trees(seed, [1 + seed % 7, 0, 30])
+        assert build_tree_metadata(trees).max_refusals == max(most(t, 0) for t in trees if t)
+    assert build_tree_metadata([list(range(-1, 9)), [-1]]).max_refusals == 0
+    assert build_tree_metadata([[-1] + [0] * 9]).max_refusals == 8
+
+
 def test_rows_entry_names_what_is_wrong():
     L = _lib.lib()
 
@@ -125,10 +137,10 @@ def test_rows_entry_names_what_is_wrong():
 
     bad, index = _lib.TB_ERR_INVALID_ARG, _lib.TB_ERR_INDEX
     st, info, (mask, positions, seq, slots) = rows()
-    assert st == _lib.TB_OK and info == [1, 16, 0, 0]
+    assert st == _lib.TB_OK and info == [0, 16, 0, 0]
     assert mask[:, 0].tolist() == [1, 3, 1] and positions.tolist() == [14, 15, 3] and seq.tolist() == [0, 0, 1]
     assert slots.tolist() == [5 * 16 + 14, 5 * 16 + 15, 7 * 16 + 3]
-    assert rows(nul=2)[1:][0] == [1, 2, 0, 0]                        # the trees alone: depths
+    assert rows(nul=2)[1:][0] == [0, 2, 0, 0]                        # the trees alone: depths
     for parents, at in (((-1, 1, -1), 1), ((-1, -1, -1), 1), ((0, 0, -1), 0), ((-1, 0, 0), 2), ((-1, -2, -1), 1)):
         st, info, _ = rows(parents=parents)
         assert st == bad and info[2:] == [1, at]

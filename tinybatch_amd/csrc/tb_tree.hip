@@ -1025,12 +1025,14 @@ extern "C" int32_t tb_build_tree_rows(const int32_t* parents, const int32_t* row
     info[2] = reason, info[3] = (int32_t)where;
     return status;
   };
-  std::vector<int32_t> children;
+  std::vector<int32_t> children, order, refusals;
   for (int b = 0; b < num_seqs; ++b) {
     const int row0 = row_starts[b], n = row_starts[b + 1] - row0, words = (n + 31) / 32;
     const int64_t start = cached ? cached[b] : 0;
     TB_CHECK_ARG(start >= 0 && start + n <= (1 << 30));
     children.assign(n, 0);
+    order.assign(n, 0);                          // of a node among its siblings
+    refusals.assign(n, 0);                       // below a node: until a child is kept, and from there on
     for (int i = 0; i < n; ++i) {
       const int p = parents[row0 + i], r = row0 + i;
       uint32_t* const m = mask + (int64_t)r * mask_words;
@@ -1039,12 +1041,17 @@ extern "C" int32_t tb_build_tree_rows(const int32_t* parents, const int32_t* row
       if (i > 0) {
         const uint32_t* const above = m - (int64_t)(i - p) * mask_words;
         std::copy(above, above + words, m);
-        info[0] = std::max(info[0], ++children[p]);
+        order[i] = children[p]++;
       }
       m[i >> 5] |= 1u << (i & 31);
       positions[r] = i > 0 ? positions[row0 + p] + 1 : start;
       row_seq[r] = b;
       info[1] = std::max<int32_t>(info[1], (int32_t)positions[r] + 1);
+    }
+    for (int i = n - 1; i >= 0; --i) {
+      refusals[i] = std::max(refusals[i], children[i] - 1);
+      if (i > 0) refusals[parents[row0 + i]] = std::max(refusals[parents[row0 + i]], order[i] + refusals[i]);
+      else info[0] = std::max(info[0], refusals[0]);
     }
   }
   if (!cached) return TB_OK;

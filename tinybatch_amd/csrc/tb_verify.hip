@@ -27,14 +27,22 @@ namespace tb {
 // needs a sum over the vocabulary, and sums its own stretch of the row; launch r + 1: every workgroup
 // adds up launch r's stretches in order, goes on with the walk, and sums its stretch again. A
 // chain, and drafts that were not drawn, need one sum whatever is refused; a tree of drawn
-// drafts one more per refusal that has a sibling behind it: up to MAX_ROUNDS of those in launches of
-// their own, the rest by one workgroup at the end. What a later launch starts from (the state,
-// the nodes' values, the sums) it loads at once.
+// drafts one more per refusal that has a sibling behind it: as many launches as the worst walk of the step's
+// trees needs (max_refusals), up to MAX_ROUNDS, the rest by one workgroup at the end. What a later
+// launch starts from (the state, the nodes' values, the sums) it loads at once.
 // The end, by one workgroup per sequence, finds the border's stretch, thread and token: the
 // workgroup of the last sum launch that arrives last where the caller gives arrival counters, else
 // a launch of its own (a graph's replays may overlap, and then no counter is theirs alone).
+//
+// What bounds it: the reads of one target row, and one draft row, per sum where there are many sequences (64
+// chains over 151936 fp32 tokens: 78 MB in 24 us, 16 us at a copy's rate), the launches and their dependent
+// loads where there are few (one sequence: 10 us in a graph, 14 on the host); each further sum of a drawn tree
+// takes 3 to 7 us. 16 trees of 12 to 20 drawn nodes: 45 us, with up to six refusals.
+// MAX_ROUNDS: a launch that turns out not to be needed costs 2 to 3 us, a sum that the end has to make up for
+// 50: those trees with at most 5 launches 48 us on average and 107 at worst, with 6 or more 45 and 55; 3 trees of
+// 15 to 60 nodes (walks of up to 8 refusals are possible, none needed 5) 32 with 5, 37 with 7, 40 with 9.
 constexpr int SUM_THREADS = 256, FIND_CHUNKS = 8;   // chunks of a thread at the end: up to 64 tokens, a lane each
-constexpr int MAX_ROUNDS = 5;
+constexpr int MAX_ROUNDS = 6;
 constexpr int MAX_STRETCHES = 64;
 constexpr int MAX_STRETCH = 1 << 17;               // tokens whose refused ones are kept as bits in LDS
 
@@ -376,22 +384,26 @@ __device__ __forceinline__ void verify_finish(const verify_args& a, int seq, ver
     return at;
   };
 
-  const bool pending = DRAWN && st.round < 0;
-  if (pending) {
-    double s = sum64(sum);
+  if (DRAWN && st.round < 0) {                     // the walk's rest: this workgroup sums all stretches
     const int len0 = st.len;
-    for (;;) {
+    do {
+      const double s = sum64(sum);
       if (wave == 0) {
         walk(t, n, true, s, st, path, lane, 0);
         if (lane == 0) f.st = st;
       }
       __syncthreads();
       st = f.st;
-      __syncthreads();
-      if (st.round >= 0) break;
       const verify_row<T, DRAWN> row(a, row0 + st.cur, st.a);
-      s = total(row.share(0, row.chunks, tid, NT));
-    }
+      for (int g = wave; g < a.stretches; g += NW) {
+        const double x = sum64(row.share(stretch_begin(row.chunks, a.stretches, g),
+                                         stretch_begin(row.chunks, a.stretches, g + 1), lane, 64));
+        if (lane == 0) f.chunk[g] = x;
+      }
+      __syncthreads();
+      sum = lane < a.stretches ? f.chunk[lane] : 0.;
+      __syncthreads();
+    } while (st.round < 0);
     for (int i = len0 + tid; i < st.len; i += NT) {
       acc[i] = path[i];
       out[i - 1] = a.tokens[row0 + path[i]];
@@ -401,23 +413,16 @@ __device__ __forceinline__ void verify_finish(const verify_args& a, int seq, ver
   verify_row<T, DRAWN> row(a, row0 + st.cur, st.a);
   const double u = (double)st.u;
   int b = 0, e = row.chunks;
-  double before = 0., border = 0., w;
-  if (!pending) {                                  // the stretch
-    const double run = scan64<64>(sum, lane);
-    w = __shfl(run, 63);
-    border = u * w;
+  double before = 0.;
+  const double run = scan64<64>(sum, lane);
+  double w = __shfl(run, 63), border = u * w;
+  if (w > 0.) {                                    // the stretch
     const uint64_t some = __ballot(sum > 0.), past = __ballot(sum > 0. && run > border);
-    if (w > 0.) {
-      const int g = past ? __ffsll((unsigned long long)past) - 1 : 63 - __clzll((long long)some);
-      b = stretch_begin(row.chunks, a.stretches, g), e = stretch_begin(row.chunks, a.stretches, g + 1);
-      before = __shfl(run - sum, g);
-      if constexpr (!DRAWN) row.refuse(t, n, st.cur, bits, b, e);
-    }
-  } else {
-    w = total(row.share(b, e, tid, NT));
-    border = u * w;
-  }
-  if (!(w > 0.)) {                                 // nothing is left: the row as it is
+    const int g = past ? __ffsll((unsigned long long)past) - 1 : 63 - __clzll((long long)some);
+    b = stretch_begin(row.chunks, a.stretches, g), e = stretch_begin(row.chunks, a.stretches, g + 1);
+    before = __shfl(run - sum, g);
+    if constexpr (!DRAWN) row.refuse(t, n, st.cur, bits, b, e);
+  } else {                                         // nothing is left: the row as it is
     row.whole();
     w = total(row.share(b, e, tid, NT));
     border = u * w;
@@ -594,7 +599,8 @@ __global__ __launch_bounds__(SUM_THREADS) void verify_find_kernel(const verify_a
 }
 
 // Workgroups of a sequence: about four per CU over the batch, few enough tokens for the end's threads
-// (one step of FIND_CHUNKS chunks each, 16-byte chunks of fp32) and for the bits.
+// (one step of FIND_CHUNKS chunks each, 16-byte chunks of fp32) and for the bits. Two per CU take 41.1 us instead
+// of 40.9 for 16 trees and one 47.0; eight 28.4 instead of 24.7 for 64 chains, 23.1 instead of 16.9 for 32 trees.
 static int verify_stretches(int num_seqs, int vocab) {
   const int fill = std::min(1024 / std::max(num_seqs, 1), std::max(vocab / 1024, 1));
   const int once = (vocab + SUM_THREADS * FIND_CHUNKS * 4 - 64) / (SUM_THREADS * FIND_CHUNKS * 4 - 64);
@@ -661,6 +667,9 @@ __global__ __launch_bounds__(64) void verify_greedy_kernel(const int64_t* target
 }
 
 // commit: node path[j] of a sequence lies at position cached + path[j] and belongs at cached + j.
+// Bound by the scattered rows: 44 MB read and written in 13.5 us (3.3 TB/s) for 64 paths in 32 layers of 8 heads of
+// 128, 9.1 us at a copy's rate; a step of one tree by its launch (2.7 us in a graph). Rows read 4 or 8 at a time ahead of
+// their stores, non-temporal loads and stores past the L2 measured 14.5 to 21.7 us.
 // path rises, so path[j] >= j: a thread that moves one 16-byte column of the rows in order never
 // reads a row it has written, and no other thread touches its column. A position outside the table or
 // a block outside the pool (a path that is none) is left out.
@@ -705,11 +714,11 @@ extern "C" size_t tb_tree_verify_workspace_bytes(int32_t num_seqs, int32_t vocab
 extern "C" int32_t tb_tree_verify(const void* probs, int64_t probs_row_stride, const void* draft_probs,
                                   int64_t draft_row_stride, int32_t vocab, int32_t dtype, const int64_t* tokens,
                                   const float* uniforms, const int32_t* parents, const int32_t* row_starts,
-                                  int32_t num_seqs, int32_t max_children, int32_t* accepted, int32_t* num_accepted,
+                                  int32_t num_seqs, int32_t max_refusals, int32_t* accepted, int32_t* num_accepted,
                                   int64_t* out_tokens, int32_t width, void* workspace, size_t workspace_bytes,
                                   uint32_t* arrivals, int32_t arrival_units, hipStream_t stream) {
   using namespace tb;
-  TB_CHECK_ARG(num_seqs >= 0 && vocab > 0 && width > 0 && max_children >= 0);
+  TB_CHECK_ARG(num_seqs >= 0 && vocab > 0 && width > 0 && max_refusals >= 0);
   TB_CHECK_ARG(dtype >= TB_DTYPE_F32 && dtype <= TB_DTYPE_BF16);
   if (width > TB_TREE_MAX_NODES || vocab > MAX_STRETCHES * (MAX_STRETCH - 64)) return TB_ERR_UNSUPPORTED;
   if (num_seqs == 0) return TB_OK;
@@ -720,7 +729,7 @@ extern "C" int32_t tb_tree_verify(const void* probs, int64_t probs_row_stride, c
   TB_CHECK_ARG(!arrivals || (arrival_units >= num_seqs && ((uintptr_t)arrivals & 3u) == 0));
   const int stretches = verify_stretches(num_seqs, vocab);
   // sums that tests of later siblings need: none in a chain, or where the drafts were not drawn
-  const int rounds = draft_probs ? std::min(std::max(max_children - 1, 0), MAX_ROUNDS) : 0;
+  const int rounds = draft_probs ? std::min(max_refusals, MAX_ROUNDS) : 0;
   verify_state* const states = (verify_state*)workspace;
   double* const sums = (double*)(states + (size_t)(MAX_ROUNDS + 1) * num_seqs);
   const verify_args a{probs, probs_row_stride, draft_probs, draft_row_stride, vocab, tokens, uniforms, parents,

@@ -44,7 +44,7 @@ class TreeMetadata:
     num_rows: int
     num_seqs: int
     max_nodes: int               # nodes of the largest tree
-    max_children: int            # of one node
+    max_refusals: int            # of a walk from the root, those that leave a sibling to test
     mask_words: int              # 32-bit words of a row's mask
     # the cache part (None / 0 without cached_lens)
     block_size: int
@@ -250,7 +250,7 @@ def build_tree_metadata(parents, cached_lens=None, block_tables=None, *, block_s
     if visible is not None:
         _see(mask, visible, row_starts)
     meta = TreeMetadata(
-        num_rows=T, num_seqs=B, max_nodes=max_nodes, max_children=int(info[0]), mask_words=words, block_size=block_size,
+        num_rows=T, num_seqs=B, max_nodes=max_nodes, max_refusals=int(info[0]), mask_words=words, block_size=block_size,
         num_blocks=num_blocks, max_blocks_per_seq=max_nb, num_heads=num_heads, num_kv_heads=num_kv_heads,
         head_dim=head_dim, dtype=dtype, parents_np=flat, row_starts_np=row_starts, positions_np=positions, mask_np=mask,
         row_seq_np=row_seq, cached_np=cached, block_tables_np=tables, slot_mapping_np=slots, longest=int(info[1]))
@@ -474,7 +474,7 @@ def verify_tree(meta: TreeMetadata, tokens: torch.Tensor, uniforms: torch.Tensor
     try:
         st = L.tb_tree_verify(
             probs.data_ptr(), stride, draft, draft_stride, vocab, _lib.DTYPE_CODE[dtype], tokens.data_ptr(),
-            uniforms.data_ptr(), meta.parents.data_ptr(), meta.row_starts.data_ptr(), B, meta.max_children,
+            uniforms.data_ptr(), meta.parents.data_ptr(), meta.row_starts.data_ptr(), B, meta.max_refusals,
             v.accepted.data_ptr(), v.num_accepted.data_ptr(), v.tokens.data_ptr(), width, ws.data_ptr(), ws_bytes,
             None if arrivals is None else arrivals.data_ptr(), units, stream)
     finally:
