@@ -75,7 +75,7 @@ __device__ __forceinline__ bool tree_sees(const uint32_t* mask, int cached, int 
   return false;
 }
 
-// Blocks of fewer than 16 positions: one wave per (row, head), lane l the positions l, l + 64, ...: each
+// The direct form, for what the tiles cannot address: blocks of fewer than 16 positions: one wave per (row, head), lane l the positions l, l + 64, ...: each
 // lane holds a softmax state of its own, merged across the wave at the end.
 template <typename Tag, int D>
 __global__ __launch_bounds__(64) void tree_rows_kernel(const tree_args a) {
@@ -356,6 +356,17 @@ __device__ __forceinline__ void tree_join_here(const tree_args& a, int row0, int
 
 // 32 CW columns: the four waves share chunks of CK positions, of which each loads a quarter. CW of them take
 // 32 columns each, 4 / CW the same columns, each a part of a chunk's positions, joined at the end.
+//
+// What bounds it: with few columns the reads of K/V (48 chains of 4 to 8 nodes behind 8192 positions at 32 / 8 heads of
+// 128, bf16: 1.9 GB in 293 to 308 us, 6.2 to 6.5 TB/s); with many the products and the softmax between them (16
+// trees of 64 nodes there: 80 GFLOP in 119 to 128 us, 620 to 670 TFLOP/s; at head dim 64 a score's exponential,
+// mask-free maximum, rounding and sum weigh twice as much: 230 TFLOP/s); fp32 products in fp32 (60 TFLOP/s of
+// 153, 32 columns a block whether used or not); a single sequence the launch, the block table and K/V reads one
+// after the other (6.8 us in a graph for 4 nodes behind 600 positions).
+// Why chunks are shared: with a ring of its own per wave, no barriers but a quarter of the bytes in flight per
+// position loaded, the chains above took 343 us instead of 295. Rows that one workgroup reads are loaded past the
+// L2s' replacement (`once`: 297 us against 314), rows that several read through the L2 (16 trees of 64 nodes behind
+// 8000 positions: 146 against 155). CK is what a ring of two leaves of the LDS to two workgroups (one at 512-byte rows).
 template <typename Tag, int D, int CW, int CK>
 __global__ __launch_bounds__(256, D * elem<Tag>::bytes * CK < 32768 ? 2 : 1) void tree_columns_kernel(const tree_args a) {
   using S = tshape<Tag, D>;
@@ -903,9 +914,13 @@ struct tree_piece {
   int seq, kvh, chunk0, chunks, slot, groups, unit, order;   // order: part | parts << 16
 };
 
-// What a unit's last workgroup joins: 4 of a thread's columns in two steps, 16 parts in two more. Such a
-// join takes 2 to 4 us; a launch of its own 2.5 us of the GPU and 3 us of the host.
-constexpr int JOIN_HERE_FLOATS = 4096, JOIN_HERE_PARTS = 16;
+// Whether a unit's last workgroup joins its parts. Its loads go past the L2s: for 4096 floats it takes 4 to 6 us, a
+// launch 2 to 3, but 3 us more of the host, for which a short step's calls wait (12.7 us a call of two launches). So
+// only little is joined there, more where the step is short and the parts come in one turn of loads. Us a call, there
+// and by a launch: 13 nodes at 14 / 2 heads of 64, 600 positions, 10.5 and 12.7; 16 sequences of 18 nodes, 2000
+// positions, 14.7 and 12.7; 8 of 13 in fp32 15.6 and 12.8; 8 nodes at 32 / 8 heads of 128 in 9 parts 15.6 and 12.6.
+constexpr int JOIN_HERE_FLOATS = 4096, JOIN_ALWAYS_FLOATS = 2047, JOIN_HERE_PARTS = 16;
+constexpr double JOIN_HERE_US = 10;
 
 }  // namespace
 
@@ -947,6 +962,7 @@ extern "C" int32_t tb_build_tree_work(const int32_t* cached, const int32_t* node
   std::vector<tree_piece> pieces;
   int64_t slots = 0, num_split = 0, row0 = 0, units = 0;
   bool here = true;
+  const bool brief = least <= JOIN_HERE_US;
   std::vector<int32_t> first(num_seqs + 1);
   for (int b = 0; b < num_seqs; ++b) {
     first[b] = (int32_t)row0;
@@ -962,7 +978,9 @@ extern "C" int32_t tb_build_tree_work(const int32_t* cached, const int32_t* node
                           parts > 1 ? (int)(slots + (int64_t)i * nodes[b]) : -1, groups, (int)(units + h * groups),
                           few ? i | parts << 16 : 0});
     if (parts > 1) {
-      here &= parts <= JOIN_HERE_PARTS && std::min(cols, nodes[b] * rep) * head_dim <= JOIN_HERE_FLOATS;
+      const int floats = std::min(cols, nodes[b] * rep) * head_dim;   // of a part
+      here &= parts <= JOIN_HERE_PARTS &&
+              (floats <= JOIN_ALWAYS_FLOATS || (brief && floats * ((parts + 7) / 8) <= JOIN_HERE_FLOATS));
       units += (int64_t)groups * num_kv_heads;
       for (int i = 0; i < nodes[b]; ++i, ++num_split)
         if (split && num_split < split_capacity) {
