@@ -705,12 +705,11 @@ int32_t tb_build_tree_rows(const int32_t* parents, const int32_t* row_starts, in
  * any query heads per kv head, any scale.
  *   q [num_rows][num_heads][head_dim], out [num_rows][num_heads * head_dim]: row strides in
  *     elements, 16-byte aligned rows; block_tables [num_seqs][max_blocks_per_seq];
- *   row_seq [num_rows]: each row's sequence (-1: a row of none, left as it is);
+ *   row_seq [num_rows]: each row's sequence;
  *   mask [num_rows][mask_words] 32-bit words, bit j % 32 of word j / 32 = node j is seen; bits
  *     past the tree are ignored;
  *   work [num_work][12], split_rows [num_split_rows][4], column_blocks, partial_slots:
- *     tb_build_tree_work's for this call's sizes (device memory, 16-byte aligned; block_size < 16
- *     needs none); workspace: tb_tree_attention_workspace_bytes, 16-byte aligned, for contexts cut
+ *     tb_build_tree_work's for this call's sizes (device memory, 16-byte aligned); workspace: tb_tree_attention_workspace_bytes, 16-byte aligned, for contexts cut
  *     into parts. Calls that may overlap in time need their own workspace;
  *   arrivals (may be NULL; only where the list's counts[4] is not 0): arrival_units >= counts[4]
  *     counters, zero before the first call and left zero by every call; they save the launch that

@@ -17,6 +17,9 @@
 // chunk's positions, and join their softmax states in LDS at the end. A context cut into parts
 // leaves a partial per part, joined by the workgroup of a (sequence, kv head, columns) that arrives
 // last where there is little to join and the caller gives arrival counters, else by a second launch.
+// Blocks of fewer than 16 positions (SMALL) give every row of a tile a block of its own; otherwise a tile has one,
+// and its rows one base address. In blocks of 8 16 trees of 16 nodes behind 4000 positions at 32 / 8 heads of 128 take
+// 50.4 us, in blocks of 16 45.6.
 //
 // Math per chunk and block of 32 columns (C rows are positions or dims, C columns the block's):
 //   S^T[pos][col] = K[pos][:] . q[col][:]        A = K rows from LDS, B = q in registers
@@ -54,7 +57,6 @@ struct tree_args {
   int32_t mask_words;          // 32-bit words
   int32_t num_heads, num_kv_heads, rep;
   int32_t log2_bs;
-  float scale;
   const int64_t* positions;    // [T], for the rotation of q
   rope_tables rope;
   const int4* work;            // three per workgroup, see tb_build_tree_work
@@ -74,101 +76,6 @@ __device__ __forceinline__ bool tree_sees(const uint32_t* mask, int cached, int 
     if (mask[w] & (n - 32 * w >= 32 ? ~0u : (1u << (n - 32 * w)) - 1)) return true;
   return false;
 }
-
-// The direct form, for what the tiles cannot address: blocks of fewer than 16 positions: one wave per (row, head), lane l the positions l, l + 64, ...: each
-// lane holds a softmax state of its own, merged across the wave at the end.
-template <typename Tag, int D>
-__global__ __launch_bounds__(64) void tree_rows_kernel(const tree_args a) {
-  using T = typename elem<Tag>::type;
-  constexpr int N = 16 / sizeof(T), CH = D / N;    // elements of a 16-byte chunk, chunks of a row
-  constexpr int RB = D * sizeof(T);
-  const int row = blockIdx.x, head = blockIdx.y, lane = threadIdx.x;
-  const int seq = a.row_seq[row];
-  if (seq < 0) return;
-  const int row0 = a.row_starts[seq], n = a.row_starts[seq + 1] - row0, c = a.cached[seq];
-  const int kvh = head / a.rep;
-
-  vec16 qc[CH];
-  const char* const qrow = a.q + (int64_t)row * a.q_row_bytes + (int64_t)head * RB;
-#pragma unroll
-  for (int i = 0; i < CH; ++i) qc[i] = ld16(qrow + 16 * i);
-  if (a.rope.cos) {
-    const int64_t r = a.rope.row(a.positions[row], D / 2);
-#pragma unroll
-    for (int i = 0; i < CH / 2; ++i)
-      rope_pair<T>(qc[i], qc[i + CH / 2], a.rope.cos + r + N * i, a.rope.sin + r + N * i);
-  }
-  float q[D];
-#pragma unroll
-  for (int i = 0; i < CH; ++i) {
-    T e[N];
-    __builtin_memcpy(e, &qc[i], 16);
-#pragma unroll
-    for (int j = 0; j < N; ++j) q[N * i + j] = (float)e[j];
-  }
-
-  const float sl2e = a.scale * 1.4426950408889634f;
-  const int bs_mask = (1 << a.log2_bs) - 1;
-  const int64_t head_bytes = ((int64_t)1 << a.log2_bs) * RB;
-  const int64_t blk_bytes = 2 * (int64_t)a.num_kv_heads * head_bytes, v_off = a.num_kv_heads * head_bytes;
-  const int32_t* const table = a.block_tables + (int64_t)seq * a.max_nb;
-  const uint32_t* const mask = a.mask + (int64_t)row * a.mask_words;
-  float m = -INFINITY, l = 0.f, acc[D];
-#pragma unroll
-  for (int i = 0; i < D; ++i) acc[i] = 0.f;
-  bool any = false;
-  for (int p = lane; p < c + n; p += 64) {
-    if (p >= c && !((mask[(p - c) >> 5] >> ((p - c) & 31)) & 1)) continue;
-    const int64_t b = table[p >> a.log2_bs];
-    if (b < 0 || b >= a.num_blocks) continue;      // host validates; stay inside the pool
-    any = true;
-    const char* const k = a.pool + b * blk_bytes + kvh * head_bytes + (int64_t)(p & bs_mask) * RB;
-    float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const vec16 v = ld16(k + 16 * i);
-      T e[N];
-      __builtin_memcpy(e, &v, 16);
-#pragma unroll
-      for (int j = 0; j < N; ++j) s = fmaf((float)e[j], q[N * i + j], s);
-    }
-    s *= sl2e;
-    if (!(s <= m)) {                               // a larger score, or NaN
-      const float f = m == -INFINITY ? 0.f : fast_exp2(m - s);
-      l *= f;
-#pragma unroll
-      for (int i = 0; i < D; ++i) acc[i] *= f;
-      m = s;
-    }
-    const float w = s == -INFINITY ? 0.f : fast_exp2(s - m);
-    l += w;
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const vec16 v = ld16(k + v_off + 16 * i);
-      T e[N];
-      __builtin_memcpy(e, &v, 16);
-#pragma unroll
-      for (int j = 0; j < N; ++j) acc[N * i + j] = fmaf(w, (float)e[j], acc[N * i + j]);
-    }
-  }
-  float mm = m;
-#pragma unroll
-  for (int x = 1; x < 64; x *= 2) {
-    const float o = __shfl_xor(mm, x);
-    mm = mm != mm || o != o ? NAN : fmaxf(mm, o);
-  }
-  const float f = m == -INFINITY && mm == -INFINITY ? 0.f : fast_exp2(m - mm);
-  l = group_sum<64>(l * f);
-  const bool some = __any(any);
-  const float inv = some ? 1.f / l : 0.f;
-  char* const orow = a.out + (int64_t)row * a.out_row_bytes + (int64_t)head * RB;
-#pragma unroll
-  for (int i = 0; i < D; ++i) {
-    const float s = group_sum<64>(m == -INFINITY ? 0.f : acc[i] * f);
-    if (lane == i % 64) reinterpret_cast<T*>(orow)[i] = (T)(some ? s * inv : 0.f);
-  }
-}
-
 
 // ---- column blocks over the matrix unit --------------------------------------------
 template <typename Tag, int D>
@@ -359,15 +266,15 @@ __device__ __forceinline__ void tree_join_here(const tree_args& a, int row0, int
 //
 // What bounds it: with few columns the reads of K/V (48 chains of 4 to 8 nodes behind 8192 positions at 32 / 8 heads of
 // 128, bf16: 1.9 GB in 293 to 308 us, 6.2 to 6.5 TB/s); with many the products and the softmax between them (16
-// trees of 64 nodes there: 80 GFLOP in 119 to 128 us, 620 to 670 TFLOP/s; at head dim 64 a score's exponential,
-// mask-free maximum, rounding and sum weigh twice as much: 230 TFLOP/s); fp32 products in fp32 (60 TFLOP/s of
-// 153, 32 columns a block whether used or not); a single sequence the launch, the block table and K/V reads one
+// trees of 64 nodes there: 80 GFLOP in 119 to 128 us, 620 to 670 TFLOP/s; at head dim 64 the softmax weighs
+// twice as much: 32 trees of 60 nodes at 14 / 2 heads behind 2000 positions in 32 us, 310 TFLOP/s); fp32 is bound by
+// the fp32 products (16 trees of 26 nodes there in 33 us, 66 TFLOP/s of a library's 153); a single sequence the launch, the block table and K/V reads one
 // after the other (6.8 us in a graph for 4 nodes behind 600 positions).
 // Why chunks are shared: with a ring of its own per wave, no barriers but a quarter of the bytes in flight per
 // position loaded, the chains above took 343 us instead of 295. Rows that one workgroup reads are loaded past the
 // L2s' replacement (`once`: 297 us against 314), rows that several read through the L2 (16 trees of 64 nodes behind
 // 8000 positions: 146 against 155). CK is what a ring of two leaves of the LDS to two workgroups (one at 512-byte rows).
-template <typename Tag, int D, int CW, int CK>
+template <typename Tag, int D, int CW, int CK, bool SMALL>
 __global__ __launch_bounds__(256, D * elem<Tag>::bytes * CK < 32768 ? 2 : 1) void tree_columns_kernel(const tree_args a) {
   using S = tshape<Tag, D>;
   constexpr bool F32 = S::EB == 4;
@@ -400,31 +307,45 @@ __global__ __launch_bounds__(256, D * elem<Tag>::bytes * CK < 32768 ? 2 : 1) voi
   // ---- direct loads ----
   const int64_t head_bytes = ((int64_t)1 << a.log2_bs) * RB;
   const int64_t blk_bytes = 2 * (int64_t)a.num_kv_heads * head_bytes, v_off = a.num_kv_heads * head_bytes;
-  const int sub_mask = (1 << (a.log2_bs - 4)) - 1;
+  const int sub_mask = SMALL ? 0 : (1 << (a.log2_bs - 4)) - 1, bs_mask = (1 << a.log2_bs) - 1;
   const int32_t* const table = a.block_tables + (int64_t)seq * a.max_nb;
   const char* const pool_kvh = a.pool + kvh * head_bytes;
   const int last_tile = (limit - 1) >> 4, tile0 = 2 * chunk0 + TILES * wave;
   const int lrow = lane / S::PPR, lpiece = lane % S::PPR;
   const int n = (32 * chunks + CK - 1) / CK;
+  constexpr int IDS = SMALL ? 16 * TILES : TILES;   // block ids of a wave's part of a slot
   int id0 = 0;
   auto tile_of = [&](int k, int t) { return min(tile0 + CK / 16 * k + t, last_tile); };
-  auto load_ids = [&](int k) {                  // lane j: the block of tile j % TILES of slot k + j / TILES
-    const int b = table[(tile_of(k + lane / TILES, lane % TILES) << 4) >> a.log2_bs];
+  auto load_ids = [&](int k) {                  // lane j: block j % IDS (of a tile; SMALL: of a row) of slot k + j / IDS
+    const int slot = k + lane / IDS, j = lane % IDS;
+    const int tile = SMALL ? tile_of(slot, j / 16) : tile_of(slot, j);
+    const int b = table[(SMALL ? min(16 * tile + j % 16, limit - 1) : 16 * tile) >> a.log2_bs];
     return (b < 0 || b >= a.num_blocks) ? 0 : b;   // host validates; stay inside the pool
   };
   int ids = load_ids(0);
   asm volatile("" : "+v"(ids));                 // the block ids have landed: no wait inside the loop
   auto issue = [&](int k) {
-    if (k - id0 >= 64 / TILES) {                // uniform, once per 64 or 32 slots
+    if (k - id0 >= 64 / IDS) {                  // uniform, once per 64 or 32 slots (SMALL: 4 or 2)
       id0 = k;
       ids = load_ids(k);
     }
 #pragma unroll
     for (int t = 0; t < TILES; ++t) {
       const int tile = tile_of(k, t), rmax = limit - 1 - 16 * tile;   // rows past it repeat the last position
-      const int64_t b = __builtin_amdgcn_readlane(ids, TILES * (k - id0) + t);
-      const char* const base = pool_kvh + b * blk_bytes + (int64_t)(tile & sub_mask) * S::TB;
       char* const dst = lds + (k & 1) * SLOT + (TILES * wave + t) * S::TB;
+      if constexpr (SMALL) {
+#pragma unroll
+        for (int i = 0; i < S::TB / 1024; ++i) {
+          const int r = S::RPL * i + lrow, at = min(r, rmax);
+          const int64_t b = __shfl(ids, IDS * (k - id0) + 16 * t + at);
+          const char* const row = pool_kvh + b * blk_bytes + (int64_t)(at & bs_mask) * RB;
+          s_dma16_l2p(row + 16 * (lpiece ^ S::kswz(r)), dst + 1024 * i);
+          s_dma16_l2p(row + v_off + 16 * (lpiece ^ S::vswz(r)), dst + HALF + 1024 * i);
+        }
+        continue;
+      }
+      const int64_t b = __builtin_amdgcn_readlane(ids, SMALL ? 0 : TILES * (k - id0) + t);
+      const char* const base = pool_kvh + b * blk_bytes + (int64_t)(tile & sub_mask) * S::TB;
 #pragma unroll
       for (int i = 0; i < S::TB / 1024; ++i) {
         const int r = S::RPL * i + lrow;
@@ -795,26 +716,25 @@ __global__ __launch_bounds__(64 * NW) void tree_join_kernel(const tree_args a) {
   st_through(a.out + (int64_t)row * a.out_row_bytes + ((int64_t)head * D + 4 * d4) * sizeof(T), t);
 }
 
-template <typename Tag, int D>
-static void launch_columns(const tree_args& a, int num_work, int blocks, int num_split, hipStream_t stream) {
+template <typename Tag, int D, bool SMALL>
+static void launch_columns_as(const tree_args& a, int num_work, int blocks, hipStream_t stream) {
   const dim3 grid(num_work), block(256);
   if constexpr (tshape<Tag, D>::RB == 128)
-    if (blocks == 1) hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 1, 128>), grid, block, 0, stream, a);
-  if (blocks == 2) hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 2, 64>), grid, block, 0, stream, a);
-  else if (blocks == 4) hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 4, 64>), grid, block, 0, stream, a);
+    if (blocks == 1) hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 1, 128, SMALL>), grid, block, 0, stream, a);
+  if (blocks == 2) hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 2, 64, SMALL>), grid, block, 0, stream, a);
+  else if (blocks == 4) hipLaunchKernelGGL((tree_columns_kernel<Tag, D, 4, 64, SMALL>), grid, block, 0, stream, a);
+}
+
+template <typename Tag, int D>
+static void launch_columns(const tree_args& a, int num_work, int blocks, int num_split, hipStream_t stream) {
+  if (a.log2_bs < 4) launch_columns_as<Tag, D, true>(a, num_work, blocks, stream);
+  else launch_columns_as<Tag, D, false>(a, num_work, blocks, stream);
   if (num_split > 0 && !a.arrivals) {
     const dim3 rows(num_split, (a.num_heads * (D / 4) + 63) / 64);
     // partial_slots / num_split: the parts of a row on average
     if (a.slots > 16 * (int64_t)num_split) hipLaunchKernelGGL((tree_join_kernel<Tag, D, 4>), rows, dim3(256), 0, stream, a);
     else hipLaunchKernelGGL((tree_join_kernel<Tag, D, 1>), rows, dim3(64), 0, stream, a);
   }
-}
-
-template <typename Tag>
-static void launch_rows(const tree_args& a, int num_rows, int head_dim, hipStream_t stream) {
-  const dim3 grid(num_rows, a.num_heads);
-  if (head_dim == 64) hipLaunchKernelGGL((tree_rows_kernel<Tag, 64>), grid, dim3(64), 0, stream, a);
-  else hipLaunchKernelGGL((tree_rows_kernel<Tag, 128>), grid, dim3(64), 0, stream, a);
 }
 
 }  // namespace tb
@@ -1164,15 +1084,8 @@ extern "C" int32_t tb_tree_attention(const void* q, int64_t q_row_stride, const 
   a.num_kv_heads = num_kv_heads;
   a.rep = num_heads / num_kv_heads;
   a.log2_bs = __builtin_ctz(block_size);
-  a.scale = scale;
   a.positions = positions;
   a.rope = rope_tables{rope_cos, rope_sin, rope_max_position};
-  if (block_size < 16) {       // a 16-position tile would lie in several blocks
-    if (dtype == TB_DTYPE_F32) launch_rows<f32_t>(a, num_rows, head_dim, stream);
-    else if (dtype == TB_DTYPE_F16) launch_rows<f16_t>(a, num_rows, head_dim, stream);
-    else launch_rows<bf16_t>(a, num_rows, head_dim, stream);
-    TB_RETURN_LAUNCH_STATUS();
-  }
   TB_CHECK_ARG(num_work >= 0 && num_split_rows >= 0 && num_split_rows <= num_rows && partial_slots >= 0);
   TB_CHECK_ARG((column_blocks == 1 && head_dim * eb == 128) || column_blocks == 2 || column_blocks == 4);
   TB_CHECK_ARG((num_split_rows == 0 || partial_slots > 0));

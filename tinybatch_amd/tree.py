@@ -387,7 +387,7 @@ def tree_attention(q: torch.Tensor, pool: torch.Tensor, meta: TreeMetadata, *, s
     scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
     lock = ws = arrivals = None
     ws_bytes = 0
-    if slots and bs >= 16:
+    if slots:
         lock, ws, ws_bytes, arrivals, units = _scratch(device, stream, slots * hq * (d + 2) * 4, units)
     try:
         st = _lib.lib().tb_tree_attention(
