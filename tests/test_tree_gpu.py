@@ -86,6 +86,21 @@ def test_attention_block_sizes(bs, dtype, d):
     c.check(tree_attention(c.q.to(DEV), c.pool.to(DEV), c.meta()))
 
 
+@pytest.mark.parametrize("bs", [1, 2, 8])
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hq,hkv,d,sizes,cached", [(8, 2, 64, [8, 3], [2000, 37]), (14, 2, 64, [9, 2, 0], [900, 0, 5]),
+                                                   (14, 2, 64, [70, 1], [1500, 300]), (8, 2, 128, [5, 33], [600, 1]),
+                                                   (8, 2, 128, [130, 17], [95, 1100])])
+def test_attention_in_small_blocks(hq, hkv, d, sizes, cached, dtype, bs):
+    """Every number of column blocks and contexts in parts, the rows of a tile in blocks of their own; an eager call
+    and one that joins its parts by a launch."""
+    c = Case(bs + d, hq, hkv, d, dtype, sizes, cached, bs=bs)
+    m, q, pool = c.meta(), c.q.to(DEV), c.pool.to(DEV)
+    c.check(tree_attention(q, pool, m))
+    m.units = 0
+    c.check(tree_attention(q, pool, m))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (8, 2, 128)])
 def test_attention_around_its_chunks(hq, hkv, d, dtype):

@@ -83,12 +83,8 @@ struct tshape {
   static constexpr int EB = elem<Tag>::bytes;
   static constexpr int RB = EB * D;             // bytes per K or V row
   static constexpr int TB = 16 * RB;            // bytes of a 16-position tile
-  static constexpr int CK = 32;                 // positions per chunk
-  static constexpr int HALF = CK * RB;          // a chunk's K (or V) rows
-  static constexpr int SLOT = 2 * HALF;
   static constexpr int PPR = RB / 16;           // 16-byte pieces per row
   static constexpr int RPL = 64 / PPR;          // rows per direct load
-  static constexpr int LD = HALF / 1024;        // direct loads per half
   static constexpr int QS = PPR / 2;            // 16-byte pieces of a lane's q (the other half's lane holds the rest)
   static constexpr int NB = D / 32;             // O^T blocks of 32 dims
   // K row r keeps its piece p in slot p ^ kswz(r), V row r in slot p ^ vswz(r), so that the operand
