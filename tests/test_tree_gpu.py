@@ -101,6 +101,20 @@ def test_attention_in_small_blocks(hq, hkv, d, sizes, cached, dtype, bs):
     c.check(tree_attention(q, pool, m))
 
 
+@pytest.mark.parametrize("seed", range(48))
+def test_attention_of_random_steps(seed):
+    """Steps of any geometry, type, block size and raggedness, every third one with masks of its own."""
+    g = np.random.default_rng(1000 + seed)
+    dtype, d = TYPES[seed % 3], (64, 128)[seed // 3 % 2]
+    hkv, rep = int(g.integers(1, 4)), int(g.choice([1, 2, 3, 5, 7, 8, 12, 33]))
+    seqs, most = int(g.integers(1, 6)), int(g.choice([1, 6, 40, 150]))
+    sizes = [int(g.integers(0 if seqs > 1 else 1, most + 1)) for _ in range(seqs)]
+    cached = [int(g.choice([0, 1, 17, 63, 64, 300, 1500])) for _ in range(seqs)]
+    visible = [g.random((n, n)) < g.choice([0.0, 0.1, 0.9]) for n in sizes] if seed % 3 == 2 else None
+    c = Case(2000 + seed, hkv * rep, hkv, d, dtype, sizes, cached, bs=int(g.choice([1, 2, 8, 16, 32, 64])), visible=visible)
+    c.check(tree_attention(c.q.to(DEV), c.pool.to(DEV), c.meta()))
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (8, 2, 128)])
 def test_attention_around_its_chunks(hq, hkv, d, dtype):
