@@ -264,12 +264,14 @@ __device__ __forceinline__ void tree_join_here(const tree_args& a, int row0, int
 // 128, bf16: 1.9 GB in 293 to 308 us, 6.2 to 6.5 TB/s); with many the products and the softmax between them (16
 // trees of 64 nodes there: 80 GFLOP in 119 to 128 us, 620 to 670 TFLOP/s; at head dim 64 the softmax weighs
 // twice as much: 32 trees of 60 nodes at 14 / 2 heads behind 2000 positions in 32 us, 310 TFLOP/s); fp32 is bound by
-// the fp32 products (16 trees of 26 nodes there in 33 us, 66 TFLOP/s of a library's 153); a single sequence the launch, the block table and K/V reads one
-// after the other (6.8 us in a graph for 4 nodes behind 600 positions).
+// the fp32 products (16 trees of 26 nodes there in 33 us, 66 TFLOP/s of a library's 153); a single sequence the
+// launch, the block table and K/V reads one after the other (6.8 us in a graph for 4 nodes behind 600 positions).
 // Why chunks are shared: with a ring of its own per wave, no barriers but a quarter of the bytes in flight per
 // position loaded, the chains above took 343 us instead of 295. Rows that one workgroup reads are loaded past the
 // L2s' replacement (`once`: 297 us against 314), rows that several read through the L2 (16 trees of 64 nodes behind
-// 8000 positions: 146 against 155). CK is what a ring of two leaves of the LDS to two workgroups (one at 512-byte rows).
+// 8000 positions: 146 against 155). CK is what a ring of two leaves of the LDS to two workgroups (one at 512-byte rows);
+// chunks of 32 positions in a ring of four, for one set of waves after the other, have half as much again under way, but
+// 301 us against 291 for 48 chains behind 12000 positions, 27.4 against 21.7 for 4 trees of 24 nodes behind 4000.
 template <typename Tag, int D, int CW, int CK, bool SMALL>
 __global__ __launch_bounds__(256, D * elem<Tag>::bytes * CK < 32768 ? 2 : 1) void tree_columns_kernel(const tree_args a) {
   using S = tshape<Tag, D>;
