@@ -414,6 +414,33 @@ def test_verify_rows_with_strides():
     check_verify(parents, tokens, u, probs, draft, got)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("vocab", [50, 5003])
+def test_verify_of_entries_that_are_no_probabilities(vocab, dtype):
+    """NaN and entries below 0 count as 0 in the draft's rows as in the target's: in the tests, in the sums
+    after refusals and in the token drawn at the end."""
+    differ = 0
+    for seed in range(8):
+        parents, tokens, u, probs, draft = verify_case(70 + seed, [30, 8, 66, 3, 1], vocab, dtype, True, sharp=1.5, noise=1.5)
+        g = torch.Generator().manual_seed(seed)
+        dirty = []
+        for t in (probs, draft):
+            r = torch.rand(t.shape, generator=g)
+            t = torch.where(r < 0.15, torch.full_like(t, float("nan")), torch.where(r < 0.3, -t, t))
+            dirty.append(t)
+        probs, draft = dirty
+        zeros = [torch.where(t > 0, t, torch.zeros_like(t)) for t in (probs, draft)]
+        got = on_gpu(parents, tokens, u, probs, draft)
+        check_verify(parents, tokens, u, *zeros, got)
+        check_verify(parents, tokens, u, zeros[0], None, on_gpu(parents, tokens, u, probs))
+        at = 0
+        for t in parents:                              # children that only a draft entry of 0 lets through
+            differ += sum(bool(zeros[0][at + p, tokens[at + i]] > 0) and not bool(draft[at + p, tokens[at + i]] > 0)
+                          for i, p in enumerate(t) if i)
+            at += len(t)
+    assert differ > 20
+
+
 def test_verify_keeps_the_target_s_distribution():
     # 20000 pairs of drafts of one distribution, drawn or taken as they are: the first emitted token's counts against the target's
     # probabilities, chi-square with 11 degrees of freedom (its 1 - 1e-9 quantile is 66)

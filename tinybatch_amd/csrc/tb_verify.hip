@@ -100,6 +100,13 @@ struct verify_tree {
       : tok((int32_t*)lds), par(tok + nodes), p((float*)(par + nodes)), q(p + nodes), u(q + nodes) {}
 };
 
+// A draft's entry as it counts: 0 where it is NaN or below 0. (The target's entries need none of it: a test and a
+// weight ask for more than 0, which neither a NaN nor a value below 0 less something gives.)
+template <typename T>
+__device__ __forceinline__ float counted(T x) {
+  return fmaxf((float)x, 0.f);
+}
+
 template <typename T>
 __device__ __forceinline__ void load_tree(const verify_args& a, const verify_tree& t, int row0, int n) {
   for (int i = threadIdx.x; i < n; i += blockDim.x) {
@@ -110,7 +117,7 @@ __device__ __forceinline__ void load_tree(const verify_args& a, const verify_tre
     t.par[i] = par;
     t.u[i] = a.uniforms[row0 + i];
     t.p[i] = known ? (float)((const T*)a.probs)[(row0 + par) * a.probs_stride + x] : 0.f;
-    t.q[i] = known && a.draft ? (float)((const T*)a.draft)[(row0 + par) * a.draft_stride + x] : 0.f;
+    t.q[i] = known && a.draft ? counted(((const T*)a.draft)[(row0 + par) * a.draft_stride + x]) : 0.f;
   }
 }
 // The same from what launch 0 kept; entries past the sequence's nodes hold anything.
@@ -272,7 +279,7 @@ struct verify_row {
   // what is left of a token whose values are x and y
   __device__ __forceinline__ double left(T x, T y, uint32_t gone) const {
     double w = (double)(float)x;
-    if constexpr (DRAWN) w = fma(-a, (double)(float)y, w);
+    if constexpr (DRAWN) w = fma(-a, (double)counted(y), w);
     else if (gone & 1) w = 0.;
     return w > 0. ? w : 0.;
   }
