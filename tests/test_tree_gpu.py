@@ -211,6 +211,49 @@ def test_attention_scores_far_apart(dtype):
     c.check(tree_attention(c.q.to(DEV), c.pool.to(DEV), c.meta()))
 
 
+@pytest.mark.parametrize("hq", [1, 33])
+def test_attention_of_a_flat_tail_behind_a_dominant_key(hq):
+    """fp16: 2^18 keys of a weight of 2^-25.4 beside one of 1 hold 0.6% of the sum. 512 sequences share them as a
+    prefix, so that contexts stay whole and a wave's weights all refer to the dominant one. A weight is rounded to a
+    multiple of 2^-24 and the reference maximum lies 7 below the first one: half a step is 2^-32 of the dominant weight, 1.1%
+    of a tail weight; 2^-10 bounds the roundings of the output, of the scores and of the sums."""
+    n, B, d, bs = 1 << 18, 512, 64, 128
+    pool = torch.zeros(n // bs + B, 2, 1, bs, d, dtype=torch.float16)
+    pool[:n // bs, 1] = 1.0
+    pool[0, 0, 0, 5, 0], pool[0, 1, 0, 5] = 17.6, 0.0              # the dominant key: its value is 0
+    pool[n // bs:, 0, :, :, 0], pool[n // bs:, 1] = -100.0, 0.0    # the nodes hold nothing
+    score = float(pool[0, 0, 0, 5, 0])
+    q = torch.zeros(B, hq, d, dtype=torch.float16)
+    q[:, :, 0] = 1.0
+    prefix = list(range(n // bs))
+    meta = build_tree_metadata([[-1]] * B, [n] * B, [prefix + [n // bs + b] for b in range(B)], block_size=bs,
+                               num_blocks=pool.shape[0], num_heads=hq, num_kv_heads=1, head_dim=d, dtype=torch.float16)
+    assert meta.split_np.shape[0] == 0                             # the case that the test is about
+    got = tree_attention(q.to(DEV), pool.to(DEV), meta.to(DEV), scale=1.0).cpu().double()
+    tail = (n - 1) * np.exp(-score)
+    want = tail / (1 + tail)
+    assert 0.005 < want < 0.007
+    assert ((got - want).abs() <= want * (2.0 ** -32 / np.exp(-score) + 2.0 ** -10)).all(), got.unique() / want
+
+
+@pytest.mark.parametrize("step", [0.0, 0.004, 0.016, 0.03])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_of_scores_past_24_bits(dtype, step):
+    # scores of about 2^25.6 (in powers of two) that rise by up to some tens: in 32 bits they are off by 1 and more
+    # themselves, and the weights with them, but a mean of the values it stays
+    c = Case(16, 2, 1, 64, dtype, [2], [700])
+    for pos in range(702):
+        block = c.pool[c.tables[0][pos // 16], 0, :, pos % 16]
+        block.fill_(2080.0)
+        block[:, 0] = step * (pos // 64)
+    c.q.fill_(2080.0)
+    got = tree_attention(c.q.to(DEV), c.pool.to(DEV), c.meta()).cpu().double().view(2, 2, 64)
+    v = torch.cat([c.pool[b, 1, 0] for b in c.tables[0]])[:702].double()
+    assert torch.isfinite(got).all()
+    slack = (HALF[dtype] + 702 * 2.0 ** -24) * v.abs().max(0).values
+    assert (got <= v.max(0).values + slack).all() and (got >= v.min(0).values - slack).all()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("d", [64, 128])
 def test_rope_positions_are_depths(dtype, d):

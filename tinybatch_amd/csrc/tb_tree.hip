@@ -28,7 +28,9 @@
 // element type for the product, and their sum is taken of the rounded ones. fp32:
 // v_mfma_f32_32x32x2_f32, nothing rounded further. The reference maximum of a column moves
 // only when a score outgrows it by 8 (weights to 2^8), so that the accumulators are rescaled
-// a few times per context.
+// a few times per context. fp16 weights end at 2^-25: they refer to a maximum 7 lower (the largest one 2^7 to
+// 2^15), so that the tail of 2^18 keys of a weight of 2^-25.4 beside one of 1 is there to 1.1% instead of
+// missing; below 2^-32 of the dominant weight it still does.
 #include <algorithm>
 #include <cmath>
 #include <exception>
@@ -283,6 +285,7 @@ __global__ __launch_bounds__(256, D * elem<Tag>::bytes * CK < 32768 ? 2 : 1) voi
   constexpr int WS = 64 * (16 * NB + 2);        // floats of a wave's state
   constexpr int LDS = SETS > 1 && NW * WS * 4 > 2 * SLOT ? NW * WS * 4 : 2 * SLOT;
   static_assert(TL >= 1 && TILES >= 1, "a tile for every wave");
+  constexpr float LIFT = std::is_same_v<T, _Float16> ? 7.f : 0.f;   // of the weights, in powers of two
   __shared__ __align__(1024) char lds[LDS];
 
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
@@ -461,8 +464,9 @@ __global__ __launch_bounds__(256, D * elem<Tag>::bytes * CK < 32768 ? 2 : 1) voi
 #pragma unroll
     for (int e = 2; e < 16 * TL; e += 2) cm = max3_f32(cm, sc[e >> 4][e & 15], sc[e >> 4][(e & 15) + 1]);
     cm *= sl2e;
-    if (__any(cm > m + 8.f)) {
-      const float m_new = fmaxf(m, max_xor32(cm));
+    // (a score of size 2^24 or more is off by 1 and more itself: what its weight may pass 2^15 by is taken off)
+    if (__any(cm > (LIFT > 0.f ? fmaf(fabsf(m), -0x1p-20f, m + (8.f + LIFT)) : m + 8.f))) {
+      const float m_new = fmaxf(m, max_xor32(cm) - LIFT);
       const float alpha = fast_exp2(m - (m_new == -INFINITY ? 0.f : m_new));   // 0 while m = -inf
       m = m_new;
       l *= alpha;
@@ -476,6 +480,7 @@ __global__ __launch_bounds__(256, D * elem<Tag>::bytes * CK < 32768 ? 2 : 1) voi
 #pragma unroll
       for (int r = 0; r < 16; ++r) sc[t][r] = fast_exp2(fmaf(sc[t][r], sl2e, neg_m));
     if constexpr (!F32) {
+      float sum = 0.f;                          // of the chunk by itself: small weights count beside a large l
 #pragma unroll
       for (int w = 0; w < 2 * TL; ++w) {
         float p[8];
@@ -483,8 +488,9 @@ __global__ __launch_bounds__(256, D * elem<Tag>::bytes * CK < 32768 ? 2 : 1) voi
         for (int j = 0; j < 8; ++j) p[j] = sc[w >> 1][8 * (w & 1) + j];
         pb[w] = smath<Tag>::pack8(p);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) l = cmath<Tag>::add2(pb[w][j], ones, l);   // of the rounded P that multiplies V
+        for (int j = 0; j < 4; ++j) sum = cmath<Tag>::add2(pb[w][j], ones, sum);   // of the rounded P that multiplies V
       }
+      l += sum;
     } else {
 #pragma unroll
       for (int t = 0; t < TL; ++t) {
