@@ -676,6 +676,7 @@ int32_t tb_rms_norm_partials(const float* partials, int32_t splits, void* residu
  * first, tb_kv_append), whatever its depth; its RoPE position is cached[b] + depth.
  * At most TB_TREE_MAX_NODES nodes per tree where a limit is named. */
 #define TB_TREE_MAX_NODES 1024
+#define TB_TREE_MOST_PARTIAL_BYTES (128 << 20)   /* of tb_tree_attention's workspace, whatever the work list */
 
 /* A step's arrays from the trees (host memory, no device call): parents [num_rows], a node's parent
  * inside its tree (-1 for node 0, else an earlier node); row_starts [num_seqs + 1] from 0. Writes

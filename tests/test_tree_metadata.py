@@ -273,3 +273,17 @@ def test_work_covers_every_context_once(hq, hkv, d, dtype, sizes, cached):
             assert sorted(by) == list(range(len(by))) and all(n == len(by) for _, n in by.values())
             assert [by[i][0] for i in range(len(by))] == sorted(x for x, _ in by.values())
     assert sorted(used) == list(range(m.partial_slots)) and sorted(m.split_np.tolist()) == sorted(records)
+
+
+@pytest.mark.parametrize("hq,hkv,d,dt,sizes,cached", [
+    (64, 8, 128, 2, [512] * 2, [500000, 499000]), (32, 8, 128, 2, [1024] * 4, [100000, 100001, 99000, 1]),
+    (64, 8, 128, 2, [1024] * 8, list(range(30000, 30008))), (40, 40, 128, 2, [773], [98924]),
+    (14, 2, 64, 1, [1024] * 64, [1 << 20] * 64), (4, 4, 128, 0, [60], [1 << 24])])
+def test_partials_stay_within_their_bound(hq, hkv, d, dt, sizes, cached):
+    """Large trees behind long contexts: what a call needs beside the cache does not grow with them."""
+    L, counts = _lib.lib(), np.zeros(5, dtype=np.int32)
+    c, n = np.array(cached, dtype=np.int32), np.array(sizes, dtype=np.int32)
+    assert L.tb_build_tree_work(c.ctypes.data, n.ctypes.data, len(sizes), hq, hkv, d, dt, 256, 8, None, 0, None, 0,
+                                counts.ctypes.data) == _lib.TB_OK
+    assert L.tb_tree_attention_workspace_bytes(int(counts[2]), hq, d) <= 128 << 20
+    assert counts[0] >= 256 or counts[2] > 0               # nor is the chip left empty for it

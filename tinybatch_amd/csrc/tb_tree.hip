@@ -774,6 +774,14 @@ inline int tree_even(int chunks, int part, int round) {
   return ((chunks + parts - 1) / parts + round - 1) / round * round;
 }
 
+// What a call's partials may take. Without a bound the search cuts long contexts of large trees into hundreds of MB for
+// what the price says is a few percent. Of 1500 random steps of up to 128 sequences and 130000 positions 63 are cut more
+// coarsely for it, at a price 2.4% higher on average and 8.5% at most; 64 MiB would touch 111, up to 24%. Us a call without
+// and with it, bf16, heads of 128: 4 trees of 1024 nodes at 32 / 8 behind 50000 to 100000 positions 4830 and 4904, 8 of
+// 1024 at 64 / 8 behind 15000 to 30000 5829 and 5734, one of 773 at 40 / 40 behind 98000 1500 and 1472, 40 of 53 at 64 / 8
+// behind 30000 to 60000 3908 and 4065.
+constexpr double MOST_PARTIAL_BYTES = TB_TREE_MOST_PARTIAL_BYTES;
+
 // The part length in rounds of least cost, and that cost; 0: no context is cut.
 int tree_part_rounds(const tree_price& price, const int32_t* cached, const int32_t* nodes, int num_seqs, int rep,
                      int cols, int num_kv_heads, double slot_bytes, double& least) {
@@ -804,6 +812,7 @@ int tree_part_rounds(const tree_price& price, const int32_t* cached, const int32
       pieces.push_back({r - even * (parts - 1), wgs});
       count += wgs * parts;
     }
+    if (slots * slot_bytes > MOST_PARTIAL_BYTES) return HUGE_VAL;
     // the longest first, each where a place is free first: a piece starts when those before it have
     // filled the places evenly
     std::sort(pieces.begin(), pieces.end(), std::greater<>());
