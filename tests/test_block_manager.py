@@ -112,3 +112,26 @@ def test_compact_moves_live_blocks_down_and_remaps_tables_and_cache():
     # allocation continues right above the live blocks
     t, _ = bm.allocate_prompt([7])
     assert t == [len(live)]
+
+
+def test_append_slot_with_blocks_reserved_behind():
+    """A table lengthened for a step of drafted tokens: later positions take the blocks that are there, and what is
+    published for the prefix cache is the block that filled."""
+    bm = bm_(num_blocks=10)
+    seq = list(range(6))
+    table, _ = bm.allocate_prompt(seq)
+    table += bm.allocate_private(2, [])                  # for drafts behind position 6
+    want = list(table)
+    for token in range(6, 17):                           # positions 6 .. 16
+        grown = bm.append_slot(table, seq)
+        seq.append(token)
+        assert grown == (token == 16) and table[:4] == want
+        assert bm.blocks[table[len(seq) // 4 - 1]].prefix_hash is not None or len(seq) % 4 != 1
+    assert len(table) == 5
+    assert bm.allocate_prompt(seq[:16])[0] == want        # the four full blocks, found by their content
+    plain = bm_(num_blocks=10)
+    t2, _ = plain.allocate_prompt(list(range(6)))
+    for n in range(6, 17):
+        plain.append_slot(t2, list(range(n)))
+    assert {k: plain.blocks[b].token_ids for k, b in plain.cache.items()} == \
+           {k: bm.blocks[b].token_ids for k, b in bm.cache.items()}

@@ -131,19 +131,23 @@ class BlockManager:
 
     def append_slot(self, table: list[int], seq_token_ids: list[int]) -> bool:
         """Make room for the token at index len(seq_token_ids) (call it before
-        that token joins the sequence). Returns True when a block was added."""
+        that token joins the sequence). Returns True when a block was added: a table
+        that reaches further already (blocks for drafted tokens) keeps its blocks."""
         bs = self.block_size
         pos = len(seq_token_ids)
-        if pos % bs == 0:
+        idx = pos // bs
+        added = pos % bs == 0 and idx >= len(table)
+        if added:
             blk = self._fresh()
             blk.ref_count = 1
             blk.token_ids = []
             table.append(blk.block_id)
-            if self.enable_prefix_caching and len(table) >= 2:
-                self._publish(table, len(table) - 2, seq_token_ids)
-            return True
-        self.blocks[table[-1]].token_ids = list(seq_token_ids[(len(table) - 1) * bs:pos])
-        return False
+        if pos % bs:
+            idx = min(idx, len(table) - 1)
+            self.blocks[table[idx]].token_ids = list(seq_token_ids[idx * bs:pos])
+        elif self.enable_prefix_caching and idx >= 1:
+            self._publish(table, idx - 1, seq_token_ids)
+        return added
 
     def _publish(self, table: list[int], idx: int, seq_token_ids: list[int]) -> None:
         blk = self.blocks[table[idx]]
