@@ -149,7 +149,7 @@ SIGNATURES = {
     "tb_tree_attention_workspace_bytes": (c_sz, [c_i32, c_i32, c_i32]),
     "tb_tree_verify_workspace_bytes": (c_sz, [c_i32, c_i32, c_i32]),
     "tb_tree_verify": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_i32, c_i32,   # probs, stride, draft, stride, vocab, dtype
-                               c_vp, c_vp, c_vp, c_vp, c_i32, c_i32,     # tokens, uniforms, parents, row starts, seqs, children
+                               c_vp, c_vp, c_vp, c_vp, c_i32, c_i32,     # tokens, uniforms, parents, row starts, seqs, max refusals
                                c_vp, c_vp, c_vp, c_i32, c_vp, c_sz,      # outputs, width, workspace, bytes
                                c_vp, c_i32, c_vp]),                      # arrivals, units, stream
     "tb_tree_verify_greedy": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp, c_i32, c_vp]),

@@ -343,21 +343,21 @@ __global__ __launch_bounds__(256, D * elem<Tag>::bytes * CK < 32768 ? 2 : 1) voi
           s_dma16_l2p(row + 16 * (lpiece ^ S::kswz(r)), dst + 1024 * i);
           s_dma16_l2p(row + v_off + 16 * (lpiece ^ S::vswz(r)), dst + HALF + 1024 * i);
         }
-        continue;
-      }
-      const int64_t b = __builtin_amdgcn_readlane(ids, SMALL ? 0 : TILES * (k - id0) + t);
-      const char* const base = pool_kvh + b * blk_bytes + (int64_t)(tile & sub_mask) * S::TB;
+      } else {
+        const int64_t b = __builtin_amdgcn_readlane(ids, TILES * (k - id0) + t);
+        const char* const base = pool_kvh + b * blk_bytes + (int64_t)(tile & sub_mask) * S::TB;
 #pragma unroll
-      for (int i = 0; i < S::TB / 1024; ++i) {
-        const int r = S::RPL * i + lrow;
-        const uint32_t row = (uint32_t)(min(r, rmax) * RB);
-        const uint32_t ko = row + 16 * (lpiece ^ S::kswz(r)), vo = row + 16 * (lpiece ^ S::vswz(r));
-        if (once) {
-          s_dma16_s(ko, base, dst + 1024 * i);
-          s_dma16_s(vo, base + v_off, dst + HALF + 1024 * i);
-        } else {
-          s_dma16_l2(ko, base, dst + 1024 * i);
-          s_dma16_l2(vo, base + v_off, dst + HALF + 1024 * i);
+        for (int i = 0; i < S::TB / 1024; ++i) {
+          const int r = S::RPL * i + lrow;
+          const uint32_t row = (uint32_t)(min(r, rmax) * RB);
+          const uint32_t ko = row + 16 * (lpiece ^ S::kswz(r)), vo = row + 16 * (lpiece ^ S::vswz(r));
+          if (once) {
+            s_dma16_s(ko, base, dst + 1024 * i);
+            s_dma16_s(vo, base + v_off, dst + HALF + 1024 * i);
+          } else {
+            s_dma16_l2(ko, base, dst + 1024 * i);
+            s_dma16_l2(vo, base + v_off, dst + HALF + 1024 * i);
+          }
         }
       }
     }
@@ -852,7 +852,12 @@ struct tree_piece {
 // only little is joined there, more where the step is short and the parts come in one turn of loads. Us a call, there
 // and by a launch: 13 nodes at 14 / 2 heads of 64, 600 positions, 10.5 and 12.7; 16 sequences of 18 nodes, 2000
 // positions, 14.7 and 12.7; 8 of 13 in fp32 15.6 and 12.8; 8 nodes at 32 / 8 heads of 128 in 9 parts 15.6 and 12.6.
-constexpr int JOIN_HERE_FLOATS = 4096, JOIN_ALWAYS_FLOATS = 2047, JOIN_HERE_PARTS = 16;
+// Fewer than 2048 floats (less than one turn of the 256 threads' loads, two of four floats each) are joined there
+// however long the step: 0.3 to 0.6 us more where the GPU is the slower side (16 sequences of 7 nodes at 8 / 2 heads of 64,
+// 4000 positions, 12.9 and 12.4), 2.5 less where the host is (1 of 7, 600, 10.1 and 12.6). A full turn in a long step goes to
+// the launch: 4 of 4 at 32 / 8 heads of 128, 4000 positions, 19.2 and 18.7 (in fp32 it would be better off there: 16 of 8 at
+// 8 / 2 heads of 64, 4000 positions, 25.9 and 27.5).
+constexpr int JOIN_HERE_FLOATS = 4096, JOIN_ALWAYS_FLOATS = 2048, JOIN_HERE_PARTS = 16;
 constexpr double JOIN_HERE_US = 10;
 
 }  // namespace
@@ -913,7 +918,7 @@ extern "C" int32_t tb_build_tree_work(const int32_t* cached, const int32_t* node
     if (parts > 1) {
       const int floats = std::min(cols, nodes[b] * rep) * head_dim;   // of a part
       here &= parts <= JOIN_HERE_PARTS &&
-              (floats <= JOIN_ALWAYS_FLOATS || (brief && floats * ((parts + 7) / 8) <= JOIN_HERE_FLOATS));
+              (floats < JOIN_ALWAYS_FLOATS || (brief && floats * ((parts + 7) / 8) <= JOIN_HERE_FLOATS));
       units += (int64_t)groups * num_kv_heads;
       for (int i = 0; i < nodes[b]; ++i, ++num_split)
         if (split && num_split < split_capacity) {
