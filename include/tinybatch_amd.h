@@ -684,8 +684,8 @@ int32_t tb_rms_norm_partials(const float* partials, int32_t splits, void* residu
  *   positions [num_rows]: cached[b] + depth, the RoPE positions; row_seq [num_rows];
  *   slot_mapping [num_rows] (tb_kv_append's): node i at position cached[b] + i of its block table.
  * cached NULL: the trees alone (depths for positions, no slots); the tables are then unread.
- * info [4]: the most refusals of a walk that leave a sibling to test (max_refusals below), the largest position plus one, and on an error what is wrong
- * and where: a parent (its row), a table too short or a block id outside the pool (the sequence;
+ * info [4]: the most refusals of a walk that leave a sibling to test (max_refusals below), the
+ * largest position plus one, and on an error what is wrong and where: a parent (its row), a table too short or a block id outside the pool (the sequence;
  * TB_ERR_INDEX for these two, TB_ERR_INVALID_ARG for the others), slots past 2^31 (the sequence), two nodes in
  * one slot, a node on a cached position of its own or another sequence (the block). */
 #define TB_TREE_FAULT_PARENT 1
@@ -710,8 +710,8 @@ int32_t tb_build_tree_rows(const int32_t* parents, const int32_t* row_starts, in
  *   mask [num_rows][mask_words] 32-bit words, bit j % 32 of word j / 32 = node j is seen; bits
  *     past the tree are ignored;
  *   work [num_work][12], split_rows [num_split_rows][4], column_blocks, partial_slots:
- *     tb_build_tree_work's for this call's sizes (device memory, 16-byte aligned); workspace: tb_tree_attention_workspace_bytes, 16-byte aligned, for contexts cut
- *     into parts. Calls that may overlap in time need their own workspace;
+ *     tb_build_tree_work's for this call's sizes (device memory, 16-byte aligned); workspace:
+ *     tb_tree_attention_workspace_bytes, 16-byte aligned, for contexts cut into parts. Calls that may overlap in time need their own workspace;
  *   arrivals (may be NULL; only where the list's counts[4] is not 0): arrival_units >= counts[4]
  *     counters, zero before the first call and left zero by every call; they save the launch that
  *     joins the parts. Calls that may overlap in time (two streams, two replayed graphs) need their own;
@@ -736,7 +736,8 @@ int32_t tb_tree_attention(const void* q, int64_t q_row_stride, const void* pool,
  * blocks per workgroup, and the arrival counters of a call that joins the parts in its one launch
  * (0: no parts, or too much to join there). work and split NULL: the counts alone. An entry is (first row, sequence,
  * cached, nodes, first column, kv head, first chunk of 32 positions, chunks, partial slot of node 0
- * or -1, whether no other entry reads its K/V rows, arrival counter, part | parts << 16), with 0 nodes for a padding entry; entry g is meant for XCD g % num_xcds. */
+ * or -1, whether no other entry of its sequence reads its K/V rows, arrival counter,
+ * part | parts << 16), with 0 nodes for a padding entry; entry g is meant for XCD g % num_xcds. */
 int32_t tb_build_tree_work(const int32_t* cached, const int32_t* nodes, int32_t num_seqs,
                            int32_t num_heads, int32_t num_kv_heads, int32_t head_dim, int32_t dtype,
                            int32_t num_cus, int32_t num_xcds, int32_t* work, int32_t work_capacity,
@@ -788,7 +789,8 @@ int32_t tb_tree_verify_greedy(const int64_t* target_ids, const int64_t* tokens, 
  * position cached + accepted[b][j] to position cached + j, j < num_accepted[b]. accepted and
  * num_accepted are tb_tree_verify's (device memory; rising nodes, entries past the count
  * unread); entries not behind their place are in it already. storage: the layers' pools,
- * layer_stride_bytes apart. Two sequences must not share the blocks that hold their nodes. */
+ * layer_stride_bytes apart. Two sequences must not share the blocks that hold their nodes. At most 65535
+ * sequences and layers. */
 int32_t tb_tree_commit(void* storage, int32_t num_layers, int64_t layer_stride_bytes, int64_t num_blocks,
                        const int32_t* block_tables, int32_t max_blocks_per_seq, const int32_t* cached,
                        int32_t num_seqs, const int32_t* accepted, int32_t width,

@@ -25,7 +25,8 @@
 //   S^T[pos][col] = K[pos][:] . q[col][:]        A = K rows from LDS, B = q in registers
 //   O^T[d][col]  += V^T[d][pos] . P^T[pos][col]  A = V^T from LDS, B = the S^T registers
 // 16-bit: v_mfma_f32_32x32x16, V^T by LDS transpose reads; the weights P are rounded to the
-// element type for the product, and their sum is taken of the rounded ones. fp32:
+// element type for the product, which takes both operands in one type (their lower halves would be a second
+// product for each V), and their sum is taken of the rounded ones. fp32:
 // v_mfma_f32_32x32x2_f32, nothing rounded further. The reference maximum of a column moves
 // only when a score outgrows it by 8 (weights to 2^8), so that the accumulators are rescaled
 // a few times per context. fp16 weights end at 2^-25: they refer to a maximum 7 lower (the largest one 2^7 to
@@ -263,17 +264,25 @@ __device__ __forceinline__ void tree_join_here(const tree_args& a, int row0, int
 // 32 columns each, 4 / CW the same columns, each a part of a chunk's positions, joined at the end.
 //
 // What bounds it: with few columns the reads of K/V (48 chains of 4 to 8 nodes behind 8192 positions at 32 / 8 heads of
-// 128, bf16: 1.9 GB in 293 to 308 us, 6.2 to 6.5 TB/s); with many the products and the softmax between them (16
-// trees of 64 nodes there: 80 GFLOP in 119 to 128 us, 620 to 670 TFLOP/s; at head dim 64 the softmax weighs
-// twice as much: 32 trees of 60 nodes at 14 / 2 heads behind 2000 positions in 32 us, 310 TFLOP/s); fp32 is bound by
-// the fp32 products (16 trees of 26 nodes there in 33 us, 66 TFLOP/s of a library's 153); a single sequence the
-// launch, the block table and K/V reads one after the other (6.8 us in a graph for 4 nodes behind 600 positions).
-// Why chunks are shared: with a ring of its own per wave, no barriers but a quarter of the bytes in flight per
-// position loaded, the chains above took 343 us instead of 295. Rows that one workgroup reads are loaded past the
-// L2s' replacement (`once`: 297 us against 314), rows that several read through the L2 (16 trees of 64 nodes behind
-// 8000 positions: 146 against 155). CK is what a ring of two leaves of the LDS to two workgroups (one at 512-byte rows);
-// chunks of 32 positions in a ring of four, for one set of waves after the other, have half as much again under way, but
-// 301 us against 291 for 48 chains behind 12000 positions, 27.4 against 21.7 for 4 trees of 24 nodes behind 4000.
+// 128, bf16: 1.9 GB in 293 to 309 us, 6.2 to 6.5 TB/s, the matrix unit busy 8% of the time). With many columns no unit
+// by itself: a wave's LDS reads, products and softmax follow one another, behind a barrier a chunk, and hide only the
+// other waves' of its SIMD. 16 trees of 64 nodes there, 80 GFLOP in 119 to 128 us (620 to 670 TFLOP/s; 137 to 151 once
+// some ms of it have brought the clock down): matrix unit 29%, vector unit 26%, LDS 15%, 4.6 of 8 waves on a CU on
+// average. 4 of 1024 nodes behind 25000 to 50000 positions: 47%, 42%, 25%, 6.8 of 8 (990 TFLOP/s behind 50000 to
+// 100000). At head dim 64 32 trees of 20 to 30 nodes at 14 / 2 heads behind 512 to 4096 positions in 22 us: 10%, 18%,
+// 5%, 3.4 of 8, waves waiting 46% of their time; 182 columns leave a quarter of two workgroups of 128 idle. fp32: 16
+// trees of 26 nodes there behind 1000 to 2000 positions in 33 us, 66 TFLOP/s of a library's 153: matrix unit 40%, 4.5
+// of 8 waves; at head dim 128 one wave a SIMD is all that the LDS has room for, and the matrix unit (44% for 8 of 32 at
+// 32 / 8 heads) waits for its softmax. A single sequence: the launch, the block table and K/V reads one after the other
+// (7.1 us in a graph for 5 nodes behind 600 positions).
+// Why chunks are shared: with a ring of its own per wave, no barriers but a quarter of the bytes in flight per position
+// loaded, the chains above took 343 us instead of 295. Rows that one workgroup of their sequence reads are loaded past
+// the L2s' replacement (`once`: 297 us against 314), rows that several read through the L2 (16 trees of 64 nodes behind
+// 8000 positions: 146 against 155). Sequences that share a prefix read its rows once each all the same (48 of 6 nodes
+// behind the same 8192 positions 122 us, behind positions of their own 256). CK is what a ring of two leaves of the LDS
+// to two workgroups (one at 512-byte rows); chunks of 32 positions in a ring of four, for one set of waves after the
+// other, have half as much again under way, but 301 us against 291 for 48 chains behind 12000 positions, 27.4 against
+// 21.7 for 4 trees of 24 nodes behind 4000.
 template <typename Tag, int D, int CW, int CK, bool SMALL>
 __global__ __launch_bounds__(256, D * elem<Tag>::bytes * CK < 32768 ? 2 : 1) void tree_columns_kernel(const tree_args a) {
   using S = tshape<Tag, D>;
@@ -294,7 +303,7 @@ __global__ __launch_bounds__(256, D * elem<Tag>::bytes * CK < 32768 ? 2 : 1) voi
   const int row0 = w0.x, seq = w0.y, cached = w0.z, nodes = w0.w;
   if (nodes == 0) return;                       // a padding entry (whole workgroup)
   const int set = wave / CW;                    // its tiles start at position 32 TL set of a chunk
-  const bool once = w2.y;                       // no other workgroup reads these K/V rows
+  const bool once = w2.y;                       // no other workgroup of its sequence reads these K/V rows
   const int col0 = w1.x + 32 * (wave % CW), kvh = w1.y, chunk0 = w1.z, chunks = w1.w;   // chunks of 32, chunk0 even
   const int limit = cached + nodes, ncols = nodes * a.rep;
   const int col = min(col0 + lcol, ncols - 1), my_row = col / a.rep, hd = kvh * a.rep + col - my_row * a.rep;
@@ -555,7 +564,10 @@ __global__ __launch_bounds__(256, D * elem<Tag>::bytes * CK < 32768 ? 2 : 1) voi
     }
   };
   // the slots that lie in the cache whole, then those with nodes: two loops, so that the mask costs the
-  // long one neither instructions nor registers
+  // long one neither instructions nor registers. The second is the slower one: a slot's mask words are loaded behind the
+  // next slot's K/V and wait for those too, and with four column blocks of 16 bits at head dim 128 it spills 21 to 27
+  // registers. Large trees behind short caches run in it: 8 of 512 nodes behind one position at 32 / 8 heads 103 us
+  // (matrix unit 14%, vector unit 43%).
   const int plain = max(0, min(n, (cached - 32 * chunk0) / CK));
   int k = 0;
   for (; k < plain; ++k) step(k, std::false_type{});
@@ -748,14 +760,15 @@ static void launch_columns(const tree_args& a, int num_work, int blocks, int num
 namespace {
 
 // What a work list costs, in us, fitted to the times of 87 steps in every number of column blocks and cut
-// (14 geometries and types, 1 to 100 sequences, contexts of 300 to 30000 positions, 2 to 128 nodes): the list it
-// picks is on average 0.9% slower than the best one, 8% at most. A round is a chunk of a workgroup. The blocks
-// of a workgroup are part of the pick: few read K/V once more per 32 CW columns, but waste fewer columns and have
-// their waves share a chunk's positions. 32 sequences of 26 nodes at 14 / 2 heads of 64 (182 columns), 2000
-// positions: 19.3 us with two blocks against 21.9 with four, in fp32 (16 sequences) 32.8 against 45.8; 32 of 32 nodes
-// at 32 / 8 heads of 128, 8000 positions: 170 against 154. Up to 64 columns a third and fourth block would stand
-// idle; one block pays in rows of 128 bytes alone (chunks of 128 positions fit the LDS twice): 64 of 4 nodes at 14 / 2
-// heads of 64, 16000 positions, 66 us against 69.
+// (14 geometries and types, 1 to 100 sequences, contexts of 300 to 30000 positions, 2 to 128 nodes). Measured again on
+// all of them, the list that it picks is 1.9% slower than the best cut on average, more than 5% in 11 and 26% in one
+// (24 trees of 40 nodes at 14 / 2 heads of 64 in fp16, where two column blocks take 33.9 us and four 42.6). A round is a
+// chunk of a workgroup. The blocks of a workgroup are part of the pick: few read K/V once more per 32 CW columns, but
+// waste fewer columns and have their waves share a chunk's positions. 32 sequences of 26 nodes at 14 / 2 heads of 64 (182
+// columns), 2000 positions: 19.3 us with two blocks against 21.9 with four, in fp32 (16 sequences) 32.8 against 45.8; 32
+// of 32 nodes at 32 / 8 heads of 128, 8000 positions: 170 against 154. Up to 64 columns a third and fourth block would
+// stand idle; one block pays in rows of 128 bytes alone (chunks of 128 positions fit the LDS twice): 64 of 4 nodes at
+// 14 / 2 heads of 64, 16000 positions, 66 us against 69.
 struct tree_price {
   int chunks_round;            // chunks of 32 positions in a round
   int on_cu;                   // workgroups a CU holds

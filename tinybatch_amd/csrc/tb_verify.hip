@@ -35,9 +35,9 @@ namespace tb {
 // a launch of its own (a graph's replays may overlap, and then no counter is theirs alone).
 //
 // What bounds it: the reads of one target row, and one draft row, per sum where there are many sequences (64
-// chains over 151936 fp32 tokens: 78 MB in 24 us, 16 us at a copy's rate), the launches and their dependent
-// loads where there are few (one sequence: 10 us in a graph, 14 on the host); each further sum of a drawn tree
-// takes 3 to 7 us. 16 trees of 12 to 20 drawn nodes: 45 us, with up to six refusals.
+// chains over 151936 fp32 tokens: 78 MB in 25 us, 16 us at a copy's rate; in 16 bits 39 MB in 19 us), the launches and
+// their dependent loads where there are few (one sequence: 10 us in a graph, 14 to 15 on the host); each further sum of a
+// drawn tree takes 3 to 7 us. 16 trees of 12 to 20 drawn nodes: 46 to 50 us, 39 to 42 in 16 bits, with up to six refusals.
 // MAX_ROUNDS: a launch that turns out not to be needed costs 2 to 3 us, a sum that the end has to make up for
 // 50: those trees with at most 5 launches 48 us on average and 107 at worst, with 6 or more 45 and 55; 3 trees of
 // 15 to 60 nodes (walks of up to 8 refusals are possible, none needed 5) 32 with 5, 37 with 7, 40 with 9.
@@ -636,7 +636,8 @@ static void launch_verify(const verify_args& a, int rounds, hipStream_t stream) 
 }
 
 // The same walk for greedy targets: a child is kept where its token is the target's choice
-// after its parent. One wave per sequence.
+// after its parent. One wave per sequence: the host's call (10.6 us) is longer than the launch (2.0 us in a graph for one
+// chain of 6, 3.0 for 32 trees of 20 to 30 nodes).
 __global__ __launch_bounds__(64) void verify_greedy_kernel(const int64_t* target_ids, const int64_t* tokens,
                                                            const int32_t* parents, const int32_t* row_starts,
                                                            int32_t* accepted, int32_t* num_accepted,
