@@ -863,3 +863,20 @@ def test_calls_that_do_not_fit_are_refused():
         commit_tree(pool[None], meta, acc, num.long())
     with pytest.raises(ValueError, match="storage"):
         commit_tree(pool, meta, acc, num)
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,d,cached", [(torch.float32, 2, 1, 64, 560), (torch.float32, 8, 2, 64, 600), (torch.bfloat16, 32, 8, 128, 1000),
+                                                   (torch.float16, 8, 4, 128, 900)])
+def test_more_than_eight_parts_joined_both_ways(dtype, hq, hkv, d, cached):
+    # a second turn of loads in either join: the same bits there and by a launch, for any values
+    seen = 0
+    for seed in range(40):
+        c = Case(100 + seed, hq, hkv, d, dtype, [1 + seed % 9], [cached - seed])
+        m, q, pool = c.meta(), c.q.to(DEV), c.pool.to(DEV)
+        if not m.units or int(m.split_np[:, 2].max()) <= 8:
+            continue
+        seen += 1
+        here = tree_attention(q, pool, m)
+        m.units = 0
+        assert torch.equal(here, tree_attention(q, pool, m)), seed
+    assert seen > 5

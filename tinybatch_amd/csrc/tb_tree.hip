@@ -195,6 +195,11 @@ __device__ __forceinline__ void tree_q(vec16 (&q)[QS], const tree_args& a, int r
     for (int i = 0; i < 4; ++i) asm volatile("" : "+v"(q[s].w[i]));
 }
 
+// o += w x, rounded once: one form for the two joins below, which give the same bits.
+__device__ __forceinline__ void tree_add(float4_t& o, float4_t x, float w) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) o[j] = fmaf(x[j], w, o[j]);
+}
 // The join of a unit's parts by its last workgroup: what the others wrote is read past the L2s, which the
 // XCDs do not share. Thread = 4 dims of a column.
 template <typename Tag, int D, int CW>
@@ -238,7 +243,7 @@ __device__ __forceinline__ void tree_join_here(const tree_args& a, int row0, int
           const float w = p0 + k < parts ? fast_exp2(ml[t][k].x - safe) : 0.f;   // 0 for a part that saw nothing
           if (p0 + k < parts) {
             L[t] = fmaf(ml[t][k].y, w, L[t]);
-            o[t] += float4_t{lo[t][k].x, lo[t][k].y, hi[t][k].x, hi[t][k].y} * w;
+            tree_add(o[t], float4_t{lo[t][k].x, lo[t][k].y, hi[t][k].x, hi[t][k].y}, w);
           }
         }
         M[t] = mb;
@@ -694,7 +699,7 @@ __global__ __launch_bounds__(64 * NW) void tree_join_kernel(const tree_args a) {
     for (int k = 0; k < BATCH; ++k) {
       const float w = fast_exp2(ml[k].x - safe);   // 0 for a part that saw nothing
       L = fmaf(ml[k].y, w, L);
-      o += av[k] * w;
+      tree_add(o, av[k], w);
     }
     M = mb;
   }
@@ -716,7 +721,7 @@ __global__ __launch_bounds__(64 * NW) void tree_join_kernel(const tree_args a) {
       const float* const s = state + w * 64 * 6 + lane;
       const float f = fast_exp2(s[0] - safe);
       L = fmaf(s[64], f, L);
-      o += float4_t{s[128], s[192], s[256], s[320]} * f;
+      tree_add(o, float4_t{s[128], s[192], s[256], s[320]}, f);
     }
   }
   if (lane + 64 * (int)blockIdx.y >= a.num_heads * QPH) return;
