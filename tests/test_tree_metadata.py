@@ -287,3 +287,15 @@ def test_partials_stay_within_their_bound(hq, hkv, d, dt, sizes, cached):
                                 counts.ctypes.data) == _lib.TB_OK
     assert L.tb_tree_attention_workspace_bytes(int(counts[2]), hq, d) <= 128 << 20
     assert counts[0] >= 256 or counts[2] > 0               # nor is the chip left empty for it
+
+
+def test_rows_of_one_head_or_none():
+    """A dimension of one entry, and a tensor without any, may hold any stride: torch's own results do."""
+    from tinybatch_amd.ops import _rows_view
+    empty = torch.empty(0, 1, 128) * 0.5
+    assert empty.stride(1) == 0 and _rows_view("q", empty, 1, 128) == 128
+    one = torch.zeros(5 * 200).as_strided((5, 1, 128), (200, 0, 1))
+    assert _rows_view("q", one, 1, 128) == 200
+    for bad in (torch.zeros(5, 128, 2)[..., 0].view(5, 1, 128), torch.zeros(5, 3, 128)[:, ::2]):
+        with pytest.raises(ValueError, match="contiguous"):
+            _rows_view("q", bad, bad.shape[1], 128)

@@ -63,12 +63,13 @@ def _rows_view(name: str, t: torch.Tensor, n_heads: int, d: int) -> int:
     if t.dim() == 3:
         if t.shape[1] != n_heads or t.shape[2] != d:
             raise ValueError(f"{name} must be [T, {n_heads}, {d}], got {tuple(t.shape)}")
-        if t.stride(2) != 1 or t.stride(1) != d:
+        # (a dimension of one entry and a tensor of none may hold any stride)
+        if t.numel() and (t.stride(2) != 1 or (t.stride(1) != d and n_heads > 1)):
             raise ValueError(f"{name} must have contiguous [heads, head_dim] rows")
     elif t.dim() == 2:
         if t.shape[1] != n_heads * d:
             raise ValueError(f"{name} must be [T, {n_heads * d}], got {tuple(t.shape)}")
-        if t.stride(1) != 1:
+        if t.numel() and t.stride(1) != 1:
             raise ValueError(f"{name} must have contiguous rows")
     else:
         raise ValueError(f"{name} must be 2-D or 3-D, got {t.dim()}-D")
