@@ -142,11 +142,11 @@ class BlockManager:
             blk.ref_count = 1
             blk.token_ids = []
             table.append(blk.block_id)
+        last = min(idx, len(table) - 1)                         # the token's block
         if pos % bs:
-            idx = min(idx, len(table) - 1)
-            self.blocks[table[idx]].token_ids = list(seq_token_ids[idx * bs:pos])
-        elif self.enable_prefix_caching and idx >= 1:
-            self._publish(table, idx - 1, seq_token_ids)
+            self.blocks[table[last]].token_ids = list(seq_token_ids[last * bs:pos])
+        elif self.enable_prefix_caching and last >= 1:
+            self._publish(table, last - 1, seq_token_ids)
         return added
 
     def _publish(self, table: list[int], idx: int, seq_token_ids: list[int]) -> None:
