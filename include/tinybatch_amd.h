@@ -797,6 +797,93 @@ int32_t tb_tree_commit(void* storage, int32_t num_layers, int64_t layer_stride_b
                        const int32_t* num_accepted, int32_t num_kv_heads, int32_t head_dim,
                        int32_t block_size, int32_t dtype, hipStream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Steps whose lengths and block tables live on the GPU, and beam search over them. No
+ * counterpart in the reference, which builds every step from host lists
+ * (src/tinybatch/engine.py:99-126, block_manager.py:117-156) and decodes one sequence per request.
+ *
+ * The state of num_rows rows (device memory), rows g * beams .. + beams - 1 the beams of request g:
+ *   block_tables [num_rows][max_blocks_per_row]: the first ceil(len / block_size) entries of a row
+ *     with len positions are its blocks;
+ *   lens [num_rows]; ref_counts [num_blocks]: how many rows (and holders outside) have a block;
+ *   free_blocks [num_blocks], num_free [1]: the free blocks, the next one to be taken last;
+ *   shared_blocks [num_rows / beams]: leading whole blocks that all of a request's rows with
+ *     positions have in common (tb_beam_reorder sets it);
+ *   status [1]: TB_TABLES_* bits are added where a call could not do its work; the caller clears them.
+ */
+#define TB_BEAMS_MAX 64
+#define TB_BEAM_CANDIDATES_MAX 128
+#define TB_TABLES_OUT_OF_BLOCKS 1u     /* more blocks needed than are free */
+#define TB_TABLES_ROW_FULL 2u          /* a row needs more than max_blocks_per_row */
+#define TB_TABLES_BAD_PARENT 4u        /* a parent outside [-1, beams) */
+#define TB_TABLES_TOO_MANY_TOKENS 8u   /* more new tokens than max_tokens (pad_tokens of a row) */
+#define TB_TABLES_BAD_LENGTH 16u       /* a length below 0, or beyond its row's blocks */
+#define TB_TABLES_TOO_MUCH_WORK 32u    /* more work items, partitions or split rows than there is room for */
+
+/* A step's arrays from the rows' lengths: row b gets new_lens[b] >= 0 tokens behind its cached_lens[b]
+ * positions, its blocks grow by what they need (the next free blocks, rows in order; ref_counts 1). Writes
+ *   context_lens [num_rows]: cached + new; num_free_out [1]: the free blocks after the step;
+ *   query_start_loc [num_rows + 1]: row b's tokens are the flat rows from query_start_loc[b] on, one row behind the
+ *     other (pad_tokens 0), or from b * pad_tokens on (then max_tokens = num_rows * pad_tokens);
+ *   positions (int64), slot_mapping (tb_kv_append's), row_ctx [max_tokens]: position, pool slot and positions seen
+ *     (position + 1) of every flat row; 0, -1 and 0 for flat rows without a token;
+ *   with partition_tokens > 0 (0: none of these): row_part_offsets [max_tokens + 1], work_items [max_items][4],
+ *     split_rows [max_split_rows][4] as tb_paged_attention takes them (no prefill tiles; up to rows_per_item <= 16
+ *     rows an item; items in row order), counts [4]: items, split rows, 0, partitions: its device_counts. Entries
+ *     behind the counts are left as they are.
+ * The cached lengths and num_free are read only, so that a step can be built again; it is taken by using
+ * context_lens and num_free_out in their place. They must not be the same memory. Where anything does not
+ * fit (status tells) the step is empty: no token, no block taken, context_lens = cached_lens.
+ * The block that a row's first new token falls into must be the row's own.
+ *   workspace: tb_device_step_workspace_bytes(num_rows) bytes (0 up to 1024 rows), 4-byte aligned. */
+size_t tb_device_step_workspace_bytes(int32_t num_rows);
+int32_t tb_device_step(int32_t* block_tables, int32_t max_blocks_per_row, const int32_t* cached_lens,
+                       const int32_t* new_lens, int32_t num_rows, int32_t* ref_counts,
+                       const int32_t* free_blocks, const int32_t* num_free, int32_t num_blocks,
+                       int32_t block_size, int32_t pad_tokens, int32_t max_tokens,
+                       int32_t* context_lens, int32_t* num_free_out, int32_t* query_start_loc,
+                       int64_t* positions, int32_t* slot_mapping, int32_t* row_ctx,
+                       int32_t partition_tokens, int32_t rows_per_item, int32_t* row_part_offsets,
+                       int32_t* work_items, int32_t max_items, int32_t max_partitions,
+                       int32_t* split_rows, int32_t max_split_rows, int32_t* counts, uint32_t* status,
+                       void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* The best continuations of every request: with s = scores[row] and x = logits[row] of beam k,
+ *   c(k, v) = s + x[v] - log(sum_u exp(x[u])),
+ * the num_candidates largest over k and v, largest first, the smaller k * vocab + v first among
+ * equals: out_scores, out_parents (k), out_tokens (v) [num_rows / beams][num_candidates]; -inf, -1, -1
+ * where no candidate above -inf is left. finished (may be NULL) [num_rows]: a beam that has ended has the one
+ * candidate (k, end_token) with c = s, and its logits are not read; nor are those of a beam whose score is -inf
+ * or NaN, which has none. A logit that is NaN counts as -inf, +inf as the largest fp32 number. Decided in 64 bits from
+ * sums of fp32 exponentials. logits fp32 / fp16 / bf16, row stride in elements, aligned to their
+ * elements; vocab <= 2^30, num_rows <= 65535; workspace: tb_beam_select_workspace_bytes, 16-byte aligned. */
+size_t tb_beam_select_workspace_bytes(int32_t num_rows, int32_t vocab);
+int32_t tb_beam_select(const void* logits, int64_t row_stride, int32_t vocab, int32_t dtype,
+                       const float* scores, const uint8_t* finished, int32_t end_token, int32_t num_rows,
+                       int32_t beams, int32_t num_candidates, float* out_scores, int32_t* out_parents,
+                       int64_t* out_tokens, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* The rows' states after a selection: row (g, k) continues row (g, parents[g * beams + k]); parent -1,
+ * or one without positions, empties it. Whole blocks are shared. A block that is not full is kept by its row's
+ * first child if the row alone holds it (ref_counts 1), and copied for every other child: its positions of K
+ * and V in every layer of storage ([num_layers][num_blocks][2][num_kv_heads][block_size][head_dim], layers
+ * layer_stride_bytes apart; num_layers 0: the tables alone) into fresh blocks, the next free ones, rows in
+ * order. Blocks that nobody holds any more go behind the free blocks, in the order (request, table column, row) of the
+ * old tables; fresh blocks are taken before. lens_in / num_free_in are the lengths and free blocks before the call
+ * (tb_device_step's context_lens and num_free_out take that step), lens_out / num_free_out may be the
+ * same memory. Entries behind a row's blocks, up to the longest old row of its request, are -1. Where a parent is
+ * out of range or the free blocks do not suffice (status tells) nothing is changed.
+ *   beams <= TB_BEAMS_MAX; head_dim * element size a multiple of 16 bytes;
+ *   workspace: tb_beam_reorder_workspace_bytes, 16-byte aligned. */
+size_t tb_beam_reorder_workspace_bytes(int32_t num_rows, int32_t beams, int32_t max_blocks_per_row);
+int32_t tb_beam_reorder(void* storage, int32_t num_layers, int64_t layer_stride_bytes, int32_t num_blocks,
+                        int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t dtype,
+                        int32_t* block_tables, int32_t max_blocks_per_row, int32_t num_rows, int32_t beams,
+                        const int32_t* lens_in, int32_t* lens_out, int32_t* ref_counts,
+                        int32_t* free_blocks, const int32_t* num_free_in, int32_t* num_free_out,
+                        int32_t* shared_blocks, const int32_t* parents, uint32_t* status, void* workspace,
+                        size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

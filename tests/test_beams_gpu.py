@@ -1,0 +1,428 @@
+"""Beam search's operators (tinybatch_amd/device_tables.py, beams.py) on the GPU against their plain forms
+(oracle/beams.py). Steps and reorderings are whole numbers and moved rows: equal, bit for bit.
+
+Selection's scores: the result is rounded to fp32 (2^-24 |c|); a term of the sum e^(x - r) has its argument rounded
+(|x - r| <= 104 where the term is not 0: 104 2^-24 relative to it) and its value by 2 of an exponential's steps, so that the sum
+and with it its logarithm is off by 106 2^-24 at most; everything else is in 64 bits.
+
+Attention's tolerance counts roundings, with h half a step of the element type: the output is off by h |out|; the weights that
+multiply V are rounded to the type (h each) and so is their sum (h): 2 h sum p|v|; a score, an fp32 sum of d products,
+by (d + 4) 2^-24 sum|q k| (its weight by that relatively, and the sum of weights again), and the sums over
+the context by 2^-24 a term."""
+import numpy as np
+import pytest
+import torch
+
+from oracle import beams as oracle
+from test_device_tables import random_state
+from tinybatch_amd import (DeviceTables, PagedKVCache, build_device_step, ops, reorder_beams, select_beams)
+from tinybatch_amd.block_manager import OutOfBlocks
+from tinybatch_amd.metadata import build_step_metadata
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+HALF = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+
+
+def check_attention(got, q, pool, tables, lens, heads, scale=None):
+    d = pool.shape[-1]
+    out, weight, spread = oracle.attention(q.cpu().double().numpy(), pool.cpu().double().numpy(), tables, lens, heads, scale)
+    h = HALF[pool.dtype]
+    exact = 2 * ((d + 4) * 2.0 ** -24 * spread[:, :, None] + (max(lens, default=0) + 64) * 2.0 ** -24)
+    tol = h * np.abs(out) + (2 * h + exact) * weight + 1e-30
+    off = np.abs(got.cpu().double().numpy().reshape(out.shape) - out)
+    assert np.isfinite(off).all() and (off <= tol).all(), (off / tol).max()
+
+
+def upload(s: oracle.State, max_blocks=None, held=()):
+    width = max([len(t) for t in s.tables] + [1]) if max_blocks is None else max_blocks
+    return DeviceTables.from_lists(s.tables, s.lens, s.free, max_blocks=width, block_size=s.bs, num_blocks=s.nb,
+                                   group_size=s.beams, device=DEV, held=held)
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def check_state(t: DeviceTables, s: oracle.State, lens=None, num_free=None):
+    assert (t.context_lens if lens is None else lens).tolist() == s.lens
+    n = int((t.num_free if num_free is None else num_free).item())
+    assert t.free_blocks[:n].tolist() == s.free
+    assert t.ref_counts.tolist() == s.refs
+    got = t.block_tables.tolist()
+    for row, want in zip(got, s.tables):
+        assert row[:len(want)] == want
+
+
+# ---- steps ------------------------------------------------------------------------
+@pytest.mark.parametrize("rows", [1, 2, 63, 256, 257, 1024, 1025, 2600])
+@pytest.mark.parametrize("bs,P,group", [(16, 64, 1), (1, 64, 3), (32, 256, 2)])
+def test_step_of_many_rows(rows, bs, P, group):
+    s = random_state(rows + bs, rows, 1, bs, 300 if rows < 300 else 40, spare=12 * rows + 60)
+    g = np.random.default_rng(rows)
+    new = [int(x) for x in g.choice([0, 1, 1, 1, 2, 7], rows)]
+    new[rows // 2] += 50
+    after, starts, positions, slots, ctx = oracle.step(s, new)
+    t = upload(s, max_blocks=max(len(x) for x in after.tables) + 1)
+    step = t.new_step(max_tokens=sum(new) + 5, partition_tokens=P, rows_per_item=group)
+    for _ in range(2):                             # a step may be built again
+        build_device_step(t, i32(new), step)
+        check_state(t, after, step.context_lens, step.num_free)
+        assert t.context_lens.tolist() == s.lens
+        n = sum(new)
+        assert step.query_start_loc.tolist() == starts
+        assert step.positions.tolist() == positions + [0] * 5
+        assert step.slot_mapping.tolist() == slots + [-1] * 5
+        assert step.row_ctx.tolist() == ctx + [0] * 5
+    live = [b for b in range(rows) if new[b]]
+    meta = build_step_metadata(positions, [(starts[b], starts[b + 1]) for b in live], [after.tables[b] for b in live],
+                               [after.lens[b] for b in live], block_size=bs, num_blocks=s.nb, partition_tokens=P,
+                               rows_per_item=group)
+    items, split, _, parts = step.counts.tolist()
+    assert (items, split, parts) == (meta.num_work_items, meta.num_split_rows, meta.total_partitions)
+    want = meta.work_np.copy()
+    want[:, 1] = np.asarray(live)[want[:, 1]]      # the host's step leaves rows without tokens out
+    assert sorted(step.work_items[:items].tolist()) == sorted(want.tolist())
+    assert step.row_part_offsets.tolist() == meta.row_part_off_np.tolist() + [parts] * 5
+    assert step.split_rows[:split].tolist() == meta.split_rows_np[:split].tolist()
+    assert not step.work_items[items:].any() and not step.split_rows[split:].any()
+    t.take(step)
+    check_state(t, after)
+    t.check()
+
+
+@pytest.mark.parametrize("padded", [1, 3])
+@pytest.mark.parametrize("rows", [5, 1200])
+def test_step_of_padded_rows(rows, padded):
+    s = random_state(rows, rows, 1, 8, 60, spare=rows + 40)
+    g = np.random.default_rng(rows)
+    new = [int(x) for x in g.integers(0, padded + 1, rows)]
+    after, starts, positions, slots, ctx = oracle.step(s, new, padded)
+    t = upload(s, max_blocks=max(len(x) for x in after.tables) + 3)
+    step = t.new_step(padded=padded, partition_tokens=16)
+    build_device_step(t, i32(new), step)
+    check_state(t, after, step.context_lens, step.num_free)
+    assert step.query_start_loc.tolist() == starts and step.positions.tolist() == positions
+    assert step.slot_mapping.tolist() == slots and step.row_ctx.tolist() == ctx
+    parts = [-(-c // 16) for c in ctx]
+    assert step.row_part_offsets.tolist() == [0] + np.cumsum(parts).tolist()
+    assert step.work_items[:sum(parts)].tolist() == [[r, r // padded, p, c] for r, c in enumerate(ctx)
+                                                     for p in range(-(-c // 16))]
+
+
+@pytest.mark.parametrize("rows", [4, 1500])
+@pytest.mark.parametrize("why", ["blocks", "row", "tokens", "length", "cached", "work", "padded"])
+def test_steps_that_do_not_fit_are_empty(rows, why):
+    s = random_state(3, rows, 1, 16, 50, spare=6 if why == "blocks" else 4 * rows + 30)
+    new = [1] * rows
+    if why == "blocks":
+        new[0] = 16 * 7
+    if why == "length":
+        new[-1] = -1
+    after_blocks = max(len(t) for t in s.tables)
+    t = upload(s, max_blocks=after_blocks if why == "row" else after_blocks + 20)
+    if why == "row":
+        new[1] = 16 * after_blocks + 1
+    if why == "cached":
+        t.context_lens[1] = -3
+        s.lens[1] = -3
+    step = (t.new_step(padded=1) if why == "padded" else
+            t.new_step(max_tokens=rows - 1 if why == "tokens" else sum(max(n, 0) for n in new), partition_tokens=16,
+                       max_items=2 if why == "work" else None))
+    if why == "padded":
+        new[2] = 2
+    build_device_step(t, i32(new), step)
+    assert step.context_lens.tolist() == s.lens and step.num_free.tolist() == [len(s.free)]
+    if why != "cached":
+        check_state(t, s)
+    assert not step.row_ctx.any() and not step.positions.any() and (step.slot_mapping == -1).all()
+    assert step.query_start_loc.tolist() == (list(range(rows + 1)) if why == "padded" else [0] * (rows + 1))
+    if why != "padded":
+        assert not step.counts.any() and not step.row_part_offsets.any()
+    with pytest.raises({"blocks": OutOfBlocks, "row": IndexError}.get(why, ValueError)):
+        t.check()
+    t.check()                                      # told once
+
+
+def test_step_without_rows_or_tokens():
+    t = DeviceTables(0, max_blocks=1, block_size=16, num_blocks=4, device=DEV)
+    step = t.new_step(max_tokens=3, partition_tokens=64)
+    build_device_step(t, i32([]), step)
+    assert step.slot_mapping.tolist() == [-1] * 3 and step.counts.tolist() == [0] * 4
+    s = random_state(1, 3, 1, 16, 40)
+    t = upload(s)
+    step = t.new_step(max_tokens=0)
+    build_device_step(t, i32([0, 0, 0]), step)
+    check_state(t, s, step.context_lens, step.num_free)
+    t.check()
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,d", [(torch.float32, 6, 2, 64), (torch.bfloat16, 14, 2, 64), (torch.float16, 8, 2, 128)])
+def test_step_serves_paged_attention(dtype, hq, hkv, d):
+    """Append and attention over a step built on the GPU against those of the host's step."""
+    s = random_state(7, 9, 1, 16, 700, spare=80)
+    new = [1, 0, 5, 1, 20, 1, 1, 3, 1]
+    after, starts, positions, slots, ctx = oracle.step(s, new)
+    g = torch.Generator().manual_seed(1)
+    pool = torch.randn(s.nb, 2, hkv, 16, d, generator=g).to(dtype).to(DEV)
+    T = len(slots)
+    q, k, v = (torch.randn(T, h, d, generator=g).to(dtype).to(DEV) for h in (hq, hkv, hkv))
+    t = upload(s, max_blocks=60)
+    step = t.new_step(max_tokens=T + 2, partition_tokens=ops.partition_tokens(dtype, d),
+                      rows_per_item=ops.rows_per_item(dtype, hq, hkv))
+    build_device_step(t, i32(new), step)
+    other = pool.clone()
+    pad = lambda x: torch.cat([x, x[:2]])
+    ops.kv_append(pool, pad(k), pad(v), step.slot_mapping)
+    got = ops.paged_attention(pad(q), pool, step.metadata(t), num_heads=hq)
+    live = [b for b in range(9) if new[b]]
+    meta = build_step_metadata(positions, [(starts[b], starts[b + 1]) for b in live], [after.tables[b] for b in live],
+                               [after.lens[b] for b in live], block_size=16, num_blocks=s.nb,
+                               partition_tokens=ops.partition_tokens(dtype, d),
+                               rows_per_item=ops.rows_per_item(dtype, hq, hkv)).to(DEV)
+    ops.kv_append(other, k, v, meta.slot_mapping)
+    want = ops.paged_attention(q, other, meta, num_heads=hq)
+    assert torch.equal(pool, other)
+    # (fp32 launches take the kernel that suits their number of work items, here the capacity)
+    assert dtype == torch.float32 or torch.equal(got[:T], want)
+    rows = [b for b in range(9) for _ in range(new[b])]
+    check_attention(got[:T], q, pool, [after.tables[b] for b in rows], ctx, hq)
+
+
+# ---- selection ----------------------------------------------------------------------
+def check_select(logits, scores, picks, finished=None, end=-1):
+    got = select_beams(logits.to(DEV), scores.to(DEV), num_candidates=picks,
+                       finished=None if finished is None else finished.to(DEV), end_token=end)
+    c, parents, tokens = oracle.select(logits.double().numpy(), scores.numpy(), picks,
+                                       None if finished is None else finished.numpy(), end)
+    assert got.parents.tolist() == parents.tolist() and got.tokens.tolist() == tokens.tolist()
+    value = got.scores.cpu().double().numpy()
+    assert (np.isinf(value) == np.isinf(c)).all() or np.abs(c[np.isinf(value) != np.isinf(c)]).min() > 3.4e38
+    both = np.isfinite(value) & np.isfinite(c)
+    assert (np.abs(value[both] - c[both]) <= 2.0 ** -24 * np.abs(c[both]) + 106 * 2.0 ** -24).all()
+    return got
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("G,K,V,M", [(1, 1, 1, 1), (1, 1, 1, 5), (2, 3, 7, 6), (1, 4, 511, 8), (3, 2, 512, 4), (2, 5, 513, 10),
+                                     (1, 1, 50257, 128), (5, 4, 32001, 8), (1, 8, 151936, 16), (2, 64, 1000, 128),
+                                     (70, 6, 257, 12)])
+def test_select(G, K, V, M, dtype):
+    g = torch.Generator().manual_seed(G * 1000 + V)
+    logits = (torch.randn(G * K, V, generator=g) * 4).to(dtype)
+    check_select(logits, torch.randn(G, K, generator=g) * 2 - 10, M)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_select_ended_and_lost_beams(dtype):
+    g = torch.Generator().manual_seed(5)
+    logits = (torch.randn(6 * 5, 3001, generator=g) * 4).to(dtype)
+    scores = torch.randn(6, 5, generator=g) * 3
+    finished = torch.rand(6, 5, generator=g) < 0.4
+    finished[0], finished[1] = True, False
+    scores[2, 1:], scores[3], scores[4, 0] = -float("inf"), -float("inf"), float("nan")
+    finished[2, 2], finished[3, 1], finished[4, 0] = True, True, True
+    got = check_select(logits, scores, 9, finished, 17)
+    assert (got.parents[3] == -1).all() and (got.scores[3] == -float("inf")).all()
+    assert got.tokens[0, :5].tolist() == [17] * 5 and got.parents[0, 5:].tolist() == [-1] * 4
+    check_select(logits, torch.full((6, 5), -float("inf")), 5)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [300, 5000, 151936])
+def test_select_ties(V, dtype):
+    """Equal logits and equal beams: the smaller beam, then the smaller token; -0 is 0."""
+    logits = torch.zeros(4, V, dtype=dtype)
+    scores = torch.zeros(1, 4)
+    got = check_select(logits, scores, 20)
+    assert got.parents.tolist() == [[0] * 20] and got.tokens.tolist() == [list(range(20))]
+    logits[:, ::2] = -0.0
+    check_select(logits, scores, 20)
+    g = torch.Generator().manual_seed(V)
+    logits[:] = torch.randint(0, 3, (1, V), generator=g).to(dtype)    # beams alike: candidates tie across them
+    check_select(logits, scores, 30)
+    logits[:, :] = torch.arange(V).to(dtype) / 256                    # rising: many of a 16-bit type's steps tie
+    check_select(logits, scores, 50)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("offset", [1, 3])
+def test_select_rows_of_any_alignment(offset, dtype):
+    """Rows inside a wider tensor, from any element on; rows alike give values alike, to the bit."""
+    g = torch.Generator().manual_seed(offset)
+    wide = torch.full((6, 2000), 1000.0, dtype=dtype, device=DEV)
+    logits = (torch.randn(1, 1403, generator=g) * 3).to(dtype).expand(6, 1403)
+    wide[:, offset:offset + 1403] = logits.to(DEV)
+    scores = torch.zeros(1, 6)
+    got = select_beams(wide[:, offset:offset + 1403], scores.to(DEV), num_candidates=24)
+    _, parents, tokens = oracle.select(logits.double().numpy(), scores.numpy(), 24)
+    assert got.parents.tolist() == parents.tolist() and got.tokens.tolist() == tokens.tolist()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_select_masked_and_special_logits(dtype):
+    inf, nan = float("inf"), float("nan")
+    g = torch.Generator().manual_seed(2)
+    V = 2100
+    x = (torch.randn(9, V, generator=g) * 3).to(dtype)
+    x[0] = -inf                                                       # nothing left
+    x[1, :V - 1] = -inf                                               # one token left
+    x[2] = torch.finfo(dtype).min                                     # masked by the lowest value
+    x[3, 5:] = torch.finfo(dtype).min
+    x[4, 7] = nan
+    x[5] = nan
+    x[6, 9], x[6, 700] = inf, inf
+    x[7, 0] = torch.finfo(dtype).max
+    x[8] = torch.arange(V, dtype=torch.float32).flip(0).mul(-0.01).to(dtype)
+    for rows in ([0], [1], [2], [3], [4], [5], [6], [7], [8], list(range(9))):
+        check_select(x[rows].clone(), torch.zeros(1, len(rows)), 12)
+
+
+def test_select_long_rows_of_small_terms():
+    """A flat row of many tokens: the sum's terms are as good as equal, nothing of it is lost."""
+    x = torch.full((2, 1_000_003), -5.0)
+    x[0, 999_999] = 3.0
+    check_select(x, torch.zeros(1, 2), 3)
+
+
+# ---- reordering ---------------------------------------------------------------------
+def random_parents(g, groups, K):
+    return [int(min(K - 1, K * g.random() ** 1.5)) if g.random() < 0.95 else -1 for _ in range(groups * K)]
+
+
+def check_reorder(s, parents, storage, t, step=None):
+    after, copies = oracle.reorder(s, parents)
+    want = storage.clone()
+    for src, dst, n in copies:
+        want[:, dst, :, :, :n] = storage[:, src, :, :, :n]
+    reorder_beams(storage, t, i32(parents).view(-1, s.beams), step)
+    check_state(t, after)
+    assert t.shared_blocks.tolist() == after.shared()
+    assert torch.equal(storage.view(torch.uint8), want.view(torch.uint8))
+    for r, row in enumerate(t.block_tables.tolist()):
+        g0 = r // s.beams * s.beams
+        width = max(len(x) for x in s.tables[g0:g0 + s.beams])
+        assert row[len(after.tables[r]):width] == [-1] * (width - len(after.tables[r]))
+    return after
+
+
+@pytest.mark.parametrize("dtype,hkv,d", [(torch.bfloat16, 2, 64), (torch.float32, 1, 128), (torch.float16, 3, 8)])
+@pytest.mark.parametrize("groups,K,bs,longest", [(1, 1, 16, 40), (3, 4, 16, 200), (2, 8, 1, 30), (40, 5, 4, 60), (2, 64, 8, 100),
+                                                 (5, 3, 2, 900)])
+def test_reorder(groups, K, bs, longest, dtype, hkv, d):
+    """Steps and selections in turn: every state, count and row as the plain form's."""
+    s = random_state(groups + K, groups, K, bs, longest, spare=8 * groups * K + 8, held=2)
+    g = np.random.default_rng(K)
+    held = s.tables[0][:2]
+    t = upload(s, max_blocks=max(len(x) for x in s.tables) + 6, held=held)
+    storage = torch.randn(3, s.nb, 2, hkv, bs, d, device=DEV).to(dtype)
+    step = t.new_step(padded=1)
+    for turn in range(4):
+        s = check_reorder(s, random_parents(g, groups, K), storage, t)
+        new = [int(n > 0 and g.random() < 0.9) for n in s.lens]
+        after, *_ = oracle.step(s, new)
+        build_device_step(t, i32(new), step)
+        s = after
+        s = check_reorder(s, random_parents(g, groups, K), storage, t, step)
+    t.check()
+
+
+def test_reorder_from_one_prompt():
+    """The first selection: one row has the prompt, the others nothing."""
+    s = oracle.State([[4, 2, 7]] + [[]] * 4, [37, 0, 0, 0, 0], [0, 1, 3, 5, 6, 8], 9, 16, 5)
+    t = upload(s, max_blocks=4)
+    storage = torch.randn(2, 9, 2, 2, 16, 64, device=DEV)
+    after = check_reorder(s, [0, 0, 0, 0, 0], storage, t)
+    assert after.shared() == [2] and len(after.free) == 2
+    after = check_reorder(after, [-1] * 5, storage, t)               # the request has ended: all its blocks are free
+    assert len(after.free) == 9 and after.lens == [0] * 5
+
+
+def test_reorder_open_block_that_someone_else_holds():
+    """Two requests on one prompt's blocks, its last one not full: every child copies it."""
+    s = oracle.State([[3, 1], [], [3, 1], []], [20, 0, 20, 0], [0, 2, 4, 5, 6], 8, 16, 2)
+    t = upload(s)
+    storage = torch.randn(1, 8, 2, 1, 16, 64, device=DEV)
+    after = check_reorder(s, [0, 0, 0, -1], storage, t)
+    assert after.free[-1] == 1 and after.refs[3] == 3
+
+
+def test_reorder_blocks_that_several_requests_let_go_of():
+    tables = [[5, 6, 7], [5, 6, 8], [5, 6, 9], [5, 10, 11]]
+    s = oracle.State(tables, [48, 48, 48, 48], [0, 1], 12, 16, 2)
+    t = upload(s)
+    storage = torch.randn(1, 12, 2, 1, 16, 64, device=DEV)
+    after = check_reorder(s, [-1, -1, -1, -1], storage, t)
+    assert after.free == [0, 1, 5, 6, 7, 8, 10, 9, 11]               # (request, column, row)
+
+
+@pytest.mark.parametrize("why", ["blocks", "parent", "low"])
+def test_reorderings_that_do_not_fit_change_nothing(why):
+    s = random_state(4, 2, 4, 16, 60, spare=1)
+    s.lens = [n + (n % 16 == 0) if n else n for n in s.lens]
+    s = oracle.State([t + [s.free[0]] * (len(t) < -(-n // 16)) for t, n in zip(s.tables, s.lens)], s.lens, [], s.nb, 16, 4)
+    t = upload(s)
+    storage = torch.randn(2, s.nb, 2, 2, 16, 64, device=DEV)
+    keep = [x.clone() for x in (storage, t.block_tables, t.context_lens, t.ref_counts, t.free_blocks, t.num_free)]
+    bad = {"blocks": [0, 0, 0, 0], "parent": [0, 1, 2, 4], "low": [-2, 1, 2, 3]}[why]
+    reorder_beams(storage, t, i32([bad, bad]))
+    for x, y in zip((storage, t.block_tables, t.context_lens, t.ref_counts, t.free_blocks, t.num_free), keep):
+        assert torch.equal(x, y)
+    with pytest.raises(OutOfBlocks if why == "blocks" else IndexError):
+        t.check()
+
+
+def test_reorder_the_tables_alone():
+    s = random_state(9, 3, 4, 16, 100, spare=12)
+    t = upload(s)
+    g = np.random.default_rng(1)
+    parents = random_parents(g, 3, 4)
+    after, _ = oracle.reorder(s, parents)
+    reorder_beams(None, t, i32(parents).view(3, 4))
+    check_state(t, after)
+
+
+# ---- refusals -------------------------------------------------------------------------
+def test_refusals():
+    logits, scores = torch.zeros(4, 10, device=DEV), torch.zeros(2, 2, device=DEV)
+    for bad in (lambda: select_beams(logits.cpu(), scores), ):
+        with pytest.raises(RuntimeError, match="GPU"):
+            bad()
+    for bad in (lambda: select_beams(logits.long(), scores), lambda: select_beams(logits, scores.double()),
+                lambda: select_beams(logits, scores.cpu()),
+                lambda: select_beams(logits, scores, finished=torch.zeros(2, 2, device=DEV), end_token=0)):
+        with pytest.raises(TypeError):
+            bad()
+    for bad in (lambda: select_beams(logits[:3], scores), lambda: select_beams(logits.t(), scores),
+                lambda: select_beams(logits[:1].expand(4, 10), scores), lambda: select_beams(logits, scores[0]),
+                lambda: select_beams(logits, scores, num_candidates=0), lambda: select_beams(logits, scores, num_candidates=129),
+                lambda: select_beams(logits, torch.zeros(4, 65, device=DEV)),
+                lambda: select_beams(logits, scores, finished=torch.zeros(2, 2, dtype=torch.bool, device=DEV), end_token=10),
+                lambda: select_beams(logits, scores, finished=torch.zeros(2, 2, dtype=torch.bool, device=DEV))):
+        with pytest.raises(ValueError):
+            bad()
+    s = random_state(1, 2, 2, 16, 40)
+    t = upload(s)
+    storage = torch.zeros(2, s.nb, 2, 1, 16, 64, device=DEV)
+    parents = i32([[0, 1], [0, 1]])
+    for bad in (lambda: reorder_beams(storage, t, parents.long()), lambda: reorder_beams(storage, t, parents[:1]),
+                lambda: reorder_beams(storage, t, parents.cpu()), lambda: reorder_beams(storage.long(), t, parents)):
+        with pytest.raises(TypeError):
+            bad()
+    other = upload(random_state(1, 3, 2, 16, 40))
+    for bad in (lambda: reorder_beams(storage[0], t, parents), lambda: reorder_beams(storage[:, 1:], t, parents),
+                lambda: reorder_beams(storage[:, 1:].contiguous(), t, parents),
+                lambda: reorder_beams(torch.zeros(1, s.nb, 2, 1, 16, 6, device=DEV), t, parents),
+                lambda: reorder_beams(storage, t, parents, other.new_step(padded=1))):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(TypeError):
+        build_device_step(t, torch.zeros(4, dtype=torch.int64, device=DEV), t.new_step(padded=1))
+    for bad in (lambda: build_device_step(t, i32([1] * 4), other.new_step(padded=1)), lambda: t.new_step(),
+                lambda: t.new_step(max_tokens=-1), lambda: t.new_step(max_tokens=5, padded=1), lambda: t.new_step(padded=-1),
+                lambda: t.new_step(max_tokens=4, partition_tokens=64, rows_per_item=17),
+                lambda: t.new_step(max_tokens=4, partition_tokens=64, max_items=1 << 24),
+                lambda: t.new_step(max_tokens=4).metadata(t)):
+        with pytest.raises(ValueError):
+            bad()

@@ -155,6 +155,25 @@ SIGNATURES = {
     "tb_tree_verify_greedy": (c_i32, [c_vp, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_vp, c_i32, c_vp]),
     "tb_tree_commit": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_vp, c_i32, c_vp, c_i32, c_vp, c_i32, c_vp, c_i32, c_i32,
                                c_i32, c_i32, c_vp]),
+    "tb_device_step_workspace_bytes": (c_sz, [c_i32]),
+    "tb_device_step": (c_i32, [
+        c_vp, c_i32, c_vp, c_vp, c_i32,          # block tables, max_nb, cached lens, new lens, rows
+        c_vp, c_vp, c_vp, c_i32, c_i32,          # ref counts, free blocks, num_free, blocks, block size
+        c_i32, c_i32,                            # pad tokens, max tokens
+        c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,      # context lens, num_free out, starts, positions, slots, row_ctx
+        c_i32, c_i32, c_vp, c_vp, c_i32, c_i32,  # partition, rows per item, offsets, items, max items, max partitions
+        c_vp, c_i32, c_vp, c_vp,                 # split rows, max split rows, counts, status
+        c_vp, c_sz, c_vp]),                      # workspace, bytes, stream
+    "tb_beam_select_workspace_bytes": (c_sz, [c_i32, c_i32]),
+    "tb_beam_select": (c_i32, [c_vp, c_i64, c_i32, c_i32,            # logits, stride, vocab, dtype
+                               c_vp, c_vp, c_i32, c_i32, c_i32, c_i32,   # scores, finished, end, rows, beams, candidates
+                               c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),     # outputs, workspace, bytes, stream
+    "tb_beam_reorder_workspace_bytes": (c_sz, [c_i32, c_i32, c_i32]),
+    "tb_beam_reorder": (c_i32, [
+        c_vp, c_i32, c_i64, c_i32, c_i32, c_i32, c_i32, c_i32,   # storage, layers, stride, blocks, kv heads, dim, block, dtype
+        c_vp, c_i32, c_i32, c_i32, c_vp, c_vp,                   # tables, max_nb, rows, beams, lens in, out
+        c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,                # refs, free, num_free in, out, shared, parents, status
+        c_vp, c_sz, c_vp]),                                      # workspace, bytes, stream
     "tb_rms_norm": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i32, c_i32, c_f32, c_i32, c_vp]),
     "tb_rope_qk": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_i32,
                            c_vp]),

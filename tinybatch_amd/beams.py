@@ -1,0 +1,134 @@
+"""Beam search over the paged cache, without the host between two steps.
+
+The reference decodes one continuation per request (src/tinybatch/engine.py:99-159). Here a request
+has ``group_size`` rows, its beams, whose paged state lives on the GPU (DeviceTables):
+
+    build_device_step(tables, new_lens, step)                    # one token per beam
+    plan.build(step.row_ctx)
+    for layer in range(n_layers):
+        ops.kv_append(cache.pools[layer], k, v, step.slot_mapping)
+        attn = beam_attention(q, cache.pools[layer], plan)
+    choice = select_beams(logits, scores, finished=finished, end_token=eos)
+    reorder_beams(cache.storage, tables, choice.parents, step=step)
+
+Everything is enqueued on the tensors' device's current stream and nothing synchronises.
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from .device_tables import MAX_BEAMS, DeviceStep, DeviceTables, _ints
+from .tree import _elsewhere, _scratch
+
+MAX_CANDIDATES = 128         # TB_BEAM_CANDIDATES_MAX
+
+
+class BeamChoice(NamedTuple):
+    """A request's best continuations, best first, on the device."""
+    scores: torch.Tensor     # [G, M] float32, -inf where no candidate is left
+    parents: torch.Tensor    # [G, M] int32: the beam that is continued, -1 where none is left
+    tokens: torch.Tensor     # [G, M] int64: with which token, -1 where none is left
+
+
+def select_beams(logits: torch.Tensor, scores: torch.Tensor, *, num_candidates: int | None = None,
+                 finished: torch.Tensor | None = None, end_token: int = -1) -> BeamChoice:
+    """The ``num_candidates`` (by default as many as beams) best continuations of every request
+    (tb_beam_select): candidate (k, v) is worth scores[g, k] + log_softmax(logits[g * K + k])[v], the
+    smaller k * vocab + v first among equals.
+
+    logits [G * K, vocab] (fp32, fp16 or bf16, contiguous rows); scores [G, K] float32, the beams' sums of
+    log-probabilities (-inf: no beam). ``finished`` [G, K] bool: a beam that has ended stands for itself
+    alone, with ``end_token`` at its score. NaN logits count as -inf.
+    """
+    _lib.require_gpu_tensor("logits", logits)
+    device = logits.device
+    if logits.dtype not in _lib.DTYPE_CODE:
+        raise TypeError(f"unsupported logits dtype {logits.dtype}")
+    if scores.dim() != 2 or not 1 <= scores.shape[1] <= MAX_BEAMS:
+        raise ValueError(f"scores must be [requests, beams] with 1 .. {MAX_BEAMS} beams, got {tuple(scores.shape)}")
+    G, K = scores.shape
+    _ints("scores", scores, torch.float32, (G, K), device)
+    if logits.dim() != 2 or logits.shape[0] != G * K or logits.shape[1] < 1 or logits.stride(1) != 1:
+        raise ValueError(f"logits must be [{G * K}, vocab] with contiguous rows, got {tuple(logits.shape)}")
+    vocab = logits.shape[1]
+    stride = logits.stride(0) if G * K > 1 else vocab
+    if stride < vocab:
+        raise ValueError("logits' rows overlap")
+    M = K if num_candidates is None else num_candidates
+    if not 1 <= M <= MAX_CANDIDATES:
+        raise ValueError(f"num_candidates must lie within 1 .. {MAX_CANDIDATES}")
+    if vocab > 1 << 30 or G * K > 65535:
+        raise ValueError(f"{G * K} rows of a vocabulary of {vocab}: at most 65535 and 2^30 are served")
+    if finished is not None:
+        _ints("finished", finished, torch.bool, (G, K), device)
+        if not 0 <= end_token < vocab:
+            raise ValueError(f"end_token {end_token} outside the vocabulary of {vocab}")
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return select_beams(logits, scores, num_candidates=M, finished=finished, end_token=end_token)
+    out = BeamChoice(torch.empty(G, M, dtype=torch.float32, device=device),
+                     torch.empty(G, M, dtype=torch.int32, device=device),
+                     torch.empty(G, M, dtype=torch.int64, device=device))
+    L, stream = _lib.lib(), _lib.stream_handle(device)
+    need = L.tb_beam_select_workspace_bytes(G * K, vocab)
+    lock, ws, ws_bytes, _, _ = _scratch(device, stream, need, 0)
+    try:
+        st = L.tb_beam_select(logits.data_ptr(), stride, vocab, _lib.DTYPE_CODE[logits.dtype], scores.data_ptr(),
+                              None if finished is None else finished.data_ptr(), end_token, G * K, K, M,
+                              out.scores.data_ptr(), out.parents.data_ptr(), out.tokens.data_ptr(), ws.data_ptr(),
+                              ws_bytes, stream)
+    finally:
+        lock.release()
+    _lib.check(st, "tb_beam_select")
+    return out
+
+
+def reorder_beams(storage: torch.Tensor | None, tables: DeviceTables, parents: torch.Tensor,
+                  step: DeviceStep | None = None) -> None:
+    """The beams' paged states follow the selection, in place (tb_beam_reorder): row (g, k) continues row
+    (g, parents[g, k]); -1 empties it. Whole blocks are shared, the block that is not full is kept by
+    its row's first child and copied for the others, in every layer; blocks that no row holds any more are
+    free again. storage: the layers' pools [layers, num_blocks, 2, kv_heads, block_size, head_dim]
+    (PagedKVCache.storage), or None for the tables alone. parents [G, K] int32. ``step``: the step that
+    has just run (its lengths become the state's); without it the state's own lengths. Where the free blocks do not
+    suffice nothing is changed (tables.check() raises)."""
+    device, K, G = tables.device, tables.group_size, tables.num_rows // tables.group_size
+    _ints("parents", parents, torch.int32, (G, K), device)
+    layers = stride = hkv = d = dtype = 0
+    if storage is not None:
+        _lib.require_gpu_tensor("storage", storage)
+        if storage.dim() != 6 or storage.shape[2] != 2 or not storage.is_contiguous():
+            raise ValueError("storage must be a contiguous [layers, num_blocks, 2, kv_heads, block_size, head_dim] tensor")
+        if storage.dtype not in _lib.DTYPE_CODE:
+            raise TypeError(f"unsupported pool dtype {storage.dtype}")
+        if storage.device != device:
+            raise ValueError(f"storage is on {storage.device}, the tables on {device}")
+        if storage.shape[1] != tables.num_blocks or storage.shape[4] != tables.block_size:
+            raise ValueError(f"tables are for {tables.num_blocks} blocks of {tables.block_size} positions")
+        layers, hkv, d, dtype = storage.shape[0], storage.shape[3], storage.shape[5], _lib.DTYPE_CODE[storage.dtype]
+        stride = storage.stride(0) * storage.element_size()
+        if d * storage.element_size() % 16:
+            raise ValueError(f"head_dim {d} is not served (rows of whole 16-byte pieces are)")
+    if step is not None and (step.context_lens.device != device or step.context_lens.shape[0] != tables.num_rows):
+        raise ValueError("the step was made for other tables (DeviceTables.new_step)")
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return reorder_beams(storage, tables, parents, step)
+    now = tables if step is None else step
+    L, stream = _lib.lib(), _lib.stream_handle(device)
+    need = L.tb_beam_reorder_workspace_bytes(tables.num_rows, K, tables.max_blocks)
+    lock, ws, ws_bytes, _, _ = _scratch(device, stream, need, 0)
+    try:
+        st = L.tb_beam_reorder(
+            None if storage is None else storage.data_ptr(), layers, stride, tables.num_blocks, hkv, d,
+            tables.block_size, dtype, tables.block_tables.data_ptr(), tables.max_blocks, tables.num_rows, K,
+            now.context_lens.data_ptr(), tables.context_lens.data_ptr(), tables.ref_counts.data_ptr(),
+            tables.free_blocks.data_ptr(), now.num_free.data_ptr(), tables.num_free.data_ptr(),
+            tables.shared_blocks.data_ptr(), parents.data_ptr(), tables.status.data_ptr(), ws.data_ptr(), ws_bytes,
+            stream)
+    finally:
+        lock.release()
+    _lib.check(st, "tb_beam_reorder")

@@ -1,0 +1,365 @@
+// The beams' paged states after a selection: tables, reference counts, free blocks and K/V.
+//
+// Row i = g K + k takes the state of row s = g K + parent(i), c = lens[s] positions:
+//   its whole blocks, c / bs of them, are shared: table'[i][j] = table[s][j];
+//   a block that is not full (c mod bs positions of it) is kept by the first child of s if s alone
+//   holds it, and copied into a fresh block for every other child: its positions of K and V, in all layers;
+//   parent -1, or a parent without positions, empties the row.
+// refs[b] counts the rows (and whoever else holds it) of block b: every row lets go of its old table
+// and takes hold of its new one. A block that nobody holds any more is free.
+//
+// Launches: 1. one workgroup: who copies, the fresh blocks (running sum over the rows), the new lengths;
+// 2. a workgroup per request and 128 columns of its tables: the new tables, what the reference counts change by,
+// the blocks that were let go of; beside them the copies; 3. one workgroup: of those blocks the ones that nobody
+// holds, each once, in the order (request, column, row) of the old tables, behind the free blocks. Every order is fixed:
+// the same state gives the same tables. Fresh blocks are taken before any is freed, so that a copy's
+// source is never its own destination. Where something does not fit nothing is changed.
+#include "tb_common.h"
+
+namespace tb {
+
+constexpr int REORDER_COLUMNS = 128;
+constexpr int32_t MARK = 1 << 30;
+
+struct reorder_args {
+  char* storage;               // [layers][NB][2][Hkv][bs][D]
+  int64_t layer_bytes;
+  int32_t layers, num_blocks, pairs;   // pairs = 2 Hkv
+  int32_t row_bytes;           // of a position of a head
+  int32_t log2_bs;
+  int32_t* tables;             // [rows][max_nb]
+  int32_t max_nb, rows, beams;
+  const int32_t* lens_in;      // [rows]
+  int32_t* lens_out;           // [rows]
+  int32_t* refs;               // [NB]
+  int32_t* free_blocks;        // [NB]
+  const int32_t* num_free_in;
+  int32_t* num_free_out;
+  int32_t* shared;             // [rows / beams]
+  const int32_t* parents;      // [rows]
+  uint32_t* status;
+  // workspace
+  int32_t* head;               // {0 or 1: nothing is done, copies}
+  int4* plan;                  // [rows]: {source row or -1, new length, fresh block or -1, old length}
+  int4* copies;                // [rows]: {source block, fresh block, positions, 0}
+  int32_t* gone_count;         // [requests * chunks]
+  int32_t* gone;               // [requests * chunks][128 beams]
+  int32_t chunks;
+};
+
+__device__ __forceinline__ int wave_scan(int x, int lane) {   // inclusive
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const int y = __shfl_up(x, o);
+    if (lane >= o) x += y;
+  }
+  return x;
+}
+// Exclusive running sum over a workgroup; `total` gets the whole. One barrier before the result, and the
+// next call's writes go to the other half of `waves` [2][THREADS / 64].
+template <int THREADS>
+__device__ __forceinline__ int group_scan(int x, int (*waves)[THREADS / 64], int turn, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int up = wave_scan(x, lane);
+  if (lane == 63) waves[turn & 1][wave] = up;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) {
+    const int y = waves[turn & 1][w];
+    if (w < wave) before += y;
+    total += y;
+  }
+  return before + up - x;
+}
+
+__global__ __launch_bounds__(1024) void reorder_plan_kernel(const reorder_args a) {
+  __shared__ int waves[2][16];
+  __shared__ uint32_t faults;
+  const int bs = 1 << a.log2_bs, K = a.beams;
+  if (threadIdx.x == 0) faults = 0;
+  __syncthreads();
+  int base = 0, turn = 0;
+  for (int i0 = 0; i0 < a.rows; i0 += 1024, ++turn) {
+    const int i = i0 + threadIdx.x;
+    bool copy = false;
+    int src = -1, ctx = 0, open = -1, old = 0;
+    if (i < a.rows) {
+      const int g0 = i / K * K, p = a.parents[i];
+      old = a.lens_in[i];
+      if (p < -1 || p >= K) {
+        atomicOr(&faults, TB_TABLES_BAD_PARENT);
+      } else if (p >= 0) {
+        ctx = a.lens_in[g0 + p];
+        if (ctx < 0 || (ctx + bs - 1) >> a.log2_bs > a.max_nb) {
+          atomicOr(&faults, TB_TABLES_BAD_LENGTH);
+          ctx = 0;
+        }
+        if (ctx > 0) src = g0 + p;
+        if (ctx & (bs - 1)) {
+          open = a.tables[(int64_t)src * a.max_nb + (ctx >> a.log2_bs)];
+          bool first = true;
+          for (int k = g0; k < i; ++k) first &= a.parents[k] != p;
+          if (open < 0 || open >= a.num_blocks) atomicOr(&faults, TB_TABLES_BAD_LENGTH);
+          else copy = !(first && a.refs[open] == 1);
+        }
+      }
+      if (old < 0 || (old + bs - 1) >> a.log2_bs > a.max_nb) atomicOr(&faults, TB_TABLES_BAD_LENGTH);
+    }
+    int total;
+    const int place = base + group_scan<1024>(copy, waves, turn, total);
+    base += total;
+    if (i < a.rows) {
+      a.plan[i] = make_int4(src, ctx, copy ? place : -1, old);
+      if (copy) a.copies[place] = make_int4(open, 0, ctx & (bs - 1), i);
+    }
+  }
+  __syncthreads();
+  const int have = a.num_free_in[0];
+  const uint32_t bad = faults | (base > have ? TB_TABLES_OUT_OF_BLOCKS : 0);
+  if (threadIdx.x == 0) {
+    a.head[0] = bad != 0;
+    a.head[1] = base;
+    if (bad) atomicOr(a.status, bad);
+  }
+  if (bad) return;
+  for (int i = threadIdx.x; i < base; i += 1024) {   // (the row's place was written by another thread: behind the barrier)
+    const int at = have - 1 - i, id = a.free_blocks[min(at, a.num_blocks - 1)];
+    const int block = id < 0 || id >= a.num_blocks ? 0 : id;
+    a.copies[i].y = block;
+    a.plan[a.copies[i].w].z = block;
+    a.refs[block] = 1;
+  }
+  // the whole blocks that every live row of a request has: an upper bound of those they share
+  for (int g = threadIdx.x; g < a.rows / K; g += 1024) {
+    int least = INT32_MAX;
+    for (int k = 0; k < K; ++k) {
+      const int len = a.plan[g * K + k].y;
+      if (len > 0) least = min(least, len >> a.log2_bs);
+    }
+    a.shared[g] = least == INT32_MAX ? 0 : least;
+  }
+}
+
+// The positions of an open block, all layers, K and V of every head: runs of n * row_bytes bytes.
+__device__ __forceinline__ void reorder_copy(const reorder_args& a, int unit, int copies) {
+  const int layer = unit / copies, c = unit - layer * copies;
+  const int4 rec = a.copies[c];
+  const int bs_bytes = a.row_bytes << a.log2_bs;
+  const int64_t block_bytes = (int64_t)a.pairs * bs_bytes;
+  const char* const from = a.storage + layer * a.layer_bytes + rec.x * block_bytes;
+  char* const to = a.storage + layer * a.layer_bytes + rec.y * block_bytes;
+  const int run = rec.z * a.row_bytes / 16, all = run * a.pairs;
+  for (int v = threadIdx.x; v < all; v += REORDER_COLUMNS) {
+    const int pair = v / run, off = pair * bs_bytes + (v - pair * run) * 16;
+    st16_through(to + off, ld16(from + off));
+  }
+}
+
+__global__ __launch_bounds__(REORDER_COLUMNS) void reorder_tables_kernel(const reorder_args a, int table_groups) {
+  extern __shared__ int32_t lds[];                 // old entries [beams][128], then per beam {children, keeps}
+  if (a.head[0]) return;
+  if ((int)blockIdx.x >= table_groups) {
+    const int copies = a.head[1], stride = gridDim.x - table_groups;
+    for (int u = blockIdx.x - table_groups; u < copies * a.layers; u += stride) reorder_copy(a, u, copies);
+    return;
+  }
+  __shared__ int waves[2][REORDER_COLUMNS / 64];
+  __shared__ int differ;
+  const int K = a.beams, g = blockIdx.x / a.chunks, chunk = blockIdx.x - g * a.chunks, row0 = g * K;
+  const int tid = threadIdx.x, j = REORDER_COLUMNS * chunk + tid, bs = 1 << a.log2_bs;
+  int32_t* const old = lds + tid;                  // [k * 128]
+  int32_t* const kids = lds + REORDER_COLUMNS * K;
+  int32_t* const keeps = kids + K;
+  const int4* const plan = a.plan + row0;
+  int width = 0;                                   // columns that the request's old tables hold
+  for (int k = 0; k < K; ++k) width = max(width, (plan[k].w + bs - 1) >> a.log2_bs);
+  if (tid < K) kids[tid] = keeps[tid] = 0;
+  if (tid == 0) differ = INT32_MAX;
+  if (chunk == 0 && tid < K) a.lens_out[row0 + tid] = plan[tid].y;
+  if (REORDER_COLUMNS * chunk >= width) {
+    if (tid == 0) a.gone_count[blockIdx.x] = 0;
+    return;
+  }
+  __syncthreads();
+  if (tid < K && plan[tid].x >= 0) {
+    atomicAdd(&kids[plan[tid].x - row0], 1);
+    if (plan[tid].z < 0) atomicOr(&keeps[plan[tid].x - row0], 1);
+  }
+  for (int k = 0; k < K; ++k) old[REORDER_COLUMNS * k] = j < width ? a.tables[(int64_t)(row0 + k) * a.max_nb + j] : -1;
+  __syncthreads();
+  // what every old row's hold on its block of this column becomes; rows of one block behind each other at once
+  auto change = [&](int k) {
+    const int len = plan[k].w;
+    if (j < len >> a.log2_bs) return kids[k] - 1;
+    if (j < (len + bs - 1) >> a.log2_bs) return keeps[k] - 1;   // the open block: one child keeps it, or none
+    return 0;
+  };
+  auto runs = [&](auto&& each) {                   // each(block, change) per run of rows that hold the same block
+    for (int k = 0; k < K;) {
+      const int id = old[REORDER_COLUMNS * k];
+      int sum = 0;
+      for (; k < K && old[REORDER_COLUMNS * k] == id; ++k) sum += change(k);
+      if (sum && id >= 0 && id < a.num_blocks) each(id, sum);
+    }
+  };
+  int lost = 0;
+  if (j < width)
+    runs([&](int id, int sum) {
+      atomicAdd(&a.refs[id], sum);
+      lost += sum < 0;
+    });
+  int total;
+  int at = group_scan<REORDER_COLUMNS>(lost, waves, 0, total);
+  int32_t* const list = a.gone + (int64_t)blockIdx.x * REORDER_COLUMNS * K;
+  if (lost)
+    runs([&](int id, int sum) {
+      if (sum < 0) list[at++] = id;
+    });
+  if (tid == 0) a.gone_count[blockIdx.x] = total;
+  // the new tables, and whether the live rows agree in this column
+  if (j < width) {
+    int one = -1;
+    bool same = true, all = true;                  // all: a whole block of every live row
+    for (int k = 0; k < K; ++k) {
+      const int4 p = plan[k];
+      int id = -1;
+      if (j < (p.y + bs - 1) >> a.log2_bs)
+        id = p.z >= 0 && j == p.y >> a.log2_bs ? p.z : old[REORDER_COLUMNS * (p.x - row0)];
+      a.tables[(int64_t)(row0 + k) * a.max_nb + j] = id;
+      if (p.y > 0) {
+        all &= j < p.y >> a.log2_bs;
+        same &= one < 0 || one == id;
+        one = id;
+      }
+    }
+    if (all && !same) atomicMin(&differ, j);
+  }
+  __syncthreads();
+  if (tid == 0 && differ != INT32_MAX) atomicMin(&a.shared[g], differ);
+}
+
+// The blocks of the lists that nobody holds, each once: the first of a block's entries marks it.
+__global__ __launch_bounds__(1024) void reorder_free_kernel(const reorder_args a, int lists) {
+  __shared__ int waves[2][16];
+  __shared__ int starts[1025];
+  if (a.head[0]) return;
+  const int tid = threadIdx.x;
+  const int left = a.num_free_in[0] - a.head[1];
+  int freed = 0, turn = 0;
+  for (int pass = 0; pass < 2; ++pass) {
+    int before = 0;                                // entries of the lists done
+    for (int l0 = 0; l0 < lists; l0 += 1024) {
+      const int mine = l0 + tid < lists ? a.gone_count[l0 + tid] : 0;
+      int total;
+      starts[tid] = group_scan<1024>(mine, waves, turn++, total);
+      if (tid == 0) starts[1024] = total;
+      __syncthreads();
+      for (int x0 = 0; x0 < total; x0 += 1024) {
+        const int x = x0 + tid;
+        bool win = false;
+        int id = 0;
+        if (x < total) {
+          int lo = 0, hi = 1024;
+          while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (starts[mid] <= x) lo = mid;
+            else hi = mid;
+          }
+          id = a.gone[(int64_t)(l0 + lo) * REORDER_COLUMNS * a.beams + x - starts[lo]];
+          const int mark = before + x - MARK;
+          if (pass == 0) {
+            if (__hip_atomic_load(&a.refs[id], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) <= 0) atomicMin(&a.refs[id], mark);
+          } else {
+            win = __hip_atomic_load(&a.refs[id], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == mark;
+          }
+        }
+        if (pass == 1) {
+          int won;
+          const int at = left + freed + group_scan<1024>(win, waves, turn++, won);
+          freed += won;
+          if (win) {
+            __hip_atomic_store(&a.refs[id], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (at < a.num_blocks) a.free_blocks[at] = id;
+          }
+        }
+      }
+      before += total;
+      __syncthreads();                             // starts is written again
+    }
+    __threadfence();
+    __syncthreads();
+  }
+  if (tid == 0) a.num_free_out[0] = left + freed;
+}
+
+struct reorder_sizes {
+  int64_t plan, copies, count, gone, all, chunks;
+  reorder_sizes(int64_t rows, int64_t beams, int64_t max_nb) {
+    chunks = (max_nb + REORDER_COLUMNS - 1) / REORDER_COLUMNS;
+    const int64_t lists = rows / beams * chunks;
+    plan = 64;
+    copies = plan + 16 * rows;
+    count = copies + 16 * rows;
+    gone = count + 4 * lists;
+    all = gone + 4 * lists * REORDER_COLUMNS * beams;
+  }
+};
+
+}  // namespace tb
+
+extern "C" size_t tb_beam_reorder_workspace_bytes(int32_t num_rows, int32_t beams, int32_t max_blocks_per_row) {
+  if (num_rows <= 0 || beams <= 0 || max_blocks_per_row <= 0) return 64;
+  return (size_t)tb::reorder_sizes(num_rows, beams, max_blocks_per_row).all;
+}
+
+extern "C" int32_t tb_beam_reorder(void* storage, int32_t num_layers, int64_t layer_stride_bytes, int32_t num_blocks,
+                                   int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int32_t dtype,
+                                   int32_t* block_tables, int32_t max_blocks_per_row, int32_t num_rows, int32_t beams,
+                                   const int32_t* lens_in, int32_t* lens_out, int32_t* ref_counts,
+                                   int32_t* free_blocks, const int32_t* num_free_in, int32_t* num_free_out,
+                                   int32_t* shared_blocks, const int32_t* parents, uint32_t* status, void* workspace,
+                                   size_t workspace_bytes, hipStream_t stream) {
+  using namespace tb;
+  TB_CHECK_ARG(num_rows >= 0 && beams > 0 && beams <= TB_BEAMS_MAX && num_rows % beams == 0);
+  TB_CHECK_ARG(max_blocks_per_row > 0 && num_blocks > 0 && num_layers >= 0 && num_layers <= 65535);
+  TB_CHECK_ARG(block_size > 0 && (block_size & (block_size - 1)) == 0);
+  TB_CHECK_ARG((int64_t)num_blocks * block_size < ((int64_t)1 << 31));
+  TB_CHECK_ARG((int64_t)max_blocks_per_row * block_size < ((int64_t)1 << 31));
+  if (num_rows == 0) return TB_OK;
+  const reorder_sizes z(num_rows, beams, max_blocks_per_row);
+  TB_CHECK_ARG((int64_t)num_rows * z.chunks * REORDER_COLUMNS < MARK);
+  TB_CHECK_ARG(block_tables && lens_in && lens_out && ref_counts && free_blocks && num_free_in && num_free_out &&
+               shared_blocks && parents && status && workspace);
+  TB_CHECK_ARG(workspace_bytes >= (size_t)z.all && ((uintptr_t)workspace & 15u) == 0);
+  reorder_args a = {};
+  if (num_layers > 0) {
+    TB_CHECK_ARG(dtype >= TB_DTYPE_F32 && dtype <= TB_DTYPE_BF16 && num_kv_heads > 0 && head_dim > 0);
+    const int64_t row = (int64_t)head_dim * (dtype == TB_DTYPE_F32 ? 4 : 2);
+    if (row % 16) return TB_ERR_UNSUPPORTED;
+    const int64_t block = 2 * (int64_t)num_kv_heads * block_size * row;
+    TB_CHECK_ARG(block < ((int64_t)1 << 31));
+    TB_CHECK_ARG(storage && ((uintptr_t)storage & 15u) == 0 && layer_stride_bytes % 16 == 0);
+    TB_CHECK_ARG(num_layers == 1 || layer_stride_bytes >= num_blocks * block);
+    TB_CHECK_ARG((int64_t)num_layers * num_rows < ((int64_t)1 << 31));
+    a.pairs = 2 * num_kv_heads, a.row_bytes = (int32_t)row;
+  }
+  a.storage = (char*)storage, a.layer_bytes = layer_stride_bytes, a.layers = num_layers, a.num_blocks = num_blocks;
+  a.log2_bs = __builtin_ctz((unsigned)block_size);
+  a.tables = block_tables, a.max_nb = max_blocks_per_row, a.rows = num_rows, a.beams = beams;
+  a.lens_in = lens_in, a.lens_out = lens_out, a.refs = ref_counts, a.free_blocks = free_blocks;
+  a.num_free_in = num_free_in, a.num_free_out = num_free_out, a.shared = shared_blocks, a.parents = parents;
+  a.status = status;
+  char* const ws = (char*)workspace;
+  a.head = (int32_t*)ws, a.plan = (int4*)(ws + z.plan), a.copies = (int4*)(ws + z.copies);
+  a.gone_count = (int32_t*)(ws + z.count), a.gone = (int32_t*)(ws + z.gone), a.chunks = (int32_t)z.chunks;
+  const int lists = (int)(num_rows / beams * z.chunks);
+  const int64_t units = (int64_t)num_rows * num_layers;
+  const int movers = (int)(units < 2048 ? units : 2048);
+  const size_t lds = sizeof(int32_t) * ((size_t)REORDER_COLUMNS * beams + 2 * beams);
+  hipLaunchKernelGGL(reorder_plan_kernel, dim3(1), dim3(1024), 0, stream, a);
+  hipLaunchKernelGGL(reorder_tables_kernel, dim3(lists + movers), dim3(REORDER_COLUMNS), lds, stream, a, lists);
+  hipLaunchKernelGGL(reorder_free_kernel, dim3(1), dim3(1024), 0, stream, a, lists);
+  TB_RETURN_LAUNCH_STATUS();
+}
