@@ -884,6 +884,32 @@ int32_t tb_beam_reorder(void* storage, int32_t num_layers, int64_t layer_stride_
                         int32_t* shared_blocks, const int32_t* parents, uint32_t* status, void* workspace,
                         size_t workspace_bytes, hipStream_t stream);
 
+/* Attention of one new token per row of the state above: row r (its K/V in the pool) sees the positions
+ * 0 .. row_ctx[r] - 1 of its table (0: none, the output is 0), out = softmax(scale q.K) V. The leading
+ * shared_blocks[g] blocks of a request's rows are read once for all of them. fp32 / fp16 / bf16, head_dim 64 or 128,
+ * block_size a power of two >= 16 (TB_ERR_UNSUPPORTED otherwise: use tb_paged_attention), any query heads per
+ * kv head, any scale.
+ *   q [num_rows][num_heads][head_dim], out [num_rows][num_heads * head_dim]: row strides in elements, 16-byte
+ *     aligned rows;
+ *   plan: tb_beam_plan's for these lengths and sizes (tb_beam_plan_bytes, 16-byte aligned), which one launch on
+ *     the GPU makes of row_ctx and shared_blocks for all the calls (layers) of a step; row_ctx beyond a
+ *     row's table counts as its end;
+ *   workspace: tb_beam_attention_workspace_bytes, 16-byte aligned. Calls that may overlap in time need their own. */
+#define TB_BEAM_PARTIAL_BYTES (128 << 20)   /* of the workspace, but for two partials a row */
+size_t tb_beam_plan_bytes(int32_t num_rows, int32_t beams, int32_t num_heads, int32_t num_kv_heads,
+                          int32_t head_dim, int32_t dtype);
+size_t tb_beam_attention_workspace_bytes(int32_t num_rows, int32_t beams, int32_t num_heads,
+                                         int32_t num_kv_heads, int32_t head_dim, int32_t dtype);
+int32_t tb_beam_plan(const int32_t* row_ctx, const int32_t* shared_blocks, int32_t num_rows, int32_t beams,
+                     int32_t max_blocks_per_row, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                     int32_t block_size, int32_t dtype, void* plan, size_t plan_bytes, hipStream_t stream);
+int32_t tb_beam_attention(const void* q, int64_t q_row_stride, const void* pool, int64_t num_blocks,
+                          void* out, int64_t out_row_stride, const int32_t* block_tables,
+                          int32_t max_blocks_per_row, int32_t num_rows, int32_t beams, int32_t num_heads,
+                          int32_t num_kv_heads, int32_t head_dim, int32_t block_size, float scale,
+                          int32_t dtype, const void* plan, size_t plan_bytes, void* workspace,
+                          size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -15,7 +15,8 @@ import torch
 
 from oracle import beams as oracle
 from test_device_tables import random_state
-from tinybatch_amd import (DeviceTables, PagedKVCache, build_device_step, ops, reorder_beams, select_beams)
+from tinybatch_amd import (BeamPlan, DeviceTables, PagedKVCache, beam_attention, build_device_step, ops, reorder_beams,
+                           select_beams)
 from tinybatch_amd.block_manager import OutOfBlocks
 from tinybatch_amd.metadata import build_step_metadata
 
@@ -383,6 +384,114 @@ def test_reorder_the_tables_alone():
     check_state(t, after)
 
 
+# ---- attention ------------------------------------------------------------------------
+def attend(s, hq, hkv, d, dtype, seed=1, magnitude=1.0, ctx=None, scale=None, spare_value=float("nan"), q=None):
+    """Attention over a plain state's rows; every slot that no row sees holds NaN."""
+    g = torch.Generator().manual_seed(seed)
+    ctx = s.lens if ctx is None else ctx
+    pool = torch.full((s.nb, 2, hkv, s.bs, d), spare_value, dtype=dtype)
+    for t, n in zip(s.tables, ctx):
+        for j in range(-(-n // s.bs)):
+            rows = min(s.bs, n - s.bs * j)
+            pool[t[j], :, :, :rows] = torch.randn(2, hkv, rows, d, generator=g).to(dtype)
+    if q is None:
+        q = (torch.randn(len(ctx), hq, d, generator=g) * magnitude).to(dtype)
+    t = upload(s)
+    plan = BeamPlan(t, num_heads=hq, num_kv_heads=hkv, head_dim=d, dtype=dtype).build(i32(ctx))
+    dev = pool.to(DEV)
+    got = beam_attention(q.to(DEV), dev, plan, scale=scale)
+    check_attention(got, q, pool, s.tables, ctx, hq, scale)
+    return got, q, dev, plan
+
+
+GEOMETRIES = [(14, 2, 64), (32, 8, 128), (4, 4, 64), (12, 1, 128), (5, 5, 128), (33, 1, 64), (70, 1, 128)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hq,hkv,d", GEOMETRIES)
+@pytest.mark.parametrize("groups,K", [(5, 1), (4, 3), (3, 8), (1, 24)])
+def test_attention(groups, K, hq, hkv, d, dtype):
+    attend(random_state(groups * K, groups, K, 16, 400), hq, hkv, d, dtype)
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.float16, 128), (torch.float32, 64)])
+@pytest.mark.parametrize("bs", [16, 32, 128])
+def test_attention_block_sizes(bs, dtype, d):
+    attend(random_state(bs, 4, 4, bs, 500), 6, 2, d, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (8, 2, 128)])
+def test_attention_around_its_chunks(hq, hkv, d, dtype):
+    """Contexts that end one position before, on and behind multiples of 16, 64 and 128."""
+    lens = [1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 127, 128, 129, 191, 255, 256, 257, 320]
+    at, tables = 0, []
+    for n in lens:
+        tables.append(list(range(at, at + -(-n // 16))))
+        at += len(tables[-1])
+    attend(oracle.State(tables, lens, [], at + 1, 16, 1), hq, hkv, d, dtype)
+    for K in (2, 5):                               # the same with shared blocks in front
+        shared = list(range(at, at + 9))
+        rows = [shared + t for t in tables[:10]]
+        attend(oracle.State(rows, [144 + n for n in lens[:10]], [], at + 9, 16, K), hq, hkv, d, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_of_long_contexts(dtype):
+    """Few rows: the contexts are cut over workgroups and joined."""
+    s = random_state(3, 1, 4, 16, 1)
+    for K, hq, hkv, d, n in ((4, 14, 2, 64, 9001), (1, 4, 2, 128, 7003), (16, 8, 1, 64, 5000)):
+        shared = list(range(n // 16))
+        own = [[n // 16 + 20 * k + j for j in range(20)] for k in range(K)]
+        lens = [n // 16 * 16 + 37 * (k % 8) + 1 for k in range(K)]
+        attend(oracle.State([shared + o for o in own], lens, [], n // 16 + 20 * K, 16, K), hq, hkv, d, dtype)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_attention_rows_that_see_nothing(dtype):
+    """Ended beams (nothing seen) among live ones, a request without any, a row's own table never read then; their
+    q may hold anything."""
+    s = random_state(6, 5, 4, 16, 200)
+    ctx = list(s.lens)
+    for r in (0, 3, 5, 6, 8, 9, 10, 11, 18):
+        ctx[r] = 0
+    q = torch.randn(20, 14, 64).to(dtype)
+    got, *_ = attend(s, 14, 2, 64, dtype, ctx=ctx, q=q)
+    assert not got[[r for r in range(20) if ctx[r] == 0]].any()
+    q = torch.where(torch.tensor(ctx)[:, None, None] > 0, q, float("nan"))
+    t = upload(s)
+    plan = BeamPlan(t, num_heads=14, num_kv_heads=2, head_dim=64, dtype=dtype).build(i32(ctx))
+    pool = torch.randn(s.nb, 2, 2, 16, 64).to(dtype).to(DEV)
+    got = beam_attention(q.to(DEV), pool, plan)
+    assert torch.isfinite(got).all() and not got[[r for r in range(20) if ctx[r] == 0]].any()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale", [0.0, -0.5, 3.0])
+def test_attention_scales_and_large_scores(dtype, scale):
+    attend(random_state(8, 3, 4, 16, 300), 8, 2, 64, dtype, scale=scale)
+    attend(random_state(9, 3, 4, 16, 300), 8, 2, 128, dtype, magnitude=6.0)
+
+
+def test_attention_into_strided_rows():
+    s = random_state(12, 3, 4, 16, 300)
+    got, q, pool, plan = attend(s, 14, 2, 64, torch.bfloat16)
+    wide = torch.full((12, 2 * 14 * 64), 7.0, dtype=torch.bfloat16, device=DEV)
+    wide[:, :896] = q.to(DEV).view(12, -1)
+    out = torch.full((12, 1000), 7.0, dtype=torch.bfloat16, device=DEV)
+    beam_attention(wide[:, :896], pool, plan, out=out[:, 8:904])
+    assert torch.equal(out[:, 8:904], got) and (out[:, :8] == 7).all() and (out[:, 904:] == 7).all()
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_attention_of_random_states(seed):
+    g = np.random.default_rng(500 + seed)
+    dtype, d = TYPES[seed % 3], (64, 128)[seed // 3 % 2]
+    hkv, rep, K = int(g.integers(1, 4)), int(g.choice([1, 2, 3, 5, 7, 8, 12, 33])), int(g.choice([1, 2, 3, 4, 8, 13]))
+    s = random_state(seed, int(g.integers(1, 7)), K, int(g.choice([16, 32, 64])), int(g.choice([20, 200, 3000])))
+    attend(s, hkv * rep, hkv, d, dtype, seed=seed)
+
+
 # ---- refusals -------------------------------------------------------------------------
 def test_refusals():
     logits, scores = torch.zeros(4, 10, device=DEV), torch.zeros(2, 2, device=DEV)
@@ -426,3 +535,33 @@ def test_refusals():
                 lambda: t.new_step(max_tokens=4).metadata(t)):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_attention_refusals():
+    s = random_state(1, 2, 2, 16, 40)
+    t = upload(s)
+    kw = dict(num_heads=4, num_kv_heads=2, head_dim=64, dtype=torch.float16)
+    plan = BeamPlan(t, **kw)
+    q, pool = torch.zeros(4, 4, 64, dtype=torch.float16, device=DEV), torch.zeros(s.nb, 2, 2, 16, 64, dtype=torch.float16, device=DEV)
+    with pytest.raises(ValueError, match="built"):
+        beam_attention(q, pool, plan)
+    plan.build()
+    for bad in (dict(num_heads=5), dict(head_dim=96), dict(num_kv_heads=0)):
+        with pytest.raises(ValueError):
+            BeamPlan(t, **{**kw, **bad})
+    with pytest.raises(ValueError):
+        BeamPlan(upload(random_state(1, 2, 2, 8, 40)), **kw)
+    with pytest.raises(TypeError):
+        BeamPlan(t, **{**kw, "dtype": torch.int8})
+    for bad in (lambda: plan.build(i32([1] * 3)), lambda: plan.build(torch.ones(4, dtype=torch.int32)),
+                lambda: beam_attention(q.float(), pool, plan), lambda: beam_attention(q.float(), pool.float(), plan)):
+        with pytest.raises(TypeError):
+            bad()
+    for bad in (lambda: beam_attention(q[:3], pool, plan), lambda: beam_attention(q, pool[:-1], plan),
+                lambda: beam_attention(q, pool[:, :, :1].contiguous(), plan), lambda: beam_attention(q[:, :3], pool, plan),
+                lambda: beam_attention(q, pool, plan, out=q.float()), lambda: beam_attention(q, pool, plan, out=q[:3]),
+                lambda: beam_attention(q.transpose(1, 2), pool, plan)):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError):
+        beam_attention(q.cpu(), pool, plan)

@@ -171,3 +171,36 @@ def test_rows_of_no_whole_pieces_are_unsupported_and_no_rows_are_nothing():
     assert call(L.tb_beam_reorder, REORDER, d=12) == _lib.TB_ERR_UNSUPPORTED
     assert call(L.tb_beam_reorder, REORDER, rows=0) == _lib.TB_OK
     assert call(L.tb_beam_select, SELECT, rows=0, logits=None) == _lib.TB_OK
+
+
+PLAN = dict(ctx=F, shared=F, rows=8, beams=4, max_nb=8, hq=4, hkv=2, d=64, bs=16, dtype=2, plan=F, bytes=1 << 20, stream=None)
+ATTEND = dict(q=F, qs=256, pool=F, nb=64, out=F, os=256, tables=F, max_nb=8, rows=8, beams=4, hq=4, hkv=2, d=64, bs=16,
+              scale=0.125, dtype=2, plan=F, bytes=1 << 20, ws=F, ws_bytes=1 << 28, stream=None)
+
+
+@pytest.mark.parametrize("bad", [
+    dict(rows=7), dict(rows=-4), dict(beams=0), dict(beams=65, rows=65), dict(hq=5), dict(hq=0), dict(hkv=0), dict(dtype=3),
+    dict(bs=24), dict(bs=0), dict(max_nb=0), dict(max_nb=1 << 27), dict(plan=None), dict(plan=ctypes.c_void_p(4104)),
+    dict(bytes=64)])
+def test_plan_and_attention_refusals(bad):
+    L = _lib.lib()
+    assert call(L.tb_beam_plan, PLAN, **bad) == _lib.TB_ERR_INVALID_ARG
+    assert call(L.tb_beam_attention, ATTEND, **bad) == _lib.TB_ERR_INVALID_ARG
+
+
+@pytest.mark.parametrize("bad", [
+    dict(q=None), dict(pool=None), dict(out=None), dict(tables=None), dict(ws=None), dict(qs=255), dict(os=255), dict(qs=260),
+    dict(os=260), dict(nb=0), dict(q=ctypes.c_void_p(4104)), dict(out=ctypes.c_void_p(4104)), dict(ws_bytes=1000)])
+def test_attention_refusals(bad):
+    assert call(_lib.lib().tb_beam_attention, ATTEND, **bad) == _lib.TB_ERR_INVALID_ARG
+
+
+def test_attention_unsupported_and_empty():
+    L = _lib.lib()
+    for bad in (dict(d=96), dict(bs=8)):
+        assert call(L.tb_beam_plan, PLAN, **bad) == _lib.TB_ERR_UNSUPPORTED
+        assert call(L.tb_beam_attention, ATTEND, **bad) == _lib.TB_ERR_UNSUPPORTED
+    assert call(L.tb_beam_plan, PLAN, rows=0, ctx=None) == _lib.TB_OK
+    assert call(L.tb_beam_attention, ATTEND, rows=0, q=None) == _lib.TB_OK
+    assert call(L.tb_beam_plan, PLAN, ctx=None) == _lib.TB_ERR_INVALID_ARG
+    assert call(L.tb_beam_plan, PLAN, shared=None) == _lib.TB_ERR_INVALID_ARG

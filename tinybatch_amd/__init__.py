@@ -9,9 +9,9 @@ from .kv_cache import PagedKVCache
 from .tree import (TreeMetadata, TreeVerdict, build_tree_metadata, commit_tree, tree_append, tree_attention,
                    verify_tree, verify_tree_greedy)
 from .device_tables import DeviceStep, DeviceTables, build_device_step
-from .beams import BeamChoice, reorder_beams, select_beams
+from .beams import BeamChoice, BeamPlan, beam_attention, reorder_beams, select_beams
 from . import ops
 
-__all__ = ["BeamChoice", "DeviceStep", "DeviceTables", "PagedKVCache", "StepMetadata", "TreeMetadata", "TreeVerdict",
-           "build_device_step", "build_step_metadata", "build_tree_metadata", "commit_tree", "ops", "reorder_beams",
+__all__ = ["BeamChoice", "BeamPlan", "DeviceStep", "DeviceTables", "PagedKVCache", "StepMetadata", "TreeMetadata",
+           "TreeVerdict", "beam_attention", "build_device_step", "build_step_metadata", "build_tree_metadata", "commit_tree", "ops", "reorder_beams",
            "select_beams", "tree_append", "tree_attention", "verify_tree", "verify_tree_greedy"]

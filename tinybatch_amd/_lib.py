@@ -174,6 +174,14 @@ SIGNATURES = {
         c_vp, c_i32, c_i32, c_i32, c_vp, c_vp,                   # tables, max_nb, rows, beams, lens in, out
         c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp,                # refs, free, num_free in, out, shared, parents, status
         c_vp, c_sz, c_vp]),                                      # workspace, bytes, stream
+    "tb_beam_plan_bytes": (c_sz, [c_i32, c_i32, c_i32, c_i32, c_i32, c_i32]),
+    "tb_beam_attention_workspace_bytes": (c_sz, [c_i32, c_i32, c_i32, c_i32, c_i32, c_i32]),
+    "tb_beam_plan": (c_i32, [c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_i32, c_vp, c_sz, c_vp]),
+    "tb_beam_attention": (c_i32, [
+        c_vp, c_i64, c_vp, c_i64, c_vp, c_i64,   # q, q stride, pool, num_blocks, out, out stride
+        c_vp, c_i32, c_i32, c_i32,               # block tables, max_nb, rows, beams
+        c_i32, c_i32, c_i32, c_i32, c_f32, c_i32,   # heads, kv heads, head_dim, block_size, scale, dtype
+        c_vp, c_sz, c_vp, c_sz, c_vp]),          # plan, bytes, workspace, bytes, stream
     "tb_rms_norm": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i32, c_i32, c_f32, c_i32, c_vp]),
     "tb_rope_qk": (c_i32, [c_vp, c_i64, c_vp, c_vp, c_vp, c_i32, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32, c_i32,
                            c_vp]),

@@ -4,7 +4,7 @@ The reference decodes one continuation per request (src/tinybatch/engine.py:99-1
 has ``group_size`` rows, its beams, whose paged state lives on the GPU (DeviceTables):
 
     build_device_step(tables, new_lens, step)                    # one token per beam
-    plan.build(step.row_ctx)
+    plan.build(step.row_ctx)                                     # a BeamPlan, for all layers
     for layer in range(n_layers):
         ops.kv_append(cache.pools[layer], k, v, step.slot_mapping)
         attn = beam_attention(q, cache.pools[layer], plan)
@@ -15,12 +15,14 @@ Everything is enqueued on the tensors' device's current stream and nothing synch
 """
 from __future__ import annotations
 
+import math
 from typing import NamedTuple
 
 import torch
 
 from . import _lib
 from .device_tables import MAX_BEAMS, DeviceStep, DeviceTables, _ints
+from .ops import _check_pool, _rows_view
 from .tree import _elsewhere, _scratch
 
 MAX_CANDIDATES = 128         # TB_BEAM_CANDIDATES_MAX
@@ -132,3 +134,91 @@ def reorder_beams(storage: torch.Tensor | None, tables: DeviceTables, parents: t
     finally:
         lock.release()
     _lib.check(st, "tb_beam_reorder")
+
+
+class BeamPlan:
+    """How a step's attention is cut over the GPU (tb_beam_plan), for one geometry: made on the GPU from
+    the lengths that are there, once for all layers of a step. A plan belongs to its tables; build() it anew for every step,
+    on the stream of the calls that use it."""
+
+    def __init__(self, tables: DeviceTables, *, num_heads: int, num_kv_heads: int, head_dim: int, dtype: torch.dtype):
+        if dtype not in _lib.DTYPE_CODE:
+            raise TypeError(f"unsupported dtype {dtype}")
+        if num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads or num_heads > 4096:
+            raise ValueError(f"num_heads {num_heads} is not a multiple of kv heads {num_kv_heads} (of at most 4096)")
+        if head_dim not in (64, 128):
+            raise ValueError(f"head_dim {head_dim} is not served (64 and 128 are)")
+        if tables.block_size < 16:
+            raise ValueError("blocks of fewer than 16 positions are not served")
+        self.tables, self.num_heads, self.num_kv_heads = tables, num_heads, num_kv_heads
+        self.head_dim, self.dtype = head_dim, dtype
+        self.built = False
+        L = _lib.lib()
+        sizes = (tables.num_rows, tables.group_size, num_heads, num_kv_heads, head_dim, _lib.DTYPE_CODE[dtype])
+        self.buffer = torch.zeros(max(16, L.tb_beam_plan_bytes(*sizes)), dtype=torch.uint8, device=tables.device)
+        self.workspace_bytes = L.tb_beam_attention_workspace_bytes(*sizes)
+
+    def build(self, row_ctx: torch.Tensor | None = None) -> "BeamPlan":
+        """The plan for rows that see row_ctx [rows] int32 positions (0: none): a step's row_ctx
+        (DeviceTables.new_step(padded=1)), by default the tables' lengths."""
+        t = self.tables
+        row_ctx = t.context_lens if row_ctx is None else row_ctx
+        _ints("row_ctx", row_ctx, torch.int32, (t.num_rows,), t.device)
+        if _elsewhere(t.device):
+            with torch.cuda.device(t.device):
+                return self.build(row_ctx)
+        st = _lib.lib().tb_beam_plan(row_ctx.data_ptr(), t.shared_blocks.data_ptr(), t.num_rows, t.group_size,
+                                     t.max_blocks, self.num_heads, self.num_kv_heads, self.head_dim, t.block_size,
+                                     _lib.DTYPE_CODE[self.dtype], self.buffer.data_ptr(), self.buffer.numel(),
+                                     _lib.stream_handle(t.device))
+        _lib.check(st, "tb_beam_plan")
+        self.built = True
+        return self
+
+
+def beam_attention(q: torch.Tensor, pool: torch.Tensor, plan: BeamPlan, *, scale: float | None = None,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of one new token per row (tb_beam_attention): row r over the positions of its table that the plan
+    was built for, the blocks that a request's rows share read once for all of them. The new tokens' K/V
+    must be in the pool (ops.kv_append, same stream).
+
+    q: [rows, num_heads, head_dim] (after rotation) in the pool's dtype; returns [rows, num_heads *
+    head_dim]. ``scale``: 1 / sqrt(head_dim) by default. A row that sees nothing gives 0."""
+    nb, hkv, bs, d = _check_pool(pool)
+    device, dtype, t = pool.device, pool.dtype, plan.tables
+    if q.device != device:
+        _lib.require_gpu_tensor("q", q)
+        raise ValueError(f"q is on {q.device}, the pool on {device}")
+    if t.device != device:
+        raise ValueError(f"the plan is on {t.device}, the pool on {device}")
+    if not plan.built:
+        raise ValueError("the plan has not been built (BeamPlan.build)")
+    if q.dtype != dtype or plan.dtype != dtype:
+        raise TypeError(f"q {q.dtype}, pool {dtype} and plan {plan.dtype} differ in dtype")
+    if hkv != plan.num_kv_heads or d != plan.head_dim or bs != t.block_size or nb < t.num_blocks:
+        raise ValueError(f"the plan is for {t.num_blocks} blocks of {t.block_size} positions, {plan.num_kv_heads} kv heads "
+                         f"of {plan.head_dim}; the pool is {tuple(pool.shape)}")
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return beam_attention(q, pool, plan, scale=scale, out=out)
+    hq, R = plan.num_heads, t.num_rows
+    qs = _rows_view("q", q, hq, d)
+    if q.shape[0] != R:
+        raise ValueError(f"q has {q.shape[0]} rows, the tables {R}")
+    if out is None:
+        out, os_ = torch.empty(R, hq * d, device=device, dtype=dtype), hq * d
+    else:
+        if out.dtype != dtype or out.shape[0] != R or out.device != device:
+            raise ValueError("out must match q's dtype, device and row count")
+        os_ = _rows_view("out", out, hq, d)
+    stream = _lib.stream_handle(device)
+    lock, ws, ws_bytes, _, _ = _scratch(device, stream, plan.workspace_bytes, 0)
+    try:
+        st = _lib.lib().tb_beam_attention(
+            q.data_ptr(), qs, pool.data_ptr(), nb, out.data_ptr(), os_, t.block_tables.data_ptr(), t.max_blocks, R,
+            t.group_size, hq, hkv, d, bs, 1.0 / math.sqrt(d) if scale is None else float(scale), _lib.DTYPE_CODE[dtype],
+            plan.buffer.data_ptr(), plan.buffer.numel(), ws.data_ptr(), ws_bytes, stream)
+    finally:
+        lock.release()
+    _lib.check(st, "tb_beam_attention")
+    return out

@@ -20,7 +20,7 @@ LIB_NAME = "libtinybatch_amd.so"
 LIB_PATH = os.path.join(PKG_DIR, LIB_NAME)
 SOURCES = ["tb_append.hip", "tb_attention.hip", "tb_copy.hip", "tb_fused.hip", "tb_linear.hip", "tb_decode.hip",
            "tb_prefill.hip", "tb_prefill_cols.hip", "tb_tree.hip", "tb_verify.hip", "tb_step.hip", "tb_beam_select.hip",
-           "tb_beam_state.hip", "tb_metadata.cpp"]
+           "tb_beam_state.hip", "tb_beam_attention.hip", "tb_metadata.cpp"]
 
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = "gfx950"
