@@ -850,14 +850,14 @@ int32_t tb_device_step(int32_t* block_tables, int32_t max_blocks_per_row, const 
 
 /* The best continuations of every request: with s = scores[row] and x = logits[row] of beam k,
  *   c(k, v) = s + x[v] - log(sum_u exp(x[u])),
- * the num_candidates largest over k and v, largest first, the smaller k * vocab + v first among
- * equals: out_scores, out_parents (k), out_tokens (v) [num_rows / beams][num_candidates]; -inf, -1, -1
+ * the num_candidates largest over k and v, largest first; among equals the smaller k first, within a beam the
+ * larger logit (c, rounded, may no longer show it), then the smaller v: out_scores, out_parents (k), out_tokens (v) [num_rows / beams][num_candidates]; -inf, -1, -1
  * where no candidate above -inf is left. finished (may be NULL) [num_rows]: a beam that has ended has the one
  * candidate (k, end_token) with c = s, and its logits are not read; nor are those of a beam whose score is -inf
  * or NaN, which has none. A logit that is NaN counts as -inf, +inf as the largest fp32 number. Decided in 64 bits from
  * sums of fp32 exponentials. logits fp32 / fp16 / bf16, row stride in elements, aligned to their
  * elements; vocab <= 2^30, num_rows <= 65535; workspace: tb_beam_select_workspace_bytes, 16-byte aligned. */
-size_t tb_beam_select_workspace_bytes(int32_t num_rows, int32_t vocab);
+size_t tb_beam_select_workspace_bytes(int32_t num_rows, int32_t vocab, int32_t num_candidates);
 int32_t tb_beam_select(const void* logits, int64_t row_stride, int32_t vocab, int32_t dtype,
                        const float* scores, const uint8_t* finished, int32_t end_token, int32_t num_rows,
                        int32_t beams, int32_t num_candidates, float* out_scores, int32_t* out_parents,

@@ -97,13 +97,14 @@ def reorder(state: State, parents):
 
 
 def select(logits, scores, picks, finished=None, end_token=-1):
-    """(scores, parents, tokens) [G, M] of float64 logits [G * K, V] and scores [G, K]."""
+    """(scores, parents, tokens) [G, M] of float64 logits [G * K, V] and scores [G, K]. Among equal scores the smaller
+    beam first, within a beam the larger logit (scores, rounded, may be equal where logits are not), then the smaller token."""
     G, K = scores.shape
     V = logits.shape[1]
     top = float(np.finfo(np.float32).max)
     out = np.full((G, picks), -np.inf), np.full((G, picks), -1), np.full((G, picks), -1)
     for g in range(G):
-        c = np.full((K, V), -np.inf)
+        c, logit = np.full((K, V), -np.inf), np.zeros((K, V))
         for k in range(K):
             s = float(scores[g, k])
             if finished is not None and finished[g, k]:
@@ -114,8 +115,9 @@ def select(logits, scores, picks, finished=None, end_token=-1):
                 m = x.max()
                 if m > -math.inf:
                     c[k] = s + ((x - m) - np.log(np.exp(x - m).sum()))
+                    logit[k] = x
         flat = c.reshape(-1)
-        at = np.argsort(-flat, kind="stable")[:picks]
+        at = np.lexsort((-logit.reshape(-1), np.arange(K * V) // V, -flat))[:picks]
         at = at[flat[at] > -np.inf]
         out[0][g, :len(at)], out[1][g, :len(at)], out[2][g, :len(at)] = flat[at], at // V, at % V
     return out

@@ -164,7 +164,7 @@ SIGNATURES = {
         c_i32, c_i32, c_vp, c_vp, c_i32, c_i32,  # partition, rows per item, offsets, items, max items, max partitions
         c_vp, c_i32, c_vp, c_vp,                 # split rows, max split rows, counts, status
         c_vp, c_sz, c_vp]),                      # workspace, bytes, stream
-    "tb_beam_select_workspace_bytes": (c_sz, [c_i32, c_i32]),
+    "tb_beam_select_workspace_bytes": (c_sz, [c_i32, c_i32, c_i32]),
     "tb_beam_select": (c_i32, [c_vp, c_i64, c_i32, c_i32,            # logits, stride, vocab, dtype
                                c_vp, c_vp, c_i32, c_i32, c_i32, c_i32,   # scores, finished, end, rows, beams, candidates
                                c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),     # outputs, workspace, bytes, stream

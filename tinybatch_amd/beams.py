@@ -38,8 +38,8 @@ class BeamChoice(NamedTuple):
 def select_beams(logits: torch.Tensor, scores: torch.Tensor, *, num_candidates: int | None = None,
                  finished: torch.Tensor | None = None, end_token: int = -1) -> BeamChoice:
     """The ``num_candidates`` (by default as many as beams) best continuations of every request
-    (tb_beam_select): candidate (k, v) is worth scores[g, k] + log_softmax(logits[g * K + k])[v], the
-    smaller k * vocab + v first among equals.
+    (tb_beam_select): candidate (k, v) is worth scores[g, k] + log_softmax(logits[g * K + k])[v]; among
+    equals the smaller k first, within a beam the larger logit, then the smaller v.
 
     logits [G * K, vocab] (fp32, fp16 or bf16, contiguous rows); scores [G, K] float32, the beams' sums of
     log-probabilities (-inf: no beam). ``finished`` [G, K] bool: a beam that has ended stands for itself
@@ -75,7 +75,7 @@ def select_beams(logits: torch.Tensor, scores: torch.Tensor, *, num_candidates: 
                      torch.empty(G, M, dtype=torch.int32, device=device),
                      torch.empty(G, M, dtype=torch.int64, device=device))
     L, stream = _lib.lib(), _lib.stream_handle(device)
-    need = L.tb_beam_select_workspace_bytes(G * K, vocab)
+    need = L.tb_beam_select_workspace_bytes(G * K, vocab, M)
     lock, ws, ws_bytes, _, _ = _scratch(device, stream, need, 0)
     try:
         st = L.tb_beam_select(logits.data_ptr(), stride, vocab, _lib.DTYPE_CODE[logits.dtype], scores.data_ptr(),

@@ -3,13 +3,18 @@
 // Beam k with score s_k and logits x_k: continuing with token v makes
 //   c(k, v) = s_k + ((x_kv - m_k) - log S_k),  m_k = max_u x_ku,  S_k = sum_u e^(x_ku - m_k);
 // a beam that has finished has one candidate, c(k, end) = s_k. Of a request's candidates the M
-// largest are told, the one of the smaller k V + v first among equals.
+// largest are told; among equals the smaller beam's first, within a beam the larger logit (which c, rounded, may
+// no longer show), then the smaller token.
 //
-// Launch 1 reads the logits once: a wave walks a run of tiles of 512 tokens (8 a lane), keeps the tile's
-// maximum (in memory) and the sum of e^(x - r) against a reference r per lane that moves only when a logit outgrows it by 8.
-// Launch 2, a workgroup per request: the M best tiles by their maxima. A request's M best tokens
-// lie in its M best tiles: the best tokens of the others are behind M better ones already. Then the M best
-// tokens of those tiles.
+// Launch 1 reads the logits once: a wave walks a run of tiles of 512 tokens (8 a lane), writes the maxima of
+// segments of the row (8 to 512 tokens, so that a row has at most 1024) and adds up e^(x - r) against a reference r per
+// lane that moves only when a logit outgrows it by 8.
+// Launch 2, a workgroup per beam: its M best tokens by (x, v), which need no sum. They lie in its M best
+// segments (the best tokens of the others are behind M better ones already): a threshold t that at least
+// M segment maxima reach, by bisection over the maxima in registers; the tokens of those segments above t, and
+// at t the first M; their order by counting the better ones of each.
+// Launch 3, a workgroup per request: of its beams' lists the M best by c. The M-th best of a sample
+// of the lists' heads bounds what can be among them, then again by counting.
 // Sums of a wave's tiles, S, its logarithm and every c are in 64 bits: the order of two beams' candidates is decided
 // by differences far below a float's step at the score's size.
 #include "tb_common.h"
@@ -18,7 +23,12 @@ namespace tb {
 
 constexpr int SELECT_TILE = 512;                   // tokens: 8 a lane
 constexpr int SELECT_WAVES = 4;                    // of a workgroup of launch 1
-constexpr int SELECT_THREADS = 1024;               // of launch 2
+constexpr int SELECT_SEGMENTS = 1024;              // of a row, at most
+constexpr int SELECT_THREADS = 512;                // of launch 2
+constexpr int SELECT_LIST = 1536, SELECT_EQUALS = 512;   // tokens above t and at t that launch 2 keeps in LDS
+constexpr int MERGE_THREADS = 1024;
+constexpr int MERGE_LIST = 4352;                   // what a sample's bound leaves of 64 lists of 128 at most
+constexpr float SELECT_MOST = 3.402823466e38f;
 
 struct select_args {
   const char* logits;          // [rows][V]
@@ -32,42 +42,54 @@ struct select_args {
   int32_t* out_parents;
   int64_t* out_tokens;
   int32_t tiles, runs, per_run;   // tiles of a row, runs of a row, tiles of a run
-  float* tile_max;             // [rows][tiles]
+  int32_t log2_lanes;          // lanes of a segment inside a tile: 2^log2_lanes
+  int32_t tops;                // segment maxima that launch 1 writes per row
+  int32_t join, segments;      // of them in a segment (1 unless a segment is several tiles), segments of a row
+  float* seg_max;              // [rows][tops]
   double2* sums;               // [rows][runs]: {S, r}
+  double2* norms;              // [rows]: {m, log S}
+  float2* lists;               // [rows][M]: {x, token}, best first, then -inf
 };
 
 // A logit as it counts: NaN as -inf, +inf as the largest number.
-__device__ __forceinline__ float select_logit(float x) {
-  return x == x ? fminf(x, 3.402823466e38f) : -INFINITY;
-}
+__device__ __forceinline__ float select_logit(float x) { return x == x ? fminf(x, SELECT_MOST) : -INFINITY; }
 __device__ __forceinline__ bool select_open(const select_args& a, int row) {   // whether the row's logits count
   return !(a.finished && a.finished[row]) && a.scores[row] > -INFINITY;
 }
 
-// 8 logits of a lane from token t0 on; past the vocabulary -inf.
+// 8 logits of a lane from token t0 on, as they lie there; past the vocabulary -inf. (Rows start at any element.)
 template <typename T>
-__device__ __forceinline__ void select_load(const char* row, int t0, int vocab, float (&x)[8]) {
-  struct __attribute__((packed, aligned(sizeof(T)))) eight {
-    T v[8];
-  };
-  if (t0 + 8 <= vocab) {
-    const eight e = *reinterpret_cast<const eight*>(row + (int64_t)t0 * sizeof(T));
+struct __attribute__((packed, aligned(sizeof(T)))) eight_logits {
+  T v[8];
+};
+template <typename T>
+__device__ __forceinline__ eight_logits<T> select_load(const char* row, int t0, int vocab) {
+  if (t0 + 8 <= vocab) return *reinterpret_cast<const eight_logits<T>*>(row + (int64_t)t0 * sizeof(T));
+  eight_logits<T> e;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = select_logit((float)e.v[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      x[i] = t0 + i < vocab ? select_logit((float)reinterpret_cast<const T*>(row)[t0 + i]) : -INFINITY;
-  }
+  for (int i = 0; i < 8; ++i) e.v[i] = t0 + i < vocab ? reinterpret_cast<const T*>(row)[t0 + i] : (T)-INFINITY;
+  return e;
 }
 
-__device__ __forceinline__ float wave_max(float x) {
-  x = fmaxf(x, dpp<DPP_QUAD_XOR1>(x));
-  x = fmaxf(x, dpp<DPP_QUAD_XOR2>(x));
-  x = fmaxf(x, dpp<DPP_ROW_HALF_MIRROR>(x));
-  x = fmaxf(x, dpp<DPP_ROW_MIRROR>(x));
-  x = max_xor16(x);
-  return max_xor32(x);
+// Maximum over aligned groups of 2^n lanes.
+__device__ __forceinline__ float lanes_max(float x, int n) {
+  if (n >= 1) x = fmaxf(x, dpp<DPP_QUAD_XOR1>(x));
+  if (n >= 2) x = fmaxf(x, dpp<DPP_QUAD_XOR2>(x));
+  if (n >= 3) x = fmaxf(x, dpp<DPP_ROW_HALF_MIRROR>(x));
+  if (n >= 4) x = fmaxf(x, dpp<DPP_ROW_MIRROR>(x));
+  if (n >= 5) x = max_xor16(x);
+  if (n >= 6) x = max_xor32(x);
+  return x;
+}
+
+// e^d for d <= 8, by the exponential of the rounded product d log2(e) and a first-order term for what the
+// rounding (and the constant's) took; -inf and NaN give 0. Off by the hardware's exponential, a step.
+__device__ __forceinline__ float select_exp(float d) {
+  constexpr float HI = 1.44269502162933349609375f, LO = 1.925963033500011e-8f, LN2 = 0.693147180559945f;
+  d = fmaxf(d, -150.f);
+  const float y = d * HI, e = fast_exp2(y);
+  const float rest = fmaf(d, LO, fmaf(d, HI, -y));
+  return fmaf(e, rest * LN2, e);
 }
 
 template <typename T>
@@ -77,147 +99,402 @@ __global__ __launch_bounds__(64 * SELECT_WAVES) void select_scan_kernel(const se
   if (run >= a.runs || !select_open(a, row)) return;
   const char* const at = a.logits + (int64_t)row * a.row_bytes;
   const int first = run * a.per_run, last = min(first + a.per_run, a.tiles);
-  float ref = -3.402823466e38f;
+  float* const tops = a.seg_max + (int64_t)row * a.tops;
+  float ref = -SELECT_MOST;
   double sum = 0.;
+  eight_logits<T> next = select_load<T>(at, first * SELECT_TILE + 8 * lane, a.vocab);
   for (int t = first; t < last; ++t) {
+    const eight_logits<T> now = next;
+    if (t + 1 < last) next = select_load<T>(at, (t + 1) * SELECT_TILE + 8 * lane, a.vocab);
     float x[8];
-    select_load<T>(at, t * SELECT_TILE + 8 * lane, a.vocab, x);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = (float)now.v[i];
     float top = x[0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);
-    if (__any(top > ref + 8.f)) {
-      const float r = fmaxf(ref, top);
-      sum *= (double)expf(ref - r);
-      ref = r;
+    for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);   // (a NaN loses against a number)
+    if (__any(!(top <= ref + 8.f))) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = select_logit(x[i]);
+      top = select_logit(top);
+      if (top > ref + 8.f) {
+        sum *= exp((double)ref - (double)top);
+        ref = top;
+      }
     }
     float part = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) part += expf(x[i] - ref);
+    for (int i = 0; i < 8; ++i) part += select_exp(x[i] - ref);
     sum += (double)part;
-    top = wave_max(top);
-    if (lane == 0) a.tile_max[(int64_t)row * a.tiles + t] = top;
+    top = lanes_max(top, a.log2_lanes);
+    const int seg = (t << (6 - a.log2_lanes)) + (lane >> a.log2_lanes);
+    if ((lane & ((1 << a.log2_lanes) - 1)) == 0 && seg < a.tops) tops[seg] = top;
   }
   // the lanes' sums against the largest reference
-  const float r = wave_max(ref);
+  const float r = lanes_max(ref, 6);
   sum *= exp((double)ref - (double)r);
 #pragma unroll
   for (int o = 1; o < 64; o *= 2) sum += __shfl_xor(sum, o);
   if (lane == 0) a.sums[(int64_t)row * a.runs + run] = make_double2(sum, (double)r);
 }
 
-// A candidate and its place in the order: larger value, then smaller index.
+// A float's place among all floats, -inf 0x007FFFFF; -0 is 0.
+__device__ __forceinline__ uint32_t select_order(float x) {
+  const uint32_t b = __float_as_uint(x + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float select_value(uint32_t o) {
+  return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+}
+constexpr uint32_t ORDER_NONE = 0x007FFFFFu;       // of -inf
+
+// Launch 2. Tokens are looked at 512 at a time and wave: 64 >> log2_lanes segments side by side, or one of several tiles.
+template <typename T>
+struct select_row {
+  const select_args& a;
+  const char* at;
+  const int* picked;           // LDS, rising segments
+  int n, lane, wave;
+  // each(piece, token, x): a lane's 8 tokens of a picked segment
+  template <typename F>
+  __device__ __forceinline__ void pieces(F&& each) const {
+    const int per = 64 >> a.log2_lanes, spot = lane >> a.log2_lanes;
+    for (int p0 = wave * per; p0 < n; p0 += SELECT_THREADS / 64 * per) {
+      const int p = p0 + spot;
+      for (int j = 0; j < a.join; ++j) {
+        int t0 = a.vocab;
+        if (p < n) t0 = (((picked[p] * a.join + j) << a.log2_lanes) + (lane & ((1 << a.log2_lanes) - 1))) * 8;
+        float x[8];
+        if (t0 < a.vocab) {
+          const eight_logits<T> e = select_load<T>(at, t0, a.vocab);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = select_logit((float)e.v[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = -INFINITY;
+        }
+        each(p, t0, x);
+      }
+    }
+  }
+};
+
+// Exclusive running sum of a wave's lanes, and its total.
+__device__ __forceinline__ int select_scan(int x, int lane, int& total) {
+  int up = x;
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const int y = __shfl_up(up, o);
+    if (lane >= o) up += y;
+  }
+  total = __builtin_amdgcn_readlane(up, 63);
+  return up - x;
+}
+
+template <typename T>
+__global__ __launch_bounds__(SELECT_THREADS) void select_rows_kernel(const select_args a) {
+  constexpr int WAVES = SELECT_THREADS / 64, WORDS = SELECT_SEGMENTS / 64;
+  constexpr int MOST = TB_BEAM_CANDIDATES_MAX + TB_BEAM_CANDIDATES_MAX / 2 + 8;
+  __shared__ float tops[SELECT_SEGMENTS];
+  __shared__ int picked[MOST];
+  __shared__ uint64_t list[SELECT_LIST + SELECT_EQUALS];   // {order of x, ~token}
+  __shared__ int ranks[SELECT_LIST + SELECT_EQUALS];
+  __shared__ int equal_of[MOST];
+  __shared__ int above, equals, counted;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x, M = a.picks;
+  float2* const out = a.lists + (int64_t)row * M;
+  if (!select_open(a, row)) {                      // one candidate, the score itself, or none
+    const bool one = a.finished && a.finished[row] && a.scores[row] > -INFINITY;
+    for (int i = tid; i < M; i += SELECT_THREADS)
+      out[i] = make_float2(one && i == 0 ? 0.f : -INFINITY, __int_as_float(a.end_token));
+    if (tid == 0) a.norms[row] = make_double2(0., 0.);
+    return;
+  }
+  for (int i = tid; i < SELECT_SEGMENTS; i += SELECT_THREADS) {
+    float x = -INFINITY;
+    if (i < a.segments)
+      for (int j = 0; j < a.join && i * a.join + j < a.tops; ++j)
+        x = fmaxf(x, select_logit(a.seg_max[(int64_t)row * a.tops + i * a.join + j]));
+    tops[i] = x;
+  }
+  if (tid == 0) above = equals = 0;
+  __syncthreads();
+  uint32_t v[WORDS];                               // every wave: all segments, lane l those of l + 64 i
+  float m = -INFINITY, least = INFINITY, mine = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < WORDS; ++i) {
+    const float x = tops[64 * i + lane];
+    mine = fmaxf(mine, x);
+    v[i] = select_order(x);
+  }
+  m = lanes_max(mine, 6);
+  least = -lanes_max(-mine, 6);                    // 64 segments at least reach it
+  if (wave == 0) {                                 // m and log S
+    double s = 0.;
+    for (int r = lane; r < a.runs; r += 64) {
+      const double2 x = a.sums[(int64_t)row * a.runs + r];
+      s += x.x * (m == -INFINITY ? 0. : exp(x.y - (double)m));
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) s += __shfl_xor(s, o);
+    if (lane == 0) a.norms[row] = make_double2((double)m, log(s));
+  }
+  // ---- the threshold ----
+  auto reach = [&](uint32_t o) {
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) c += __popcll(__ballot(v[i] >= o));
+    return c;
+  };
+  uint32_t lo = ORDER_NONE, hi = select_order(m) + 1;
+  bool exact = true;
+  if (reach(ORDER_NONE + 1) >= M) {                // else everything above -inf
+    lo = M <= 64 && least > -INFINITY ? select_order(least) : ORDER_NONE + 1;
+    while (hi - lo > 1) {
+      const uint32_t mid = lo + (hi - lo) / 2;
+      const int c = reach(mid);
+      if (c >= M) {
+        lo = mid;
+        if (c <= M + M / 2 + 8) {
+          exact = false;                           // near enough: all of them
+          break;
+        }
+      } else {
+        hi = mid;
+      }
+    }
+  }
+  // ---- the segments that reach it: rising, at most M where several equal it ----
+  int n = 0;
+  {
+    int over = reach(lo + 1), eq0 = 0;
+    const int need = lo == ORDER_NONE ? 0 : exact ? M - over : SELECT_SEGMENTS;
+    const uint64_t below = ((uint64_t)1 << lane) - 1;
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) {
+      const uint64_t eq = __ballot(v[i] == lo);
+      const bool take = v[i] > lo || (v[i] == lo && eq0 + __popcll(eq & below) < need);
+      const uint64_t took = __ballot(take);
+      if (take && i % WAVES == wave) picked[n + __popcll(took & below)] = 64 * i + lane;
+      eq0 += __popcll(eq);
+      n += __popcll(took);
+    }
+  }
+  __syncthreads();
+  const select_row<T> part{a, a.logits + (int64_t)row * a.row_bytes, picked, n, lane, wave};
+  // ---- the tokens above the threshold, and those at it ----
+  auto push = [&](uint32_t t, bool keep) {
+    part.pieces([&](int, int t0, const float(&x)[8]) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t o = select_order(x[i]);
+        if (o > t) {
+          const int at = atomicAdd(&above, 1);
+          if (at < SELECT_LIST && keep) list[at] = (uint64_t)o << 32 | (uint32_t) ~(t0 + i);
+        } else if (o == t && o != ORDER_NONE) {
+          const int at = atomicAdd(&equals, 1);
+          if (at < SELECT_EQUALS && keep) list[SELECT_LIST + at] = (uint64_t)o << 32 | (uint32_t) ~(t0 + i);
+        }
+      }
+    });
+    __syncthreads();
+  };
+  push(lo, true);
+  if (above > SELECT_LIST) {                       // many tokens above it (whole ranges of high ones): the M-th best token
+    uint32_t t0 = lo, t1 = select_order(m) + 1;    // t0 is reached by M tokens, t1 by none
+    while (t1 - t0 > 1) {
+      const uint32_t mid = t0 + (t1 - t0) / 2;
+      __syncthreads();
+      if (tid == 0) counted = 0;
+      __syncthreads();
+      part.pieces([&](int, int, const float(&x)[8]) {
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c += select_order(x[i]) >= mid;
+        if (c) atomicAdd(&counted, c);
+      });
+      __syncthreads();
+      if (counted >= M) t0 = mid;
+      else t1 = mid;
+    }
+    lo = t0;
+    __syncthreads();
+    if (tid == 0) above = equals = 0;
+    __syncthreads();
+    push(lo, true);
+  }
+  int count_above = above, count_equal = equals;
+  if (count_equal > SELECT_EQUALS) {               // the first M of them: numbered segment by segment
+    const int want = M - min(count_above, M);
+    for (int i = tid; i < n; i += SELECT_THREADS) equal_of[i] = 0;
+    __syncthreads();
+    part.pieces([&](int p, int, const float(&x)[8]) {
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c += select_order(x[i]) == lo;
+      if (c) atomicAdd(&equal_of[p], c);
+    });
+    __syncthreads();
+    if (wave == 0) {                               // running sums over the segments
+      int base = 0;
+      for (int i0 = 0; i0 < n; i0 += 64) {
+        const int i = i0 + lane;
+        int total;
+        const int before = select_scan(i < n ? equal_of[i] : 0, lane, total);
+        if (i < n) equal_of[i] = base + before;
+        base += total;
+      }
+    }
+    __syncthreads();
+    // one wave after the other within a segment's tiles: a segment's tokens are one wave's, in order
+    const int width = 1 << a.log2_lanes;
+    int seen = 0, of = -1;                         // (segments of several tiles: equals of the tiles before)
+    part.pieces([&](int p, int t0, const float(&x)[8]) {
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) c += select_order(x[i]) == lo;
+      int up = c;
+      for (int o = 1; o < width; o *= 2) {
+        const int y = __shfl_up(up, o);
+        if ((lane & (width - 1)) >= o) up += y;
+      }
+      const int all = __shfl(up, (lane & ~(width - 1)) + width - 1);
+      if (p != of) of = p, seen = 0;
+      if (p < n) {
+        int at = equal_of[p] + seen + up - c;
+        for (int i = 0; i < 8; ++i)
+          if (select_order(x[i]) == lo) {
+            if (at < want) list[SELECT_LIST + at] = (uint64_t)lo << 32 | (uint32_t) ~(t0 + i);
+            ++at;
+          }
+      }
+      seen += all;
+    });
+    count_equal = want;
+    __syncthreads();
+  }
+  // ---- their order: how many are better ----
+  const int all = count_above + count_equal;
+  auto entry = [&](int i) { return list[i < count_above ? i : SELECT_LIST + i - count_above]; };
+  for (int i = tid; i < all; i += SELECT_THREADS) ranks[i] = 0;
+  for (int i = tid; i < M; i += SELECT_THREADS)
+    if (i >= all) out[i] = make_float2(-INFINITY, 0.f);
+  __syncthreads();
+  int share = 1;                                   // threads that count for one entry
+  while (share < 64 && 2 * share * all <= SELECT_THREADS) share *= 2;
+  for (int i0 = tid / share; i0 < all; i0 += SELECT_THREADS / share) {
+    const uint64_t e = entry(i0);
+    int c = 0;
+    for (int j = tid % share; j < all; j += share) c += entry(j) > e;
+    if (c) atomicAdd(&ranks[i0], c);
+  }
+  __syncthreads();
+  for (int i = tid; i < all; i += SELECT_THREADS)
+    if (ranks[i] < M) {
+      const uint64_t e = entry(i);
+      out[ranks[i]] = make_float2(select_value((uint32_t)(e >> 32)), __uint_as_float(~(uint32_t)e));
+    }
+}
+
+// Launch 3: a candidate and its place in the order: larger value, then smaller beam, then the beam's own order.
 struct cand {
   double c;
   int64_t at;
 };
 __device__ __forceinline__ bool better(const cand& x, const cand& y) { return x.c > y.c || (x.c == y.c && x.at < y.at); }
-__device__ __forceinline__ cand better_of(const cand& x, const cand& y) { return better(x, y) ? x : y; }
 
-// The workgroup's best candidate, in every thread.
-__device__ __forceinline__ cand group_best(cand x, cand* lds, int turn) {
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) {
-    cand y;
-    y.c = __shfl_xor(x.c, o);
-    y.at = __shfl_xor(x.at, o);
-    x = better_of(x, y);
+// How many of cands[0 .. n) are better than each, in ranks (zero before, a barrier before and behind).
+__device__ __forceinline__ void merge_ranks(const cand* cands, int n, int* ranks) {
+  int share = 1;
+  while (share < 64 && 2 * share * n <= MERGE_THREADS) share *= 2;
+  for (int i = threadIdx.x / share; i < n; i += MERGE_THREADS / share) {
+    const cand e = cands[i];
+    int c = 0;
+    for (int j = threadIdx.x % share; j < n; j += share) c += better(cands[j], e);
+    if (c) atomicAdd(&ranks[i], c);
   }
-  cand* const mine = lds + 16 * (turn & 1);
-  if ((threadIdx.x & 63) == 0) mine[threadIdx.x >> 6] = x;
-  __syncthreads();
-  x = mine[0];
-  for (int w = 1; w < SELECT_THREADS / 64; ++w) x = better_of(x, mine[w]);
-  return x;
 }
 
-template <typename T>
-__global__ __launch_bounds__(SELECT_THREADS) void select_pick_kernel(const select_args a) {
-  __shared__ cand lds[32];
-  __shared__ double top[TB_BEAMS_MAX], norm[TB_BEAMS_MAX];   // m and log S of every beam
-  __shared__ int64_t picked[TB_BEAM_CANDIDATES_MAX];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row0 = blockIdx.x * a.beams;
-  const cand none = {-INFINITY, INT64_MAX};
-  for (int k = wave; k < a.beams; k += SELECT_THREADS / 64) {
-    const int row = row0 + k;
-    float m = -INFINITY;
-    double s = 0.;
-    if (select_open(a, row)) {
-      for (int t = lane; t < a.tiles; t += 64) m = fmaxf(m, a.tile_max[(int64_t)row * a.tiles + t]);
-      m = wave_max(m);
-      for (int r = lane; r < a.runs; r += 64) {
-        const double2 x = a.sums[(int64_t)row * a.runs + r];
-        s += x.x * (m == -INFINITY ? 0. : exp(x.y - (double)m));
-      }
-#pragma unroll
-      for (int o = 1; o < 64; o *= 2) s += __shfl_xor(s, o);
+__global__ __launch_bounds__(MERGE_THREADS) void select_merge_kernel(const select_args a) {
+  __shared__ cand cands[MERGE_LIST];
+  __shared__ int ranks[MERGE_LIST];
+  __shared__ cand bound;
+  __shared__ int held;
+  const int tid = threadIdx.x, M = a.picks, K = a.beams, row0 = blockIdx.x * K;
+  auto look = [&](int k, int p) {
+    const float2 e = a.lists[(int64_t)(row0 + k) * M + p];
+    cand x = {-INFINITY, INT64_MAX};
+    if (e.x > -INFINITY) {
+      const double2 n = a.norms[row0 + k];
+      x.c = (double)a.scores[row0 + k] + (((double)e.x - n.x) - n.y);
+      x.at = (int64_t)k << 32 | p;
     }
-    if (lane == 0) top[k] = (double)m, norm[k] = log(s);
-  }
-  __syncthreads();
-  auto value = [&](int k, float x) {               // c(k, .) of a logit
-    return x == -INFINITY ? -INFINITY : (double)a.scores[row0 + k] + (((double)x - top[k]) - norm[k]);
+    return x;
   };
-  // ---- the M best tiles ----
-  int turn = 0;
-  const int64_t all = (int64_t)a.beams * a.tiles;
-  cand last = {INFINITY, -1};
-  int n = 0;
-  for (; n < a.picks; ++n) {
-    cand best = none;
-    for (int64_t i = tid; i < all; i += SELECT_THREADS) {
-      const int k = (int)(i / a.tiles), t = (int)(i - (int64_t)k * a.tiles), row = row0 + k;
-      cand x = none;
-      if (select_open(a, row)) x = {value(k, a.tile_max[(int64_t)row * a.tiles + t]), i};
-      else if (a.finished && a.finished[row] && t == 0) x = {(double)a.scores[row], i};
-      if (x.c > -INFINITY && better(last, x)) best = better_of(best, x);
+  // the heads of the lists, twice as many as asked for
+  const int depth = min(M, (2 * M + K - 1) / K), sample = K * depth;
+  if (tid == 0) held = 0, bound = cand{-INFINITY, INT64_MAX};
+  for (int i = tid; i < sample; i += MERGE_THREADS) cands[i] = look(i / depth, i % depth), ranks[i] = 0;
+  __syncthreads();
+  merge_ranks(cands, sample, ranks);
+  __syncthreads();
+  int n = sample;
+  if (depth < M) {
+    // what is better than the M-th best of the sample, or is it
+    for (int i = tid; i < sample; i += MERGE_THREADS)
+      if (ranks[i] == M - 1 && cands[i].c > -INFINITY) bound = cands[i];
+    __syncthreads();
+    const cand least = bound;
+    for (int i = tid; i < K * M; i += MERGE_THREADS) {
+      const cand x = look(i / M, i % M);
+      if (x.c > -INFINITY && !better(least, x)) {
+        const int at = atomicAdd(&held, 1);
+        if (at < MERGE_LIST) cands[at] = x, ranks[at] = 0;
+      }
     }
-    best = group_best(best, lds, turn++);
-    if (best.at == INT64_MAX) break;
-    last = best;
-    if (tid == 0) picked[n] = best.at;
+    __syncthreads();
+    n = min(held, MERGE_LIST);
+    merge_ranks(cands, n, ranks);
+    __syncthreads();
+  }
+  const int64_t at = (int64_t)blockIdx.x * M;
+  if (tid == 0) held = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += MERGE_THREADS) {
+    const cand x = cands[i];
+    if (x.c == -INFINITY) continue;
+    atomicAdd(&held, 1);
+    if (ranks[i] >= M) continue;
+    a.out_scores[at + ranks[i]] = (float)x.c;
+    const int k = (int)(x.at >> 32);
+    a.out_parents[at + ranks[i]] = k;
+    a.out_tokens[at + ranks[i]] = __float_as_int(a.lists[(int64_t)(row0 + k) * M + (uint32_t)x.at].y);
   }
   __syncthreads();
-  // ---- the M best tokens of those tiles ----
-  last = {INFINITY, -1};
-  for (int o = 0; o < a.picks; ++o) {
-    cand best = none;
-    for (int p = wave; p < n; p += SELECT_THREADS / 64) {
-      const int k = (int)(picked[p] / a.tiles), t = (int)(picked[p] - (int64_t)k * a.tiles), row = row0 + k;
-      if (!select_open(a, row)) {
-        const cand x = {(double)a.scores[row], (int64_t)k * a.vocab + a.end_token};
-        if (better(last, x)) best = better_of(best, x);
-        continue;
-      }
-      float x[8];
-      select_load<T>(a.logits + (int64_t)row * a.row_bytes, t * SELECT_TILE + 8 * lane, a.vocab, x);
-      for (int i = 0; i < 8; ++i) {
-        const cand y = {value(k, x[i]), (int64_t)k * a.vocab + t * SELECT_TILE + 8 * lane + i};
-        if (y.c > -INFINITY && better(last, y)) best = better_of(best, y);
-      }
-    }
-    best = group_best(best, lds, turn++);
-    last = best;
-    if (tid == 0) {
-      const int64_t at = (int64_t)blockIdx.x * a.picks + o;
-      const bool some = best.at != INT64_MAX;
-      a.out_scores[at] = some ? (float)best.c : -INFINITY;
-      a.out_parents[at] = some ? (int32_t)(best.at / a.vocab) : -1;
-      a.out_tokens[at] = some ? best.at % a.vocab : -1;
-    }
+  for (int i = held + tid; i < M; i += MERGE_THREADS) {
+    a.out_scores[at + i] = -INFINITY;
+    a.out_parents[at + i] = -1;
+    a.out_tokens[at + i] = -1;
   }
 }
 
 struct select_sizes {
-  int32_t tiles, runs, per_run;
-  size_t sums, all;
-  select_sizes(int64_t rows, int64_t vocab) {
+  int32_t tiles, runs, per_run, log2_lanes, tops, join, segments;
+  size_t norms, lists, maxima, all;                // of the workspace; the sums first
+  select_sizes(int64_t rows, int64_t vocab, int64_t picks) {
     tiles = (int32_t)((vocab + SELECT_TILE - 1) / SELECT_TILE);
-    // as many runs as give every CU some 16 waves
-    const int64_t want = (4096 + rows - 1) / rows;
+    // as many runs as give every CU some 32 waves
+    const int64_t want = (8192 + rows - 1) / rows;
     per_run = (int32_t)((tiles + want - 1) / want);
     runs = (tiles + per_run - 1) / per_run;
-    sums = ((size_t)rows * tiles * 4 + 15) / 16 * 16;
-    all = sums + (size_t)rows * runs * 16;
+    log2_lanes = 0;
+    while (log2_lanes < 6 && (vocab + (8 << log2_lanes) - 1) / (8 << log2_lanes) > SELECT_SEGMENTS) ++log2_lanes;
+    tops = (int32_t)((vocab + (8 << log2_lanes) - 1) / (8 << log2_lanes));
+    join = (tops + SELECT_SEGMENTS - 1) / SELECT_SEGMENTS;
+    segments = (tops + join - 1) / join;
+    norms = (size_t)rows * runs * 16;
+    lists = norms + (size_t)rows * 16;
+    maxima = lists + (size_t)rows * picks * 8;
+    all = maxima + (size_t)rows * tops * 4;
   }
 };
 
@@ -225,13 +502,14 @@ template <typename T>
 static void launch_select(const select_args& a, hipStream_t stream) {
   const dim3 grid((a.runs + SELECT_WAVES - 1) / SELECT_WAVES, a.rows);
   hipLaunchKernelGGL(select_scan_kernel<T>, grid, dim3(64 * SELECT_WAVES), 0, stream, a);
-  hipLaunchKernelGGL(select_pick_kernel<T>, dim3(a.rows / a.beams), dim3(SELECT_THREADS), 0, stream, a);
+  hipLaunchKernelGGL(select_rows_kernel<T>, dim3(a.rows), dim3(SELECT_THREADS), 0, stream, a);
+  hipLaunchKernelGGL(select_merge_kernel, dim3(a.rows / a.beams), dim3(MERGE_THREADS), 0, stream, a);
 }
 
 }  // namespace tb
 
-extern "C" size_t tb_beam_select_workspace_bytes(int32_t num_rows, int32_t vocab) {
-  return num_rows > 0 && vocab > 0 ? tb::select_sizes(num_rows, vocab).all : 0;
+extern "C" size_t tb_beam_select_workspace_bytes(int32_t num_rows, int32_t vocab, int32_t num_candidates) {
+  return num_rows > 0 && vocab > 0 && num_candidates > 0 ? tb::select_sizes(num_rows, vocab, num_candidates).all : 0;
 }
 
 extern "C" int32_t tb_beam_select(const void* logits, int64_t row_stride, int32_t vocab, int32_t dtype,
@@ -248,14 +526,17 @@ extern "C" int32_t tb_beam_select(const void* logits, int64_t row_stride, int32_
   TB_CHECK_ARG(num_rows == 1 || row_stride >= vocab);
   const int size = dtype == TB_DTYPE_F32 ? 4 : 2;
   TB_CHECK_ARG((uintptr_t)logits % size == 0 && ((uintptr_t)workspace & 15u) == 0);
-  const select_sizes z(num_rows, vocab);
+  const select_sizes z(num_rows, vocab, num_candidates);
   TB_CHECK_ARG(workspace_bytes >= z.all);
   select_args a;
   a.logits = (const char*)logits, a.row_bytes = row_stride * size, a.rows = num_rows, a.beams = beams, a.vocab = vocab;
   a.scores = scores, a.finished = finished, a.end_token = end_token, a.picks = num_candidates;
   a.out_scores = out_scores, a.out_parents = out_parents, a.out_tokens = out_tokens;
   a.tiles = z.tiles, a.runs = z.runs, a.per_run = z.per_run;
-  a.tile_max = (float*)workspace, a.sums = (double2*)((char*)workspace + z.sums);
+  a.log2_lanes = z.log2_lanes, a.tops = z.tops, a.join = z.join, a.segments = z.segments;
+  char* const ws = (char*)workspace;
+  a.sums = (double2*)ws, a.norms = (double2*)(ws + z.norms), a.lists = (float2*)(ws + z.lists);
+  a.seg_max = (float*)(ws + z.maxima);
   if (dtype == TB_DTYPE_F32) launch_select<float>(a, stream);
   else if (dtype == TB_DTYPE_F16) launch_select<_Float16>(a, stream);
   else launch_select<__bf16>(a, stream);
