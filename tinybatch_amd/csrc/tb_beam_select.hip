@@ -13,8 +13,7 @@
 // segments (the best tokens of the others are behind M better ones already): a threshold t that at least
 // M segment maxima reach, by bisection over the maxima in registers; the tokens of those segments above t, and
 // at t the first M; their order by counting the better ones of each.
-// Launch 3, a workgroup per request: of its beams' lists the M best by c. The M-th best of a sample
-// of the lists' heads bounds what can be among them, then again by counting.
+// Launch 3, a workgroup per request: of its beams' lists the M best by c, many candidates again by a threshold first.
 // Sums of a wave's tiles, S, its logarithm and every c are in 64 bits: the order of two beams' candidates is decided
 // by differences far below a float's step at the score's size.
 #include "tb_common.h"
@@ -23,11 +22,13 @@ namespace tb {
 
 constexpr int SELECT_TILE = 512;                   // tokens: 8 a lane
 constexpr int SELECT_WAVES = 4;                    // of a workgroup of launch 1
+constexpr int SELECT_AHEAD = 8;                    // bytes of a lane's tokens' width that it loads ahead: 2 tiles of fp32, 4 of 16 bits
 constexpr int SELECT_SEGMENTS = 1024;              // of a row, at most
 constexpr int SELECT_THREADS = 512;                // of launch 2
 constexpr int SELECT_LIST = 1536, SELECT_EQUALS = 512;   // tokens above t and at t that launch 2 keeps in LDS
 constexpr int MERGE_THREADS = 1024;
-constexpr int MERGE_LIST = 4352;                   // what a sample's bound leaves of 64 lists of 128 at most
+constexpr int MERGE_DIRECT = 512;                  // candidates that are ranked as they are
+constexpr int MERGE_LIST = 512;                    // else at most M + M / 2 + 8 of them
 constexpr float SELECT_MOST = 3.402823466e38f;
 
 struct select_args {
@@ -71,69 +72,116 @@ __device__ __forceinline__ eight_logits<T> select_load(const char* row, int t0, 
   return e;
 }
 
-// Maximum over aligned groups of 2^n lanes.
-__device__ __forceinline__ float lanes_max(float x, int n) {
-  if (n >= 1) x = fmaxf(x, dpp<DPP_QUAD_XOR1>(x));
-  if (n >= 2) x = fmaxf(x, dpp<DPP_QUAD_XOR2>(x));
-  if (n >= 3) x = fmaxf(x, dpp<DPP_ROW_HALF_MIRROR>(x));
-  if (n >= 4) x = fmaxf(x, dpp<DPP_ROW_MIRROR>(x));
-  if (n >= 5) x = max_xor16(x);
-  if (n >= 6) x = max_xor32(x);
+// Maximum over aligned groups of 2^N lanes, of numbers and infinities.
+template <int CTRL>
+__device__ __forceinline__ float max_dpp(float x) {   // (every lane has a partner: the move folds into the maximum)
+  return max_f32(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true)));
+}
+template <int N>
+__device__ __forceinline__ float lanes_max(float x) {
+  if constexpr (N >= 1) x = max_dpp<DPP_QUAD_XOR1>(x);
+  if constexpr (N >= 2) x = max_dpp<DPP_QUAD_XOR2>(x);
+  if constexpr (N >= 3) x = max_dpp<DPP_ROW_HALF_MIRROR>(x);
+  if constexpr (N >= 4) x = max_dpp<DPP_ROW_MIRROR>(x);
+  if constexpr (N >= 5) x = max_xor16(x);
+  if constexpr (N >= 6) x = max_xor32(x);
   return x;
 }
 
-// e^d for d <= 8, by the exponential of the rounded product d log2(e) and a first-order term for what the
-// rounding (and the constant's) took; -inf and NaN give 0. Off by the hardware's exponential, a step.
+// e^d for d <= 8: the exponential of the rounded product y = d log2(e), and a first-order term for what y, rounded,
+// is off by, d - y ln 2 (with an ln 2 that is itself 2^-28 off); -inf and NaN give 0.
 __device__ __forceinline__ float select_exp(float d) {
-  constexpr float HI = 1.44269502162933349609375f, LO = 1.925963033500011e-8f, LN2 = 0.693147180559945f;
   d = fmaxf(d, -150.f);
-  const float y = d * HI, e = fast_exp2(y);
-  const float rest = fmaf(d, LO, fmaf(d, HI, -y));
-  return fmaf(e, rest * LN2, e);
+  const float y = d * 1.44269504088896f, e = fast_exp2(y);
+  return fmaf(e, fmaf(-y, 0.693147180559945f, d), e);
 }
 
-template <typename T>
+// Sum over the wave's lanes, in every lane.
+__device__ __forceinline__ double lanes_sum(double x) {
+  auto move = [](double v, auto&& f) {
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    return __longlong_as_double((int64_t)((uint64_t)f((uint32_t)(b >> 32)) << 32 | f((uint32_t)b)));
+  };
+  x += move(x, [](uint32_t w) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, DPP_QUAD_XOR1, 0xf, 0xf, false); });
+  x += move(x, [](uint32_t w) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, DPP_QUAD_XOR2, 0xf, 0xf, false); });
+  x += move(x, [](uint32_t w) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, DPP_ROW_HALF_MIRROR, 0xf, 0xf, false); });
+  x += move(x, [](uint32_t w) { return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)w, DPP_ROW_MIRROR, 0xf, 0xf, false); });
+  const int lane = threadIdx.x & 63;
+  x += move(x, [&](uint32_t w) {
+    const auto r = __builtin_amdgcn_permlane16_swap(w, w, false, false);
+    return lane & 16 ? (uint32_t)r[0] : (uint32_t)r[1];
+  });
+  x += move(x, [&](uint32_t w) {
+    const auto r = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+    return lane & 32 ? (uint32_t)r[0] : (uint32_t)r[1];
+  });
+  return x;
+}
+
+template <typename T, int LANES>                   // 2^LANES lanes of a segment
 __global__ __launch_bounds__(64 * SELECT_WAVES) void select_scan_kernel(const select_args a) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
   const int run = blockIdx.x * SELECT_WAVES + wave, row = blockIdx.y;
   if (run >= a.runs || !select_open(a, row)) return;
   const char* const at = a.logits + (int64_t)row * a.row_bytes;
-  const int first = run * a.per_run, last = min(first + a.per_run, a.tiles);
+  const int first = run * a.per_run, last = min(first + a.per_run, a.tiles), whole = min(last, a.vocab / SELECT_TILE);
+  constexpr int PER = 64 >> LANES;
+  const bool tells = (lane & ((1 << LANES) - 1)) == 0;
   float* const tops = a.seg_max + (int64_t)row * a.tops;
-  float ref = -SELECT_MOST;
+  float ref = -SELECT_MOST, limit = -SELECT_MOST;   // limit: ref + 8
   double sum = 0.;
-  eight_logits<T> next = select_load<T>(at, first * SELECT_TILE + 8 * lane, a.vocab);
-  for (int t = first; t < last; ++t) {
-    const eight_logits<T> now = next;
-    if (t + 1 < last) next = select_load<T>(at, (t + 1) * SELECT_TILE + 8 * lane, a.vocab);
+  auto add = [&](int t, const eight_logits<T>& e) {
     float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (float)now.v[i];
+    for (int i = 0; i < 8; ++i) x[i] = (float)e.v[i];
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);   // (a NaN loses against a number)
-    if (__any(!(top <= ref + 8.f))) {
+    if (__any(!(top <= limit))) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = select_logit(x[i]);
       top = select_logit(top);
-      if (top > ref + 8.f) {
+      if (top > limit) {
         sum *= exp((double)ref - (double)top);
         ref = top;
+        limit = top + 8.f;
       }
     }
-    float part = 0.f;
+    float part[2] = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) part += select_exp(x[i] - ref);
-    sum += (double)part;
-    top = lanes_max(top, a.log2_lanes);
-    const int seg = (t << (6 - a.log2_lanes)) + (lane >> a.log2_lanes);
-    if ((lane & ((1 << a.log2_lanes) - 1)) == 0 && seg < a.tops) tops[seg] = top;
+    for (int i = 0; i < 8; ++i) part[i & 1] += select_exp(x[i] - ref);
+    sum += (double)(part[0] + part[1]);
+    top = lanes_max<LANES>(top);
+    if (tells && t * PER + (lane >> LANES) < a.tops) tops[t * PER + (lane >> LANES)] = top;
+  };
+  // whole tiles, B loaded while the B before are added up; the row's last, partial one by itself
+  constexpr int B = SELECT_AHEAD / sizeof(T);
+  struct __attribute__((packed, aligned(sizeof(T)))) raw_t {
+    uint32_t w[2 * sizeof(T)];
+  };
+  raw_t next[B];
+  const uint32_t mine = 8 * lane * sizeof(T);
+  auto fetch = [&](int t) {
+#pragma unroll
+    for (int u = 0; u < B; ++u) {                  // (past the run: its last tile again)
+      const char* const tile = at + (int64_t)min(t + u, whole - 1) * (int64_t)(SELECT_TILE * sizeof(T));
+      next[u] = *reinterpret_cast<const raw_t*>(tile + mine);
+    }
+  };
+  if (first < whole) fetch(first);
+  for (int t0 = first; t0 < whole; t0 += B) {
+    raw_t now[B];
+#pragma unroll
+    for (int u = 0; u < B; ++u) now[u] = next[u];
+    if (t0 + B < whole) fetch(t0 + B);
+#pragma unroll
+    for (int u = 0; u < B; ++u)
+      if (t0 + u < whole) add(t0 + u, __builtin_bit_cast(eight_logits<T>, now[u]));
   }
+  if (whole < last) add(whole, select_load<T>(at, whole * SELECT_TILE + 8 * lane, a.vocab));
   // the lanes' sums against the largest reference
-  const float r = lanes_max(ref, 6);
-  sum *= exp((double)ref - (double)r);
-#pragma unroll
-  for (int o = 1; o < 64; o *= 2) sum += __shfl_xor(sum, o);
+  const float r = lanes_max<6>(ref);
+  sum = lanes_sum(sum * exp((double)ref - (double)r));
   if (lane == 0) a.sums[(int64_t)row * a.runs + run] = make_double2(sum, (double)r);
 }
 
@@ -219,23 +267,23 @@ __global__ __launch_bounds__(SELECT_THREADS) void select_rows_kernel(const selec
   if (tid == 0) above = equals = 0;
   __syncthreads();
   uint32_t v[WORDS];                               // every wave: all segments, lane l those of l + 64 i
-  float m = -INFINITY, least = INFINITY, mine = -INFINITY;
+  float m = -INFINITY, mine = -INFINITY, mine2 = -INFINITY;   // a lane's best and second best
 #pragma unroll
   for (int i = 0; i < WORDS; ++i) {
     const float x = tops[64 * i + lane];
+    mine2 = fmaxf(mine2, fminf(mine, x));
     mine = fmaxf(mine, x);
     v[i] = select_order(x);
   }
-  m = lanes_max(mine, 6);
-  least = -lanes_max(-mine, 6);                    // 64 segments at least reach it
+  m = lanes_max<6>(mine);
+  const float least = -lanes_max<6>(M <= 64 ? -mine : -mine2);   // 64, or 128, segments at least reach it
   if (wave == 0) {                                 // m and log S
     double s = 0.;
     for (int r = lane; r < a.runs; r += 64) {
       const double2 x = a.sums[(int64_t)row * a.runs + r];
       s += x.x * (m == -INFINITY ? 0. : exp(x.y - (double)m));
     }
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) s += __shfl_xor(s, o);
+    s = lanes_sum(s);
     if (lane == 0) a.norms[row] = make_double2((double)m, log(s));
   }
   // ---- the threshold ----
@@ -248,7 +296,7 @@ __global__ __launch_bounds__(SELECT_THREADS) void select_rows_kernel(const selec
   uint32_t lo = ORDER_NONE, hi = select_order(m) + 1;
   bool exact = true;
   if (reach(ORDER_NONE + 1) >= M) {                // else everything above -inf
-    lo = M <= 64 && least > -INFINITY ? select_order(least) : ORDER_NONE + 1;
+    lo = least > -INFINITY ? select_order(least) : ORDER_NONE + 1;
     while (hi - lo > 1) {
       const uint32_t mid = lo + (hi - lo) / 2;
       const int c = reach(mid);
@@ -384,6 +432,7 @@ __global__ __launch_bounds__(SELECT_THREADS) void select_rows_kernel(const selec
   for (int i0 = tid / share; i0 < all; i0 += SELECT_THREADS / share) {
     const uint64_t e = entry(i0);
     int c = 0;
+#pragma unroll 8
     for (int j = tid % share; j < all; j += share) c += entry(j) > e;
     if (c) atomicAdd(&ranks[i0], c);
   }
@@ -409,53 +458,115 @@ __device__ __forceinline__ void merge_ranks(const cand* cands, int n, int* ranks
   for (int i = threadIdx.x / share; i < n; i += MERGE_THREADS / share) {
     const cand e = cands[i];
     int c = 0;
+#pragma unroll 8
     for (int j = threadIdx.x % share; j < n; j += share) c += better(cands[j], e);
     if (c) atomicAdd(&ranks[i], c);
   }
 }
 
+// A double's place among all doubles.
+__device__ __forceinline__ uint64_t merge_order(double x) {
+  const uint64_t b = (uint64_t)__double_as_longlong(x + 0.);
+  return b >> 63 ? ~b : b | (uint64_t)1 << 63;
+}
+constexpr uint64_t MERGE_NONE = 0x000FFFFFFFFFFFFFull;   // of -inf
+
 __global__ __launch_bounds__(MERGE_THREADS) void select_merge_kernel(const select_args a) {
+  constexpr int EACH = TB_BEAMS_MAX * TB_BEAM_CANDIDATES_MAX / MERGE_THREADS, WAVES = MERGE_THREADS / 64;
   __shared__ cand cands[MERGE_LIST];
   __shared__ int ranks[MERGE_LIST];
-  __shared__ cand bound;
+  __shared__ int waves[2][WAVES];
+  __shared__ uint64_t tops[WAVES];
   __shared__ int held;
-  const int tid = threadIdx.x, M = a.picks, K = a.beams, row0 = blockIdx.x * K;
-  auto look = [&](int k, int p) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, M = a.picks, K = a.beams, row0 = blockIdx.x * K, all = K * M;
+  auto look = [&](int i) {                         // candidate i of the lists, one beam's behind the other's
+    const int k = i / M, p = i - k * M;
     const float2 e = a.lists[(int64_t)(row0 + k) * M + p];
-    cand x = {-INFINITY, INT64_MAX};
+    cand x = {-INFINITY, (int64_t)k << 32 | p};
     if (e.x > -INFINITY) {
       const double2 n = a.norms[row0 + k];
       x.c = (double)a.scores[row0 + k] + (((double)e.x - n.x) - n.y);
-      x.at = (int64_t)k << 32 | p;
     }
     return x;
   };
-  // the heads of the lists, twice as many as asked for
-  const int depth = min(M, (2 * M + K - 1) / K), sample = K * depth;
-  if (tid == 0) held = 0, bound = cand{-INFINITY, INT64_MAX};
-  for (int i = tid; i < sample; i += MERGE_THREADS) cands[i] = look(i / depth, i % depth), ranks[i] = 0;
-  __syncthreads();
-  merge_ranks(cands, sample, ranks);
-  __syncthreads();
-  int n = sample;
-  if (depth < M) {
-    // what is better than the M-th best of the sample, or is it
-    for (int i = tid; i < sample; i += MERGE_THREADS)
-      if (ranks[i] == M - 1 && cands[i].c > -INFINITY) bound = cands[i];
+  if (tid == 0) held = 0;
+  int n;
+  if (all <= MERGE_DIRECT) {
+    if (tid < all) cands[tid] = look(tid), ranks[tid] = 0;
+    n = all;
+  } else {
+    uint64_t v[EACH], top = MERGE_NONE;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      v[i] = MERGE_NONE;
+      if (i * MERGE_THREADS + tid < all) v[i] = merge_order(look(i * MERGE_THREADS + tid).c);
+      top = max(top, v[i]);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) top = max(top, (uint64_t)__shfl_xor((unsigned long long)top, o));
+    if (lane == 0) tops[wave] = top;
     __syncthreads();
-    const cand least = bound;
-    for (int i = tid; i < K * M; i += MERGE_THREADS) {
-      const cand x = look(i / M, i % M);
-      if (x.c > -INFINITY && !better(least, x)) {
-        const int at = atomicAdd(&held, 1);
-        if (at < MERGE_LIST) cands[at] = x, ranks[at] = 0;
+    for (int w = 0; w < WAVES; ++w) top = max(top, tops[w]);
+    int turn = 0;
+    auto reach = [&](uint64_t o) {
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i)
+        if (i * MERGE_THREADS < all) c += __popcll(__ballot(v[i] >= o));
+      if (lane == 0) waves[turn & 1][wave] = c;
+      __syncthreads();
+      c = 0;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) c += waves[turn & 1][w];
+      ++turn;
+      return c;
+    };
+    uint64_t lo = MERGE_NONE, hi = top + 1;
+    bool exact = true;
+    if (reach(MERGE_NONE + 1) > M) {
+      lo = MERGE_NONE + 1;
+      while (hi - lo > 1) {
+        const uint64_t mid = lo + (hi - lo) / 2;
+        const int c = reach(mid);
+        if (c >= M) {
+          lo = mid;
+          if (c <= M + M / 2 + 8) {
+            exact = false;
+            break;
+          }
+        } else {
+          hi = mid;
+        }
       }
     }
+    // those above it, and those at it: all where they are few, else the first ones in order
+    int need = lo == MERGE_NONE ? 0 : exact ? M - reach(lo + 1) : all;
     __syncthreads();
-    n = min(held, MERGE_LIST);
-    merge_ranks(cands, n, ranks);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      if (i * MERGE_THREADS >= all) continue;
+      const bool eq = v[i] == lo;
+      const uint64_t mask = __ballot(eq);
+      if (lane == 0) waves[i & 1][wave] = __popcll(mask);
+      __syncthreads();
+      int before = 0, here = 0;
+#pragma unroll
+      for (int w = 0; w < WAVES; ++w) {
+        if (w < wave) before += waves[i & 1][w];
+        here += waves[i & 1][w];
+      }
+      if (v[i] > lo || (eq && before + __popcll(mask & (((uint64_t)1 << lane) - 1)) < need)) {
+        const int at = atomicAdd(&held, 1);        // at most M + M / 2 + 8
+        cands[at] = look(i * MERGE_THREADS + tid), ranks[at] = 0;
+      }
+      need -= here;
+    }
     __syncthreads();
+    n = held;
   }
+  __syncthreads();
+  merge_ranks(cands, n, ranks);
+  __syncthreads();
   const int64_t at = (int64_t)blockIdx.x * M;
   if (tid == 0) held = 0;
   __syncthreads();
@@ -498,10 +609,17 @@ struct select_sizes {
   }
 };
 
+template <typename T, int LANES>
+static void launch_scan(const select_args& a, hipStream_t stream) {
+  if constexpr (LANES < 6)
+    if (a.log2_lanes > LANES) return launch_scan<T, LANES + 1>(a, stream);
+  const dim3 grid((a.runs + SELECT_WAVES - 1) / SELECT_WAVES, a.rows);
+  hipLaunchKernelGGL((select_scan_kernel<T, LANES>), grid, dim3(64 * SELECT_WAVES), 0, stream, a);
+}
+
 template <typename T>
 static void launch_select(const select_args& a, hipStream_t stream) {
-  const dim3 grid((a.runs + SELECT_WAVES - 1) / SELECT_WAVES, a.rows);
-  hipLaunchKernelGGL(select_scan_kernel<T>, grid, dim3(64 * SELECT_WAVES), 0, stream, a);
+  launch_scan<T, 0>(a, stream);
   hipLaunchKernelGGL(select_rows_kernel<T>, dim3(a.rows), dim3(SELECT_THREADS), 0, stream, a);
   hipLaunchKernelGGL(select_merge_kernel, dim3(a.rows / a.beams), dim3(MERGE_THREADS), 0, stream, a);
 }
