@@ -856,7 +856,8 @@ int32_t tb_device_step(int32_t* block_tables, int32_t max_blocks_per_row, const 
  * candidate (k, end_token) with c = s, and its logits are not read; nor are those of a beam whose score is -inf
  * or NaN, which has none. A logit that is NaN counts as -inf, +inf as the largest fp32 number. Decided in 64 bits from
  * sums of fp32 exponentials. logits fp32 / fp16 / bf16, row stride in elements, aligned to their
- * elements; vocab <= 2^30, num_rows <= 65535; workspace: tb_beam_select_workspace_bytes, 16-byte aligned. */
+ * elements; vocab <= 2^30, num_rows <= 65535; workspace: tb_beam_select_workspace_bytes, 16-byte aligned; calls
+ * that may overlap in time need their own. */
 size_t tb_beam_select_workspace_bytes(int32_t num_rows, int32_t vocab, int32_t num_candidates);
 int32_t tb_beam_select(const void* logits, int64_t row_stride, int32_t vocab, int32_t dtype,
                        const float* scores, const uint8_t* finished, int32_t end_token, int32_t num_rows,

@@ -287,6 +287,46 @@ def test_select_long_rows_of_small_terms():
     check_select(x, torch.zeros(1, 2), 3)
 
 
+def replayed(run, outputs, between=lambda: None, inputs=()):
+    """The outputs of `run` captured into a graph and replayed three times, other work between the replays; before each one
+    the inputs' copies are what they were."""
+    keep = [x.clone() for x in inputs]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        run()                                      # what is allocated once is allocated
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        held = run()
+    got = []
+    for _ in range(3):
+        for x, y in zip(inputs, keep):
+            x.copy_(y)
+        between()
+        graph.replay()
+        torch.cuda.synchronize()
+        got.append([x.clone() for x in outputs(held)])
+        torch.randn(1 << 16, device=DEV).sum().item()
+    for x, y in zip(inputs, keep):
+        x.copy_(y)
+    return got
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("G,K,V,M", [(3, 4, 32001, 8), (1, 48, 5000, 96), (5, 2, 300, 4)])
+def test_select_captured(G, K, V, M, dtype):
+    """Captured and replayed beside eager calls: the same values, to the bit."""
+    g = torch.Generator().manual_seed(V)
+    logits = (torch.randn(G * K, V, generator=g) * 3).to(dtype).to(DEV)
+    scores = (torch.randn(G, K, generator=g) - 5).to(DEV)
+    finished = (torch.rand(G, K, generator=g) < 0.3).to(DEV)
+    call = lambda: select_beams(logits, scores, num_candidates=M, finished=finished, end_token=3)
+    want = call()
+    for got in replayed(call, list, between=call):
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+
+
 # ---- reordering ---------------------------------------------------------------------
 def random_parents(g, groups, K):
     return [int(min(K - 1, K * g.random() ** 1.5)) if g.random() < 0.95 else -1 for _ in range(groups * K)]

@@ -6,14 +6,14 @@
 // largest are told; among equals the smaller beam's first, within a beam the larger logit (which c, rounded, may
 // no longer show), then the smaller token.
 //
-// Launch 1 reads the logits once: a wave walks a run of tiles of 512 tokens (8 a lane), writes the maxima of
+// Three launches. Part 1 reads the logits once: a wave walks a run of tiles of 512 tokens (8 a lane), writes the maxima of
 // segments of the row (8 to 512 tokens, so that a row has at most 1024) and adds up e^(x - r) against a reference r per
 // lane that moves only when a logit outgrows it by 8.
-// Launch 2, a workgroup per beam: its M best tokens by (x, v), which need no sum. They lie in its M best
+// Part 2, a workgroup per beam: its M best tokens by (x, v), which need no sum. They lie in its M best
 // segments (the best tokens of the others are behind M better ones already): a threshold t that at least
 // M segment maxima reach, by bisection over the maxima in registers; the tokens of those segments above t, and
 // at t the first M; their order by counting the better ones of each.
-// Launch 3, a workgroup per request: of its beams' lists the M best by c, many candidates again by a threshold first.
+// Part 3, a workgroup per request: of its beams' lists the M best by c, many candidates again by a threshold first.
 // Sums of a wave's tiles, S, its logarithm and every c are in 64 bits: the order of two beams' candidates is decided
 // by differences far below a float's step at the score's size.
 #include "tb_common.h"
@@ -21,14 +21,12 @@
 namespace tb {
 
 constexpr int SELECT_TILE = 512;                   // tokens: 8 a lane
-constexpr int SELECT_WAVES = 4;                    // of a workgroup of launch 1
 constexpr int SELECT_AHEAD = 8;                    // bytes of a lane's tokens' width that it loads ahead: 2 tiles of fp32, 4 of 16 bits
 constexpr int SELECT_SEGMENTS = 1024;              // of a row, at most
-constexpr int SELECT_THREADS = 512;                // of launch 2
-constexpr int SELECT_LIST = 1536, SELECT_EQUALS = 512;   // tokens above t and at t that launch 2 keeps in LDS
-constexpr int MERGE_THREADS = 1024;
-constexpr int MERGE_DIRECT = 512;                  // candidates that are ranked as they are
-constexpr int MERGE_LIST = 512;                    // else at most M + M / 2 + 8 of them
+constexpr int SELECT_THREADS = 512;
+constexpr int SELECT_LIST = 2048;                  // tokens from the threshold up that part 2 keeps in LDS
+constexpr int MERGE_LIST = 512;                    // candidates that are ranked as they are; of more M + M / 2 + 8 at most
+static_assert(MERGE_LIST >= SELECT_THREADS, "a list for a workgroup's candidates");
 constexpr float SELECT_MOST = 3.402823466e38f;
 
 struct select_args {
@@ -44,7 +42,7 @@ struct select_args {
   int64_t* out_tokens;
   int32_t tiles, runs, per_run;   // tiles of a row, runs of a row, tiles of a run
   int32_t log2_lanes;          // lanes of a segment inside a tile: 2^log2_lanes
-  int32_t tops;                // segment maxima that launch 1 writes per row
+  int32_t tops;                // segment maxima that part 1 writes per row
   int32_t join, segments;      // of them in a segment (1 unless a segment is several tiles), segments of a row
   float* seg_max;              // [rows][tops]
   double2* sums;               // [rows][runs]: {S, r}
@@ -118,11 +116,9 @@ __device__ __forceinline__ double lanes_sum(double x) {
   return x;
 }
 
+// One wave's run of a row whose logits count.
 template <typename T, int LANES>                   // 2^LANES lanes of a segment
-__global__ __launch_bounds__(64 * SELECT_WAVES) void select_scan_kernel(const select_args a) {
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-  const int run = blockIdx.x * SELECT_WAVES + wave, row = blockIdx.y;
-  if (run >= a.runs || !select_open(a, row)) return;
+__device__ __forceinline__ void select_run(const select_args& a, int row, int run, int lane) {
   const char* const at = a.logits + (int64_t)row * a.row_bytes;
   const int first = run * a.per_run, last = min(first + a.per_run, a.tiles), whole = min(last, a.vocab / SELECT_TILE);
   constexpr int PER = 64 >> LANES;
@@ -195,36 +191,38 @@ __device__ __forceinline__ float select_value(uint32_t o) {
 }
 constexpr uint32_t ORDER_NONE = 0x007FFFFFu;       // of -inf
 
-// Launch 2. Tokens are looked at 512 at a time and wave: 64 >> log2_lanes segments side by side, or one of several tiles.
-template <typename T>
-struct select_row {
-  const select_args& a;
-  const char* at;
-  const int* picked;           // LDS, rising segments
-  int n, lane, wave;
-  // each(piece, token, x): a lane's 8 tokens of a picked segment
-  template <typename F>
-  __device__ __forceinline__ void pieces(F&& each) const {
-    const int per = 64 >> a.log2_lanes, spot = lane >> a.log2_lanes;
-    for (int p0 = wave * per; p0 < n; p0 += SELECT_THREADS / 64 * per) {
-      const int p = p0 + spot;
-      for (int j = 0; j < a.join; ++j) {
-        int t0 = a.vocab;
-        if (p < n) t0 = (((picked[p] * a.join + j) << a.log2_lanes) + (lane & ((1 << a.log2_lanes) - 1))) * 8;
-        float x[8];
-        if (t0 < a.vocab) {
-          const eight_logits<T> e = select_load<T>(at, t0, a.vocab);
+// Part 2. Tokens are looked at 512 at a time and wave: 64 >> log2_lanes segments side by side, or one of several tiles.
+// each(place of the segment in `picked`, first token, x): a lane's 8 tokens, -inf where there are none.
+template <typename T, typename F>
+__device__ __forceinline__ void select_pieces(const select_args& a, const char* at, const int* picked, int n, int lane,
+                                              int wave, F&& each) {
+  constexpr int AHEAD = 4, WAVES = SELECT_THREADS / 64;
+  const int per = 64 >> a.log2_lanes, spot = lane >> a.log2_lanes, mine = lane & ((1 << a.log2_lanes) - 1);
+  const int rounds = (n + WAVES * per - 1) / (WAVES * per) * a.join;   // of all waves
+  for (int r0 = 0; r0 < rounds; r0 += AHEAD) {
+    eight_logits<T> e[AHEAD];
+    int p[AHEAD], t0[AHEAD];
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = select_logit((float)e.v[i]);
-        } else {
+    for (int u = 0; u < AHEAD; ++u) {              // (past the end: the last round's again)
+      const int r = min(r0 + u, rounds - 1), turn = r / a.join, j = r - turn * a.join;
+      p[u] = (turn * WAVES + wave) * per + spot;
+      t0[u] = p[u] < n ? (((picked[p[u]] * a.join + j) << a.log2_lanes) + mine) * 8 : a.vocab;
+      if (a.vocab >= 8)                            // 8 tokens inside the row: the last ones moved up
+        e[u] = *reinterpret_cast<const eight_logits<T>*>(at + (int64_t)min(t0[u], a.vocab - 8) * sizeof(T));
+      else
+        e[u] = select_load<T>(at, 0, a.vocab);
+    }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = -INFINITY;
-        }
-        each(p, t0, x);
-      }
+    for (int u = 0; u < AHEAD; ++u) {
+      if (r0 + u >= rounds) break;
+      const int from = max(0, min(t0[u], a.vocab - 8));
+      float x[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = from + i < t0[u] ? -INFINITY : select_logit((float)e[u].v[i]);
+      each(p[u], from, x);
     }
   }
-};
+}
 
 // Exclusive running sum of a wave's lanes, and its total.
 __device__ __forceinline__ int select_scan(int x, int lane, int& total) {
@@ -238,18 +236,29 @@ __device__ __forceinline__ int select_scan(int x, int lane, int& total) {
   return up - x;
 }
 
+struct rows_lds {
+  static constexpr int MOST = TB_BEAM_CANDIDATES_MAX + TB_BEAM_CANDIDATES_MAX / 2 + 8;
+  uint64_t list[SELECT_LIST];                      // {order of x, ~token}
+  int ranks[SELECT_LIST];
+  float tops[SELECT_SEGMENTS];
+  int picked[MOST], equal_of[MOST];
+  int chosen, listed, counted;
+};
+
+// A row's list, by a workgroup of SELECT_THREADS.
 template <typename T>
-__global__ __launch_bounds__(SELECT_THREADS) void select_rows_kernel(const select_args a) {
+__device__ void select_list(const select_args& a, rows_lds& s, int row) {
   constexpr int WAVES = SELECT_THREADS / 64, WORDS = SELECT_SEGMENTS / 64;
-  constexpr int MOST = TB_BEAM_CANDIDATES_MAX + TB_BEAM_CANDIDATES_MAX / 2 + 8;
-  __shared__ float tops[SELECT_SEGMENTS];
-  __shared__ int picked[MOST];
-  __shared__ uint64_t list[SELECT_LIST + SELECT_EQUALS];   // {order of x, ~token}
-  __shared__ int ranks[SELECT_LIST + SELECT_EQUALS];
-  __shared__ int equal_of[MOST];
-  __shared__ int above, equals, counted;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, row = blockIdx.x, M = a.picks;
+  uint64_t* const list = s.list;
+  int *const ranks = s.ranks, *const picked = s.picked, *const equal_of = s.equal_of;
+  float* const tops = s.tops;
+  int &chosen = s.chosen, &listed = s.listed, &counted = s.counted;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), M = a.picks;
   float2* const out = a.lists + (int64_t)row * M;
+  float first[SELECT_SEGMENTS / SELECT_THREADS];   // (of a row whose logits do not count: whatever is there)
+#pragma unroll
+  for (int i = 0; i < SELECT_SEGMENTS / SELECT_THREADS; ++i)
+    first[i] = a.seg_max[(int64_t)row * a.tops + min((i * SELECT_THREADS + tid) * a.join, a.tops - 1)];
   if (!select_open(a, row)) {                      // one candidate, the score itself, or none
     const bool one = a.finished && a.finished[row] && a.scores[row] > -INFINITY;
     for (int i = tid; i < M; i += SELECT_THREADS)
@@ -257,14 +266,15 @@ __global__ __launch_bounds__(SELECT_THREADS) void select_rows_kernel(const selec
     if (tid == 0) a.norms[row] = make_double2(0., 0.);
     return;
   }
-  for (int i = tid; i < SELECT_SEGMENTS; i += SELECT_THREADS) {
-    float x = -INFINITY;
-    if (i < a.segments)
-      for (int j = 0; j < a.join && i * a.join + j < a.tops; ++j)
-        x = fmaxf(x, select_logit(a.seg_max[(int64_t)row * a.tops + i * a.join + j]));
-    tops[i] = x;
+#pragma unroll
+  for (int i = 0; i < SELECT_SEGMENTS / SELECT_THREADS; ++i) {
+    const int seg = i * SELECT_THREADS + tid;
+    float x = seg < a.segments ? select_logit(first[i]) : -INFINITY;
+    for (int k = 1; k < a.join && seg * a.join + k < a.tops; ++k)
+      x = fmaxf(x, select_logit(a.seg_max[(int64_t)row * a.tops + seg * a.join + k]));
+    tops[seg] = x;
   }
-  if (tid == 0) above = equals = 0;
+  if (tid == 0) chosen = listed = 0;
   __syncthreads();
   uint32_t v[WORDS];                               // every wave: all segments, lane l those of l + 64 i
   float m = -INFINITY, mine = -INFINITY, mine2 = -INFINITY;   // a lane's best and second best
@@ -277,14 +287,14 @@ __global__ __launch_bounds__(SELECT_THREADS) void select_rows_kernel(const selec
   }
   m = lanes_max<6>(mine);
   const float least = -lanes_max<6>(M <= 64 ? -mine : -mine2);   // 64, or 128, segments at least reach it
-  if (wave == 0) {                                 // m and log S
-    double s = 0.;
+  if (wave == WAVES - 1) {                         // m and log S
+    double sum = 0.;
     for (int r = lane; r < a.runs; r += 64) {
       const double2 x = a.sums[(int64_t)row * a.runs + r];
-      s += x.x * (m == -INFINITY ? 0. : exp(x.y - (double)m));
+      sum += x.x * (m == -INFINITY ? 0. : exp(x.y - (double)m));
     }
-    s = lanes_sum(s);
-    if (lane == 0) a.norms[row] = make_double2((double)m, log(s));
+    sum = log(lanes_sum(sum));
+    if (lane == 0) a.norms[row] = make_double2((double)m, sum);
   }
   // ---- the threshold ----
   auto reach = [&](uint32_t o) {
@@ -311,12 +321,10 @@ __global__ __launch_bounds__(SELECT_THREADS) void select_rows_kernel(const selec
       }
     }
   }
-  // ---- the segments that reach it: rising, at most M where several equal it ----
-  int n = 0;
-  {
-    int over = reach(lo + 1), eq0 = 0;
-    const int need = lo == ORDER_NONE ? 0 : exact ? M - over : SELECT_SEGMENTS;
+  // ---- the segments that reach it; where several equal it and not all are wanted, the first ones ----
+  auto rising = [&](int need) {                    // in order; how many
     const uint64_t below = ((uint64_t)1 << lane) - 1;
+    int n = 0, eq0 = 0;
 #pragma unroll
     for (int i = 0; i < WORDS; ++i) {
       const uint64_t eq = __ballot(v[i] == lo);
@@ -326,35 +334,45 @@ __global__ __launch_bounds__(SELECT_THREADS) void select_rows_kernel(const selec
       eq0 += __popcll(eq);
       n += __popcll(took);
     }
-  }
-  __syncthreads();
-  const select_row<T> part{a, a.logits + (int64_t)row * a.row_bytes, picked, n, lane, wave};
-  // ---- the tokens above the threshold, and those at it ----
-  auto push = [&](uint32_t t, bool keep) {
-    part.pieces([&](int, int t0, const float(&x)[8]) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t o = select_order(x[i]);
-        if (o > t) {
-          const int at = atomicAdd(&above, 1);
-          if (at < SELECT_LIST && keep) list[at] = (uint64_t)o << 32 | (uint32_t) ~(t0 + i);
-        } else if (o == t && o != ORDER_NONE) {
-          const int at = atomicAdd(&equals, 1);
-          if (at < SELECT_EQUALS && keep) list[SELECT_LIST + at] = (uint64_t)o << 32 | (uint32_t) ~(t0 + i);
-        }
-      }
-    });
     __syncthreads();
+    return n;
   };
-  push(lo, true);
-  if (above > SELECT_LIST) {                       // many tokens above it (whole ranges of high ones): the M-th best token
+  const int want_equal = lo == ORDER_NONE ? 0 : exact ? M - reach(lo + 1) : SELECT_SEGMENTS;
+  int n;
+  if (want_equal == SELECT_SEGMENTS || lo == ORDER_NONE) {
+    for (int i = tid; i < SELECT_SEGMENTS; i += SELECT_THREADS) {
+      const uint32_t o = select_order(tops[i]);
+      if (o > lo || (o == lo && want_equal)) picked[atomicAdd(&chosen, 1)] = i;
+    }
+    __syncthreads();
+    n = chosen;
+  } else {
+    n = rising(want_equal);
+  }
+  const char* const at = a.logits + (int64_t)row * a.row_bytes;
+  // ---- the tokens from the threshold up ----
+  select_pieces<T>(a, at, picked, n, lane, wave, [&](int, int t, const float(&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t o = select_order(x[i]);
+      if (o >= lo && o != ORDER_NONE) {
+        const int place = atomicAdd(&listed, 1);
+        if (place < SELECT_LIST) list[place] = (uint64_t)o << 32 | (uint32_t) ~(t + i);
+      }
+    }
+  });
+  __syncthreads();
+  int all = listed;
+  if (all > SELECT_LIST) {
+    // many of them (whole ranges of high or equal tokens): the M-th best token's value, what is above it, and as many
+    // of its equals as are wanted, in order
     uint32_t t0 = lo, t1 = select_order(m) + 1;    // t0 is reached by M tokens, t1 by none
     while (t1 - t0 > 1) {
       const uint32_t mid = t0 + (t1 - t0) / 2;
       __syncthreads();
       if (tid == 0) counted = 0;
       __syncthreads();
-      part.pieces([&](int, int, const float(&x)[8]) {
+      select_pieces<T>(a, at, picked, n, lane, wave, [&](int, int, const float(&x)[8]) {
         int c = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) c += select_order(x[i]) >= mid;
@@ -364,21 +382,18 @@ __global__ __launch_bounds__(SELECT_THREADS) void select_rows_kernel(const selec
       if (counted >= M) t0 = mid;
       else t1 = mid;
     }
-    lo = t0;
-    __syncthreads();
-    if (tid == 0) above = equals = 0;
-    __syncthreads();
-    push(lo, true);
-  }
-  int count_above = above, count_equal = equals;
-  if (count_equal > SELECT_EQUALS) {               // the first M of them: numbered segment by segment
-    const int want = M - min(count_above, M);
+    n = rising(want_equal);                        // (segments are numbered below: in order)
     for (int i = tid; i < n; i += SELECT_THREADS) equal_of[i] = 0;
+    if (tid == 0) listed = 0;
     __syncthreads();
-    part.pieces([&](int p, int, const float(&x)[8]) {
+    select_pieces<T>(a, at, picked, n, lane, wave, [&](int p, int t, const float(&x)[8]) {
       int c = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) c += select_order(x[i]) == lo;
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t o = select_order(x[i]);
+        c += o == t0;
+        if (o > t0) list[atomicAdd(&listed, 1)] = (uint64_t)o << 32 | (uint32_t) ~(t + i);   // (fewer than M)
+      }
       if (c) atomicAdd(&equal_of[p], c);
     });
     __syncthreads();
@@ -393,36 +408,33 @@ __global__ __launch_bounds__(SELECT_THREADS) void select_rows_kernel(const selec
       }
     }
     __syncthreads();
-    // one wave after the other within a segment's tiles: a segment's tokens are one wave's, in order
-    const int width = 1 << a.log2_lanes;
-    int seen = 0, of = -1;                         // (segments of several tiles: equals of the tiles before)
-    part.pieces([&](int p, int t0, const float(&x)[8]) {
+    const int over = listed, want = M - over, width = 1 << a.log2_lanes;
+    int seen = 0, of = -1;                         // (segments of several tiles, one wave's: equals of the tiles before)
+    select_pieces<T>(a, at, picked, n, lane, wave, [&](int p, int t, const float(&x)[8]) {
       int c = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) c += select_order(x[i]) == lo;
+      for (int i = 0; i < 8; ++i) c += select_order(x[i]) == t0;
       int up = c;
       for (int o = 1; o < width; o *= 2) {
         const int y = __shfl_up(up, o);
         if ((lane & (width - 1)) >= o) up += y;
       }
-      const int all = __shfl(up, (lane & ~(width - 1)) + width - 1);
+      const int here = __shfl(up, (lane & ~(width - 1)) + width - 1);
       if (p != of) of = p, seen = 0;
       if (p < n) {
-        int at = equal_of[p] + seen + up - c;
+        int place = equal_of[p] + seen + up - c;
         for (int i = 0; i < 8; ++i)
-          if (select_order(x[i]) == lo) {
-            if (at < want) list[SELECT_LIST + at] = (uint64_t)lo << 32 | (uint32_t) ~(t0 + i);
-            ++at;
+          if (select_order(x[i]) == t0) {
+            if (place < want) list[over + place] = (uint64_t)t0 << 32 | (uint32_t) ~(t + i);
+            ++place;
           }
       }
-      seen += all;
+      seen += here;
     });
-    count_equal = want;
     __syncthreads();
+    all = M;
   }
   // ---- their order: how many are better ----
-  const int all = count_above + count_equal;
-  auto entry = [&](int i) { return list[i < count_above ? i : SELECT_LIST + i - count_above]; };
   for (int i = tid; i < all; i += SELECT_THREADS) ranks[i] = 0;
   for (int i = tid; i < M; i += SELECT_THREADS)
     if (i >= all) out[i] = make_float2(-INFINITY, 0.f);
@@ -430,39 +442,35 @@ __global__ __launch_bounds__(SELECT_THREADS) void select_rows_kernel(const selec
   int share = 1;                                   // threads that count for one entry
   while (share < 64 && 2 * share * all <= SELECT_THREADS) share *= 2;
   for (int i0 = tid / share; i0 < all; i0 += SELECT_THREADS / share) {
-    const uint64_t e = entry(i0);
+    const uint64_t e = list[i0];
     int c = 0;
 #pragma unroll 8
-    for (int j = tid % share; j < all; j += share) c += entry(j) > e;
+    for (int j = tid % share; j < all; j += share) c += list[j] > e;
     if (c) atomicAdd(&ranks[i0], c);
   }
   __syncthreads();
   for (int i = tid; i < all; i += SELECT_THREADS)
     if (ranks[i] < M) {
-      const uint64_t e = entry(i);
+      const uint64_t e = list[i];
       out[ranks[i]] = make_float2(select_value((uint32_t)(e >> 32)), __uint_as_float(~(uint32_t)e));
     }
 }
 
-// Launch 3: a candidate and its place in the order: larger value, then smaller beam, then the beam's own order.
+// Part 3: a candidate and its place in the order: larger value, then smaller beam, then the beam's own order.
 struct cand {
   double c;
   int64_t at;
 };
 __device__ __forceinline__ bool better(const cand& x, const cand& y) { return x.c > y.c || (x.c == y.c && x.at < y.at); }
 
-// How many of cands[0 .. n) are better than each, in ranks (zero before, a barrier before and behind).
-__device__ __forceinline__ void merge_ranks(const cand* cands, int n, int* ranks) {
-  int share = 1;
-  while (share < 64 && 2 * share * n <= MERGE_THREADS) share *= 2;
-  for (int i = threadIdx.x / share; i < n; i += MERGE_THREADS / share) {
-    const cand e = cands[i];
-    int c = 0;
-#pragma unroll 8
-    for (int j = threadIdx.x % share; j < n; j += share) c += better(cands[j], e);
-    if (c) atomicAdd(&ranks[i], c);
-  }
-}
+struct merge_lds {
+  double norms[TB_BEAMS_MAX][3];                   // m, log S, the score
+  cand cands[MERGE_LIST];
+  int ranks[MERGE_LIST];
+  int waves[2][SELECT_THREADS / 64];
+  uint64_t tops[SELECT_THREADS / 64], leasts[SELECT_THREADS / 64];
+  int held;
+};
 
 // A double's place among all doubles.
 __device__ __forceinline__ uint64_t merge_order(double x) {
@@ -470,49 +478,61 @@ __device__ __forceinline__ uint64_t merge_order(double x) {
   return b >> 63 ? ~b : b | (uint64_t)1 << 63;
 }
 constexpr uint64_t MERGE_NONE = 0x000FFFFFFFFFFFFFull;   // of -inf
+__device__ __forceinline__ uint64_t merge_xor(uint64_t x, int o) {
+  return (uint64_t)__shfl_xor((unsigned long long)x, o);
+}
 
-__global__ __launch_bounds__(MERGE_THREADS) void select_merge_kernel(const select_args a) {
-  constexpr int EACH = TB_BEAMS_MAX * TB_BEAM_CANDIDATES_MAX / MERGE_THREADS, WAVES = MERGE_THREADS / 64;
-  __shared__ cand cands[MERGE_LIST];
-  __shared__ int ranks[MERGE_LIST];
-  __shared__ int waves[2][WAVES];
-  __shared__ uint64_t tops[WAVES];
-  __shared__ int held;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, M = a.picks, K = a.beams, row0 = blockIdx.x * K, all = K * M;
-  auto look = [&](int i) {                         // candidate i of the lists, one beam's behind the other's
-    const int k = i / M, p = i - k * M;
-    const float2 e = a.lists[(int64_t)(row0 + k) * M + p];
-    cand x = {-INFINITY, (int64_t)k << 32 | p};
-    if (e.x > -INFINITY) {
-      const double2 n = a.norms[row0 + k];
-      x.c = (double)a.scores[row0 + k] + (((double)e.x - n.x) - n.y);
-    }
+// A request's candidates from its beams' lists, by a workgroup of SELECT_THREADS.
+__device__ void select_merge(const select_args& a, merge_lds& s, int request) {
+  constexpr int EACH = TB_BEAMS_MAX * TB_BEAM_CANDIDATES_MAX / SELECT_THREADS, WAVES = SELECT_THREADS / 64;
+  cand* const cands = s.cands;
+  int *const ranks = s.ranks, &held = s.held;
+  int(*const waves)[SELECT_THREADS / 64] = s.waves;
+  uint64_t *const tops = s.tops, *const leasts = s.leasts;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int M = a.picks, K = a.beams, row0 = request * K, all = K * M;
+  double(*const norms)[3] = s.norms;
+  const float2* const lists = a.lists + (int64_t)row0 * M;
+  auto entry = [&](int i) { return lists[min(i, all - 1)]; };   // one beam's behind the other's
+  auto look = [&](int i, float2 e) {               // candidate i
+    const int k = i / M;
+    cand x = {-INFINITY, (int64_t)k << 32 | (i - k * M)};
+    if (i < all && e.x > -INFINITY) x.c = norms[k][2] + (((double)e.x - norms[k][0]) - norms[k][1]);
     return x;
   };
+  float2 mine[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i)
+    if (i * SELECT_THREADS < all) mine[i] = entry(i * SELECT_THREADS + tid);
+  for (int i = tid; i < 2 * K; i += SELECT_THREADS) norms[i >> 1][i & 1] = (&a.norms[row0].x)[i];
+  for (int i = tid; i < K; i += SELECT_THREADS) norms[i][2] = (double)a.scores[row0 + i];
+  __syncthreads();
   if (tid == 0) held = 0;
   int n;
-  if (all <= MERGE_DIRECT) {
-    if (tid < all) cands[tid] = look(tid), ranks[tid] = 0;
+  if (all <= SELECT_THREADS) {
+    if (tid < all) cands[tid] = look(tid, mine[0]), ranks[tid] = 0;
     n = all;
   } else {
     uint64_t v[EACH], top = MERGE_NONE;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
       v[i] = MERGE_NONE;
-      if (i * MERGE_THREADS + tid < all) v[i] = merge_order(look(i * MERGE_THREADS + tid).c);
+      if (i * SELECT_THREADS < all) v[i] = merge_order(look(i * SELECT_THREADS + tid, mine[i]).c);
       top = max(top, v[i]);
     }
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) top = max(top, (uint64_t)__shfl_xor((unsigned long long)top, o));
-    if (lane == 0) tops[wave] = top;
+    // the best of every 4 threads: the least of these, which 128 candidates reach, and the largest
+    for (int o = 1; o < 4; o *= 2) top = max(top, merge_xor(top, o));
+    uint64_t least = top;
+    for (int o = 4; o < 64; o *= 2) top = max(top, merge_xor(top, o)), least = min(least, merge_xor(least, o));
+    if (lane == 0) tops[wave] = top, leasts[wave] = least;
     __syncthreads();
-    for (int w = 0; w < WAVES; ++w) top = max(top, tops[w]);
+    for (int w = 0; w < WAVES; ++w) top = max(top, tops[w]), least = min(least, leasts[w]);
     int turn = 0;
     auto reach = [&](uint64_t o) {
       int c = 0;
 #pragma unroll
       for (int i = 0; i < EACH; ++i)
-        if (i * MERGE_THREADS < all) c += __popcll(__ballot(v[i] >= o));
+        if (i * SELECT_THREADS < all) c += __popcll(__ballot(v[i] >= o));
       if (lane == 0) waves[turn & 1][wave] = c;
       __syncthreads();
       c = 0;
@@ -523,8 +543,8 @@ __global__ __launch_bounds__(MERGE_THREADS) void select_merge_kernel(const selec
     };
     uint64_t lo = MERGE_NONE, hi = top + 1;
     bool exact = true;
-    if (reach(MERGE_NONE + 1) > M) {
-      lo = MERGE_NONE + 1;
+    if (least > MERGE_NONE || reach(MERGE_NONE + 1) > M) {
+      lo = max(least, MERGE_NONE + 1);
       while (hi - lo > 1) {
         const uint64_t mid = lo + (hi - lo) / 2;
         const int c = reach(mid);
@@ -540,52 +560,86 @@ __global__ __launch_bounds__(MERGE_THREADS) void select_merge_kernel(const selec
       }
     }
     // those above it, and those at it: all where they are few, else the first ones in order
-    int need = lo == MERGE_NONE ? 0 : exact ? M - reach(lo + 1) : all;
-    __syncthreads();
+    auto keep = [&](int i) {
+      const int at = atomicAdd(&held, 1);          // at most M + M / 2 + 8
+      cands[at] = look(i * SELECT_THREADS + tid, mine[i]), ranks[at] = 0;
+    };
+    if (!exact || lo == MERGE_NONE) {
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-      if (i * MERGE_THREADS >= all) continue;
-      const bool eq = v[i] == lo;
-      const uint64_t mask = __ballot(eq);
-      if (lane == 0) waves[i & 1][wave] = __popcll(mask);
+      for (int i = 0; i < EACH; ++i)
+        if (i * SELECT_THREADS < all && v[i] >= max(lo, MERGE_NONE + 1)) keep(i);
+    } else {
+      int need = M - reach(lo + 1);
       __syncthreads();
-      int before = 0, here = 0;
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) {
-        if (w < wave) before += waves[i & 1][w];
-        here += waves[i & 1][w];
+      for (int i = 0; i < EACH; ++i) {
+        if (i * SELECT_THREADS >= all) continue;
+        const bool eq = v[i] == lo;
+        const uint64_t mask = __ballot(eq);
+        if (lane == 0) waves[i & 1][wave] = __popcll(mask);
+        __syncthreads();
+        int before = 0, here = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w) {
+          if (w < wave) before += waves[i & 1][w];
+          here += waves[i & 1][w];
+        }
+        if (v[i] > lo || (eq && before + __popcll(mask & (((uint64_t)1 << lane) - 1)) < need)) keep(i);
+        need -= here;
       }
-      if (v[i] > lo || (eq && before + __popcll(mask & (((uint64_t)1 << lane) - 1)) < need)) {
-        const int at = atomicAdd(&held, 1);        // at most M + M / 2 + 8
-        cands[at] = look(i * MERGE_THREADS + tid), ranks[at] = 0;
-      }
-      need -= here;
     }
     __syncthreads();
     n = held;
   }
   __syncthreads();
-  merge_ranks(cands, n, ranks);
-  __syncthreads();
-  const int64_t at = (int64_t)blockIdx.x * M;
   if (tid == 0) held = 0;
+  {
+    int share = 1;                                 // threads that count for one candidate
+    while (share < 64 && 2 * share * n <= SELECT_THREADS) share *= 2;
+    for (int i = tid / share; i < n; i += SELECT_THREADS / share) {
+      const cand e = cands[i];
+      int c = 0;
+#pragma unroll 8
+      for (int j = tid % share; j < n; j += share) c += better(cands[j], e);
+      if (c) atomicAdd(&ranks[i], c);
+    }
+  }
   __syncthreads();
-  for (int i = tid; i < n; i += MERGE_THREADS) {
+  const int64_t at = (int64_t)request * M;
+  for (int i = tid; i < n; i += SELECT_THREADS) {
     const cand x = cands[i];
     if (x.c == -INFINITY) continue;
     atomicAdd(&held, 1);
     if (ranks[i] >= M) continue;
-    a.out_scores[at + ranks[i]] = (float)x.c;
     const int k = (int)(x.at >> 32);
+    const float2 e = lists[k * M + (int)(uint32_t)x.at];
+    a.out_scores[at + ranks[i]] = (float)x.c;
     a.out_parents[at + ranks[i]] = k;
-    a.out_tokens[at + ranks[i]] = __float_as_int(a.lists[(int64_t)(row0 + k) * M + (uint32_t)x.at].y);
+    a.out_tokens[at + ranks[i]] = __float_as_int(e.y);
   }
   __syncthreads();
-  for (int i = held + tid; i < M; i += MERGE_THREADS) {
+  for (int i = held + tid; i < M; i += SELECT_THREADS) {
     a.out_scores[at + i] = -INFINITY;
     a.out_parents[at + i] = -1;
     a.out_tokens[at + i] = -1;
   }
+}
+
+template <typename T, int LANES>
+__global__ __launch_bounds__(256) void select_scan_kernel(const select_args a) {
+  const int run = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+  if (run < a.runs && select_open(a, blockIdx.y)) select_run<T, LANES>(a, blockIdx.y, run, threadIdx.x & 63);
+}
+
+template <typename T>
+__global__ __launch_bounds__(SELECT_THREADS) void select_rows_kernel(const select_args a) {
+  __shared__ rows_lds lds;
+  select_list<T>(a, lds, blockIdx.x);
+}
+
+__global__ __launch_bounds__(SELECT_THREADS) void select_merge_kernel(const select_args a) {
+  __shared__ merge_lds lds;
+  select_merge(a, lds, blockIdx.x);
 }
 
 struct select_sizes {
@@ -610,18 +664,13 @@ struct select_sizes {
 };
 
 template <typename T, int LANES>
-static void launch_scan(const select_args& a, hipStream_t stream) {
-  if constexpr (LANES < 6)
-    if (a.log2_lanes > LANES) return launch_scan<T, LANES + 1>(a, stream);
-  const dim3 grid((a.runs + SELECT_WAVES - 1) / SELECT_WAVES, a.rows);
-  hipLaunchKernelGGL((select_scan_kernel<T, LANES>), grid, dim3(64 * SELECT_WAVES), 0, stream, a);
-}
-
-template <typename T>
 static void launch_select(const select_args& a, hipStream_t stream) {
-  launch_scan<T, 0>(a, stream);
-  hipLaunchKernelGGL(select_rows_kernel<T>, dim3(a.rows), dim3(SELECT_THREADS), 0, stream, a);
-  hipLaunchKernelGGL(select_merge_kernel, dim3(a.rows / a.beams), dim3(MERGE_THREADS), 0, stream, a);
+  if constexpr (LANES < 6)
+    if (a.log2_lanes > LANES) return launch_select<T, LANES + 1>(a, stream);
+  const dim3 block(SELECT_THREADS);
+  hipLaunchKernelGGL((select_scan_kernel<T, LANES>), dim3((a.runs + 3) / 4, a.rows), dim3(256), 0, stream, a);
+  hipLaunchKernelGGL(select_rows_kernel<T>, dim3(a.rows), block, 0, stream, a);
+  hipLaunchKernelGGL(select_merge_kernel, dim3(a.rows / a.beams), block, 0, stream, a);
 }
 
 }  // namespace tb
@@ -655,8 +704,8 @@ extern "C" int32_t tb_beam_select(const void* logits, int64_t row_stride, int32_
   char* const ws = (char*)workspace;
   a.sums = (double2*)ws, a.norms = (double2*)(ws + z.norms), a.lists = (float2*)(ws + z.lists);
   a.seg_max = (float*)(ws + z.maxima);
-  if (dtype == TB_DTYPE_F32) launch_select<float>(a, stream);
-  else if (dtype == TB_DTYPE_F16) launch_select<_Float16>(a, stream);
-  else launch_select<__bf16>(a, stream);
+  if (dtype == TB_DTYPE_F32) launch_select<float, 0>(a, stream);
+  else if (dtype == TB_DTYPE_F16) launch_select<_Float16, 0>(a, stream);
+  else launch_select<__bf16, 0>(a, stream);
   TB_RETURN_LAUNCH_STATUS();
 }
