@@ -7,8 +7,8 @@
 // no longer show), then the smaller token.
 //
 // Three launches. Part 1 reads the logits once: a wave walks a run of tiles of 512 tokens (8 a lane), writes the maxima of
-// segments of the row (8 to 512 tokens, so that a row has at most 1024) and adds up e^(x - r) against a reference r per
-// lane that moves only when a logit outgrows it by 8.
+// segments of the row (8 to 512 tokens, so that a row has at most 1024) and adds up e^(x - r) against a reference r of
+// the wave.
 // Part 2, a workgroup per beam: its M best tokens by (x, v), which need no sum. They lie in its M best
 // segments (the best tokens of the others are behind M better ones already): a threshold t that at least
 // M segment maxima reach, by bisection over the maxima in registers; the tokens of those segments above t, and
@@ -21,7 +21,7 @@
 namespace tb {
 
 constexpr int SELECT_TILE = 512;                   // tokens: 8 a lane
-constexpr int SELECT_AHEAD = 8;                    // bytes of a lane's tokens' width that it loads ahead: 2 tiles of fp32, 4 of 16 bits
+constexpr int SELECT_AHEAD = 4;                    // tiles that a wave loads ahead, times the bytes of a token
 constexpr int SELECT_SEGMENTS = 1024;              // of a row, at most
 constexpr int SELECT_THREADS = 512;
 constexpr int SELECT_LIST = 2048;                  // tokens from the threshold up that part 2 keeps in LDS
@@ -86,14 +86,6 @@ __device__ __forceinline__ float lanes_max(float x) {
   return x;
 }
 
-// e^d for d <= 8: the exponential of the rounded product y = d log2(e), and a first-order term for what y, rounded,
-// is off by, d - y ln 2 (with an ln 2 that is itself 2^-28 off); -inf and NaN give 0.
-__device__ __forceinline__ float select_exp(float d) {
-  d = fmaxf(d, -150.f);
-  const float y = d * 1.44269504088896f, e = fast_exp2(y);
-  return fmaf(e, fmaf(-y, 0.693147180559945f, d), e);
-}
-
 // Sum over the wave's lanes, in every lane.
 __device__ __forceinline__ double lanes_sum(double x) {
   auto move = [](double v, auto&& f) {
@@ -124,7 +116,8 @@ __device__ __forceinline__ void select_run(const select_args& a, int row, int ru
   constexpr int PER = 64 >> LANES;
   const bool tells = (lane & ((1 << LANES) - 1)) == 0;
   float* const tops = a.seg_max + (int64_t)row * a.tops;
-  float ref = -SELECT_MOST, limit = -SELECT_MOST;   // limit: ref + 8
+  // the wave's reference, moved where a logit outgrows it by 1
+  float ref = 0.f, limit = -INFINITY;              // limit: ref + 1, -inf before there is one
   double sum = 0.;
   auto add = [&](int t, const eight_logits<T>& e) {
     float x[8];
@@ -133,20 +126,27 @@ __device__ __forceinline__ void select_run(const select_args& a, int row, int ru
     float top = x[0];
 #pragma unroll
     for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);   // (a NaN loses against a number)
-    if (__any(!(top <= limit))) {
+    auto terms = [&] {
+      float part[2] = {0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < 8; ++i) part[i & 1] += fast_exp2((x[i] - ref) * 1.44269504088896f);
+      return part[0] + part[1];
+    };
+    float part = 0.f;
+    if (!__any(!(top <= limit))) part = terms();
+    if (__any(!(top <= limit) || part != part)) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = select_logit(x[i]);
       top = select_logit(top);
-      if (top > limit) {
-        sum *= exp((double)ref - (double)top);
-        ref = top;
-        limit = top + 8.f;
+      const float r = lanes_max<6>(top);
+      if (r > limit) {
+        if (limit > -INFINITY) sum *= exp((double)ref - (double)r);
+        ref = r;
+        limit = r + 1.f;
       }
+      part = limit > -INFINITY ? terms() : 0.f;
     }
-    float part[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) part[i & 1] += select_exp(x[i] - ref);
-    sum += (double)(part[0] + part[1]);
+    sum += (double)part;
     top = lanes_max<LANES>(top);
     if (tells && t * PER + (lane >> LANES) < a.tops) tops[t * PER + (lane >> LANES)] = top;
   };
@@ -175,10 +175,8 @@ __device__ __forceinline__ void select_run(const select_args& a, int row, int ru
       if (t0 + u < whole) add(t0 + u, __builtin_bit_cast(eight_logits<T>, now[u]));
   }
   if (whole < last) add(whole, select_load<T>(at, whole * SELECT_TILE + 8 * lane, a.vocab));
-  // the lanes' sums against the largest reference
-  const float r = lanes_max<6>(ref);
-  sum = lanes_sum(sum * exp((double)ref - (double)r));
-  if (lane == 0) a.sums[(int64_t)row * a.runs + run] = make_double2(sum, (double)r);
+  sum = lanes_sum(sum);
+  if (lane == 0) a.sums[(int64_t)row * a.runs + run] = make_double2(sum, (double)ref);
 }
 
 // A float's place among all floats, -inf 0x007FFFFF; -0 is 0.
@@ -196,7 +194,7 @@ constexpr uint32_t ORDER_NONE = 0x007FFFFFu;       // of -inf
 template <typename T, typename F>
 __device__ __forceinline__ void select_pieces(const select_args& a, const char* at, const int* picked, int n, int lane,
                                               int wave, F&& each) {
-  constexpr int AHEAD = 4, WAVES = SELECT_THREADS / 64;
+  constexpr int AHEAD = 1, WAVES = SELECT_THREADS / 64;
   const int per = 64 >> a.log2_lanes, spot = lane >> a.log2_lanes, mine = lane & ((1 << a.log2_lanes) - 1);
   const int rounds = (n + WAVES * per - 1) / (WAVES * per) * a.join;   // of all waves
   for (int r0 = 0; r0 < rounds; r0 += AHEAD) {
@@ -647,8 +645,8 @@ struct select_sizes {
   size_t norms, lists, maxima, all;                // of the workspace; the sums first
   select_sizes(int64_t rows, int64_t vocab, int64_t picks) {
     tiles = (int32_t)((vocab + SELECT_TILE - 1) / SELECT_TILE);
-    // as many runs as give every CU some 32 waves
-    const int64_t want = (8192 + rows - 1) / rows;
+    // runs that fill the GPU twice
+    const int64_t want = (16384 + rows - 1) / rows;
     per_run = (int32_t)((tiles + want - 1) / want);
     runs = (tiles + per_run - 1) / per_run;
     log2_lanes = 0;

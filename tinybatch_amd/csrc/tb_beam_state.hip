@@ -10,10 +10,10 @@
 //
 // Launches: 1. one workgroup: who copies, the fresh blocks (running sum over the rows), the new lengths;
 // 2. a workgroup per request and 128 columns of its tables: the new tables, what the reference counts change by,
-// the blocks that were let go of; beside them the copies; 3. one workgroup: of those blocks the ones that nobody
-// holds, each once, in the order (request, column, row) of the old tables, behind the free blocks. Every order is fixed:
-// the same state gives the same tables. Fresh blocks are taken before any is freed, so that a copy's
-// source is never its own destination. Where something does not fit nothing is changed.
+// the blocks that were let go of; beside them the copies; the last of the former puts those of these blocks that nobody
+// holds, each once, in the order (request, column, row) of the old tables, behind the free blocks. Every order is
+// fixed: the same state gives the same tables. Fresh blocks are taken before any is freed, so that a copy's source
+// is never its own destination. Where something does not fit nothing is changed.
 #include "tb_common.h"
 
 namespace tb {
@@ -39,9 +39,10 @@ struct reorder_args {
   const int32_t* parents;      // [rows]
   uint32_t* status;
   // workspace
-  int32_t* head;               // {0 or 1: nothing is done, copies}
+  int32_t* head;               // {0 or 1: nothing is done, copies, workgroups that have listed their blocks}
   int4* plan;                  // [rows]: {source row or -1, new length, fresh block or -1, old length}
   int4* copies;                // [rows]: {source block, fresh block, positions, 0}
+  int32_t* least;              // [requests]: whole blocks of every live row
   int32_t* gone_count;         // [requests * chunks]
   int32_t* gone;               // [requests * chunks][128 beams]
   int32_t chunks;
@@ -76,70 +77,76 @@ __device__ __forceinline__ int group_scan(int x, int (*waves)[THREADS / 64], int
 
 __global__ __launch_bounds__(1024) void reorder_plan_kernel(const reorder_args a) {
   __shared__ int waves[2][16];
+  __shared__ int lens[1024], parents[1024], fresh[1024];
   __shared__ uint32_t faults;
-  const int bs = 1 << a.log2_bs, K = a.beams;
-  if (threadIdx.x == 0) faults = 0;
-  __syncthreads();
+  const int bs = 1 << a.log2_bs, K = a.beams, tid = threadIdx.x, each = 1024 / K * K;   // rows of whole requests
+  const int have = a.num_free_in[0];
+  if (tid == 0) faults = 0, a.head[2] = 0;
   int base = 0, turn = 0;
-  for (int i0 = 0; i0 < a.rows; i0 += 1024, ++turn) {
-    const int i = i0 + threadIdx.x;
+  for (int i0 = 0; i0 < a.rows; i0 += each, ++turn) {
+    const int i = i0 + tid;
+    const bool mine = tid < each && i < a.rows;
+    const int p = mine ? a.parents[i] : -1, old = mine ? a.lens_in[i] : 0;
+    __syncthreads();                               // (the round before has been read)
+    lens[tid] = old;
+    parents[tid] = p;
+    {                                              // free block number base + tid of the step
+      const int at = have - 1 - base - tid, id = a.free_blocks[min(max(at, 0), a.num_blocks - 1)];
+      fresh[tid] = id < 0 || id >= a.num_blocks ? 0 : id;
+    }
+    __syncthreads();
+    uint32_t bad = old < 0 || (old + bs - 1) >> a.log2_bs > a.max_nb ? TB_TABLES_BAD_LENGTH : 0;
     bool copy = false;
-    int src = -1, ctx = 0, open = -1, old = 0;
-    if (i < a.rows) {
-      const int g0 = i / K * K, p = a.parents[i];
-      old = a.lens_in[i];
-      if (p < -1 || p >= K) {
-        atomicOr(&faults, TB_TABLES_BAD_PARENT);
-      } else if (p >= 0) {
-        ctx = a.lens_in[g0 + p];
-        if (ctx < 0 || (ctx + bs - 1) >> a.log2_bs > a.max_nb) {
-          atomicOr(&faults, TB_TABLES_BAD_LENGTH);
-          ctx = 0;
-        }
-        if (ctx > 0) src = g0 + p;
-        if (ctx & (bs - 1)) {
-          open = a.tables[(int64_t)src * a.max_nb + (ctx >> a.log2_bs)];
+    int src = -1, ctx = 0, open = -1;
+    if (mine && (p < -1 || p >= K)) bad |= TB_TABLES_BAD_PARENT;
+    else if (p >= 0) {
+      const int g0 = tid / K * K;
+      ctx = lens[g0 + p];
+      if (ctx < 0 || (ctx + bs - 1) >> a.log2_bs > a.max_nb) ctx = 0;   // (its own row says so)
+      if (ctx > 0) src = i0 + g0 + p;
+      if (ctx & (bs - 1)) {
+        open = a.tables[(int64_t)src * a.max_nb + (ctx >> a.log2_bs)];
+        if (open < 0 || open >= a.num_blocks) {
+          bad |= TB_TABLES_BAD_LENGTH;
+        } else {
+          const int held = a.refs[open];
           bool first = true;
-          for (int k = g0; k < i; ++k) first &= a.parents[k] != p;
-          if (open < 0 || open >= a.num_blocks) atomicOr(&faults, TB_TABLES_BAD_LENGTH);
-          else copy = !(first && a.refs[open] == 1);
+          for (int k = g0; k < tid; ++k) first &= parents[k] != p;
+          copy = !(first && held == 1);
         }
       }
-      if (old < 0 || (old + bs - 1) >> a.log2_bs > a.max_nb) atomicOr(&faults, TB_TABLES_BAD_LENGTH);
     }
+    if (bad) atomicOr(&faults, bad);
     int total;
-    const int place = base + group_scan<1024>(copy, waves, turn, total);
-    base += total;
-    if (i < a.rows) {
-      a.plan[i] = make_int4(src, ctx, copy ? place : -1, old);
-      if (copy) a.copies[place] = make_int4(open, 0, ctx & (bs - 1), i);
+    const int at = group_scan<1024>(copy, waves, turn, total);
+    if (mine) {
+      a.plan[i] = make_int4(src, ctx, copy ? fresh[at] : -1, old);
+      if (copy) a.copies[base + at] = make_int4(open, fresh[at], ctx & (bs - 1), i);
     }
+    // the whole blocks that every live row of a request has: an upper bound of those they share
+    __syncthreads();
+    lens[tid] = ctx;
+    __syncthreads();
+    if (tid < each / K && i0 + tid * K < a.rows) {
+      int least = INT32_MAX;
+      for (int k = 0; k < K; ++k) {
+        const int len = lens[tid * K + k];
+        if (len > 0) least = min(least, len >> a.log2_bs);
+      }
+      a.least[i0 / K + tid] = least == INT32_MAX ? 0 : least;
+    }
+    base += total;
   }
   __syncthreads();
-  const int have = a.num_free_in[0];
   const uint32_t bad = faults | (base > have ? TB_TABLES_OUT_OF_BLOCKS : 0);
-  if (threadIdx.x == 0) {
+  if (tid == 0) {
     a.head[0] = bad != 0;
     a.head[1] = base;
     if (bad) atomicOr(a.status, bad);
   }
   if (bad) return;
-  for (int i = threadIdx.x; i < base; i += 1024) {   // (the row's place was written by another thread: behind the barrier)
-    const int at = have - 1 - i, id = a.free_blocks[min(at, a.num_blocks - 1)];
-    const int block = id < 0 || id >= a.num_blocks ? 0 : id;
-    a.copies[i].y = block;
-    a.plan[a.copies[i].w].z = block;
-    a.refs[block] = 1;
-  }
-  // the whole blocks that every live row of a request has: an upper bound of those they share
-  for (int g = threadIdx.x; g < a.rows / K; g += 1024) {
-    int least = INT32_MAX;
-    for (int k = 0; k < K; ++k) {
-      const int len = a.plan[g * K + k].y;
-      if (len > 0) least = min(least, len >> a.log2_bs);
-    }
-    a.shared[g] = least == INT32_MAX ? 0 : least;
-  }
+  for (int i = tid; i < base; i += 1024) a.refs[a.copies[i].y] = 1;
+  for (int g = tid; g < a.rows / K; g += 1024) a.shared[g] = a.least[g];
 }
 
 // The positions of an open block, all layers, K and V of every head: runs of n * row_bytes bytes.
@@ -157,8 +164,73 @@ __device__ __forceinline__ void reorder_copy(const reorder_args& a, int unit, in
   }
 }
 
+// The blocks of the lists that nobody holds, each once, behind the free blocks. An entry whose change made the
+// count 0 has CLOSED set; where another one's count is 0 too its block was held by several requests, or by rows of one with
+// another block between, which have let go of it at once: the first of its entries counts, not the one that closed it.
+constexpr int32_t CLOSED = INT32_MIN;
+__device__ void reorder_free(const reorder_args& a, int lists) {
+  constexpr int N = REORDER_COLUMNS;
+  __shared__ int waves[2][N / 64], starts[N + 1], several;
+  const int tid = threadIdx.x;
+  const int left = a.num_free_in[0] - a.head[1];
+  auto load = [](const int32_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+  int freed = 0, turn = 0;
+  // each(number of the entry, entry): of all entries in order, N at a time; a barrier within
+  auto entries = [&](auto&& each) {
+    int before = 0;                                // entries of the lists done
+    for (int l0 = 0; l0 < lists; l0 += N) {
+      const int mine = l0 + tid < lists ? load(&a.gone_count[l0 + tid]) : 0;
+      int total;
+      __syncthreads();                             // starts has been read
+      starts[tid] = group_scan<N>(mine, waves, turn++, total);
+      __syncthreads();
+      for (int x0 = 0; x0 < total; x0 += N) {
+        const int x = x0 + tid;
+        int32_t e = -1;
+        if (x < total) {
+          int lo = 0, hi = N;
+          while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (starts[mid] <= x) lo = mid;
+            else hi = mid;
+          }
+          e = load(&a.gone[(int64_t)(l0 + lo) * REORDER_COLUMNS * a.beams + x - starts[lo]]);
+        }
+        each(x < total, before + x, e);
+      }
+      before += total;
+    }
+  };
+  auto push = [&](bool win, int32_t id) {
+    int won;
+    const int at = left + freed + group_scan<N>(win, waves, turn++, won);
+    freed += won;
+    if (win && at < a.num_blocks) a.free_blocks[at] = id;
+  };
+  if (tid == 0) several = 0;
+  entries([&](bool there, int, int32_t e) {
+    if (there && e >= 0 && load(&a.refs[e]) == 0) several = 1;
+  });
+  __syncthreads();
+  if (!several) {
+    entries([&](bool there, int, int32_t e) { push(there && e < 0, e & ~CLOSED); });
+  } else {
+    entries([&](bool there, int x, int32_t e) {    // the first entry of a block marks it
+      if (there && load(&a.refs[e & ~CLOSED]) <= 0) atomicMin(&a.refs[e & ~CLOSED], x - MARK);
+    });
+    __threadfence();
+    __syncthreads();
+    entries([&](bool there, int x, int32_t e) {
+      const bool win = there && load(&a.refs[e & ~CLOSED]) == x - MARK;
+      push(win, e & ~CLOSED);
+      if (win) __hip_atomic_store(&a.refs[e & ~CLOSED], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    });
+  }
+  if (tid == 0) a.num_free_out[0] = left + freed;
+}
+
 __global__ __launch_bounds__(REORDER_COLUMNS) void reorder_tables_kernel(const reorder_args a, int table_groups) {
-  extern __shared__ int32_t lds[];                 // old entries [beams][128], then per beam {children, keeps}
+  extern __shared__ int32_t lds[];                 // old entries [beams][128], the plan [beams][4], {children, keeps} [beams]
   if (a.head[0]) return;
   if ((int)blockIdx.x >= table_groups) {
     const int copies = a.head[1], stride = gridDim.x - table_groups;
@@ -166,58 +238,63 @@ __global__ __launch_bounds__(REORDER_COLUMNS) void reorder_tables_kernel(const r
     return;
   }
   __shared__ int waves[2][REORDER_COLUMNS / 64];
-  __shared__ int differ;
+  __shared__ int differ, arrived;
   const int K = a.beams, g = blockIdx.x / a.chunks, chunk = blockIdx.x - g * a.chunks, row0 = g * K;
   const int tid = threadIdx.x, j = REORDER_COLUMNS * chunk + tid, bs = 1 << a.log2_bs;
   int32_t* const old = lds + tid;                  // [k * 128]
-  int32_t* const kids = lds + REORDER_COLUMNS * K;
+  int4* const plan = (int4*)(lds + REORDER_COLUMNS * K);
+  int32_t* const kids = lds + (REORDER_COLUMNS + 4) * K;
   int32_t* const keeps = kids + K;
-  const int4* const plan = a.plan + row0;
-  int width = 0;                                   // columns that the request's old tables hold
-  for (int k = 0; k < K; ++k) width = max(width, (plan[k].w + bs - 1) >> a.log2_bs);
-  if (tid < K) kids[tid] = keeps[tid] = 0;
+  if (tid < K) {
+    plan[tid] = a.plan[row0 + tid];
+    kids[tid] = keeps[tid] = 0;
+  }
   if (tid == 0) differ = INT32_MAX;
-  if (chunk == 0 && tid < K) a.lens_out[row0 + tid] = plan[tid].y;
-  if (REORDER_COLUMNS * chunk >= width) {
-    if (tid == 0) a.gone_count[blockIdx.x] = 0;
-    return;
+  // (columns are loaded before the request's width is known; the tables have them all)
+  for (int k0 = 0; k0 < K; k0 += 8) {
+    int32_t e[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) e[u] = a.tables[(int64_t)(row0 + min(k0 + u, K - 1)) * a.max_nb + min(j, a.max_nb - 1)];
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (k0 + u < K) old[REORDER_COLUMNS * (k0 + u)] = e[u];
   }
   __syncthreads();
+  int width = 0;                                   // columns that the request's old tables hold
+  for (int k = 0; k < K; ++k) width = max(width, (plan[k].w + bs - 1) >> a.log2_bs);
+  if (chunk == 0 && tid < K) a.lens_out[row0 + tid] = plan[tid].y;
   if (tid < K && plan[tid].x >= 0) {
     atomicAdd(&kids[plan[tid].x - row0], 1);
     if (plan[tid].z < 0) atomicOr(&keeps[plan[tid].x - row0], 1);
   }
-  for (int k = 0; k < K; ++k) old[REORDER_COLUMNS * k] = j < width ? a.tables[(int64_t)(row0 + k) * a.max_nb + j] : -1;
   __syncthreads();
   // what every old row's hold on its block of this column becomes; rows of one block behind each other at once
-  auto change = [&](int k) {
-    const int len = plan[k].w;
-    if (j < len >> a.log2_bs) return kids[k] - 1;
-    if (j < (len + bs - 1) >> a.log2_bs) return keeps[k] - 1;   // the open block: one child keeps it, or none
-    return 0;
-  };
-  auto runs = [&](auto&& each) {                   // each(block, change) per run of rows that hold the same block
+  uint64_t lost = 0, closed = 0;                   // rows that begin such a run which lets go; whose count is 0 then
+  if (j < width) {
     for (int k = 0; k < K;) {
-      const int id = old[REORDER_COLUMNS * k];
+      const int id = old[REORDER_COLUMNS * k], from = k;
       int sum = 0;
-      for (; k < K && old[REORDER_COLUMNS * k] == id; ++k) sum += change(k);
-      if (sum && id >= 0 && id < a.num_blocks) each(id, sum);
+      for (; k < K && old[REORDER_COLUMNS * k] == id; ++k) {
+        const int len = plan[k].w;
+        if (j < len >> a.log2_bs) sum += kids[k] - 1;
+        else if (j < (len + bs - 1) >> a.log2_bs) sum += keeps[k] - 1;   // the open block: one child keeps it, or none
+      }
+      if (sum && id >= 0 && id < a.num_blocks) {
+        const int was = atomicAdd(&a.refs[id], sum);
+        if (sum < 0) lost |= (uint64_t)1 << from;
+        if (sum < 0 && was + sum == 0) closed |= (uint64_t)1 << from;
+      }
     }
-  };
-  int lost = 0;
-  if (j < width)
-    runs([&](int id, int sum) {
-      atomicAdd(&a.refs[id], sum);
-      lost += sum < 0;
-    });
+  }
   int total;
-  int at = group_scan<REORDER_COLUMNS>(lost, waves, 0, total);
+  int at = group_scan<REORDER_COLUMNS>(__popcll(lost), waves, 0, total);
   int32_t* const list = a.gone + (int64_t)blockIdx.x * REORDER_COLUMNS * K;
-  if (lost)
-    runs([&](int id, int sum) {
-      if (sum < 0) list[at++] = id;
-    });
-  if (tid == 0) a.gone_count[blockIdx.x] = total;
+  for (uint64_t left = lost; left; left &= left - 1) {
+    const int k = __ffsll((unsigned long long)left) - 1;
+    __hip_atomic_store(&list[at++], old[REORDER_COLUMNS * k] | (closed >> k & 1 ? CLOSED : 0), __ATOMIC_RELAXED,
+                       __HIP_MEMORY_SCOPE_AGENT);
+  }
+  if (tid == 0) __hip_atomic_store(&a.gone_count[blockIdx.x], total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   // the new tables, and whether the live rows agree in this column
   if (j < width) {
     int one = -1;
@@ -236,72 +313,25 @@ __global__ __launch_bounds__(REORDER_COLUMNS) void reorder_tables_kernel(const r
     }
     if (all && !same) atomicMin(&differ, j);
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the wave's list and counts are in memory
   __syncthreads();
-  if (tid == 0 && differ != INT32_MAX) atomicMin(&a.shared[g], differ);
-}
-
-// The blocks of the lists that nobody holds, each once: the first of a block's entries marks it.
-__global__ __launch_bounds__(1024) void reorder_free_kernel(const reorder_args a, int lists) {
-  __shared__ int waves[2][16];
-  __shared__ int starts[1025];
-  if (a.head[0]) return;
-  const int tid = threadIdx.x;
-  const int left = a.num_free_in[0] - a.head[1];
-  int freed = 0, turn = 0;
-  for (int pass = 0; pass < 2; ++pass) {
-    int before = 0;                                // entries of the lists done
-    for (int l0 = 0; l0 < lists; l0 += 1024) {
-      const int mine = l0 + tid < lists ? a.gone_count[l0 + tid] : 0;
-      int total;
-      starts[tid] = group_scan<1024>(mine, waves, turn++, total);
-      if (tid == 0) starts[1024] = total;
-      __syncthreads();
-      for (int x0 = 0; x0 < total; x0 += 1024) {
-        const int x = x0 + tid;
-        bool win = false;
-        int id = 0;
-        if (x < total) {
-          int lo = 0, hi = 1024;
-          while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (starts[mid] <= x) lo = mid;
-            else hi = mid;
-          }
-          id = a.gone[(int64_t)(l0 + lo) * REORDER_COLUMNS * a.beams + x - starts[lo]];
-          const int mark = before + x - MARK;
-          if (pass == 0) {
-            if (__hip_atomic_load(&a.refs[id], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) <= 0) atomicMin(&a.refs[id], mark);
-          } else {
-            win = __hip_atomic_load(&a.refs[id], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == mark;
-          }
-        }
-        if (pass == 1) {
-          int won;
-          const int at = left + freed + group_scan<1024>(win, waves, turn++, won);
-          freed += won;
-          if (win) {
-            __hip_atomic_store(&a.refs[id], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            if (at < a.num_blocks) a.free_blocks[at] = id;
-          }
-        }
-      }
-      before += total;
-      __syncthreads();                             // starts is written again
-    }
-    __threadfence();
-    __syncthreads();
+  if (tid == 0) {
+    if (differ != INT32_MAX) atomicMin(&a.shared[g], differ);
+    arrived = __hip_atomic_fetch_add(&a.head[2], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
-  if (tid == 0) a.num_free_out[0] = left + freed;
+  __syncthreads();
+  if (arrived == table_groups - 1) reorder_free(a, table_groups);
 }
 
 struct reorder_sizes {
-  int64_t plan, copies, count, gone, all, chunks;
+  int64_t plan, copies, least, count, gone, all, chunks;
   reorder_sizes(int64_t rows, int64_t beams, int64_t max_nb) {
     chunks = (max_nb + REORDER_COLUMNS - 1) / REORDER_COLUMNS;
     const int64_t lists = rows / beams * chunks;
     plan = 64;
     copies = plan + 16 * rows;
-    count = copies + 16 * rows;
+    least = copies + 16 * rows;
+    count = least + 4 * (rows / beams);
     gone = count + 4 * lists;
     all = gone + 4 * lists * REORDER_COLUMNS * beams;
   }
@@ -353,13 +383,12 @@ extern "C" int32_t tb_beam_reorder(void* storage, int32_t num_layers, int64_t la
   a.status = status;
   char* const ws = (char*)workspace;
   a.head = (int32_t*)ws, a.plan = (int4*)(ws + z.plan), a.copies = (int4*)(ws + z.copies);
-  a.gone_count = (int32_t*)(ws + z.count), a.gone = (int32_t*)(ws + z.gone), a.chunks = (int32_t)z.chunks;
+  a.least = (int32_t*)(ws + z.least), a.gone_count = (int32_t*)(ws + z.count), a.gone = (int32_t*)(ws + z.gone), a.chunks = (int32_t)z.chunks;
   const int lists = (int)(num_rows / beams * z.chunks);
   const int64_t units = (int64_t)num_rows * num_layers;
   const int movers = (int)(units < 2048 ? units : 2048);
-  const size_t lds = sizeof(int32_t) * ((size_t)REORDER_COLUMNS * beams + 2 * beams);
+  const size_t lds = sizeof(int32_t) * (REORDER_COLUMNS + 6) * (size_t)beams;
   hipLaunchKernelGGL(reorder_plan_kernel, dim3(1), dim3(1024), 0, stream, a);
   hipLaunchKernelGGL(reorder_tables_kernel, dim3(lists + movers), dim3(REORDER_COLUMNS), lds, stream, a, lists);
-  hipLaunchKernelGGL(reorder_free_kernel, dim3(1), dim3(1024), 0, stream, a, lists);
   TB_RETURN_LAUNCH_STATUS();
 }
