@@ -389,6 +389,18 @@ def test_reorder_open_block_that_someone_else_holds():
     assert after.free[-1] == 1 and after.refs[3] == 3
 
 
+@pytest.mark.parametrize("groups,K,shared", [(3, 2, 5), (40, 8, 3), (70, 8, 40), (300, 2, 2)])
+def test_reorder_many_requests_on_one_prompt(groups, K, shared):
+    """Blocks that all requests hold are let go of by all at once: in few and in many lists."""
+    tables = [list(range(shared)) + [shared + 3 * r + j for j in range(3)] for r in range(groups * K)]
+    nb = shared + 3 * groups * K + 5
+    s = oracle.State(tables, [16 * (shared + 2) + 1 + r % 16 for r in range(groups * K)], [nb - 1, nb - 2], nb, 16, K)
+    t = upload(s)
+    storage = torch.randn(1, nb, 2, 1, 16, 8, device=DEV)
+    s = check_reorder(s, [0 if r % K else -1 for r in range(groups * K)][::-1] if groups < 5 else [-1] * (groups * K), storage, t)
+    check_reorder(s, [-1] * (groups * K), storage, t)
+
+
 def test_reorder_blocks_that_several_requests_let_go_of():
     tables = [[5, 6, 7], [5, 6, 8], [5, 6, 9], [5, 10, 11]]
     s = oracle.State(tables, [48, 48, 48, 48], [0, 1], 12, 16, 2)

@@ -26,6 +26,7 @@ struct reorder_args {
   int64_t layer_bytes;
   int32_t layers, num_blocks, pairs;   // pairs = 2 Hkv
   int32_t row_bytes;           // of a position of a head
+  int32_t unit_pairs, parts;   // pairs of a copy's unit, units of a block
   int32_t log2_bs;
   int32_t* tables;             // [rows][max_nb]
   int32_t max_nb, rows, beams;
@@ -149,92 +150,153 @@ __global__ __launch_bounds__(1024) void reorder_plan_kernel(const reorder_args a
   for (int g = tid; g < a.rows / K; g += 1024) a.shared[g] = a.least[g];
 }
 
-// The positions of an open block, all layers, K and V of every head: runs of n * row_bytes bytes.
+// The positions of an open block, all layers, K and V of every head: runs of n * row_bytes bytes, `unit_pairs` of
+// them a unit. Every thread has its loads under way before its first store.
 __device__ __forceinline__ void reorder_copy(const reorder_args& a, int unit, int copies) {
-  const int layer = unit / copies, c = unit - layer * copies;
+  constexpr int AHEAD = 4;
+  const int part = unit % a.parts, at = unit / a.parts, layer = at / copies, c = at - layer * copies;
   const int4 rec = a.copies[c];
-  const int bs_bytes = a.row_bytes << a.log2_bs;
-  const int64_t block_bytes = (int64_t)a.pairs * bs_bytes;
-  const char* const from = a.storage + layer * a.layer_bytes + rec.x * block_bytes;
-  char* const to = a.storage + layer * a.layer_bytes + rec.y * block_bytes;
-  const int run = rec.z * a.row_bytes / 16, all = run * a.pairs;
-  for (int v = threadIdx.x; v < all; v += REORDER_COLUMNS) {
-    const int pair = v / run, off = pair * bs_bytes + (v - pair * run) * 16;
-    st16_through(to + off, ld16(from + off));
+  const int bs_bytes = a.row_bytes << a.log2_bs, first = part * a.unit_pairs;
+  const int64_t block_bytes = (int64_t)a.pairs * bs_bytes, in = (int64_t)first * bs_bytes;
+  const char* const from = a.storage + layer * a.layer_bytes + rec.x * block_bytes + in;
+  char* const to = a.storage + layer * a.layer_bytes + rec.y * block_bytes + in;
+  const int run = rec.z * a.row_bytes / 16, all = run * min(a.unit_pairs, a.pairs - first);
+  for (int v0 = threadIdx.x; v0 < all; v0 += AHEAD * REORDER_COLUMNS) {
+    vec16 x[AHEAD];
+    int off[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) {
+      const int v = min(v0 + u * REORDER_COLUMNS, all - 1), pair = v / run;   // (past the end: the last vector again)
+      off[u] = pair * bs_bytes + (v - pair * run) * 16;
+      x[u] = ld16(from + off[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (v0 + u * REORDER_COLUMNS < all) st16_through(to + off[u], x[u]);
   }
 }
 
-// The blocks of the lists that nobody holds, each once, behind the free blocks. An entry whose change made the
-// count 0 has CLOSED set; where another one's count is 0 too its block was held by several requests, or by rows of one with
-// another block between, which have let go of it at once: the first of its entries counts, not the one that closed it.
-constexpr int32_t CLOSED = INT32_MIN;
-__device__ void reorder_free(const reorder_args& a, int lists) {
-  constexpr int N = REORDER_COLUMNS;
-  __shared__ int waves[2][N / 64], starts[N + 1], several;
-  const int tid = threadIdx.x;
-  const int left = a.num_free_in[0] - a.head[1];
-  auto load = [](const int32_t* p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
-  int freed = 0, turn = 0;
-  // each(number of the entry, entry): of all entries in order, N at a time; a barrier within
-  auto entries = [&](auto&& each) {
-    int before = 0;                                // entries of the lists done
-    for (int l0 = 0; l0 < lists; l0 += N) {
-      const int mine = l0 + tid < lists ? load(&a.gone_count[l0 + tid]) : 0;
-      int total;
-      __syncthreads();                             // starts has been read
-      starts[tid] = group_scan<N>(mine, waves, turn++, total);
-      __syncthreads();
-      for (int x0 = 0; x0 < total; x0 += N) {
-        const int x = x0 + tid;
-        int32_t e = -1;
-        if (x < total) {
-          int lo = 0, hi = N;
-          while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (starts[mid] <= x) lo = mid;
-            else hi = mid;
-          }
-          e = load(&a.gone[(int64_t)(l0 + lo) * REORDER_COLUMNS * a.beams + x - starts[lo]]);
-        }
-        each(x < total, before + x, e);
-      }
-      before += total;
-    }
-  };
-  auto push = [&](bool win, int32_t id) {
-    int won;
-    const int at = left + freed + group_scan<N>(win, waves, turn++, won);
-    freed += won;
-    if (win && at < a.num_blocks) a.free_blocks[at] = id;
-  };
-  if (tid == 0) several = 0;
-  entries([&](bool there, int, int32_t e) {
-    if (there && e >= 0 && load(&a.refs[e]) == 0) several = 1;
-  });
-  __syncthreads();
-  if (!several) {
-    entries([&](bool there, int, int32_t e) { push(there && e < 0, e & ~CLOSED); });
-  } else {
-    entries([&](bool there, int x, int32_t e) {    // the first entry of a block marks it
-      if (there && load(&a.refs[e & ~CLOSED]) <= 0) atomicMin(&a.refs[e & ~CLOSED], x - MARK);
-    });
-    __threadfence();
+// The blocks of the lists that nobody holds, each once, behind the free blocks: by the workgroup whose counts and list
+// were the last. A block may stand in several lists (requests that shared it and have let go of it at once); the first
+// of its entries counts.
+struct free_lds {
+  static constexpr int N = REORDER_COLUMNS, MOST = 4 * N, SLOTS = 1024, NONE = -1;
+  int waves[2][N / 64], starts[MOST], seen[SLOTS], several;
+};
+__device__ __forceinline__ int32_t free_load(const int32_t* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <int EACH>                                // of EACH * N lists from l0 on
+struct free_lists {
+  static constexpr int N = free_lds::N;
+  const reorder_args& a;
+  free_lds& s;
+  int& turn;
+  // their running sums into starts, and the whole
+  __device__ __forceinline__ int count(int l0, int lists) const {
+    const int tid = threadIdx.x;
+    int mine[EACH], sum = 0, total;
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) mine[u] = l0 + EACH * tid + u < lists ? free_load(&a.gone_count[l0 + EACH * tid + u]) : 0;
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) sum += mine[u];
+    __syncthreads();                               // starts has been read
+    int at = group_scan<N>(sum, s.waves, turn++, total);
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) s.starts[EACH * tid + u] = at, at += mine[u];
     __syncthreads();
-    entries([&](bool there, int x, int32_t e) {
-      const bool win = there && load(&a.refs[e & ~CLOSED]) == x - MARK;
-      push(win, e & ~CLOSED);
-      if (win) __hip_atomic_store(&a.refs[e & ~CLOSED], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    });
+    return total;
+  }
+  __device__ __forceinline__ int32_t entry(int l0, int x) const {
+    int lo = 0, hi = EACH * N;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (s.starts[mid] <= x) lo = mid;
+      else hi = mid;
+    }
+    return free_load(&a.gone[(int64_t)(l0 + lo) * N * a.beams + x - s.starts[lo]]);
+  }
+  // this thread's next n blocks behind the free ones; how many all have
+  __device__ __forceinline__ int push(int from, int n, const int32_t* ids) const {
+    int won;
+    int at = from + group_scan<N>(n, s.waves, turn++, won);
+    for (int u = 0; u < n; ++u, ++at)
+      if (at < a.num_blocks) a.free_blocks[at] = ids[u];
+    return won;
+  }
+  // all at once, where every block stands in one list: how many are free, or -1
+  __device__ __forceinline__ int few(int from, int total) const {
+    const int tid = threadIdx.x;
+    for (int i = tid; i < free_lds::SLOTS; i += N) s.seen[i] = free_lds::NONE;
+    if (tid == 0) s.several = 0;
+    int32_t id[EACH], refs[EACH], mine[EACH];
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) id[u] = EACH * tid + u < total ? entry(0, EACH * tid + u) : free_lds::NONE;
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) refs[u] = id[u] != free_lds::NONE ? free_load(&a.refs[id[u]]) : 1;
+    __syncthreads();
+    int n = 0;
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) {
+      if (refs[u] != 0) continue;
+      mine[n++] = id[u];
+      for (uint32_t slot = (uint32_t)id[u] * 2654435761u >> 22;; slot = (slot + 1) % free_lds::SLOTS) {   // (half of them at most)
+        const int was = atomicCAS(&s.seen[slot], free_lds::NONE, id[u]);
+        if (was == id[u]) s.several = 1;
+        if (was == free_lds::NONE || was == id[u]) break;
+      }
+    }
+    __syncthreads();
+    return s.several ? -1 : push(from, n, mine);
+  }
+};
+__device__ void reorder_free(const reorder_args& a, int lists) {
+  constexpr int N = free_lds::N;
+  __shared__ free_lds s;
+  const int tid = threadIdx.x, left = a.num_free_in[0] - a.head[1];
+  int turn = 0, freed = -1;
+  const free_lists<1> one{a, s, turn};
+  const free_lists<4> four{a, s, turn};
+  int total = N + 1;
+  if (lists <= N) total = one.count(0, lists);
+  if (total <= N) {
+    freed = one.few(left, total);
+  } else if (lists <= 4 * N) {
+    total = four.count(0, lists);
+    if (total <= 4 * N) freed = four.few(left, total);
+  }
+  if (freed < 0) {
+    freed = 0;
+    for (int pass = 0; pass < 2; ++pass) {         // the first entry of a block marks it; the marks are read
+      int before = 0;
+      for (int l0 = 0; l0 < lists; l0 += N) {
+        total = one.count(l0, lists);
+        for (int x0 = 0; x0 < total; x0 += N) {
+          const int x = x0 + tid, mark = before + x - MARK;
+          const int32_t id = x < total ? one.entry(l0, x) : free_lds::NONE;
+          const int32_t refs = id != free_lds::NONE ? free_load(&a.refs[id]) : 1;
+          if (pass == 0) {
+            if (refs <= 0) atomicMin(&a.refs[id], mark);
+          } else {
+            freed += one.push(left + freed, refs == mark, &id);
+            if (refs == mark) __hip_atomic_store(&a.refs[id], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          }
+        }
+        before += total;
+      }
+      __threadfence();
+      __syncthreads();
+    }
   }
   if (tid == 0) a.num_free_out[0] = left + freed;
 }
 
 __global__ __launch_bounds__(REORDER_COLUMNS) void reorder_tables_kernel(const reorder_args a, int table_groups) {
-  extern __shared__ int32_t lds[];                 // old entries [beams][128], the plan [beams][4], {children, keeps} [beams]
+  extern __shared__ int32_t lds[];                 // old entries [beams][128], the plan [beams], what rows hold [beams]
   if (a.head[0]) return;
   if ((int)blockIdx.x >= table_groups) {
     const int copies = a.head[1], stride = gridDim.x - table_groups;
-    for (int u = blockIdx.x - table_groups; u < copies * a.layers; u += stride) reorder_copy(a, u, copies);
+    for (int u = blockIdx.x - table_groups; u < copies * a.layers * a.parts; u += stride) reorder_copy(a, u, copies);
     return;
   }
   __shared__ int waves[2][REORDER_COLUMNS / 64];
@@ -243,11 +305,11 @@ __global__ __launch_bounds__(REORDER_COLUMNS) void reorder_tables_kernel(const r
   const int tid = threadIdx.x, j = REORDER_COLUMNS * chunk + tid, bs = 1 << a.log2_bs;
   int32_t* const old = lds + tid;                  // [k * 128]
   int4* const plan = (int4*)(lds + REORDER_COLUMNS * K);
-  int32_t* const kids = lds + (REORDER_COLUMNS + 4) * K;
-  int32_t* const keeps = kids + K;
+  int4* const holds = plan + K;                    // {whole blocks, blocks, children - 1, -1 unless a child keeps the open block}
   if (tid < K) {
-    plan[tid] = a.plan[row0 + tid];
-    kids[tid] = keeps[tid] = 0;
+    const int4 p = a.plan[row0 + tid];
+    plan[tid] = p;
+    holds[tid] = make_int4(p.w >> a.log2_bs, (p.w + bs - 1) >> a.log2_bs, -1, -1);
   }
   if (tid == 0) differ = INT32_MAX;
   // (columns are loaded before the request's width is known; the tables have them all)
@@ -260,50 +322,61 @@ __global__ __launch_bounds__(REORDER_COLUMNS) void reorder_tables_kernel(const r
       if (k0 + u < K) old[REORDER_COLUMNS * (k0 + u)] = e[u];
   }
   __syncthreads();
-  int width = 0;                                   // columns that the request's old tables hold
-  for (int k = 0; k < K; ++k) width = max(width, (plan[k].w + bs - 1) >> a.log2_bs);
-  if (chunk == 0 && tid < K) a.lens_out[row0 + tid] = plan[tid].y;
-  if (tid < K && plan[tid].x >= 0) {
-    atomicAdd(&kids[plan[tid].x - row0], 1);
-    if (plan[tid].z < 0) atomicOr(&keeps[plan[tid].x - row0], 1);
+  if (tid < K) {
+    const int4 p = plan[tid];
+    if (chunk == 0) a.lens_out[row0 + tid] = p.y;
+    if (p.x >= 0) {
+      atomicAdd(&holds[p.x - row0].z, 1);
+      if (p.z < 0) atomicMax(&holds[p.x - row0].w, 0);
+    }
   }
   __syncthreads();
-  // what every old row's hold on its block of this column becomes; rows of one block behind each other at once
-  uint64_t lost = 0, closed = 0;                   // rows that begin such a run which lets go; whose count is 0 then
-  if (j < width) {
-    for (int k = 0; k < K;) {
-      const int id = old[REORDER_COLUMNS * k], from = k;
-      int sum = 0;
-      for (; k < K && old[REORDER_COLUMNS * k] == id; ++k) {
-        const int len = plan[k].w;
-        if (j < len >> a.log2_bs) sum += kids[k] - 1;
-        else if (j < (len + bs - 1) >> a.log2_bs) sum += keeps[k] - 1;   // the open block: one child keeps it, or none
-      }
-      if (sum && id >= 0 && id < a.num_blocks) {
-        const int was = atomicAdd(&a.refs[id], sum);
+  // what every old row's hold on its block of this column becomes, rows of one block behind each other at once
+  int width = 0;                                   // columns that the request's old tables hold
+  uint64_t lost = 0;                               // rows that begin a run that lets go
+  {
+    int id = -1, from = 0, sum = 0;
+    auto end = [&] {
+      if (sum != 0 && id >= 0 && id < a.num_blocks) {
+        atomicAdd(&a.refs[id], sum);
         if (sum < 0) lost |= (uint64_t)1 << from;
-        if (sum < 0 && was + sum == 0) closed |= (uint64_t)1 << from;
       }
+    };
+#pragma unroll 4
+    for (int k = 0; k < K; ++k) {
+      const int4 h = holds[k];
+      const int next = j < h.y ? old[REORDER_COLUMNS * k] : -1;
+      width = max(width, h.y);
+      if (next != id) {
+        end();
+        id = next, from = k, sum = 0;
+      }
+      sum += j < h.x ? h.z : j < h.y ? h.w : 0;
     }
+    end();
   }
   int total;
   int at = group_scan<REORDER_COLUMNS>(__popcll(lost), waves, 0, total);
   int32_t* const list = a.gone + (int64_t)blockIdx.x * REORDER_COLUMNS * K;
   for (uint64_t left = lost; left; left &= left - 1) {
     const int k = __ffsll((unsigned long long)left) - 1;
-    __hip_atomic_store(&list[at++], old[REORDER_COLUMNS * k] | (closed >> k & 1 ? CLOSED : 0), __ATOMIC_RELAXED,
-                       __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(&list[at++], old[REORDER_COLUMNS * k], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   if (tid == 0) __hip_atomic_store(&a.gone_count[blockIdx.x], total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the wave's list and counts are in memory
+  __syncthreads();
+  int place = 0;
+  if (tid == 0) place = __hip_atomic_fetch_add(&a.head[2], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   // the new tables, and whether the live rows agree in this column
   if (j < width) {
     int one = -1;
     bool same = true, all = true;                  // all: a whole block of every live row
+#pragma unroll 4
     for (int k = 0; k < K; ++k) {
       const int4 p = plan[k];
-      int id = -1;
-      if (j < (p.y + bs - 1) >> a.log2_bs)
-        id = p.z >= 0 && j == p.y >> a.log2_bs ? p.z : old[REORDER_COLUMNS * (p.x - row0)];
+      int id = old[REORDER_COLUMNS * max(p.x - row0, 0)];
+      if (p.z >= 0 && j == p.y >> a.log2_bs) id = p.z;
+      if (j >= (p.y + bs - 1) >> a.log2_bs) id = -1;
       a.tables[(int64_t)(row0 + k) * a.max_nb + j] = id;
       if (p.y > 0) {
         all &= j < p.y >> a.log2_bs;
@@ -313,13 +386,9 @@ __global__ __launch_bounds__(REORDER_COLUMNS) void reorder_tables_kernel(const r
     }
     if (all && !same) atomicMin(&differ, j);
   }
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // the wave's list and counts are in memory
+  if (tid == 0) arrived = place;
   __syncthreads();
-  if (tid == 0) {
-    if (differ != INT32_MAX) atomicMin(&a.shared[g], differ);
-    arrived = __hip_atomic_fetch_add(&a.head[2], 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  __syncthreads();
+  if (tid == 0 && differ != INT32_MAX) atomicMin(&a.shared[g], differ);
   if (arrived == table_groups - 1) reorder_free(a, table_groups);
 }
 
@@ -372,8 +441,13 @@ extern "C" int32_t tb_beam_reorder(void* storage, int32_t num_layers, int64_t la
     TB_CHECK_ARG(block < ((int64_t)1 << 31));
     TB_CHECK_ARG(storage && ((uintptr_t)storage & 15u) == 0 && layer_stride_bytes % 16 == 0);
     TB_CHECK_ARG(num_layers == 1 || layer_stride_bytes >= num_blocks * block);
-    TB_CHECK_ARG((int64_t)num_layers * num_rows < ((int64_t)1 << 31));
     a.pairs = 2 * num_kv_heads, a.row_bytes = (int32_t)row;
+    // units of some 512 vectors: half a block's positions on average
+    const int64_t vectors = block_size * row / 32;
+    a.unit_pairs = (int32_t)(vectors >= 512 ? 1 : vectors < 1 ? a.pairs : 512 / vectors);
+    if (a.unit_pairs > a.pairs) a.unit_pairs = a.pairs;
+    a.parts = (a.pairs + a.unit_pairs - 1) / a.unit_pairs;
+    TB_CHECK_ARG((int64_t)num_layers * num_rows * a.parts < ((int64_t)1 << 31));
   }
   a.storage = (char*)storage, a.layer_bytes = layer_stride_bytes, a.layers = num_layers, a.num_blocks = num_blocks;
   a.log2_bs = __builtin_ctz((unsigned)block_size);
@@ -385,9 +459,9 @@ extern "C" int32_t tb_beam_reorder(void* storage, int32_t num_layers, int64_t la
   a.head = (int32_t*)ws, a.plan = (int4*)(ws + z.plan), a.copies = (int4*)(ws + z.copies);
   a.least = (int32_t*)(ws + z.least), a.gone_count = (int32_t*)(ws + z.count), a.gone = (int32_t*)(ws + z.gone), a.chunks = (int32_t)z.chunks;
   const int lists = (int)(num_rows / beams * z.chunks);
-  const int64_t units = (int64_t)num_rows * num_layers;
-  const int movers = (int)(units < 2048 ? units : 2048);
-  const size_t lds = sizeof(int32_t) * (REORDER_COLUMNS + 6) * (size_t)beams;
+  const int64_t units = (int64_t)num_rows * num_layers * a.parts;
+  const int movers = (int)(units < 1024 ? units : 1024);
+  const size_t lds = sizeof(int32_t) * (REORDER_COLUMNS + 8) * (size_t)beams;
   hipLaunchKernelGGL(reorder_plan_kernel, dim3(1), dim3(1024), 0, stream, a);
   hipLaunchKernelGGL(reorder_tables_kernel, dim3(lists + movers), dim3(REORDER_COLUMNS), lds, stream, a, lists);
   TB_RETURN_LAUNCH_STATUS();
