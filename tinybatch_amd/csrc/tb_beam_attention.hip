@@ -30,6 +30,11 @@ namespace tb {
 
 constexpr int PLAN_THREADS = 1024;
 constexpr int PLAN_STEP = 128;                     // parts are multiples of it
+// K/V of this many bytes are loaded past the caches' replacement, where one workgroup alone reads them: 1.1 GB (24 requests of 4
+// beams at 32 / 8 heads of 128) 178 us against 190. Less may still lie in the 256 MB behind the L2s from the last time: 57 MB (32
+// of 8 at 14 / 2 heads of 64, three such pools in turn) 16.7 us against 20.8.
+constexpr int64_t PLAN_STREAM = (int64_t)256 << 20;
+constexpr int PLAN_CUS = 256, PLAN_MOST = 2048;    // parts, over all kv heads: at least, where there is enough to read; at most
 
 struct beam_args {
   const char* q;               // [R][Hq][D]
@@ -42,7 +47,7 @@ struct beam_args {
   int32_t max_nb, rows, beams;
   int32_t num_heads, num_kv_heads, rep;
   int32_t log2_bs;
-  const int32_t* head;         // of the plan: {entries, ..}
+  const int32_t* head;         // of the plan: {entries, P, whether K/V are loaded past the caches' replacement}
   const int4* entries;         // two per part
   const int4* row_parts;       // [R]: {first slot, parts} of the shared positions, {first slot, parts} of its own
   float* ws_acc;               // [slots][Hq][D]
@@ -59,10 +64,10 @@ struct plan_args {
   int32_t col_blocks;          // workgroups that a part of shared positions takes for its columns
   int32_t own_blocks;          // the same of a row's own positions
   int32_t block_cols, own_cols;   // columns of one
-  int32_t target;              // parts that fill the GPU
+  int32_t kv_heads, row_bytes;    // row_bytes: of a position's K and V of a kv head
   int32_t max_entries;
   int64_t max_slots;
-  int32_t* head;               // {entries, P}
+  int32_t* head;               // {entries, P, whether the K/V are more than the caches behind the L2s hold}
   int4* entries;
   int4* row_parts;
 };
@@ -78,108 +83,123 @@ __device__ __forceinline__ int64_t plan_sum(int64_t x, int64_t* lds) {
   for (int w = 0; w < PLAN_THREADS / 64; ++w) x += lds[w];
   return x;
 }
-
-// The positions of request g's rows that are read once for all: whole blocks that every row which
-// sees anything sees whole; `from`: the first such row (its table is read), -1 without one.
-__device__ __forceinline__ int plan_ctx(const plan_args& a, int r) {   // (never beyond the row's table)
-  return max(0, min(a.row_ctx[r], a.max_nb << a.log2_bs));
-}
-__device__ __forceinline__ int plan_shared(const plan_args& a, int g, int& from) {
-  int least = INT32_MAX;
-  from = -1;
-  for (int k = 0; k < a.beams; ++k) {
-    const int n = plan_ctx(a, g * a.beams + k);
-    if (n > 0) {
-      least = min(least, n);
-      if (from < 0) from = g * a.beams + k;
-    }
+// Exclusive running sum over the workgroup, and the whole.
+__device__ __forceinline__ int plan_scan(int x, int (*waves)[PLAN_THREADS / 64], int turn, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int up = x;
+#pragma unroll
+  for (int o = 1; o < 64; o *= 2) {
+    const int y = __shfl_up(up, o);
+    if (lane >= o) up += y;
   }
-  if (from < 0 || a.beams == 1) return 0;
-  return max(0, min(a.shared[g], least >> a.log2_bs)) << a.log2_bs;
+  if (lane == 63) waves[turn & 1][wave] = up;
+  __syncthreads();
+  int before = 0;
+  total = 0;
+  for (int w = 0; w < PLAN_THREADS / 64; ++w) {
+    if (w < wave) before += waves[turn & 1][w];
+    total += waves[turn & 1][w];
+  }
+  return before + up - x;
 }
 
+// The length of the parts: a part has a start and an end (its first loads, its partials) that cost as much as a few hundred
+// positions, and the last parts to run leave the GPU half empty, the longer the longer they are. Both weigh the
+// same near 32 sqrt(bytes in all) bytes a part: bf16, 32 requests of 8 beams at 14 / 2 heads of 64 (51 MB of K/V) 17 us at
+// parts of 900, 19 at 512, 23 at 256; 24 of 4 at 32 / 8 heads of 128 (1.1 GB) 191 us at 1920, 204 at 3840, 197 at 1024.
+// With little to read, parts for every CU.
+__device__ __forceinline__ int64_t plan_length(int64_t positions, const plan_args& a) {
+  const int64_t all = positions * a.kv_heads;
+  const int64_t even = (int64_t)(32.f * sqrtf((float)all / (float)a.row_bytes));
+  int64_t P = min(even, all / PLAN_CUS);
+  P = max(P, all / PLAN_MOST + 1);
+  return (P + PLAN_STEP - 1) / PLAN_STEP * PLAN_STEP;
+}
+
+// Rows are looked at one a thread, requests by the thread of their first row.
 __global__ __launch_bounds__(PLAN_THREADS) void beam_plan_kernel(const plan_args a) {
   __shared__ int64_t lds[PLAN_THREADS / 64];
-  __shared__ int32_t waves[2][PLAN_THREADS / 64][2];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, groups = a.rows / a.beams;
-  // positions of all parts
-  int64_t all = 0;
-  for (int g = tid; g < groups; g += PLAN_THREADS) {
-    int from;
-    const int c = plan_shared(a, g, from);
-    all += (int64_t)c * a.col_blocks;
-    for (int k = 0; k < a.beams; ++k) all += (int64_t)max(0, plan_ctx(a, g * a.beams + k) - c) * a.own_blocks;
-  }
-  all = plan_sum(all, lds);
-  int64_t P = (all / max(a.target, 1) + PLAN_STEP) / PLAN_STEP * PLAN_STEP;
-  for (;;) {                                       // longer parts until the partials fit
-    int64_t slots = 0;
-    for (int g = tid; g < groups; g += PLAN_THREADS) {
-      int from;
-      const int c = plan_shared(a, g, from);
-      slots += (c + P - 1) / P * a.beams;
-      for (int k = 0; k < a.beams; ++k) slots += (max(0, plan_ctx(a, g * a.beams + k) - c) + P - 1) / P;
-    }
-    slots = plan_sum(slots, lds);
-    if (slots <= a.max_slots || P >= ((int64_t)1 << 31)) break;
-    P *= 2;
-  }
-  // entries and slots: a request's shared parts, then its rows' own
-  int entry0 = 0, slot0 = 0;
-  for (int g0 = 0, turn = 0; g0 < groups; g0 += PLAN_THREADS, turn ^= 1) {
-    const int g = g0 + tid;
-    int from = -1, c = 0, parts = 0, mine[2] = {0, 0};
-    if (g < groups) {
-      c = plan_shared(a, g, from);
-      parts = (int)((c + P - 1) / P);
-      mine[0] = parts * a.col_blocks;
-      mine[1] = parts * a.beams;
-      for (int k = 0; k < a.beams; ++k) {
-        const int own = (int)((max(0, plan_ctx(a, g * a.beams + k) - c) + P - 1) / P);
-        mine[0] += own * a.own_blocks;
-        mine[1] += own;
-      }
-    }
-    int up[2] = {mine[0], mine[1]};
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int o = 1; o < 64; o *= 2) {
-        const int y = __shfl_up(up[i], o);
-        if (lane >= o) up[i] += y;
-      }
-      if (lane == 63) waves[turn][wave][i] = up[i];
+  __shared__ int waves[2][PLAN_THREADS / 64];
+  __shared__ int ctx[PLAN_THREADS], common[PLAN_THREADS], at[PLAN_THREADS], from[PLAN_THREADS];
+  const int tid = threadIdx.x, K = a.beams, each = PLAN_THREADS / K * K;   // rows of whole requests
+  const int bs = 1 << a.log2_bs;
+  // rows i0 .. of the round: positions seen; the request's shared positions and its first row that sees any
+  auto look = [&](int i0) {
+    const int r = i0 + tid;
+    const bool mine = tid < each && r < a.rows;
+    __syncthreads();                               // (the round before has been read)
+    ctx[tid] = mine ? max(0, min(a.row_ctx[r], a.max_nb << a.log2_bs)) : 0;   // (never beyond the row's table)
+    const int given = mine && tid % K == 0 ? a.shared[r / K] : 0;
+    __syncthreads();
+    if (mine && tid % K == 0) {
+      int least = INT32_MAX, live = -1;
+      for (int k = K - 1; k >= 0; --k)
+        if (ctx[tid + k] > 0) least = min(least, ctx[tid + k]), live = r + k;
+      // whole blocks that every row which sees anything sees whole
+      common[tid] = live < 0 || K == 1 ? 0 : max(0, min(given, least >> a.log2_bs)) * bs;
+      from[tid] = live;
     }
     __syncthreads();
-    int e = entry0 + up[0] - mine[0], s = slot0 + up[1] - mine[1];
-    for (int w = 0; w < PLAN_THREADS / 64; ++w) {
-      if (w < wave) e += waves[turn][w][0], s += waves[turn][w][1];
-      entry0 += waves[turn][w][0];
-      slot0 += waves[turn][w][1];
+    return mine;
+  };
+  auto parts = [](int64_t n, int64_t P) { return (int)((max(n, (int64_t)0) + P - 1) / P); };
+  int64_t all = 0;
+  for (int i0 = 0; i0 < a.rows; i0 += each) {
+    if (!look(i0)) continue;
+    const int c = common[tid / K * K];
+    all += (int64_t)max(0, ctx[tid] - c) * a.own_blocks + (tid % K == 0 ? (int64_t)c * a.col_blocks : 0);
+  }
+  all = plan_sum(all, lds);
+  int64_t P = plan_length(all, a), shared_parts;
+  for (;;) {                                       // longer parts until the partials fit
+    int64_t shared = 0, own = 0;
+    for (int i0 = 0; i0 < a.rows; i0 += each) {
+      if (!look(i0)) continue;
+      const int c = common[tid / K * K];
+      own += parts(ctx[tid] - c, P);
+      if (tid % K == 0) shared += parts(c, P);
     }
-    if (g >= groups) continue;
-    auto put = [&](int row0, int n, int table, int p0, int p1, int col, int part, int first) {
-      if (e < a.max_entries) {
-        a.entries[2 * e] = make_int4(row0, n, table, p0);
-        a.entries[2 * e + 1] = make_int4(p1, col, part, first);
-      }
-      ++e;
-    };
-    const int first = s;
-    s += parts * a.beams;
-    for (int p = 0; p < parts; ++p)
-      for (int b = 0; b < a.col_blocks; ++b)
-        put(g * a.beams, a.beams, from, (int)(p * P), (int)min((p + 1) * P, (int64_t)c), b * a.block_cols, p, 1);
-    for (int k = 0; k < a.beams; ++k) {
-      const int r = g * a.beams + k, n = plan_ctx(a, r), own = (int)((max(0, n - c) + P - 1) / P);
-      a.row_parts[r] = n > 0 ? make_int4(first + k, parts, s, own) : make_int4(0, 0, 0, 0);
-      for (int p = 0; p < own; ++p)
-        for (int b = 0; b < a.own_blocks; ++b)
-          put(r, 1, r, (int)(c + p * P), (int)min(c + (p + 1) * P, (int64_t)n), b * a.own_cols, p, 0);
-      s += own;
+    shared_parts = plan_sum(shared, lds);
+    if (shared_parts * K + plan_sum(own, lds) <= a.max_slots || P >= ((int64_t)1 << 31)) break;
+    P *= 2;
+  }
+  // entries and slots: all requests' shared parts, which are the longer ones, then the rows' own
+  auto put = [&](int64_t e, int row0, int n, int table, int64_t p0, int64_t p1, int col, int part, int shared) {
+    if (e >= a.max_entries) return;
+    a.entries[2 * e] = make_int4(row0, n, table, (int)p0);
+    a.entries[2 * e + 1] = make_int4((int)p1, col, part, shared);
+  };
+  int part0 = 0, own0 = 0, turn = 0;
+  for (int i0 = 0; i0 < a.rows; i0 += each) {
+    const bool mine = look(i0);
+    const int head = tid / K * K, c = mine ? common[head] : 0, n = ctx[tid], r = i0 + tid;
+    const int shared = mine && tid == head ? parts(c, P) : 0, own = mine ? parts(n - c, P) : 0;
+    int total;
+    const int s = part0 + plan_scan(shared, waves, turn++, total);
+    part0 += total;
+    const int o = own0 + plan_scan(own, waves, turn++, total);
+    own0 += total;
+    at[tid] = s;
+    __syncthreads();
+    if (!mine) continue;
+    const int first = at[head], mine_shared = parts(c, P);
+    a.row_parts[r] = n > 0 ? make_int4(first * K + tid - head, mine_shared, (int)shared_parts * K + o, own) : make_int4(0, 0, 0, 0);
+    for (int x = tid - head; x < mine_shared * a.col_blocks; x += K) {   // the request's threads in turn
+      const int p = x / a.col_blocks, b = x - p * a.col_blocks;
+      put((int64_t)(first + p) * a.col_blocks + b, i0 + head, K, from[head], p * P, min((p + 1) * P, (int64_t)c), b * a.block_cols,
+          p, 1);
+    }
+    for (int x = 0; x < own * a.own_blocks; ++x) {
+      const int p = x / a.own_blocks, b = x - p * a.own_blocks;
+      put(shared_parts * a.col_blocks + (int64_t)(o + p) * a.own_blocks + b, r, 1, r, c + p * P, min(c + (p + 1) * P, (int64_t)n),
+          b * a.own_cols, p, 0);
     }
   }
-  if (tid == 0) a.head[0] = min(entry0, a.max_entries), a.head[1] = (int)min(P, (int64_t)INT32_MAX);
+  if (tid == 0) {
+    a.head[0] = (int)min(shared_parts * a.col_blocks + (int64_t)own0 * a.own_blocks, (int64_t)a.max_entries);
+    a.head[1] = (int)min(P, (int64_t)INT32_MAX);
+    a.head[2] = all * a.kv_heads * a.row_bytes >= PLAN_STREAM;
+  }
 }
 
 // ---- columns over the matrix unit -----------------------------------------------------
@@ -224,8 +244,9 @@ __device__ __forceinline__ void beam_part(const beam_args& a, char* lds, const i
   const int row0 = e0.x, nrows = e0.y, table_row = e0.z, p0 = e0.w, p1 = e1.x, part = e1.z;
   const int ncols = nrows * a.rep, col0 = e1.y + 32 * (wave % CW), set = wave / CW;
   const int col = min(col0 + lcol, ncols - 1), my_row = col / a.rep, hd = kvh * a.rep + col - my_row * a.rep;
-  const bool busy = col0 < ncols;
+  const bool busy = col0 < ncols, once = ncols <= 32 * CW && a.head[2];   // (no other workgroup reads these K/V rows)
 
+  const int4 parts = a.row_parts[row0 + my_row];
   vec16 q[QS];
   {
     const char* const qrow = a.q + (int64_t)(row0 + my_row) * a.q_row_bytes + (int64_t)hd * RB + 16 * half;
@@ -264,8 +285,14 @@ __device__ __forceinline__ void beam_part(const beam_args& a, char* lds, const i
       for (int i = 0; i < S::TB / 1024; ++i) {
         const int r = S::RPL * i + lrow;
         const uint32_t row = (uint32_t)(min(r, rmax) * RB);
-        s_dma16_l2(row + 16 * (lpiece ^ S::kswz(r)), base, dst + 1024 * i);
-        s_dma16_l2(row + 16 * (lpiece ^ S::vswz(r)), base + v_off, dst + HALF + 1024 * i);
+        const uint32_t ko = row + 16 * (lpiece ^ S::kswz(r)), vo = row + 16 * (lpiece ^ S::vswz(r));
+        if (once) {
+          s_dma16_s(ko, base, dst + 1024 * i);
+          s_dma16_s(vo, base + v_off, dst + HALF + 1024 * i);
+        } else {
+          s_dma16_l2(ko, base, dst + 1024 * i);
+          s_dma16_l2(vo, base + v_off, dst + HALF + 1024 * i);
+        }
       }
     }
   };
@@ -494,7 +521,6 @@ __device__ __forceinline__ void beam_part(const beam_args& a, char* lds, const i
     }
   }
   if (!mine) return;
-  const int4 parts = a.row_parts[row];
   if (parts.y + parts.w == 0) return;           // a row that sees nothing, among rows that do
   const bool whole = parts.y + parts.w == 1;
   const int slot = e1.w ? parts.x + part * a.beams : parts.z + part;
@@ -597,7 +623,7 @@ __global__ __launch_bounds__(256) void beam_join_kernel(const beam_args a) {
 // What a plan of these sizes holds, the same for the plan's launch, the attention's and their callers.
 struct beam_sizes {
   int cw, own;                 // sets of 32 columns of a workgroup: shared positions, a row's own
-  int col_blocks, own_blocks, target;
+  int col_blocks, own_blocks;
   int64_t entries, slots, row_parts, list, plan_bytes;
   beam_sizes(int64_t rows, int64_t beams, int64_t heads, int64_t kv_heads, int64_t head_dim, int32_t dtype) {
     const int64_t rep = heads / kv_heads, cols = beams * rep, row_bytes = head_dim * (dtype == TB_DTYPE_F32 ? 4 : 2);
@@ -605,11 +631,11 @@ struct beam_sizes {
     cw = cols <= 32 * own ? own : cols <= 64 ? 2 : 4;
     col_blocks = (int)((cols + 32 * cw - 1) / (32 * cw));
     own_blocks = (int)((rep + 32 * own - 1) / (32 * own));
-    target = (int)((512 + kv_heads - 1) / kv_heads);
-    entries = rows / beams * col_blocks + rows * own_blocks + target;
+    const int64_t most_parts = PLAN_MOST / kv_heads + 1;   // but for a part of every request and row
+    entries = rows / beams * col_blocks + rows * own_blocks + most_parts;
     const int64_t slot_bytes = heads * (head_dim + 2) * 4, least = 2 * rows;
     slots = TB_BEAM_PARTIAL_BYTES / slot_bytes;
-    const int64_t most = target * beams + least;   // a part of shared positions has a slot per beam
+    const int64_t most = most_parts * beams + least;   // a part of shared positions has a slot per beam
     if (slots > most) slots = most;
     if (slots < least) slots = least;
     row_parts = 64;
@@ -669,7 +695,8 @@ extern "C" int32_t tb_beam_plan(const int32_t* row_ctx, const int32_t* shared_bl
   a.row_ctx = row_ctx, a.shared = shared_blocks, a.rows = num_rows, a.beams = beams;
   a.log2_bs = __builtin_ctz((unsigned)block_size), a.max_nb = max_blocks_per_row;
   a.col_blocks = z.col_blocks, a.own_blocks = z.own_blocks, a.block_cols = 32 * z.cw, a.own_cols = 32 * z.own;
-  a.target = z.target, a.max_entries = (int32_t)z.entries, a.max_slots = z.slots;
+  a.kv_heads = num_kv_heads, a.row_bytes = 2 * head_dim * (dtype == TB_DTYPE_F32 ? 4 : 2);
+  a.max_entries = (int32_t)z.entries, a.max_slots = z.slots;
   char* const p = (char*)plan;
   a.head = (int32_t*)p, a.row_parts = (int4*)(p + z.row_parts), a.entries = (int4*)(p + z.list);
   hipLaunchKernelGGL(beam_plan_kernel, dim3(1), dim3(PLAN_THREADS), 0, stream, a);

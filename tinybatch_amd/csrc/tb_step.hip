@@ -52,17 +52,18 @@ struct step_args {
   int32_t* sums;               // [STEP_SUMS][rows + 1] and the faults, where a launch made them before
 };
 
-__device__ __forceinline__ int64_t step_parts(int64_t m, int32_t P) {   // F(m)
-  const int64_t a = m / P, r = m - a * P;
-  return P * (a * (a + 1) / 2) + r * (a + 1);
+// (lengths are below 2^31: divisions in 32 bits)
+__device__ __forceinline__ int64_t step_parts(uint32_t m, uint32_t P) {   // F(m)
+  const uint32_t a = m / P, r = m - a * P;
+  return (int64_t)P * ((int64_t)a * (a + 1) / 2) + (int64_t)r * (a + 1);
 }
 // Items of a row's first n tokens behind c positions, n at the end of an item.
-__device__ __forceinline__ int64_t step_items(int64_t c, int64_t n, int32_t P, int32_t group) {
-  if (n <= 0) return 0;
-  auto some = [&](int64_t rows) { return (rows + group - 1) / group; };
-  const int64_t n0 = (c + P) / P, n1 = (c + n + P - 1) / P;   // partitions of the first and the last token
+__device__ __forceinline__ int64_t step_items(uint32_t c, uint32_t n, uint32_t P, uint32_t group) {
+  if (n == 0) return 0;
+  auto some = [&](uint32_t rows) { return (int64_t)((rows + group - 1) / group); };
+  const uint32_t n0 = c / P + 1, n1 = (c + n - 1) / P + 1;    // partitions of the first and the last token
   if (n0 == n1) return n0 * some(n);
-  const int64_t between = (n0 + n1) * (n1 - n0 - 1) / 2;      // n0 + 1 + .. + n1 - 1
+  const int64_t between = (int64_t)(n0 + n1) * (n1 - n0 - 1) / 2;   // n0 + 1 + .. + n1 - 1
   return n0 * some(n0 * P - c) + between * some(P) + n1 * some(c + n - (n1 - 1) * P);
 }
 
