@@ -37,6 +37,7 @@ from dataclasses import dataclass, field
 import torch
 
 from . import ops
+from .beam_search import BeamResult, beam_search
 from .block_manager import BlockManager
 from .config import EngineConfig
 from .decode_graphs import DecodeGraphs, MergeErrors
@@ -99,6 +100,19 @@ class LLMEngine:
         while self.has_work():
             self.step()
         return [r.output_token_ids for r in reqs]
+
+    def beam_search(self, prompts: list[list[int]], *, num_beams: int = 4, max_new_tokens: int | None = None,
+                    length_penalty: float = 1.0, num_return: int = 1) -> list[list[BeamResult]]:
+        """Per prompt the ``num_return`` best of ``num_beams`` beams (beam_search.py), by score / length **
+        length_penalty. Runs to its end on the blocks that are free now, between two steps of the requests
+        that are being served; a captured step (EngineConfig.decode_graphs) is replayed from the second token on."""
+        new = self.cfg.max_new_tokens if max_new_tokens is None else max_new_tokens
+        longest = max((len(p) for p in prompts), default=0)
+        if longest + new > self.cfg.max_model_len:
+            raise ValueError(f"a prompt of {longest} tokens and {new} new ones exceed max_model_len {self.cfg.max_model_len}")
+        return beam_search(self.model, self.kv_cache, self.block_manager, prompts, num_beams=num_beams, max_new=new,
+                           eos_ids=tuple(self.cfg.stop_token_ids), length_penalty=length_penalty, num_return=num_return,
+                           budget=self.cfg.max_batch_tokens, graph=self.cfg.decode_graphs)
 
     # ---- one iteration ---------------------------------------------------------
     @staticmethod
