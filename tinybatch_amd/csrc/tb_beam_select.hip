@@ -26,7 +26,7 @@ constexpr int SELECT_SEGMENTS = 1024;              // of a row, at most
 constexpr int SELECT_THREADS = 512;
 constexpr int SELECT_LIST = 2048;                  // tokens from the threshold up that part 2 keeps in LDS
 constexpr int MERGE_LIST = 512;                    // candidates that are ranked as they are; of more M + M / 2 + 8 at most
-static_assert(MERGE_LIST >= SELECT_THREADS, "a list for a workgroup's candidates");
+static_assert(MERGE_LIST == SELECT_THREADS, "a thread for every one");
 constexpr float SELECT_MOST = 3.402823466e38f;
 
 struct select_args {
@@ -301,23 +301,26 @@ __device__ void select_list(const select_args& a, rows_lds& s, int row) {
     for (int i = 0; i < WORDS; ++i) c += __popcll(__ballot(v[i] >= o));
     return c;
   };
-  uint32_t lo = ORDER_NONE, hi = select_order(m) + 1;
-  bool exact = true;
-  if (reach(ORDER_NONE + 1) >= M) {                // else everything above -inf
-    lo = least > -INFINITY ? select_order(least) : ORDER_NONE + 1;
-    while (hi - lo > 1) {
-      const uint32_t mid = lo + (hi - lo) / 2;
-      const int c = reach(mid);
-      if (c >= M) {
-        lo = mid;
-        if (c <= M + M / 2 + 8) {
-          exact = false;                           // near enough: all of them
-          break;
-        }
-      } else {
-        hi = mid;
+  uint32_t lo = ORDER_NONE, hi = select_order(m) + 1, probe = least > -INFINITY ? 0 : ORDER_NONE + 1;
+  int over = 0;                                    // segments that reach hi
+  bool exact = true;                               // else: all that reach lo
+  if (!probe) lo = select_order(least);
+  while (hi - lo > 1) {
+    const uint32_t mid = probe ? probe : lo + (hi - lo) / 2;
+    const int c = reach(mid);
+    if (c >= M) {
+      lo = mid;
+      if (c <= M + M / 2 + 8) {
+        exact = false;
+        break;
       }
+    } else if (probe) {                            // everything above -inf
+      break;
+    } else {
+      hi = mid;
+      over = c;
     }
+    probe = 0;
   }
   // ---- the segments that reach it; where several equal it and not all are wanted, the first ones ----
   auto rising = [&](int need) {                    // in order; how many
@@ -335,7 +338,7 @@ __device__ void select_list(const select_args& a, rows_lds& s, int row) {
     __syncthreads();
     return n;
   };
-  const int want_equal = lo == ORDER_NONE ? 0 : exact ? M - reach(lo + 1) : SELECT_SEGMENTS;
+  const int want_equal = lo == ORDER_NONE ? 0 : exact ? M - over : SELECT_SEGMENTS;
   int n;
   if (want_equal == SELECT_SEGMENTS || lo == ORDER_NONE) {
     for (int i = tid; i < SELECT_SEGMENTS; i += SELECT_THREADS) {
@@ -454,12 +457,27 @@ __device__ void select_list(const select_args& a, rows_lds& s, int row) {
     }
 }
 
+// A double's place among all doubles.
+__device__ __forceinline__ uint64_t merge_order(double x) {
+  const uint64_t b = (uint64_t)__double_as_longlong(x + 0.);
+  return b >> 63 ? ~b : b | (uint64_t)1 << 63;
+}
+__device__ __forceinline__ double merge_value(uint64_t o) {
+  return __longlong_as_double((int64_t)(o >> 63 ? o ^ (uint64_t)1 << 63 : ~o));
+}
+constexpr uint64_t MERGE_NONE = 0x000FFFFFFFFFFFFFull;   // of -inf
+__device__ __forceinline__ uint64_t merge_xor(uint64_t x, int o) {
+  return (uint64_t)__shfl_xor((unsigned long long)x, o);
+}
+
 // Part 3: a candidate and its place in the order: larger value, then smaller beam, then the beam's own order.
 struct cand {
-  double c;
-  int64_t at;
+  uint64_t c;                  // merge_order of the value
+  uint64_t at;                 // beam << 32 | place in its list
 };
-__device__ __forceinline__ bool better(const cand& x, const cand& y) { return x.c > y.c || (x.c == y.c && x.at < y.at); }
+__device__ __forceinline__ bool better(const cand& x, const cand& y) {   // (no branches)
+  return (x.c > y.c) | ((x.c == y.c) & (x.at < y.at));
+}
 
 struct merge_lds {
   double norms[TB_BEAMS_MAX][3];                   // m, log S, the score
@@ -469,16 +487,6 @@ struct merge_lds {
   uint64_t tops[SELECT_THREADS / 64], leasts[SELECT_THREADS / 64];
   int held;
 };
-
-// A double's place among all doubles.
-__device__ __forceinline__ uint64_t merge_order(double x) {
-  const uint64_t b = (uint64_t)__double_as_longlong(x + 0.);
-  return b >> 63 ? ~b : b | (uint64_t)1 << 63;
-}
-constexpr uint64_t MERGE_NONE = 0x000FFFFFFFFFFFFFull;   // of -inf
-__device__ __forceinline__ uint64_t merge_xor(uint64_t x, int o) {
-  return (uint64_t)__shfl_xor((unsigned long long)x, o);
-}
 
 // A request's candidates from its beams' lists, by a workgroup of SELECT_THREADS.
 __device__ void select_merge(const select_args& a, merge_lds& s, int request) {
@@ -492,10 +500,19 @@ __device__ void select_merge(const select_args& a, merge_lds& s, int request) {
   double(*const norms)[3] = s.norms;
   const float2* const lists = a.lists + (int64_t)row0 * M;
   auto entry = [&](int i) { return lists[min(i, all - 1)]; };   // one beam's behind the other's
-  auto look = [&](int i, float2 e) {               // candidate i
-    const int k = i / M;
-    cand x = {-INFINITY, (int64_t)k << 32 | (i - k * M)};
-    if (i < all && e.x > -INFINITY) x.c = norms[k][2] + (((double)e.x - norms[k][0]) - norms[k][1]);
+  // the candidates of a thread, SELECT_THREADS behind each other: beam and place in its list
+  const uint32_t k0 = tid / M, p0 = tid - k0 * M, dk = SELECT_THREADS / M, dp = SELECT_THREADS - dk * M;
+  struct spot {
+    uint32_t k, p;
+  };
+  auto next = [&](spot& x) {
+    x.k += dk;
+    x.p += dp;
+    if (x.p >= (uint32_t)M) x.p -= M, ++x.k;
+  };
+  auto look = [&](spot at, float2 e) {
+    cand x = {MERGE_NONE, (uint64_t)at.k << 32 | at.p};
+    if (at.k < (uint32_t)K && e.x > -INFINITY) x.c = merge_order(norms[at.k][2] + (((double)e.x - norms[at.k][0]) - norms[at.k][1]));
     return x;
   };
   float2 mine[EACH];
@@ -508,15 +525,17 @@ __device__ void select_merge(const select_args& a, merge_lds& s, int request) {
   if (tid == 0) held = 0;
   int n;
   if (all <= SELECT_THREADS) {
-    if (tid < all) cands[tid] = look(tid, mine[0]), ranks[tid] = 0;
+    if (tid < all) cands[tid] = look({k0, p0}, mine[0]), ranks[tid] = 0;
     n = all;
   } else {
     uint64_t v[EACH], top = MERGE_NONE;
+    spot at = {k0, p0};
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
       v[i] = MERGE_NONE;
-      if (i * SELECT_THREADS < all) v[i] = merge_order(look(i * SELECT_THREADS + tid, mine[i]).c);
+      if (i * SELECT_THREADS < all) v[i] = look(at, mine[i]).c;
       top = max(top, v[i]);
+      next(at);
     }
     // the best of every 4 threads: the least of these, which 128 candidates reach, and the largest
     for (int o = 1; o < 4; o *= 2) top = max(top, merge_xor(top, o));
@@ -539,52 +558,53 @@ __device__ void select_merge(const select_args& a, merge_lds& s, int request) {
       ++turn;
       return c;
     };
-    uint64_t lo = MERGE_NONE, hi = top + 1;
+    uint64_t lo = least, hi = top + 1, probe = least > MERGE_NONE ? 0 : MERGE_NONE + 1;   // as above
+    int over = 0;
     bool exact = true;
-    if (least > MERGE_NONE || reach(MERGE_NONE + 1) > M) {
-      lo = max(least, MERGE_NONE + 1);
-      while (hi - lo > 1) {
-        const uint64_t mid = lo + (hi - lo) / 2;
-        const int c = reach(mid);
-        if (c >= M) {
-          lo = mid;
-          if (c <= M + M / 2 + 8) {
-            exact = false;
-            break;
-          }
-        } else {
-          hi = mid;
+    while (hi - lo > 1) {
+      const uint64_t mid = probe ? probe : lo + (hi - lo) / 2;
+      const int c = reach(mid);
+      if (c >= M) {
+        lo = mid;
+        if (c <= M + M / 2 + 8) {
+          exact = false;
+          break;
         }
+      } else if (probe) {
+        break;
+      } else {
+        hi = mid;
+        over = c;
       }
+      probe = 0;
     }
     // those above it, and those at it: all where they are few, else the first ones in order
-    auto keep = [&](int i) {
-      const int at = atomicAdd(&held, 1);          // at most M + M / 2 + 8
-      cands[at] = look(i * SELECT_THREADS + tid, mine[i]), ranks[at] = 0;
-    };
-    if (!exact || lo == MERGE_NONE) {
+    exact &= lo > MERGE_NONE;
+    int need = M - over;
+    at = {k0, p0};
+    __syncthreads();
 #pragma unroll
-      for (int i = 0; i < EACH; ++i)
-        if (i * SELECT_THREADS < all && v[i] >= max(lo, MERGE_NONE + 1)) keep(i);
-    } else {
-      int need = M - reach(lo + 1);
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < EACH; ++i) {
-        if (i * SELECT_THREADS >= all) continue;
-        const bool eq = v[i] == lo;
-        const uint64_t mask = __ballot(eq);
-        if (lane == 0) waves[i & 1][wave] = __popcll(mask);
-        __syncthreads();
-        int before = 0, here = 0;
-#pragma unroll
-        for (int w = 0; w < WAVES; ++w) {
-          if (w < wave) before += waves[i & 1][w];
-          here += waves[i & 1][w];
+    for (int i = 0; i < EACH; ++i) {
+      if (i * SELECT_THREADS < all) {
+        bool keep = v[i] >= max(lo, MERGE_NONE + 1);
+        if (exact) {
+          const uint64_t mask = __ballot(v[i] == lo);
+          if (lane == 0) waves[i & 1][wave] = __popcll(mask);
+          __syncthreads();
+          int before = 0, here = 0;
+          for (int w = 0; w < WAVES; ++w) {
+            if (w < wave) before += waves[i & 1][w];
+            here += waves[i & 1][w];
+          }
+          if (v[i] == lo) keep = before + __popcll(mask & (((uint64_t)1 << lane) - 1)) < need;
+          need -= here;
         }
-        if (v[i] > lo || (eq && before + __popcll(mask & (((uint64_t)1 << lane) - 1)) < need)) keep(i);
-        need -= here;
+        if (keep) {
+          const int place = atomicAdd(&held, 1);   // at most M + M / 2 + 8
+          cands[place] = look(at, mine[i]), ranks[place] = 0;
+        }
       }
+      next(at);
     }
     __syncthreads();
     n = held;
@@ -597,23 +617,25 @@ __device__ void select_merge(const select_args& a, merge_lds& s, int request) {
     for (int i = tid / share; i < n; i += SELECT_THREADS / share) {
       const cand e = cands[i];
       int c = 0;
-#pragma unroll 8
+#pragma unroll 4
       for (int j = tid % share; j < n; j += share) c += better(cands[j], e);
       if (c) atomicAdd(&ranks[i], c);
     }
   }
   __syncthreads();
   const int64_t at = (int64_t)request * M;
-  for (int i = tid; i < n; i += SELECT_THREADS) {
-    const cand x = cands[i];
-    if (x.c == -INFINITY) continue;
-    atomicAdd(&held, 1);
-    if (ranks[i] >= M) continue;
-    const int k = (int)(x.at >> 32);
-    const float2 e = lists[k * M + (int)(uint32_t)x.at];
-    a.out_scores[at + ranks[i]] = (float)x.c;
-    a.out_parents[at + ranks[i]] = k;
-    a.out_tokens[at + ranks[i]] = __float_as_int(e.y);
+  if (tid < n) {                                   // (n is SELECT_THREADS at most)
+    const cand x = cands[tid];
+    const bool some = x.c > MERGE_NONE;
+    const uint64_t there = __ballot(some);
+    if (lane == 0) atomicAdd(&held, __popcll(there));
+    if (some && ranks[tid] < M) {
+      const int k = (int)(x.at >> 32);
+      const float2 e = lists[k * M + (int)(uint32_t)x.at];
+      a.out_scores[at + ranks[tid]] = (float)merge_value(x.c);
+      a.out_parents[at + ranks[tid]] = k;
+      a.out_tokens[at + ranks[tid]] = __float_as_int(e.y);
+    }
   }
   __syncthreads();
   for (int i = held + tid; i < M; i += SELECT_THREADS) {
