@@ -9,14 +9,15 @@ Attention's tolerance counts roundings, with h half a step of the element type: 
 multiply V are rounded to the type (h each) and so is their sum (h): 2 h sum p|v|; a score, an fp32 sum of d products,
 by (d + 4) 2^-24 sum|q k| (its weight by that relatively, and the sum of weights again), and the sums over
 the context by 2^-24 a term."""
+import threading
+
 import numpy as np
 import pytest
 import torch
 
 from oracle import beams as oracle
 from test_device_tables import random_state
-from tinybatch_amd import (BeamPlan, DeviceTables, PagedKVCache, beam_attention, build_device_step, ops, reorder_beams,
-                           select_beams)
+from tinybatch_amd import BeamPlan, DeviceTables, beam_attention, build_device_step, ops, reorder_beams, select_beams
 from tinybatch_amd.block_manager import OutOfBlocks
 from tinybatch_amd.metadata import build_step_metadata
 
@@ -426,6 +427,34 @@ def test_reorderings_that_do_not_fit_change_nothing(why):
         t.check()
 
 
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 2 ** 31 - 16, 16 * 9 + 1, -1, -2 ** 31])
+def test_reorder_lengths_that_no_table_holds(length):
+    s = random_state(2, 2, 3, 16, 90, spare=9)
+    t = upload(s, max_blocks=9)
+    storage = torch.randn(1, s.nb, 2, 1, 16, 64, device=DEV)
+    step = t.new_step(padded=1)
+    t.take(build_device_step(t, i32([0] * 6), step))
+    step.context_lens[4] = length
+    keep = [x.clone() for x in (storage, t._buffer[:-64])]
+    reorder_beams(storage, t, i32([[0, 1, 2], [1, 1, 1]]), step)
+    assert torch.equal(storage, keep[0]) and torch.equal(t._buffer[:-64], keep[1])
+    with pytest.raises(ValueError):
+        t.check()
+
+
+@pytest.mark.parametrize("groups,K", [(130, 8), (17, 64), (1100, 1)])
+def test_reorder_and_attention_of_many_rows(groups, K):
+    """More rows than a workgroup has threads."""
+    s = random_state(groups, groups, K, 16, 40, spare=2 * groups * K)
+    g = np.random.default_rng(K)
+    t = upload(s, max_blocks=max(len(x) for x in s.tables) + 1)
+    storage = torch.randn(1, s.nb, 2, 1, 16, 64, device=DEV, dtype=torch.bfloat16)
+    s = check_reorder(s, random_parents(g, groups, K), storage, t)
+    q = torch.randn(groups * K, 2, 64).bfloat16()
+    plan = BeamPlan(t, num_heads=2, num_kv_heads=1, head_dim=64, dtype=torch.bfloat16).build()
+    check_attention(beam_attention(q.to(DEV), storage[0], plan), q, storage[0].cpu(), s.tables, s.lens, 2)
+
+
 def test_reorder_the_tables_alone():
     s = random_state(9, 3, 4, 16, 100, spare=12)
     t = upload(s)
@@ -542,6 +571,139 @@ def test_attention_of_random_states(seed):
     hkv, rep, K = int(g.integers(1, 4)), int(g.choice([1, 2, 3, 5, 7, 8, 12, 33])), int(g.choice([1, 2, 3, 4, 8, 13]))
     s = random_state(seed, int(g.integers(1, 7)), K, int(g.choice([16, 32, 64])), int(g.choice([20, 200, 3000])))
     attend(s, hkv * rep, hkv, d, dtype, seed=seed)
+
+
+# ---- large offsets, graphs, streams, threads -------------------------------------------
+def test_blocks_behind_the_first_4_gb():
+    """The same rows in the last blocks of a pool of 4.8 GB a layer as in a small one: copies, appended rows, attention."""
+    s = random_state(31, 2, 4, 16, 300, spare=16)
+    nb, far = s.nb, 300_000
+    move = lambda ids: [far - 1 - b for b in ids]
+    small = torch.randn(1, nb, 2, 2, 16, 64, device=DEV)
+    big = torch.zeros(1, far, 2, 2, 16, 64, device=DEV)
+    big[0, far - nb:] = small[0].flip(0)
+    q, k, v = (torch.randn(8, h, 64, device=DEV) for h in (4, 2, 2))
+    outs = []
+    for storage, tables, free, blocks in ((small, s.tables, s.free, nb), (big, map(move, s.tables), move(s.free), far)):
+        t = DeviceTables.from_lists(list(tables), s.lens, free, max_blocks=24, block_size=16, num_blocks=blocks, group_size=4, device=DEV)
+        reorder_beams(storage, t, i32([[1, 1, 0, 3], [2, 2, 2, 2]]))
+        step = build_device_step(t, i32([1] * 8), t.new_step(padded=1))
+        ops.kv_append(storage[0], k, v, step.slot_mapping)
+        plan = BeamPlan(t, num_heads=4, num_kv_heads=2, head_dim=64, dtype=torch.float32).build(step.row_ctx)
+        outs.append(beam_attention(q, storage[0], plan))
+        t.check()
+    assert torch.equal(*outs) and torch.equal(big[0, far - nb:].flip(0), small[0]) and not big[0, :far - nb].any()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_select_rows_far_apart(dtype):
+    logits = (torch.randn(6, 5000, device=DEV) * 3).to(dtype)
+    stride = (5 << 30) // logits.element_size() // 5
+    wide = torch.empty(5 * stride + 5000, dtype=dtype, device=DEV).as_strided((6, 5000), (stride, 1))
+    wide.copy_(logits)
+    scores = torch.randn(2, 3, device=DEV)
+    for x, y in zip(select_beams(wide, scores, num_candidates=7), select_beams(logits, scores, num_candidates=7)):
+        assert torch.equal(x, y)
+
+
+class Loop:
+    """A search's step on its own state: run() it, or reset() and run() again."""
+
+    def __init__(self, seed, groups=3, K=4, dtype=torch.bfloat16):
+        g = torch.Generator().manual_seed(seed)
+        self.s = s = random_state(seed, groups, K, 16, 500, spare=3 * groups * K)
+        R, d = groups * K, 64
+        self.t = upload(s, max_blocks=max(len(x) for x in s.tables) + 2)
+        self.storage = torch.randn(2, s.nb, 2, 2, 16, d, generator=g).to(dtype).to(DEV)
+        self.q, self.k, self.v = (torch.randn(R, h, d, generator=g).to(dtype).to(DEV) for h in (6, 2, 2))
+        self.logits = torch.randn(R, 20011, generator=g).to(dtype).to(DEV)
+        self.scores, self.new = (torch.randn(groups, K, generator=g) - 9).to(DEV), i32([1] * R)
+        self.step = self.t.new_step(padded=1)
+        self.plan = BeamPlan(self.t, num_heads=6, num_kv_heads=2, head_dim=d, dtype=dtype)
+        self.state = [self.t._buffer, self.storage]
+        self.start = [x.clone() for x in self.state]
+
+    def reset(self):
+        for x, y in zip(self.state, self.start):
+            x.copy_(y)
+
+    def run(self):
+        build_device_step(self.t, self.new, self.step)
+        self.plan.build(self.step.row_ctx)
+        outs = []
+        for pool in self.storage:
+            ops.kv_append(pool, self.k, self.v, self.step.slot_mapping)
+            outs.append(beam_attention(self.q, pool, self.plan))
+        choice = select_beams(self.logits, self.scores)
+        reorder_beams(self.storage, self.t, choice.parents, self.step)
+        return [*outs, *choice]
+
+    def results(self, outs):
+        return [x.clone() for x in [*outs, *self.state]]
+
+
+def same(a, b):
+    return all(torch.equal(x, y) for x, y in zip(a, b, strict=True))
+
+
+def test_a_whole_step_captured():
+    """Two captured steps, replayed in turn beside eager steps of a third state: each as it runs by itself."""
+    loops = [Loop(1), Loop(2, 5, 2), Loop(3, 1, 9)]
+    want = []
+    for x in loops:
+        outs = x.run()
+        want.append(x.results(outs))
+        x.reset()
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graphs = []
+    for x in loops[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            outs = x.run()
+        graphs.append((graph, outs))
+    for _ in range(3):
+        for x in loops:
+            x.reset()
+        for graph, _ in graphs:
+            graph.replay()
+        third = loops[2].run()
+        torch.cuda.synchronize()
+        for x, outs, w in zip(loops, [graphs[0][1], graphs[1][1], third], want):
+            assert same(x.results(outs), w)
+        torch.randn(1 << 16, device=DEV).sum().item()
+    for x in loops:
+        x.t.check()
+
+
+def test_steps_on_several_streams_and_threads():
+    """Three threads, two of them on one stream: every state goes its own way."""
+    loops = [Loop(4), Loop(5, 5, 2), Loop(6, 1, 9)]
+    want = []
+    for x in loops:
+        want.append([x.results(x.run()) for _ in range(3)])
+        x.reset()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    failed = []
+
+    def work(x, stream, w):
+        try:
+            with torch.cuda.stream(stream):
+                for _ in range(10):
+                    got = [x.results(x.run()) for _ in range(3)]
+                    x.reset()
+                    stream.synchronize()
+                    assert all(same(a, b) for a, b in zip(got, w))
+        except BaseException as e:
+            failed.append(e)
+
+    threads = [threading.Thread(target=work, args=(x, streams[i % 2], w)) for i, (x, w) in enumerate(zip(loops, want))]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join()
+    assert not failed, failed[0]
 
 
 # ---- refusals -------------------------------------------------------------------------

@@ -81,6 +81,7 @@ __global__ __launch_bounds__(1024) void reorder_plan_kernel(const reorder_args a
   __shared__ int lens[1024], parents[1024], fresh[1024];
   __shared__ uint32_t faults;
   const int bs = 1 << a.log2_bs, K = a.beams, tid = threadIdx.x, each = 1024 / K * K;   // rows of whole requests
+  const int room = a.max_nb << a.log2_bs;          // positions of a table
   const int have = a.num_free_in[0];
   if (tid == 0) faults = 0, a.head[2] = 0;
   int base = 0, turn = 0;
@@ -96,14 +97,14 @@ __global__ __launch_bounds__(1024) void reorder_plan_kernel(const reorder_args a
       fresh[tid] = id < 0 || id >= a.num_blocks ? 0 : id;
     }
     __syncthreads();
-    uint32_t bad = old < 0 || (old + bs - 1) >> a.log2_bs > a.max_nb ? TB_TABLES_BAD_LENGTH : 0;
+    uint32_t bad = old < 0 || old > room ? TB_TABLES_BAD_LENGTH : 0;
     bool copy = false;
     int src = -1, ctx = 0, open = -1;
     if (mine && (p < -1 || p >= K)) bad |= TB_TABLES_BAD_PARENT;
     else if (p >= 0) {
       const int g0 = tid / K * K;
       ctx = lens[g0 + p];
-      if (ctx < 0 || (ctx + bs - 1) >> a.log2_bs > a.max_nb) ctx = 0;   // (its own row says so)
+      if (ctx < 0 || ctx > room) ctx = 0;   // (its own row says so)
       if (ctx > 0) src = i0 + g0 + p;
       if (ctx & (bs - 1)) {
         open = a.tables[(int64_t)src * a.max_nb + (ctx >> a.log2_bs)];
