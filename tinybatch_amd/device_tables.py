@@ -85,7 +85,7 @@ class DeviceTables:
     the free blocks. Rows g * group_size .. belong to request g (its beams)."""
 
     def __init__(self, num_rows: int, *, max_blocks: int, block_size: int, num_blocks: int, device,
-                 group_size: int = 1):
+                 group_size: int = 1, _arrays=None):
         device = torch.device(device)
         if device.type != "cuda":
             raise RuntimeError("DeviceTables needs a GPU device (no CPU fallback)")
@@ -94,14 +94,22 @@ class DeviceTables:
         _check_sizes(num_rows, max_blocks, block_size, num_blocks, group_size)
         self.num_rows, self.max_blocks, self.block_size = num_rows, max_blocks, block_size
         self.num_blocks, self.group_size, self.device = num_blocks, group_size, device
-        i32 = dict(dtype=torch.int32, device=device)
-        self._counted = torch.zeros(num_rows + 1, **i32)
+        # one buffer, so that a state from lists is one copy; each array begins at a multiple of 256 bytes
+        sizes = (num_rows + 1, num_rows * max_blocks, num_blocks, num_blocks, num_rows // group_size, 1)
+        begins = np.cumsum([0] + [-(-n // 64) * 64 for n in sizes]).tolist()
+        if _arrays is None:
+            self._buffer = torch.zeros(begins[-1], dtype=torch.int32, device=device)
+        else:
+            host = np.zeros(begins[-1], np.int32)
+            for at, x in zip(begins, _arrays):
+                host[at:at + x.size] = x.reshape(-1)
+            self._buffer = torch.from_numpy(host).to(device)
+        parts = [self._buffer[at:at + n] for at, n in zip(begins, sizes)]
+        self._counted, self.ref_counts, self.free_blocks, self.shared_blocks, self.status = parts[0], *parts[2:]
         self.context_lens, self.num_free = self._counted[:num_rows], self._counted[num_rows:]
-        self.block_tables = torch.full((num_rows, max_blocks), -1, **i32)
-        self.ref_counts = torch.zeros(num_blocks, **i32)
-        self.free_blocks = torch.zeros(num_blocks, **i32)
-        self.shared_blocks = torch.zeros(num_rows // group_size, **i32)
-        self.status = torch.zeros(1, **i32)
+        self.block_tables = parts[1].view(num_rows, max_blocks)
+        if _arrays is None:
+            self.block_tables.fill_(-1)
 
     @classmethod
     def from_lists(cls, block_tables, context_lens, free_blocks, *, max_blocks: int, block_size: int, num_blocks: int,
@@ -112,11 +120,8 @@ class DeviceTables:
         cache), once for every holder."""
         rows = len(block_tables)
         arrays = _state_arrays(block_tables, context_lens, free_blocks, max_blocks, block_size, num_blocks, group_size, held)
-        self = cls(rows, max_blocks=max_blocks, block_size=block_size, num_blocks=num_blocks, device=device,
-                   group_size=group_size)
-        for to, x in zip((self._counted, self.block_tables, self.ref_counts, self.free_blocks, self.shared_blocks), arrays):
-            to.copy_(torch.from_numpy(x))
-        return self
+        return cls(rows, max_blocks=max_blocks, block_size=block_size, num_blocks=num_blocks, device=device,
+                   group_size=group_size, _arrays=arrays)
 
     def new_step(self, *, max_tokens: int | None = None, padded: int = 0, partition_tokens: int = 0,
                  rows_per_item: int = 1, max_items: int | None = None, max_partitions: int | None = None,
@@ -191,40 +196,38 @@ def _state_arrays(block_tables, context_lens, free_blocks, max_blocks, block_siz
     _check_sizes(rows, max_blocks, block_size, num_blocks, group_size)
     if len(context_lens) != rows:
         raise ValueError("block_tables and context_lens need one entry per row")
+    lens = np.fromiter(context_lens, np.int64, rows)
+    if rows and lens.min() < 0:
+        raise ValueError(f"context_lens[{int(lens.argmin())}] is {lens.min()}")
+    need, have = -(-lens // block_size), np.fromiter(map(len, block_tables), np.int64, rows)
+    if (need > max_blocks).any():
+        b = int(np.argmax(need > max_blocks))
+        raise IndexError(f"row {b} needs {need[b]} blocks, its table holds {max_blocks}")
+    if (have < need).any():
+        b = int(np.argmax(have < need))
+        raise IndexError(f"row {b} needs {need[b]} blocks for {lens[b]} positions, table has {have[b]}")
+    used = block_tables if (have == need).all() else [t[:n] for t, n in zip(block_tables, need)]
     tables = np.full((rows, max_blocks), -1, dtype=np.int32)
-    refs = np.zeros(num_blocks, dtype=np.int64)
-    ids = lambda name, x: _ids(name, x, num_blocks)
-    for b, (t, n) in enumerate(zip(block_tables, context_lens)):
-        if n < 0:
-            raise ValueError(f"context_lens[{b}] is {n}")
-        need = -(-n // block_size)
-        if need > max_blocks:
-            raise IndexError(f"row {b} needs {need} blocks, its table holds {max_blocks}")
-        if len(t) < need:
-            raise IndexError(f"row {b} needs {need} blocks for {n} positions, table has {len(t)}")
-        tables[b, :need] = ids(f"block_tables[{b}]", t[:need])
-    inside = np.arange(max_blocks) < (-(-np.asarray(list(context_lens), dtype=np.int64) // block_size))[:, None]
-    np.add.at(refs, tables[inside], 1)
-    np.add.at(refs, ids("held", held), 1)
-    free = ids("free_blocks", free_blocks)
-    if np.unique(free).size != free.size or (refs[free] > 0).any():
+    ids = _ids("block_tables", itertools.chain.from_iterable(used), num_blocks)
+    tables[np.arange(max_blocks) < need[:, None]] = ids
+    refs = np.bincount(ids, minlength=num_blocks) + np.bincount(_ids("held", held, num_blocks), minlength=num_blocks)
+    free = _ids("free_blocks", free_blocks, num_blocks)
+    if free.size and (np.bincount(free).max() > 1 or (refs[free] > 0).any()):
         raise ValueError("free_blocks must be distinct blocks that no row holds")
-    counted = np.zeros(rows + 1, dtype=np.int32)
-    counted[:rows], counted[rows] = list(context_lens), free.size
-    stack = np.zeros(num_blocks, dtype=np.int32)
-    stack[:free.size] = free
-    shared = np.zeros(rows // group_size, dtype=np.int32)
-    for g in range(rows // group_size):
-        live = [b for b in range(g * group_size, (g + 1) * group_size) if context_lens[b] > 0]
-        if live:
-            n = min(context_lens[b] for b in live) // block_size
-            same = (tables[live, :n] == tables[live[0], :n]).all(0)
-            shared[g] = n if same.all() else int(np.argmin(same))
-    return counted, tables, refs.astype(np.int32), stack, shared
+    counted, stack = np.zeros(rows + 1, dtype=np.int32), np.zeros(num_blocks, dtype=np.int32)
+    counted[:rows], counted[rows], stack[:free.size] = lens, free.size, free
+    # leading whole blocks that the rows of a group with positions have in common
+    groups = tables.reshape(rows // group_size, group_size, max_blocks)
+    live = (lens > 0).reshape(rows // group_size, group_size)
+    first = groups[np.arange(groups.shape[0]), live.argmax(1)]
+    whole = np.where(live, lens.reshape(rows // group_size, group_size) // block_size, max_blocks).min(1, initial=max_blocks)
+    agree = ((groups == first[:, None]) | ~live[:, :, None]).all(1) & (np.arange(max_blocks) < whole[:, None])
+    shared = np.where(live.any(1), np.cumprod(agree, axis=1).sum(1), 0)
+    return counted, tables, refs.astype(np.int32), stack, shared.astype(np.int32)
 
 
 def _ids(name: str, x, num_blocks: int) -> np.ndarray:
-    a = np.asarray(list(itertools.islice(x, None)), dtype=np.int64).reshape(-1)
+    a = np.fromiter(x, np.int64)
     if a.size and (a.min() < 0 or a.max() >= num_blocks):
         raise IndexError(f"{name} holds a block id outside [0, {num_blocks})")
     return a
