@@ -119,18 +119,17 @@ def reorder_beams(storage: torch.Tensor | None, tables: DeviceTables, parents: t
     if _elsewhere(device):
         with torch.cuda.device(device):
             return reorder_beams(storage, tables, parents, step)
-    now = tables if step is None else step
+    p = tables._ptr
+    lens, free = (p["context_lens"], p["num_free"]) if step is None else step._args[2:4]
     L, stream = _lib.lib(), _lib.stream_handle(device)
     need = L.tb_beam_reorder_workspace_bytes(tables.num_rows, K, tables.max_blocks)
     lock, ws, ws_bytes, _, _ = _scratch(device, stream, need, 0)
     try:
         st = L.tb_beam_reorder(
             None if storage is None else storage.data_ptr(), layers, stride, tables.num_blocks, hkv, d,
-            tables.block_size, dtype, tables.block_tables.data_ptr(), tables.max_blocks, tables.num_rows, K,
-            now.context_lens.data_ptr(), tables.context_lens.data_ptr(), tables.ref_counts.data_ptr(),
-            tables.free_blocks.data_ptr(), now.num_free.data_ptr(), tables.num_free.data_ptr(),
-            tables.shared_blocks.data_ptr(), parents.data_ptr(), tables.status.data_ptr(), ws.data_ptr(), ws_bytes,
-            stream)
+            tables.block_size, dtype, p["block_tables"], tables.max_blocks, tables.num_rows, K, lens, p["context_lens"],
+            p["ref_counts"], p["free_blocks"], free, p["num_free"], p["shared_blocks"], parents.data_ptr(), p["status"],
+            ws.data_ptr(), ws_bytes, stream)
     finally:
         lock.release()
     _lib.check(st, "tb_beam_reorder")
@@ -157,20 +156,25 @@ class BeamPlan:
         sizes = (tables.num_rows, tables.group_size, num_heads, num_kv_heads, head_dim, _lib.DTYPE_CODE[dtype])
         self.buffer = torch.zeros(max(16, L.tb_beam_plan_bytes(*sizes)), dtype=torch.uint8, device=tables.device)
         self.workspace_bytes = L.tb_beam_attention_workspace_bytes(*sizes)
+        # of the usual call, once: a call is as short as its launches
+        self._pool_shape = (tables.num_blocks, 2, num_kv_heads, tables.block_size, head_dim)
+        self._q_shape = (tables.num_rows, num_heads, head_dim)
+        self._scale, self._dtype_code = 1.0 / math.sqrt(head_dim), _lib.DTYPE_CODE[dtype]
+        self._ptr, self._bytes = self.buffer.data_ptr(), self.buffer.numel()
 
     def build(self, row_ctx: torch.Tensor | None = None) -> "BeamPlan":
         """The plan for rows that see row_ctx [rows] int32 positions (0: none): a step's row_ctx
         (DeviceTables.new_step(padded=1)), by default the tables' lengths."""
         t = self.tables
-        row_ctx = t.context_lens if row_ctx is None else row_ctx
+        if row_ctx is None:
+            row_ctx = t.context_lens
         _ints("row_ctx", row_ctx, torch.int32, (t.num_rows,), t.device)
         if _elsewhere(t.device):
             with torch.cuda.device(t.device):
                 return self.build(row_ctx)
-        st = _lib.lib().tb_beam_plan(row_ctx.data_ptr(), t.shared_blocks.data_ptr(), t.num_rows, t.group_size,
+        st = _lib.lib().tb_beam_plan(row_ctx.data_ptr(), t._ptr["shared_blocks"], t.num_rows, t.group_size,
                                      t.max_blocks, self.num_heads, self.num_kv_heads, self.head_dim, t.block_size,
-                                     _lib.DTYPE_CODE[self.dtype], self.buffer.data_ptr(), self.buffer.numel(),
-                                     _lib.stream_handle(t.device))
+                                     self._dtype_code, self._ptr, self._bytes, _lib.stream_handle(t.device))
         _lib.check(st, "tb_beam_plan")
         self.built = True
         return self
@@ -184,6 +188,37 @@ def beam_attention(q: torch.Tensor, pool: torch.Tensor, plan: BeamPlan, *, scale
 
     q: [rows, num_heads, head_dim] (after rotation) in the pool's dtype; returns [rows, num_heads *
     head_dim]. ``scale``: 1 / sqrt(head_dim) by default. A row that sees nothing gives 0."""
+    device, dtype, t, hq, d, R = pool.device, plan.dtype, plan.tables, plan.num_heads, plan.head_dim, plan.tables.num_rows
+    if not plan.built:
+        raise ValueError("the plan has not been built (BeamPlan.build)")
+    nb, qs, os_ = t.num_blocks, hq * d, hq * d
+    if not (pool.shape == plan._pool_shape and q.shape == plan._q_shape and device == t.device == q.device
+            and pool.dtype == q.dtype == dtype and pool.is_contiguous() and q.is_contiguous()):
+        nb, qs = _check_attention(q, pool, plan)   # (what is not as usual)
+    if out is not None:
+        if out.dtype != dtype or out.shape[0] != R or out.device != device:
+            raise ValueError("out must match q's dtype, device and row count")
+        os_ = _rows_view("out", out, hq, d)
+    if _elsewhere(device):
+        with torch.cuda.device(device):
+            return beam_attention(q, pool, plan, scale=scale, out=out)
+    if out is None:
+        out = torch.empty(R, hq * d, device=device, dtype=dtype)
+    stream = _lib.stream_handle(device)
+    lock, ws, ws_bytes, _, _ = _scratch(device, stream, plan.workspace_bytes, 0)
+    try:
+        st = _lib.lib().tb_beam_attention(
+            q.data_ptr(), qs, pool.data_ptr(), nb, out.data_ptr(), os_, t._ptr["block_tables"], t.max_blocks, R,
+            t.group_size, hq, plan.num_kv_heads, d, t.block_size, plan._scale if scale is None else float(scale),
+            plan._dtype_code, plan._ptr, plan._bytes, ws.data_ptr(), ws_bytes, stream)
+    finally:
+        lock.release()
+    _lib.check(st, "tb_beam_attention")
+    return out
+
+
+def _check_attention(q: torch.Tensor, pool: torch.Tensor, plan: BeamPlan) -> tuple[int, int]:
+    """The pool's blocks and q's row stride, where both may serve the plan."""
     nb, hkv, bs, d = _check_pool(pool)
     device, dtype, t = pool.device, pool.dtype, plan.tables
     if q.device != device:
@@ -191,34 +226,12 @@ def beam_attention(q: torch.Tensor, pool: torch.Tensor, plan: BeamPlan, *, scale
         raise ValueError(f"q is on {q.device}, the pool on {device}")
     if t.device != device:
         raise ValueError(f"the plan is on {t.device}, the pool on {device}")
-    if not plan.built:
-        raise ValueError("the plan has not been built (BeamPlan.build)")
     if q.dtype != dtype or plan.dtype != dtype:
         raise TypeError(f"q {q.dtype}, pool {dtype} and plan {plan.dtype} differ in dtype")
     if hkv != plan.num_kv_heads or d != plan.head_dim or bs != t.block_size or nb < t.num_blocks:
         raise ValueError(f"the plan is for {t.num_blocks} blocks of {t.block_size} positions, {plan.num_kv_heads} kv heads "
                          f"of {plan.head_dim}; the pool is {tuple(pool.shape)}")
-    if _elsewhere(device):
-        with torch.cuda.device(device):
-            return beam_attention(q, pool, plan, scale=scale, out=out)
-    hq, R = plan.num_heads, t.num_rows
-    qs = _rows_view("q", q, hq, d)
-    if q.shape[0] != R:
-        raise ValueError(f"q has {q.shape[0]} rows, the tables {R}")
-    if out is None:
-        out, os_ = torch.empty(R, hq * d, device=device, dtype=dtype), hq * d
-    else:
-        if out.dtype != dtype or out.shape[0] != R or out.device != device:
-            raise ValueError("out must match q's dtype, device and row count")
-        os_ = _rows_view("out", out, hq, d)
-    stream = _lib.stream_handle(device)
-    lock, ws, ws_bytes, _, _ = _scratch(device, stream, plan.workspace_bytes, 0)
-    try:
-        st = _lib.lib().tb_beam_attention(
-            q.data_ptr(), qs, pool.data_ptr(), nb, out.data_ptr(), os_, t.block_tables.data_ptr(), t.max_blocks, R,
-            t.group_size, hq, hkv, d, bs, 1.0 / math.sqrt(d) if scale is None else float(scale), _lib.DTYPE_CODE[dtype],
-            plan.buffer.data_ptr(), plan.buffer.numel(), ws.data_ptr(), ws_bytes, stream)
-    finally:
-        lock.release()
-    _lib.check(st, "tb_beam_attention")
-    return out
+    qs = _rows_view("q", q, plan.num_heads, d)
+    if q.shape[0] != t.num_rows:
+        raise ValueError(f"q has {q.shape[0]} rows, the tables {t.num_rows}")
+    return nb, qs

@@ -41,7 +41,7 @@ def _ints(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: 
 @dataclass
 class DeviceStep:
     """One step's arrays on the GPU (tb_device_step), allocated once (DeviceTables.new_step) and
-    filled by build_device_step."""
+    filled by build_device_step: they may be written to, not replaced."""
     max_tokens: int
     padded: int                        # > 0: row b's tokens are the flat rows from b * padded on
     partition_tokens: int              # 0: no work items
@@ -58,6 +58,7 @@ class DeviceStep:
     counts: torch.Tensor | None = None             # [4] int32: items, split rows, 0, partitions
     max_partitions: int = 0
     _counted: torch.Tensor | None = field(default=None, repr=False)   # context_lens and num_free, one behind the other
+    _args: tuple = field(default=(), repr=False)   # tb_device_step's arguments from pad_tokens to counts
 
     def metadata(self, tables: "DeviceTables") -> StepMetadata:
         """The step as ops.paged_attention and ops.kv_append take it: the arrays above, sized to their
@@ -82,7 +83,8 @@ class DeviceStep:
 
 class DeviceTables:
     """The paged state of ``num_rows`` rows on the GPU: block tables, lengths, reference counts and
-    the free blocks. Rows g * group_size .. belong to request g (its beams)."""
+    the free blocks. Rows g * group_size .. belong to request g (its beams). Its arrays are allocated
+    once: they may be written to, not replaced."""
 
     def __init__(self, num_rows: int, *, max_blocks: int, block_size: int, num_blocks: int, device,
                  group_size: int = 1, _arrays=None):
@@ -110,6 +112,9 @@ class DeviceTables:
         self.block_tables = parts[1].view(num_rows, max_blocks)
         if _arrays is None:
             self.block_tables.fill_(-1)
+        # addresses, taken once: a step's calls are short, and every data_ptr() is a part of them
+        self._ptr = {name: getattr(self, name).data_ptr() for name in
+                     ("block_tables", "context_lens", "num_free", "ref_counts", "free_blocks", "shared_blocks", "status")}
 
     @classmethod
     def from_lists(cls, block_tables, context_lens, free_blocks, *, max_blocks: int, block_size: int, num_blocks: int,
@@ -154,6 +159,12 @@ class DeviceTables:
             s.work_items, s.split_rows = torch.zeros(sizes[0], 4, **i32), torch.zeros(sizes[2], 4, **i32)
             s.max_partitions = sizes[1]
             s.counts = torch.zeros(4, **i32)
+        ptr = lambda t: None if t is None else t.data_ptr()
+        entries = lambda t: 0 if t is None else t.shape[0]
+        s._args = (padded, max_tokens, s.context_lens.data_ptr(), s.num_free.data_ptr(), s.query_start_loc.data_ptr(),
+                   s.positions.data_ptr(), s.slot_mapping.data_ptr(), s.row_ctx.data_ptr(), partition_tokens, rows_per_item,
+                   ptr(s.row_part_offsets), ptr(s.work_items), entries(s.work_items), s.max_partitions, ptr(s.split_rows),
+                   entries(s.split_rows), ptr(s.counts))
         return s
 
     def take(self, step: DeviceStep) -> None:
@@ -238,30 +249,22 @@ def build_device_step(tables: DeviceTables, new_lens: torch.Tensor, step: Device
     are taken from the free blocks, and the step's arrays are filled (tb_device_step). ``tables`` keeps
     its lengths and free blocks until tables.take(step) or reorder_beams(..., step=step), so a step may be
     built again. Where something does not fit the step is empty (tables.check() raises)."""
-    device = tables.device
-    _ints("new_lens", new_lens, torch.int32, (tables.num_rows,), device)
-    if step.context_lens.device != device or step.context_lens.shape[0] != tables.num_rows:
+    device, rows = tables.device, tables.num_rows
+    _ints("new_lens", new_lens, torch.int32, (rows,), device)
+    if step.context_lens.device != device or step.context_lens.shape[0] != rows:
         raise ValueError("the step was made for other tables (DeviceTables.new_step)")
     if _elsewhere(device):
         with torch.cuda.device(device):
             return build_device_step(tables, new_lens, step)
-    L, stream = _lib.lib(), _lib.stream_handle(device)
-    need = L.tb_device_step_workspace_bytes(tables.num_rows)
+    L, stream, p = _lib.lib(), _lib.stream_handle(device), tables._ptr
+    need = L.tb_device_step_workspace_bytes(rows)
     lock = ws = None
     if need:
         lock, ws, _, _, _ = _scratch(device, stream, need, 0)
-    ptr = lambda t: None if t is None else t.data_ptr()
-    items, split = step.work_items, step.split_rows
     try:
-        st = L.tb_device_step(
-            tables.block_tables.data_ptr(), tables.max_blocks, tables.context_lens.data_ptr(), new_lens.data_ptr(),
-            tables.num_rows, tables.ref_counts.data_ptr(), tables.free_blocks.data_ptr(), tables.num_free.data_ptr(),
-            tables.num_blocks, tables.block_size, step.padded, step.max_tokens, step.context_lens.data_ptr(),
-            step.num_free.data_ptr(), step.query_start_loc.data_ptr(), step.positions.data_ptr(),
-            step.slot_mapping.data_ptr(), step.row_ctx.data_ptr(), step.partition_tokens, step.rows_per_item,
-            ptr(step.row_part_offsets), ptr(items), 0 if items is None else items.shape[0], step.max_partitions,
-            ptr(split), 0 if split is None else split.shape[0], ptr(step.counts), tables.status.data_ptr(),
-            ptr(ws), need, stream)
+        st = L.tb_device_step(p["block_tables"], tables.max_blocks, p["context_lens"], new_lens.data_ptr(), rows,
+                              p["ref_counts"], p["free_blocks"], p["num_free"], tables.num_blocks, tables.block_size,
+                              *step._args, p["status"], None if ws is None else ws.data_ptr(), need, stream)
     finally:
         if lock is not None:
             lock.release()

@@ -267,8 +267,9 @@ class _Scratch:
 
     def __init__(self, device: torch.device):
         self.lock = threading.RLock()
-        self.workspace = torch.empty(1 << 20, dtype=torch.uint8, device=device)
-        self.arrivals = torch.zeros(4096, dtype=torch.int32, device=device)
+        self.bytes, self.units = 1 << 20, 4096
+        self.workspace = torch.empty(self.bytes, dtype=torch.uint8, device=device)
+        self.arrivals = torch.zeros(self.units, dtype=torch.int32, device=device)
 
 
 _SCRATCH: dict[tuple[int, int], _Scratch] = {}
@@ -290,12 +291,14 @@ def _scratch(device: torch.device, stream: int, nbytes: int, units: int):
             s = _SCRATCH.setdefault((device.index, stream), _Scratch(device))
     s.lock.acquire()
     try:
-        if s.arrivals.shape[0] < units:
+        if s.units < units:
             s.arrivals = torch.zeros(2 * units, dtype=torch.int32, device=device)
+            s.units = 2 * units
         if nbytes > _KEPT_BYTES:
             return s.lock, torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes, s.arrivals, units
-        if s.workspace.shape[0] < nbytes:
+        if s.bytes < nbytes:
             s.workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+            s.bytes = nbytes
     except BaseException:
         s.lock.release()
         raise
