@@ -281,6 +281,31 @@ def test_select_masked_and_special_logits(dtype):
         check_select(x[rows].clone(), torch.zeros(1, len(rows)), 12)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("few", [-1000.0, "lowest", 60000.0, 3e38])
+def test_select_of_few_far_logits(few, dtype):
+    """Runs of -inf alone in rows of few logits, which lie far from 0, or on both sides of where the terms change form."""
+    few = torch.finfo(dtype).min if few == "lowest" else min(few, torch.finfo(dtype).max)
+    x = torch.full((4, 40_000), -float("inf"), dtype=dtype)
+    x[:, 39_000], x[:, 39_990] = few, few
+    x[1, 7::1000] = 3.0
+    x[2, 20_000:20_600] = 65_500.0 + torch.arange(600).to(dtype)
+    x[3] = few
+    for rows in ([0], [1], [2], [3], [0, 1, 2, 3]):
+        check_select(x[rows].clone(), torch.zeros(1, len(rows)), 12)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [5000, 151936])
+def test_select_rising_rows(V, dtype):
+    """Every tile's largest logit above the last one's: the reference moves again and again, at every size of logits."""
+    g = torch.Generator().manual_seed(V)
+    x = torch.stack([torch.arange(V) * by for by in (1e-4, 0.01, 0.4, 100.0)]) + torch.randn(4, V, generator=g)
+    x = torch.cat([x, -x.flip(1)]).clamp(-60000, 60000).to(dtype)
+    for rows in range(8):
+        check_select(x[rows:rows + 1], torch.zeros(1, 1), 9)
+
+
 def test_select_long_rows_of_small_terms():
     """A flat row of many tokens: the sum's terms are as good as equal, nothing of it is lost."""
     x = torch.full((2, 1_000_003), -5.0)

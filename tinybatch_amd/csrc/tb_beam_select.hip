@@ -20,8 +20,7 @@
 
 namespace tb {
 
-constexpr int SELECT_TILE = 512;                   // tokens: 8 a lane
-constexpr int SELECT_AHEAD = 4;                    // tiles that a wave loads ahead, times the bytes of a token
+constexpr int SELECT_LANE = 32, SELECT_TILE = 64 * SELECT_LANE;   // bytes of a lane and a wave at a time
 constexpr int SELECT_SEGMENTS = 1024;              // of a row, at most
 constexpr int SELECT_THREADS = 512;
 constexpr int SELECT_LIST = 2048;                  // tokens from the threshold up that part 2 keeps in LDS
@@ -41,11 +40,11 @@ struct select_args {
   int32_t* out_parents;
   int64_t* out_tokens;
   int32_t tiles, runs, per_run;   // tiles of a row, runs of a row, tiles of a run
-  int32_t log2_lanes;          // lanes of a segment inside a tile: 2^log2_lanes
+  int32_t log2_lanes;          // 8 tokens 2^log2_lanes times: a segment, or the part of one in a tile
   int32_t tops;                // segment maxima that part 1 writes per row
   int32_t join, segments;      // of them in a segment (1 unless a segment is several tiles), segments of a row
   float* seg_max;              // [rows][tops]
-  double2* sums;               // [rows][runs]: {S, r}
+  double2* sums;               // [rows][runs]: {S, r}, r -inf where nothing counts
   double2* norms;              // [rows]: {m, log S}
   float2* lists;               // [rows][M]: {x, token}, best first, then -inf
 };
@@ -70,21 +69,23 @@ __device__ __forceinline__ eight_logits<T> select_load(const char* row, int t0, 
   return e;
 }
 
-// Maximum over aligned groups of 2^N lanes, of numbers and infinities.
-template <int CTRL>
-__device__ __forceinline__ float max_dpp(float x) {   // (every lane has a partner: the move folds into the maximum)
-  return max_f32(x, __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(x), CTRL, 0xf, 0xf, true)));
-}
+// Maximum over aligned groups of 2^N lanes, of numbers and infinities. (One instruction a step: the compiler makes a move
+// and a three-operand maximum of it. A DPP source needs two wait states behind its writer.)
+#define SELECT_MAX_DPP(CTRL) \
+  asm("s_nop 1\n\tv_max_f32_dpp %0, %1, %1 " CTRL " row_mask:0xf bank_mask:0xf" : "=v"(y) : "v"(x)); \
+  x = y
 template <int N>
 __device__ __forceinline__ float lanes_max(float x) {
-  if constexpr (N >= 1) x = max_dpp<DPP_QUAD_XOR1>(x);
-  if constexpr (N >= 2) x = max_dpp<DPP_QUAD_XOR2>(x);
-  if constexpr (N >= 3) x = max_dpp<DPP_ROW_HALF_MIRROR>(x);
-  if constexpr (N >= 4) x = max_dpp<DPP_ROW_MIRROR>(x);
+  float y;
+  if constexpr (N >= 1) { SELECT_MAX_DPP("quad_perm:[1,0,3,2]"); }
+  if constexpr (N >= 2) { SELECT_MAX_DPP("quad_perm:[2,3,0,1]"); }
+  if constexpr (N >= 3) { SELECT_MAX_DPP("row_half_mirror"); }
+  if constexpr (N >= 4) { SELECT_MAX_DPP("row_mirror"); }
   if constexpr (N >= 5) x = max_xor16(x);
   if constexpr (N >= 6) x = max_xor32(x);
   return x;
 }
+#undef SELECT_MAX_DPP
 
 // Sum over the wave's lanes, in every lane.
 __device__ __forceinline__ double lanes_sum(double x) {
@@ -108,75 +109,97 @@ __device__ __forceinline__ double lanes_sum(double x) {
   return x;
 }
 
-// One wave's run of a row whose logits count.
+// One wave's run of a row whose logits count: tiles of 2048 bytes, 32 a lane. Terms are 2^(x l - c) with l = log2(e) and c = r l, both
+// as floats, in one fused product each; what c lost is in the term of x = r as well, and the sum is divided by it: a row of
+// one token sums to 1 exactly. From |r| = 2^16 on, where c could lose as much as the terms' size, they are 2^((x - r) l) (floats
+// that far out differ by 0 or by more than counts, nearly).
 template <typename T, int LANES>                   // 2^LANES lanes of a segment
 __device__ __forceinline__ void select_run(const select_args& a, int row, int run, int lane) {
+  constexpr int U = SELECT_LANE / sizeof(T), TILE = 64 * U, PER = 64 >> LANES;
+  constexpr float LOG2E = 1.44269504088896f, FAR = 0x1p16f;
+  constexpr float MOST = 50.f;                     // of a lane's terms: the reference moves when a logit outgrows it by log 50 at most
   const char* const at = a.logits + (int64_t)row * a.row_bytes;
-  const int first = run * a.per_run, last = min(first + a.per_run, a.tiles), whole = min(last, a.vocab / SELECT_TILE);
-  constexpr int PER = 64 >> LANES;
+  const int first = run * a.per_run, last = min(first + a.per_run, a.tiles), whole = min(last, a.vocab / TILE);
   const bool tells = (lane & ((1 << LANES) - 1)) == 0;
   float* const tops = a.seg_max + (int64_t)row * a.tops;
-  // the wave's reference, moved where a logit outgrows it by 1
-  float ref = 0.f, limit = -INFINITY;              // limit: ref + 1, -inf before there is one
-  double sum = 0.;
-  auto add = [&](int t, const eight_logits<T>& e) {
-    float x[8];
+  float ref = -INFINITY, shift = NAN, unit = 1.f;   // r; -c, NaN: none or far; the term of x = r
+  double sum = 0.;                                 // in units
+  auto move = [&](float r) {
+    const float c = r * LOG2E, was = unit;
+    const bool near = fabsf(r) < FAR;
+    shift = near ? -c : NAN;
+    unit = near ? fast_exp2(fmaf(r, LOG2E, shift)) : 1.f;
+    if (sum > 0.) sum *= exp((double)ref - (double)r) * ((double)unit / (double)was);
+    ref = r;
+  };
+  auto most = [](const float(&x)[U]) {
+    float top = fmaxf(x[0], x[1]);                 // (a NaN loses against a number)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = (float)e.v[i];
-    float top = x[0];
+    for (int i = 2; i < U; ++i) top = fmaxf(top, x[i]);
+    return top;
+  };
+  auto add_up = [](auto&& term) {
+    float part[2] = {term(0), term(1)};
 #pragma unroll
-    for (int i = 1; i < 8; ++i) top = fmaxf(top, x[i]);   // (a NaN loses against a number)
-    auto terms = [&] {
-      float part[2] = {0.f, 0.f};
+    for (int i = 2; i < U; ++i) part[i & 1] += term(i);
+    return part[0] + part[1];
+  };
+  auto add = [&](int t, float(&x)[U]) {
+    float top = most(x);
+    float part = add_up([&](int i) { return fast_exp2(fmaf(x[i], LOG2E, shift)); });
+    if (__any(!(part <= MOST))) {                  // a logit outgrew the reference, or is none, or there is no reference
 #pragma unroll
-      for (int i = 0; i < 8; ++i) part[i & 1] += fast_exp2((x[i] - ref) * 1.44269504088896f);
-      return part[0] + part[1];
-    };
-    float part = 0.f;
-    if (!__any(!(top <= limit))) part = terms();
-    if (__any(!(top <= limit) || part != part)) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = select_logit(x[i]);
+      for (int i = 0; i < U; ++i) x[i] = select_logit(x[i]);
       top = select_logit(top);
       const float r = lanes_max<6>(top);
-      if (r > limit) {
-        if (limit > -INFINITY) sum *= exp((double)ref - (double)r);
-        ref = r;
-        limit = r + 1.f;
-      }
-      part = limit > -INFINITY ? terms() : 0.f;
+      if (r > ref) move(r);
+      part = 0.f;
+      if (shift == shift) part = add_up([&](int i) { return fast_exp2(fmaf(x[i], LOG2E, shift)); });
+      else if (ref > -INFINITY) part = add_up([&](int i) { return fast_exp2((x[i] - ref) * LOG2E); });
     }
     sum += (double)part;
     top = lanes_max<LANES>(top);
     if (tells && t * PER + (lane >> LANES) < a.tops) tops[t * PER + (lane >> LANES)] = top;
   };
-  // whole tiles, B loaded while the B before are added up; the row's last, partial one by itself
-  constexpr int B = SELECT_AHEAD / sizeof(T);
+  // whole tiles, the next one on its way while one is added up; the row's last, partial one by itself
   struct __attribute__((packed, aligned(sizeof(T)))) raw_t {
-    uint32_t w[2 * sizeof(T)];
+    T v[U];
   };
-  raw_t next[B];
-  const uint32_t mine = 8 * lane * sizeof(T);
+  raw_t next;
   auto fetch = [&](int t) {
-#pragma unroll
-    for (int u = 0; u < B; ++u) {                  // (past the run: its last tile again)
-      const char* const tile = at + (int64_t)min(t + u, whole - 1) * (int64_t)(SELECT_TILE * sizeof(T));
-      next[u] = *reinterpret_cast<const raw_t*>(tile + mine);
-    }
+    next = *reinterpret_cast<const raw_t*>(at + (int64_t)t * SELECT_TILE + SELECT_LANE * lane);
   };
-  if (first < whole) fetch(first);
-  for (int t0 = first; t0 < whole; t0 += B) {
-    raw_t now[B];
+  auto take = [&](float(&x)[U]) {
 #pragma unroll
-    for (int u = 0; u < B; ++u) now[u] = next[u];
-    if (t0 + B < whole) fetch(t0 + B);
+    for (int i = 0; i < U; ++i) x[i] = (float)next.v[i];
 #pragma unroll
-    for (int u = 0; u < B; ++u)
-      if (t0 + u < whole) add(t0 + u, __builtin_bit_cast(eight_logits<T>, now[u]));
+    for (int i = 0; i < U; ++i) asm volatile("" : "+v"(x[i]));   // (taken before the next load goes to the same registers)
+  };
+  if (first < whole) {
+    fetch(first);
+    float x[U];
+    take(x);
+    const float r = lanes_max<6>(most(x));
+    if (fabsf(r) < FAR) move(r);
   }
-  if (whole < last) add(whole, select_load<T>(at, whole * SELECT_TILE + 8 * lane, a.vocab));
+  for (int t = first; t < whole; ++t) {
+    float x[U];
+    take(x);
+    if (t + 1 < whole) fetch(t + 1);
+    add(t, x);
+  }
+  if (whole < last) {
+    float x[U];
+    const int t0 = whole * TILE + U * lane;
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      x[i] = (float)reinterpret_cast<const T*>(at)[min(t0 + i, a.vocab - 1)];
+      if (t0 + i >= a.vocab) x[i] = -INFINITY;
+    }
+    add(whole, x);
+  }
   sum = lanes_sum(sum);
-  if (lane == 0) a.sums[(int64_t)row * a.runs + run] = make_double2(sum, (double)ref);
+  if (lane == 0) a.sums[(int64_t)row * a.runs + run] = make_double2(sum / (double)unit, (double)ref);
 }
 
 // A float's place among all floats, -inf 0x007FFFFF; -0 is 0.
@@ -665,13 +688,14 @@ __global__ __launch_bounds__(SELECT_THREADS) void select_merge_kernel(const sele
 struct select_sizes {
   int32_t tiles, runs, per_run, log2_lanes, tops, join, segments;
   size_t norms, lists, maxima, all;                // of the workspace; the sums first
-  select_sizes(int64_t rows, int64_t vocab, int64_t picks) {
-    tiles = (int32_t)((vocab + SELECT_TILE - 1) / SELECT_TILE);
+  select_sizes(int64_t rows, int64_t vocab, int64_t picks, int size) {
+    const int64_t tile = SELECT_TILE / size;
+    tiles = (int32_t)((vocab + tile - 1) / tile);
     // runs that fill the GPU twice
     const int64_t want = (16384 + rows - 1) / rows;
     per_run = (int32_t)((tiles + want - 1) / want);
     runs = (tiles + per_run - 1) / per_run;
-    log2_lanes = 0;
+    log2_lanes = 1;                                // (a lane's 16 tokens of 16 bits)
     while (log2_lanes < 6 && (vocab + (8 << log2_lanes) - 1) / (8 << log2_lanes) > SELECT_SEGMENTS) ++log2_lanes;
     tops = (int32_t)((vocab + (8 << log2_lanes) - 1) / (8 << log2_lanes));
     join = (tops + SELECT_SEGMENTS - 1) / SELECT_SEGMENTS;
@@ -685,8 +709,9 @@ struct select_sizes {
 
 template <typename T, int LANES>
 static void launch_select(const select_args& a, hipStream_t stream) {
-  if constexpr (LANES < 6)
-    if (a.log2_lanes > LANES) return launch_select<T, LANES + 1>(a, stream);
+  constexpr int MORE = sizeof(T) == 2 ? 1 : 0;     // of a lane's tokens: 8 << MORE
+  if constexpr (LANES + MORE < 6)
+    if (a.log2_lanes > LANES + MORE) return launch_select<T, LANES + 1>(a, stream);
   const dim3 block(SELECT_THREADS);
   hipLaunchKernelGGL((select_scan_kernel<T, LANES>), dim3((a.runs + 3) / 4, a.rows), dim3(256), 0, stream, a);
   hipLaunchKernelGGL(select_rows_kernel<T>, dim3(a.rows), block, 0, stream, a);
@@ -696,7 +721,7 @@ static void launch_select(const select_args& a, hipStream_t stream) {
 }  // namespace tb
 
 extern "C" size_t tb_beam_select_workspace_bytes(int32_t num_rows, int32_t vocab, int32_t num_candidates) {
-  return num_rows > 0 && vocab > 0 && num_candidates > 0 ? tb::select_sizes(num_rows, vocab, num_candidates).all : 0;
+  return num_rows > 0 && vocab > 0 && num_candidates > 0 ? max(tb::select_sizes(num_rows, vocab, num_candidates, 2).all, tb::select_sizes(num_rows, vocab, num_candidates, 4).all) : 0;
 }
 
 extern "C" int32_t tb_beam_select(const void* logits, int64_t row_stride, int32_t vocab, int32_t dtype,
@@ -713,7 +738,7 @@ extern "C" int32_t tb_beam_select(const void* logits, int64_t row_stride, int32_
   TB_CHECK_ARG(num_rows == 1 || row_stride >= vocab);
   const int size = dtype == TB_DTYPE_F32 ? 4 : 2;
   TB_CHECK_ARG((uintptr_t)logits % size == 0 && ((uintptr_t)workspace & 15u) == 0);
-  const select_sizes z(num_rows, vocab, num_candidates);
+  const select_sizes z(num_rows, vocab, num_candidates, size);
   TB_CHECK_ARG(workspace_bytes >= z.all);
   select_args a;
   a.logits = (const char*)logits, a.row_bytes = row_stride * size, a.rows = num_rows, a.beams = beams, a.vocab = vocab;
@@ -724,7 +749,7 @@ extern "C" int32_t tb_beam_select(const void* logits, int64_t row_stride, int32_
   char* const ws = (char*)workspace;
   a.sums = (double2*)ws, a.norms = (double2*)(ws + z.norms), a.lists = (float2*)(ws + z.lists);
   a.seg_max = (float*)(ws + z.maxima);
-  if (dtype == TB_DTYPE_F32) launch_select<float, 0>(a, stream);
+  if (dtype == TB_DTYPE_F32) launch_select<float, 1>(a, stream);
   else if (dtype == TB_DTYPE_F16) launch_select<_Float16, 0>(a, stream);
   else launch_select<__bf16, 0>(a, stream);
   TB_RETURN_LAUNCH_STATUS();
