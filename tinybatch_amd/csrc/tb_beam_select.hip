@@ -55,36 +55,45 @@ __device__ __forceinline__ bool select_open(const select_args& a, int row) {   /
   return !(a.finished && a.finished[row]) && a.scores[row] > -INFINITY;
 }
 
-// 8 logits of a lane from token t0 on, as they lie there; past the vocabulary -inf. (Rows start at any element.)
+// 8 logits as they lie there. (Rows start at any element.)
 template <typename T>
 struct __attribute__((packed, aligned(sizeof(T)))) eight_logits {
   T v[8];
 };
-template <typename T>
-__device__ __forceinline__ eight_logits<T> select_load(const char* row, int t0, int vocab) {
-  if (t0 + 8 <= vocab) return *reinterpret_cast<const eight_logits<T>*>(row + (int64_t)t0 * sizeof(T));
-  eight_logits<T> e;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) e.v[i] = t0 + i < vocab ? reinterpret_cast<const T*>(row)[t0 + i] : (T)-INFINITY;
-  return e;
-}
 
-// Maximum over aligned groups of 2^N lanes, of numbers and infinities. (One instruction a step: the compiler makes a move
-// and a three-operand maximum of it. A DPP source needs two wait states behind its writer.)
-#define SELECT_MAX_DPP(CTRL) \
-  asm("s_nop 1\n\tv_max_f32_dpp %0, %1, %1 " CTRL " row_mask:0xf bank_mask:0xf" : "=v"(y) : "v"(x)); \
+// Maximum over aligned groups of 2^N lanes, of numbers and infinities, or of whole numbers. (One instruction a step: the compiler
+// makes a move and a three-operand maximum of a float's. A DPP source needs two wait states behind its writer.)
+#define SELECT_MAX_DPP(TYPE, CTRL) \
+  asm("s_nop 1\n\tv_max_" TYPE "_dpp %0, %1, %1 " CTRL " row_mask:0xf bank_mask:0xf" : "=v"(y) : "v"(x)); \
   x = y
+#define SELECT_MAX_ROWS(TYPE)                                                   \
+  if constexpr (N >= 1) { SELECT_MAX_DPP(TYPE, "quad_perm:[1,0,3,2]"); }        \
+  if constexpr (N >= 2) { SELECT_MAX_DPP(TYPE, "quad_perm:[2,3,0,1]"); }        \
+  if constexpr (N >= 3) { SELECT_MAX_DPP(TYPE, "row_half_mirror"); }            \
+  if constexpr (N >= 4) { SELECT_MAX_DPP(TYPE, "row_mirror"); }
 template <int N>
 __device__ __forceinline__ float lanes_max(float x) {
   float y;
-  if constexpr (N >= 1) { SELECT_MAX_DPP("quad_perm:[1,0,3,2]"); }
-  if constexpr (N >= 2) { SELECT_MAX_DPP("quad_perm:[2,3,0,1]"); }
-  if constexpr (N >= 3) { SELECT_MAX_DPP("row_half_mirror"); }
-  if constexpr (N >= 4) { SELECT_MAX_DPP("row_mirror"); }
+  SELECT_MAX_ROWS("f32")
   if constexpr (N >= 5) x = max_xor16(x);
   if constexpr (N >= 6) x = max_xor32(x);
   return x;
 }
+template <int N>
+__device__ __forceinline__ uint32_t lanes_max(uint32_t x) {
+  uint32_t y;
+  SELECT_MAX_ROWS("u32")
+  if constexpr (N >= 5) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    x = max((uint32_t)r[0], (uint32_t)r[1]);
+  }
+  if constexpr (N >= 6) {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x = max((uint32_t)r[0], (uint32_t)r[1]);
+  }
+  return x;
+}
+#undef SELECT_MAX_ROWS
 #undef SELECT_MAX_DPP
 
 // Sum over the wave's lanes, in every lane.
@@ -212,12 +221,28 @@ __device__ __forceinline__ float select_value(uint32_t o) {
 }
 constexpr uint32_t ORDER_NONE = 0x007FFFFFu;       // of -inf
 
+// A token's place among all of a row, larger ones first: its logit's order, then 2^30 - 1 - token, below 2^62: a positive double,
+// which is compared in one instruction.
+__device__ __forceinline__ double select_key(uint32_t order, int token) {
+  return __longlong_as_double((int64_t)((uint64_t)order << 30 | (uint32_t)((1 << 30) - 1 - token)));
+}
+
+struct rows_lds {
+  static constexpr int MOST = TB_BEAM_CANDIDATES_MAX + TB_BEAM_CANDIDATES_MAX / 2 + 8;
+  double list[SELECT_LIST];                        // select_key
+  uint32_t tops[SELECT_SEGMENTS];                  // orders of the segments' maxima
+  double sums[SELECT_THREADS / 64];
+  int picked[MOST], equal_of[MOST];
+  int listed, counted;
+};
+
 // Part 2. Tokens are looked at 512 at a time and wave: 64 >> log2_lanes segments side by side, or one of several tiles.
-// each(place of the segment in `picked`, first token, x): a lane's 8 tokens, -inf where there are none.
-template <typename T, typename F>
+// each(place of the segment in `picked`, first token, how many of the 8 are not the piece's, x): as they lie there.
+// TINY: rows of fewer than 8 tokens.
+template <typename T, bool TINY, int AHEAD, typename F>
 __device__ __forceinline__ void select_pieces(const select_args& a, const char* at, const int* picked, int n, int lane,
                                               int wave, F&& each) {
-  constexpr int AHEAD = 1, WAVES = SELECT_THREADS / 64;
+  constexpr int WAVES = SELECT_THREADS / 64;
   const int per = 64 >> a.log2_lanes, spot = lane >> a.log2_lanes, mine = lane & ((1 << a.log2_lanes) - 1);
   const int rounds = (n + WAVES * per - 1) / (WAVES * per) * a.join;   // of all waves
   for (int r0 = 0; r0 < rounds; r0 += AHEAD) {
@@ -227,20 +252,23 @@ __device__ __forceinline__ void select_pieces(const select_args& a, const char* 
     for (int u = 0; u < AHEAD; ++u) {              // (past the end: the last round's again)
       const int r = min(r0 + u, rounds - 1), turn = r / a.join, j = r - turn * a.join;
       p[u] = (turn * WAVES + wave) * per + spot;
-      t0[u] = p[u] < n ? (((picked[p[u]] * a.join + j) << a.log2_lanes) + mine) * 8 : a.vocab;
-      if (a.vocab >= 8)                            // 8 tokens inside the row: the last ones moved up
+      const int segment = picked[min(p[u], rows_lds::MOST - 1)];
+      t0[u] = p[u] < n ? (((segment * a.join + j) << a.log2_lanes) + mine) * 8 : a.vocab;
+      if constexpr (TINY) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) e[u].v[i] = reinterpret_cast<const T*>(at)[min(i, a.vocab - 1)];
+      } else {                                     // 8 tokens inside the row: the last ones moved up
         e[u] = *reinterpret_cast<const eight_logits<T>*>(at + (int64_t)min(t0[u], a.vocab - 8) * sizeof(T));
-      else
-        e[u] = select_load<T>(at, 0, a.vocab);
+      }
     }
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
       if (r0 + u >= rounds) break;
-      const int from = max(0, min(t0[u], a.vocab - 8));
+      const int from = TINY ? 0 : min(t0[u], a.vocab - 8), skip = min(t0[u] - from, 8);
       float x[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = from + i < t0[u] ? -INFINITY : select_logit((float)e[u].v[i]);
-      each(p[u], from, x);
+      for (int i = 0; i < 8; ++i) x[i] = TINY && i >= a.vocab ? -INFINITY : (float)e[u].v[i];
+      each(p[u], from, skip, x);
     }
   }
 }
@@ -257,29 +285,22 @@ __device__ __forceinline__ int select_scan(int x, int lane, int& total) {
   return up - x;
 }
 
-struct rows_lds {
-  static constexpr int MOST = TB_BEAM_CANDIDATES_MAX + TB_BEAM_CANDIDATES_MAX / 2 + 8;
-  uint64_t list[SELECT_LIST];                      // {order of x, ~token}
-  int ranks[SELECT_LIST];
-  float tops[SELECT_SEGMENTS];
-  int picked[MOST], equal_of[MOST];
-  int chosen, listed, counted;
-};
-
 // A row's list, by a workgroup of SELECT_THREADS.
-template <typename T>
+template <typename T, bool TINY>
 __device__ void select_list(const select_args& a, rows_lds& s, int row) {
   constexpr int WAVES = SELECT_THREADS / 64, WORDS = SELECT_SEGMENTS / 64;
-  uint64_t* const list = s.list;
-  int *const ranks = s.ranks, *const picked = s.picked, *const equal_of = s.equal_of;
-  float* const tops = s.tops;
-  int &chosen = s.chosen, &listed = s.listed, &counted = s.counted;
+  double* const list = s.list;
+  int *const picked = s.picked, *const equal_of = s.equal_of;
+  uint32_t* const tops = s.tops;
+  int &listed = s.listed, &counted = s.counted;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), M = a.picks;
   float2* const out = a.lists + (int64_t)row * M;
   float first[SELECT_SEGMENTS / SELECT_THREADS];   // (of a row whose logits do not count: whatever is there)
 #pragma unroll
   for (int i = 0; i < SELECT_SEGMENTS / SELECT_THREADS; ++i)
     first[i] = a.seg_max[(int64_t)row * a.tops + min((i * SELECT_THREADS + tid) * a.join, a.tops - 1)];
+  const double2* const sums = a.sums + (int64_t)row * a.runs;
+  const double2 part = sums[min(tid, a.runs - 1)];
   if (!select_open(a, row)) {                      // one candidate, the score itself, or none
     const bool one = a.finished && a.finished[row] && a.scores[row] > -INFINITY;
     for (int i = tid; i < M; i += SELECT_THREADS)
@@ -293,96 +314,112 @@ __device__ void select_list(const select_args& a, rows_lds& s, int row) {
     float x = seg < a.segments ? select_logit(first[i]) : -INFINITY;
     for (int k = 1; k < a.join && seg * a.join + k < a.tops; ++k)
       x = fmaxf(x, select_logit(a.seg_max[(int64_t)row * a.tops + seg * a.join + k]));
-    tops[seg] = x;
+    tops[seg] = select_order(x);
   }
-  if (tid == 0) chosen = listed = 0;
+  if (tid == 0) listed = 0;
   __syncthreads();
-  uint32_t v[WORDS];                               // every wave: all segments, lane l those of l + 64 i
-  float m = -INFINITY, mine = -INFINITY, mine2 = -INFINITY;   // a lane's best and second best
+  uint32_t v[WORDS], mine = 0, mine2 = 0;          // every wave: all segments, lane l those of l + 64 i; its best and second best
 #pragma unroll
   for (int i = 0; i < WORDS; ++i) {
-    const float x = tops[64 * i + lane];
-    mine2 = fmaxf(mine2, fminf(mine, x));
-    mine = fmaxf(mine, x);
-    v[i] = select_order(x);
+    v[i] = tops[64 * i + lane];
+    mine2 = max(mine2, min(mine, v[i]));
+    mine = max(mine, v[i]);
   }
-  m = lanes_max<6>(mine);
-  const float least = -lanes_max<6>(M <= 64 ? -mine : -mine2);   // 64, or 128, segments at least reach it
-  if (wave == WAVES - 1) {                         // m and log S
+  auto uniform = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
+  const uint32_t most = uniform(lanes_max<6>(mine));
+  const float m = select_value(most);
+  if (64 * wave < a.runs) {                        // S, a wave's part of the runs; their sum and its logarithm at the end
     double sum = 0.;
-    for (int r = lane; r < a.runs; r += 64) {
-      const double2 x = a.sums[(int64_t)row * a.runs + r];
-      sum += x.x * (m == -INFINITY ? 0. : exp(x.y - (double)m));
+    if (m > -INFINITY) {
+      if (tid < a.runs) sum = part.x * exp(part.y - (double)m);
+      for (int r = tid + SELECT_THREADS; r < a.runs; r += SELECT_THREADS) sum += sums[r].x * exp(sums[r].y - (double)m);
     }
-    sum = log(lanes_sum(sum));
-    if (lane == 0) a.norms[row] = make_double2((double)m, sum);
+    sum = lanes_sum(sum);
+    if (lane == 0) s.sums[wave] = sum;
   }
-  // ---- the threshold ----
+  // ---- the threshold: what M segments reach, or all above -inf do, and not many more ----
   auto reach = [&](uint32_t o) {
+    uint64_t mask[WORDS];                          // (each in registers of its own: one register pair in turn waits 16 times)
     int c = 0;
 #pragma unroll
-    for (int i = 0; i < WORDS; ++i) c += __popcll(__ballot(v[i] >= o));
+    for (int i = 0; i < WORDS; ++i) asm("v_cmp_le_u32 %0, %1, %2" : "=s"(mask[i]) : "s"(o), "v"(v[i]));
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) c += __popcll(mask[i]);
     return c;
   };
-  uint32_t lo = ORDER_NONE, hi = select_order(m) + 1, probe = least > -INFINITY ? 0 : ORDER_NONE + 1;
-  int over = 0;                                    // segments that reach hi
-  bool exact = true;                               // else: all that reach lo
-  if (!probe) lo = select_order(least);
-  while (hi - lo > 1) {
-    const uint32_t mid = probe ? probe : lo + (hi - lo) / 2;
+  // first the least of the best of as many groups of lanes as there are candidates wanted, at least (both of a lane's from 65 on)
+  uint32_t least = M > 64 ? mine2 : mine;
+  if (M <= 32) least = lanes_max<1>(least);
+  if (M <= 16) least = max(least, (uint32_t)__shfl_xor((int)least, 2));
+  if (M <= 8) least = max(least, (uint32_t)__shfl_xor((int)least, 4));
+  uint32_t from = max(uniform(~lanes_max<6>(~least)), ORDER_NONE + 1), beyond = most + 1;
+  int reached = reach(from), over = 0;             // segments that reach `from`, `beyond`
+  const int few = M + M / 2 + 8;
+  while (reached > few && beyond - from > 1) {
+    const uint32_t mid = from + (beyond - from) / 2;
     const int c = reach(mid);
-    if (c >= M) {
-      lo = mid;
-      if (c <= M + M / 2 + 8) {
-        exact = false;
-        break;
-      }
-    } else if (probe) {                            // everything above -inf
-      break;
-    } else {
-      hi = mid;
-      over = c;
-    }
-    probe = 0;
+    if (c >= M) from = mid, reached = c;
+    else beyond = mid, over = c;
   }
-  // ---- the segments that reach it; where several equal it and not all are wanted, the first ones ----
-  auto rising = [&](int need) {                    // in order; how many
-    const uint64_t below = ((uint64_t)1 << lane) - 1;
-    int n = 0, eq0 = 0;
+  // ---- these segments, in order; where many equal the threshold, the first ones of them ----
+  const uint64_t below = ((uint64_t)1 << lane) - 1;
+  int n = 0;
+  if (reached <= few) {
+    int n0 = 0, n1 = 0;                            // before the wave's two words
 #pragma unroll
     for (int i = 0; i < WORDS; ++i) {
-      const uint64_t eq = __ballot(v[i] == lo);
-      const bool take = v[i] > lo || (v[i] == lo && eq0 + __popcll(eq & below) < need);
+      if (i == wave) n0 = n;
+      if (i == wave + WAVES) n1 = n;
+      n += __popcll(__ballot(v[i] >= from));
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int seg = 64 * (wave + WAVES * h) + lane;
+      const bool take = tops[seg] >= from;
+      const uint64_t took = __ballot(take);
+      if (take) picked[(h ? n1 : n0) + __popcll(took & below)] = seg;
+    }
+  } else {
+    const int need = M - over;
+    int equals = 0;
+    for (int i = 0; i < WORDS; ++i) {
+      const uint32_t o = tops[64 * i + lane];
+      const uint64_t eq = __ballot(o == from);
+      const bool take = o > from || (o == from && equals + __popcll(eq & below) < need);
       const uint64_t took = __ballot(take);
       if (take && i % WAVES == wave) picked[n + __popcll(took & below)] = 64 * i + lane;
-      eq0 += __popcll(eq);
+      equals += __popcll(eq);
       n += __popcll(took);
     }
-    __syncthreads();
-    return n;
-  };
-  const int want_equal = lo == ORDER_NONE ? 0 : exact ? M - over : SELECT_SEGMENTS;
-  int n;
-  if (want_equal == SELECT_SEGMENTS || lo == ORDER_NONE) {
-    for (int i = tid; i < SELECT_SEGMENTS; i += SELECT_THREADS) {
-      const uint32_t o = select_order(tops[i]);
-      if (o > lo || (o == lo && want_equal)) picked[atomicAdd(&chosen, 1)] = i;
-    }
-    __syncthreads();
-    n = chosen;
-  } else {
-    n = rising(want_equal);
   }
+  __syncthreads();
   const char* const at = a.logits + (int64_t)row * a.row_bytes;
   // ---- the tokens from the threshold up ----
-  select_pieces<T>(a, at, picked, n, lane, wave, [&](int, int t, const float(&x)[8]) {
+  const float threshold = select_value(from);
+  select_pieces<T, TINY, 2>(a, at, picked, n, lane, wave, [&](int, int t, int skip, float(&x)[8]) {
+    if (__any(skip > 0 && skip < 8)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < skip) x[i] = -INFINITY;
+    }
+    const float least = skip < 8 ? threshold : NAN;
+    uint64_t reach[8];
+    int total = 0;                                 // (of the wave, one addition for all)
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const uint32_t o = select_order(x[i]);
-      if (o >= lo && o != ORDER_NONE) {
-        const int place = atomicAdd(&listed, 1);
-        if (place < SELECT_LIST) list[place] = (uint64_t)o << 32 | (uint32_t) ~(t + i);
-      }
+      reach[i] = __ballot(x[i] >= least);          // (not NaN)
+      total += __popcll(reach[i]);
+    }
+    if (total == 0) return;
+    int place = 0;
+    if (lane == 0) place = atomicAdd(&listed, total);
+    place = __builtin_amdgcn_readfirstlane(place);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (reach[i] == 0) continue;
+      const int mine = place + __popcll(reach[i] & (((uint64_t)1 << lane) - 1));
+      if (x[i] >= least && mine < SELECT_LIST) list[mine] = select_key(select_order(select_logit(x[i])), t + i);
+      place += __popcll(reach[i]);
     }
   });
   __syncthreads();
@@ -390,13 +427,18 @@ __device__ void select_list(const select_args& a, rows_lds& s, int row) {
   if (all > SELECT_LIST) {
     // many of them (whole ranges of high or equal tokens): the M-th best token's value, what is above it, and as many
     // of its equals as are wanted, in order
-    uint32_t t0 = lo, t1 = select_order(m) + 1;    // t0 is reached by M tokens, t1 by none
+    auto clean = [](float(&x)[8], int skip) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = i < skip ? -INFINITY : select_logit(x[i]);
+    };
+    uint32_t t0 = from, t1 = most + 1;             // t0 is reached by M tokens, t1 by none
     while (t1 - t0 > 1) {
       const uint32_t mid = t0 + (t1 - t0) / 2;
       __syncthreads();
       if (tid == 0) counted = 0;
       __syncthreads();
-      select_pieces<T>(a, at, picked, n, lane, wave, [&](int, int, const float(&x)[8]) {
+      select_pieces<T, TINY, 1>(a, at, picked, n, lane, wave, [&](int, int, int skip, float(&x)[8]) {
+        clean(x, skip);
         int c = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) c += select_order(x[i]) >= mid;
@@ -406,17 +448,17 @@ __device__ void select_list(const select_args& a, rows_lds& s, int row) {
       if (counted >= M) t0 = mid;
       else t1 = mid;
     }
-    n = rising(want_equal);                        // (segments are numbered below: in order)
     for (int i = tid; i < n; i += SELECT_THREADS) equal_of[i] = 0;
     if (tid == 0) listed = 0;
     __syncthreads();
-    select_pieces<T>(a, at, picked, n, lane, wave, [&](int p, int t, const float(&x)[8]) {
+    select_pieces<T, TINY, 1>(a, at, picked, n, lane, wave, [&](int p, int t, int skip, float(&x)[8]) {
+      clean(x, skip);
       int c = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const uint32_t o = select_order(x[i]);
         c += o == t0;
-        if (o > t0) list[atomicAdd(&listed, 1)] = (uint64_t)o << 32 | (uint32_t) ~(t + i);   // (fewer than M)
+        if (o > t0) list[atomicAdd(&listed, 1)] = select_key(o, t + i);   // (fewer than M)
       }
       if (c) atomicAdd(&equal_of[p], c);
     });
@@ -434,7 +476,8 @@ __device__ void select_list(const select_args& a, rows_lds& s, int row) {
     __syncthreads();
     const int over = listed, want = M - over, width = 1 << a.log2_lanes;
     int seen = 0, of = -1;                         // (segments of several tiles, one wave's: equals of the tiles before)
-    select_pieces<T>(a, at, picked, n, lane, wave, [&](int p, int t, const float(&x)[8]) {
+    select_pieces<T, TINY, 1>(a, at, picked, n, lane, wave, [&](int p, int t, int skip, float(&x)[8]) {
+      clean(x, skip);
       int c = 0;
 #pragma unroll
       for (int i = 0; i < 8; ++i) c += select_order(x[i]) == t0;
@@ -449,7 +492,7 @@ __device__ void select_list(const select_args& a, rows_lds& s, int row) {
         int place = equal_of[p] + seen + up - c;
         for (int i = 0; i < 8; ++i)
           if (select_order(x[i]) == t0) {
-            if (place < want) list[over + place] = (uint64_t)t0 << 32 | (uint32_t) ~(t + i);
+            if (place < want) list[over + place] = select_key(t0, t + i);
             ++place;
           }
       }
@@ -458,26 +501,26 @@ __device__ void select_list(const select_args& a, rows_lds& s, int row) {
     __syncthreads();
     all = M;
   }
-  // ---- their order: how many are better ----
-  for (int i = tid; i < all; i += SELECT_THREADS) ranks[i] = 0;
+  // ---- their order: how many are better, counted by a group of lanes for every entry ----
+  if (tid == SELECT_THREADS - 1) {
+    double sum = 0.;
+    for (int w = 0; w < WAVES && 64 * w < a.runs; ++w) sum += s.sums[w];
+    a.norms[row] = make_double2((double)m, log(sum));
+  }
   for (int i = tid; i < M; i += SELECT_THREADS)
     if (i >= all) out[i] = make_float2(-INFINITY, 0.f);
-  __syncthreads();
-  int share = 1;                                   // threads that count for one entry
+  int share = 1;
   while (share < 64 && 2 * share * all <= SELECT_THREADS) share *= 2;
-  for (int i0 = tid / share; i0 < all; i0 += SELECT_THREADS / share) {
-    const uint64_t e = list[i0];
+  for (int i = tid / share; i < all; i += SELECT_THREADS / share) {
+    const double e = list[i];
     int c = 0;
 #pragma unroll 8
     for (int j = tid % share; j < all; j += share) c += list[j] > e;
-    if (c) atomicAdd(&ranks[i0], c);
+    for (int o = 1; o < share; o *= 2) c += __shfl_xor(c, o);
+    const uint64_t key = (uint64_t)__double_as_longlong(e);
+    const int token = (1 << 30) - 1 - (int)(key & ((1 << 30) - 1));
+    if (tid % share == 0 && c < M) out[c] = make_float2(select_value((uint32_t)(key >> 30)), __int_as_float(token));
   }
-  __syncthreads();
-  for (int i = tid; i < all; i += SELECT_THREADS)
-    if (ranks[i] < M) {
-      const uint64_t e = list[i];
-      out[ranks[i]] = make_float2(select_value((uint32_t)(e >> 32)), __uint_as_float(~(uint32_t)e));
-    }
 }
 
 // A double's place among all doubles.
@@ -674,10 +717,10 @@ __global__ __launch_bounds__(256) void select_scan_kernel(const select_args a) {
   if (run < a.runs && select_open(a, blockIdx.y)) select_run<T, LANES>(a, blockIdx.y, run, threadIdx.x & 63);
 }
 
-template <typename T>
+template <typename T, bool TINY>
 __global__ __launch_bounds__(SELECT_THREADS) void select_rows_kernel(const select_args a) {
   __shared__ rows_lds lds;
-  select_list<T>(a, lds, blockIdx.x);
+  select_list<T, TINY>(a, lds, blockIdx.x);
 }
 
 __global__ __launch_bounds__(SELECT_THREADS) void select_merge_kernel(const select_args a) {
@@ -714,7 +757,8 @@ static void launch_select(const select_args& a, hipStream_t stream) {
     if (a.log2_lanes > LANES + MORE) return launch_select<T, LANES + 1>(a, stream);
   const dim3 block(SELECT_THREADS);
   hipLaunchKernelGGL((select_scan_kernel<T, LANES>), dim3((a.runs + 3) / 4, a.rows), dim3(256), 0, stream, a);
-  hipLaunchKernelGGL(select_rows_kernel<T>, dim3(a.rows), block, 0, stream, a);
+  if (a.vocab < 8) hipLaunchKernelGGL((select_rows_kernel<T, true>), dim3(a.rows), block, 0, stream, a);
+  else hipLaunchKernelGGL((select_rows_kernel<T, false>), dim3(a.rows), block, 0, stream, a);
   hipLaunchKernelGGL(select_merge_kernel, dim3(a.rows / a.beams), block, 0, stream, a);
 }
 
