@@ -306,6 +306,28 @@ def test_select_rising_rows(V, dtype):
         check_select(x[rows:rows + 1], torch.zeros(1, 1), 9)
 
 
+@pytest.mark.parametrize("K,M", [(64, 128), (48, 96), (64, 9), (9, 64)])
+def test_select_of_many_beams(K, M):
+    """More candidates than are ranked at once: alike to the bit, alike in fp32 alone, few left, none left."""
+    g = torch.Generator().manual_seed(K)
+    inf = float("inf")
+    check_select(torch.zeros(K, 300), torch.zeros(1, K), M)
+    check_select(torch.zeros(K, 300), torch.randint(0, 2, (1, K), generator=g) * -1.0, M)
+    x = torch.randn(K, 700, generator=g)
+    check_select(x, torch.full((1, K), -3e9), M)                      # fp32 scores of steps of 256
+    check_select(x, -3e9 - 256.0 * torch.randint(0, 3, (1, K), generator=g), M)
+    check_select(x, torch.randn(1, K, generator=g) * 1e-3 - 4.0, M)
+    masked = torch.full((K, 300), -inf)
+    masked[3, 5], masked[7, 200:203] = 1.0, 0.5
+    check_select(masked, torch.zeros(1, K), M)
+    check_select(x, torch.full((1, K), -inf), M)
+    lowest = torch.full((K, 300), torch.finfo(torch.float32).min)     # values below fp32's range count
+    lowest[:, 0] = torch.finfo(torch.float32).max
+    check_select(lowest, torch.zeros(1, K), M)
+    ended = torch.rand(1, K, generator=g) < 0.7
+    check_select(x, torch.randn(1, K, generator=g) - 5.0, M, ended, 3)
+
+
 def test_select_long_rows_of_small_terms():
     """A flat row of many tokens: the sum's terms are as good as equal, nothing of it is lost."""
     x = torch.full((2, 1_000_003), -5.0)

@@ -385,7 +385,7 @@ __device__ void select_list(const select_args& a, rows_lds& s, int row) {
     for (int i = 0; i < WORDS; ++i) {
       const uint32_t o = tops[64 * i + lane];
       const uint64_t eq = __ballot(o == from);
-      const bool take = o > from || (o == from && equals + __popcll(eq & below) < need);
+      const bool take = o > from || (o == from && equals + (int)__popcll(eq & below) < need);
       const uint64_t took = __ballot(take);
       if (take && i % WAVES == wave) picked[n + __popcll(took & below)] = 64 * i + lane;
       equals += __popcll(eq);
@@ -523,49 +523,28 @@ __device__ void select_list(const select_args& a, rows_lds& s, int row) {
   }
 }
 
+// Part 3. A candidate's place in the order: larger value, then smaller beam, then the beam's own order.
+struct merge_lds {
+  double norms[TB_BEAMS_MAX][3];                   // m, log S, the score
+  double value[MERGE_LIST];
+  uint32_t place[MERGE_LIST];                      // beam << 8 | place in its list
+  int ranks[MERGE_LIST];
+  int waves[2][SELECT_THREADS / 64];
+  uint32_t tops[SELECT_THREADS / 64], leasts[SELECT_THREADS / 64];
+  int held;
+};
 // A double's place among all doubles.
 __device__ __forceinline__ uint64_t merge_order(double x) {
   const uint64_t b = (uint64_t)__double_as_longlong(x + 0.);
   return b >> 63 ? ~b : b | (uint64_t)1 << 63;
 }
-__device__ __forceinline__ double merge_value(uint64_t o) {
-  return __longlong_as_double((int64_t)(o >> 63 ? o ^ (uint64_t)1 << 63 : ~o));
-}
-constexpr uint64_t MERGE_NONE = 0x000FFFFFFFFFFFFFull;   // of -inf
-__device__ __forceinline__ uint64_t merge_xor(uint64_t x, int o) {
-  return (uint64_t)__shfl_xor((unsigned long long)x, o);
-}
-
-// Part 3: a candidate and its place in the order: larger value, then smaller beam, then the beam's own order.
-struct cand {
-  uint64_t c;                  // merge_order of the value
-  uint64_t at;                 // beam << 32 | place in its list
-};
-__device__ __forceinline__ bool better(const cand& x, const cand& y) {   // (no branches)
-  return (x.c > y.c) | ((x.c == y.c) & (x.at < y.at));
-}
-
-struct merge_lds {
-  double norms[TB_BEAMS_MAX][3];                   // m, log S, the score
-  cand cands[MERGE_LIST];
-  int ranks[MERGE_LIST];
-  int waves[2][SELECT_THREADS / 64];
-  uint64_t tops[SELECT_THREADS / 64], leasts[SELECT_THREADS / 64];
-  int held;
-};
 
 // A request's candidates from its beams' lists, by a workgroup of SELECT_THREADS.
 __device__ void select_merge(const select_args& a, merge_lds& s, int request) {
   constexpr int EACH = TB_BEAMS_MAX * TB_BEAM_CANDIDATES_MAX / SELECT_THREADS, WAVES = SELECT_THREADS / 64;
-  cand* const cands = s.cands;
-  int *const ranks = s.ranks, &held = s.held;
-  int(*const waves)[SELECT_THREADS / 64] = s.waves;
-  uint64_t *const tops = s.tops, *const leasts = s.leasts;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int M = a.picks, K = a.beams, row0 = request * K, all = K * M;
-  double(*const norms)[3] = s.norms;
   const float2* const lists = a.lists + (int64_t)row0 * M;
-  auto entry = [&](int i) { return lists[min(i, all - 1)]; };   // one beam's behind the other's
   // the candidates of a thread, SELECT_THREADS behind each other: beam and place in its list
   const uint32_t k0 = tid / M, p0 = tid - k0 * M, dk = SELECT_THREADS / M, dp = SELECT_THREADS - dk * M;
   struct spot {
@@ -576,138 +555,191 @@ __device__ void select_merge(const select_args& a, merge_lds& s, int request) {
     x.p += dp;
     if (x.p >= (uint32_t)M) x.p -= M, ++x.k;
   };
-  auto look = [&](spot at, float2 e) {
-    cand x = {MERGE_NONE, (uint64_t)at.k << 32 | at.p};
-    if (at.k < (uint32_t)K && e.x > -INFINITY) x.c = merge_order(norms[at.k][2] + (((double)e.x - norms[at.k][0]) - norms[at.k][1]));
-    return x;
+  auto value = [&](spot at, float x) {             // -inf: none
+    if (at.k >= (uint32_t)K || !(x > -INFINITY)) return -(double)INFINITY;
+    return s.norms[at.k][2] + (((double)x - s.norms[at.k][0]) - s.norms[at.k][1]);
   };
-  float2 mine[EACH];
+  float mine[EACH];
 #pragma unroll
   for (int i = 0; i < EACH; ++i)
-    if (i * SELECT_THREADS < all) mine[i] = entry(i * SELECT_THREADS + tid);
-  for (int i = tid; i < 2 * K; i += SELECT_THREADS) norms[i >> 1][i & 1] = (&a.norms[row0].x)[i];
-  for (int i = tid; i < K; i += SELECT_THREADS) norms[i][2] = (double)a.scores[row0 + i];
+    if (i * SELECT_THREADS < all) mine[i] = lists[min(i * SELECT_THREADS + tid, all - 1)].x;
+  for (int i = tid; i < 2 * K; i += SELECT_THREADS) s.norms[i >> 1][i & 1] = (&a.norms[row0].x)[i];
+  for (int i = tid; i < K; i += SELECT_THREADS) s.norms[i][2] = (double)a.scores[row0 + i];
+  if (tid == 0) s.held = 0;
+  s.ranks[tid] = 0;
   __syncthreads();
-  if (tid == 0) held = 0;
-  int n;
-  if (all <= SELECT_THREADS) {
-    if (tid < all) cands[tid] = look({k0, p0}, mine[0]), ranks[tid] = 0;
+  int n;                                           // candidates in LDS
+  if (all <= MERGE_LIST) {
     n = all;
+    if (tid < n) {
+      s.value[tid] = value({k0, p0}, mine[0]);
+      s.place[tid] = k0 << 8 | p0;
+    }
+    __syncthreads();
+    // how many are better: in its own list those before it, in another one by halving it
+    const int groups = SELECT_THREADS / n, group = tid / n, i = tid - group * n;
+    const double c = s.value[i];
+    if (group < groups && c > -INFINITY) {
+      const int k = s.place[i] >> 8, half = 1 << (31 - __clz(M));
+      int better = group == 0 ? (int)(s.place[i] & 255) : 0;
+      for (int other = group; other < K; other += groups) {
+        if (other == k) continue;
+        const double* const list = s.value + other * M;
+        int lo = 0;
+        for (int step = half; step; step >>= 1) {
+          const double x = list[min(lo + step, M) - 1];
+          if (lo + step <= M && (x > c || (x == c && other < k))) lo += step;
+        }
+        better += lo;
+      }
+      if (better) atomicAdd(&s.ranks[i], better);
+    }
   } else {
-    uint64_t v[EACH], top = MERGE_NONE;
+    // by values rounded to fp32, which keeps their order but for new equals: what M candidates reach, or all there are do, and
+    // not many more
+    uint32_t v[EACH], top = 0;
     spot at = {k0, p0};
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
-      v[i] = MERGE_NONE;
-      if (i * SELECT_THREADS < all) v[i] = look(at, mine[i]).c;
+      v[i] = 0;
+      if (i * SELECT_THREADS < all) {
+        const double x = value(at, mine[i]);
+        if (x > -INFINITY) v[i] = select_order(fmaxf((float)x, -SELECT_MOST));
+      }
       top = max(top, v[i]);
       next(at);
     }
-    // the best of every 4 threads: the least of these, which 128 candidates reach, and the largest
-    for (int o = 1; o < 4; o *= 2) top = max(top, merge_xor(top, o));
-    uint64_t least = top;
-    for (int o = 4; o < 64; o *= 2) top = max(top, merge_xor(top, o)), least = min(least, merge_xor(least, o));
-    if (lane == 0) tops[wave] = top, leasts[wave] = least;
+    top = lanes_max<2>(top);                       // the best of every 4 threads: the least of these, which 128 candidates reach
+    const uint32_t wave_top = lanes_max<6>(top), wave_least = ~lanes_max<6>(~top);
+    if (lane == 0) s.tops[wave] = wave_top, s.leasts[wave] = wave_least;
     __syncthreads();
-    for (int w = 0; w < WAVES; ++w) top = max(top, tops[w]), least = min(least, leasts[w]);
-    int turn = 0;
-    auto reach = [&](uint64_t o) {
-      int c = 0;
+    uint32_t most = 0, least = ~0u;
 #pragma unroll
-      for (int i = 0; i < EACH; ++i)
-        if (i * SELECT_THREADS < all) c += __popcll(__ballot(v[i] >= o));
-      if (lane == 0) waves[turn & 1][wave] = c;
+    for (int w = 0; w < WAVES; ++w) most = max(most, s.tops[w]), least = min(least, s.leasts[w]);
+    int turn = 0;
+    auto sum_up = [&](int c) {                     // over the waves
+      if (lane == 0) s.waves[turn & 1][wave] = c;
       __syncthreads();
       c = 0;
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) c += waves[turn & 1][w];
+      for (int w = 0; w < WAVES; ++w) c += s.waves[turn & 1][w];
       ++turn;
+      return __builtin_amdgcn_readfirstlane(c);
+    };
+    auto uniform = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
+    uint64_t mask[EACH];
+    auto reach = [&](uint32_t o) {
+      int c = 0;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) asm("v_cmp_le_u32 %0, %1, %2" : "=s"(mask[i]) : "s"(o), "v"(v[i]));
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) c += __popcll(mask[i]);
       return c;
     };
-    uint64_t lo = least, hi = top + 1, probe = least > MERGE_NONE ? 0 : MERGE_NONE + 1;   // as above
-    int over = 0;
-    bool exact = true;
-    while (hi - lo > 1) {
-      const uint64_t mid = probe ? probe : lo + (hi - lo) / 2;
-      const int c = reach(mid);
-      if (c >= M) {
-        lo = mid;
-        if (c <= M + M / 2 + 8) {
-          exact = false;
-          break;
-        }
-      } else if (probe) {
-        break;
-      } else {
-        hi = mid;
-        over = c;
-      }
-      probe = 0;
+    uint32_t from = max(uniform(least), 1u), beyond = uniform(most) + 1;
+    int reached = sum_up(reach(from));
+    const int few = M + M / 2 + 8;
+    while (reached > few && beyond - from > 1) {
+      const uint32_t mid = from + (beyond - from) / 2;
+      const int c = sum_up(reach(mid));
+      if (c >= M) from = mid, reached = c;
+      else beyond = mid;
     }
-    // those above it, and those at it: all where they are few, else the first ones in order
-    exact &= lo > MERGE_NONE;
-    int need = M - over;
     at = {k0, p0};
-    __syncthreads();
+    if (reached <= MERGE_LIST) {
+      const int c = reach(from);
+      int to = 0;
+      if (c && lane == 0) to = atomicAdd(&s.held, c);
+      to = __builtin_amdgcn_readfirstlane(to);
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-      if (i * SELECT_THREADS < all) {
-        bool keep = v[i] >= max(lo, MERGE_NONE + 1);
-        if (exact) {
-          const uint64_t mask = __ballot(v[i] == lo);
-          if (lane == 0) waves[i & 1][wave] = __popcll(mask);
-          __syncthreads();
-          int before = 0, here = 0;
-          for (int w = 0; w < WAVES; ++w) {
-            if (w < wave) before += waves[i & 1][w];
-            here += waves[i & 1][w];
+      for (int i = 0; i < EACH; ++i) {
+        if (mask[i]) {
+          if (v[i] >= from) {
+            const int x = to + __popcll(mask[i] & (((uint64_t)1 << lane) - 1));
+            s.value[x] = value(at, mine[i]);
+            s.place[x] = at.k << 8 | at.p;
           }
-          if (v[i] == lo) keep = before + __popcll(mask & (((uint64_t)1 << lane) - 1)) < need;
-          need -= here;
+          to += __popcll(mask[i]);
         }
-        if (keep) {
-          const int place = atomicAdd(&held, 1);   // at most M + M / 2 + 8
-          cands[place] = look(at, mine[i]), ranks[place] = 0;
-        }
+        next(at);
       }
-      next(at);
+      n = reached;
+    } else {
+      // many whose values round to one: by the values themselves the M best, of equals the first ones
+      auto order = [&](int i, spot at) { return i * SELECT_THREADS < all ? merge_order(value(at, mine[i])) : 0; };
+      uint64_t lo = merge_order(-(double)INFINITY) + 1, hi = ~(uint64_t)0;   // lo is reached by M, hi by fewer
+      int over = 0;
+      while (hi - lo > 1) {
+        const uint64_t mid = lo + (hi - lo) / 2;
+        int c = 0;
+        at = {k0, p0};
+#pragma unroll
+        for (int i = 0; i < EACH; ++i) {
+          c += __popcll(__ballot(order(i, at) >= mid));
+          next(at);
+        }
+        c = sum_up(c);
+        if (c >= M) lo = mid;
+        else hi = mid, over = c;
+      }
+      int need = M - over;
+      at = {k0, p0};
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const uint64_t o = order(i, at), equal = __ballot(o == lo);
+        if (lane == 0) s.waves[turn & 1][wave] = __popcll(equal);
+        __syncthreads();
+        int before = 0, here = 0;
+        for (int w = 0; w < WAVES; ++w) {
+          if (w < wave) before += s.waves[turn & 1][w];
+          here += s.waves[turn & 1][w];
+        }
+        ++turn;
+        if (o > lo || (o == lo && before + (int)__popcll(equal & (((uint64_t)1 << lane) - 1)) < need)) {
+          const int x = atomicAdd(&s.held, 1);
+          s.value[x] = value(at, mine[i]);
+          s.place[x] = at.k << 8 | at.p;
+        }
+        need -= here;
+        next(at);
+      }
+      n = M;
     }
     __syncthreads();
-    n = held;
-  }
-  __syncthreads();
-  if (tid == 0) held = 0;
-  {
-    int share = 1;                                 // threads that count for one candidate
-    while (share < 64 && 2 * share * n <= SELECT_THREADS) share *= 2;
-    for (int i = tid / share; i < n; i += SELECT_THREADS / share) {
-      const cand e = cands[i];
-      int c = 0;
+    const int groups = SELECT_THREADS / max(n, 1), group = tid / max(n, 1), i = tid - group * n;
+    if (n > 0 && group < groups) {                 // threads of a wave meet the same one at once
+      const double c = s.value[i];
+      const uint32_t place = s.place[i];
+      int better = 0;
 #pragma unroll 4
-      for (int j = tid % share; j < n; j += share) c += better(cands[j], e);
-      if (c) atomicAdd(&ranks[i], c);
+      for (int j = group; j < n; j += groups) {
+        const double x = s.value[j];
+        better += (x > c) | ((x == c) & (s.place[j] < place));
+      }
+      if (better) atomicAdd(&s.ranks[i], better);
     }
   }
   __syncthreads();
-  const int64_t at = (int64_t)request * M;
-  if (tid < n) {                                   // (n is SELECT_THREADS at most)
-    const cand x = cands[tid];
-    const bool some = x.c > MERGE_NONE;
+  if (tid == 0) s.held = 0;
+  __syncthreads();
+  const int64_t to = (int64_t)request * M;
+  if (tid < n) {
+    const double c = s.value[tid];
+    const bool some = c > -INFINITY;
     const uint64_t there = __ballot(some);
-    if (lane == 0) atomicAdd(&held, __popcll(there));
-    if (some && ranks[tid] < M) {
-      const int k = (int)(x.at >> 32);
-      const float2 e = lists[k * M + (int)(uint32_t)x.at];
-      a.out_scores[at + ranks[tid]] = (float)merge_value(x.c);
-      a.out_parents[at + ranks[tid]] = k;
-      a.out_tokens[at + ranks[tid]] = __float_as_int(e.y);
+    if (lane == 0) atomicAdd(&s.held, __popcll(there));
+    const int rank = s.ranks[tid], k = s.place[tid] >> 8;
+    if (some && rank < M) {
+      a.out_scores[to + rank] = (float)c;
+      a.out_parents[to + rank] = k;
+      a.out_tokens[to + rank] = __float_as_int(lists[k * M + (int)(s.place[tid] & 255)].y);
     }
   }
   __syncthreads();
-  for (int i = held + tid; i < M; i += SELECT_THREADS) {
-    a.out_scores[at + i] = -INFINITY;
-    a.out_parents[at + i] = -1;
-    a.out_tokens[at + i] = -1;
+  for (int i = s.held + tid; i < M; i += SELECT_THREADS) {
+    a.out_scores[to + i] = -INFINITY;
+    a.out_parents[to + i] = -1;
+    a.out_tokens[to + i] = -1;
   }
 }
 
