@@ -588,7 +588,8 @@ __device__ void select_merge(const select_args& a, merge_lds& s, int request) {
         int lo = 0;
         for (int step = half; step; step >>= 1) {
           const double x = list[min(lo + step, M) - 1];
-          if (lo + step <= M && (x > c || (x == c && other < k))) lo += step;
+          const bool in = (lo + step <= M) & ((x > c) | ((x == c) & (other < k)));
+          lo += in ? step : 0;
         }
         better += lo;
       }
