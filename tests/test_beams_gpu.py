@@ -1,9 +1,10 @@
 """Beam search's operators (tinybatch_amd/device_tables.py, beams.py) on the GPU against their plain forms
 (oracle/beams.py). Steps and reorderings are whole numbers and moved rows: equal, bit for bit.
 
-Selection's scores: the result is rounded to fp32 (2^-24 |c|); a term of the sum e^(x - r) has its argument rounded
-(|x - r| <= 104 where the term is not 0: 104 2^-24 relative to it) and its value by 2 of an exponential's steps, so that the sum
-and with it its logarithm is off by 106 2^-24 at most; everything else is in 64 bits.
+Selection's scores: the result is rounded to fp32 (2^-24 |c|). A term of the sum e^(x - r) has its argument rounded and log2(e) in
+it, 2^-24 |x - r| each at most, and its value by 2 of an exponential's steps, as has the reference's; 16 terms are added in fp32.
+|x - r| is at most (m - x) + 4, and the mean of m - x under the terms is at most log V <= 21 (the terms' entropy): the sum, and
+with it its logarithm, is off by (2 (21 + 4) + 4 + 16) 2^-24 < 106 2^-24 at most; everything else is in 64 bits.
 
 Attention's tolerance counts roundings, with h half a step of the element type: the output is off by h |out|; the weights that
 multiply V are rounded to the type (h each) and so is their sum (h): 2 h sum p|v|; a score, an fp32 sum of d products,
@@ -328,9 +329,10 @@ def test_select_of_many_beams(K, M):
     check_select(x, torch.randn(1, K, generator=g) - 5.0, M, ended, 3)
 
 
-def test_select_long_rows_of_small_terms():
+@pytest.mark.parametrize("dtype", TYPES)
+def test_select_long_rows_of_small_terms(dtype):
     """A flat row of many tokens: the sum's terms are as good as equal, nothing of it is lost."""
-    x = torch.full((2, 1_000_003), -5.0)
+    x = torch.full((2, 1_000_003), -5.0, dtype=dtype)
     x[0, 999_999] = 3.0
     check_select(x, torch.zeros(1, 2), 3)
 

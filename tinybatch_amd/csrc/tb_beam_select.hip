@@ -6,16 +6,25 @@
 // largest are told; among equals the smaller beam's first, within a beam the larger logit (which c, rounded, may
 // no longer show), then the smaller token.
 //
-// Three launches. Part 1 reads the logits once: a wave walks a run of tiles of 512 tokens (8 a lane), writes the maxima of
-// segments of the row (8 to 512 tokens, so that a row has at most 1024) and adds up e^(x - r) against a reference r of
-// the wave.
+// Three launches (in one, with the last workgroups to end going on, it was slower: 44 us against 33 for 32 requests of 8 beams,
+// since code that does not fit the instruction cache is read again by every workgroup).
+// Part 1 reads the logits once: a wave walks a run of tiles of 2048 bytes, writes the maxima of segments of the row (16 to 512
+// tokens, so that a row has at most 1024, beyond 2^19 tokens several of these together) and adds up e^(x - r) against a reference r
+// of the wave. Few beams: the GPU is filled by cutting rows into 16384 runs in all (8192: 26.3 us against 26.6 at 256 rows of
+// 151936 in bf16, 45.3 against 44.3 at 192 rows of 128256 in fp32).
 // Part 2, a workgroup per beam: its M best tokens by (x, v), which need no sum. They lie in its M best
-// segments (the best tokens of the others are behind M better ones already): a threshold t that at least
-// M segment maxima reach, by bisection over the maxima in registers; the tokens of those segments above t, and
-// at t the first M; their order by counting the better ones of each.
-// Part 3, a workgroup per request: of its beams' lists the M best by c, many candidates again by a threshold first.
+// segments (the best tokens of the others are behind M better ones already): a threshold that at least
+// M segment maxima reach and not many more, by bisection over the maxima in registers; the tokens of these segments from it up;
+// their order by counting the better ones of each. Where these are many (flat rows), the M-th best of them by bisection first.
+// Part 3, a workgroup per request: of its beams' lists the M best by c; up to 512 candidates find their places by halving
+// the other beams' lists, of more the best ones are found by a threshold first.
 // Sums of a wave's tiles, S, its logarithm and every c are in 64 bits: the order of two beams' candidates is decided
 // by differences far below a float's step at the score's size.
+//
+// What bounds it: part 1 the vector instructions in 16 bits (4.5 a token and an exponential, which counts four: 32 requests
+// of 8 beams, bf16, 54 MB that count, 14 us) and the memory in fp32 (192 rows, 98 MB, 18 us: 5.4 TB/s); parts 2 and 3 chains
+// of dependent steps of some 100 ns: 6 and 3 us for one request of 4 beams, 7 and 4 for 32 of 8 (M = 16), 11 and 10 for 4 of 48
+// (M = 96, 150 segments a beam). In all, from a captured graph: one request 11.5 us, 32 requests 24.9, 4 of 48 beams 38.7.
 #include "tb_common.h"
 
 namespace tb {
@@ -121,7 +130,9 @@ __device__ __forceinline__ double lanes_sum(double x) {
 // One wave's run of a row whose logits count: tiles of 2048 bytes, 32 a lane. Terms are 2^(x l - c) with l = log2(e) and c = r l, both
 // as floats, in one fused product each; what c lost is in the term of x = r as well, and the sum is divided by it: a row of
 // one token sums to 1 exactly. From |r| = 2^16 on, where c could lose as much as the terms' size, they are 2^((x - r) l) (floats
-// that far out differ by 0 or by more than counts, nearly).
+// that far out differ by 0 or by more than counts, nearly). Both a subtraction and a product for every term, 8 tokens a lane and the
+// reference found anew wherever a logit outgrew it by 1: 121 instructions for 8 tokens against 36, 16.6 us against 14.1 at 32
+// requests of 8 beams in bf16.
 template <typename T, int LANES>                   // 2^LANES lanes of a segment
 __device__ __forceinline__ void select_run(const select_args& a, int row, int run, int lane) {
   constexpr int U = SELECT_LANE / sizeof(T), TILE = 64 * U, PER = 64 >> LANES;
@@ -236,7 +247,7 @@ struct rows_lds {
   int listed, counted;
 };
 
-// Part 2. Tokens are looked at 512 at a time and wave: 64 >> log2_lanes segments side by side, or one of several tiles.
+// Part 2's tokens. They are looked at 512 at a time and wave: 64 >> log2_lanes segments side by side, or one of several tiles.
 // each(place of the segment in `picked`, first token, how many of the 8 are not the piece's, x): as they lie there.
 // TINY: rows of fewer than 8 tokens.
 template <typename T, bool TINY, int AHEAD, typename F>

@@ -14,6 +14,11 @@
 // holds, each once, in the order (request, column, row) of the old tables, behind the free blocks. Every order is
 // fixed: the same state gives the same tables. Fresh blocks are taken before any is freed, so that a copy's source
 // is never its own destination. Where something does not fit nothing is changed.
+//
+// What bounds it: the way of the counts. Tables, counts, lists, the last workgroup's look at all of them and the free blocks are
+// five accesses to memory one behind the other, 1 to 2 us each across XCDs, beside which the copies run: a request of 4 beams
+// 4 + 7 us, 32 requests of 8 beams (14.6 MB of tables and K/V read and written) 5 + 15, 16 of 4 at 32 layers of 8 heads of 128
+// (42.7 MB) 5 + 14. Counts that were waited for one by one and a third launch for the free blocks: 25 us instead of 19 at 32 of 8.
 #include "tb_common.h"
 
 namespace tb {
