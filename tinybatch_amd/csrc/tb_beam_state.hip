@@ -183,23 +183,23 @@ __device__ __forceinline__ void reorder_copy(const reorder_args& a, int unit, in
 }
 
 // The blocks of the lists that nobody holds, each once, behind the free blocks: by the workgroup whose counts and list
-// were the last. A block may stand in several lists (requests that shared it and have let go of it at once); the first
-// of its entries counts.
+// were the last. A block may have several entries (rows that are not neighbours, requests that shared it); the first one
+// counts: up to 512 entries by a hash table in LDS, more by marks in the counts, in two passes.
 struct free_lds {
   static constexpr int N = REORDER_COLUMNS, MOST = 4 * N, SLOTS = 1024, NONE = -1;
-  int waves[2][N / 64], starts[MOST], seen[SLOTS], several;
+  int waves[2][N / 64], starts[MOST], seen[SLOTS], first[SLOTS];   // blocks by hash, the first entry of each
 };
 __device__ __forceinline__ int32_t free_load(const int32_t* p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-template <int EACH>                                // of EACH * N lists from l0 on
 struct free_lists {
   static constexpr int N = free_lds::N;
   const reorder_args& a;
   free_lds& s;
-  int& turn;
-  // their running sums into starts, and the whole
-  __device__ __forceinline__ int count(int l0, int lists) const {
+  int turn, span;                                  // span: of `starts`
+  // the running sums of EACH * N lists from l0 on into starts, and the whole
+  template <int EACH>
+  __device__ __forceinline__ int count(int l0, int lists) {
     const int tid = threadIdx.x;
     int mine[EACH], sum = 0, total;
 #pragma unroll
@@ -210,82 +210,102 @@ struct free_lists {
     int at = group_scan<N>(sum, s.waves, turn++, total);
 #pragma unroll
     for (int u = 0; u < EACH; ++u) s.starts[EACH * tid + u] = at, at += mine[u];
+    span = EACH * N;
     __syncthreads();
     return total;
   }
-  __device__ __forceinline__ int32_t entry(int l0, int x) const {
-    int lo = 0, hi = EACH * N;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (s.starts[mid] <= x) lo = mid;
-      else hi = mid;
-    }
-    return free_load(&a.gone[(int64_t)(l0 + lo) * N * a.beams + x - s.starts[lo]]);
-  }
-  // this thread's next n blocks behind the free ones; how many all have
-  __device__ __forceinline__ int push(int from, int n, const int32_t* ids) const {
-    int won;
-    int at = from + group_scan<N>(n, s.waves, turn++, won);
-    for (int u = 0; u < n; ++u, ++at)
-      if (at < a.num_blocks) a.free_blocks[at] = ids[u];
-    return won;
-  }
-  // all at once, where every block stands in one list: how many are free, or -1
-  __device__ __forceinline__ int few(int from, int total) const {
-    const int tid = threadIdx.x;
-    for (int i = tid; i < free_lds::SLOTS; i += N) s.seen[i] = free_lds::NONE;
-    if (tid == 0) s.several = 0;
-    int32_t id[EACH], refs[EACH], mine[EACH];
+  // entries x of the lists, several searches side by side
+  template <int EACH>
+  __device__ __forceinline__ void entries(int l0, const int (&x)[EACH], int total, int32_t (&id)[EACH]) const {
+    int lo[EACH] = {};
+    for (int step = span / 2; step; step /= 2)
 #pragma unroll
-    for (int u = 0; u < EACH; ++u) id[u] = EACH * tid + u < total ? entry(0, EACH * tid + u) : free_lds::NONE;
-#pragma unroll
-    for (int u = 0; u < EACH; ++u) refs[u] = id[u] != free_lds::NONE ? free_load(&a.refs[id[u]]) : 1;
-    __syncthreads();
-    int n = 0;
+      for (int u = 0; u < EACH; ++u) lo[u] += s.starts[lo[u] + step] <= x[u] ? step : 0;
 #pragma unroll
     for (int u = 0; u < EACH; ++u) {
+      id[u] = free_lds::NONE;
+      if (x[u] < total) id[u] = free_load(&a.gone[(int64_t)(l0 + lo[u]) * N * a.beams + x[u] - s.starts[lo[u]]]);
+    }
+  }
+  template <int EACH>
+  __device__ __forceinline__ void counts(const int32_t (&id)[EACH], int32_t (&refs)[EACH]) const {
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) {
+      refs[u] = 1;
+      if (id[u] != free_lds::NONE) refs[u] = free_load(&a.refs[id[u]]);
+    }
+  }
+  // this thread's blocks that are free behind the free ones; how many all have
+  template <int EACH>
+  __device__ __forceinline__ int push(int from, const bool (&free)[EACH], const int32_t (&id)[EACH]) {
+    int n = 0, won;
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) n += free[u];
+    int at = from + group_scan<N>(n, s.waves, turn++, won);
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) {
+      if (free[u] && at < a.num_blocks) a.free_blocks[at] = id[u];
+      at += free[u];
+    }
+    return won;
+  }
+  // up to EACH * N entries at once: how many are free
+  template <int EACH>
+  __device__ __forceinline__ int few(int from, int total) {
+    const int tid = threadIdx.x;
+    for (int i = tid; i < free_lds::SLOTS; i += N) s.seen[i] = free_lds::NONE, s.first[i] = INT32_MAX;
+    int x[EACH], slot[EACH];
+    int32_t id[EACH], refs[EACH];
+    bool free[EACH];
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) x[u] = EACH * tid + u;
+    entries(0, x, total, id);
+    counts(id, refs);
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) {
+      slot[u] = (uint32_t)id[u] * 2654435761u >> 22;
       if (refs[u] != 0) continue;
-      mine[n++] = id[u];
-      for (uint32_t slot = (uint32_t)id[u] * 2654435761u >> 22;; slot = (slot + 1) % free_lds::SLOTS) {   // (half of them at most)
-        const int was = atomicCAS(&s.seen[slot], free_lds::NONE, id[u]);
-        if (was == id[u]) s.several = 1;
+      for (;; slot[u] = (slot[u] + 1) % free_lds::SLOTS) {   // (half of them at most)
+        const int was = atomicCAS(&s.seen[slot[u]], free_lds::NONE, id[u]);
         if (was == free_lds::NONE || was == id[u]) break;
       }
+      atomicMin(&s.first[slot[u]], x[u]);
     }
     __syncthreads();
-    return s.several ? -1 : push(from, n, mine);
+#pragma unroll
+    for (int u = 0; u < EACH; ++u) free[u] = refs[u] == 0 && s.first[slot[u]] == x[u];
+    return push(from, free, id);
   }
 };
 __device__ void reorder_free(const reorder_args& a, int lists) {
   constexpr int N = free_lds::N;
   __shared__ free_lds s;
   const int tid = threadIdx.x, left = a.num_free_in[0] - a.head[1];
-  int turn = 0, freed = -1;
-  const free_lists<1> one{a, s, turn};
-  const free_lists<4> four{a, s, turn};
-  int total = N + 1;
-  if (lists <= N) total = one.count(0, lists);
+  free_lists all{a, s, 0, N};
+  int total = 4 * N + 1, freed = 0;
+  if (lists <= N) total = all.count<1>(0, lists);
+  else if (lists <= 4 * N) total = all.count<4>(0, lists);
   if (total <= N) {
-    freed = one.few(left, total);
-  } else if (lists <= 4 * N) {
-    total = four.count(0, lists);
-    if (total <= 4 * N) freed = four.few(left, total);
-  }
-  if (freed < 0) {
-    freed = 0;
+    freed = all.few<1>(left, total);
+  } else if (total <= 4 * N) {
+    freed = all.few<4>(left, total);
+  } else {
     for (int pass = 0; pass < 2; ++pass) {         // the first entry of a block marks it; the marks are read
       int before = 0;
       for (int l0 = 0; l0 < lists; l0 += N) {
-        total = one.count(l0, lists);
+        total = all.count<1>(l0, lists);
         for (int x0 = 0; x0 < total; x0 += N) {
-          const int x = x0 + tid, mark = before + x - MARK;
-          const int32_t id = x < total ? one.entry(l0, x) : free_lds::NONE;
-          const int32_t refs = id != free_lds::NONE ? free_load(&a.refs[id]) : 1;
+          const int x[1] = {x0 + tid}, mark = before + x[0] - MARK;
+          int32_t id[1], refs[1];
+          all.entries(l0, x, total, id);
+          all.counts(id, refs);
+          const bool free[1] = {refs[0] == mark};
           if (pass == 0) {
-            if (refs <= 0) atomicMin(&a.refs[id], mark);
+            if (refs[0] <= 0) atomicMin(&a.refs[id[0]], mark);
           } else {
-            freed += one.push(left + freed, refs == mark, &id);
-            if (refs == mark) __hip_atomic_store(&a.refs[id], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            freed += all.push(left + freed, free, id);
+            if (free[0]) __hip_atomic_store(&a.refs[id[0]], 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
           }
         }
         before += total;
