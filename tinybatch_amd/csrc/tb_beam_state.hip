@@ -17,8 +17,9 @@
 //
 // What bounds it: the way of the counts. Tables, counts, lists, the last workgroup's look at all of them and the free blocks are
 // five accesses to memory one behind the other, 1 to 2 us each across XCDs, beside which the copies run: a request of 4 beams
-// 4 + 7 us, 32 requests of 8 beams (14.6 MB of tables and K/V read and written) 5 + 15, 16 of 4 at 32 layers of 8 heads of 128
-// (42.7 MB) 5 + 14. Counts that were waited for one by one and a third launch for the free blocks: 25 us instead of 19 at 32 of 8.
+// 4 + 7 us, 32 requests of 8 beams (14.6 MB of tables and K/V read and written) 5 + 12, 16 of 4 at 32 layers of 8 heads of 128
+// (42.7 MB) 5 + 14. Counts that were waited for one by one and a third launch for the free blocks took 25 us at 32 of 8, freed blocks
+// searched for one behind the other 19, now 16.4.
 #include "tb_common.h"
 
 namespace tb {
