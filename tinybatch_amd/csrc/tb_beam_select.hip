@@ -809,7 +809,9 @@ static void launch_select(const select_args& a, hipStream_t stream) {
 }  // namespace tb
 
 extern "C" size_t tb_beam_select_workspace_bytes(int32_t num_rows, int32_t vocab, int32_t num_candidates) {
-  return num_rows > 0 && vocab > 0 && num_candidates > 0 ? max(tb::select_sizes(num_rows, vocab, num_candidates, 2).all, tb::select_sizes(num_rows, vocab, num_candidates, 4).all) : 0;
+  if (num_rows <= 0 || vocab <= 0 || num_candidates <= 0) return 0;
+  const size_t a = tb::select_sizes(num_rows, vocab, num_candidates, 2).all, b = tb::select_sizes(num_rows, vocab, num_candidates, 4).all;
+  return a > b ? a : b;
 }
 
 extern "C" int32_t tb_beam_select(const void* logits, int64_t row_stride, int32_t vocab, int32_t dtype,
