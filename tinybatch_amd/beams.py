@@ -15,6 +15,7 @@ Everything is enqueued on the tensors' device's current stream and nothing synch
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple
 
@@ -46,24 +47,24 @@ def select_beams(logits: torch.Tensor, scores: torch.Tensor, *, num_candidates: 
     alone, with ``end_token`` at its score. NaN logits count as -inf.
     """
     _lib.require_gpu_tensor("logits", logits)
-    device = logits.device
-    if logits.dtype not in _lib.DTYPE_CODE:
+    device, code, shape = logits.device, _lib.DTYPE_CODE.get(logits.dtype), scores.shape
+    if code is None:
         raise TypeError(f"unsupported logits dtype {logits.dtype}")
-    if scores.dim() != 2 or not 1 <= scores.shape[1] <= MAX_BEAMS:
-        raise ValueError(f"scores must be [requests, beams] with 1 .. {MAX_BEAMS} beams, got {tuple(scores.shape)}")
-    G, K = scores.shape
+    if len(shape) != 2 or not 1 <= shape[1] <= MAX_BEAMS:
+        raise ValueError(f"scores must be [requests, beams] with 1 .. {MAX_BEAMS} beams, got {tuple(shape)}")
+    G, K = shape
     _ints("scores", scores, torch.float32, (G, K), device)
-    if logits.dim() != 2 or logits.shape[0] != G * K or logits.shape[1] < 1 or logits.stride(1) != 1:
+    rows, vocab = logits.shape if logits.dim() == 2 else (-1, 0)
+    if rows != G * K or vocab < 1 or logits.stride(1) != 1:
         raise ValueError(f"logits must be [{G * K}, vocab] with contiguous rows, got {tuple(logits.shape)}")
-    vocab = logits.shape[1]
-    stride = logits.stride(0) if G * K > 1 else vocab
+    stride = logits.stride(0) if rows > 1 else vocab
     if stride < vocab:
         raise ValueError("logits' rows overlap")
     M = K if num_candidates is None else num_candidates
     if not 1 <= M <= MAX_CANDIDATES:
         raise ValueError(f"num_candidates must lie within 1 .. {MAX_CANDIDATES}")
-    if vocab > 1 << 30 or G * K > 65535:
-        raise ValueError(f"{G * K} rows of a vocabulary of {vocab}: at most 65535 and 2^30 are served")
+    if vocab > 1 << 30 or rows > 65535:
+        raise ValueError(f"{rows} rows of a vocabulary of {vocab}: at most 65535 and 2^30 are served")
     if finished is not None:
         _ints("finished", finished, torch.bool, (G, K), device)
         if not 0 <= end_token < vocab:
@@ -71,21 +72,29 @@ def select_beams(logits: torch.Tensor, scores: torch.Tensor, *, num_candidates: 
     if _elsewhere(device):
         with torch.cuda.device(device):
             return select_beams(logits, scores, num_candidates=M, finished=finished, end_token=end_token)
-    out = BeamChoice(torch.empty(G, M, dtype=torch.float32, device=device),
-                     torch.empty(G, M, dtype=torch.int32, device=device),
-                     torch.empty(G, M, dtype=torch.int64, device=device))
-    L, stream = _lib.lib(), _lib.stream_handle(device)
-    need = L.tb_beam_select_workspace_bytes(G * K, vocab, M)
+    best = torch.empty(G, M, dtype=torch.float32, device=device)
+    parents = torch.empty(G, M, dtype=torch.int32, device=device)
+    tokens = torch.empty(G, M, dtype=torch.int64, device=device)
+    L, stream, need = _lib.lib(), _lib.stream_handle(device), _select_bytes(rows, vocab, M)
     lock, ws, ws_bytes, _, _ = _scratch(device, stream, need, 0)
     try:
-        st = L.tb_beam_select(logits.data_ptr(), stride, vocab, _lib.DTYPE_CODE[logits.dtype], scores.data_ptr(),
-                              None if finished is None else finished.data_ptr(), end_token, G * K, K, M,
-                              out.scores.data_ptr(), out.parents.data_ptr(), out.tokens.data_ptr(), ws.data_ptr(),
-                              ws_bytes, stream)
+        st = L.tb_beam_select(logits.data_ptr(), stride, vocab, code, scores.data_ptr(),
+                              None if finished is None else finished.data_ptr(), end_token, rows, K, M,
+                              best.data_ptr(), parents.data_ptr(), tokens.data_ptr(), ws.data_ptr(), ws_bytes, stream)
     finally:
         lock.release()
     _lib.check(st, "tb_beam_select")
-    return out
+    return BeamChoice(best, parents, tokens)
+
+
+@functools.lru_cache(maxsize=256)
+def _select_bytes(rows: int, vocab: int, picks: int) -> int:
+    return _lib.lib().tb_beam_select_workspace_bytes(rows, vocab, picks)
+
+
+@functools.lru_cache(maxsize=256)
+def _reorder_bytes(rows: int, beams: int, max_blocks: int) -> int:
+    return _lib.lib().tb_beam_reorder_workspace_bytes(rows, beams, max_blocks)
 
 
 def reorder_beams(storage: torch.Tensor | None, tables: DeviceTables, parents: torch.Tensor,
@@ -121,8 +130,7 @@ def reorder_beams(storage: torch.Tensor | None, tables: DeviceTables, parents: t
             return reorder_beams(storage, tables, parents, step)
     p = tables._ptr
     lens, free = (p["context_lens"], p["num_free"]) if step is None else step._args[2:4]
-    L, stream = _lib.lib(), _lib.stream_handle(device)
-    need = L.tb_beam_reorder_workspace_bytes(tables.num_rows, K, tables.max_blocks)
+    L, stream, need = _lib.lib(), _lib.stream_handle(device), _reorder_bytes(tables.num_rows, K, tables.max_blocks)
     lock, ws, ws_bytes, _, _ = _scratch(device, stream, need, 0)
     try:
         st = L.tb_beam_reorder(
