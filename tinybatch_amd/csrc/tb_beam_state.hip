@@ -319,7 +319,8 @@ __device__ void reorder_free(const reorder_args& a, int lists) {
 }
 
 __global__ __launch_bounds__(REORDER_COLUMNS) void reorder_tables_kernel(const reorder_args a, int table_groups) {
-  extern __shared__ int32_t lds[];                 // old entries [beams][128], the plan [beams], what rows hold [beams]
+  // (aligned: the plan and the holds are read 16 bytes at a time, and 512 K bytes of entries keep them there)
+  extern __shared__ __align__(16) int32_t lds[];   // old entries [beams][128], the plan [beams], what rows hold [beams]
   if (a.head[0]) return;
   if ((int)blockIdx.x >= table_groups) {
     const int copies = a.head[1], stride = gridDim.x - table_groups;
