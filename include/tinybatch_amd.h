@@ -808,7 +808,8 @@ int32_t tb_tree_commit(void* storage, int32_t num_layers, int64_t layer_stride_b
  *   lens [num_rows]; ref_counts [num_blocks]: how many rows (and holders outside) have a block;
  *   free_blocks [num_blocks], num_free [1]: the free blocks, the next one to be taken last;
  *   shared_blocks [num_rows / beams]: leading whole blocks that all of a request's rows with
- *     positions have in common (tb_beam_reorder sets it);
+ *     positions have in common, or fewer (tb_beam_reorder sets it, tb_beam_step keeps it true; who writes lengths
+ *     or tables by other means sets what holds, 0 always does);
  *   status [1]: TB_TABLES_* bits are added where a call could not do its work; the caller clears them.
  */
 #define TB_BEAMS_MAX 64
@@ -847,6 +848,19 @@ int32_t tb_device_step(int32_t* block_tables, int32_t max_blocks_per_row, const 
                        int32_t* work_items, int32_t max_items, int32_t max_partitions,
                        int32_t* split_rows, int32_t max_split_rows, int32_t* counts, uint32_t* status,
                        void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* The same step of a state whose rows are requests' beams, with the state's shared_blocks: 0 for every request of which a row
+ * without positions gets tokens (they go to blocks of its own, which the other rows do not have), as they are for the
+ * others and where the step does not fit. With tb_device_step the caller does that, before tb_beam_plan. */
+int32_t tb_beam_step(int32_t* block_tables, int32_t max_blocks_per_row, const int32_t* cached_lens,
+                     const int32_t* new_lens, int32_t num_rows, int32_t* shared_blocks, int32_t beams,
+                     int32_t* ref_counts, const int32_t* free_blocks, const int32_t* num_free, int32_t num_blocks,
+                     int32_t block_size, int32_t pad_tokens, int32_t max_tokens, int32_t* context_lens,
+                     int32_t* num_free_out, int32_t* query_start_loc, int64_t* positions, int32_t* slot_mapping,
+                     int32_t* row_ctx, int32_t partition_tokens, int32_t rows_per_item, int32_t* row_part_offsets,
+                     int32_t* work_items, int32_t max_items, int32_t max_partitions, int32_t* split_rows,
+                     int32_t max_split_rows, int32_t* counts, uint32_t* status, void* workspace,
+                     size_t workspace_bytes, hipStream_t stream);
 
 /* The best continuations of every request: with s = scores[row] and x = logits[row] of beam k,
  *   c(k, v) = s + x[v] - log(sum_u exp(x[u])),

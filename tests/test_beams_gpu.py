@@ -828,3 +828,71 @@ def test_attention_refusals():
             bad()
     with pytest.raises(RuntimeError):
         beam_attention(q.cpu(), pool, plan)
+
+
+# ---- rows that were empty --------------------------------------------------------------
+def refill(s, t, new, chunk, pool):
+    """Steps of up to ``chunk`` new tokens a row until every row has its new[r], each taken; their K/V rows are random."""
+    new, d, hkv = list(new), pool.shape[-1], pool.shape[2]
+    step = t.new_step(padded=chunk)
+    g = torch.Generator().manual_seed(sum(new))
+    while any(new):
+        part = [min(n, chunk) for n in new]
+        s = oracle.step(s, part, chunk)[0]
+        build_device_step(t, i32(part), step)
+        k, v = (torch.randn(len(new) * chunk, hkv, d, generator=g).to(pool.dtype).to(DEV) for _ in range(2))
+        ops.kv_append(pool, k, v, step.slot_mapping)
+        yield s, step
+        t.take(step)
+        new = [n - p for n, p in zip(new, part)]
+    t.check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("chunk", [1, 7, 32])
+@pytest.mark.parametrize("lens,new", [([37, 0], [0, 32]), ([37, 0], [3, 40]), ([33, 40, 0, 36, 32, 0, 0, 50], [1, 0, 33, 0, 0, 0, 48, 17]),
+                                      ([0, 0, 40, 37], [20, 35, 1, 1])])
+def test_attention_of_rows_that_were_empty(lens, new, chunk, dtype):
+    """A row without positions gets tokens, in blocks of its own: it shares none with its request's other rows, whatever they
+    shared before; the request beside it still does."""
+    K = 2 if len(lens) < 8 else 4
+    tables, at = [], 40
+    for r, n in enumerate(lens):                   # two whole blocks in common, the rest a row's own
+        whole = [2 * (r // K), 2 * (r // K) + 1][:n // 16]
+        own = -(-n // 16) - len(whole)
+        tables.append(whole + list(range(at, at + own)))
+        at += own
+    s = oracle.State(tables, lens, list(range(10, 34)), 64, 16, K)
+    t = upload(s, max_blocks=6)
+    assert t.shared_blocks.tolist() == s.shared()
+    pool = torch.randn(64, 2, 2, 16, 64, device=DEV).to(dtype)
+    plan = BeamPlan(t, num_heads=6, num_kv_heads=2, head_dim=64, dtype=dtype)
+    q = torch.randn(len(lens), 6, 64).to(dtype)
+    for after, step in refill(s, t, new, chunk, pool):
+        # before it is taken: over the step's lengths, and over the lengths that are still the state's
+        for n, rows in ((after.lens, step.context_lens), (s.lens, None)):
+            check_attention(beam_attention(q.to(DEV), pool, plan.build(rows)), q, pool.cpu(), after.tables, n, 6)
+        s = after
+    check_state(t, s)
+    check_attention(beam_attention(q.to(DEV), pool, plan.build()), q, pool.cpu(), s.tables, s.lens, 6)
+    assert all(x <= y for x, y in zip(t.shared_blocks.tolist(), s.shared()))
+    assert all(t.shared_blocks[g // K] == 2 for g in range(0, len(lens), K) if all(lens[g:g + K]))
+
+
+def test_steps_keep_what_rows_share():
+    """Steps whose new tokens go to rows with positions, steps that do not fit, steps of one row a request: as shared as before."""
+    s = oracle.State([[0, 1, 4], [0, 1, 5], [2, 3], []], [37, 40, 32, 0], [10, 11], 16, 16, 2)
+    t = upload(s, max_blocks=4)
+    assert t.shared_blocks.tolist() == [2, 2]
+    step = t.new_step(padded=40)
+    build_device_step(t, i32([1, 8, 1, 0]), step)
+    assert t.shared_blocks.tolist() == [2, 2]
+    build_device_step(t, i32([0, 0, 0, 40]), step)                     # three blocks of two
+    assert t.shared_blocks.tolist() == [2, 2] and not step.row_ctx.any()
+    with pytest.raises(OutOfBlocks):
+        t.check()
+    build_device_step(t, i32([0, 0, 0, 20]), step)
+    assert t.shared_blocks.tolist() == [2, 0]
+    one = DeviceTables.from_lists([[0], []], [16, 0], [3], max_blocks=2, block_size=16, num_blocks=4, device=DEV)
+    build_device_step(one, i32([0, 1]), one.new_step(padded=1))
+    one.check()

@@ -204,3 +204,14 @@ def test_attention_unsupported_and_empty():
     assert call(L.tb_beam_attention, ATTEND, rows=0, q=None) == _lib.TB_OK
     assert call(L.tb_beam_plan, PLAN, ctx=None) == _lib.TB_ERR_INVALID_ARG
     assert call(L.tb_beam_plan, PLAN, shared=None) == _lib.TB_ERR_INVALID_ARG
+
+
+BEAM_STEP = {k: v for name in STEP for k, v in ([(name, STEP[name])] if name != "refs" else
+                                               [("shared", F), ("beams", 2), ("refs", F)])}
+
+
+@pytest.mark.parametrize("bad", [
+    dict(beams=0), dict(beams=-1), dict(beams=3), dict(beams=65, rows=65), dict(shared=None), dict(rows=-2), dict(bs=12),
+    dict(tokens=1 << 24), dict(num_free_out=F), dict(lens=F), dict(status=None), dict(group=17), dict(rows=2000, tokens=32)])
+def test_beam_step_refusals(bad):
+    assert call(_lib.lib().tb_beam_step, BEAM_STEP, **bad) == _lib.TB_ERR_INVALID_ARG

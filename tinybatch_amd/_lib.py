@@ -164,6 +164,11 @@ SIGNATURES = {
         c_i32, c_i32, c_vp, c_vp, c_i32, c_i32,  # partition, rows per item, offsets, items, max items, max partitions
         c_vp, c_i32, c_vp, c_vp,                 # split rows, max split rows, counts, status
         c_vp, c_sz, c_vp]),                      # workspace, bytes, stream
+    "tb_beam_step": (c_i32, [
+        c_vp, c_i32, c_vp, c_vp, c_i32, c_vp, c_i32,   # block tables, max_nb, cached lens, new lens, rows, shared, beams
+        c_vp, c_vp, c_vp, c_i32, c_i32, c_i32, c_i32,  # as tb_device_step from here on
+        c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_vp, c_vp, c_i32, c_i32, c_vp, c_i32, c_vp, c_vp, c_vp, c_sz,
+        c_vp]),
     "tb_beam_select_workspace_bytes": (c_sz, [c_i32, c_i32, c_i32]),
     "tb_beam_select": (c_i32, [c_vp, c_i64, c_i32, c_i32,            # logits, stride, vocab, dtype
                                c_vp, c_vp, c_i32, c_i32, c_i32, c_i32,   # scores, finished, end, rows, beams, candidates

@@ -12,6 +12,8 @@
 // other: every workgroup makes them itself (rows in LDS, 256 at a time), and then writes its own tokens. Nothing that is
 // read here is written here (new blocks are read from the free blocks, not from the tables),
 // so that one launch does, and a step that is built again gives the same arrays.
+// A row without positions that gets tokens has no block in common with the other rows of its request, which shared theirs
+// without it: shared[b / beams] = 0.
 //
 // What bounds it: the launch and a chain of dependent loads (lengths, the sums, a free block): 256 rows of one token 8.1 us a call,
 // 300 rows of up to 100 tokens each with their work items 10.0, where the smallest of launches takes 4.
@@ -32,6 +34,8 @@ struct step_args {
   const int32_t* cached;       // [rows]
   const int32_t* new_lens;     // [rows]
   int32_t rows;
+  int32_t* shared;             // [rows / beams] or null
+  int32_t beams;
   int32_t* refs;               // [num_blocks]
   const int32_t* free_blocks;  // [num_blocks]
   const int32_t* num_free;     // [1]
@@ -209,7 +213,11 @@ __global__ __launch_bounds__(STEP_THREADS) void step_fill_kernel(const step_args
   }
   for (int b = first; b <= a.rows; b += all) {
     a.starts[b] = a.pad ? b * a.pad : bad ? 0 : tok[b];
-    if (b < a.rows) a.lens[b] = a.cached[b] + (bad ? 0 : a.new_lens[b]);
+    if (b < a.rows) {
+      const int c = a.cached[b], n = bad ? 0 : a.new_lens[b];
+      a.lens[b] = c + n;
+      if (a.shared && c == 0 && n > 0) a.shared[b / a.beams] = 0;
+    }
   }
   if (!bad)
     for (int x = first; x < blk[a.rows]; x += all) {
@@ -267,16 +275,16 @@ extern "C" size_t tb_device_step_workspace_bytes(int32_t num_rows) {
   return num_rows > tb::STEP_LDS_ROWS ? ((size_t)tb::STEP_SUMS * ((size_t)num_rows + 1) + 1) * 4 : 0;
 }
 
-extern "C" int32_t tb_device_step(int32_t* block_tables, int32_t max_blocks_per_row, const int32_t* cached_lens,
-                                  const int32_t* new_lens, int32_t num_rows, int32_t* ref_counts,
-                                  const int32_t* free_blocks, const int32_t* num_free, int32_t num_blocks,
-                                  int32_t block_size, int32_t pad_tokens, int32_t max_tokens,
-                                  int32_t* context_lens, int32_t* num_free_out, int32_t* query_start_loc,
-                                  int64_t* positions, int32_t* slot_mapping, int32_t* row_ctx,
-                                  int32_t partition_tokens, int32_t rows_per_item, int32_t* row_part_offsets,
-                                  int32_t* work_items, int32_t max_items, int32_t max_partitions,
-                                  int32_t* split_rows, int32_t max_split_rows, int32_t* counts, uint32_t* status,
-                                  void* workspace, size_t workspace_bytes, hipStream_t stream) {
+static int32_t device_step(int32_t* block_tables, int32_t max_blocks_per_row, const int32_t* cached_lens,
+                           const int32_t* new_lens, int32_t num_rows, int32_t* shared_blocks, int32_t beams,
+                           int32_t* ref_counts, const int32_t* free_blocks, const int32_t* num_free, int32_t num_blocks,
+                           int32_t block_size, int32_t pad_tokens, int32_t max_tokens,
+                           int32_t* context_lens, int32_t* num_free_out, int32_t* query_start_loc,
+                           int64_t* positions, int32_t* slot_mapping, int32_t* row_ctx,
+                           int32_t partition_tokens, int32_t rows_per_item, int32_t* row_part_offsets,
+                           int32_t* work_items, int32_t max_items, int32_t max_partitions,
+                           int32_t* split_rows, int32_t max_split_rows, int32_t* counts, uint32_t* status,
+                           void* workspace, size_t workspace_bytes, hipStream_t stream) {
   using namespace tb;
   TB_CHECK_ARG(num_rows >= 0 && num_rows < STEP_MOST && max_blocks_per_row > 0 && num_blocks > 0);
   TB_CHECK_ARG(block_size > 0 && (block_size & (block_size - 1)) == 0);
@@ -299,7 +307,7 @@ extern "C" int32_t tb_device_step(int32_t* block_tables, int32_t max_blocks_per_
   TB_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need && ((uintptr_t)workspace & 3u) == 0));
   step_args a;
   a.block_tables = block_tables, a.max_nb = max_blocks_per_row, a.cached = cached_lens, a.new_lens = new_lens;
-  a.rows = num_rows, a.refs = ref_counts, a.free_blocks = free_blocks, a.num_free = num_free;
+  a.rows = num_rows, a.shared = shared_blocks, a.beams = beams, a.refs = ref_counts, a.free_blocks = free_blocks, a.num_free = num_free;
   a.num_blocks = num_blocks, a.log2_bs = __builtin_ctz((unsigned)block_size);
   a.pad = pad_tokens, a.max_tokens = max_tokens;
   a.P = partition_tokens, a.group = rows_per_item, a.max_items = max_items, a.max_parts = max_partitions;
@@ -317,4 +325,39 @@ extern "C" int32_t tb_device_step(int32_t* block_tables, int32_t max_blocks_per_
     hipLaunchKernelGGL(step_fill_kernel<false>, dim3(grid < 2048 ? grid : 2048), dim3(STEP_THREADS), 0, stream, a);
   }
   TB_RETURN_LAUNCH_STATUS();
+}
+
+extern "C" int32_t tb_device_step(int32_t* block_tables, int32_t max_blocks_per_row, const int32_t* cached_lens,
+                                  const int32_t* new_lens, int32_t num_rows, int32_t* ref_counts,
+                                  const int32_t* free_blocks, const int32_t* num_free, int32_t num_blocks,
+                                  int32_t block_size, int32_t pad_tokens, int32_t max_tokens,
+                                  int32_t* context_lens, int32_t* num_free_out, int32_t* query_start_loc,
+                                  int64_t* positions, int32_t* slot_mapping, int32_t* row_ctx,
+                                  int32_t partition_tokens, int32_t rows_per_item, int32_t* row_part_offsets,
+                                  int32_t* work_items, int32_t max_items, int32_t max_partitions,
+                                  int32_t* split_rows, int32_t max_split_rows, int32_t* counts, uint32_t* status,
+                                  void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  return device_step(block_tables, max_blocks_per_row, cached_lens, new_lens, num_rows, nullptr, 1, ref_counts, free_blocks,
+                     num_free, num_blocks, block_size, pad_tokens, max_tokens, context_lens, num_free_out, query_start_loc,
+                     positions, slot_mapping, row_ctx, partition_tokens, rows_per_item, row_part_offsets, work_items,
+                     max_items, max_partitions, split_rows, max_split_rows, counts, status, workspace, workspace_bytes, stream);
+}
+
+extern "C" int32_t tb_beam_step(int32_t* block_tables, int32_t max_blocks_per_row, const int32_t* cached_lens,
+                                const int32_t* new_lens, int32_t num_rows, int32_t* shared_blocks, int32_t beams,
+                                int32_t* ref_counts, const int32_t* free_blocks, const int32_t* num_free,
+                                int32_t num_blocks, int32_t block_size, int32_t pad_tokens, int32_t max_tokens,
+                                int32_t* context_lens, int32_t* num_free_out, int32_t* query_start_loc,
+                                int64_t* positions, int32_t* slot_mapping, int32_t* row_ctx,
+                                int32_t partition_tokens, int32_t rows_per_item, int32_t* row_part_offsets,
+                                int32_t* work_items, int32_t max_items, int32_t max_partitions,
+                                int32_t* split_rows, int32_t max_split_rows, int32_t* counts, uint32_t* status,
+                                void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  TB_CHECK_ARG(beams > 0 && beams <= TB_BEAMS_MAX && num_rows >= 0 && num_rows % beams == 0);
+  TB_CHECK_ARG(num_rows == 0 || shared_blocks);
+  return device_step(block_tables, max_blocks_per_row, cached_lens, new_lens, num_rows, shared_blocks, beams, ref_counts,
+                     free_blocks, num_free, num_blocks, block_size, pad_tokens, max_tokens, context_lens, num_free_out,
+                     query_start_loc, positions, slot_mapping, row_ctx, partition_tokens, rows_per_item, row_part_offsets,
+                     work_items, max_items, max_partitions, split_rows, max_split_rows, counts, status, workspace,
+                     workspace_bytes, stream);
 }

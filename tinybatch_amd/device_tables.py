@@ -40,7 +40,7 @@ def _ints(name: str, t: torch.Tensor, dtype: torch.dtype, shape: tuple, device: 
 
 @dataclass
 class DeviceStep:
-    """One step's arrays on the GPU (tb_device_step), allocated once (DeviceTables.new_step) and
+    """One step's arrays on the GPU (tb_beam_step), allocated once (DeviceTables.new_step) and
     filled by build_device_step: they may be written to, not replaced."""
     max_tokens: int
     padded: int                        # > 0: row b's tokens are the flat rows from b * padded on
@@ -58,7 +58,7 @@ class DeviceStep:
     counts: torch.Tensor | None = None             # [4] int32: items, split rows, 0, partitions
     max_partitions: int = 0
     _counted: torch.Tensor | None = field(default=None, repr=False)   # context_lens and num_free, one behind the other
-    _args: tuple = field(default=(), repr=False)   # tb_device_step's arguments from pad_tokens to counts
+    _args: tuple = field(default=(), repr=False)   # tb_beam_step's arguments from pad_tokens to counts
 
     def metadata(self, tables: "DeviceTables") -> StepMetadata:
         """The step as ops.paged_attention and ops.kv_append take it: the arrays above, sized to their
@@ -84,7 +84,8 @@ class DeviceStep:
 class DeviceTables:
     """The paged state of ``num_rows`` rows on the GPU: block tables, lengths, reference counts and
     the free blocks. Rows g * group_size .. belong to request g (its beams). Its arrays are allocated
-    once: they may be written to, not replaced."""
+    once: they may be written to, not replaced (who writes lengths or tables sets shared_blocks, the leading whole blocks
+    that all of a request's rows with positions have in common, to what holds: 0 always does)."""
 
     def __init__(self, num_rows: int, *, max_blocks: int, block_size: int, num_blocks: int, device,
                  group_size: int = 1, _arrays=None):
@@ -246,9 +247,10 @@ def _ids(name: str, x, num_blocks: int) -> np.ndarray:
 
 def build_device_step(tables: DeviceTables, new_lens: torch.Tensor, step: DeviceStep) -> DeviceStep:
     """Row b gets new_lens[b] (int32, on the GPU) tokens behind its cached positions: the blocks they need
-    are taken from the free blocks, and the step's arrays are filled (tb_device_step). ``tables`` keeps
+    are taken from the free blocks, and the step's arrays are filled (tb_beam_step). ``tables`` keeps
     its lengths and free blocks until tables.take(step) or reorder_beams(..., step=step), so a step may be
-    built again. Where something does not fit the step is empty (tables.check() raises)."""
+    built again; a request of which an empty row gets tokens shares no block from here to its next reordering.
+    Where something does not fit the step is empty (tables.check() raises)."""
     device, rows = tables.device, tables.num_rows
     _ints("new_lens", new_lens, torch.int32, (rows,), device)
     if step.context_lens.device != device or step.context_lens.shape[0] != rows:
@@ -262,11 +264,12 @@ def build_device_step(tables: DeviceTables, new_lens: torch.Tensor, step: Device
     if need:
         lock, ws, _, _, _ = _scratch(device, stream, need, 0)
     try:
-        st = L.tb_device_step(p["block_tables"], tables.max_blocks, p["context_lens"], new_lens.data_ptr(), rows,
-                              p["ref_counts"], p["free_blocks"], p["num_free"], tables.num_blocks, tables.block_size,
-                              *step._args, p["status"], None if ws is None else ws.data_ptr(), need, stream)
+        st = L.tb_beam_step(p["block_tables"], tables.max_blocks, p["context_lens"], new_lens.data_ptr(), rows,
+                            p["shared_blocks"], tables.group_size, p["ref_counts"], p["free_blocks"], p["num_free"],
+                            tables.num_blocks, tables.block_size, *step._args, p["status"],
+                            None if ws is None else ws.data_ptr(), need, stream)
     finally:
         if lock is not None:
             lock.release()
-    _lib.check(st, "tb_device_step")
+    _lib.check(st, "tb_beam_step")
     return step
