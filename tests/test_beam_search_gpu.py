@@ -171,3 +171,26 @@ def test_search_in_16_bits(dtype):
         if graphs:
             assert got == first
         first = got
+
+
+def test_prompts_of_a_search_that_failed_are_not_found(monkeypatch):
+    """The second of two prompts' forward passes fails: the next calls compute both prompts again, to the right tokens."""
+    eng = sharpen(engine(max_batch_tokens=64))
+    prompts = random_prompts(13, [50, 64])
+    forward, calls = eng.model.forward, []
+
+    def failing(*args):
+        calls.append(args)
+        if len(calls) == 2:
+            raise RuntimeError("out of memory")
+        return forward(*args)
+
+    monkeypatch.setattr(eng.model, "forward", failing)
+    with pytest.raises(RuntimeError, match="out of memory"):
+        eng.beam_search(prompts, num_beams=3, max_new_tokens=6)
+    assert len(calls) == 2 and eng.block_manager.num_free() == 400
+    out = eng.generate([prompts[1]], max_new_tokens=2)
+    assert eng.block_manager.prefix_hits == 0
+    assert out[0][0] == int(log_probs(cpu_weights(eng.model), eng.model.cfg, [prompts[1]])[0].argmax())
+    check(eng, prompts, 3, 6)
+    assert eng.block_manager.prefix_hits == 4      # the second prompt's blocks, which generate() wrote

@@ -176,7 +176,8 @@ def beam_search(model: Qwen2Paged, cache: PagedKVCache, blocks: BlockManager, pr
     own = blocks.blocks_needed(max_new) + 2
     done: list[list[BeamResult]] = []
     while len(done) < len(prompts):
-        some, tables, cached, spare = [], [], [], []
+        some, tables, cached, spare, made = [], [], [], [], []
+        written = False
         try:
             for p in prompts[len(done):]:
                 need = blocks.blocks_needed(len(p)) + num_beams * own
@@ -184,6 +185,7 @@ def beam_search(model: Qwen2Paged, cache: PagedKVCache, blocks: BlockManager, pr
                     break
                 table, n = blocks.allocate_prompt(list(p))
                 tables.append(table)
+                made.append(table[n // blocks.block_size:])
                 spare.append(blocks.allocate_private(num_beams * own, []))
                 some.append(list(p))
                 cached.append(min(n, len(p) - 1))
@@ -191,6 +193,7 @@ def beam_search(model: Qwen2Paged, cache: PagedKVCache, blocks: BlockManager, pr
                 raise OutOfBlocks(f"a prompt of {len(prompts[len(done)])} tokens with {num_beams} beams needs {need} blocks, "
                                   f"{blocks.num_free()} are free")
             logits = prefill(model, cache, some, tables, cached, budget)
+            written = True
             rows, lens = [], []
             for t, p in zip(tables, some):         # the prompt in a request's first row; its beams follow from there
                 rows += [t] + [[]] * (num_beams - 1)
@@ -206,6 +209,9 @@ def beam_search(model: Qwen2Paged, cache: PagedKVCache, blocks: BlockManager, pr
             search.run(max_new - 1, graph)
             done += search.results(length_penalty, num_return)
         finally:
+            if not written:                        # nobody may find the prompts' blocks, whose K/V are not there
+                for t in made:
+                    blocks.unpublish(t)
             for t in tables + spare:
                 blocks.free_table(t)
     return done
