@@ -5,7 +5,7 @@ from types import SimpleNamespace
 import pytest
 
 from tinybatch_amd import beam_search as bs
-from tinybatch_amd.block_manager import BlockManager
+from tinybatch_amd.block_manager import BlockManager, OutOfBlocks
 
 
 class Failed(Exception):
@@ -78,3 +78,16 @@ def test_unpublish():
     blocks.free_table(table)
     blocks.free_table(again)
     assert blocks.num_free() == 10 and len(blocks.free_ids) == 8
+
+
+def test_a_prompt_that_can_never_fit_is_told_before_any_search(monkeypatch):
+    """Behind prompts that fit, which are searched in turns: nothing is computed and thrown away."""
+    blocks, calls = BlockManager(40, 16), []
+    monkeypatch.setattr(bs, "prefill", lambda *_: calls.append(1))
+    monkeypatch.setattr(bs.DeviceTables, "from_lists", fail)
+    with pytest.raises(OutOfBlocks, match="prompt of 560 tokens"):
+        search(blocks, [PROMPT, PROMPT[:20], list(range(560))], num_beams=4)
+    assert not calls and blocks.num_free() == 40 and not blocks.cache
+    with pytest.raises(Failed):                                       # 36 of 40 blocks: searched
+        search(blocks, [list(range(24 * 16))], num_beams=4)
+    assert calls == [1] and blocks.num_free() == 40

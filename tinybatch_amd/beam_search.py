@@ -164,7 +164,8 @@ def beam_search(model: Qwen2Paged, cache: PagedKVCache, blocks: BlockManager, pr
                 eos_ids=(), length_penalty: float = 1.0, num_return: int = 1, budget: int = 2048,
                 graph: bool = True) -> list[list[BeamResult]]:
     """The ``num_return`` best of ``num_beams`` beams for every prompt (token ids), of up to ``max_new`` tokens. Blocks
-    for the beams come from ``blocks`` and go back to it; as many prompts as its free blocks allow are searched together."""
+    for the beams come from ``blocks`` and go back to it; as many prompts as its free blocks allow are searched together. A
+    prompt that does not fit by itself raises OutOfBlocks before anything is computed."""
     if not 1 <= num_beams <= MAX_BEAMS or not 1 <= num_return <= num_beams or max_new < 1:
         raise ValueError(f"1 .. {MAX_BEAMS} beams, of which as many are returned at most, and one new token at least")
     vocab = model.cfg.vocab_size
@@ -174,13 +175,17 @@ def beam_search(model: Qwen2Paged, cache: PagedKVCache, blocks: BlockManager, pr
         raise ValueError("empty prompt")
     # a beam's own blocks: its tokens', the copy of the prompt's last block, and one more while a selection copies
     own = blocks.blocks_needed(max_new) + 2
+    needs = [blocks.blocks_needed(len(p)) + num_beams * own for p in prompts]
+    for p, need in zip(prompts, needs):            # (every turn gives its blocks back: what fits now fits then)
+        if need > blocks.num_free():
+            raise OutOfBlocks(f"a prompt of {len(p)} tokens with {num_beams} beams needs {need} blocks, "
+                              f"{blocks.num_free()} are free")
     done: list[list[BeamResult]] = []
     while len(done) < len(prompts):
         some, tables, cached, spare, made = [], [], [], [], []
         written = False
         try:
-            for p in prompts[len(done):]:
-                need = blocks.blocks_needed(len(p)) + num_beams * own
+            for p, need in zip(prompts[len(done):], needs[len(done):]):
                 if need > blocks.num_free() or (len(some) + 1) * num_beams > 65535:
                     break
                 table, n = blocks.allocate_prompt(list(p))
@@ -189,9 +194,6 @@ def beam_search(model: Qwen2Paged, cache: PagedKVCache, blocks: BlockManager, pr
                 spare.append(blocks.allocate_private(num_beams * own, []))
                 some.append(list(p))
                 cached.append(min(n, len(p) - 1))
-            if not some:
-                raise OutOfBlocks(f"a prompt of {len(prompts[len(done)])} tokens with {num_beams} beams needs {need} blocks, "
-                                  f"{blocks.num_free()} are free")
             logits = prefill(model, cache, some, tables, cached, budget)
             written = True
             rows, lens = [], []
