@@ -151,6 +151,9 @@ int32_t tb_kv_gather(const void* pool, int64_t num_blocks,
  * (src/tinybatch/kv_cache.py:33-38). A step with a shared slot must use
  * tb_kv_append (its slot_mapping marks the superseded rows -1) and then this
  * call without k_new. The kernels do not read slot_mapping and cannot detect it.
+ * Nor may a slot that the step writes hold an earlier position of another
+ * sequence of the step (a prefix that the step itself makes): that sequence's
+ * rows would read it while it is written. Append with tb_kv_append first.
  * RoPE in the prologue (rope_cos != NULL, the tables of tb_kv_append_rope):
  * q holds the projections before rotation; every query row is rotated at its
  * position row_ctx - 1 as it is loaded (the engine's _rope of q,
@@ -236,7 +239,9 @@ int32_t tb_build_step_metadata(const int32_t* query_start_loc, int32_t num_seqs,
  *     for bit). With rope tables the K rows are rotated at their positions
  *     first, as tb_kv_append_rope does (model.py:125,128). The new rows' slots
  *     must not be written by another row of the step (slot_mapping's superseded
- *     rows, tb_build_step_metadata's counts[5], must be 0).
+ *     rows, tb_build_step_metadata's counts[5], must be 0), nor hold earlier
+ *     positions of another of its sequences, which would read them while they
+ *     are written (two prompts on one prefix that the step makes: append first).
  *   work: tb_build_prefill_work's list (device memory), num_work entries;
  *     max_tiles: the value the builder returned.
  * q, out, strides, scale, dtype, rope: as tb_paged_attention. */

@@ -191,7 +191,8 @@ class PagedKVCache:
         """write() then attention() (model.py:128-147) with the append folded into the
         attention kernels where the step's kernels can do both: decode-only steps, steps
         of whole prefills (tb_paged_prefill) and mixed steps split into those two sides,
-        when no slot is written by two rows of the step; otherwise the two calls. With
+        when no slot is written by two rows of the step, or by one and read as an earlier
+        position of another; otherwise the two calls. With
         ``rope`` q and k are the projections before rotation."""
         hq = num_heads if num_heads is not None else q.shape[1]
         rows = self.rows_per_item(hq)
@@ -204,8 +205,8 @@ class PagedKVCache:
 
     @staticmethod
     def _fusable(meta: StepMetadata) -> bool:
-        if meta.has_superseded():
-            return False                                  # a superseded writer: the separate append
+        if meta.has_superseded() or meta.reads_new:
+            return False                # a superseded writer, a prefix that the step itself makes: the separate append
         if meta.parts is not None or meta.decode_only:
             return True
         return meta.whole_prefills_only()

@@ -126,6 +126,10 @@ class StepMetadata:
     # -1): no fused append then. Found by the builder; None: found from the arrays when asked
     superseded: bool | None = None
 
+    # whether a sequence has earlier positions in slots that another row of the step writes (two prompts on one prefix, of which
+    # the first one's step makes it): no fused append then, whose kernels read those slots while they are written
+    reads_new: bool = False
+
     def has_superseded(self) -> bool:
         if self.superseded is not None:
             return self.superseded
@@ -442,7 +446,7 @@ def build_step_metadata(positions, seq_slices, block_tables, context_lens, *, bl
         slots[row_ids] = s
         # last writer wins: keep only the final occurrence of each slot
         rev = s[::-1]
-        _, first_in_rev = np.unique(rev, return_index=True)
+        written, first_in_rev = np.unique(rev, return_index=True)
         keep = np.zeros(tot, dtype=bool)
         keep[tot - 1 - first_in_rev] = True
         slots[row_ids[~keep]] = -1
@@ -456,6 +460,7 @@ def build_step_metadata(positions, seq_slices, block_tables, context_lens, *, bl
     columns_work, columns_part = None, 0
     tiled = np.zeros(T, dtype=bool)
     nparts_by_row = np.zeros(T, dtype=np.int64)
+    reads_new = False
     if tot and context_lens is not None:
         ctx = np.asarray(context_lens, dtype=np.int64)
         if np.any(ctx < qlens):
@@ -468,6 +473,15 @@ def build_step_metadata(positions, seq_slices, block_tables, context_lens, *, bl
                 b = int(np.argmax(short))
                 raise IndexError(f"context_len {int(ctx[b])} of sequence {b} needs {int(need[b])} blocks "
                                  f"but its table has {int(tab_lens[b])}")
+        if B > 1:
+            # the tables' entries that the step writes to: the first slot of their blocks that is written (of several the
+            # one set last), against the earlier positions there (a sequence's own new rows lie behind them)
+            mark, first = np.zeros(num_blocks, dtype=bool), np.zeros(num_blocks, dtype=np.int64)
+            blocks = written[::-1] // block_size
+            mark[blocks], first[blocks] = True, written[::-1] % block_size
+            seq, col = np.divmod(np.flatnonzero(mark[tables[:B]]), max_nb)
+            earlier = np.where(qlens > 0, ctx - qlens, 0)[seq] - col * block_size
+            reads_new = bool(np.any(first[tables[seq, col]] < np.minimum(earlier, block_size)))
         row_ctx = np.repeat(ctx - qlens, qlens) + row_i + 1
         row_ctx_by_row[row_ids] = row_ctx
         nparts_by_row[row_ids] = (row_ctx + P - 1) // P
@@ -593,6 +607,7 @@ def build_step_metadata(positions, seq_slices, block_tables, context_lens, *, bl
         columns_seqs=column_seqs or None,
         columns_partition=columns_part,
         superseded=bool(np.any((slots < 0) & (row_ctx_by_row > 0))),
+        reads_new=reads_new,
     )
 
 

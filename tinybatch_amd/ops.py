@@ -409,6 +409,13 @@ def decode_buffers(device: torch.device, piece_bytes: int, units: int) -> Decode
     return b
 
 
+def _check_reads_new(meta: StepMetadata) -> None:
+    if meta.reads_new:
+        raise ValueError("a sequence of the step has earlier positions in slots that another one's new rows are written to; "
+                         "the fused append cannot serve the step: append with kv_append, then call paged_attention "
+                         "without k_new")
+
+
 def paged_decode(q: torch.Tensor, pool: torch.Tensor, meta: StepMetadata, *, num_heads: int,
                  scale: float | None = None, out: torch.Tensor | None = None,
                  k_new: torch.Tensor | None = None, v_new: torch.Tensor | None = None,
@@ -447,6 +454,7 @@ def paged_decode(q: torch.Tensor, pool: torch.Tensor, meta: StepMetadata, *, num
         if sm.size and np.any(sm[:B] < 0):
             raise ValueError("two decode rows write one pool slot; the fused append cannot serve the "
                              "step: append with kv_append, then call paged_attention without k_new")
+        _check_reads_new(meta)
         for name, t in (("k_new", k_new), ("v_new", v_new)):
             _lib.require_gpu_tensor(name, t)
             if t.dtype != pool.dtype or t.shape[0] != B:
@@ -510,6 +518,7 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, meta: StepMetadata, *, 
             if meta.has_superseded():
                 raise ValueError("two rows of the step write one pool slot; the fused append cannot serve "
                                  "the step: append with kv_append, then call paged_attention without k_new")
+            _check_reads_new(meta)
         for r0, r1, m in meta.parts:
             paged_attention(q[r0:r1], pool, m, num_heads=num_heads, scale=scale, out=out[r0:r1], rope=rope,
                             k_new=k_new[r0:r1] if fused else None, v_new=v_new[r0:r1] if fused else None)
@@ -564,6 +573,7 @@ def paged_attention(q: torch.Tensor, pool: torch.Tensor, meta: StepMetadata, *, 
             # row's own K/V where the reference's last writer wins (kv_cache.py:33-38)
             raise ValueError("two decode rows write one pool slot; the fused append cannot serve the "
                              "step: append with kv_append, then call paged_attention without k_new")
+        _check_reads_new(meta)
         for name, t in (("k_new", k_new), ("v_new", v_new)):
             _lib.require_gpu_tensor(name, t)
             if t.dtype != pool.dtype or t.shape[0] != T:
