@@ -194,3 +194,61 @@ def test_prompts_of_a_search_that_failed_are_not_found(monkeypatch):
     assert out[0][0] == int(log_probs(cpu_weights(eng.model), eng.model.cfg, [prompts[1]])[0].argmax())
     check(eng, prompts, 3, 6)
     assert eng.block_manager.prefix_hits == 4      # the second prompt's blocks, which generate() wrote
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_a_loop_of_ones_own(dtype):
+    """The loop of the integration notes on the model's layers, its requests with beams that end on the way: the engine's search."""
+    from tinybatch_amd import BeamPlan, DeviceTables, beam_attention, build_device_step, ops, reorder_beams, select_beams
+
+    eng = sharpen(engine(dtype, decode_graphs=False, enable_prefix_caching=False), 12.0)
+    m, cache, mc, K, new = eng.model, eng.kv_cache, eng.model.cfg, 3, 14
+    prompts = random_prompts(21, [30, 45])
+    plain = eng.beam_search(prompts, num_beams=K, max_new_tokens=new, num_return=K)
+    eos = plain[0][0].token_ids[4]
+    eng.eos_ids, eng.cfg.stop_token_ids = {eos}, (eos,)
+    want = eng.beam_search(prompts, num_beams=K, max_new_tokens=new, num_return=K, length_penalty=0.0)
+    assert any(len(r.token_ids) < new for found in want for r in found)
+    blocks, logits = [], []
+    for p in prompts:
+        table = eng.block_manager.allocate_private(-(-len(p) // 16), p)
+        blocks.append(table)
+        logits.append(m.forward(torch.tensor(p, device=DEV), torch.arange(len(p), device=DEV), [(0, len(p))], [table], [len(p)], cache))
+    free = eng.block_manager.allocate_private(40, [])
+    tables = DeviceTables.from_lists([t for b in blocks for t in (b, [], [])], [n for p in prompts for n in (len(p), 0, 0)], free,
+                                     max_blocks=6, block_size=16, num_blocks=cache.num_blocks, group_size=K, device=DEV)
+    step = tables.new_step(padded=1)
+    plan = BeamPlan(tables, num_heads=mc.n_heads, num_kv_heads=mc.n_kv_heads, head_dim=mc.head_dim, dtype=cache.dtype)
+    choice = select_beams(torch.cat(logits), torch.zeros(2, 1, device=DEV), num_candidates=K)
+    reorder_beams(cache.storage, tables, choice.parents)
+    finished = choice.tokens == eos
+    told = [choice]
+    for _ in range(new - 1):
+        live = ~finished & (choice.scores > -float("inf"))
+        build_device_step(tables, live.view(-1).int(), step)
+        plan.build(step.row_ctx)
+
+        def attention(i, q, k, v):
+            ops.kv_append(cache.pools[i], k, v, step.slot_mapping)
+            return beam_attention(q, cache.pools[i], plan)
+
+        x = m.run_layers(choice.tokens.view(-1).clamp(min=0), step.positions, attention)
+        choice = select_beams((x @ m.lm_head.T).float(), choice.scores, finished=finished, end_token=eos)
+        reorder_beams(cache.storage, tables, choice.parents, step)
+        finished = finished.gather(1, choice.parents.clamp(min=0).long()) & (choice.parents >= 0) | (choice.tokens == eos)
+        told.append(choice)
+    tables.check()
+    for g, found in enumerate(want):
+        got = []
+        for k in range(K):
+            ids, at = [], k
+            for c in reversed(told):
+                ids.append(int(c.tokens[g, at]))
+                at = int(c.parents[g, at])
+            ids.reverse()
+            got.append((float(choice.scores[g, k]), ids[:ids.index(eos) + 1] if eos in ids else ids))
+        if dtype == "float32":
+            assert [ids for _, ids in got] == [r.token_ids for r in found]
+            assert all(abs(s - r.score) <= 2e-3 * len(ids) for (s, ids), r in zip(got, found))
+        else:                                      # (other products of the LM head: near candidates may change places)
+            assert max(s for s, _ in got) >= found[0].score - 2 * 2.0 ** -8 * 40 * new

@@ -3,8 +3,8 @@
 The reference samples one continuation per request (src/tinybatch/engine.py:145-159). Here every prompt
 is prefilled once, its ``num_beams`` best first tokens become its beams, and each step continues them
 by one token: the operators of beams.py, with nothing read back between two steps. A beam that has
-ended stays among the candidates with its score, so that the search may end early only when
-every beam has.
+ended stays among the candidates with its score, which live beams of any length are measured against as it is (length_penalty
+orders the results alone), so that the search may end early only when every beam has.
 """
 from __future__ import annotations
 

@@ -3,13 +3,14 @@
 The reference decodes one continuation per request (src/tinybatch/engine.py:99-159). Here a request
 has ``group_size`` rows, its beams, whose paged state lives on the GPU (DeviceTables):
 
-    build_device_step(tables, new_lens, step)                    # one token per beam
+    build_device_step(tables, live, step)                        # one token per live beam (1; ended or lost: 0)
     plan.build(step.row_ctx)                                     # a BeamPlan, for all layers
     for layer in range(n_layers):
         ops.kv_append(cache.pools[layer], k, v, step.slot_mapping)
         attn = beam_attention(q, cache.pools[layer], plan)
     choice = select_beams(logits, scores, finished=finished, end_token=eos)
     reorder_beams(cache.storage, tables, choice.parents, step=step)
+    # finished and live follow choice.parents and choice.tokens (BeamState.advance in beam_search.py)
 
 Everything is enqueued on the tensors' device's current stream and nothing synchronises.
 """

@@ -104,7 +104,7 @@ class LLMEngine:
     def beam_search(self, prompts: list[list[int]], *, num_beams: int = 4, max_new_tokens: int | None = None,
                     length_penalty: float = 1.0, num_return: int = 1) -> list[list[BeamResult]]:
         """Per prompt the ``num_return`` best of ``num_beams`` beams (beam_search.py), by score / length **
-        length_penalty. Runs to its end on the blocks that are free now, between two steps of the requests
+        length_penalty (which beams are kept goes by their scores alone). Runs to its end on the blocks that are free now, between two steps of the requests
         that are being served; a captured step (EngineConfig.decode_graphs) is replayed from the second token on."""
         new = self.cfg.max_new_tokens if max_new_tokens is None else max_new_tokens
         longest = max((len(p) for p in prompts), default=0)
