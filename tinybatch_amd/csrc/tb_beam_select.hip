@@ -21,10 +21,12 @@
 // Sums of a wave's tiles, S, its logarithm and every c are in 64 bits: the order of two beams' candidates is decided
 // by differences far below a float's step at the score's size.
 //
-// What bounds it: part 1 the vector instructions in 16 bits (4.5 a token and an exponential, which counts four: 32 requests
-// of 8 beams, bf16, 54 MB that count, 14 us) and the memory in fp32 (192 rows, 98 MB, 18 us: 5.4 TB/s); parts 2 and 3 chains
+// What bounds it: part 1 in fp32 the memory (192 rows, 98 MB, 18 us: 5.4 TB/s), in 16 bits the way through a wave, which has three
+// tiles of a row of 151936: who counts, the first tile, its maximum, two more tiles, a sum over the lanes in 64 bits, each behind the
+// one before (32 requests of 8 beams, bf16, 54 MB that count, 13.9 us: 3.9 TB/s; counted, a wave waits 69 % of its cycles, and the vector
+// unit is busy 16300 of a CU's 27900 with 400 instructions a wave, half of them its tiles'). Parts 2 and 3 are chains
 // of dependent steps of some 100 ns: 6 and 3 us for one request of 4 beams, 7 and 4 for 32 of 8 (M = 16), 11 and 10 for 4 of 48
-// (M = 96, 150 segments a beam). In all, from a captured graph: one request 11.5 us, 32 requests 24.9, 4 of 48 beams 38.7.
+// (M = 96, 150 segments a beam). In all, from a captured graph: one request 11.5 us, 32 requests 25.2, 4 of 48 beams 38.7.
 #include "tb_common.h"
 
 namespace tb {

@@ -173,7 +173,7 @@ class DeviceTables:
         self._counted.copy_(step._counted)
 
     def check(self) -> None:
-        """Raise what a call could not do since the last check (synchronises the device)."""
+        """Raise what a call could not do since the last check (waits for the current stream, which is to be the calls')."""
         st = int(self.status.item())
         if not st:
             return
