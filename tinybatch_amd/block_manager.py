@@ -162,17 +162,13 @@ class BlockManager:
 
     # ---- release -------------------------------------------------------------
     def unpublish(self, table: list[int]) -> None:
-        """Take these blocks out of the prefix cache: what was to be written to them was not.
-        Their counts stay; freed, they are free."""
+        """Take a table's blocks out of the prefix cache, before it is freed: what was to be
+        written to them was not. (No reference counterpart.)"""
         for bid in table:
             blk = self.blocks[bid]
             if blk.prefix_hash is not None and self.cache.get(blk.prefix_hash) == bid:
                 del self.cache[blk.prefix_hash]
             blk.prefix_hash = None
-            if bid in self.evictable:
-                del self.evictable[bid]
-                blk.token_ids = []
-                self.free_ids.append(bid)
 
     def free_table(self, table: list[int]) -> None:
         for bid in table:
